@@ -12,8 +12,13 @@ Three operators around the FP8 block-scaled linear layer (e4m3 values, one bf16 
 framework's kernels; ``exact`` computes it from the definitions in 64 bits.
 """
 import math
+import os
+import sys
 
 import torch
+
+sys.path.append(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                             "my-nano-vllm_b200"))     # where the package lies
 
 own = False
 
