@@ -260,6 +260,62 @@ FP8ATTN_API int fp8attn_fp8_tp_linear(const void* x, int64_t x_row_stride, const
                    int64_t workspace_bytes, void* stream);
 
 /*
+ * Feed-forward activations written in 8 bits, in the format fp8attn_fp8_block_gemm reads (no
+ * counterpart in the reference, which runs norm, SiLU and fp8_dyn_quant_kernel one after another:
+ * nanovllm/layers/layernorm.py:28-50, layers/activation.py:8-11, kernels/fp8_linear.py:11-31).
+ * Quantisation, per row and 128 columns of the fp32 result y: a = max|y| (NaN left out), d = a / 448
+ * (1 for an all-zero group), q = e4m3(y / d), scale = bf16(d).
+ *   dtype: type of the 16-bit tensors, FP8ATTN_BF16 or FP8ATTN_FP16.  Every 16-bit pointer is
+ *   16-byte aligned, its row stride (elements) a multiple of 8 and at least the row's width; q is
+ *   8-byte aligned, scale 2-byte aligned; outputs are contiguous.  M = 0 is a no-op.
+ *   fp8attn_add_rms_norm_quant: s = x + residual (s = x if residual is NULL), y = s / sqrt(mean(s^2)
+ *     + eps) * weight, all in fp32.  x, residual [M, K], weight [K]; K a multiple of 128 up to 16384.
+ *     q [M, K], scale [M, K / 128]; residual_out [M, K]: s rounded to dtype (given exactly when
+ *     residual is; may be the residual itself where its rows are K apart); norm_out [M, K]: y rounded
+ *     to dtype, or NULL.
+ *   fp8attn_silu_mul_quant: y = g / (1 + exp(-g)) * u.  gate_up [M, 2 I]: g's columns, then u's; I a
+ *     multiple of 128.  q [M, I], scale [M, I / 128].
+ */
+#define FP8ATTN_BF16 0
+#define FP8ATTN_FP16 1
+FP8ATTN_API int fp8attn_add_rms_norm_quant(const void* x, int64_t x_row_stride, const void* residual,
+                   int64_t residual_row_stride, const void* weight, float eps, void* q, void* scale,
+                   void* residual_out, void* norm_out, int64_t M, int K, int dtype, void* stream);
+FP8ATTN_API int fp8attn_silu_mul_quant(const void* gate_up, int64_t row_stride, void* q, void* scale,
+                   int64_t M, int I, int dtype, void* stream);
+
+/*
+ * A mixture-of-experts layer for a few tokens, weights in the format of fp8attn_fp8_block_linear (no
+ * counterpart in the reference, whose model is dense).  Per token: l = x . router^T; p = softmax(l);
+ * the top_k largest p (ties: the lower expert first; a NaN is chosen last) with weights c = p, divided
+ * by their sum if renormalize; for each chosen expert e: g, u = the halves of xq . w13[e]^T,
+ * h = g / (1 + exp(-g)) * u quantised as above, y_e = hq . w2[e]^T (block-scaled products as in
+ * fp8attn_fp8_block_gemm); out = bf16(sum of c_e y_e, in the order chosen).
+ *   x bf16 [T, H] and its quantised form xq e4m3 [T, H], x_scale bf16 [T, H / 128] (contiguous), as
+ *     fp8attn_add_rms_norm_quant or fp8attn_fp8_dyn_quant leave them; router bf16 [E, H];
+ *     w13 e4m3 [E, 2 I, H] (gate rows, then up rows), w13_scale bf16 [E, 2 I / 128, H / 128];
+ *     w2 e4m3 [E, H, I], w2_scale bf16 [E, H / 128, I / 128]; all contiguous but x, xq and out, whose
+ *     row strides are in elements.  out bf16 [T, H].
+ *   topk_weights fp32 [T, top_k], topk_ids int32 [T, top_k]: the router's choice, or NULL.
+ *   Sizes: H and I multiples of 128 up to 16384, 1 <= E <= 512, 1 <= top_k <= min(E, 32),
+ *     0 <= T <= 1024, T * top_k <= 8192.  T = 0 is a no-op.
+ *   Alignment: x, xq, router, w13, w2 and out 16 bytes, x's and out's row strides multiples of 8 and
+ *     xq's of 16, scales 2 bytes, topk arrays 4.
+ *   workspace: fp8attn_fp8_moe_workspace_bytes(T, H, I, E, top_k) bytes (-1 for invalid sizes), 256-byte
+ *     aligned; its contents need not be initialised and are not kept.  One workspace must not serve
+ *     two calls that can overlap.
+ *   error: device int32 (4-byte aligned) that a bounded device wait which gives up sets to 1 (see
+ *     fp8attn_read_error, which takes it for a workspace's word), or NULL.
+ */
+FP8ATTN_API int64_t fp8attn_fp8_moe_workspace_bytes(int64_t T, int H, int I, int E, int top_k);
+FP8ATTN_API int fp8attn_fp8_moe(const void* x, int64_t x_row_stride, const void* xq,
+                   int64_t xq_row_stride, const void* x_scale, const void* router, const void* w13,
+                   const void* w13_scale, const void* w2, const void* w2_scale, void* out,
+                   int64_t out_row_stride, float* topk_weights, int32_t* topk_ids, int64_t T, int H,
+                   int I, int E, int top_k, int renormalize, void* workspace,
+                   int64_t workspace_bytes, int32_t* error, void* stream);
+
+/*
  * Self-checks of device-side mechanisms (no counterpart in the reference; used by the tests).
  *   fp8attn_diag_wait_timeout: num_ctas CTAs each claim one work item from the control block at
  *     `workspace` (ints: [0] error word, [1] next item, [2] CTAs finished, zeroed by the caller)

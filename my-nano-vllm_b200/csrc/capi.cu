@@ -790,3 +790,206 @@ int fp8attn_fp8_tp_linear(const void* x, int64_t x_row_stride, const void* w, co
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------- FP8 feed-forward activations
+namespace {
+
+int check_dtype(int dtype) {
+  if (dtype != FP8ATTN_BF16 && dtype != FP8ATTN_FP16)
+    return fail(FP8ATTN_EINVAL, "dtype must be FP8ATTN_BF16 or FP8ATTN_FP16 (got %d)", dtype);
+  return FP8ATTN_OK;
+}
+
+// Rows of a 16-bit tensor that kernels read and write 16 bytes at a time.
+int check_rows16(const char* what, const void* p, int64_t row_stride, int64_t columns) {
+  if (p == nullptr) return fail(FP8ATTN_EINVAL, "%s: null pointer argument", what);
+  if (!aligned(p, 16) || row_stride < columns || row_stride % 8 != 0)
+    return fail(FP8ATTN_EINVAL, "%s must be 16-byte aligned with a row stride >= %lld that is a "
+                "multiple of 8 elements", what, static_cast<long long>(columns));
+  return FP8ATTN_OK;
+}
+
+int check_quant_out(const char* what, const void* q, const void* scale) {
+  if (q == nullptr || scale == nullptr)
+    return fail(FP8ATTN_EINVAL, "%s: null pointer argument", what);
+  if (!aligned(q, 8) || !aligned(scale, 2))
+    return fail(FP8ATTN_EINVAL, "%s: q must be 8-byte aligned and scale 2-byte aligned", what);
+  return FP8ATTN_OK;
+}
+
+// A launch has at most 2^31 - 1 CTAs; the kernels run a thread per 8 elements or more.
+constexpr int64_t kMaxVectors = (1LL << 31) * 64;
+
+}  // namespace
+
+extern "C" {
+
+int fp8attn_add_rms_norm_quant(const void* x, int64_t x_row_stride, const void* residual,
+                               int64_t residual_row_stride, const void* weight, float eps, void* q,
+                               void* scale, void* residual_out, void* norm_out, int64_t M, int K,
+                               int dtype, void* stream) {
+  int rc = check_dtype(dtype);
+  if (rc) return rc;
+  if (M < 0 || M > INT32_MAX || K <= 0 || K % 128 != 0 || K > fp8attn::kNormMaxColumns)
+    return fail(FP8ATTN_EINVAL, "norm quant needs 0 <= M < 2^31 and K a multiple of 128 up to %d "
+                "(got M=%lld K=%d)", fp8attn::kNormMaxColumns, static_cast<long long>(M), K);
+  if (M == 0) return FP8ATTN_OK;
+  rc = check_rows16("norm quant: x", x, x_row_stride, K);
+  if (rc) return rc;
+  rc = check_rows16("norm quant: weight", weight, K, K);
+  if (rc) return rc;
+  rc = check_quant_out("norm quant", q, scale);
+  if (rc) return rc;
+  if ((residual == nullptr) != (residual_out == nullptr))
+    return fail(FP8ATTN_EINVAL, "norm quant: residual and residual_out must both be given or both "
+                "be null");
+  if (residual != nullptr) {
+    rc = check_rows16("norm quant: residual", residual, residual_row_stride, K);
+    if (rc) return rc;
+    rc = check_rows16("norm quant: residual_out", residual_out, K, K);
+    if (rc) return rc;
+    if (residual == residual_out && residual_row_stride != K && M > 1)
+      return fail(FP8ATTN_EINVAL, "norm quant: residual_out may be the residual only where its "
+                  "rows are K apart");
+  }
+  if (norm_out != nullptr) {
+    rc = check_rows16("norm quant: norm_out", norm_out, K, K);
+    if (rc) return rc;
+  }
+  fp8attn::NormQuantParams p;
+  p.x = static_cast<const uint16_t*>(x);
+  p.x_row_stride = x_row_stride;
+  p.residual = static_cast<const uint16_t*>(residual);
+  p.residual_row_stride = residual_row_stride;
+  p.weight = static_cast<const uint16_t*>(weight);
+  p.eps = eps;
+  p.q = static_cast<uint8_t*>(q);
+  p.scale = static_cast<uint16_t*>(scale);
+  p.residual_out = static_cast<uint16_t*>(residual_out);
+  p.norm_out = static_cast<uint16_t*>(norm_out);
+  p.M = M;
+  p.K = K;
+  p.fp16 = dtype == FP8ATTN_FP16;
+  const cudaError_t e = fp8attn::launch_add_rms_norm_quant(p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FP8ATTN_OK : cuda_fail(e, "norm quant launch");
+}
+
+int fp8attn_silu_mul_quant(const void* gate_up, int64_t row_stride, void* q, void* scale, int64_t M,
+                           int I, int dtype, void* stream) {
+  int rc = check_dtype(dtype);
+  if (rc) return rc;
+  if (M < 0 || I <= 0 || I % 128 != 0 || I > INT32_MAX / 4 || M > kMaxVectors / (I / 8))
+    return fail(FP8ATTN_EINVAL, "silu quant needs M >= 0, I a positive multiple of 128 and M * I < "
+                "2^40 (got M=%lld I=%d)", static_cast<long long>(M), I);
+  if (M == 0) return FP8ATTN_OK;
+  rc = check_rows16("silu quant: gate_up", gate_up, row_stride, 2LL * I);
+  if (rc) return rc;
+  rc = check_quant_out("silu quant", q, scale);
+  if (rc) return rc;
+  fp8attn::SiluQuantParams p;
+  p.gate_up = static_cast<const uint16_t*>(gate_up);
+  p.row_stride = row_stride;
+  p.q = static_cast<uint8_t*>(q);
+  p.scale = static_cast<uint16_t*>(scale);
+  p.M = M;
+  p.I = I;
+  p.fp16 = dtype == FP8ATTN_FP16;
+  const cudaError_t e = fp8attn::launch_silu_mul_quant(p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FP8ATTN_OK : cuda_fail(e, "silu quant launch");
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- mixture of experts
+namespace {
+
+int check_moe_sizes(int64_t T, int H, int I, int E, int top_k) {
+  constexpr int kMaxColumns = 16384;
+  if (H <= 0 || H % 128 != 0 || H > kMaxColumns || I <= 0 || I % 128 != 0 || I > kMaxColumns)
+    return fail(FP8ATTN_EINVAL, "moe: H and I must be multiples of 128 up to %d (got H=%d I=%d)",
+                kMaxColumns, H, I);
+  if (E < 1 || E > fp8attn::kMoeMaxExperts || top_k < 1 || top_k > E ||
+      top_k > fp8attn::kMoeMaxTopK)
+    return fail(FP8ATTN_EINVAL, "moe: 1 <= E <= %d and 1 <= top_k <= min(E, %d) (got E=%d top_k=%d)",
+                fp8attn::kMoeMaxExperts, fp8attn::kMoeMaxTopK, E, top_k);
+  if (T < 0 || T > fp8attn::kMoeMaxTokens || T * top_k > fp8attn::kMoeMaxSlots)
+    return fail(FP8ATTN_EINVAL, "moe: at most %d tokens and %d token-expert pairs a call (got T=%lld "
+                "top_k=%d)", fp8attn::kMoeMaxTokens, fp8attn::kMoeMaxSlots,
+                static_cast<long long>(T), top_k);
+  return FP8ATTN_OK;
+}
+
+fp8attn::MoeParams moe_sizes(int64_t T, int H, int I, int E, int top_k) {
+  fp8attn::MoeParams p = {};
+  p.T = T;
+  p.H = H;
+  p.I = I;
+  p.E = E;
+  p.top_k = top_k;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t fp8attn_fp8_moe_workspace_bytes(int64_t T, int H, int I, int E, int top_k) {
+  if (check_moe_sizes(T, H, I, E, top_k)) return -1;
+  fp8attn::MoeParams p = moe_sizes(T, H, I, E, top_k);
+  return fp8attn::moe_layout(p, nullptr, device_sms());
+}
+
+int fp8attn_fp8_moe(const void* x, int64_t x_row_stride, const void* xq, int64_t xq_row_stride,
+                    const void* x_scale, const void* router, const void* w13, const void* w13_scale,
+                    const void* w2, const void* w2_scale, void* out, int64_t out_row_stride,
+                    float* topk_weights, int32_t* topk_ids, int64_t T, int H, int I, int E,
+                    int top_k, int renormalize, void* workspace, int64_t workspace_bytes,
+                    int32_t* error, void* stream) {
+  int rc = check_moe_sizes(T, H, I, E, top_k);
+  if (rc) return rc;
+  if (T == 0) return FP8ATTN_OK;
+  rc = check_rows16("moe: x", x, x_row_stride, H);
+  if (rc) return rc;
+  rc = check_rows16("moe: out", out, out_row_stride, H);
+  if (rc) return rc;
+  if (xq == nullptr || x_scale == nullptr || router == nullptr || w13 == nullptr ||
+      w13_scale == nullptr || w2 == nullptr || w2_scale == nullptr)
+    return fail(FP8ATTN_EINVAL, "moe: null pointer argument");
+  if (!aligned(xq, 16) || xq_row_stride < H || xq_row_stride % 16 != 0)
+    return fail(FP8ATTN_EINVAL, "moe: xq must be 16-byte aligned with a row stride >= H that is a "
+                "multiple of 16 bytes");
+  if (!aligned(router, 16) || !aligned(w13, 16) || !aligned(w2, 16))
+    return fail(FP8ATTN_EINVAL, "moe: router, w13 and w2 must be 16-byte aligned");
+  if (!aligned(x_scale, 2) || !aligned(w13_scale, 2) || !aligned(w2_scale, 2) ||
+      !aligned(topk_weights, 4) || !aligned(topk_ids, 4) || !aligned(error, 4))
+    return fail(FP8ATTN_EINVAL, "moe: misaligned scales, topk_weights, topk_ids or error");
+  const int sms = device_sms();
+  fp8attn::MoeParams p = moe_sizes(T, H, I, E, top_k);
+  const int64_t need = fp8attn::moe_layout(p, nullptr, sms);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(FP8ATTN_EWORKSPACE, "moe: workspace of %lld bytes needed, got %lld",
+                static_cast<long long>(need), static_cast<long long>(workspace_bytes));
+  if (!aligned(workspace, 256)) return fail(FP8ATTN_EINVAL, "moe: workspace must be 256-byte aligned");
+  p.x = static_cast<const uint16_t*>(x);
+  p.x_row_stride = x_row_stride;
+  p.xq = static_cast<const uint8_t*>(xq);
+  p.xq_row_stride = xq_row_stride;
+  p.x_scale = static_cast<const uint16_t*>(x_scale);
+  p.router = static_cast<const uint16_t*>(router);
+  p.w13 = static_cast<const uint8_t*>(w13);
+  p.w13_scale = static_cast<const uint16_t*>(w13_scale);
+  p.w2 = static_cast<const uint8_t*>(w2);
+  p.w2_scale = static_cast<const uint16_t*>(w2_scale);
+  p.out = static_cast<uint16_t*>(out);
+  p.out_row_stride = out_row_stride;
+  p.ids = topk_ids;
+  p.weights = topk_weights;
+  p.renormalize = renormalize ? 1 : 0;
+  p.err = error;
+  fp8attn::moe_layout(p, workspace, sms);
+  const cudaError_t e = fp8attn::launch_moe(p, sms, static_cast<cudaStream_t>(stream));
+  if (e == cudaErrorInvalidValue) return fail(FP8ATTN_EINVAL, "moe: launch rejected");
+  return e == cudaSuccess ? FP8ATTN_OK : cuda_fail(e, "moe launch");
+}
+
+}  // extern "C"

@@ -105,6 +105,70 @@ struct Fp8TpParams {
 cudaError_t launch_fp8_tp_gemm(const Fp8GemmParams& p, const Fp8TpParams& tp, int num_sms,
                                cudaStream_t stream);
 
+// ------------------------------------------------------------------ FP8 feed-forward activations
+// add + RMS norm with an 8-bit output (per row and 128 columns one bf16 scale).
+struct NormQuantParams {
+  const uint16_t* x;         // bf16 or fp16 [M, K], rows x_row_stride elements apart
+  int64_t x_row_stride;
+  const uint16_t* residual;  // the same type, or null
+  int64_t residual_row_stride;
+  const uint16_t* weight;    // [K], the same type
+  float eps;
+  uint8_t* q;                // e4m3 [M, K]
+  uint16_t* scale;           // bf16 [M, K / 128]
+  uint16_t* residual_out;    // [M, K]: x + residual (null without a residual; may be the residual)
+  uint16_t* norm_out;        // [M, K]: the unquantised result, or null
+  int64_t M;
+  int K;
+  int fp16;                  // 0: bf16, 1: fp16
+};
+constexpr int kNormMaxColumns = 16384;
+cudaError_t launch_add_rms_norm_quant(const NormQuantParams& p, cudaStream_t stream);
+
+// silu(gate) * up with an 8-bit output.
+struct SiluQuantParams {
+  const uint16_t* gate_up;  // bf16 or fp16 [M, 2 I]: gate columns, then up; rows row_stride apart
+  int64_t row_stride;
+  uint8_t* q;               // e4m3 [M, I]
+  uint16_t* scale;          // bf16 [M, I / 128]
+  int64_t M;
+  int I;
+  int fp16;
+};
+cudaError_t launch_silu_mul_quant(const SiluQuantParams& p, cudaStream_t stream);
+
+// ------------------------------------------------------------------ mixture of experts
+constexpr int kMoeMaxExperts = 512;
+constexpr int kMoeMaxTopK = 32;
+constexpr int kMoeMaxTokens = 1024;
+constexpr int kMoeMaxSlots = 8192;  // tokens * top_k
+struct MoeParams {
+  const uint16_t* x;  // bf16 [T, H] (router)
+  int64_t x_row_stride;
+  const uint8_t* xq;  // e4m3 [T, H], rows xq_row_stride bytes apart
+  int64_t xq_row_stride;
+  const uint16_t* x_scale;    // bf16 [T, H / 128]
+  const uint16_t* router;     // bf16 [E, H]
+  const uint8_t* w13;         // e4m3 [E, 2 I, H]: gate rows, then up rows
+  const uint16_t* w13_scale;  // bf16 [E, 2 I / 128, H / 128]
+  const uint8_t* w2;          // e4m3 [E, H, I]
+  const uint16_t* w2_scale;   // bf16 [E, H / 128, I / 128]
+  uint16_t* out;              // bf16 [T, H], rows out_row_stride elements apart
+  int64_t out_row_stride;
+  int32_t* ids;    // [T, top_k]: the caller's, or in the workspace
+  float* weights;  // [T, top_k]
+  int64_t T;
+  int H, I, E, top_k, renormalize;
+  int* err;  // device error word, or null
+  // workspace
+  uint8_t* hq;        // e4m3 [T top_k, I]
+  uint16_t* h_scale;  // bf16 [T top_k, I / 128]
+  float* y;           // fp32 [T top_k, H]
+};
+// Lays the workspace out (pointers set where `workspace` is not null); returns its bytes.
+int64_t moe_layout(MoeParams& p, void* workspace, int num_sms);
+cudaError_t launch_moe(const MoeParams& p, int num_sms, cudaStream_t stream);
+
 // ------------------------------------------------------------------ decode engine
 // Control block at the head of the decode workspace (ints):
 //   [0] sticky device error code, [1] next work item, [2] CTAs finished.

@@ -12,6 +12,7 @@ import re
 from .build import LIB_PATH, INCLUDE
 
 OK, EINVAL, EWORKSPACE, ECUDA = 0, 1, 2, 3
+BF16, FP16 = 0, 1  # FP8ATTN_BF16, FP8ATTN_FP16
 WS_ERROR_OFFSET = 0
 NOALLOC_SCRATCH_BYTES = 32 << 20  # FP8ATTN_NOALLOC_SCRATCH_BYTES
 
@@ -69,6 +70,16 @@ def _load() -> ctypes.CDLL:
                                           i64, i32, i32, vp, i64, vp]
     lib.fp8attn_fp8_block_linear.restype = i32
     lib.fp8attn_fp8_block_linear.argtypes = [vp, i64, vp, vp, vp, i64, i64, i32, i32, vp, i64, vp]
+    lib.fp8attn_add_rms_norm_quant.restype = i32
+    lib.fp8attn_add_rms_norm_quant.argtypes = [vp, i64, vp, i64, vp, f32, vp, vp, vp, vp, i64, i32,
+                                               i32, vp]
+    lib.fp8attn_silu_mul_quant.restype = i32
+    lib.fp8attn_silu_mul_quant.argtypes = [vp, i64, vp, vp, i64, i32, i32, vp]
+    lib.fp8attn_fp8_moe_workspace_bytes.restype = i64
+    lib.fp8attn_fp8_moe_workspace_bytes.argtypes = [i64, i32, i32, i32, i32]
+    lib.fp8attn_fp8_moe.restype = i32
+    lib.fp8attn_fp8_moe.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp, vp, i64,
+                                    i32, i32, i32, i32, i32, vp, i64, vp, vp]
     lib.fp8attn_diag_wait_timeout.restype = i32
     lib.fp8attn_diag_wait_timeout.argtypes = [vp, i64, i32, vp]
     lib.fp8attn_diag_exp2.restype = i32
