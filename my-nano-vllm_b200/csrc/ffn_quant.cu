@@ -70,10 +70,21 @@ __device__ __forceinline__ uint2 quantise8(const float (&y)[8], float& scale, un
   for (int off = 8; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, off));
   scale = __fdiv_rn(a, 448.0f);
   if (!(scale > 0.f)) scale = 1.0f;
+  // y / d as y times 1 / d, an ulp from the quotient (31 instead of 60 instructions an element in the
+  // SiLU kernel), but for scales whose inverse overflows
+  float v[8];
+  if (scale > 1.0e-37f) {
+    const float inv = __frcp_rn(scale);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = y[i] * inv;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(y[i], scale);
+  }
   uint32_t b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)  // saturating: a quotient may round to just above 448
-    b[i] = f32x2_to_e4m3x2(__fdiv_rn(y[2 * i], scale), __fdiv_rn(y[2 * i + 1], scale));
+    b[i] = f32x2_to_e4m3x2(v[2 * i], v[2 * i + 1]);
   return make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
 }
 
@@ -170,7 +181,7 @@ __global__ void __launch_bounds__(kSiluThreads) silu_mul_quant_kernel(const Silu
   widen8<T>(gr, g);
   widen8<T>(ur, u);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) g[k] = __fdiv_rn(g[k], 1.0f + expf(-g[k])) * u[k];
+  for (int k = 0; k < 8; ++k) g[k] = __fdividef(g[k], 1.0f + expf(-g[k])) * u[k];
   float scale;
   const uint2 q = quantise8(g, scale, mask);
   *reinterpret_cast<uint2*>(p.q + row * p.I + 8 * v) = q;

@@ -600,8 +600,8 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// [rows, row_bytes] e4m3 (row stride `stride` bytes) in boxes of 128 bytes x box_rows rows, 128B
-// swizzle; rows past the end read as zeros.
+}  // namespace
+
 bool make_rows_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes,
                    int64_t stride, int box_rows) {
   EncodeTiledFn fn = encode_fn();
@@ -614,8 +614,6 @@ bool make_rows_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row
             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
-}  // namespace
 
 cudaError_t launch_fp8_dyn_quant(const Fp8QuantParams& p, cudaStream_t stream) {
   const int64_t groups = p.M * (p.K / kBlk);

@@ -81,6 +81,10 @@ struct Fp8GemmParams {
   int splits;               // K blocks are divided into this many ranges (one unit each)
 };
 constexpr int kFp8GemmTokens = 128;  // tokens per work unit (the MMA's N)
+// [rows, row_bytes] e4m3 (row stride `stride` bytes) in boxes of 128 bytes x box_rows rows, 128B
+// swizzle; rows past the end read as zeros.
+bool make_rows_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes,
+                   int64_t stride, int box_rows);
 int fp8_gemm_splits(int64_t M, int N, int K, int num_sms);
 int64_t fp8_gemm_workspace_bytes(int64_t M, int N, int K, int num_sms);
 cudaError_t launch_fp8_block_gemm(const Fp8GemmParams& p, int num_sms, cudaStream_t stream);
@@ -161,9 +165,12 @@ struct MoeParams {
   int H, I, E, top_k, renormalize;
   int* err;  // device error word, or null
   // workspace
+  int* counters;      // see moe_layout
+  int64_t num_counters;
   uint8_t* hq;        // e4m3 [T top_k, I]
   uint16_t* h_scale;  // bf16 [T top_k, I / 128]
   float* y;           // fp32 [T top_k, H]
+  float* parts[2];    // sums of cut items, by phase
 };
 // Lays the workspace out (pointers set where `workspace` is not null); returns its bytes.
 int64_t moe_layout(MoeParams& p, void* workspace, int num_sms);

@@ -9,49 +9,58 @@
 //
 // Products are block scaled: the exact dot of 128 columns times (activation scale * weight scale),
 // summed over the blocks in fp32.  A slot is a (token, place in its top-k) pair, n = T top_k of them.
+//
+// Bound: HBM, by the weights of the experts that are chosen (a token's 38 MB of small experts take
+// 6 us, its products 0.05 us), so the weights have to stream without a pause.  Two kernels:
+//
+// moe_router_kernel: a cluster of 8 CTAs per few tokens; its warps share the experts' rows, the
+//   logits meet in distributed shared memory, one warp per token chooses.
+// moe_experts_kernel: one CTA per SM, both products.  Tokens are sorted by expert into tiles of up to
+//   NT (16 or 64).  An item is 128 output columns of a tile (phase 0: 128 of gate and the same of up;
+//   phase 1: 128 of the result), a unit one step of its sum, 32 KB of weights (phase 0: 128 columns of
+//   K for both halves; phase 1: 256 columns of K).  A phase's units, items in order, are cut into
+//   equal ranges, one per CTA, wherever the cuts fall (few tokens make few items): the parts of a cut
+//   item are added, in order, by the CTA that finishes last.  CTAs take ranges by tickets, phase 0
+//   first; phase 1 of a tile waits for its hidden values (a counter), which are held by ranges with
+//   lower tickets, that is by CTAs that run, so the wait ends whatever else is on the GPU; meanwhile
+//   the ring already holds the weights.  Sums run in an order that the choice of experts alone
+//   fixes: results do not depend on timing.
+//   Warps: one issues weight tiles by TMA, four gather the tokens' rows (cp.async into the same
+//   swizzled layout) and scale products, one issues tcgen05 MMAs (D[128 weight rows, N tokens] per
+//   128 columns of K, weights and tokens both from shared memory), eight take D from tensor memory,
+//   scale and add it, and finish items.
 #include <climits>
 #include <type_traits>
 
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "kernels.h"
+#include "tcgen05.cuh"
 
 namespace fp8attn {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kBlk = 128;
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t b) {
   return __uint_as_float(static_cast<uint32_t>(b) << 16);
 }
-__device__ __forceinline__ float e4m3_to_f32(uint8_t b) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
+__device__ __forceinline__ uint16_t f32_to_bf16(float x) {
+  return __bfloat16_as_ushort(__float2bfloat16_rn(x));
 }
 
 // ------------------------------------------------------------------ router
-// One CTA per token.  Logits: fp32 products of 8 columns at a time, added up in fp64, so that which
-// experts are chosen does not hang on the order of a sum.
 constexpr int kRouterThreads = 256;
+constexpr int kRouterCluster = 8;
 constexpr int kExpertsPerLane = kMoeMaxExperts / 32;
 
-__global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoeParams p) {
-  __shared__ float logits[kMoeMaxExperts];
-  const int64_t token = blockIdx.x;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint16_t* x = p.x + token * p.x_row_stride;
-  for (int e = warp; e < p.E; e += kRouterThreads / 32) {
-    const uint16_t* w = p.router + static_cast<int64_t>(e) * p.H;
-    double acc = 0.0;
-    for (int c = 8 * lane; c < p.H; c += 256) {
-      float s = 0.f;
-      for (int i = 0; i < 8; ++i) s = fmaf(bf16_to_f32(x[c + i]), bf16_to_f32(w[c + i]), s);
-      acc += s;
-    }
-    for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-    if (lane == 0) logits[e] = static_cast<float>(acc);
-  }
-  __syncthreads();
-  if (warp != 0) return;
-  // top-k: every lane keeps experts lane, lane + 32, ...; a NaN logit is chosen last
+// One token's choice by one warp, its logits in shared memory.
+__device__ __forceinline__ void choose_experts(const MoeParams& p, int64_t token,
+                                               const float* logits, int lane) {
+  // lane keeps experts lane, lane + 32, ...; a NaN logit is chosen last
   float v[kExpertsPerLane];
   uint32_t taken = 0;
 #pragma unroll
@@ -108,85 +117,718 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const MoePar
   }
 }
 
-// ------------------------------------------------------------------ products
-// Sum over the blocks of one weight row, the activation row (values and scales) in shared memory.
-__device__ float block_scaled_dot(const uint8_t* w, const uint16_t* w_scale, const float* a,
-                                  const float* a_scale, int K) {
-  float acc = 0.f;
-  for (int kb = 0; kb < K / kBlk; ++kb) {
-    float d = 0.f;
-    for (int c = 0; c < kBlk; ++c) d = fmaf(a[kb * kBlk + c], e4m3_to_f32(w[kb * kBlk + c]), d);
-    acc = fmaf(d, a_scale[kb] * bf16_to_f32(w_scale[kb]), acc);
+// Cluster c: tokens c kTok .. + kTok - 1.  Logits: fp32 products of 8 columns at a time, added up in
+// fp64, so that which experts are chosen does not hang on the order of a sum.
+template <int kTok>
+__global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads)
+    moe_router_kernel(const MoeParams p) {
+  static_assert(kTok <= kRouterCluster, "a CTA chooses for one token at most");
+  __shared__ float logits[kMoeMaxExperts];  // of token (cluster's first + this CTA's rank)
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();  // every CTA has started: its shared memory may be written
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // the counters of the next kernel
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kRouterThreads + threadIdx.x; i < p.num_counters;
+       i += static_cast<int64_t>(gridDim.x) * kRouterThreads)
+    p.counters[i] = 0;
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x / kRouterCluster) * kTok;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int e = rank * (kRouterThreads / 32) + warp; e < p.E; e += kRouterCluster * kRouterThreads / 32) {
+    const uint16_t* w = p.router + static_cast<int64_t>(e) * p.H;
+    double acc[kTok];
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) acc[t] = 0.0;
+#pragma unroll 4
+    for (int c = 8 * lane; c < p.H; c += 256) {
+      const uint4 wr = __ldg(reinterpret_cast<const uint4*>(w + c));
+      const uint32_t ww[4] = {wr.x, wr.y, wr.z, wr.w};
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) {
+        const int64_t token = min(t0 + t, p.T - 1);
+        const uint4 xr = *reinterpret_cast<const uint4*>(p.x + token * p.x_row_stride + c);
+        const uint32_t xx[4] = {xr.x, xr.y, xr.z, xr.w};
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s = fmaf(__uint_as_float(xx[i] << 16), __uint_as_float(ww[i] << 16), s);
+          s = fmaf(__uint_as_float(xx[i] & 0xFFFF0000u), __uint_as_float(ww[i] & 0xFFFF0000u), s);
+        }
+        acc[t] += s;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) {
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], off);
+      if (lane == t) *cluster.map_shared_rank(&logits[e], t) = static_cast<float>(acc[t]);
+    }
   }
-  return acc;
+  cluster.sync();
+  if (warp == 0 && rank < kTok && t0 + rank < p.T) choose_experts(p, t0 + rank, logits, lane);
 }
 
-// CTA (slot, 128 columns of I): threads 0-127 the gate rows, 128-255 the up rows.
-__global__ void __launch_bounds__(256) moe_gate_up_kernel(const MoeParams p) {
-  extern __shared__ float sh[];
-  __shared__ float up[kBlk], warp_max[4];
-  const int slot = blockIdx.x, ib = blockIdx.y, t = threadIdx.x;
-  const int64_t token = slot / p.top_k;
-  const int e = p.ids[slot];
-  const int kc = p.H / kBlk;
-  float *a = sh, *as = sh + p.H;
-  for (int c = t; c < p.H; c += 256) a[c] = e4m3_to_f32(p.xq[token * p.xq_row_stride + c]);
-  for (int c = t; c < kc; c += 256) as[c] = bf16_to_f32(p.x_scale[token * kc + c]);
-  __syncthreads();
-  const int r = t & 127, half = t >> 7;
-  const int64_t row = static_cast<int64_t>(e) * 2 * p.I + half * p.I + ib * kBlk + r;
-  const float y = block_scaled_dot(p.w13 + row * p.H, p.w13_scale + row / kBlk * kc, a, as, p.H);
-  if (half) up[r] = y;
-  __syncthreads();
-  float h = 0.f;
-  if (!half) {
-    h = __fdiv_rn(y, 1.0f + expf(-y)) * up[r];
-    float m = fmaxf(fabsf(h), 0.f);
-    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    if ((r & 31) == 0) warp_max[r / 32] = m;
-  }
-  __syncthreads();
-  if (half) return;
-  const float m = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
-  float scale = __fdiv_rn(m, 448.0f);
-  if (!(scale > 0.f)) scale = 1.0f;
-  p.hq[static_cast<int64_t>(slot) * p.I + ib * kBlk + r] =
-      static_cast<uint8_t>(f32x2_to_e4m3x2(__fdiv_rn(h, scale), 0.f) & 0xFFu);
-  if (r == 0)
-    p.h_scale[static_cast<int64_t>(slot) * (p.I / kBlk) + ib] =
-        __bfloat16_as_ushort(__float2bfloat16_rn(scale));
+// ------------------------------------------------------------------ experts
+constexpr int kPromoWarps = 8;  // warps 0-7
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kLoaderWarp = 10;  // and after
+// Gather warps.  With 64 tokens a tile only two, so that 12 warps leave the promotion threads, whose
+// sums take 64 registers, 168 of them (14 warps: 128, and 1.5 KB of spills).
+template <int NT>
+constexpr int kLoaders = NT == 16 ? 4 : 2;
+template <int NT>
+constexpr int moe_warps = kLoaderWarp + kLoaders<NT>;
+constexpr int kDBufs = 4;
+constexpr int kMaxTiles = 640;  // experts + slots / 64, or slots of 16 tokens
+static_assert(kMoeMaxExperts + kMoeMaxSlots / 64 <= kMaxTiles && 16 * kMoeMaxTopK <= kMaxTiles, "tiles");
+
+// Units [begin, end) of one phase.
+struct Phase {
+  int blocks;   // items per tile (output columns / 128)
+  int steps;    // units per item
+  int ranges;   // equal ranges the units are cut into
+  int whole;    // cut between items only
+  int units;
+  int items;
+};
+__device__ __forceinline__ int range_begin(const Phase& f, int r) {
+  return f.whole ? static_cast<int>(static_cast<int64_t>(f.items) * r / f.ranges) * f.steps
+                 : static_cast<int>(static_cast<int64_t>(f.units) * r / f.ranges);
+}
+// The range that holds unit x (not whole): the largest r with floor(units r / ranges) <= x.
+__device__ __forceinline__ int range_of(const Phase& f, int x) {
+  return static_cast<int>((static_cast<int64_t>(x + 1) * f.ranges + f.units - 1) / f.units) - 1;
 }
 
-// CTA (slot, 128 columns of H).
-__global__ void __launch_bounds__(128) moe_down_kernel(const MoeParams p) {
-  extern __shared__ float sh[];
-  const int slot = blockIdx.x, hb = blockIdx.y, t = threadIdx.x;
-  const int e = p.ids[slot];
-  const int kc = p.I / kBlk;
-  float *a = sh, *as = sh + p.I;
-  for (int c = t; c < p.I; c += 128) a[c] = e4m3_to_f32(p.hq[static_cast<int64_t>(slot) * p.I + c]);
-  for (int c = t; c < kc; c += 128) as[c] = bf16_to_f32(p.h_scale[static_cast<int64_t>(slot) * kc + c]);
-  __syncthreads();
-  const int64_t row = static_cast<int64_t>(e) * p.H + hb * kBlk + t;
-  p.y[static_cast<int64_t>(slot) * p.H + hb * kBlk + t] =
-      block_scaled_dot(p.w2 + row * p.I, p.w2_scale + row / kBlk * kc, a, as, p.I);
+template <int NT>
+struct __align__(1024) MoeSmem {
+  static constexpr int kStages = NT == 16 ? 5 : 4;
+  uint8_t w[kStages][2][kBlk * kBlk];  // weight tiles: 128 rows x 128 bytes, 128B swizzle
+  uint8_t x[kStages][2][NT * kBlk];    // token tiles: NT rows x 128 bytes, 128B swizzle
+  float scale[kStages][2][NT];         // activation scale * weight scale of the stage's two tiles
+  float amax[4][NT];                   // a quadrant's largest |h| per token
+  uint64_t w_full[kStages], x_full[kStages], empty[kStages];
+  uint64_t d_full[kDBufs], d_empty[kDBufs];
+  uint64_t claim_full[2], claim_empty[2];
+  int claim[2];
+  Phase phase[2];
+  int last;                            // promotion threads: this CTA finishes the item
+  int done[NT];                        // ... and the token
+  uint32_t tmem_base;
+  int tiles;
+  uint32_t tile[kMaxTiles];            // expert << 16 | index of the tile among the expert's
+  uint16_t first[kMoeMaxExperts + 1];  // the expert's slots: order[first[e] .. first[e + 1])
+  uint16_t order[kMoeMaxSlots];        // slots by expert (the last member: NT = 16 needs 512 of them)
+};
+constexpr int kOrder16 = 16 * kMoeMaxTopK;
+template <int NT>
+constexpr size_t moe_smem_bytes() {
+  return sizeof(MoeSmem<NT>) - (NT == 16 ? (kMoeMaxSlots - kOrder16) * 2 : 0) + 1024;
+}
+static_assert(moe_smem_bytes<16>() <= 227 * 1024 && moe_smem_bytes<64>() <= 227 * 1024, "smem");
+
+__device__ __forceinline__ void promo_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
 }
 
-__global__ void __launch_bounds__(128) moe_combine_kernel(const MoeParams p) {
-  const int64_t token = blockIdx.x;
-  const int c = blockIdx.y * 128 + threadIdx.x;
-  float acc = 0.f;
-  for (int k = 0; k < p.top_k; ++k) {
-    const int64_t slot = token * p.top_k + k;
-    acc = fmaf(p.weights[slot], p.y[slot * p.H + c], acc);
+// Wait until *p >= want; gives up after kWaitLimitNs, recording kDevErrWaitTimeout.
+__device__ __forceinline__ bool wait_counter(const int* p, int want, int* err) {
+  unsigned long long t0 = 0;
+  for (uint32_t polls = 1;; ++polls) {
+    if (load_acquire(p) >= want) return true;
+    if ((polls & 255u) == 0) {
+      const unsigned long long now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > kWaitLimitNs) {
+        if (err) atomicExch(err, kDevErrWaitTimeout);
+        return false;
+      }
+    }
   }
-  p.out[token * p.out_row_stride + c] = __bfloat16_as_ushort(__float2bfloat16_rn(acc));
+}
+
+// Slots sorted by expert (stable: results must not depend on timing), the tiles, and the two phases'
+// cuts; every CTA does the same.  Scratch in the ring, which is not in use yet.
+template <int NT>
+__device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
+  constexpr int kWarps = moe_warps<NT>, kThreads = kWarps * 32;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int n = static_cast<int>(p.T) * p.top_k, E = p.E;
+  uint16_t* const eid = reinterpret_cast<uint16_t*>(&sm.w[0][0][0]);          // [n]
+  uint16_t* const hist = reinterpret_cast<uint16_t*>(&sm.w[1][0][0]);         // [kWarps][E]
+  uint16_t* const total = hist + kWarps * kMoeMaxExperts;                     // [E]
+  static_assert(kMoeMaxSlots * 2 <= 2 * kBlk * kBlk, "expert ids fit a stage");
+  static_assert((kWarps + 1) * kMoeMaxExperts * 2 <= 2 * kBlk * kBlk, "histograms fit a stage");
+  for (int i = tid; i < kWarps * E; i += kThreads) hist[i] = 0;
+  const int per = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;  // a warp's slots: [warp per, + per)
+  const int lo = min(warp * per, n), hi = min(lo + per, n);
+  __syncthreads();
+  for (int i0 = lo; i0 < hi; i0 += 32) {
+    const int i = i0 + lane;
+    const bool ok = i < hi;
+    const int e = ok ? min(max(p.ids[i], 0), E - 1) : -1;
+    if (ok) eid[i] = static_cast<uint16_t>(e);
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    if (ok && lane == __ffs(same) - 1) hist[warp * E + e] += static_cast<uint16_t>(__popc(same));
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int e = tid; e < E; e += kThreads) {  // a warp's counts -> where its slots of e begin
+    int sum = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      const int c = hist[w * E + e];
+      hist[w * E + e] = static_cast<uint16_t>(sum);
+      sum += c;
+    }
+    total[e] = static_cast<uint16_t>(sum);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int slots = 0, tiles = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane;
+      const int c = e < E ? total[e] : 0;
+      const int nt = (c + NT - 1) / NT;
+      int cs = c, ts = nt;  // inclusive sums over the lanes
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, cs, off), b = __shfl_up_sync(0xffffffffu, ts, off);
+        if (lane >= off) {
+          cs += a;
+          ts += b;
+        }
+      }
+      if (e < E) {
+        sm.first[e] = static_cast<uint16_t>(slots + cs - c);
+        for (int j = 0; j < nt; ++j)
+          sm.tile[tiles + ts - nt + j] = static_cast<uint32_t>(e) << 16 | static_cast<uint32_t>(j);
+      }
+      slots += __shfl_sync(0xffffffffu, cs, 31);
+      tiles += __shfl_sync(0xffffffffu, ts, 31);
+    }
+    if (lane == 0) sm.first[E] = static_cast<uint16_t>(slots);
+    if (lane < 2) {
+      Phase f;
+      f.blocks = lane == 0 ? p.I / kBlk : p.H / kBlk;
+      f.steps = lane == 0 ? p.H / kBlk : (p.I / kBlk + 1) / 2;
+      f.items = tiles * f.blocks;
+      f.units = f.items * f.steps;
+      // Whole items where that costs at most 2 units' time more than equal ranges: a cut item's
+      // parts go through memory
+      const int grid = static_cast<int>(gridDim.x);
+      const int even = (f.units + grid - 1) / grid;
+      f.whole = (f.items + grid - 1) / grid * f.steps <= even + 2;
+      f.ranges = min(grid, f.whole ? f.items : f.units);
+      sm.phase[lane] = f;
+    }
+    if (lane == 0) sm.tiles = tiles;
+  }
+  __syncthreads();
+  for (int i0 = lo; i0 < hi; i0 += 32) {
+    const int i = i0 + lane;
+    const bool ok = i < hi;
+    const int e = ok ? eid[i] : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    if (ok)
+      sm.order[sm.first[e] + hist[warp * E + e] + __popc(same & ((1u << lane) - 1))] =
+          static_cast<uint16_t>(i);
+    __syncwarp();
+    if (ok && lane == __ffs(same) - 1) hist[warp * E + e] += static_cast<uint16_t>(__popc(same));
+    __syncwarp();
+  }
+  // the ring's next writer is the async proxy
+  fence_proxy_async_smem();
+  __syncthreads();
+}
+
+// A range's place in the work: item (tile, blk), step k of it; advances unit by unit.
+struct Cursor {
+  int tile, blk, k;
+  __device__ __forceinline__ Cursor(const Phase& f, int unit) {
+    const int item = unit / f.steps;
+    k = unit - item * f.steps;
+    tile = item / f.blocks;
+    blk = item - tile * f.blocks;
+  }
+  __device__ __forceinline__ void next(const Phase& f) {
+    if (++k == f.steps) {
+      k = 0;
+      if (++blk == f.blocks) {
+        blk = 0;
+        ++tile;
+      }
+    }
+  }
+};
+
+template <int NT>
+struct Tile {
+  int expert, begin, count;  // slots order[begin .. begin + count)
+  __device__ __forceinline__ Tile(const MoeSmem<NT>& sm, int tile) {
+    const uint32_t t = sm.tile[tile];
+    expert = static_cast<int>(t >> 16);
+    begin = sm.first[expert] + static_cast<int>(t & 0xFFFFu) * NT;
+    count = min(NT, sm.first[expert + 1] - begin);
+  }
+  __device__ __forceinline__ int columns() const { return (count + 15) & ~15; }  // the MMA's N
+};
+
+// The next range, for every warp but the producer.  False: no more.
+template <int NT>
+__device__ __forceinline__ bool next_claim(MoeSmem<NT>& sm, int i, int lane, int* err, int& ticket) {
+  if (!mbar_wait(&sm.claim_full[i & 1], (i >> 1) & 1, err)) return false;
+  ticket = sm.claim[i & 1];
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&sm.claim_empty[i & 1]);
+  return ticket >= 0;
+}
+
+template <int NT>
+__device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* tm13,
+                        const CUtensorMap* tm2) {
+  constexpr int kStages = MoeSmem<NT>::kStages;
+  const int total = sm.phase[0].ranges + sm.phase[1].ranges;
+  uint32_t r = 0;
+  bool ok = true;
+  int ticket = atomicAdd(p.counters, 1);
+  for (int i = 0;; ++i) {
+    ok = ok && mbar_wait(&sm.claim_empty[i & 1], ((i >> 1) & 1) ^ 1, p.err);
+    const bool more = ok && ticket < total;
+    sm.claim[i & 1] = more ? ticket : -1;
+    mbar_arrive(&sm.claim_full[i & 1]);
+    if (!more) return;
+    const int ph = ticket >= sm.phase[0].ranges;
+    const Phase f = sm.phase[ph];
+    const int range = ticket - (ph ? sm.phase[0].ranges : 0);
+    const int begin = range_begin(f, range), end = range_begin(f, range + 1);
+    Cursor c(f, begin);
+    for (int u = begin; u < end && ok; ++u, ++r, c.next(f)) {
+      // the next ticket: its latency hides behind this range, whose first half lets a CTA that starts
+      // late have its turn (one that held two ranges of a phase would take twice as long)
+      if (u == begin + (end - begin) / 2) ticket = atomicAdd(p.counters, 1);
+      const int stage = r % kStages;
+      const int expert = static_cast<int>(sm.tile[c.tile] >> 16);
+      if (!mbar_wait(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err)) {
+        ok = false;
+        break;
+      }
+      if (ph == 0) {
+        mbar_arrive_expect_tx(&sm.w_full[stage], 2 * kBlk * kBlk);
+        const int row = expert * 2 * p.I + c.blk * kBlk;
+        tma_load_2d(sm.w[stage][0], tm13, &sm.w_full[stage], c.k * kBlk, row);
+        tma_load_2d(sm.w[stage][1], tm13, &sm.w_full[stage], c.k * kBlk, row + p.I);
+      } else {
+        const bool two = (2 * c.k + 1) * kBlk < p.I;
+        mbar_arrive_expect_tx(&sm.w_full[stage], (two ? 2 : 1) * kBlk * kBlk);
+        const int row = expert * p.H + c.blk * kBlk;
+        tma_load_2d(sm.w[stage][0], tm2, &sm.w_full[stage], 2 * c.k * kBlk, row);
+        if (two) tma_load_2d(sm.w[stage][1], tm2, &sm.w_full[stage], (2 * c.k + 1) * kBlk, row);
+      }
+    }
+  }
+}
+
+// One of the gather warps: its share of the units, round robin, so that the loads of several are in
+// flight.
+template <int NT>
+__device__ void gather(MoeSmem<NT>& sm, const MoeParams& p, int which, int lane) {
+  constexpr int kStages = MoeSmem<NT>::kStages;
+  const int kc1 = p.H / kBlk, kc2 = p.I / kBlk;
+  uint32_t r = 0;
+  bool ok = true;
+  int ticket;
+  for (int i = 0; next_claim(sm, i, lane, p.err, ticket); ++i) {
+    const int ph = ticket >= sm.phase[0].ranges;
+    const Phase f = sm.phase[ph];
+    const int range = ticket - (ph ? sm.phase[0].ranges : 0);
+    const int begin = range_begin(f, range), end = range_begin(f, range + 1);
+    Cursor c(f, begin);
+    int ready = -1;
+    for (int u = begin; u < end; ++u, ++r, c.next(f)) {
+      if (static_cast<int>(r % kLoaders<NT>) != which) continue;
+      const int stage = r % kStages;
+      const Tile<NT> t(sm, c.tile);
+      if (ok && ph == 1 && c.tile != ready) {
+        // the tile's hidden values: written by other CTAs
+        ok = wait_counter(p.counters + 1 + c.tile, kc2, p.err);
+        ready = c.tile;
+      }
+      ok = ok && mbar_wait(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err);
+      if (!ok) continue;  // the others stop by themselves: their waits on this stage end, bounded
+      const int subs = ph == 0 ? 1 : (2 * c.k + 1 < kc2 ? 2 : 1);
+      // scale products, lane = token (and token + 32); loads issued before the copies
+      float s[2][NT > 32 ? 2 : 1];
+#pragma unroll
+      for (int h = 0; h < (NT > 32 ? 2 : 1); ++h) {
+        const int m = lane + 32 * h;
+        s[0][h] = s[1][h] = 0.f;
+        if (m < t.count) {
+          const int slot = sm.order[t.begin + m];
+          if (ph == 0) {
+            const float xs = bf16_to_f32(__ldg(p.x_scale + static_cast<int64_t>(slot / p.top_k) * kc1 + c.k));
+            const uint16_t* ws =
+                p.w13_scale + (static_cast<int64_t>(t.expert) * 2 * kc2 + c.blk) * kc1 + c.k;
+            s[0][h] = xs * bf16_to_f32(__ldg(ws));
+            s[1][h] = xs * bf16_to_f32(__ldg(ws + static_cast<int64_t>(kc2) * kc1));
+          } else {
+            const uint16_t* hs = p.h_scale + static_cast<int64_t>(slot) * kc2 + 2 * c.k;
+            const uint16_t* ws = p.w2_scale + (static_cast<int64_t>(t.expert) * kc1 + c.blk) * kc2 + 2 * c.k;
+            s[0][h] = bf16_to_f32(__ldcg(hs)) * bf16_to_f32(__ldg(ws));
+            if (subs == 2) s[1][h] = bf16_to_f32(__ldcg(hs + 1)) * bf16_to_f32(__ldg(ws + 1));
+          }
+        }
+      }
+      // rows: 8 lanes copy a row's 128 bytes; rows past the tile's tokens are zeros
+      const int rows = t.columns(), chunk = lane & 7;
+      for (int m = lane >> 3; m < rows; m += 4) {
+        const bool real = m < t.count;
+        const int slot = real ? sm.order[t.begin + m] : 0;
+        const uint8_t* src =
+            ph == 0 ? p.xq + static_cast<int64_t>(slot / p.top_k) * p.xq_row_stride + c.k * kBlk
+                    : p.hq + static_cast<int64_t>(slot) * p.I + 2 * c.k * kBlk;
+        const uint32_t at = m * kBlk + ((chunk ^ (m & 7)) << 4);
+        cp_async16(smem_u32(sm.x[stage][0]) + at, src + chunk * 16, real);
+        if (subs == 2) cp_async16(smem_u32(sm.x[stage][1]) + at, src + kBlk + chunk * 16, real);
+      }
+      cp_async_commit();
+#pragma unroll
+      for (int h = 0; h < (NT > 32 ? 2 : 1); ++h)
+        if (lane + 32 * h < NT) {
+          sm.scale[stage][0][lane + 32 * h] = s[0][h];
+          sm.scale[stage][1][lane + 32 * h] = s[1][h];
+        }
+      cp_async_wait<0>();
+      fence_proxy_async_smem();  // the tensor cores read the rows through the async proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.x_full[stage]);
+    }
+  }
+}
+
+template <int NT>
+__device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int lane) {
+  constexpr int kStages = MoeSmem<NT>::kStages;
+  const uint32_t tmem = sm.tmem_base;
+  uint32_t r = 0;
+  bool ok = true;
+  int ticket;
+  for (int i = 0; next_claim(sm, i, lane, p.err, ticket); ++i) {
+    if (lane == 0) {
+      const int ph = ticket >= sm.phase[0].ranges;
+      const Phase f = sm.phase[ph];
+      const int range = ticket - (ph ? sm.phase[0].ranges : 0);
+      const int begin = range_begin(f, range), end = range_begin(f, range + 1);
+      Cursor c(f, begin);
+      for (int u = begin; u < end && ok; ++u, ++r, c.next(f)) {
+        const int stage = r % kStages, buf = r % kDBufs;
+        ok = mbar_wait(&sm.w_full[stage], (r / kStages) & 1, p.err) &&
+             mbar_wait(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
+             mbar_wait(&sm.d_empty[buf], ((r / kDBufs) & 1) ^ 1, p.err);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const uint32_t idesc = tc::idesc_e4m3(kBlk, Tile<NT>(sm, c.tile).columns(), false, false);
+        const int subs = ph == 0 || (2 * c.k + 1) * kBlk < p.I ? 2 : 1;
+        for (int s = 0; s < subs; ++s) {
+          const uint64_t wd = tc::smem_desc(smem_u32(sm.w[stage][s]), 16, 1024, tc::kSw128);
+          const uint64_t xd = tc::smem_desc(smem_u32(sm.x[stage][ph == 0 ? 0 : s]), 16, 1024, tc::kSw128);
+#pragma unroll
+          for (int ks = 0; ks < kBlk / 32; ++ks)  // 32 bytes of K add 2 to the start address / 16
+            tc::mma_f8_plain(tmem + (buf * 2 + s) * NT, wd + static_cast<uint64_t>(2 * ks),
+                             xd + static_cast<uint64_t>(2 * ks), idesc, ks > 0 ? 1u : 0u);
+        }
+        tc::commit(&sm.d_full[buf]);
+        tc::commit(&sm.empty[stage]);
+      }
+    }
+    __syncwarp();
+  }
+}
+
+// acc[j] += d[j] * s[j] over one of the unit's two tiles: this thread's weight row, `groups` groups of 8
+// tokens from column `col`.
+template <int NT>
+__device__ __forceinline__ void scale_add(float (&acc)[NT / 2], uint32_t taddr, const float* s,
+                                          int groups) {
+  constexpr int kBatch = NT / 16 < 2 ? 1 : 2;  // loads in flight together; more of them spill
+#pragma unroll
+  for (int q0 = 0; q0 < NT / 16; q0 += kBatch) {
+    if (q0 >= groups) break;
+    float d[kBatch][8];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      if (q0 + q < groups) tc::ld8(taddr + 8 * (q0 + q), d[q]);
+    tc::wait_ld();
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      if (q0 + q < groups) {
+        const float4 a = *reinterpret_cast<const float4*>(s + 8 * (q0 + q));
+        const float4 b = *reinterpret_cast<const float4*>(s + 8 * (q0 + q) + 4);
+        const float sc[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          acc[8 * (q0 + q) + j] = fmaf(d[q][j], sc[j], acc[8 * (q0 + q) + j]);
+      }
+  }
+}
+
+// The promotion warps: warp w has tensor-memory lanes 32 (w % 4) .. + 31 (an item's output columns)
+// and half w / 4 of the tile's tokens.
+template <int NT>
+__device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane) {
+  constexpr int kStages = MoeSmem<NT>::kStages;
+  constexpr int kHalf = NT / 2;
+  const int quad = warp & 3, half = warp >> 2, tid = warp * 32 + lane;
+  const int col = 32 * quad + lane;  // output column of the item
+  const uint32_t tmem = sm.tmem_base + (static_cast<uint32_t>(32 * quad) << 16);
+  const int kc2 = p.I / kBlk;
+  int* const ready = p.counters + 1;
+  int* const part_count = ready + kMaxTiles;               // [2][grid]
+  int* const token_count = part_count + 2 * gridDim.x;     // [T][H / 128]
+  uint32_t r = 0;
+  bool ok = true;
+  int ticket;
+  for (int i = 0; next_claim(sm, i, lane, p.err, ticket); ++i) {
+    const int ph = ticket >= sm.phase[0].ranges;
+    const Phase f = sm.phase[ph];
+    const int range = ticket - (ph ? sm.phase[0].ranges : 0);
+    const int begin = range_begin(f, range), end = range_begin(f, range + 1);
+    Cursor c(f, begin);
+    int u = begin;
+    while (u < end) {
+      // ---- one item, or the part of it that this range holds
+      const Tile<NT> t(sm, c.tile);
+      const int groups = t.columns() / 16, m0 = half * 8 * groups;  // tokens m0 .. m0 + 8 groups - 1
+      const int item_begin = u - c.k;
+      const int stop = min(end, item_begin + f.steps);
+      const bool cut = u != item_begin || stop != item_begin + f.steps;
+      const int tile = c.tile, blk = c.blk;
+      float g[kHalf], v[kHalf];
+#pragma unroll
+      for (int j = 0; j < kHalf; ++j) g[j] = v[j] = 0.f;
+      const bool at_head = u != item_begin;
+      for (; u < stop; ++u, ++r, c.next(f)) {
+        const int stage = r % kStages, buf = r % kDBufs;
+        ok = ok && mbar_wait(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
+             mbar_wait(&sm.d_full[buf], (r / kDBufs) & 1, p.err);
+        if (!ok) continue;
+        tc::fence_after_sync();
+        const uint32_t d = tmem + buf * 2 * NT + m0;
+        scale_add<NT>(g, d, &sm.scale[stage][0][m0], groups);
+        if (ph == 0) {
+          scale_add<NT>(v, d + NT, &sm.scale[stage][1][m0], groups);
+        } else if (2 * c.k + 1 < kc2) {
+          scale_add<NT>(g, d + NT, &sm.scale[stage][1][m0], groups);
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.d_empty[buf]);
+          mbar_arrive(&sm.empty[stage]);
+        }
+      }
+      // ---- the parts of a cut item meet in memory; the CTA that comes last adds them, in order
+      if (cut) {
+        constexpr int kPart = NT * kBlk;  // floats; phase 0 has two of them (gate, up)
+        float* const parts = ph == 0 ? p.parts[0] : p.parts[1];
+        const int64_t size = ph == 0 ? 2 * kPart : kPart;
+        float* mine = parts + (2 * static_cast<int64_t>(range) + (at_head ? 0 : 1)) * size;
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j)
+          if (j < 8 * groups) {
+            __stcg(mine + (m0 + j) * kBlk + col, g[j]);
+            if (ph == 0) __stcg(mine + kPart + (m0 + j) * kBlk + col, v[j]);
+          }
+        const int r0 = range_of(f, item_begin), r1 = range_of(f, item_begin + f.steps - 1);
+        promo_sync();
+        if (tid == 0) {
+          __threadfence();
+          const int before = atomicAdd(part_count + ph * gridDim.x + r0, 1);
+          __threadfence();
+          sm.last = before == r1 - r0;
+        }
+        promo_sync();
+        if (!sm.last) continue;
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) g[j] = v[j] = 0.f;
+        for (int q = r0; q <= r1; ++q) {
+          const float* part = parts + (2 * static_cast<int64_t>(q) + (q == r0 ? 1 : 0)) * size;
+#pragma unroll
+          for (int j = 0; j < kHalf; ++j)
+            if (j < 8 * groups) {
+              g[j] += __ldcg(part + (m0 + j) * kBlk + col);
+              if (ph == 0) v[j] += __ldcg(part + kPart + (m0 + j) * kBlk + col);
+            }
+        }
+      }
+      if (ph == 0) {
+        // ---- h = silu(g) u, quantised over the item's 128 columns (4 quadrants of 32 lanes)
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j)
+          if (j < 8 * groups) {
+            g[j] = __fdividef(g[j], 1.0f + expf(-g[j])) * v[j];
+            const float a = g[j] == g[j] ? fabsf(g[j]) : 0.f;  // NaN left out
+            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(a));
+            if (lane == (j & 31)) sm.amax[quad][m0 + j] = __uint_as_float(top);
+          }
+        promo_sync();
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j)
+          if (m0 + j < t.count && j < 8 * groups) {
+            const int m = m0 + j;
+            const float a = fmaxf(fmaxf(sm.amax[0][m], sm.amax[1][m]), fmaxf(sm.amax[2][m], sm.amax[3][m]));
+            float scale = __fdiv_rn(a, 448.0f);
+            if (!(scale > 0.f)) scale = 1.0f;
+            const int64_t slot = sm.order[t.begin + m];
+            p.hq[slot * p.I + blk * kBlk + col] =
+                static_cast<uint8_t>(f32x2_to_e4m3x2(__fdiv_rn(g[j], scale), 0.f) & 0xFFu);
+            if (col == 0) p.h_scale[slot * kc2 + blk] = f32_to_bf16(scale);
+          }
+        promo_sync();  // also: amax is free again
+        if (tid == 0) {
+          __threadfence();
+          atomicAdd(ready + tile, 1);
+        }
+      } else {
+        // ---- the slots' results; the CTA that brings a token its last adds the token's up
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j)
+          if (m0 + j < t.count && j < 8 * groups)
+            __stcg(p.y + static_cast<int64_t>(sm.order[t.begin + m0 + j]) * p.H + blk * kBlk + col, g[j]);
+        promo_sync();
+        if (tid < t.count) {
+          const int64_t token = sm.order[t.begin + tid] / p.top_k;
+          __threadfence();
+          const int before = atomicAdd(token_count + token * f.blocks + blk, 1);
+          __threadfence();
+          sm.done[tid] = before == p.top_k - 1;
+        }
+        promo_sync();
+        for (int m = tid >> 7; m < t.count; m += 2) {
+          if (!sm.done[m]) continue;
+          const int64_t token = sm.order[t.begin + m] / p.top_k;
+          const int at = blk * kBlk + (tid & 127);
+          const float* y = p.y + token * p.top_k * p.H + at;
+          float acc = 0.f;
+          for (int k = 0; k < p.top_k; ++k)
+            acc = fmaf(__ldg(p.weights + token * p.top_k + k), __ldcg(y + static_cast<int64_t>(k) * p.H), acc);
+          p.out[token * p.out_row_stride + at] = f32_to_bf16(acc);
+        }
+        promo_sync();  // done is free again
+      }
+    }
+  }
+}
+
+template <int NT>
+__global__ void __launch_bounds__(moe_warps<NT> * 32, 1)
+    moe_experts_kernel(const __grid_constant__ CUtensorMap tm13, const __grid_constant__ CUtensorMap tm2,
+                       const MoeParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  MoeSmem<NT>& sm = *reinterpret_cast<MoeSmem<NT>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  constexpr uint32_t kColumns = kDBufs * 2 * NT;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < MoeSmem<NT>::kStages; ++i) {
+      mbar_init(&sm.w_full[i], 1);
+      mbar_init(&sm.x_full[i], 1);
+      mbar_init(&sm.empty[i], 1 + kPromoWarps);
+    }
+    for (int i = 0; i < kDBufs; ++i) {
+      mbar_init(&sm.d_full[i], 1);
+      mbar_init(&sm.d_empty[i], kPromoWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.claim_full[i], 1);
+      mbar_init(&sm.claim_empty[i], kPromoWarps + 1 + kLoaders<NT>);
+    }
+    fence_mbar_init();
+  }
+  if (warp == kProducerWarp && lane == 0) {
+    prefetch_tensormap(&tm13);
+    prefetch_tensormap(&tm2);
+  }
+  if (warp == kMmaWarp) {
+    tc::tmem_alloc(&sm.tmem_base, kColumns);
+    tc::tmem_relinquish();
+  }
+  // launched as a programmatic dependent of the router: its choice is read only when it has ended
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  tc::fence_before_sync();
+  plan<NT>(sm, p);  // begins and ends with barriers of the whole CTA
+  tc::fence_after_sync();
+  if (warp == kProducerWarp) {
+    if (lane == 0) produce<NT>(sm, p, &tm13, &tm2);
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    multiply<NT>(sm, p, lane);
+  } else if (warp >= kLoaderWarp) {
+    gather<NT>(sm, p, warp - kLoaderWarp, lane);
+  } else {
+    promote<NT>(sm, p, warp, lane);
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (warp == kMmaWarp) tc::tmem_dealloc(sm.tmem_base, kColumns);
+}
+
+// Tokens per tile: 16 where no expert can have more, which leaves the ring more room for weights.
+int tile_tokens(int64_t T) { return T <= 16 ? 16 : 64; }
+
+template <int NT>
+cudaError_t launch_experts(const MoeParams& p, int num_sms, cudaStream_t stream) {
+  CUtensorMap tm13, tm2;
+  if (!make_rows_map(&tm13, p.w13, static_cast<int64_t>(p.E) * 2 * p.I, p.H, p.H, kBlk) ||
+      !make_rows_map(&tm2, p.w2, static_cast<int64_t>(p.E) * p.H, p.I, p.I, kBlk))
+    return cudaErrorInvalidValue;
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  constexpr int smem = static_cast<int>(moe_smem_bytes<NT>());
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(moe_experts_kernel<NT>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(num_sms);
+  cfg.blockDim = dim3(moe_warps<NT> * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, moe_experts_kernel<NT>, tm13, tm2, p);
+}
+
+template <int kTok>
+cudaError_t launch_router(const MoeParams& p, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.T + kTok - 1) / kTok) * kRouterCluster);
+  cfg.blockDim = dim3(kRouterThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, moe_router_kernel<kTok>, p);
 }
 
 }  // namespace
 
 int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
-  (void)num_sms;
   uint8_t* const base = static_cast<uint8_t*>(workspace);
   int64_t off = 0;
   auto take = [&](auto*& ptr, int64_t bytes) {
@@ -194,27 +836,30 @@ int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
       ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(base + off);
     off += (bytes + 255) / 256 * 256;
   };
-  const int64_t n = p.T * p.top_k;
-  take(p.ids, n * 4);      // where the caller gives none
+  const int64_t n = p.T * p.top_k, part = static_cast<int64_t>(tile_tokens(p.T)) * kBlk * 4;
+  // counters: the next ticket; finished items of each tile (phase 0); arrived parts of the item that
+  // each range leaves unfinished, by phase; arrived results per token and 128 columns
+  p.num_counters = 1 + kMaxTiles + 2 * num_sms + p.T * (p.H / kBlk);
+  take(p.counters, p.num_counters * 4);
+  take(p.ids, n * 4);  // where the caller gives none
   take(p.weights, n * 4);
   take(p.hq, n * p.I);
   take(p.h_scale, n * (p.I / kBlk) * 2);
   take(p.y, n * p.H * 4);
+  take(p.parts[0], 2 * num_sms * 2 * part);
+  take(p.parts[1], 2 * num_sms * part);
   return off;
 }
 
 cudaError_t launch_moe(const MoeParams& p, int num_sms, cudaStream_t stream) {
-  (void)num_sms;
-  const unsigned n = static_cast<unsigned>(p.T * p.top_k);
-  moe_router_kernel<<<static_cast<unsigned>(p.T), kRouterThreads, 0, stream>>>(p);
-  const size_t sh1 = (p.H + p.H / kBlk) * 4, sh2 = (p.I + p.I / kBlk) * 4;
-  if (sh1 > 200 * 1024 || sh2 > 200 * 1024) return cudaErrorInvalidValue;
-  cudaFuncSetAttribute(moe_gate_up_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-  cudaFuncSetAttribute(moe_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-  moe_gate_up_kernel<<<dim3(n, p.I / kBlk), 256, sh1, stream>>>(p);
-  moe_down_kernel<<<dim3(n, p.H / kBlk), 128, sh2, stream>>>(p);
-  moe_combine_kernel<<<dim3(static_cast<unsigned>(p.T), p.H / kBlk), 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  if (p.T == 0) return cudaSuccess;
+  // tokens per cluster: few, for the most CTAs, until the experts' rows are read often enough to count
+  const cudaError_t e = p.T <= 16   ? launch_router<1>(p, stream)
+                        : p.T <= 64 ? launch_router<4>(p, stream)
+                                    : launch_router<8>(p, stream);
+  if (e != cudaSuccess) return e;
+  return tile_tokens(p.T) == 16 ? launch_experts<16>(p, num_sms, stream)
+                                : launch_experts<64>(p, num_sms, stream);
 }
 
 }  // namespace fp8attn
