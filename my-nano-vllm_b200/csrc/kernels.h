@@ -167,6 +167,7 @@ struct MoeParams {
   // workspace
   int* counters;      // see moe_layout
   int64_t num_counters;
+  uint32_t top_k_inverse;  // 2^18 / top_k, rounded up
   uint8_t* hq;        // e4m3 [T top_k, I]
   uint16_t* h_scale;  // bf16 [T top_k, I / 128]
   float* y;           // fp32 [T top_k, H]

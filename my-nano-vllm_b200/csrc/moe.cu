@@ -29,7 +29,6 @@
 //   swizzled layout) and scale products, one issues tcgen05 MMAs (D[128 weight rows, N tokens] per
 //   128 columns of K, weights and tokens both from shared memory), eight take D from tensor memory,
 //   scale and add it, and finish items.
-#include <climits>
 #include <type_traits>
 
 #include <cooperative_groups.h>
@@ -53,55 +52,47 @@ __device__ __forceinline__ uint16_t f32_to_bf16(float x) {
 }
 
 // ------------------------------------------------------------------ router
-constexpr int kRouterThreads = 256;
+constexpr int kRouterThreads = 512;
 constexpr int kRouterCluster = 8;
 constexpr int kExpertsPerLane = kMoeMaxExperts / 32;
 
-// One token's choice by one warp, its logits in shared memory.
+// Order of the choice: larger logits first, a NaN after every number; 0 is not to be chosen.
+__device__ __forceinline__ uint32_t choice_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return x == x ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 1u;  // -infinity: 0x007FFFFF
+}
+
+// One token's choice by one warp, its logits in shared memory.  Lane l keeps experts l, l + 32, ...
 __device__ __forceinline__ void choose_experts(const MoeParams& p, int64_t token,
                                                const float* logits, int lane) {
-  // lane keeps experts lane, lane + 32, ...; a NaN logit is chosen last
-  float v[kExpertsPerLane];
-  uint32_t taken = 0;
+  uint32_t key[kExpertsPerLane];
 #pragma unroll
-  for (int j = 0; j < kExpertsPerLane; ++j) {
-    const int e = lane + 32 * j;
-    v[j] = e < p.E ? logits[e] : 0.f;
-    if (e >= p.E) taken |= 1u << j;
-  }
+  for (int j = 0; j < kExpertsPerLane; ++j)
+    key[j] = lane + 32 * j < p.E ? choice_key(logits[lane + 32 * j]) : 0u;
   float top = 0.f, chosen = 0.f;
   int my_id = 0;
   for (int k = 0; k < p.top_k; ++k) {
-    float best = -INFINITY;
-    int at = INT_MAX;
+    uint32_t best = 0u;
 #pragma unroll
-    for (int j = 0; j < kExpertsPerLane; ++j) {
-      const float c = v[j] == v[j] ? v[j] : -INFINITY;
-      if (!((taken >> j) & 1u) && (at == INT_MAX || c > best)) {
-        best = c;
-        at = lane + 32 * j;
-      }
-    }
+    for (int j = 0; j < kExpertsPerLane; ++j) best = max(best, key[j]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    uint32_t at = 0xffffffffu;  // the lowest of the experts that have it
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const float ob = __shfl_xor_sync(0xffffffffu, best, off);
-      const int oa = __shfl_xor_sync(0xffffffffu, at, off);
-      if (oa != INT_MAX && (at == INT_MAX || ob > best || (ob == best && oa < at))) {
-        best = ob;
-        at = oa;
-      }
-    }
-    if (k == 0) top = best;
-    if ((at & 31) == lane) taken |= 1u << (at >> 5);
+    for (int j = kExpertsPerLane - 1; j >= 0; --j)
+      if (key[j] == best) at = lane + 32 * j;
+    at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int j = 0; j < kExpertsPerLane; ++j)
+      if (static_cast<int>(at) == lane + 32 * j) key[j] = 0u;
+    const float l = logits[at];
+    if (k == 0) top = l;
     if (lane == k) {
-      my_id = at;
-      chosen = logits[at];
+      my_id = static_cast<int>(at);
+      chosen = l;
     }
   }
   float sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < kExpertsPerLane; ++j)
-    if (lane + 32 * j < p.E) sum += expf(v[j] - top);
+  for (int e = lane; e < p.E; e += 32) sum += expf(logits[e] - top);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   float c = lane < p.top_k ? expf(chosen - top) / sum : 0.f;
@@ -140,7 +131,7 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     double acc[kTok];
 #pragma unroll
     for (int t = 0; t < kTok; ++t) acc[t] = 0.0;
-#pragma unroll 4
+#pragma unroll (kTok == 1 ? 8 : kTok == 4 ? 4 : 2)
     for (int c = 8 * lane; c < p.H; c += 256) {
       const uint4 wr = __ldg(reinterpret_cast<const uint4*>(w + c));
       const uint32_t ww[4] = {wr.x, wr.y, wr.z, wr.w};
@@ -181,8 +172,16 @@ constexpr int kLoaders = NT == 16 ? 4 : 2;
 template <int NT>
 constexpr int moe_warps = kLoaderWarp + kLoaders<NT>;
 constexpr int kDBufs = 4;
-constexpr int kMaxTiles = 640;  // experts + slots / 64, or slots of 16 tokens
-static_assert(kMoeMaxExperts + kMoeMaxSlots / 64 <= kMaxTiles && 16 * kMoeMaxTopK <= kMaxTiles, "tiles");
+// counters: the next ticket, finished ranges of phase 1, finished items of each tile (phase 0), arrived
+// parts of the item that each range leaves unfinished (by phase)
+constexpr int kDoneAt = 1, kReadyAt = 2;
+// Tokens per tile: 16 where an expert has 8 tokens or fewer on average (its tiles past the first read
+// the weights again, from L2), which leaves the ring more room for weights; else 64.
+constexpr int kFewTokens = 8;
+constexpr int kMaxTiles = 768;  // at most the experts and the full tiles
+static_assert(kMoeMaxExperts + kMoeMaxSlots / 64 <= kMaxTiles &&
+                  kMoeMaxExperts + kFewTokens * kMoeMaxExperts / 16 <= kMaxTiles, "tiles");
+int tile_tokens(int64_t T, int E, int top_k) { return T <= 16 || T * top_k <= kFewTokens * E ? 16 : 64; }
 
 // Units [begin, end) of one phase.
 struct Phase {
@@ -213,19 +212,16 @@ struct __align__(1024) MoeSmem {
   uint64_t d_full[kDBufs], d_empty[kDBufs];
   uint64_t claim_full[2], claim_empty[2];
   int claim[2];
-  Phase phase[2];
+  Phase phase[3];
   int last;                            // promotion threads: this CTA finishes the item
-  int done[NT];                        // ... and the token
   uint32_t tmem_base;
-  int tiles;
   uint32_t tile[kMaxTiles];            // expert << 16 | index of the tile among the expert's
   uint16_t first[kMoeMaxExperts + 1];  // the expert's slots: order[first[e] .. first[e + 1])
-  uint16_t order[kMoeMaxSlots];        // slots by expert (the last member: NT = 16 needs 512 of them)
+  uint16_t order[kMoeMaxSlots];        // slots by expert
 };
-constexpr int kOrder16 = 16 * kMoeMaxTopK;
 template <int NT>
 constexpr size_t moe_smem_bytes() {
-  return sizeof(MoeSmem<NT>) - (NT == 16 ? (kMoeMaxSlots - kOrder16) * 2 : 0) + 1024;
+  return sizeof(MoeSmem<NT>) + 1024;
 }
 static_assert(moe_smem_bytes<16>() <= 227 * 1024 && moe_smem_bytes<64>() <= 227 * 1024, "smem");
 
@@ -235,6 +231,44 @@ __device__ __forceinline__ int load_acquire(const int* p) {
   int v;
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
+}
+
+// Adds 1 once the CTA's writes before it (its threads' by a barrier) can be seen by the GPU.
+__device__ __forceinline__ void add_release(int* p) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(p) : "memory");
+}
+__device__ __forceinline__ int add_acq_rel(int* p) {
+  int v;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// 16 bits that stay in flight until they are used (the compiler may not sink or merge the load).
+__device__ __forceinline__ uint32_t load16(const uint16_t* p) {
+  uint16_t v;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t load16_fresh(const uint16_t* p) {  // written during this kernel
+  uint16_t v;
+  asm volatile("ld.relaxed.gpu.global.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+  return v;
+}
+// slot / top_k: exact for slots < 2^13 and top_k <= 32, where slot (top_k - 1) < 2^18
+__device__ __forceinline__ int token_of(const MoeParams& p, int slot) {
+  static_assert(kMoeMaxSlots <= 1 << 13 && kMoeMaxTopK <= 32, "token_of");
+  return static_cast<int>(static_cast<uint32_t>(slot) * p.top_k_inverse >> 18);
 }
 
 // Wait until *p >= want; gives up after kWaitLimitNs, recording kDevErrWaitTimeout.
@@ -328,7 +362,15 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
       f.ranges = min(grid, f.whole ? f.items : f.units);
       sm.phase[lane] = f;
     }
-    if (lane == 0) sm.tiles = tiles;
+    if (lane == 2) {  // 256 columns of a token
+      Phase f;
+      f.blocks = (p.H + 255) / 256;
+      f.steps = 1;
+      f.items = f.units = static_cast<int>(p.T) * f.blocks;
+      f.whole = 1;
+      f.ranges = min(static_cast<int>(gridDim.x), f.items);
+      sm.phase[2] = f;
+    }
   }
   __syncthreads();
   for (int i0 = lo; i0 < hi; i0 += 32) {
@@ -351,6 +393,7 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
 // A range's place in the work: item (tile, blk), step k of it; advances unit by unit.
 struct Cursor {
   int tile, blk, k;
+  __device__ __forceinline__ Cursor(int t, int b, int s) : tile(t), blk(b), k(s) {}
   __device__ __forceinline__ Cursor(const Phase& f, int unit) {
     const int item = unit / f.steps;
     k = unit - item * f.steps;
@@ -380,6 +423,16 @@ struct Tile {
   __device__ __forceinline__ int columns() const { return (count + 15) & ~15; }  // the MMA's N
 };
 
+// Tickets: the ranges of phase 0, of phase 1, then of the weighted sums.
+template <int NT>
+__device__ __forceinline__ int phase_of(const MoeSmem<NT>& sm, int ticket) {
+  return (ticket >= sm.phase[0].ranges) + (ticket >= sm.phase[0].ranges + sm.phase[1].ranges);
+}
+template <int NT>
+__device__ __forceinline__ int range_in(const MoeSmem<NT>& sm, int ticket, int phase) {
+  return ticket - (phase > 0 ? sm.phase[0].ranges : 0) - (phase > 1 ? sm.phase[1].ranges : 0);
+}
+
 // The next range, for every warp but the producer.  False: no more.
 template <int NT>
 __device__ __forceinline__ bool next_claim(MoeSmem<NT>& sm, int i, int lane, int* err, int& ticket) {
@@ -392,22 +445,25 @@ __device__ __forceinline__ bool next_claim(MoeSmem<NT>& sm, int i, int lane, int
 
 template <int NT>
 __device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* tm13,
-                        const CUtensorMap* tm2) {
+                        const CUtensorMap* tm2, int ticket) {
   constexpr int kStages = MoeSmem<NT>::kStages;
-  const int total = sm.phase[0].ranges + sm.phase[1].ranges;
+  const int total = sm.phase[0].ranges + sm.phase[1].ranges + sm.phase[2].ranges;
   uint32_t r = 0;
   bool ok = true;
-  int ticket = atomicAdd(p.counters, 1);
   for (int i = 0;; ++i) {
     ok = ok && mbar_wait(&sm.claim_empty[i & 1], ((i >> 1) & 1) ^ 1, p.err);
     const bool more = ok && ticket < total;
     sm.claim[i & 1] = more ? ticket : -1;
     mbar_arrive(&sm.claim_full[i & 1]);
     if (!more) return;
-    const int ph = ticket >= sm.phase[0].ranges;
+    const int ph = phase_of(sm, ticket);
     const Phase f = sm.phase[ph];
-    const int range = ticket - (ph ? sm.phase[0].ranges : 0);
+    const int range = range_in(sm, ticket, ph);
     const int begin = range_begin(f, range), end = range_begin(f, range + 1);
+    if (ph == 2) {  // nothing to load
+      ticket = atomicAdd(p.counters, 1);
+      continue;
+    }
     Cursor c(f, begin);
     for (int u = begin; u < end && ok; ++u, ++r, c.next(f)) {
       // the next ticket: its latency hides behind this range, whose first half lets a CTA that starts
@@ -435,82 +491,156 @@ __device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* 
   }
 }
 
-// One of the gather warps: its share of the units, round robin, so that the loads of several are in
-// flight.
+// One of the gather warps: its share of the units, round robin.  A unit's copies and scales are in
+// flight while the next one's are issued; the two sets of scale registers alternate, since a copy of a
+// register waits for its load (measured: 470 instead of 190 us for 64 tokens).
 template <int NT>
-__device__ void gather(MoeSmem<NT>& sm, const MoeParams& p, int which, int lane) {
-  constexpr int kStages = MoeSmem<NT>::kStages;
-  const int kc1 = p.H / kBlk, kc2 = p.I / kBlk;
+struct Gather {
+  static constexpr int kStages = MoeSmem<NT>::kStages;
+  static constexpr int kPer = (NT + 31) / 32;  // tokens a lane scales
+
+  struct Unit {
+    int stage = -1;  // -1: none in flight
+    uint32_t act[2][kPer], weight[2];  // bf16 bits: lane's activation scales and the weight's, by tile
+  };
+
+  MoeSmem<NT>& sm;
+  const MoeParams& p;
+  const int which, lane, kc1, kc2;
+  Phase f;
+  Cursor c{0, 0, 0};
+  int u = 0, end = 0, ph = 0, claims = 0, ready = -1;
   uint32_t r = 0;
   bool ok = true;
-  int ticket;
-  for (int i = 0; next_claim(sm, i, lane, p.err, ticket); ++i) {
-    const int ph = ticket >= sm.phase[0].ranges;
-    const Phase f = sm.phase[ph];
-    const int range = ticket - (ph ? sm.phase[0].ranges : 0);
-    const int begin = range_begin(f, range), end = range_begin(f, range + 1);
-    Cursor c(f, begin);
-    int ready = -1;
-    for (int u = begin; u < end; ++u, ++r, c.next(f)) {
-      if (static_cast<int>(r % kLoaders<NT>) != which) continue;
-      const int stage = r % kStages;
-      const Tile<NT> t(sm, c.tile);
-      if (ok && ph == 1 && c.tile != ready) {
-        // the tile's hidden values: written by other CTAs
-        ok = wait_counter(p.counters + 1 + c.tile, kc2, p.err);
-        ready = c.tile;
-      }
-      ok = ok && mbar_wait(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err);
-      if (!ok) continue;  // the others stop by themselves: their waits on this stage end, bounded
-      const int subs = ph == 0 ? 1 : (2 * c.k + 1 < kc2 ? 2 : 1);
-      // scale products, lane = token (and token + 32); loads issued before the copies
-      float s[2][NT > 32 ? 2 : 1];
+
+  __device__ Gather(MoeSmem<NT>& s, const MoeParams& q, int w, int l)
+      : sm(s), p(q), which(w), lane(l), kc1(q.H / kBlk), kc2(q.I / kBlk) {}
+
+  // The unit's tiles are complete: newer: another unit's copies were issued after its own.
+  __device__ __forceinline__ void finish(Unit& unit, bool newer) {
+    if (unit.stage < 0) return;
 #pragma unroll
-      for (int h = 0; h < (NT > 32 ? 2 : 1); ++h) {
-        const int m = lane + 32 * h;
-        s[0][h] = s[1][h] = 0.f;
-        if (m < t.count) {
-          const int slot = sm.order[t.begin + m];
-          if (ph == 0) {
-            const float xs = bf16_to_f32(__ldg(p.x_scale + static_cast<int64_t>(slot / p.top_k) * kc1 + c.k));
-            const uint16_t* ws =
-                p.w13_scale + (static_cast<int64_t>(t.expert) * 2 * kc2 + c.blk) * kc1 + c.k;
-            s[0][h] = xs * bf16_to_f32(__ldg(ws));
-            s[1][h] = xs * bf16_to_f32(__ldg(ws + static_cast<int64_t>(kc2) * kc1));
-          } else {
-            const uint16_t* hs = p.h_scale + static_cast<int64_t>(slot) * kc2 + 2 * c.k;
-            const uint16_t* ws = p.w2_scale + (static_cast<int64_t>(t.expert) * kc1 + c.blk) * kc2 + 2 * c.k;
-            s[0][h] = bf16_to_f32(__ldcg(hs)) * bf16_to_f32(__ldg(ws));
-            if (subs == 2) s[1][h] = bf16_to_f32(__ldcg(hs + 1)) * bf16_to_f32(__ldg(ws + 1));
-          }
-        }
-      }
-      // rows: 8 lanes copy a row's 128 bytes; rows past the tile's tokens are zeros
-      const int rows = t.columns(), chunk = lane & 7;
-      for (int m = lane >> 3; m < rows; m += 4) {
-        const bool real = m < t.count;
-        const int slot = real ? sm.order[t.begin + m] : 0;
-        const uint8_t* src =
-            ph == 0 ? p.xq + static_cast<int64_t>(slot / p.top_k) * p.xq_row_stride + c.k * kBlk
-                    : p.hq + static_cast<int64_t>(slot) * p.I + 2 * c.k * kBlk;
-        const uint32_t at = m * kBlk + ((chunk ^ (m & 7)) << 4);
-        cp_async16(smem_u32(sm.x[stage][0]) + at, src + chunk * 16, real);
-        if (subs == 2) cp_async16(smem_u32(sm.x[stage][1]) + at, src + kBlk + chunk * 16, real);
-      }
-      cp_async_commit();
+    for (int h = 0; h < kPer; ++h)
+      if (lane + 32 * h < NT) {
 #pragma unroll
-      for (int h = 0; h < (NT > 32 ? 2 : 1); ++h)
-        if (lane + 32 * h < NT) {
-          sm.scale[stage][0][lane + 32 * h] = s[0][h];
-          sm.scale[stage][1][lane + 32 * h] = s[1][h];
-        }
+        for (int s = 0; s < 2; ++s)
+          sm.scale[unit.stage][s][lane + 32 * h] =
+              __uint_as_float(unit.act[s][h] << 16) * __uint_as_float(unit.weight[s] << 16);
+      }
+    if (newer) {
+      cp_async_wait<1>();
+    } else {
       cp_async_wait<0>();
-      fence_proxy_async_smem();  // the tensor cores read the rows through the async proxy
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.x_full[stage]);
+    }
+    fence_proxy_async_smem();  // the tensor cores read the rows through the async proxy
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.x_full[unit.stage]);
+    unit.stage = -1;
+  }
+
+  // To this warp's next unit; false: no more.  Whatever may have to wait lets the unit in flight go
+  // first: the wait may depend on it.
+  __device__ __forceinline__ bool advance(Unit& flying) {
+    for (;;) {
+      while (u == end) {
+        int ticket;
+        finish(flying, false);
+        if (!next_claim(sm, claims++, lane, p.err, ticket)) return false;
+        ph = phase_of(sm, ticket);
+        if (ph == 2) continue;
+        f = sm.phase[ph];
+        const int range = range_in(sm, ticket, ph);
+        u = range_begin(f, range);
+        end = range_begin(f, range + 1);
+        c = Cursor(f, u);
+        ready = -1;
+      }
+      if (static_cast<int>(r % kLoaders<NT>) == which) return true;
+      step();
     }
   }
-}
+  __device__ __forceinline__ void step() {
+    ++u;
+    ++r;
+    c.next(f);
+  }
+
+  // Issues the next unit into `mine`, then completes `other`.
+  __device__ __forceinline__ bool run(Unit& mine, Unit& other) {
+    if (!advance(other)) return false;
+    const int stage = r % kStages;
+    if (ok && ph == 1 && c.tile != ready) {  // the tile's hidden values: written by other CTAs
+      const int* counter = p.counters + kReadyAt + c.tile;
+      if (load_acquire(counter) < kc2) {
+        finish(other, false);
+        ok = wait_counter(counter, kc2, p.err);
+      }
+      ready = c.tile;
+    }
+    if (ok && !mbar_test(&sm.empty[stage], ((r / kStages) & 1) ^ 1)) {
+      finish(other, false);
+      ok = mbar_wait(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err);
+    }
+    if (ok) {  // else: the others stop by themselves, their waits on this stage are bounded
+      issue(mine, stage);
+      finish(other, true);
+    }
+    step();
+    return true;
+  }
+
+  __device__ __forceinline__ void issue(Unit& unit, int stage) {
+    unit.stage = stage;
+    const Tile<NT> t(sm, c.tile);
+    const int subs = ph == 0 ? 1 : (2 * c.k + 1 < kc2 ? 2 : 1);
+    if (ph == 0) {
+      const uint16_t* ws = p.w13_scale + (static_cast<int64_t>(t.expert) * 2 * kc2 + c.blk) * kc1 + c.k;
+      unit.weight[0] = load16(ws);
+      unit.weight[1] = load16(ws + static_cast<int64_t>(kc2) * kc1);
+    } else {
+      const uint16_t* ws = p.w2_scale + (static_cast<int64_t>(t.expert) * kc1 + c.blk) * kc2 + 2 * c.k;
+      unit.weight[0] = load16(ws);
+      unit.weight[1] = subs == 2 ? load16(ws + 1) : 0u;
+    }
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      const int m = lane + 32 * h;
+      unit.act[0][h] = unit.act[1][h] = 0u;
+      if (m < t.count) {
+        const int slot = sm.order[t.begin + m];
+        if (ph == 0) {
+          unit.act[0][h] = load16(p.x_scale + static_cast<int64_t>(token_of(p, slot)) * kc1 + c.k);
+          unit.act[1][h] = unit.act[0][h];
+        } else {
+          const uint16_t* hs = p.h_scale + static_cast<int64_t>(slot) * kc2 + 2 * c.k;
+          unit.act[0][h] = load16_fresh(hs);
+          if (subs == 2) unit.act[1][h] = load16_fresh(hs + 1);
+        }
+      }
+    }
+    // rows: 8 lanes copy a row's 128 bytes; rows past the tile's tokens are zeros
+    const int rows = t.columns(), chunk = lane & 7;
+    for (int m = lane >> 3; m < rows; m += 4) {
+      const bool real = m < t.count;
+      const int slot = real ? sm.order[t.begin + m] : 0;
+      const uint8_t* src =
+          ph == 0 ? p.xq + static_cast<int64_t>(token_of(p, slot)) * p.xq_row_stride + c.k * kBlk
+                  : p.hq + static_cast<int64_t>(slot) * p.I + 2 * c.k * kBlk;
+      const uint32_t at = m * kBlk + ((chunk ^ (m & 7)) << 4);
+      cp_async16(smem_u32(sm.x[stage][0]) + at, src + chunk * 16, real);
+      if (subs == 2) cp_async16(smem_u32(sm.x[stage][1]) + at, src + kBlk + chunk * 16, real);
+    }
+    cp_async_commit();
+  }
+
+  __device__ void run_all() {
+    Unit a, b;
+    while (run(a, b) && run(b, a)) {
+    }
+    finish(a, false);
+    finish(b, false);
+  }
+};
 
 template <int NT>
 __device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int lane) {
@@ -520,10 +650,10 @@ __device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int lane) {
   bool ok = true;
   int ticket;
   for (int i = 0; next_claim(sm, i, lane, p.err, ticket); ++i) {
-    if (lane == 0) {
-      const int ph = ticket >= sm.phase[0].ranges;
+    const int ph = phase_of(sm, ticket);
+    if (lane == 0 && ph < 2) {
       const Phase f = sm.phase[ph];
-      const int range = ticket - (ph ? sm.phase[0].ranges : 0);
+      const int range = range_in(sm, ticket, ph);
       const int begin = range_begin(f, range), end = range_begin(f, range + 1);
       Cursor c(f, begin);
       for (int u = begin; u < end && ok; ++u, ++r, c.next(f)) {
@@ -588,17 +718,33 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
   const int col = 32 * quad + lane;  // output column of the item
   const uint32_t tmem = sm.tmem_base + (static_cast<uint32_t>(32 * quad) << 16);
   const int kc2 = p.I / kBlk;
-  int* const ready = p.counters + 1;
-  int* const part_count = ready + kMaxTiles;               // [2][grid]
-  int* const token_count = part_count + 2 * gridDim.x;     // [T][H / 128]
+  int* const ready = p.counters + kReadyAt;
+  int* const part_count = ready + kMaxTiles;  // [2][grid]
   uint32_t r = 0;
   bool ok = true;
   int ticket;
   for (int i = 0; next_claim(sm, i, lane, p.err, ticket); ++i) {
-    const int ph = ticket >= sm.phase[0].ranges;
+    const int ph = phase_of(sm, ticket);
     const Phase f = sm.phase[ph];
-    const int range = ticket - (ph ? sm.phase[0].ranges : 0);
+    const int range = range_in(sm, ticket, ph);
     const int begin = range_begin(f, range), end = range_begin(f, range + 1);
+    if (ph == 2) {
+      // ---- weighted sums, once phase 1 has ended: its ranges are held by CTAs that run
+      ok = ok && wait_counter(p.counters + kDoneAt, sm.phase[1].ranges, p.err);
+      for (int item = begin; item < end && ok; ++item) {
+        const int64_t token = item / f.blocks;
+        const int at = (item - static_cast<int>(token) * f.blocks) * 256 + tid;
+        if (at >= p.H) continue;
+        const float* y = p.y + token * p.top_k * p.H + at;
+        const float* w = p.weights + token * p.top_k;
+        float acc = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < p.top_k; ++k)
+          acc = fmaf(__ldg(w + k), __ldcg(y + static_cast<int64_t>(k) * p.H), acc);
+        p.out[token * p.out_row_stride + at] = f32_to_bf16(acc);
+      }
+      continue;
+    }
     Cursor c(f, begin);
     int u = begin;
     while (u < end) {
@@ -647,23 +793,31 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
           }
         const int r0 = range_of(f, item_begin), r1 = range_of(f, item_begin + f.steps - 1);
         promo_sync();
-        if (tid == 0) {
-          __threadfence();
-          const int before = atomicAdd(part_count + ph * gridDim.x + r0, 1);
-          __threadfence();
-          sm.last = before == r1 - r0;
-        }
+        if (tid == 0) sm.last = add_acq_rel(part_count + ph * gridDim.x + r0) == r1 - r0;
         promo_sync();
         if (!sm.last) continue;
 #pragma unroll
         for (int j = 0; j < kHalf; ++j) g[j] = v[j] = 0.f;
-        for (int q = r0; q <= r1; ++q) {
-          const float* part = parts + (2 * static_cast<int64_t>(q) + (q == r0 ? 1 : 0)) * size;
+        constexpr int kTogether = NT == 16 ? 4 : 1;  // parts whose loads are in flight together
+        for (int q0 = r0; q0 <= r1; q0 += kTogether) {
+          float pg[kTogether][kHalf], pv[kTogether][kHalf];
 #pragma unroll
-          for (int j = 0; j < kHalf; ++j)
-            if (j < 8 * groups) {
-              g[j] += __ldcg(part + (m0 + j) * kBlk + col);
-              if (ph == 0) v[j] += __ldcg(part + kPart + (m0 + j) * kBlk + col);
+          for (int d = 0; d < kTogether; ++d) {
+            const int q = q0 + d;
+            const float* part = parts + (2 * static_cast<int64_t>(q) + (q == r0 ? 1 : 0)) * size;
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) {
+              const bool have = q <= r1 && j < 8 * groups;
+              pg[d][j] = have ? __ldcg(part + (m0 + j) * kBlk + col) : 0.f;
+              pv[d][j] = have && ph == 0 ? __ldcg(part + kPart + (m0 + j) * kBlk + col) : 0.f;
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < kTogether; ++d)
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) {
+              g[j] += pg[d][j];
+              v[j] += pv[d][j];
             }
         }
       }
@@ -691,37 +845,18 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
             if (col == 0) p.h_scale[slot * kc2 + blk] = f32_to_bf16(scale);
           }
         promo_sync();  // also: amax is free again
-        if (tid == 0) {
-          __threadfence();
-          atomicAdd(ready + tile, 1);
-        }
+        if (tid == 0) add_release(ready + tile);
       } else {
-        // ---- the slots' results; the CTA that brings a token its last adds the token's up
+        // ---- the slots' results
 #pragma unroll
         for (int j = 0; j < kHalf; ++j)
           if (m0 + j < t.count && j < 8 * groups)
             __stcg(p.y + static_cast<int64_t>(sm.order[t.begin + m0 + j]) * p.H + blk * kBlk + col, g[j]);
-        promo_sync();
-        if (tid < t.count) {
-          const int64_t token = sm.order[t.begin + tid] / p.top_k;
-          __threadfence();
-          const int before = atomicAdd(token_count + token * f.blocks + blk, 1);
-          __threadfence();
-          sm.done[tid] = before == p.top_k - 1;
-        }
-        promo_sync();
-        for (int m = tid >> 7; m < t.count; m += 2) {
-          if (!sm.done[m]) continue;
-          const int64_t token = sm.order[t.begin + m] / p.top_k;
-          const int at = blk * kBlk + (tid & 127);
-          const float* y = p.y + token * p.top_k * p.H + at;
-          float acc = 0.f;
-          for (int k = 0; k < p.top_k; ++k)
-            acc = fmaf(__ldg(p.weights + token * p.top_k + k), __ldcg(y + static_cast<int64_t>(k) * p.H), acc);
-          p.out[token * p.out_row_stride + at] = f32_to_bf16(acc);
-        }
-        promo_sync();  // done is free again
       }
+    }
+    if (ph == 1) {
+      promo_sync();
+      if (tid == 0) add_release(p.counters + kDoneAt);
     }
   }
 }
@@ -761,16 +896,18 @@ __global__ void __launch_bounds__(moe_warps<NT> * 32, 1)
   }
   // launched as a programmatic dependent of the router: its choice is read only when it has ended
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  int ticket = 0;
+  if (warp == kProducerWarp && lane == 0) ticket = atomicAdd(p.counters, 1);
   tc::fence_before_sync();
   plan<NT>(sm, p);  // begins and ends with barriers of the whole CTA
   tc::fence_after_sync();
   if (warp == kProducerWarp) {
-    if (lane == 0) produce<NT>(sm, p, &tm13, &tm2);
+    if (lane == 0) produce<NT>(sm, p, &tm13, &tm2, ticket);
     __syncwarp();
   } else if (warp == kMmaWarp) {
     multiply<NT>(sm, p, lane);
   } else if (warp >= kLoaderWarp) {
-    gather<NT>(sm, p, warp - kLoaderWarp, lane);
+    Gather<NT>(sm, p, warp - kLoaderWarp, lane).run_all();
   } else {
     promote<NT>(sm, p, warp, lane);
   }
@@ -779,9 +916,6 @@ __global__ void __launch_bounds__(moe_warps<NT> * 32, 1)
   tc::fence_after_sync();
   if (warp == kMmaWarp) tc::tmem_dealloc(sm.tmem_base, kColumns);
 }
-
-// Tokens per tile: 16 where no expert can have more, which leaves the ring more room for weights.
-int tile_tokens(int64_t T) { return T <= 16 ? 16 : 64; }
 
 template <int NT>
 cudaError_t launch_experts(const MoeParams& p, int num_sms, cudaStream_t stream) {
@@ -836,10 +970,9 @@ int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
       ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(base + off);
     off += (bytes + 255) / 256 * 256;
   };
-  const int64_t n = p.T * p.top_k, part = static_cast<int64_t>(tile_tokens(p.T)) * kBlk * 4;
-  // counters: the next ticket; finished items of each tile (phase 0); arrived parts of the item that
-  // each range leaves unfinished, by phase; arrived results per token and 128 columns
-  p.num_counters = 1 + kMaxTiles + 2 * num_sms + p.T * (p.H / kBlk);
+  const int64_t n = p.T * p.top_k, part = static_cast<int64_t>(tile_tokens(p.T, p.E, p.top_k)) * kBlk * 4;
+  p.num_counters = kReadyAt + kMaxTiles + 2 * num_sms;
+  p.top_k_inverse = ((1u << 18) + p.top_k - 1) / p.top_k;
   take(p.counters, p.num_counters * 4);
   take(p.ids, n * 4);  // where the caller gives none
   take(p.weights, n * 4);
@@ -858,7 +991,7 @@ cudaError_t launch_moe(const MoeParams& p, int num_sms, cudaStream_t stream) {
                         : p.T <= 64 ? launch_router<4>(p, stream)
                                     : launch_router<8>(p, stream);
   if (e != cudaSuccess) return e;
-  return tile_tokens(p.T) == 16 ? launch_experts<16>(p, num_sms, stream)
+  return tile_tokens(p.T, p.E, p.top_k) == 16 ? launch_experts<16>(p, num_sms, stream)
                                 : launch_experts<64>(p, num_sms, stream);
 }
 
