@@ -16,7 +16,7 @@
 // moe_router_kernel: a cluster of 8 CTAs per few tokens; its warps share the experts' rows, the
 //   logits meet in distributed shared memory, one warp per token chooses.
 // moe_experts_kernel: one CTA per SM, both products.  Tokens are sorted by expert into tiles of up to
-//   NT (16 or 64).  An item is 128 output columns of a tile (phase 0: 128 of gate and the same of up;
+//   NT (16 or 32).  An item is 128 output columns of a tile (phase 0: 128 of gate and the same of up;
 //   phase 1: 128 of the result), a unit one step of its sum, 32 KB of weights (phase 0: 128 columns of
 //   K for both halves; phase 1: 256 columns of K).  A phase's units, items in order, are cut into
 //   equal ranges, one per CTA, wherever the cuts fall (few tokens make few items): the parts of a cut
@@ -44,15 +44,15 @@ namespace cg = cooperative_groups;
 
 constexpr int kBlk = 128;
 
-__device__ __forceinline__ float bf16_to_f32(uint16_t b) {
-  return __uint_as_float(static_cast<uint32_t>(b) << 16);
-}
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
 __device__ __forceinline__ uint16_t f32_to_bf16(float x) {
   return __bfloat16_as_ushort(__float2bfloat16_rn(x));
 }
 
 // ------------------------------------------------------------------ router
-constexpr int kRouterThreads = 512;
+template <int kTok>
+constexpr int kRouterThreads = kTok == 1 ? 512 : 256;
+
 constexpr int kRouterCluster = 8;
 constexpr int kExpertsPerLane = kMoeMaxExperts / 32;
 
@@ -111,7 +111,7 @@ __device__ __forceinline__ void choose_experts(const MoeParams& p, int64_t token
 // Cluster c: tokens c kTok .. + kTok - 1.  Logits: fp32 products of 8 columns at a time, added up in
 // fp64, so that which experts are chosen does not hang on the order of a sum.
 template <int kTok>
-__global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads)
+__global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads<kTok>)
     moe_router_kernel(const MoeParams p) {
   static_assert(kTok <= kRouterCluster, "a CTA chooses for one token at most");
   __shared__ float logits[kMoeMaxExperts];  // of token (cluster's first + this CTA's rank)
@@ -120,18 +120,18 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the counters of the next kernel
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kRouterThreads + threadIdx.x; i < p.num_counters;
-       i += static_cast<int64_t>(gridDim.x) * kRouterThreads)
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kRouterThreads<kTok> + threadIdx.x; i < p.num_counters;
+       i += static_cast<int64_t>(gridDim.x) * kRouterThreads<kTok>)
     p.counters[i] = 0;
   const int rank = static_cast<int>(cluster.block_rank());
   const int64_t t0 = static_cast<int64_t>(blockIdx.x / kRouterCluster) * kTok;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int e = rank * (kRouterThreads / 32) + warp; e < p.E; e += kRouterCluster * kRouterThreads / 32) {
+  for (int e = rank * (kRouterThreads<kTok> / 32) + warp; e < p.E; e += kRouterCluster * kRouterThreads<kTok> / 32) {
     const uint16_t* w = p.router + static_cast<int64_t>(e) * p.H;
     double acc[kTok];
 #pragma unroll
     for (int t = 0; t < kTok; ++t) acc[t] = 0.0;
-#pragma unroll (kTok == 1 ? 8 : kTok == 4 ? 4 : 2)
+#pragma unroll (kTok == 1 ? 8 : 2)
     for (int c = 8 * lane; c < p.H; c += 256) {
       const uint4 wr = __ldg(reinterpret_cast<const uint4*>(w + c));
       const uint32_t ww[4] = {wr.x, wr.y, wr.z, wr.w};
@@ -165,23 +165,20 @@ constexpr int kPromoWarps = 8;  // warps 0-7
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kLoaderWarp = 10;  // and after
-// Gather warps.  With 64 tokens a tile only two, so that 12 warps leave the promotion threads, whose
-// sums take 64 registers, 168 of them (14 warps: 128, and 1.5 KB of spills).
-template <int NT>
-constexpr int kLoaders = NT == 16 ? 4 : 2;
-template <int NT>
-constexpr int moe_warps = kLoaderWarp + kLoaders<NT>;
+constexpr int kLoaders = 4;
+constexpr int kWarps = kLoaderWarp + kLoaders;
+constexpr int kThreads = kWarps * 32;
 constexpr int kDBufs = 4;
 // counters: the next ticket, finished ranges of phase 1, finished items of each tile (phase 0), arrived
 // parts of the item that each range leaves unfinished (by phase)
 constexpr int kDoneAt = 1, kReadyAt = 2;
 // Tokens per tile: 16 where an expert has 8 tokens or fewer on average (its tiles past the first read
-// the weights again, from L2), which leaves the ring more room for weights; else 64.
+// the weights again, from L2), which leaves the ring more room for weights; else 32.
 constexpr int kFewTokens = 8;
 constexpr int kMaxTiles = 768;  // at most the experts and the full tiles
-static_assert(kMoeMaxExperts + kMoeMaxSlots / 64 <= kMaxTiles &&
+static_assert(kMoeMaxExperts + kMoeMaxSlots / 32 <= kMaxTiles &&
                   kMoeMaxExperts + kFewTokens * kMoeMaxExperts / 16 <= kMaxTiles, "tiles");
-int tile_tokens(int64_t T, int E, int top_k) { return T <= 16 || T * top_k <= kFewTokens * E ? 16 : 64; }
+int tile_tokens(int64_t T, int E, int top_k) { return T <= 16 || T * top_k <= kFewTokens * E ? 16 : 32; }
 
 // Units [begin, end) of one phase.
 struct Phase {
@@ -207,7 +204,7 @@ struct __align__(1024) MoeSmem {
   uint8_t w[kStages][2][kBlk * kBlk];  // weight tiles: 128 rows x 128 bytes, 128B swizzle
   uint8_t x[kStages][2][NT * kBlk];    // token tiles: NT rows x 128 bytes, 128B swizzle
   float scale[kStages][2][NT];         // activation scale * weight scale of the stage's two tiles
-  float amax[4][NT];                   // a quadrant's largest |h| per token
+  float item[2][NT][kBlk];             // an item's sums (gate, up), token by token
   uint64_t w_full[kStages], x_full[kStages], empty[kStages];
   uint64_t d_full[kDBufs], d_empty[kDBufs];
   uint64_t claim_full[2], claim_empty[2];
@@ -215,6 +212,7 @@ struct __align__(1024) MoeSmem {
   Phase phase[3];
   int last;                            // promotion threads: this CTA finishes the item
   uint32_t tmem_base;
+  int tiles;
   uint32_t tile[kMaxTiles];            // expert << 16 | index of the tile among the expert's
   uint16_t first[kMoeMaxExperts + 1];  // the expert's slots: order[first[e] .. first[e + 1])
   uint16_t order[kMoeMaxSlots];        // slots by expert
@@ -223,7 +221,7 @@ template <int NT>
 constexpr size_t moe_smem_bytes() {
   return sizeof(MoeSmem<NT>) + 1024;
 }
-static_assert(moe_smem_bytes<16>() <= 227 * 1024 && moe_smem_bytes<64>() <= 227 * 1024, "smem");
+static_assert(moe_smem_bytes<16>() <= 227 * 1024 && moe_smem_bytes<32>() <= 227 * 1024, "smem");
 
 __device__ __forceinline__ void promo_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
@@ -291,24 +289,28 @@ __device__ __forceinline__ bool wait_counter(const int* p, int want, int* err) {
 // Slots sorted by expert (stable: results must not depend on timing), the tiles, and the two phases'
 // cuts; every CTA does the same.  Scratch in the ring, which is not in use yet.
 template <int NT>
+__device__ __forceinline__ uint16_t* plan_counts(MoeSmem<NT>& sm) {  // [kWarps][E], zero when plan begins
+  return reinterpret_cast<uint16_t*>(&sm.w[1][0][0]);
+}
+template <int NT>
 __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
-  constexpr int kWarps = moe_warps<NT>, kThreads = kWarps * 32;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int n = static_cast<int>(p.T) * p.top_k, E = p.E;
   uint16_t* const eid = reinterpret_cast<uint16_t*>(&sm.w[0][0][0]);          // [n]
-  uint16_t* const hist = reinterpret_cast<uint16_t*>(&sm.w[1][0][0]);         // [kWarps][E]
+  uint16_t* const hist = plan_counts(sm);
   uint16_t* const total = hist + kWarps * kMoeMaxExperts;                     // [E]
   static_assert(kMoeMaxSlots * 2 <= 2 * kBlk * kBlk, "expert ids fit a stage");
   static_assert((kWarps + 1) * kMoeMaxExperts * 2 <= 2 * kBlk * kBlk, "histograms fit a stage");
-  for (int i = tid; i < kWarps * E; i += kThreads) hist[i] = 0;
   const int per = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;  // a warp's slots: [warp per, + per)
   const int lo = min(warp * per, n), hi = min(lo + per, n);
+#pragma unroll 4
+  for (int i = tid; i < n; i += kThreads)
+    eid[i] = static_cast<uint16_t>(min(max(p.ids[i], 0), E - 1));
   __syncthreads();
   for (int i0 = lo; i0 < hi; i0 += 32) {
     const int i = i0 + lane;
     const bool ok = i < hi;
-    const int e = ok ? min(max(p.ids[i], 0), E - 1) : -1;
-    if (ok) eid[i] = static_cast<uint16_t>(e);
+    const int e = ok ? eid[i] : -1;
     const unsigned same = __match_any_sync(0xffffffffu, e);
     if (ok && lane == __ffs(same) - 1) hist[warp * E + e] += static_cast<uint16_t>(__popc(same));
     __syncwarp();
@@ -362,6 +364,7 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
       f.ranges = min(grid, f.whole ? f.items : f.units);
       sm.phase[lane] = f;
     }
+    if (lane == 0) sm.tiles = tiles;
     if (lane == 2) {  // 256 columns of a token
       Phase f;
       f.blocks = (p.H + 255) / 256;
@@ -390,24 +393,37 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
   __syncthreads();
 }
 
-// A range's place in the work: item (tile, blk), step k of it; advances unit by unit.
+// A range's place in the work; advances unit by unit.  Items run over an expert's tiles first, then over
+// the column blocks, then over the experts: tiles of one expert read the same weights one after another.
+template <int NT>
 struct Cursor {
+  int first, count;  // the expert's tiles
   int tile, blk, k;
-  __device__ __forceinline__ Cursor(int t, int b, int s) : tile(t), blk(b), k(s) {}
-  __device__ __forceinline__ Cursor(const Phase& f, int unit) {
+  __device__ __forceinline__ Cursor() {}
+  __device__ __forceinline__ Cursor(const MoeSmem<NT>& sm, const Phase& f, int unit) {
     const int item = unit / f.steps;
     k = unit - item * f.steps;
-    tile = item / f.blocks;
-    blk = item - tile * f.blocks;
+    expert_of(sm, item / f.blocks);
+    const int in = item - first * f.blocks;
+    blk = in / count;
+    tile = first + in - blk * count;
   }
-  __device__ __forceinline__ void next(const Phase& f) {
-    if (++k == f.steps) {
-      k = 0;
-      if (++blk == f.blocks) {
-        blk = 0;
-        ++tile;
-      }
+  __device__ __forceinline__ void expert_of(const MoeSmem<NT>& sm, int some_tile) {
+    const uint32_t t = sm.tile[some_tile];
+    const int e = static_cast<int>(t >> 16);
+    first = some_tile - static_cast<int>(t & 0xFFFFu);
+    count = (sm.first[e + 1] - sm.first[e] + NT - 1) / NT;
+  }
+  __device__ __forceinline__ void next(const MoeSmem<NT>& sm, const Phase& f) {
+    if (++k < f.steps) return;
+    k = 0;
+    if (++tile < first + count) return;
+    if (++blk < f.blocks) {
+      tile = first;
+      return;
     }
+    blk = 0;
+    if (tile < sm.tiles) expert_of(sm, tile);
   }
 };
 
@@ -464,8 +480,8 @@ __device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* 
       ticket = atomicAdd(p.counters, 1);
       continue;
     }
-    Cursor c(f, begin);
-    for (int u = begin; u < end && ok; ++u, ++r, c.next(f)) {
+    Cursor<NT> c(sm, f, begin);
+    for (int u = begin; u < end && ok; ++u, ++r, c.next(sm, f)) {
       // the next ticket: its latency hides behind this range, whose first half lets a CTA that starts
       // late have its turn (one that held two ranges of a phase would take twice as long)
       if (u == begin + (end - begin) / 2) ticket = atomicAdd(p.counters, 1);
@@ -508,7 +524,7 @@ struct Gather {
   const MoeParams& p;
   const int which, lane, kc1, kc2;
   Phase f;
-  Cursor c{0, 0, 0};
+  Cursor<NT> c;
   int u = 0, end = 0, ph = 0, claims = 0, ready = -1;
   uint32_t r = 0;
   bool ok = true;
@@ -552,17 +568,17 @@ struct Gather {
         const int range = range_in(sm, ticket, ph);
         u = range_begin(f, range);
         end = range_begin(f, range + 1);
-        c = Cursor(f, u);
+        c = Cursor<NT>(sm, f, u);
         ready = -1;
       }
-      if (static_cast<int>(r % kLoaders<NT>) == which) return true;
+      if (static_cast<int>(r % kLoaders) == which) return true;
       step();
     }
   }
   __device__ __forceinline__ void step() {
     ++u;
     ++r;
-    c.next(f);
+    c.next(sm, f);
   }
 
   // Issues the next unit into `mine`, then completes `other`.
@@ -655,8 +671,8 @@ __device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int lane) {
       const Phase f = sm.phase[ph];
       const int range = range_in(sm, ticket, ph);
       const int begin = range_begin(f, range), end = range_begin(f, range + 1);
-      Cursor c(f, begin);
-      for (int u = begin; u < end && ok; ++u, ++r, c.next(f)) {
+      Cursor<NT> c(sm, f, begin);
+      for (int u = begin; u < end && ok; ++u, ++r, c.next(sm, f)) {
         const int stage = r % kStages, buf = r % kDBufs;
         ok = mbar_wait(&sm.w_full[stage], (r / kStages) & 1, p.err) &&
              mbar_wait(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
@@ -731,21 +747,39 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
     if (ph == 2) {
       // ---- weighted sums, once phase 1 has ended: its ranges are held by CTAs that run
       ok = ok && wait_counter(p.counters + kDoneAt, sm.phase[1].ranges, p.err);
-      for (int item = begin; item < end && ok; ++item) {
+      for (int item = begin + warp / 2; item < end && ok; item += kPromoWarps / 2) {
+        // two warps an item, four columns a thread
         const int64_t token = item / f.blocks;
-        const int at = (item - static_cast<int>(token) * f.blocks) * 256 + tid;
+        const int at = (item - static_cast<int>(token) * f.blocks) * 256 + (tid & 63) * 4;
         if (at >= p.H) continue;
         const float* y = p.y + token * p.top_k * p.H + at;
         const float* w = p.weights + token * p.top_k;
-        float acc = 0.f;
-#pragma unroll 8
-        for (int k = 0; k < p.top_k; ++k)
-          acc = fmaf(__ldg(w + k), __ldcg(y + static_cast<int64_t>(k) * p.H), acc);
-        p.out[token * p.out_row_stride + at] = f32_to_bf16(acc);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < p.top_k; k0 += 8) {  // eight slots' loads in flight
+          float4 v[8];
+          float c[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const bool have = k0 + k < p.top_k;
+            v[k] = have ? __ldcg(reinterpret_cast<const float4*>(y + static_cast<int64_t>(k0 + k) * p.H))
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+            c[k] = have ? __ldg(w + k0 + k) : 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            acc.x = fmaf(c[k], v[k].x, acc.x);
+            acc.y = fmaf(c[k], v[k].y, acc.y);
+            acc.z = fmaf(c[k], v[k].z, acc.z);
+            acc.w = fmaf(c[k], v[k].w, acc.w);
+          }
+        }
+        const uint32_t lo = f32_to_bf16(acc.x) | static_cast<uint32_t>(f32_to_bf16(acc.y)) << 16;
+        const uint32_t hi = f32_to_bf16(acc.z) | static_cast<uint32_t>(f32_to_bf16(acc.w)) << 16;
+        *reinterpret_cast<uint2*>(p.out + token * p.out_row_stride + at) = make_uint2(lo, hi);
       }
       continue;
     }
-    Cursor c(f, begin);
+    Cursor<NT> c(sm, f, begin);
     int u = begin;
     while (u < end) {
       // ---- one item, or the part of it that this range holds
@@ -759,7 +793,7 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
 #pragma unroll
       for (int j = 0; j < kHalf; ++j) g[j] = v[j] = 0.f;
       const bool at_head = u != item_begin;
-      for (; u < stop; ++u, ++r, c.next(f)) {
+      for (; u < stop; ++u, ++r, c.next(sm, f)) {
         const int stage = r % kStages, buf = r % kDBufs;
         ok = ok && mbar_wait(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
              mbar_wait(&sm.d_full[buf], (r / kDBufs) & 1, p.err);
@@ -779,80 +813,75 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
           mbar_arrive(&sm.empty[stage]);
         }
       }
-      // ---- the parts of a cut item meet in memory; the CTA that comes last adds them, in order
-      if (cut) {
-        constexpr int kPart = NT * kBlk;  // floats; phase 0 has two of them (gate, up)
-        float* const parts = ph == 0 ? p.parts[0] : p.parts[1];
-        const int64_t size = ph == 0 ? 2 * kPart : kPart;
-        float* mine = parts + (2 * static_cast<int64_t>(range) + (at_head ? 0 : 1)) * size;
+      // ---- the item's sums, token by token: through shared memory, or, of a cut item, through global
+      // memory, where the CTA that comes last adds the parts, in order
+      constexpr int kPart = NT * kBlk;  // floats; phase 0 has two of them (gate, up)
+      float* const parts = p.parts[ph];
+      const int size = ph == 0 ? 2 * kPart : kPart;
+      float* mine = cut ? parts + (2 * static_cast<int64_t>(range) + (at_head ? 0 : 1)) * size
+                        : &sm.item[0][0][0];
 #pragma unroll
-        for (int j = 0; j < kHalf; ++j)
-          if (j < 8 * groups) {
-            __stcg(mine + (m0 + j) * kBlk + col, g[j]);
-            if (ph == 0) __stcg(mine + kPart + (m0 + j) * kBlk + col, v[j]);
-          }
-        const int r0 = range_of(f, item_begin), r1 = range_of(f, item_begin + f.steps - 1);
-        promo_sync();
+      for (int j = 0; j < kHalf; ++j)
+        if (j < 8 * groups) {
+          mine[(m0 + j) * kBlk + col] = g[j];
+          if (ph == 0) mine[kPart + (m0 + j) * kBlk + col] = v[j];
+        }
+      promo_sync();
+      int r0 = 0, r1 = 0;
+      if (cut) {
+        r0 = range_of(f, item_begin);
+        r1 = range_of(f, item_begin + f.steps - 1);
         if (tid == 0) sm.last = add_acq_rel(part_count + ph * gridDim.x + r0) == r1 - r0;
         promo_sync();
         if (!sm.last) continue;
+      }
+      // a warp takes tokens warp, warp + 8, ...; lane: 4 of the 128 columns
+      for (int m = warp; m < t.count; m += kPromoWarps) {
+        float4 a, b = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!cut) {
+          a = *reinterpret_cast<const float4*>(&sm.item[0][m][4 * lane]);
+          if (ph == 0) b = *reinterpret_cast<const float4*>(&sm.item[1][m][4 * lane]);
+        } else {
+          a = b;
+#pragma unroll 1
+          for (int q0 = r0; q0 <= r1; q0 += 4) {  // four parts' loads in flight
+            float4 pa[4], pb[4];
 #pragma unroll
-        for (int j = 0; j < kHalf; ++j) g[j] = v[j] = 0.f;
-        constexpr int kTogether = NT == 16 ? 4 : 1;  // parts whose loads are in flight together
-        for (int q0 = r0; q0 <= r1; q0 += kTogether) {
-          float pg[kTogether][kHalf], pv[kTogether][kHalf];
+            for (int d = 0; d < 4; ++d) {
+              const float* part = parts + (2 * static_cast<int64_t>(q0 + d) + (q0 + d == r0 ? 1 : 0)) * size +
+                                  m * kBlk + 4 * lane;
+              pa[d] = pb[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (q0 + d <= r1) {
+                pa[d] = __ldcg(reinterpret_cast<const float4*>(part));
+                if (ph == 0) pb[d] = __ldcg(reinterpret_cast<const float4*>(part + kPart));
+              }
+            }
 #pragma unroll
-          for (int d = 0; d < kTogether; ++d) {
-            const int q = q0 + d;
-            const float* part = parts + (2 * static_cast<int64_t>(q) + (q == r0 ? 1 : 0)) * size;
-#pragma unroll
-            for (int j = 0; j < kHalf; ++j) {
-              const bool have = q <= r1 && j < 8 * groups;
-              pg[d][j] = have ? __ldcg(part + (m0 + j) * kBlk + col) : 0.f;
-              pv[d][j] = have && ph == 0 ? __ldcg(part + kPart + (m0 + j) * kBlk + col) : 0.f;
+            for (int d = 0; d < 4; ++d) {
+              a = make_float4(a.x + pa[d].x, a.y + pa[d].y, a.z + pa[d].z, a.w + pa[d].w);
+              b = make_float4(b.x + pb[d].x, b.y + pb[d].y, b.z + pb[d].z, b.w + pb[d].w);
             }
           }
-#pragma unroll
-          for (int d = 0; d < kTogether; ++d)
-#pragma unroll
-            for (int j = 0; j < kHalf; ++j) {
-              g[j] += pg[d][j];
-              v[j] += pv[d][j];
-            }
         }
+        const int64_t slot = sm.order[t.begin + m];
+        if (ph == 1) {
+          __stcg(reinterpret_cast<float4*>(p.y + slot * p.H + blk * kBlk + 4 * lane), a);
+          continue;
+        }
+        // h = silu(gate) up, quantised over the item's 128 columns
+        float h[4] = {silu(a.x) * b.x, silu(a.y) * b.y, silu(a.z) * b.z, silu(a.w) * b.w};
+        const float most = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])),
+                                 fmaxf(fmaxf(fabsf(h[2]), fabsf(h[3])), 0.f));  // NaN left out
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+        float scale = __fdiv_rn(top, 448.0f);
+        if (!(scale > 0.f)) scale = 1.0f;
+        const uint32_t lo = f32x2_to_e4m3x2(__fdiv_rn(h[0], scale), __fdiv_rn(h[1], scale));
+        const uint32_t hi = f32x2_to_e4m3x2(__fdiv_rn(h[2], scale), __fdiv_rn(h[3], scale));
+        *reinterpret_cast<uint32_t*>(p.hq + slot * p.I + blk * kBlk + 4 * lane) = lo | (hi << 16);
+        if (lane == 0) p.h_scale[slot * kc2 + blk] = f32_to_bf16(scale);
       }
-      if (ph == 0) {
-        // ---- h = silu(g) u, quantised over the item's 128 columns (4 quadrants of 32 lanes)
-#pragma unroll
-        for (int j = 0; j < kHalf; ++j)
-          if (j < 8 * groups) {
-            g[j] = __fdividef(g[j], 1.0f + expf(-g[j])) * v[j];
-            const float a = g[j] == g[j] ? fabsf(g[j]) : 0.f;  // NaN left out
-            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(a));
-            if (lane == (j & 31)) sm.amax[quad][m0 + j] = __uint_as_float(top);
-          }
-        promo_sync();
-#pragma unroll
-        for (int j = 0; j < kHalf; ++j)
-          if (m0 + j < t.count && j < 8 * groups) {
-            const int m = m0 + j;
-            const float a = fmaxf(fmaxf(sm.amax[0][m], sm.amax[1][m]), fmaxf(sm.amax[2][m], sm.amax[3][m]));
-            float scale = __fdiv_rn(a, 448.0f);
-            if (!(scale > 0.f)) scale = 1.0f;
-            const int64_t slot = sm.order[t.begin + m];
-            p.hq[slot * p.I + blk * kBlk + col] =
-                static_cast<uint8_t>(f32x2_to_e4m3x2(__fdiv_rn(g[j], scale), 0.f) & 0xFFu);
-            if (col == 0) p.h_scale[slot * kc2 + blk] = f32_to_bf16(scale);
-          }
-        promo_sync();  // also: amax is free again
-        if (tid == 0) add_release(ready + tile);
-      } else {
-        // ---- the slots' results
-#pragma unroll
-        for (int j = 0; j < kHalf; ++j)
-          if (m0 + j < t.count && j < 8 * groups)
-            __stcg(p.y + static_cast<int64_t>(sm.order[t.begin + m0 + j]) * p.H + blk * kBlk + col, g[j]);
-      }
+      promo_sync();  // what was written is complete; the shared item is free again
+      if (ph == 0 && tid == 0) add_release(ready + tile);
     }
     if (ph == 1) {
       promo_sync();
@@ -862,7 +891,7 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
 }
 
 template <int NT>
-__global__ void __launch_bounds__(moe_warps<NT> * 32, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     moe_experts_kernel(const __grid_constant__ CUtensorMap tm13, const __grid_constant__ CUtensorMap tm2,
                        const MoeParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -882,7 +911,7 @@ __global__ void __launch_bounds__(moe_warps<NT> * 32, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.claim_full[i], 1);
-      mbar_init(&sm.claim_empty[i], kPromoWarps + 1 + kLoaders<NT>);
+      mbar_init(&sm.claim_empty[i], kPromoWarps + 1 + kLoaders);
     }
     fence_mbar_init();
   }
@@ -894,12 +923,13 @@ __global__ void __launch_bounds__(moe_warps<NT> * 32, 1)
     tc::tmem_alloc(&sm.tmem_base, kColumns);
     tc::tmem_relinquish();
   }
+  for (int i = threadIdx.x; i < kWarps * p.E; i += kThreads) plan_counts(sm)[i] = 0;
   // launched as a programmatic dependent of the router: its choice is read only when it has ended
   asm volatile("griddepcontrol.wait;" ::: "memory");
   int ticket = 0;
   if (warp == kProducerWarp && lane == 0) ticket = atomicAdd(p.counters, 1);
   tc::fence_before_sync();
-  plan<NT>(sm, p);  // begins and ends with barriers of the whole CTA
+  plan<NT>(sm, p);  // barriers of the whole CTA
   tc::fence_after_sync();
   if (warp == kProducerWarp) {
     if (lane == 0) produce<NT>(sm, p, &tm13, &tm2, ticket);
@@ -938,7 +968,7 @@ cudaError_t launch_experts(const MoeParams& p, int num_sms, cudaStream_t stream)
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(num_sms);
-  cfg.blockDim = dim3(moe_warps<NT> * 32);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -953,7 +983,7 @@ cudaError_t launch_router(const MoeParams& p, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.T + kTok - 1) / kTok) * kRouterCluster);
-  cfg.blockDim = dim3(kRouterThreads);
+  cfg.blockDim = dim3(kRouterThreads<kTok>);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -987,12 +1017,10 @@ int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
 cudaError_t launch_moe(const MoeParams& p, int num_sms, cudaStream_t stream) {
   if (p.T == 0) return cudaSuccess;
   // tokens per cluster: few, for the most CTAs, until the experts' rows are read often enough to count
-  const cudaError_t e = p.T <= 16   ? launch_router<1>(p, stream)
-                        : p.T <= 64 ? launch_router<4>(p, stream)
-                                    : launch_router<8>(p, stream);
+  const cudaError_t e = p.T <= 16 ? launch_router<1>(p, stream) : launch_router<4>(p, stream);
   if (e != cudaSuccess) return e;
   return tile_tokens(p.T, p.E, p.top_k) == 16 ? launch_experts<16>(p, num_sms, stream)
-                                : launch_experts<64>(p, num_sms, stream);
+                                : launch_experts<32>(p, num_sms, stream);
 }
 
 }  // namespace fp8attn
