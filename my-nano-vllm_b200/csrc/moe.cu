@@ -50,9 +50,8 @@ __device__ __forceinline__ uint16_t f32_to_bf16(float x) {
 }
 
 // ------------------------------------------------------------------ router
-template <int kTok>
-constexpr int kRouterThreads = kTok == 1 ? 512 : 256;
-
+constexpr int kRouterWarps = 8;
+constexpr int kRouterThreads = kRouterWarps * 32;
 constexpr int kRouterCluster = 8;
 constexpr int kExpertsPerLane = kMoeMaxExperts / 32;
 
@@ -108,56 +107,87 @@ __device__ __forceinline__ void choose_experts(const MoeParams& p, int64_t token
   }
 }
 
-// Cluster c: tokens c kTok .. + kTok - 1.  Logits: fp32 products of 8 columns at a time, added up in
-// fp64, so that which experts are chosen does not hang on the order of a sum.
-template <int kTok>
-__global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads<kTok>)
+// d += a . b^T: a 16 x 16, b 8 x 16 bf16.  Lane l holds a's rows l / 4 and l / 4 + 8, b's row l / 4, and
+// d's rows l / 4 (d0, d1) and l / 4 + 8 (d2, d3), columns 2 (l % 4) and the next.
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Cluster c: tokens 8 c .. 8 c + 7; CTA r of it: experts 16 r .. 16 r + 15, then 128 on, ...; a CTA's
+// warps share the columns, 32 at a time, each lane loading 16 contiguous bytes of a row (which
+// columns a product's step takes does not matter as long as both operands agree), a warp's loads
+// all in flight.  Sums of 32 products in fp32, then fp64, so that which experts are chosen does not
+// hang on the order of a sum.  The logits of token 8 c + r meet in CTA r.
+// Bound: latency (a launch, a load from HBM, two cluster barriers, the choice).
+constexpr int kRouterTokens = 8;
+static_assert(kRouterTokens <= kRouterCluster, "a CTA chooses for one token at most");
+
+__global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads)
     moe_router_kernel(const MoeParams p) {
-  static_assert(kTok <= kRouterCluster, "a CTA chooses for one token at most");
-  __shared__ float logits[kMoeMaxExperts];  // of token (cluster's first + this CTA's rank)
+  __shared__ float logits[kMoeMaxExperts];
+  __shared__ double part[kRouterWarps][16][kRouterTokens];
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();  // every CTA has started: its shared memory may be written
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the counters of the next kernel
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kRouterThreads<kTok> + threadIdx.x; i < p.num_counters;
-       i += static_cast<int64_t>(gridDim.x) * kRouterThreads<kTok>)
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kRouterThreads + threadIdx.x; i < p.num_counters;
+       i += static_cast<int64_t>(gridDim.x) * kRouterThreads)
     p.counters[i] = 0;
   const int rank = static_cast<int>(cluster.block_rank());
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x / kRouterCluster) * kTok;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x / kRouterCluster) * kRouterTokens;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int e = rank * (kRouterThreads<kTok> / 32) + warp; e < p.E; e += kRouterCluster * kRouterThreads<kTok> / 32) {
-    const uint16_t* w = p.router + static_cast<int64_t>(e) * p.H;
-    double acc[kTok];
+  const int row = lane >> 2, col = 8 * (lane & 3);
+  const bool real = t0 + row < p.T;
+  const uint16_t* x = p.x + (t0 + row) * p.x_row_stride + col;
+  for (int e0 = 16 * rank; e0 < p.E; e0 += 16 * kRouterCluster) {
+    const uint16_t* w = p.router + static_cast<int64_t>(e0 + row) * p.H + col;
+    const bool lo = e0 + row < p.E, hi = e0 + row + 8 < p.E;
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    constexpr int kAhead = 8;  // steps whose loads are in flight
+    const int stride = 32 * kRouterWarps;
+    for (int c0 = 32 * warp; c0 < p.H; c0 += kAhead * stride) {
+      uint4 wl[kAhead], wh[kAhead], xv[kAhead];
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) acc[t] = 0.0;
-#pragma unroll (kTok == 1 ? 8 : 2)
-    for (int c = 8 * lane; c < p.H; c += 256) {
-      const uint4 wr = __ldg(reinterpret_cast<const uint4*>(w + c));
-      const uint32_t ww[4] = {wr.x, wr.y, wr.z, wr.w};
-#pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        const int64_t token = min(t0 + t, p.T - 1);
-        const uint4 xr = *reinterpret_cast<const uint4*>(p.x + token * p.x_row_stride + c);
-        const uint32_t xx[4] = {xr.x, xr.y, xr.z, xr.w};
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s = fmaf(__uint_as_float(xx[i] << 16), __uint_as_float(ww[i] << 16), s);
-          s = fmaf(__uint_as_float(xx[i] & 0xFFFF0000u), __uint_as_float(ww[i] & 0xFFFF0000u), s);
+      for (int s = 0; s < kAhead; ++s) {
+        const int c = c0 + s * stride;
+        wl[s] = wh[s] = xv[s] = make_uint4(0, 0, 0, 0);
+        if (c < p.H) {
+          if (lo) wl[s] = __ldg(reinterpret_cast<const uint4*>(w + c));
+          if (hi) wh[s] = __ldg(reinterpret_cast<const uint4*>(w + 8LL * p.H + c));
+          if (real) xv[s] = *reinterpret_cast<const uint4*>(x + c);
         }
-        acc[t] += s;
+      }
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_bf16(d, wl[s].x, wh[s].x, wl[s].y, wh[s].y, xv[s].x, xv[s].y);
+        mma_bf16(d, wl[s].z, wh[s].z, wl[s].w, wh[s].w, xv[s].z, xv[s].w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += d[i];
       }
     }
+    part[warp][row][2 * (lane & 3)] = acc[0];
+    part[warp][row][2 * (lane & 3) + 1] = acc[1];
+    part[warp][row + 8][2 * (lane & 3)] = acc[2];
+    part[warp][row + 8][2 * (lane & 3) + 1] = acc[3];
+    __syncthreads();
+    if (threadIdx.x < 16 * kRouterTokens) {
+      const int e = threadIdx.x / kRouterTokens, t = threadIdx.x % kRouterTokens;
+      double sum = 0.0;
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], off);
-      if (lane == t) *cluster.map_shared_rank(&logits[e], t) = static_cast<float>(acc[t]);
+      for (int k = 0; k < kRouterWarps; ++k) sum += part[k][e][t];
+      if (e0 + e < p.E) *cluster.map_shared_rank(&logits[e0 + e], t) = static_cast<float>(sum);
     }
+    __syncthreads();
   }
   cluster.sync();
-  if (warp == 0 && rank < kTok && t0 + rank < p.T) choose_experts(p, t0 + rank, logits, lane);
+  if (warp == 0 && rank < kRouterTokens && t0 + rank < p.T) choose_experts(p, t0 + rank, logits, lane);
 }
 
 // ------------------------------------------------------------------ experts
@@ -189,13 +219,15 @@ struct Phase {
   int units;
   int items;
 };
+constexpr int kMaxRanges = 256;
+static_assert(static_cast<uint64_t>(kMaxTiles) * 128 * 128 * (kMaxRanges + 1) < 1ull << 32, "32-bit cuts");
 __device__ __forceinline__ int range_begin(const Phase& f, int r) {
-  return f.whole ? static_cast<int>(static_cast<int64_t>(f.items) * r / f.ranges) * f.steps
-                 : static_cast<int>(static_cast<int64_t>(f.units) * r / f.ranges);
+  return static_cast<int>(f.whole ? static_cast<uint32_t>(f.items) * r / f.ranges * f.steps
+                                  : static_cast<uint32_t>(f.units) * r / f.ranges);
 }
 // The range that holds unit x (not whole): the largest r with floor(units r / ranges) <= x.
 __device__ __forceinline__ int range_of(const Phase& f, int x) {
-  return static_cast<int>((static_cast<int64_t>(x + 1) * f.ranges + f.units - 1) / f.units) - 1;
+  return static_cast<int>((static_cast<uint32_t>(x + 1) * f.ranges + f.units - 1) / f.units) - 1;
 }
 
 template <int NT>
@@ -967,7 +999,7 @@ cudaError_t launch_experts(const MoeParams& p, int num_sms, cudaStream_t stream)
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(num_sms);
+  cfg.gridDim = dim3(num_sms < kMaxRanges ? num_sms : kMaxRanges);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -976,18 +1008,17 @@ cudaError_t launch_experts(const MoeParams& p, int num_sms, cudaStream_t stream)
   return cudaLaunchKernelEx(&cfg, moe_experts_kernel<NT>, tm13, tm2, p);
 }
 
-template <int kTok>
 cudaError_t launch_router(const MoeParams& p, cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.T + kTok - 1) / kTok) * kRouterCluster);
-  cfg.blockDim = dim3(kRouterThreads<kTok>);
+  cfg.gridDim = dim3(static_cast<unsigned>((p.T + kRouterTokens - 1) / kRouterTokens) * kRouterCluster);
+  cfg.blockDim = dim3(kRouterThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, moe_router_kernel<kTok>, p);
+  return cudaLaunchKernelEx(&cfg, moe_router_kernel, p);
 }
 
 }  // namespace
@@ -1016,8 +1047,7 @@ int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
 
 cudaError_t launch_moe(const MoeParams& p, int num_sms, cudaStream_t stream) {
   if (p.T == 0) return cudaSuccess;
-  // tokens per cluster: few, for the most CTAs, until the experts' rows are read often enough to count
-  const cudaError_t e = p.T <= 16 ? launch_router<1>(p, stream) : launch_router<4>(p, stream);
+  const cudaError_t e = launch_router(p, stream);
   if (e != cudaSuccess) return e;
   return tile_tokens(p.T, p.E, p.top_k) == 16 ? launch_experts<16>(p, num_sms, stream)
                                 : launch_experts<32>(p, num_sms, stream);
