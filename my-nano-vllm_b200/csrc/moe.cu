@@ -26,7 +26,7 @@
 //   the ring already holds the weights.  Sums run in an order that the choice of experts alone
 //   fixes: results do not depend on timing.
 //   Warps: one issues weight tiles by TMA, four gather the tokens' rows (cp.async into the same
-//   swizzled layout) and scale products, one issues tcgen05 MMAs (D[128 weight rows, N tokens] per
+//   swizzled layout) and scale products, two issue tcgen05 MMAs (D[128 weight rows, N tokens] per
 //   128 columns of K, weights and tokens both from shared memory), eight take D from tensor memory,
 //   scale and add it, and finish items.
 #include <type_traits>
@@ -194,7 +194,8 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
 constexpr int kPromoWarps = 8;  // warps 0-7
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
-constexpr int kLoaderWarp = 10;  // and after
+constexpr int kMmaWarps = 2;     // 9, 10: one for each of a unit's two tiles
+constexpr int kLoaderWarp = 11;  // .. 14
 constexpr int kLoaders = 4;
 constexpr int kWarps = kLoaderWarp + kLoaders;
 constexpr int kThreads = kWarps * 32;
@@ -723,10 +724,15 @@ struct Gather {
   }
 };
 
+// MMA issuer `which`: that one of each unit's two tiles.  An MMA holds its issuing thread for about 100
+// cycles: one thread for both tiles took 0.83 us a unit, 39 GB/s an SM, and paced the whole kernel.
 template <int NT>
-__device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int lane) {
+__device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int which, int lane) {
   constexpr int kStages = MoeSmem<NT>::kStages;
-  const uint32_t tmem = sm.tmem_base;
+  const uint32_t tmem = sm.tmem_base + which * NT;
+  // descriptors of stage 0; a stage and 32 bytes of K add to the start address / 16
+  const uint64_t w0 = tc::smem_desc(smem_u32(sm.w[0][which]), 16, 1024, tc::kSw128);
+  const uint64_t x0 = tc::smem_desc(smem_u32(sm.x[0][0]), 16, 1024, tc::kSw128);
   uint32_t r = 0;
   bool ok = true;
   int ticket;
@@ -737,21 +743,25 @@ __device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int lane) {
       const int range = range_in(sm, ticket, ph);
       const int begin = sm.start[ph][range].unit, end = sm.start[ph][range + 1].unit;
       Cursor<NT> c(sm, sm.start[ph][range]);
+      const uint64_t xs = x0 + (ph == 1 ? which * (sizeof(sm.x[0][0]) >> 4) : 0);
+      int tile = -1;
+      uint32_t idesc = 0;
       for (int u = begin; u < end && ok; ++u, ++r, c.next(sm, f)) {
         const int stage = r % kStages, buf = r % kDBufs;
+        if (c.tile != tile) {
+          tile = c.tile;
+          idesc = tc::idesc_e4m3(kBlk, Tile<NT>(sm, tile).columns(), false, false);
+        }
         ok = mbar_wait(&sm.w_full[stage], (r / kStages) & 1, p.err) &&
              mbar_wait(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
              mbar_wait(&sm.d_empty[buf], ((r / kDBufs) & 1) ^ 1, p.err);
         if (!ok) break;
         tc::fence_after_sync();
-        const uint32_t idesc = tc::idesc_e4m3(kBlk, Tile<NT>(sm, c.tile).columns(), false, false);
-        const int subs = ph == 0 || (2 * c.k + 1) * kBlk < p.I ? 2 : 1;
-        for (int s = 0; s < subs; ++s) {
-          const uint64_t wd = tc::smem_desc(smem_u32(sm.w[stage][s]), 16, 1024, tc::kSw128);
-          const uint64_t xd = tc::smem_desc(smem_u32(sm.x[stage][ph == 0 ? 0 : s]), 16, 1024, tc::kSw128);
+        if (which == 0 || ph == 0 || (2 * c.k + 1) * kBlk < p.I) {
+          const uint64_t wd = w0 + stage * (sizeof(sm.w[0]) >> 4), xd = xs + stage * (sizeof(sm.x[0]) >> 4);
 #pragma unroll
-          for (int ks = 0; ks < kBlk / 32; ++ks)  // 32 bytes of K add 2 to the start address / 16
-            tc::mma_f8_plain(tmem + (buf * 2 + s) * NT, wd + static_cast<uint64_t>(2 * ks),
+          for (int ks = 0; ks < kBlk / 32; ++ks)
+            tc::mma_f8_plain(tmem + buf * 2 * NT, wd + static_cast<uint64_t>(2 * ks),
                              xd + static_cast<uint64_t>(2 * ks), idesc, ks > 0 ? 1u : 0u);
         }
         tc::commit(&sm.d_full[buf]);
@@ -969,15 +979,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < MoeSmem<NT>::kStages; ++i) {
       mbar_init(&sm.w_full[i], 1);
       mbar_init(&sm.x_full[i], 1);
-      mbar_init(&sm.empty[i], 1 + kPromoWarps);
+      mbar_init(&sm.empty[i], kMmaWarps + kPromoWarps);
     }
     for (int i = 0; i < kDBufs; ++i) {
-      mbar_init(&sm.d_full[i], 1);
+      mbar_init(&sm.d_full[i], kMmaWarps);
       mbar_init(&sm.d_empty[i], kPromoWarps);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.claim_full[i], 1);
-      mbar_init(&sm.claim_empty[i], kPromoWarps + 1 + kLoaders);
+      mbar_init(&sm.claim_empty[i], kPromoWarps + kMmaWarps + kLoaders);
     }
     fence_mbar_init();
   }
@@ -1001,8 +1011,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kProducerWarp) {
     if (lane == 0) produce<NT>(sm, p, &tm13, &tm2, ticket);
     __syncwarp();
-  } else if (warp == kMmaWarp) {
-    multiply<NT>(sm, p, lane);
+  } else if (warp >= kMmaWarp && warp < kLoaderWarp) {
+    multiply<NT>(sm, p, warp - kMmaWarp, lane);
   } else if (warp >= kLoaderWarp) {
     Gather<NT>(sm, p, warp - kLoaderWarp, lane).run_all();
   } else {
