@@ -211,29 +211,31 @@ static_assert(kMoeMaxExperts + kMoeMaxSlots / 32 <= kMaxTiles &&
                   kMoeMaxExperts + kFewTokens * kMoeMaxExperts / 16 <= kMaxTiles, "tiles");
 int tile_tokens(int64_t T, int E, int top_k) { return T <= 16 || T * top_k <= kFewTokens * E ? 16 : 32; }
 
-// A phase's units, items in order, are cut into equal ranges.
+// A phase's units, items in order, are cut into equal ranges, one per CTA.  (Handing an eighth of the work
+// out in smaller ranges, for SMs that get less bandwidth, cost 5 to 30 %: more items are cut.)
 struct Phase {
-  int blocks;   // items per tile (output columns / 128)
-  int steps;    // units per item
-  int ranges;
-  int whole;    // cut between items only
-  int units;
+  int blocks;  // items per tile (output columns / 128)
+  int steps;   // units per item
   int items;
+  int units;
+  int whole;   // cut between items only
+  int ranges;
 };
-constexpr int kMaxRanges = 256;
-static_assert(static_cast<uint64_t>(kMaxTiles) * 128 * 128 * (kMaxRanges + 1) < 1ull << 32, "32-bit cuts");
+constexpr int kMaxGrid = 256;
+static_assert(static_cast<uint64_t>(kMaxTiles) * 128 * 128 * (kMaxGrid + 1) < 1ull << 32, "32-bit cuts");
 __device__ __forceinline__ int range_begin(const Phase& f, int r) {
   return static_cast<int>(f.whole ? static_cast<uint32_t>(f.items) * r / f.ranges * f.steps
                                   : static_cast<uint32_t>(f.units) * r / f.ranges);
 }
-// The range that holds unit x (not whole): the largest r with floor(units r / ranges) <= x.
+// The range that holds unit x (not whole): the largest r with range_begin(r) <= x.
 __device__ __forceinline__ int range_of(const Phase& f, int x) {
   return static_cast<int>((static_cast<uint32_t>(x + 1) * f.ranges + f.units - 1) / f.units) - 1;
 }
-// Where a range begins.
-struct Start {
-  int unit;
-  uint16_t tile, blk, k, pad;
+// A range to work through: units [begin, end) of a phase, the first being step k of item (tile, blk).
+struct Claim {
+  int phase;  // -1: no more
+  int range, begin, end;
+  int tile, blk, k;
 };
 
 template <int NT>
@@ -246,10 +248,11 @@ struct __align__(1024) MoeSmem {
   uint64_t w_full[kStages], x_full[kStages], empty[kStages];
   uint64_t d_full[kDBufs], d_empty[kDBufs];
   uint64_t claim_full[2], claim_empty[2];
-  int claim[2];
+  Claim claim[2];
   Phase phase[3];
-  Start start[2][kMaxRanges + 1];
-  int last;                            // promotion threads: this CTA finishes the item
+  // promotion threads, of a cut item: the other parts have come; this CTA came last.  Two words: each is
+  // written again only after a barrier that follows its last reading.
+  int others_here, last;
   uint32_t tmem_base;
   int tiles;
   uint32_t tile[kMaxTiles];            // expert << 16 | index of the tile among the expert's
@@ -364,16 +367,49 @@ __device__ __forceinline__ Phase make_phase(const MoeParams& p, int which, int t
   f.units = f.items * f.steps;
   // Whole items where that costs at most two units' time more than equal ranges: a cut item's parts
   // go through memory
-  const int even = (f.units + grid - 1) / grid;
-  f.whole = (f.items + grid - 1) / grid * f.steps <= even + 2;
+  f.whole = (f.items + grid - 1) / grid * f.steps <= (f.units + grid - 1) / grid + 2;
   f.ranges = min(grid, f.whole ? f.items : f.units);
   return f;
 }
 
+// The range of a ticket.  Tickets: the ranges of phase 0, of phase 1, then of the weighted sums.
 template <int NT>
-__device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
+__device__ __forceinline__ Claim make_claim(const MoeSmem<NT>& sm, int ticket) {
+  Claim c = {0, ticket, 0, 0, 0, 0, 0};
+  while (c.phase < 3 && c.range >= sm.phase[c.phase].ranges) c.range -= sm.phase[c.phase++].ranges;
+  if (c.phase == 3) {
+    c.phase = -1;
+    return c;
+  }
+  const Phase f = sm.phase[c.phase];
+  c.begin = range_begin(f, c.range);
+  c.end = range_begin(f, c.range + 1);
+  if (c.phase == 2) return c;
+  const int item = c.begin / f.steps, some = item / f.blocks;  // some: a tile of the item's expert
+  const uint32_t tile = sm.tile[some];
+  const int e = static_cast<int>(tile >> 16), first = some - static_cast<int>(tile & 0xFFFFu);
+  const int count = (sm.first[e + 1] - sm.first[e] + NT - 1) / NT, in = item - first * f.blocks;
+  c.k = c.begin - item * f.steps;
+  c.blk = in / count;
+  c.tile = first + in - c.blk * count;
+  return c;
+}
+
+// The lanes that have the same e (of `bits` bits) as this one, among those that are ok.
+__device__ __forceinline__ unsigned same_expert(int e, bool ok, int bits) {
+  unsigned same = __ballot_sync(0xffffffffu, ok);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (e >> b) & 1;
+    const unsigned v = __ballot_sync(0xffffffffu, one);
+    same &= one ? v : ~v;
+  }
+  return same;
+}
+
+template <int NT>
+__device__ void plan(MoeSmem<NT>& sm, const MoeParams& p, int ticket) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int n = static_cast<int>(p.T) * p.top_k;
+  const int n = static_cast<int>(p.T) * p.top_k, bits = 32 - __clz(p.E - 1);
   PlanScratch& s = plan_scratch(sm);
   const int per = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;  // a warp's slots: [warp per, + per)
   const int lo = min(warp * per, n), hi = min(lo + per, n);
@@ -384,8 +420,8 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
   for (int i0 = lo; i0 < hi; i0 += 32) {
     const int i = i0 + lane;
     const bool ok = i < hi;
-    const int e = ok ? s.expert[i] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const int e = ok ? s.expert[i] : 0;
+    const unsigned same = same_expert(e, ok, bits);
     if (ok && lane == __ffs(same) - 1) s.count[warp][e] += static_cast<uint16_t>(__popc(same));
     __syncwarp();
   }
@@ -429,34 +465,18 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p) {
     if (lane == 0) sm.tiles = tiles;
   }
   __syncthreads();
+  if (warp == kProducerWarp && lane == 0) sm.claim[0] = make_claim(sm, ticket);
   for (int i0 = lo; i0 < hi; i0 += 32) {
     const int i = i0 + lane;
     const bool ok = i < hi;
-    const int e = ok ? s.expert[i] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const int e = ok ? s.expert[i] : 0;
+    const unsigned same = same_expert(e, ok, bits);
     if (ok)
       sm.order[sm.first[e] + s.count[warp][e] + __popc(same & ((1u << lane) - 1))] =
           static_cast<uint16_t>(i);
     __syncwarp();
     if (ok && lane == __ffs(same) - 1) s.count[warp][e] += static_cast<uint16_t>(__popc(same));
     __syncwarp();
-  }
-  // the ranges' beginnings, whose divisions would hold every role up
-  for (int i = tid; i < 2 * (kMaxRanges + 1); i += kThreads) {
-    const int ph = i / (kMaxRanges + 1), r = i % (kMaxRanges + 1);
-    const Phase f = sm.phase[ph];
-    if (r > f.ranges) continue;
-    Start at = {range_begin(f, r), 0, 0, 0, 0};
-    if (r < f.ranges) {
-      const int item = at.unit / f.steps, some = item / f.blocks;  // some: a tile of the item's expert
-      const uint32_t tile = sm.tile[some];
-      const int e = static_cast<int>(tile >> 16), first = some - static_cast<int>(tile & 0xFFFFu);
-      const int count = (sm.first[e + 1] - sm.first[e] + NT - 1) / NT, in = item - first * f.blocks;
-      at.k = static_cast<uint16_t>(at.unit - item * f.steps);
-      at.blk = static_cast<uint16_t>(in / count);
-      at.tile = static_cast<uint16_t>(first + in - at.blk * count);
-    }
-    sm.start[ph][r] = at;
   }
   // the ring's next writer is the async proxy
   fence_proxy_async_smem();
@@ -470,7 +490,7 @@ struct Cursor {
   int first, count;  // the expert's tiles
   int tile, blk, k;
   __device__ __forceinline__ Cursor() {}
-  __device__ __forceinline__ Cursor(const MoeSmem<NT>& sm, const Start& at)
+  __device__ __forceinline__ Cursor(const MoeSmem<NT>& sm, const Claim& at)
       : tile(at.tile), blk(at.blk), k(at.k) {
     expert_of(sm, tile);
   }
@@ -505,52 +525,44 @@ struct Tile {
   __device__ __forceinline__ int columns() const { return (count + 15) & ~15; }  // the MMA's N
 };
 
-// Tickets: the ranges of phase 0, of phase 1, then of the weighted sums.
-template <int NT>
-__device__ __forceinline__ int phase_of(const MoeSmem<NT>& sm, int ticket) {
-  return (ticket >= sm.phase[0].ranges) + (ticket >= sm.phase[0].ranges + sm.phase[1].ranges);
-}
-template <int NT>
-__device__ __forceinline__ int range_in(const MoeSmem<NT>& sm, int ticket, int phase) {
-  return ticket - (phase > 0 ? sm.phase[0].ranges : 0) - (phase > 1 ? sm.phase[1].ranges : 0);
-}
-
 // The next range, for every warp but the producer.  False: no more.
 template <int NT>
-__device__ __forceinline__ bool next_claim(MoeSmem<NT>& sm, int i, int lane, int* err, int& ticket) {
+__device__ __forceinline__ bool next_claim(MoeSmem<NT>& sm, int i, int lane, int* err, Claim& claim) {
   if (!mbar_wait(&sm.claim_full[i & 1], (i >> 1) & 1, err)) return false;
-  ticket = sm.claim[i & 1];
+  claim = sm.claim[i & 1];
   __syncwarp();
   if (lane == 0) mbar_arrive(&sm.claim_empty[i & 1]);
-  return ticket >= 0;
+  return claim.phase >= 0;
 }
 
 template <int NT>
 __device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* tm13,
-                        const CUtensorMap* tm2, int ticket) {
+                        const CUtensorMap* tm2) {
   constexpr int kStages = MoeSmem<NT>::kStages;
-  const int total = sm.phase[0].ranges + sm.phase[1].ranges + sm.phase[2].ranges;
   uint32_t r = 0;
   bool ok = true;
+  int ticket = 0;
   for (int i = 0;; ++i) {
-    ok = ok && mbar_wait(&sm.claim_empty[i & 1], ((i >> 1) & 1) ^ 1, p.err);
-    const bool more = ok && ticket < total;
-    sm.claim[i & 1] = more ? ticket : -1;
+    Claim claim = sm.claim[0];  // the first one was made with the plan
+    if (i > 0) {
+      claim = make_claim(sm, ticket);
+      ok = ok && mbar_wait(&sm.claim_empty[i & 1], ((i >> 1) & 1) ^ 1, p.err);
+      if (!ok) claim.phase = -1;
+      sm.claim[i & 1] = claim;
+    }
     mbar_arrive(&sm.claim_full[i & 1]);
-    if (!more) return;
-    const int ph = phase_of(sm, ticket);
-    const Phase f = sm.phase[ph];
-    const int range = range_in(sm, ticket, ph);
+    const int ph = claim.phase;
+    if (ph < 0) return;
     if (ph == 2) {  // nothing to load
       ticket = atomicAdd(p.counters, 1);
       continue;
     }
-    const int begin = sm.start[ph][range].unit, end = sm.start[ph][range + 1].unit;
-    Cursor<NT> c(sm, sm.start[ph][range]);
-    for (int u = begin; u < end && ok; ++u, ++r, c.next(sm, f)) {
+    const Phase f = sm.phase[ph];
+    Cursor<NT> c(sm, claim);
+    for (int u = claim.begin; u < claim.end && ok; ++u, ++r, c.next(sm, f)) {
       // the next ticket: its latency hides behind this range, whose first half lets a CTA that starts
       // late have its turn (one that held two ranges of a phase would take twice as long)
-      if (u == begin + (end - begin) / 2) ticket = atomicAdd(p.counters, 1);
+      if (u == claim.begin + (claim.end - claim.begin) / 2) ticket = atomicAdd(p.counters, 1);
       const int stage = r % kStages;
       const int expert = static_cast<int>(sm.tile[c.tile] >> 16);
       if (!mbar_wait(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err)) {
@@ -625,16 +637,15 @@ struct Gather {
   __device__ __forceinline__ bool advance(Unit& flying) {
     for (;;) {
       while (u == end) {
-        int ticket;
+        Claim claim;
         finish(flying, false);
-        if (!next_claim(sm, claims++, lane, p.err, ticket)) return false;
-        ph = phase_of(sm, ticket);
+        if (!next_claim(sm, claims++, lane, p.err, claim)) return false;
+        ph = claim.phase;
         if (ph == 2) continue;
         f = sm.phase[ph];
-        const int range = range_in(sm, ticket, ph);
-        u = sm.start[ph][range].unit;
-        end = sm.start[ph][range + 1].unit;
-        c = Cursor<NT>(sm, sm.start[ph][range]);
+        u = claim.begin;
+        end = claim.end;
+        c = Cursor<NT>(sm, claim);
         ready = -1;
       }
       if (static_cast<int>(r % kLoaders) == which) return true;
@@ -735,18 +746,16 @@ __device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int which, int lan
   const uint64_t x0 = tc::smem_desc(smem_u32(sm.x[0][0]), 16, 1024, tc::kSw128);
   uint32_t r = 0;
   bool ok = true;
-  int ticket;
-  for (int i = 0; next_claim(sm, i, lane, p.err, ticket); ++i) {
-    const int ph = phase_of(sm, ticket);
+  Claim claim;
+  for (int i = 0; next_claim(sm, i, lane, p.err, claim); ++i) {
+    const int ph = claim.phase;
     if (lane == 0 && ph < 2) {
       const Phase f = sm.phase[ph];
-      const int range = range_in(sm, ticket, ph);
-      const int begin = sm.start[ph][range].unit, end = sm.start[ph][range + 1].unit;
-      Cursor<NT> c(sm, sm.start[ph][range]);
+      Cursor<NT> c(sm, claim);
       const uint64_t xs = x0 + (ph == 1 ? which * (sizeof(sm.x[0][0]) >> 4) : 0);
       int tile = -1;
       uint32_t idesc = 0;
-      for (int u = begin; u < end && ok; ++u, ++r, c.next(sm, f)) {
+      for (int u = claim.begin; u < claim.end && ok; ++u, ++r, c.next(sm, f)) {
         const int stage = r % kStages, buf = r % kDBufs;
         if (c.tile != tile) {
           tile = c.tile;
@@ -813,13 +822,11 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
   int* const part_count = ready + kMaxTiles;  // [2][grid]
   uint32_t r = 0;
   bool ok = true;
-  int ticket;
-  for (int i = 0; next_claim(sm, i, lane, p.err, ticket); ++i) {
-    const int ph = phase_of(sm, ticket);
+  Claim claim;
+  for (int i = 0; next_claim(sm, i, lane, p.err, claim); ++i) {
+    const int ph = claim.phase, range = claim.range, begin = claim.begin, end = claim.end;
     const Phase f = sm.phase[ph];
-    const int range = range_in(sm, ticket, ph);
     if (ph == 2) {
-      const int begin = range_begin(f, range), end = range_begin(f, range + 1);
       // ---- weighted sums, once phase 1 has ended: its ranges are held by CTAs that run
       ok = ok && wait_counter(p.counters + kDoneAt, sm.phase[1].ranges, p.err);
       for (int item = begin + warp / 2; item < end && ok; item += kPromoWarps / 2) {
@@ -854,8 +861,7 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
       }
       continue;
     }
-    const int begin = sm.start[ph][range].unit, end = sm.start[ph][range + 1].unit;
-    Cursor<NT> c(sm, sm.start[ph][range]);
+    Cursor<NT> c(sm, claim);
     int u = begin;
     while (u < end) {
       // ---- one item, or the part of it that this range holds
@@ -869,8 +875,15 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
 #pragma unroll
       for (int j = 0; j < kHalf; ++j) g[j] = v[j] = 0.f;
       const bool at_head = u != item_begin;
+      // a cut item's parts: those of ranges r0 .. r1
+      const int r0 = cut ? range_of(f, item_begin) : 0;
+      const int r1 = cut ? range_of(f, item_begin + f.steps - 1) : 0;
+      int* const arrived = part_count + ph * gridDim.x + r0;
+      int others = 0;
       for (; u < stop; ++u, ++r, c.next(sm, f)) {
         const int stage = r % kStages, buf = r % kDBufs;
+        // whoever begins an item usually comes last to it: are the other parts there already?
+        if (u == stop - 1 && cut && !at_head && tid == 0) others = load_acquire(arrived);
         ok = ok && mbar_wait(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
              mbar_wait(&sm.d_full[buf], (r / kDBufs) & 1, p.err);
         if (!ok) continue;
@@ -889,54 +902,57 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
           mbar_arrive(&sm.empty[stage]);
         }
       }
-      // ---- the item's sums, token by token: through shared memory, or, of a cut item, through global
+      // ---- the item's sums, token by token: through shared memory, and, of a cut item, through global
       // memory, where the CTA that comes last adds the parts, in order
       constexpr int kPart = NT * kBlk;  // floats; phase 0 has two of them (gate, up)
       float* const parts = p.parts[ph];
       const int size = ph == 0 ? 2 * kPart : kPart;
-      float* mine = cut ? parts + (2 * static_cast<int64_t>(range) + (at_head ? 0 : 1)) * size
-                        : &sm.item[0][0][0];
+      auto put = [&](float* to) {
 #pragma unroll
-      for (int j = 0; j < kHalf; ++j)
-        if (j < 8 * groups) {
-          mine[(m0 + j) * kBlk + col] = g[j];
-          if (ph == 0) mine[kPart + (m0 + j) * kBlk + col] = v[j];
-        }
+        for (int j = 0; j < kHalf; ++j)
+          if (j < 8 * groups) {
+            to[(m0 + j) * kBlk + col] = g[j];
+            if (ph == 0) to[kPart + (m0 + j) * kBlk + col] = v[j];
+          }
+      };
+      float* const mine = parts + (2 * static_cast<int64_t>(range) + (at_head ? 0 : 1)) * size;
+      put(at_head ? mine : &sm.item[0][0][0]);
+      if (tid == 0) sm.others_here = others == r1 - r0;
       promo_sync();
-      int r0 = 0, r1 = 0;
-      if (cut) {
-        r0 = range_of(f, item_begin);
-        r1 = range_of(f, item_begin + f.steps - 1);
-        if (tid == 0) sm.last = add_acq_rel(part_count + ph * gridDim.x + r0) == r1 - r0;
+      const bool here = !cut || (!at_head && sm.others_here);  // part 0 in shared memory, the others complete
+      if (!here) {
+        if (!at_head) {
+          put(mine);
+          promo_sync();
+        }
+        if (tid == 0) sm.last = add_acq_rel(arrived) == r1 - r0;
         promo_sync();
         if (!sm.last) continue;
       }
       // a warp takes tokens warp, warp + 8, ...; lane: 4 of the 128 columns
       for (int m = warp; m < t.count; m += kPromoWarps) {
-        float4 a, b = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!cut) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (here) {
           a = *reinterpret_cast<const float4*>(&sm.item[0][m][4 * lane]);
           if (ph == 0) b = *reinterpret_cast<const float4*>(&sm.item[1][m][4 * lane]);
-        } else {
-          a = b;
+        }
 #pragma unroll 1
-          for (int q0 = r0; q0 <= r1; q0 += 4) {  // four parts' loads in flight
-            float4 pa[4], pb[4];
+        for (int q0 = here ? r0 + 1 : r0; cut && q0 <= r1; q0 += 4) {  // four parts' loads in flight
+          float4 pa[4], pb[4];
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              const float* part = parts + (2 * static_cast<int64_t>(q0 + d) + (q0 + d == r0 ? 1 : 0)) * size +
-                                  m * kBlk + 4 * lane;
-              pa[d] = pb[d] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (q0 + d <= r1) {
-                pa[d] = __ldcg(reinterpret_cast<const float4*>(part));
-                if (ph == 0) pb[d] = __ldcg(reinterpret_cast<const float4*>(part + kPart));
-              }
+          for (int d = 0; d < 4; ++d) {
+            const float* part = parts + (2 * static_cast<int64_t>(q0 + d) + (q0 + d == r0 ? 1 : 0)) * size +
+                                m * kBlk + 4 * lane;
+            pa[d] = pb[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (q0 + d <= r1) {
+              pa[d] = __ldcg(reinterpret_cast<const float4*>(part));
+              if (ph == 0) pb[d] = __ldcg(reinterpret_cast<const float4*>(part + kPart));
             }
+          }
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              a = make_float4(a.x + pa[d].x, a.y + pa[d].y, a.z + pa[d].z, a.w + pa[d].w);
-              b = make_float4(b.x + pb[d].x, b.y + pb[d].y, b.z + pb[d].z, b.w + pb[d].w);
-            }
+          for (int d = 0; d < 4; ++d) {
+            a = make_float4(a.x + pa[d].x, a.y + pa[d].y, a.z + pa[d].z, a.w + pa[d].w);
+            b = make_float4(b.x + pb[d].x, b.y + pb[d].y, b.z + pb[d].z, b.w + pb[d].w);
           }
         }
         const int64_t slot = sm.order[t.begin + m];
@@ -1006,10 +1022,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   int ticket = 0;
   if (warp == kProducerWarp && lane == 0) ticket = atomicAdd(p.counters, 1);
   tc::fence_before_sync();
-  plan<NT>(sm, p);  // barriers of the whole CTA
+  plan<NT>(sm, p, ticket);  // barriers of the whole CTA
   tc::fence_after_sync();
   if (warp == kProducerWarp) {
-    if (lane == 0) produce<NT>(sm, p, &tm13, &tm2, ticket);
+    if (lane == 0) produce<NT>(sm, p, &tm13, &tm2);
     __syncwarp();
   } else if (warp >= kMmaWarp && warp < kLoaderWarp) {
     multiply<NT>(sm, p, warp - kMmaWarp, lane);
@@ -1023,6 +1039,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   if (warp == kMmaWarp) tc::tmem_dealloc(sm.tmem_base, kColumns);
 }
+
+int moe_grid(int num_sms) { return num_sms < kMaxGrid ? num_sms : kMaxGrid; }
 
 template <int NT>
 cudaError_t launch_experts(const MoeParams& p, int num_sms, cudaStream_t stream) {
@@ -1044,7 +1062,7 @@ cudaError_t launch_experts(const MoeParams& p, int num_sms, cudaStream_t stream)
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(num_sms < kMaxRanges ? num_sms : kMaxRanges);
+  cfg.gridDim = dim3(moe_grid(num_sms));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1077,7 +1095,8 @@ int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
     off += (bytes + 255) / 256 * 256;
   };
   const int64_t n = p.T * p.top_k, part = static_cast<int64_t>(tile_tokens(p.T, p.E, p.top_k)) * kBlk * 4;
-  p.num_counters = kReadyAt + kMaxTiles + 2 * num_sms;
+  const int64_t ranges = moe_grid(num_sms);
+  p.num_counters = kReadyAt + kMaxTiles + 2 * ranges;
   p.top_k_inverse = ((1u << 18) + p.top_k - 1) / p.top_k;
   take(p.counters, p.num_counters * 4);
   take(p.ids, n * 4);  // where the caller gives none
@@ -1085,8 +1104,8 @@ int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
   take(p.hq, n * p.I);
   take(p.h_scale, n * (p.I / kBlk) * 2);
   take(p.y, n * p.H * 4);
-  take(p.parts[0], 2 * num_sms * 2 * part);
-  take(p.parts[1], 2 * num_sms * part);
+  take(p.parts[0], 2 * ranges * 2 * part);
+  take(p.parts[1], 2 * ranges * part);
   return off;
 }
 
