@@ -24,35 +24,47 @@ with ``torch.empty`` and never synchronise, so they can be captured into CUDA gr
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
-from .fp8_attention import _stream, workspace
+from .fp8_attention import _WORKSPACES, workspace
 from .fp8_linear import BLOCK_SIZE
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
+_BF16, _E4M3 = torch.bfloat16, torch.float8_e4m3fn
 MAX_TOKENS = 1024       # tokens in one fp8_moe call
 MAX_SLOTS = 8192        # tokens * top_k in one fp8_moe call
 
+# The kernels of a decoded token take 2 to 25 us, so the host side counts: raw stream handles and
+# empty_strided cost 0.1 and 1.5 us a call where current_stream() and empty() cost 2.2 and 2.4.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
-def _call(device: torch.device, fn, *args) -> None:
+
+def _launch(device: int, fn, *args) -> None:
     """fn(*args, stream) on the current stream of ``device``, which is made the current device for
     the launch where it is not."""
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, _stream(device)))
+    if device == _current_device():
+        rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, _stream(device)))
+            rc = fn(*args, _raw_stream(device))
+    if rc:
+        _lib.check(rc)
 
 
-def _rows(t: torch.Tensor) -> int:
-    """Row stride in elements; that of a single row is never used, and torch leaves it arbitrary."""
+def _rows(t: torch.Tensor, dtype: torch.dtype, device: int) -> int:
+    """Checks a 2-D operand; its row stride in elements (that of a single row is never used, and torch
+    leaves it arbitrary)."""
+    assert t.get_device() == device and t.dtype == dtype and t.dim() == 2 and t.stride(1) == 1, \
+        "expected rows of unit stride, of the first operand's device"
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _check_rows(t: torch.Tensor, device: torch.device, dtype: torch.dtype):
-    assert t.device == device and t.dtype == dtype and t.dim() == 2
-    assert t.stride(1) == 1 or t.shape[1] <= 1
+def _new(m: int, n: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    return torch.empty_strided((m, n), (n, 1), dtype=dtype, device=device)
 
 
 def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor,
@@ -66,50 +78,67 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: tor
     with ``return_norm``, y, both rounded to x's type (else None; residual_out is None without a
     residual).
     """
-    assert x.is_cuda and x.dtype in _DTYPES, "x must be a bf16 or fp16 CUDA tensor"
-    _check_rows(x, x.device, x.dtype)
+    dtype, device = x.dtype, x.get_device()
+    assert dtype in _DTYPES and device >= 0, "x must be a bf16 or fp16 CUDA tensor"
+    x_stride = _rows(x, dtype, device)
     M, K = x.shape
-    assert weight.device == x.device and weight.dtype == x.dtype and weight.is_contiguous()
+    assert weight.get_device() == device and weight.dtype == dtype and weight.is_contiguous()
     assert weight.numel() == K and K % BLOCK_SIZE == 0 and K > 0
+    dev = x.device
+    res_in = res_stride = res_out = y_out = 0
+    res = y = None
     if residual is not None:
-        _check_rows(residual, x.device, x.dtype)
+        res_stride = _rows(residual, dtype, device)
         assert residual.shape == x.shape
-    xq = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
-    xs = torch.empty((M, K // BLOCK_SIZE), dtype=torch.bfloat16, device=x.device)
-    res = torch.empty((M, K), dtype=x.dtype, device=x.device) if residual is not None else None
-    y = torch.empty((M, K), dtype=x.dtype, device=x.device) if return_norm else None
-    if M == 0:
-        return xq, xs, res, y
-    _call(x.device, _lib.lib.fp8attn_add_rms_norm_quant, x.data_ptr(), _rows(x),
-          residual.data_ptr() if residual is not None else 0,
-          _rows(residual) if residual is not None else 0, weight.data_ptr(), float(eps),
-          xq.data_ptr(), xs.data_ptr(), res.data_ptr() if res is not None else 0,
-          y.data_ptr() if y is not None else 0, M, K, _DTYPES[x.dtype])
+        res = _new(M, K, dtype, dev)
+        res_in, res_out = residual.data_ptr(), res.data_ptr()
+    if return_norm:
+        y = _new(M, K, dtype, dev)
+        y_out = y.data_ptr()
+    xq = _new(M, K, _E4M3, dev)
+    xs = _new(M, K // BLOCK_SIZE, _BF16, dev)
+    if M > 0:
+        _launch(device, _lib.lib.fp8attn_add_rms_norm_quant, x.data_ptr(), x_stride, res_in,
+                res_stride, weight.data_ptr(), eps, xq.data_ptr(), xs.data_ptr(), res_out, y_out, M,
+                K, _DTYPES[dtype])
     return xq, xs, res, y
 
 
 def silu_mul_fp8(gate_up: torch.Tensor):
     """gate_up: bf16 or fp16 [M, 2 I] (rows may be strided), gate columns first; I a multiple of 128.
     Returns (hq, h_scale): gate / (1 + exp(-gate)) * up as e4m3 [M, I] with scales bf16 [M, I / 128]."""
-    assert gate_up.is_cuda and gate_up.dtype in _DTYPES, "gate_up must be a bf16 or fp16 CUDA tensor"
-    _check_rows(gate_up, gate_up.device, gate_up.dtype)
+    dtype, device = gate_up.dtype, gate_up.get_device()
+    assert dtype in _DTYPES and device >= 0, "gate_up must be a bf16 or fp16 CUDA tensor"
+    stride = _rows(gate_up, dtype, device)
     M, I2 = gate_up.shape
     assert I2 % (2 * BLOCK_SIZE) == 0 and I2 > 0
-    hq = torch.empty((M, I2 // 2), dtype=torch.float8_e4m3fn, device=gate_up.device)
-    hs = torch.empty((M, I2 // 2 // BLOCK_SIZE), dtype=torch.bfloat16, device=gate_up.device)
-    if M == 0:
-        return hq, hs
-    _call(gate_up.device, _lib.lib.fp8attn_silu_mul_quant, gate_up.data_ptr(), _rows(gate_up),
-          hq.data_ptr(), hs.data_ptr(), M, I2 // 2, _DTYPES[gate_up.dtype])
+    inner, dev = I2 // 2, gate_up.device
+    hq = _new(M, inner, _E4M3, dev)
+    hs = _new(M, inner // BLOCK_SIZE, _BF16, dev)
+    if M > 0:
+        _launch(device, _lib.lib.fp8attn_silu_mul_quant, gate_up.data_ptr(), stride, hq.data_ptr(),
+                hs.data_ptr(), M, inner, _DTYPES[dtype])
     return hq, hs
 
 
-def _check_experts(w: torch.Tensor, scale: torch.Tensor, device: torch.device, shape):
-    assert w.device == device and w.dtype == torch.float8_e4m3fn and w.is_contiguous()
-    assert scale.device == device and scale.dtype == torch.bfloat16 and scale.is_contiguous()
-    e, n, k = shape
-    assert tuple(w.shape) == (e, n, k), (tuple(w.shape), shape)
-    assert tuple(scale.shape) == (e, n // BLOCK_SIZE, k // BLOCK_SIZE)
+@functools.lru_cache(maxsize=1024)
+def _moe_scratch_bytes(device: int, T: int, H: int, I: int, E: int, top_k: int) -> int:
+    with torch.cuda.device(device):
+        return _lib.lib.fp8attn_fp8_moe_workspace_bytes(T, H, I, E, top_k)
+
+
+def _error_word(device: int) -> int:
+    """Address of the device error word of the current stream's workspace (``device_error``)."""
+    ws = _WORKSPACES.get((device, _raw_stream(device)))
+    if ws is None:
+        ws = workspace(torch.device("cuda", device), 4)
+    return ws.data_ptr() + _lib.WS_ERROR_OFFSET
+
+
+def _check_experts(w: torch.Tensor, scale: torch.Tensor, device: int, e: int, n: int, k: int):
+    assert w.get_device() == device and w.dtype == _E4M3 and w.is_contiguous()
+    assert scale.get_device() == device and scale.dtype == _BF16 and scale.is_contiguous()
+    assert w.shape == (e, n, k) and scale.shape == (e, n // BLOCK_SIZE, k // BLOCK_SIZE)
 
 
 def fp8_moe(x: torch.Tensor, xq: torch.Tensor, x_scale: torch.Tensor, router_weight: torch.Tensor,
@@ -129,35 +158,34 @@ def fp8_moe(x: torch.Tensor, xq: torch.Tensor, x_scale: torch.Tensor, router_wei
     Returns bf16 [T, H], or with ``return_router`` (out, weights fp32 [T, top_k], ids int32
     [T, top_k]).
     """
-    assert x.is_cuda and x.dtype == torch.bfloat16, "x must be a bf16 CUDA tensor"
-    dev = x.device
-    _check_rows(x, dev, torch.bfloat16)
-    _check_rows(xq, dev, torch.float8_e4m3fn)
+    device = x.get_device()
+    assert device >= 0, "x must be a CUDA tensor"
+    x_stride, xq_stride = _rows(x, _BF16, device), _rows(xq, _E4M3, device)
     T, H = x.shape
     assert xq.shape == x.shape and H % BLOCK_SIZE == 0 and H > 0
-    assert x_scale.device == dev and x_scale.dtype == torch.bfloat16 and x_scale.is_contiguous()
-    assert tuple(x_scale.shape) == (T, H // BLOCK_SIZE)
-    assert router_weight.device == dev and router_weight.dtype == torch.bfloat16
+    assert x_scale.get_device() == device and x_scale.dtype == _BF16 and x_scale.is_contiguous()
+    assert x_scale.shape == (T, H // BLOCK_SIZE)
+    assert router_weight.get_device() == device and router_weight.dtype == _BF16
     assert router_weight.is_contiguous() and router_weight.dim() == 2 and router_weight.shape[1] == H
-    E = router_weight.shape[0]
-    I = down_weight.shape[-1]
+    E, I = router_weight.shape[0], down_weight.shape[-1]
     assert I % BLOCK_SIZE == 0 and I > 0
-    _check_experts(gate_up_weight, gate_up_scale, dev, (E, 2 * I, H))
-    _check_experts(down_weight, down_scale, dev, (E, H, I))
-    out = torch.empty((T, H), dtype=torch.bfloat16, device=dev)
+    _check_experts(gate_up_weight, gate_up_scale, device, E, 2 * I, H)
+    _check_experts(down_weight, down_scale, device, E, H, I)
+    dev = x.device
+    out = _new(T, H, _BF16, dev)
     weights = ids = None
+    weights_out = ids_out = 0
     if return_router:
-        weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+        weights = _new(T, top_k, torch.float32, dev)
+        ids = _new(T, top_k, torch.int32, dev)
+        weights_out, ids_out = weights.data_ptr(), ids.data_ptr()
     if T > 0:
-        nbytes = _lib.lib.fp8attn_fp8_moe_workspace_bytes(T, H, I, E, top_k)
+        nbytes = _moe_scratch_bytes(device, T, H, I, E, top_k)
         # scratch of this call alone: calls on other streams and captured graphs share none
-        scratch = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=dev)
-        _call(dev, _lib.lib.fp8attn_fp8_moe, x.data_ptr(), _rows(x), xq.data_ptr(), _rows(xq),
-              x_scale.data_ptr(), router_weight.data_ptr(), gate_up_weight.data_ptr(),
-              gate_up_scale.data_ptr(), down_weight.data_ptr(), down_scale.data_ptr(),
-              out.data_ptr(), H, weights.data_ptr() if return_router else 0,
-              ids.data_ptr() if return_router else 0, T, H, I, E, int(top_k),
-              1 if renormalize else 0, scratch.data_ptr(), nbytes,
-              workspace(dev, 4).data_ptr() + _lib.WS_ERROR_OFFSET)
+        scratch = _new(1, max(nbytes, 0), torch.uint8, dev)
+        _launch(device, _lib.lib.fp8attn_fp8_moe, x.data_ptr(), x_stride, xq.data_ptr(), xq_stride,
+                x_scale.data_ptr(), router_weight.data_ptr(), gate_up_weight.data_ptr(),
+                gate_up_scale.data_ptr(), down_weight.data_ptr(), down_scale.data_ptr(),
+                out.data_ptr(), H, weights_out, ids_out, T, H, I, E, top_k, 1 if renormalize else 0,
+                scratch.data_ptr(), nbytes, _error_word(device))
     return (out, weights, ids) if return_router else out
