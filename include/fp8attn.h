@@ -267,14 +267,14 @@ FP8ATTN_API int fp8attn_fp8_tp_linear(const void* x, int64_t x_row_stride, const
  * (1 for an all-zero group), q = e4m3(y / d), scale = bf16(d).
  *   dtype: type of the 16-bit tensors, FP8ATTN_BF16 or FP8ATTN_FP16.  Every 16-bit pointer is
  *   16-byte aligned, its row stride (elements) a multiple of 8 and at least the row's width; q is
- *   8-byte aligned, scale 2-byte aligned; outputs are contiguous.  M = 0 is a no-op.
+ *   8-byte aligned, scale 2-byte aligned; outputs are contiguous.  M below 2^31; M = 0 is a no-op.
  *   fp8attn_add_rms_norm_quant: s = x + residual (s = x if residual is NULL), y = s / sqrt(mean(s^2)
  *     + eps) * weight, all in fp32.  x, residual [M, K], weight [K]; K a multiple of 128 up to 16384.
  *     q [M, K], scale [M, K / 128]; residual_out [M, K]: s rounded to dtype (given exactly when
  *     residual is; may be the residual itself where its rows are K apart); norm_out [M, K]: y rounded
  *     to dtype, or NULL.
  *   fp8attn_silu_mul_quant: y = g / (1 + exp(-g)) * u.  gate_up [M, 2 I]: g's columns, then u's; I a
- *     multiple of 128.  q [M, I], scale [M, I / 128].
+ *     multiple of 128 up to 2^20.  q [M, I], scale [M, I / 128].
  */
 #define FP8ATTN_BF16 0
 #define FP8ATTN_FP16 1

@@ -817,9 +817,6 @@ int check_quant_out(const char* what, const void* q, const void* scale) {
   return FP8ATTN_OK;
 }
 
-// A launch has at most 2^31 - 1 CTAs; the kernels run a thread per 8 elements or more.
-constexpr int64_t kMaxVectors = (1LL << 31) * 64;
-
 }  // namespace
 
 extern "C" {
@@ -878,9 +875,9 @@ int fp8attn_silu_mul_quant(const void* gate_up, int64_t row_stride, void* q, voi
                            int I, int dtype, void* stream) {
   int rc = check_dtype(dtype);
   if (rc) return rc;
-  if (M < 0 || I <= 0 || I % 128 != 0 || I > INT32_MAX / 4 || M > kMaxVectors / (I / 8))
-    return fail(FP8ATTN_EINVAL, "silu quant needs M >= 0, I a positive multiple of 128 and M * I < "
-                "2^40 (got M=%lld I=%d)", static_cast<long long>(M), I);
+  if (M < 0 || M > INT32_MAX || I <= 0 || I % 128 != 0 || I > fp8attn::kSiluMaxColumns)
+    return fail(FP8ATTN_EINVAL, "silu quant needs 0 <= M < 2^31 and I a multiple of 128 up to %d (got "
+                "M=%lld I=%d)", fp8attn::kSiluMaxColumns, static_cast<long long>(M), I);
   if (M == 0) return FP8ATTN_OK;
   rc = check_rows16("silu quant: gate_up", gate_up, row_stride, 2LL * I);
   if (rc) return rc;

@@ -222,6 +222,12 @@ __device__ __forceinline__ uint64_t f2_sub(uint64_t a, uint64_t b) {
   return d;
 }
 
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // 2^x for two values on the FMA pipe instead of the MUFU unit (whose ex2 rate bounds the
 // attention softmax): relative error < 1e-4 for x >= -125 (smaller x gives ~2^-125).  x = n + f
 // with n = round(x) from the 1.5 * 2^23 shifter (round to nearest), 2^f on [-0.5, 0.5] by a
@@ -244,6 +250,13 @@ __device__ __forceinline__ void exp2_poly_x2(float x0, float x1, float& r0, floa
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 1 / x; 0 for |x| above 2^126.
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 

@@ -18,35 +18,44 @@ namespace {
 
 constexpr int kGroup = 128;
 
-__device__ __forceinline__ float load_elem(uint32_t bits16, __nv_bfloat16) {
-  return __uint_as_float(bits16 << 16);
-}
-__device__ __forceinline__ float load_elem(uint32_t bits16, __half) {
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
-}
-__device__ __forceinline__ uint32_t store_elem(float x, __nv_bfloat16) {
-  return __bfloat16_as_ushort(__float2bfloat16_rn(x));
-}
-__device__ __forceinline__ uint32_t store_elem(float x, __half) {
-  return __half_as_ushort(__float2half_rn(x));
-}
+// 8 values as four fp32 pairs: the kernels are bound by instruction issue before HBM, and one packed
+// operation serves two values.
+struct Eight {
+  uint64_t p[4];
+};
 
-template <typename T>
-__device__ __forceinline__ void widen8(const uint4& raw, float (&x)[8]) {
+__device__ __forceinline__ Eight widen8(const uint4& raw, __nv_bfloat16) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = load_elem(w[i] & 0xFFFFu, T());
-    x[2 * i + 1] = load_elem(w[i] >> 16, T());
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ uint4 narrow8(const float (&x)[8]) {
-  uint32_t w[4];
+  Eight e;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    w[i] = store_elem(x[2 * i], T()) | (store_elem(x[2 * i + 1], T()) << 16);
+    e.p[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+  return e;
+}
+__device__ __forceinline__ Eight widen8(const uint4& raw, __half) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  Eight e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    e.p[i] = f2_pack(f.x, f.y);
+  }
+  return e;
+}
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi, __half) { return pack_f16x2(lo, hi); }
+template <typename T>
+__device__ __forceinline__ uint4 narrow8(const Eight& e) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    f2_unpack(e.p[i], lo, hi);
+    w[i] = narrow2(lo, hi, T());
+  }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -62,24 +71,29 @@ __device__ __forceinline__ uint4 load_once(const void* p) {
 
 // This lane's 8 of a group's 128 values, the group being the 16 lanes of its half-warp: the e4m3
 // bytes, and the group's scale.  The lanes of `mask` call together.
-__device__ __forceinline__ uint2 quantise8(const float (&y)[8], float& scale, unsigned mask) {
-  float a = 0.f;
+__device__ __forceinline__ uint2 quantise8(const Eight& y, float& scale, unsigned mask) {
+  float v[8], a = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(y[i]));  // fmaxf leaves NaN out
+  for (int i = 0; i < 4; ++i) {
+    f2_unpack(y.p[i], v[2 * i], v[2 * i + 1]);
+    a = fmaxf(a, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));  // fmaxf leaves NaN out
+  }
 #pragma unroll
   for (int off = 8; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, off));
-  scale = __fdiv_rn(a, 448.0f);
-  if (!(scale > 0.f)) scale = 1.0f;
-  // y / d as y times 1 / d, an ulp from the quotient (31 instead of 60 instructions an element in the
-  // SiLU kernel), but for scales whose inverse overflows
-  float v[8];
-  if (scale > 1.0e-37f) {
-    const float inv = __frcp_rn(scale);
+  if (a > 1.0e-30f && a < INFINITY) {
+    // a / 448 rounded to nearest: a product with the rounded 1 / 448 and one correction by the exact
+    // remainder (Markstein); y / d as y times 1 / d, two ulps from the quotient at most
+    const float k = 1.0f / 448.0f, q = a * k;
+    scale = fmaf(fmaf(-448.0f, q, a), k, q);
+    const float inv = rcp(scale);
+    const uint64_t inv2 = f2_pack(inv, inv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = y[i] * inv;
-  } else {
+    for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(y.p[i], inv2), v[2 * i], v[2 * i + 1]);
+  } else {  // where remainders and inverses leave fp32's range, and infinity
+    scale = __fdiv_rn(a, 448.0f);
+    if (!(scale > 0.f)) scale = 1.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(y[i], scale);
+    for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(v[i], scale);
   }
   uint32_t b[4];
 #pragma unroll
@@ -117,19 +131,22 @@ __global__ void __launch_bounds__(kTpr* kRows) add_rms_norm_quant_kernel(const N
     if (ok && p.residual != nullptr) rr[j] = load_once(p.residual + row * p.residual_row_stride + 8 * v);
     if (ok) wr[j] = __ldg(reinterpret_cast<const uint4*>(p.weight) + v);
   }
-  float s[kVec][8], ss = 0.f;
+  Eight s[kVec];
+  uint64_t sq = f2_pack(0.f, 0.f);
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
-    widen8<T>(xr[j], s[j]);
+    s[j] = widen8(xr[j], T());
     if (p.residual != nullptr) {
-      float q[8];
-      widen8<T>(rr[j], q);
+      const Eight q = widen8(rr[j], T());
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[j][i] += q[i];
+      for (int i = 0; i < 4; ++i) s[j].p[i] = f2_add(s[j].p[i], q.p[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(s[j][i], s[j][i], ss);
+    for (int i = 0; i < 4; ++i) sq = f2_fma(s[j].p[i], s[j].p[i], sq);
   }
+  float ss, ss_hi;
+  f2_unpack(sq, ss, ss_hi);
+  ss += ss_hi;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
   if (kWarps > 1) {
@@ -148,10 +165,10 @@ __global__ void __launch_bounds__(kTpr* kRows) add_rms_norm_quant_kernel(const N
     if (!ok) continue;
     if (p.residual_out != nullptr)
       *reinterpret_cast<uint4*>(p.residual_out + row * p.K + 8 * v) = narrow8<T>(s[j]);
-    float w[8], y[8];
-    widen8<T>(wr[j], w);
+    const Eight w = widen8(wr[j], T());
+    Eight y;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = s[j][i] * rms * w[i];
+    for (int i = 0; i < 4; ++i) y.p[i] = f2_mul(f2_mul(s[j].p[i], f2_pack(rms, rms)), w.p[i]);
     if (p.norm_out != nullptr)
       *reinterpret_cast<uint4*>(p.norm_out + row * p.K + 8 * v) = narrow8<T>(y);
     float scale;
@@ -162,51 +179,91 @@ __global__ void __launch_bounds__(kTpr* kRows) add_rms_norm_quant_kernel(const N
 }
 
 // ------------------------------------------------------------------ SiLU * up + quantise
-constexpr int kSiluThreads = 256;
-
-template <typename T>
-__global__ void __launch_bounds__(kSiluThreads) silu_mul_quant_kernel(const SiluQuantParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int vecs = p.I / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kSiluThreads + threadIdx.x;
-  const bool ok = i < p.M * vecs;  // the 16 lanes of a group agree: vecs is a multiple of 16
-  const unsigned mask = __ballot_sync(0xffffffffu, ok);
-  if (!ok) return;
-  const int64_t row = i / vecs;
-  const int v = static_cast<int>(i - row * vecs);
-  const uint16_t* src = p.gate_up + row * p.row_stride + 8 * v;
-  const uint4 gr = load_once(src), ur = load_once(src + p.I);
-  float g[8], u[8];
-  widen8<T>(gr, g);
-  widen8<T>(ur, u);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) g[k] = __fdividef(g[k], 1.0f + expf(-g[k])) * u[k];
-  float scale;
-  const uint2 q = quantise8(g, scale, mask);
-  *reinterpret_cast<uint2*>(p.q + row * p.I + 8 * v) = q;
-  if ((v & 15) == 0) p.scale[row * (p.I / kGroup) + v / 16] = bf16_bits(scale);
+// g / (1 + e^-g) of two values.  e^-g = 2^(-g log2 e): the product's rounding error, which the power
+// would multiply by |g|, is recovered by a fused multiply-add (error-free product) and applied to first
+// order, 2^(t + d) = 2^t (1 + d ln 2).  g is held below 200, where e^-g is 0, so that the product does not
+// overflow; where it overflows below, 1 + e^-g is infinite either way.
+__device__ __forceinline__ uint64_t silu2(uint64_t g) {
+  const float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+  // log2 e - float(log2 e)
+  const float kLog2eRest = static_cast<float>(1.44269504088896340736 - 1.44269502162933349609375);
+  float g0, g1;
+  f2_unpack(g, g0, g1);
+  const uint64_t c = f2_pack(fminf(g0, 200.f), fminf(g1, 200.f));
+  const uint64_t minus = f2_pack(-kLog2e, -kLog2e);
+  const uint64_t t = f2_mul(c, minus);
+  float t0, t1;
+  f2_unpack(t, t0, t1);
+  const uint64_t exact = f2_fma(c, minus, f2_pack(-t0, -t1));
+  const uint64_t d = f2_fma(c, f2_pack(-kLog2eRest, -kLog2eRest), exact);
+  const uint64_t e = f2_mul(f2_pack(ex2(t0), ex2(t1)), f2_fma(d, f2_pack(kLn2, kLn2), f2_pack(1.f, 1.f)));
+  float q0, q1;
+  f2_unpack(f2_add(e, f2_pack(1.f, 1.f)), q0, q1);
+  return f2_mul(g, f2_pack(rcp(q0), rcp(q1)));
 }
 
-template <typename Kernel, typename Params>
-cudaError_t launch_dependent(Kernel kernel, int64_t blocks, int threads, const Params& p,
-                             cudaStream_t stream) {
+constexpr int kSiluThreads = 256;
+
+// A CTA (x, y) takes 512 vectors of a row from 512 y on, or, of short rows, several rows: 2^tpr_log2 threads
+// a row, two vectors each (one vector a thread issued 25 instructions a value, a third of them indexing).
+constexpr int kSiluVec = 2;
+
+template <typename T>
+__global__ void __launch_bounds__(kSiluThreads)
+    silu_mul_quant_kernel(const SiluQuantParams p, int tpr_log2) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tpr = 1 << tpr_log2, vecs = p.I / 8;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) << (8 - tpr_log2)) + (threadIdx.x >> tpr_log2);
+  const int v0 = blockIdx.y * (kSiluThreads * kSiluVec) + (threadIdx.x & (tpr - 1));
+  const uint16_t* src = p.gate_up + row * p.row_stride + 8 * v0;
+  uint4 gr[kSiluVec], ur[kSiluVec];
+#pragma unroll
+  for (int j = 0; j < kSiluVec; ++j) {
+    const bool ok = row < p.M && v0 + j * tpr < vecs;
+    gr[j] = ur[j] = make_uint4(0, 0, 0, 0);
+    if (ok) {
+      gr[j] = load_once(src + 8 * j * tpr);
+      ur[j] = load_once(src + 8 * j * tpr + p.I);
+    }
+  }
+  uint8_t* const q = p.q + row * p.I;
+  uint16_t* const scales = p.scale + row * (p.I / kGroup);
+#pragma unroll
+  for (int j = 0; j < kSiluVec; ++j) {
+    const int v = v0 + j * tpr;
+    const bool ok = row < p.M && v < vecs;  // the 16 lanes of a group agree: vecs is a multiple of 16
+    const unsigned mask = __ballot_sync(0xffffffffu, ok);
+    if (!ok) continue;
+    Eight h = widen8(gr[j], T());
+    const Eight u = widen8(ur[j], T());
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h.p[i] = f2_mul(silu2(h.p[i]), u.p[i]);
+    float scale;
+    *reinterpret_cast<uint2*>(q + 8 * v) = quantise8(h, scale, mask);
+    if ((v & 15) == 0) scales[v / 16] = bf16_bits(scale);
+  }
+}
+
+template <typename Kernel, typename... Args>
+cudaError_t launch_dependent(Kernel kernel, dim3 blocks, int threads, cudaStream_t stream,
+                             const Args&... args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.gridDim = blocks;
   cfg.blockDim = dim3(threads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename T, int kTpr, int kVec, int kRows>
 cudaError_t launch_norm(const NormQuantParams& p, cudaStream_t stream) {
-  return launch_dependent(add_rms_norm_quant_kernel<T, kTpr, kVec, kRows>, (p.M + kRows - 1) / kRows,
-                          kTpr * kRows, p, stream);
+  return launch_dependent(add_rms_norm_quant_kernel<T, kTpr, kVec, kRows>,
+                          dim3(static_cast<unsigned>((p.M + kRows - 1) / kRows)), kTpr * kRows, stream, p);
 }
 
 template <typename T>
@@ -228,10 +285,15 @@ cudaError_t launch_add_rms_norm_quant(const NormQuantParams& p, cudaStream_t str
 
 cudaError_t launch_silu_mul_quant(const SiluQuantParams& p, cudaStream_t stream) {
   if (p.M == 0) return cudaSuccess;
-  const int64_t blocks = (p.M * (p.I / 8) + kSiluThreads - 1) / kSiluThreads;
-  return p.fp16 ? launch_dependent(silu_mul_quant_kernel<__half>, blocks, kSiluThreads, p, stream)
-                : launch_dependent(silu_mul_quant_kernel<__nv_bfloat16>, blocks, kSiluThreads, p,
-                                   stream);
+  const int vecs = p.I / 8;
+  int tpr_log2 = 4;
+  while (tpr_log2 < 8 && kSiluVec << tpr_log2 < vecs) ++tpr_log2;
+  const int64_t rows = kSiluThreads >> tpr_log2;
+  const dim3 grid(static_cast<unsigned>((p.M + rows - 1) / rows),
+                  (vecs + kSiluThreads * kSiluVec - 1) / (kSiluThreads * kSiluVec));
+  return p.fp16 ? launch_dependent(silu_mul_quant_kernel<__half>, grid, kSiluThreads, stream, p, tpr_log2)
+                : launch_dependent(silu_mul_quant_kernel<__nv_bfloat16>, grid, kSiluThreads, stream, p,
+                                   tpr_log2);
 }
 
 }  // namespace fp8attn

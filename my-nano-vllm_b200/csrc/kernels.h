@@ -139,6 +139,7 @@ struct SiluQuantParams {
   int I;
   int fp16;
 };
+constexpr int kSiluMaxColumns = 1 << 20;
 cudaError_t launch_silu_mul_quant(const SiluQuantParams& p, cudaStream_t stream);
 
 // ------------------------------------------------------------------ mixture of experts
