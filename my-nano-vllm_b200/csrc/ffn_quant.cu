@@ -107,24 +107,24 @@ __device__ __forceinline__ uint16_t bf16_bits(float x) {
 }
 
 // ------------------------------------------------------------------ add + RMS norm + quantise
-// kTpr threads per row (a power of two from 32), kVec vectors of 8 per thread: vector j of thread t
-// is columns 8 (t + j kTpr).  kRows rows per CTA.
-template <typename T, int kTpr, int kVec, int kRows>
-__global__ void __launch_bounds__(kTpr* kRows) add_rms_norm_quant_kernel(const NormQuantParams p) {
-  static_assert(kTpr % 32 == 0, "groups of 16 lanes must not straddle rows");
-  constexpr int kWarps = kTpr / 32;
-  __shared__ float part[kRows][kWarps];
+// CTA: blockDim.y rows of blockDim.x threads (whole warps), kVec vectors of 8 per thread: vector j of
+// thread t is columns 8 (t + j blockDim.x).
+constexpr int kNormMaxWarps = 16;
+
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kNormMaxWarps * 32) add_rms_norm_quant_kernel(const NormQuantParams p) {
+  __shared__ float part[kNormMaxWarps];  // a row's warps side by side
   // launched as a programmatic dependent of the previous kernel: nothing is read before it ends
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int t = threadIdx.x % kTpr, r = threadIdx.x / kTpr;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + r;
+  const int t = threadIdx.x, tpr = blockDim.x, warps = tpr / 32;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const bool row_ok = row < p.M;  // whole warps; every thread reaches the barrier
   const int vecs = p.K / 8;
   uint4 xr[kVec], rr[kVec], wr[kVec];
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
-    const int v = t + j * kTpr;
+    const int v = t + j * tpr;
     const bool ok = row_ok && v < vecs;
     xr[j] = rr[j] = wr[j] = make_uint4(0, 0, 0, 0);
     if (ok) xr[j] = load_once(p.x + row * p.x_row_stride + 8 * v);
@@ -149,17 +149,17 @@ __global__ void __launch_bounds__(kTpr* kRows) add_rms_norm_quant_kernel(const N
   ss += ss_hi;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-  if (kWarps > 1) {
-    if ((t & 31) == 0) part[r][t / 32] = ss;
+  if (warps > 1) {
+    float* const mine = part + threadIdx.y * warps;
+    if ((t & 31) == 0) mine[t / 32] = ss;
     __syncthreads();
     ss = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) ss += part[r][w];
+    for (int w = 0; w < warps; ++w) ss += mine[w];
   }
   const float rms = rsqrtf(ss / static_cast<float>(p.K) + p.eps);
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
-    const int v = t + j * kTpr;
+    const int v = t + j * tpr;
     const bool ok = row_ok && v < vecs;  // the 16 lanes of a group agree: vecs is a multiple of 16
     const unsigned mask = __ballot_sync(0xffffffffu, ok);
     if (!ok) continue;
@@ -246,34 +246,38 @@ __global__ void __launch_bounds__(kSiluThreads)
 }
 
 template <typename Kernel, typename... Args>
-cudaError_t launch_dependent(Kernel kernel, dim3 blocks, int threads, cudaStream_t stream,
+cudaError_t launch_dependent(Kernel kernel, dim3 blocks, dim3 threads, cudaStream_t stream,
                              const Args&... args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = blocks;
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = threads;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <typename T, int kTpr, int kVec, int kRows>
+template <typename T, int kVec>
 cudaError_t launch_norm(const NormQuantParams& p, cudaStream_t stream) {
-  return launch_dependent(add_rms_norm_quant_kernel<T, kTpr, kVec, kRows>,
-                          dim3(static_cast<unsigned>((p.M + kRows - 1) / kRows)), kTpr * kRows, stream, p);
+  const int tpr = (p.K / 8 + 32 * kVec - 1) / (32 * kVec) * 32;
+  const int rows = tpr >= 128 ? 1 : 128 / tpr;
+  return launch_dependent(add_rms_norm_quant_kernel<T, kVec>,
+                          dim3(static_cast<unsigned>((p.M + rows - 1) / rows)), dim3(tpr, rows), stream, p);
 }
 
 template <typename T>
 cudaError_t launch_norm_for(const NormQuantParams& p, cudaStream_t stream) {
-  const int vecs = p.K / 8;
-  if (vecs <= 64) return launch_norm<T, 32, 2, 4>(p, stream);
-  if (vecs <= 256) return launch_norm<T, 128, 2, 2>(p, stream);
-  if (vecs <= 512) return launch_norm<T, 256, 2, 1>(p, stream);
-  if (vecs <= 1024) return launch_norm<T, 512, 2, 1>(p, stream);
-  return launch_norm<T, 512, 4, 1>(p, stream);
+  // Few rows: a row over as many threads as there are, for its latency (1 row of 4096: 1.75 us with one
+  // vector a thread, 1.92 with two, 2.56 with four; 256 of 8192: 4.3, two, and 5.1, four).  Many: more work
+  // a thread, but rows of 320 threads or fewer (8192 of 4096: 46.4, 39.6 and 40.3 us; of 8192: 93.1, two,
+  // and 80.4, four).  512 rows is where they meet.
+  const bool few = p.M <= 512;
+  if (few && p.K <= 4096) return launch_norm<T, 1>(p, stream);
+  if (p.K <= (few ? 8192 : 5120)) return launch_norm<T, 2>(p, stream);
+  return launch_norm<T, 4>(p, stream);
 }
 
 }  // namespace
