@@ -260,6 +260,30 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
+// The scale of a quantised group, a / 448 for its largest magnitude a (1 for an all-zero group), and the
+// group's values divided by it.
+template <int N>
+__device__ __forceinline__ float divide_by_scale(float (&v)[N], float a) {
+  if (a > 1.0e-30f && a < INFINITY) {
+    // a / 448 rounded to nearest: a product with the rounded 1 / 448 and one correction by the exact
+    // remainder (Markstein); v / scale as v times 1 / scale, two ulps from the quotient at most
+    const float k = 1.0f / 448.0f, q = a * k;
+    const float scale = fmaf(fmaf(-448.0f, q, a), k, q);
+    const float inv = rcp(scale);
+    static_assert(N % 2 == 0, "pairs");
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      f2_unpack(f2_mul(f2_pack(v[i], v[i + 1]), f2_pack(inv, inv)), v[i], v[i + 1]);
+    return scale;
+  }
+  // where remainders and inverses leave fp32's range, and infinity
+  float scale = __fdiv_rn(a, 448.0f);
+  if (!(scale > 0.f)) scale = 1.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __fdiv_rn(v[i], scale);
+  return scale;
+}
+
 // fp32 -> fp16 -> bf16, the reference output path (.to(tl.float16) stored into bf16).
 __device__ __forceinline__ __nv_bfloat16 out_round(float x) {
   return __float2bfloat16_rn(__half2float(__float2half_rn(x)));

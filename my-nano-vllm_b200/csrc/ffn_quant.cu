@@ -80,21 +80,7 @@ __device__ __forceinline__ uint2 quantise8(const Eight& y, float& scale, unsigne
   }
 #pragma unroll
   for (int off = 8; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, off));
-  if (a > 1.0e-30f && a < INFINITY) {
-    // a / 448 rounded to nearest: a product with the rounded 1 / 448 and one correction by the exact
-    // remainder (Markstein); y / d as y times 1 / d, two ulps from the quotient at most
-    const float k = 1.0f / 448.0f, q = a * k;
-    scale = fmaf(fmaf(-448.0f, q, a), k, q);
-    const float inv = rcp(scale);
-    const uint64_t inv2 = f2_pack(inv, inv);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(y.p[i], inv2), v[2 * i], v[2 * i + 1]);
-  } else {  // where remainders and inverses leave fp32's range, and infinity
-    scale = __fdiv_rn(a, 448.0f);
-    if (!(scale > 0.f)) scale = 1.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(v[i], scale);
-  }
+  scale = divide_by_scale(v, a);
   uint32_t b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)  // saturating: a quotient may round to just above 448

@@ -42,6 +42,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+// mbar_wait with its polling loop out of line: the roles' loops stay small (1 % of the layer's time).
+__device__ __noinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, int* err) {
+  return mbar_wait(bar, parity, err);
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* err) {
+  return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, err);
+}
+
 constexpr int kBlk = 128;
 
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
@@ -203,16 +211,20 @@ constexpr int kDBufs = 4;
 // counters: the next ticket, finished ranges of phase 1, finished items of each tile (phase 0), arrived
 // parts of the item that each range leaves unfinished (by phase)
 constexpr int kDoneAt = 1, kReadyAt = 2;
-// Tokens per tile: 16 where an expert has 8 tokens or fewer on average (its tiles past the first read
-// the weights again, from L2), which leaves the ring more room for weights; else 32.
-constexpr int kFewTokens = 8;
-constexpr int kMaxTiles = 768;  // at most the experts and the full tiles
+// Tokens per tile: 16 where an expert has 12 tokens or fewer on average (its tiles past the first read
+// the weights again, from L2), which leaves the ring more room for weights and the promotion threads
+// less to do; else 32.  64 experts of 4096 x 1408, 9 tokens each: 187 us with 16, 195 with 32; 12
+// each: the same; 60 experts of 1152 x 640, 25 each: 59 us with 32.
+constexpr int kFewTokens = 12;
+constexpr int kMaxTiles = 896;  // at most the experts and the full tiles
 static_assert(kMoeMaxExperts + kMoeMaxSlots / 32 <= kMaxTiles &&
                   kMoeMaxExperts + kFewTokens * kMoeMaxExperts / 16 <= kMaxTiles, "tiles");
 int tile_tokens(int64_t T, int E, int top_k) { return T <= 16 || T * top_k <= kFewTokens * E ? 16 : 32; }
 
-// A phase's units, items in order, are cut into equal ranges, one per CTA.  (Handing an eighth of the work
-// out in smaller ranges, for SMs that get less bandwidth, cost 5 to 30 %: more items are cut.)
+// A phase's units, items in order, are cut into equal ranges, one per CTA.  (Cutting each of few items
+// into equal parts, one a range, was no faster; handing an eighth of the work out in smaller ranges,
+// for SMs that get less bandwidth, was 5 to 30 % slower, since more items are cut; dealing whole
+// items out in turn and cutting the rest alone was 10 % slower, since the CTAs then pause in step.)
 struct Phase {
   int blocks;  // items per tile (output columns / 128)
   int steps;   // units per item
@@ -224,8 +236,8 @@ struct Phase {
 constexpr int kMaxGrid = 256;
 static_assert(static_cast<uint64_t>(kMaxTiles) * 128 * 128 * (kMaxGrid + 1) < 1ull << 32, "32-bit cuts");
 __device__ __forceinline__ int range_begin(const Phase& f, int r) {
-  return static_cast<int>(f.whole ? static_cast<uint32_t>(f.items) * r / f.ranges * f.steps
-                                  : static_cast<uint32_t>(f.units) * r / f.ranges);
+  if (f.whole) return static_cast<int>(static_cast<uint32_t>(f.items) * r / f.ranges * f.steps);
+  return static_cast<int>(static_cast<uint32_t>(f.units) * r / f.ranges);
 }
 // The range that holds unit x (not whole): the largest r with range_begin(r) <= x.
 __device__ __forceinline__ int range_of(const Phase& f, int x) {
@@ -344,6 +356,7 @@ __device__ __forceinline__ bool wait_counter(const int* p, int want, int* err) {
 // cuts; every CTA does the same.  Scratch in the ring, which is not in use yet.
 struct PlanScratch {
   uint16_t expert[kMoeMaxSlots];
+  uint16_t rank[kMoeMaxSlots];             // a slot's place among its warp's slots of the expert
   uint16_t count[kWarps][kMoeMaxExperts];  // a warp's slots of an expert; zero when plan begins
   uint32_t warp_total[kMoeMaxExperts / 64];
 };
@@ -355,8 +368,8 @@ __device__ __forceinline__ PlanScratch& plan_scratch(MoeSmem<NT>& sm) {
 
 __device__ __forceinline__ Phase make_phase(const MoeParams& p, int which, int tiles, int grid) {
   Phase f;
-  if (which == 2) {  // 256 columns of a token
-    f.blocks = (p.H + 255) / 256;
+  if (which == 2) {  // 128 columns of a token
+    f.blocks = p.H / kBlk;
     f.steps = 1;
     f.items = static_cast<int>(p.T) * f.blocks;
   } else {
@@ -395,10 +408,12 @@ __device__ __forceinline__ Claim make_claim(const MoeSmem<NT>& sm, int ticket) {
   return c;
 }
 
-// The lanes that have the same e (of `bits` bits) as this one, among those that are ok.
-__device__ __forceinline__ unsigned same_expert(int e, bool ok, int bits) {
+// The lanes that have the same e as this one, among those that are ok.
+__device__ __forceinline__ unsigned same_expert(int e, bool ok) {
+  static_assert(kMoeMaxExperts == 512, "nine bits");
   unsigned same = __ballot_sync(0xffffffffu, ok);
-  for (int b = 0; b < bits; ++b) {
+#pragma unroll
+  for (int b = 0; b < 9; ++b) {
     const bool one = (e >> b) & 1;
     const unsigned v = __ballot_sync(0xffffffffu, one);
     same &= one ? v : ~v;
@@ -409,7 +424,7 @@ __device__ __forceinline__ unsigned same_expert(int e, bool ok, int bits) {
 template <int NT>
 __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p, int ticket) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int n = static_cast<int>(p.T) * p.top_k, bits = 32 - __clz(p.E - 1);
+  const int n = static_cast<int>(p.T) * p.top_k;
   PlanScratch& s = plan_scratch(sm);
   const int per = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;  // a warp's slots: [warp per, + per)
   const int lo = min(warp * per, n), hi = min(lo + per, n);
@@ -421,8 +436,13 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p, int ticket) {
     const int i = i0 + lane;
     const bool ok = i < hi;
     const int e = ok ? s.expert[i] : 0;
-    const unsigned same = same_expert(e, ok, bits);
-    if (ok && lane == __ffs(same) - 1) s.count[warp][e] += static_cast<uint16_t>(__popc(same));
+    const unsigned same = same_expert(e, ok);
+    const int base = s.count[warp][e];
+    __syncwarp();
+    if (ok) {
+      s.rank[i] = static_cast<uint16_t>(base + __popc(same & ((1u << lane) - 1)));
+      if (lane == __ffs(same) - 1) s.count[warp][e] = static_cast<uint16_t>(base + __popc(same));
+    }
     __syncwarp();
   }
   __syncthreads();
@@ -430,6 +450,7 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p, int ticket) {
   const bool mine = tid < kMoeMaxExperts / 2;
   uint32_t sum = 0, before = 0;  // (slots << 16) + tiles of the experts before
   if (mine) {
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {  // a warp's counts -> where its slots of the expert begin
       uint32_t* c = reinterpret_cast<uint32_t*>(s.count[w]) + tid;
       const uint32_t v = *c;
@@ -466,17 +487,9 @@ __device__ void plan(MoeSmem<NT>& sm, const MoeParams& p, int ticket) {
   }
   __syncthreads();
   if (warp == kProducerWarp && lane == 0) sm.claim[0] = make_claim(sm, ticket);
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane;
-    const bool ok = i < hi;
-    const int e = ok ? s.expert[i] : 0;
-    const unsigned same = same_expert(e, ok, bits);
-    if (ok)
-      sm.order[sm.first[e] + s.count[warp][e] + __popc(same & ((1u << lane) - 1))] =
-          static_cast<uint16_t>(i);
-    __syncwarp();
-    if (ok && lane == __ffs(same) - 1) s.count[warp][e] += static_cast<uint16_t>(__popc(same));
-    __syncwarp();
+  for (int i = tid; i < n; i += kThreads) {
+    const int e = s.expert[i];
+    sm.order[sm.first[e] + s.count[i / per][e] + s.rank[i]] = static_cast<uint16_t>(i);
   }
   // the ring's next writer is the async proxy
   fence_proxy_async_smem();
@@ -528,7 +541,7 @@ struct Tile {
 // The next range, for every warp but the producer.  False: no more.
 template <int NT>
 __device__ __forceinline__ bool next_claim(MoeSmem<NT>& sm, int i, int lane, int* err, Claim& claim) {
-  if (!mbar_wait(&sm.claim_full[i & 1], (i >> 1) & 1, err)) return false;
+  if (!wait_for(&sm.claim_full[i & 1], (i >> 1) & 1, err)) return false;
   claim = sm.claim[i & 1];
   __syncwarp();
   if (lane == 0) mbar_arrive(&sm.claim_empty[i & 1]);
@@ -546,7 +559,7 @@ __device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* 
     Claim claim = sm.claim[0];  // the first one was made with the plan
     if (i > 0) {
       claim = make_claim(sm, ticket);
-      ok = ok && mbar_wait(&sm.claim_empty[i & 1], ((i >> 1) & 1) ^ 1, p.err);
+      ok = ok && wait_for(&sm.claim_empty[i & 1], ((i >> 1) & 1) ^ 1, p.err);
       if (!ok) claim.phase = -1;
       sm.claim[i & 1] = claim;
     }
@@ -565,7 +578,7 @@ __device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* 
       if (u == claim.begin + (claim.end - claim.begin) / 2) ticket = atomicAdd(p.counters, 1);
       const int stage = r % kStages;
       const int expert = static_cast<int>(sm.tile[c.tile] >> 16);
-      if (!mbar_wait(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err)) {
+      if (!wait_for(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err)) {
         ok = false;
         break;
       }
@@ -672,7 +685,7 @@ struct Gather {
     }
     if (ok && !mbar_test(&sm.empty[stage], ((r / kStages) & 1) ^ 1)) {
       finish(other, false);
-      ok = mbar_wait(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err);
+      ok = wait_for(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err);
     }
     if (ok) {  // else: the others stop by themselves, their waits on this stage are bounded
       issue(mine, stage);
@@ -761,9 +774,9 @@ __device__ void multiply(MoeSmem<NT>& sm, const MoeParams& p, int which, int lan
           tile = c.tile;
           idesc = tc::idesc_e4m3(kBlk, Tile<NT>(sm, tile).columns(), false, false);
         }
-        ok = mbar_wait(&sm.w_full[stage], (r / kStages) & 1, p.err) &&
-             mbar_wait(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
-             mbar_wait(&sm.d_empty[buf], ((r / kDBufs) & 1) ^ 1, p.err);
+        ok = wait_for(&sm.w_full[stage], (r / kStages) & 1, p.err) &&
+             wait_for(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
+             wait_for(&sm.d_empty[buf], ((r / kDBufs) & 1) ^ 1, p.err);
         if (!ok) break;
         tc::fence_after_sync();
         if (which == 0 || ph == 0 || (2 * c.k + 1) * kBlk < p.I) {
@@ -829,11 +842,9 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
     if (ph == 2) {
       // ---- weighted sums, once phase 1 has ended: its ranges are held by CTAs that run
       ok = ok && wait_counter(p.counters + kDoneAt, sm.phase[1].ranges, p.err);
-      for (int item = begin + warp / 2; item < end && ok; item += kPromoWarps / 2) {
-        // two warps an item, four columns a thread
+      for (int item = begin + warp; item < end && ok; item += kPromoWarps) {
         const int64_t token = item / f.blocks;
-        const int at = (item - static_cast<int>(token) * f.blocks) * 256 + (tid & 63) * 4;
-        if (at >= p.H) continue;
+        const int at = (item - static_cast<int>(token) * f.blocks) * kBlk + lane * 4;
         const float* y = p.y + token * p.top_k * p.H + at;
         const float* w = p.weights + token * p.top_k;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -884,8 +895,8 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
         const int stage = r % kStages, buf = r % kDBufs;
         // whoever begins an item usually comes last to it: are the other parts there already?
         if (u == stop - 1 && cut && !at_head && tid == 0) others = load_acquire(arrived);
-        ok = ok && mbar_wait(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
-             mbar_wait(&sm.d_full[buf], (r / kDBufs) & 1, p.err);
+        ok = ok && wait_for(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
+             wait_for(&sm.d_full[buf], (r / kDBufs) & 1, p.err);
         if (!ok) continue;
         tc::fence_after_sync();
         const uint32_t d = tmem + buf * 2 * NT + m0;
@@ -930,6 +941,7 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
         if (!sm.last) continue;
       }
       // a warp takes tokens warp, warp + 8, ...; lane: 4 of the 128 columns
+#pragma unroll 1  // one at a time: unrolled by two, the larger code cost 2 to 7 %
       for (int m = warp; m < t.count; m += kPromoWarps) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
         if (here) {
@@ -958,19 +970,17 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
         const int64_t slot = sm.order[t.begin + m];
         if (ph == 1) {
           __stcg(reinterpret_cast<float4*>(p.y + slot * p.H + blk * kBlk + 4 * lane), a);
-          continue;
+        } else {
+          // h = silu(gate) up, quantised over the item's 128 columns
+          float h[4] = {silu(a.x) * b.x, silu(a.y) * b.y, silu(a.z) * b.z, silu(a.w) * b.w};
+          const float most = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])),
+                                   fmaxf(fmaxf(fabsf(h[2]), fabsf(h[3])), 0.f));  // NaN left out
+          const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+          const float scale = divide_by_scale(h, top);
+          *reinterpret_cast<uint32_t*>(p.hq + slot * p.I + blk * kBlk + 4 * lane) =
+              f32x2_to_e4m3x2(h[0], h[1]) | (f32x2_to_e4m3x2(h[2], h[3]) << 16);
+          if (lane == 0) p.h_scale[slot * kc2 + blk] = f32_to_bf16(scale);
         }
-        // h = silu(gate) up, quantised over the item's 128 columns
-        float h[4] = {silu(a.x) * b.x, silu(a.y) * b.y, silu(a.z) * b.z, silu(a.w) * b.w};
-        const float most = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])),
-                                 fmaxf(fmaxf(fabsf(h[2]), fabsf(h[3])), 0.f));  // NaN left out
-        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-        float scale = __fdiv_rn(top, 448.0f);
-        if (!(scale > 0.f)) scale = 1.0f;
-        const uint32_t lo = f32x2_to_e4m3x2(__fdiv_rn(h[0], scale), __fdiv_rn(h[1], scale));
-        const uint32_t hi = f32x2_to_e4m3x2(__fdiv_rn(h[2], scale), __fdiv_rn(h[3], scale));
-        *reinterpret_cast<uint32_t*>(p.hq + slot * p.I + blk * kBlk + 4 * lane) = lo | (hi << 16);
-        if (lane == 0) p.h_scale[slot * kc2 + blk] = f32_to_bf16(scale);
       }
       promo_sync();  // what was written is complete; the shared item is free again
       if (ph == 0 && tid == 0) add_release(ready + tile);
