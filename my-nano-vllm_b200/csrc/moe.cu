@@ -50,6 +50,11 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* er
   return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, err);
 }
 
+// The same for a whole warp, whose lanes go on together also when a wait has given up.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, wait_for(bar, parity, err));
+}
+
 constexpr int kBlk = 128;
 
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
@@ -278,6 +283,19 @@ constexpr size_t moe_smem_bytes() {
 static_assert(moe_smem_bytes<16>() <= 227 * 1024 && moe_smem_bytes<32>() <= 227 * 1024, "smem");
 
 __device__ __forceinline__ void promo_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// The same, and whether every thread said yes.
+__device__ __forceinline__ bool promo_all(bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(yes))
+      : "memory");
+  return all != 0;
+}
 
 __device__ __forceinline__ int load_acquire(const int* p) {
   int v;
@@ -335,13 +353,17 @@ __device__ __forceinline__ void tma_load_once(void* dst, const CUtensorMap* map,
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
       : "memory");
 }
-// Wait until *p >= want; gives up after kWaitLimitNs, recording kDevErrWaitTimeout.
-__device__ __forceinline__ bool wait_counter(const int* p, int want, int* err) {
+// A warp's wait until *p >= want; gives up after kWaitLimitNs, recording kDevErrWaitTimeout.  Lane 0
+// decides for all.
+__device__ __forceinline__ bool counter_reached(const int* p, int want) {
+  return __shfl_sync(0xffffffffu, load_acquire(p), 0) >= want;
+}
+__device__ __noinline__ bool wait_counter(const int* p, int want, int* err) {
   unsigned long long t0 = 0;
   for (uint32_t polls = 1;; ++polls) {
-    if (load_acquire(p) >= want) return true;
+    if (counter_reached(p, want)) return true;
     if ((polls & 255u) == 0) {
-      const unsigned long long now = globaltimer_ns();
+      const unsigned long long now = __shfl_sync(0xffffffffu, globaltimer_ns(), 0);
       if (t0 == 0) {
         t0 = now;
       } else if (now - t0 > kWaitLimitNs) {
@@ -541,7 +563,7 @@ struct Tile {
 // The next range, for every warp but the producer.  False: no more.
 template <int NT>
 __device__ __forceinline__ bool next_claim(MoeSmem<NT>& sm, int i, int lane, int* err, Claim& claim) {
-  if (!wait_for(&sm.claim_full[i & 1], (i >> 1) & 1, err)) return false;
+  if (!wait_warp(&sm.claim_full[i & 1], (i >> 1) & 1, err)) return false;
   claim = sm.claim[i & 1];
   __syncwarp();
   if (lane == 0) mbar_arrive(&sm.claim_empty[i & 1]);
@@ -565,7 +587,7 @@ __device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* 
     }
     mbar_arrive(&sm.claim_full[i & 1]);
     const int ph = claim.phase;
-    if (ph < 0) return;
+    if (ph < 0) break;
     if (ph == 2) {  // nothing to load
       ticket = atomicAdd(p.counters, 1);
       continue;
@@ -596,6 +618,9 @@ __device__ void produce(MoeSmem<NT>& sm, const MoeParams& p, const CUtensorMap* 
       }
     }
   }
+  // After a wait that gave up: the copies still in flight land before the CTA ends.
+  for (uint32_t u = r < kStages ? 0 : r - kStages; !ok && u < r; ++u)
+    wait_for(&sm.w_full[u % kStages], (u / kStages) & 1, p.err);
 }
 
 // One of the gather warps: its share of the units, round robin.  A unit's copies and scales are in
@@ -677,15 +702,15 @@ struct Gather {
     const int stage = r % kStages;
     if (ok && ph == 1 && c.tile != ready) {  // the tile's hidden values: written by other CTAs
       const int* counter = p.counters + kReadyAt + c.tile;
-      if (load_acquire(counter) < kc2) {
+      if (!counter_reached(counter, kc2)) {
         finish(other, false);
         ok = wait_counter(counter, kc2, p.err);
       }
       ready = c.tile;
     }
-    if (ok && !mbar_test(&sm.empty[stage], ((r / kStages) & 1) ^ 1)) {
+    if (ok && !__all_sync(0xffffffffu, mbar_test(&sm.empty[stage], ((r / kStages) & 1) ^ 1))) {
       finish(other, false);
-      ok = wait_for(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err);
+      ok = wait_warp(&sm.empty[stage], ((r / kStages) & 1) ^ 1, p.err);
     }
     if (ok) {  // else: the others stop by themselves, their waits on this stage are bounded
       issue(mine, stage);
@@ -836,7 +861,7 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
   uint32_t r = 0;
   bool ok = true;
   Claim claim;
-  for (int i = 0; next_claim(sm, i, lane, p.err, claim); ++i) {
+  for (int i = 0; promo_all(next_claim(sm, i, lane, p.err, claim)); ++i) {
     const int ph = claim.phase, range = claim.range, begin = claim.begin, end = claim.end;
     const Phase f = sm.phase[ph];
     if (ph == 2) {
@@ -895,9 +920,9 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
         const int stage = r % kStages, buf = r % kDBufs;
         // whoever begins an item usually comes last to it: are the other parts there already?
         if (u == stop - 1 && cut && !at_head && tid == 0) others = load_acquire(arrived);
-        ok = ok && wait_for(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
-             wait_for(&sm.d_full[buf], (r / kDBufs) & 1, p.err);
-        if (!ok) continue;
+        ok = ok && wait_warp(&sm.x_full[stage], (r / kStages) & 1, p.err) &&
+             wait_warp(&sm.d_full[buf], (r / kDBufs) & 1, p.err);
+        if (!ok) continue;  // and on through the barriers, which need every warp
         tc::fence_after_sync();
         const uint32_t d = tmem + buf * 2 * NT + m0;
         scale_add<NT>(g, d, &sm.scale[stage][0][m0], groups);
