@@ -66,7 +66,6 @@ __device__ __forceinline__ uint16_t f32_to_bf16(float x) {
 constexpr int kRouterWarps = 8;
 constexpr int kRouterThreads = kRouterWarps * 32;
 constexpr int kRouterCluster = 8;
-constexpr int kExpertsPerLane = kMoeMaxExperts / 32;
 
 // Order of the choice: larger logits first, a NaN after every number; 0 is not to be chosen.
 __device__ __forceinline__ uint32_t choice_key(float x) {
@@ -74,37 +73,36 @@ __device__ __forceinline__ uint32_t choice_key(float x) {
   return x == x ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 1u;  // -infinity: 0x007FFFFF
 }
 
-// One token's choice by one warp, its logits in shared memory.  Lane l keeps experts l, l + 32, ...
+// One token's choice by one warp, its logits in shared memory.  Lane l keeps experts l, l + 32, ...,
+// kPer of them at most.
+template <int kPer>
 __device__ __forceinline__ void choose_experts(const MoeParams& p, int64_t token,
                                                const float* logits, int lane) {
-  uint32_t key[kExpertsPerLane];
+  uint32_t key[kPer];
 #pragma unroll
-  for (int j = 0; j < kExpertsPerLane; ++j)
+  for (int j = 0; j < kPer; ++j)
     key[j] = lane + 32 * j < p.E ? choice_key(logits[lane + 32 * j]) : 0u;
-  float top = 0.f, chosen = 0.f;
   int my_id = 0;
   for (int k = 0; k < p.top_k; ++k) {
     uint32_t best = 0u;
 #pragma unroll
-    for (int j = 0; j < kExpertsPerLane; ++j) best = max(best, key[j]);
+    for (int j = 0; j < kPer; ++j) best = max(best, key[j]);
     best = __reduce_max_sync(0xffffffffu, best);
     uint32_t at = 0xffffffffu;  // the lowest of the experts that have it
 #pragma unroll
-    for (int j = kExpertsPerLane - 1; j >= 0; --j)
+    for (int j = kPer - 1; j >= 0; --j)
       if (key[j] == best) at = lane + 32 * j;
     at = __reduce_min_sync(0xffffffffu, at);
 #pragma unroll
-    for (int j = 0; j < kExpertsPerLane; ++j)
+    for (int j = 0; j < kPer; ++j)
       if (static_cast<int>(at) == lane + 32 * j) key[j] = 0u;
-    const float l = logits[at];
-    if (k == 0) top = l;
-    if (lane == k) {
-      my_id = static_cast<int>(at);
-      chosen = l;
-    }
+    if (lane == k) my_id = static_cast<int>(at);
   }
+  const float chosen = logits[my_id], top = __shfl_sync(0xffffffffu, chosen, 0);
   float sum = 0.f;
-  for (int e = lane; e < p.E; e += 32) sum += expf(logits[e] - top);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (lane + 32 * j < p.E) sum += expf(logits[lane + 32 * j] - top);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   float c = lane < p.top_k ? expf(chosen - top) / sum : 0.f;
@@ -145,7 +143,7 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
   __shared__ float logits[kMoeMaxExperts];
   __shared__ double part[kRouterWarps][16][kRouterTokens];
   cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();  // every CTA has started: its shared memory may be written
+  cluster.barrier_arrive();  // this CTA has started: its shared memory may be written
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the counters of the next kernel
@@ -157,6 +155,7 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int row = lane >> 2, col = 8 * (lane & 3);
   const bool real = t0 + row < p.T;
+  bool started = false;
   const uint16_t* x = p.x + (t0 + row) * p.x_row_stride + col;
   for (int e0 = 16 * rank; e0 < p.E; e0 += 16 * kRouterCluster) {
     const uint16_t* w = p.router + static_cast<int64_t>(e0 + row) * p.H + col;
@@ -190,6 +189,8 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     part[warp][row + 8][2 * (lane & 3)] = acc[2];
     part[warp][row + 8][2 * (lane & 3) + 1] = acc[3];
     __syncthreads();
+    if (!started) cluster.barrier_wait();
+    started = true;
     if (threadIdx.x < 16 * kRouterTokens) {
       const int e = threadIdx.x / kRouterTokens, t = threadIdx.x % kRouterTokens;
       double sum = 0.0;
@@ -199,8 +200,15 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     }
     __syncthreads();
   }
+  if (!started) cluster.barrier_wait();  // no experts left for this CTA
   cluster.sync();
-  if (warp == 0 && rank < kRouterTokens && t0 + rank < p.T) choose_experts(p, t0 + rank, logits, lane);
+  if (warp == 0 && rank < kRouterTokens && t0 + rank < p.T) {
+    if (p.E <= 128) {  // 128 experts: 1.1 instead of 2 us
+      choose_experts<4>(p, t0 + rank, logits, lane);
+    } else {
+      choose_experts<kMoeMaxExperts / 32>(p, t0 + rank, logits, lane);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ experts
