@@ -104,6 +104,15 @@ def route(x, router, top_k, renormalize):
     return (c / c.sum(-1, keepdim=True) if renormalize else c), order
 
 
+def route_rel(x, router):
+    """[T, 1]: how far, relatively, the router's weights may be off.  A logit is a sum of fp32 sums of 32
+    products, 32 additions of at most 2^-23 of their absolute terms each (tensor cores truncate), and
+    one rounding to fp32; a weight is a ratio of exponentials of differences of logits: twice a logit's
+    error, and a few ulps of the exponentials and the fp32 sums of up to 512 of them."""
+    terms = (x.double().abs() @ router.double().abs().t()).amax(-1, keepdim=True)
+    return 2 * terms * (32 * 2.0 ** -23 + 2.0 ** -24) + 2.0 ** -19
+
+
 def moe(x, xq, x_scale, router, w13, w13_scale, w2, w2_scale, top_k, renormalize):
     """(out float64 [T, H], err [T, H], weights, ids).  ``err`` bounds what fp32 sums may change
     before the last rounding:
@@ -113,9 +122,10 @@ def moe(x, xq, x_scale, router, w13, w13_scale, w2, w2_scale, top_k, renormalize
     * h = silu(g) u then moves by at most 1.1 |u| err_g + |silu(g)| err_u (|silu'| <= 1.1) and a few
       ulps; its scale and quotient follow, and a quotient that may cross a midpoint between two e4m3
       values moves its dequantised value by up to the distance of the interval's two roundings;
-    * the second product adds its own n 2^-24, the router's weights 2^-20.
+    * the second product adds its own n 2^-24, the router's weights route_rel.
     """
     c, ids = route(x, router, top_k, renormalize)
+    rel_c = torch.nan_to_num(route_rel(x, router), posinf=0.0)
     T, H = x.shape
     I = w2.shape[-1]
     out = torch.zeros(T, H, dtype=torch.float64, device=x.device)
@@ -151,5 +161,5 @@ def moe(x, xq, x_scale, router, w13, w13_scale, w2, w2_scale, top_k, renormalize
         ey = torch.nan_to_num(ehv) @ v2.abs().t() + rel2 * (hv.abs() @ v2.abs().t())
         w = c[t, place][:, None]
         out.index_add_(0, t, w * y)
-        err.index_add_(0, t, w * (ey + y.abs() * 2.0 ** -19))
+        err.index_add_(0, t, w * (ey + y.abs() * (2.0 ** -21 + rel_c[t])))
     return out, err, c, ids

@@ -2,7 +2,7 @@
 
 The tolerance is the oracle's own bound on what fp32 sums may change (n 2^-24 of a dot product's
 absolute terms, and what that may move across the midpoints of the 8-bit hidden values), then the
-bf16 rounding of the result.  Router weights: an fp32 softmax within 2^-20; chosen experts are equal.
+bf16 rounding of the result.  Router weights: within what the logits' sums allow; chosen experts are equal.
 """
 import pytest
 import torch
@@ -50,7 +50,7 @@ def _check(a, top_k, renormalize=True):
     ref, err, c64, ids64 = ffn.moe(a["x"], a["xq"], a["x_scale"], a["router"], a["w13"],
                                    a["w13_scale"], a["w2"], a["w2_scale"], top_k, renormalize)
     assert torch.equal(ids.long(), ids64)
-    assert bool(((c.double() - c64).abs() <= c64 * 2.0 ** -20).all())
+    assert bool(((c.double() - c64).abs() <= c64 * ffn.route_rel(a["x"], a["router"])).all())
     ffn.assert_within(out, ref, err, ffn.bf16, "out")
     _no_device_error()
     return out, c, ids
