@@ -3,8 +3,8 @@
 Tolerances, from the arithmetic: the norm's fp32 sum runs over at most 32 terms in a thread, 5 in a warp
 and 16 warps, so it is off by at most 53 2^-24, its inverse root by half of that and 2 ulps, and three
 more products by half an ulp each: under 2^-18.  SiLU: exp within 2 ulps, an addition, a division and a
-product: under 2^-20, and where exp(-g) overflows (g < -88) the result is 0 for a true |h| below
-2^-120 |u|.  Outputs in 8 and 16 bits are then the rounding of a value within that of the definition's.
+product: under 2^-20, and where 1 + exp(-g) is above 2^126 (g < -87.3), whose inverse is below fp32's
+normal numbers, the result is 0 for a true |h| of at most 87.4 2^-126 |u|, below 2^-119 |u|.  Outputs in 8 and 16 bits are then the rounding of a value within that of the definition's.
 """
 import pytest
 import torch
@@ -144,7 +144,7 @@ def _check_silu(gu):
     assert q.is_contiguous() and d.is_contiguous() and d.dtype == torch.bfloat16
     h = ffn.silu_mul(gu[:, :i], gu[:, i:])
     top = float(torch.nan_to_num(gu[:, i:].double(), posinf=0, neginf=0).abs().max()) if m else 0
-    ffn.assert_quantised(q, d, h, SILU_REL, absolute=2.0 ** -120 * max(1.0, top))
+    ffn.assert_quantised(q, d, h, SILU_REL, absolute=2.0 ** -119 * max(1.0, top))
     return q, d
 
 
