@@ -977,9 +977,13 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
 #pragma unroll 1  // one at a time: unrolled by two, the larger code cost 2 to 7 %
       for (int m = warp; m < t.count; m += kPromoWarps) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-        if (here) {
-          a = *reinterpret_cast<const float4*>(&sm.item[0][m][4 * lane]);
-          if (ph == 0) b = *reinterpret_cast<const float4*>(&sm.item[1][m][4 * lane]);
+        if (here) {  // added to 0 as a part from memory is: the sign of a zero must not depend on timing
+          const float4 s = *reinterpret_cast<const float4*>(&sm.item[0][m][4 * lane]);
+          a = make_float4(a.x + s.x, a.y + s.y, a.z + s.z, a.w + s.w);
+          if (ph == 0) {
+            const float4 z = *reinterpret_cast<const float4*>(&sm.item[1][m][4 * lane]);
+            b = make_float4(b.x + z.x, b.y + z.y, b.z + z.z, b.w + z.w);
+          }
         }
 #pragma unroll 1
         for (int q0 = here ? r0 + 1 : r0; cut && q0 <= r1; q0 += 4) {  // four parts' loads in flight

@@ -167,12 +167,21 @@ def test_strided_inputs_and_single_rows():
         assert torch.equal(p[3:4], q)
 
 
-def test_repeated_calls_are_equal_bit_for_bit():
-    a = _inputs(48, 1024, 512, 32, 3500)
+def _bits(t):
+    return t.contiguous().view(torch.uint8)
+
+
+@pytest.mark.parametrize("sd", [1.0, 0.0])
+def test_repeated_calls_are_equal_bit_for_bit(sd):
+    """Whichever CTA comes last: zeros and their signs included (zero inputs under weights of both
+    signs)."""
+    a = _inputs(48, 1024, 512, 32, 3500, sd=sd)
+    if sd == 0.0:
+        a["xq"].view(torch.uint8)[::2] = 0x80                # minus zero
     want = _run(a, 4)
     for _ in range(20):
         for p, q in zip(want, _run(a, 4)):
-            assert torch.equal(p, q)
+            assert torch.equal(_bits(p), _bits(q))
 
 
 def test_a_token_s_result_does_not_depend_on_its_batch():
