@@ -165,28 +165,6 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) add_rms_norm_quant_kernel(
 }
 
 // ------------------------------------------------------------------ SiLU * up + quantise
-// g / (1 + e^-g) of two values.  e^-g = 2^(-g log2 e): the product's rounding error, which the power
-// would multiply by |g|, is recovered by a fused multiply-add (error-free product) and applied to first
-// order, 2^(t + d) = 2^t (1 + d ln 2).  g is held below 200, where e^-g is 0, so that the product does not
-// overflow; where it overflows below, 1 + e^-g is infinite either way.
-__device__ __forceinline__ uint64_t silu2(uint64_t g) {
-  const float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
-  // log2 e - float(log2 e)
-  const float kLog2eRest = static_cast<float>(1.44269504088896340736 - 1.44269502162933349609375);
-  float g0, g1;
-  f2_unpack(g, g0, g1);
-  const uint64_t c = f2_pack(fminf(g0, 200.f), fminf(g1, 200.f));
-  const uint64_t t = f2_mul(c, f2_pack(kLog2e, kLog2e));
-  const uint64_t rest = f2_fma(c, f2_pack(-kLog2e, -kLog2e), t);  // t - c log2 e, exactly
-  const uint64_t d = f2_fma(c, f2_pack(-kLog2eRest, -kLog2eRest), rest);
-  float t0, t1;
-  f2_unpack(t, t0, t1);
-  const uint64_t e = f2_mul(f2_pack(ex2(-t0), ex2(-t1)), f2_fma(d, f2_pack(kLn2, kLn2), f2_pack(1.f, 1.f)));
-  float q0, q1;
-  f2_unpack(f2_add(e, f2_pack(1.f, 1.f)), q0, q1);
-  return f2_mul(g, f2_pack(rcp(q0), rcp(q1)));
-}
-
 constexpr int kSiluThreads = 128;  // 78.7 us for 8192 x 12288, 8.1 for 333 x 25600 (256: 79.5 and 8.7)
 constexpr int kSiluThreadsLog2 = 7;
 static_assert(kSiluThreads == 1 << kSiluThreadsLog2, "shifts");

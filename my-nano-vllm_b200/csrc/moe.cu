@@ -57,7 +57,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* e
 
 constexpr int kBlk = 128;
 
-__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
 __device__ __forceinline__ uint16_t f32_to_bf16(float x) {
   return __bfloat16_as_ushort(__float2bfloat16_rn(x));
 }
@@ -951,24 +950,24 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
       constexpr int kPart = NT * kBlk;  // floats; phase 0 has two of them (gate, up)
       float* const parts = p.parts[ph];
       const int size = ph == 0 ? 2 * kPart : kPart;
-      auto put = [&](float* to) {
+      float* const mine = parts + (2 * static_cast<int64_t>(range) + (at_head ? 0 : 1)) * size;
+      float* to = at_head ? mine : &sm.item[0][0][0];
+      if (tid == 0) sm.others_here = others == r1 - r0;
+      bool here;  // part 0 in shared memory, the others complete
+#pragma unroll 1
+      for (;;) {  // once, or, for the beginner of an item whose other parts are not there, twice
 #pragma unroll
         for (int j = 0; j < kHalf; ++j)
           if (j < 8 * groups) {
             to[(m0 + j) * kBlk + col] = g[j];
             if (ph == 0) to[kPart + (m0 + j) * kBlk + col] = v[j];
           }
-      };
-      float* const mine = parts + (2 * static_cast<int64_t>(range) + (at_head ? 0 : 1)) * size;
-      put(at_head ? mine : &sm.item[0][0][0]);
-      if (tid == 0) sm.others_here = others == r1 - r0;
-      promo_sync();
-      const bool here = !cut || (!at_head && sm.others_here);  // part 0 in shared memory, the others complete
+        promo_sync();
+        here = to != mine && (!cut || sm.others_here);
+        if (here || to == mine) break;
+        to = mine;
+      }
       if (!here) {
-        if (!at_head) {
-          put(mine);
-          promo_sync();
-        }
         if (tid == 0) sm.last = add_acq_rel(arrived) == r1 - r0;
         promo_sync();
         if (!sm.last) continue;
@@ -1009,7 +1008,9 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
           __stcg(reinterpret_cast<float4*>(p.y + slot * p.H + blk * kBlk + 4 * lane), a);
         } else {
           // h = silu(gate) up, quantised over the item's 128 columns
-          float h[4] = {silu(a.x) * b.x, silu(a.y) * b.y, silu(a.z) * b.z, silu(a.w) * b.w};
+          float h[4];
+          f2_unpack(f2_mul(silu2(f2_pack(a.x, a.y)), f2_pack(b.x, b.y)), h[0], h[1]);
+          f2_unpack(f2_mul(silu2(f2_pack(a.z, a.w)), f2_pack(b.z, b.w)), h[2], h[3]);
           const float most = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])),
                                    fmaxf(fmaxf(fabsf(h[2]), fabsf(h[3])), 0.f));  // NaN left out
           const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
