@@ -38,33 +38,14 @@ MAX_TOKENS = 1024       # tokens in one fp8_moe call
 MAX_SLOTS = 8192        # tokens * top_k in one fp8_moe call
 
 # The kernels of a decoded token take 2 to 25 us, so the host side counts: raw stream handles and
-# empty_strided cost 0.1 and 1.5 us a call where current_stream() and empty() cost 2.2 and 2.4.
+# empty_strided cost 0.1 and 1.4 us a call where current_stream() and empty() cost 2.2 and 2.4, and a
+# helper's call 0.3.
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
-
-
-def _launch(device: int, fn, *args) -> None:
-    """fn(*args, stream) on the current stream of ``device``, which is made the current device for
-    the launch where it is not."""
-    if device == _current_device():
-        rc = fn(*args, _raw_stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device))
-    if rc:
-        _lib.check(rc)
-
-
-def _rows(t: torch.Tensor, dtype: torch.dtype, device: int) -> int:
-    """Checks a 2-D operand; its row stride in elements (that of a single row is never used, and torch
-    leaves it arbitrary)."""
-    assert t.get_device() == device and t.dtype == dtype and t.dim() == 2 and t.stride(1) == 1, \
-        "expected rows of unit stride, of the first operand's device"
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _new(m: int, n: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    return torch.empty_strided((m, n), (n, 1), dtype=dtype, device=device)
+_empty = torch.empty_strided
+_norm_quant = _lib.lib.fp8attn_add_rms_norm_quant
+_silu_quant = _lib.lib.fp8attn_silu_mul_quant
+_moe = _lib.lib.fp8attn_fp8_moe
 
 
 def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor,
@@ -79,52 +60,70 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: tor
     residual).
     """
     dtype, device = x.dtype, x.get_device()
-    assert dtype in _DTYPES and device >= 0, "x must be a bf16 or fp16 CUDA tensor"
-    x_stride = _rows(x, dtype, device)
+    code = _DTYPES.get(dtype)
+    assert code is not None and device >= 0, "x must be a bf16 or fp16 CUDA tensor"
+    assert x.dim() == 2 and x.stride(1) == 1
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return add_rms_norm_fp8(x, residual, weight, eps, return_norm)
     M, K = x.shape
     assert weight.get_device() == device and weight.dtype == dtype and weight.is_contiguous()
     assert weight.numel() == K and K % BLOCK_SIZE == 0 and K > 0
     dev = x.device
-    res_in = res_stride = res_out = y_out = 0
+    # the row stride of a single row is never used, and torch leaves it arbitrary
+    x_stride = x.stride(0) if M > 1 else K
     res = y = None
+    res_in = res_stride = res_out = y_out = 0
     if residual is not None:
-        res_stride = _rows(residual, dtype, device)
-        assert residual.shape == x.shape
-        res = _new(M, K, dtype, dev)
+        assert residual.get_device() == device and residual.dtype == dtype
+        assert residual.shape == x.shape and residual.stride(1) == 1
+        res_stride = residual.stride(0) if M > 1 else K
+        res = _empty((M, K), (K, 1), dtype=dtype, device=dev)
         res_in, res_out = residual.data_ptr(), res.data_ptr()
     if return_norm:
-        y = _new(M, K, dtype, dev)
+        y = _empty((M, K), (K, 1), dtype=dtype, device=dev)
         y_out = y.data_ptr()
-    xq = _new(M, K, _E4M3, dev)
-    xs = _new(M, K // BLOCK_SIZE, _BF16, dev)
+    groups = K // BLOCK_SIZE
+    xq = _empty((M, K), (K, 1), dtype=_E4M3, device=dev)
+    xs = _empty((M, groups), (groups, 1), dtype=_BF16, device=dev)
     if M > 0:
-        _launch(device, _lib.lib.fp8attn_add_rms_norm_quant, x.data_ptr(), x_stride, res_in,
-                res_stride, weight.data_ptr(), eps, xq.data_ptr(), xs.data_ptr(), res_out, y_out, M,
-                K, _DTYPES[dtype])
+        rc = _norm_quant(x.data_ptr(), x_stride, res_in, res_stride, weight.data_ptr(), eps,
+                         xq.data_ptr(), xs.data_ptr(), res_out, y_out, M, K, code,
+                         _raw_stream(device))
+        if rc:
+            _lib.check(rc)
     return xq, xs, res, y
 
 
 def silu_mul_fp8(gate_up: torch.Tensor):
-    """gate_up: bf16 or fp16 [M, 2 I] (rows may be strided), gate columns first; I a multiple of 128.
-    Returns (hq, h_scale): gate / (1 + exp(-gate)) * up as e4m3 [M, I] with scales bf16 [M, I / 128]."""
-    dtype, device = gate_up.dtype, gate_up.get_device()
-    assert dtype in _DTYPES and device >= 0, "gate_up must be a bf16 or fp16 CUDA tensor"
-    stride = _rows(gate_up, dtype, device)
-    M, I2 = gate_up.shape
-    assert I2 % (2 * BLOCK_SIZE) == 0 and I2 > 0
-    inner, dev = I2 // 2, gate_up.device
-    hq = _new(M, inner, _E4M3, dev)
-    hs = _new(M, inner // BLOCK_SIZE, _BF16, dev)
+    """gate_up: bf16 or fp16 [M, 2 I] (rows may be strided), gate columns first; I a multiple of 128 up
+    to 2^20.  Returns (hq, h_scale): gate / (1 + exp(-gate)) * up as e4m3 [M, I] with scales bf16
+    [M, I / 128]."""
+    device = gate_up.get_device()
+    code = _DTYPES.get(gate_up.dtype)
+    assert code is not None and device >= 0, "gate_up must be a bf16 or fp16 CUDA tensor"
+    assert gate_up.dim() == 2 and gate_up.stride(1) == 1
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return silu_mul_fp8(gate_up)
+    M, columns = gate_up.shape
+    assert columns % (2 * BLOCK_SIZE) == 0 and columns > 0
+    inner, dev = columns // 2, gate_up.device
+    groups = inner // BLOCK_SIZE
+    hq = _empty((M, inner), (inner, 1), dtype=_E4M3, device=dev)
+    hs = _empty((M, groups), (groups, 1), dtype=_BF16, device=dev)
     if M > 0:
-        _launch(device, _lib.lib.fp8attn_silu_mul_quant, gate_up.data_ptr(), stride, hq.data_ptr(),
-                hs.data_ptr(), M, inner, _DTYPES[dtype])
+        rc = _silu_quant(gate_up.data_ptr(), gate_up.stride(0) if M > 1 else columns, hq.data_ptr(),
+                         hs.data_ptr(), M, inner, code, _raw_stream(device))
+        if rc:
+            _lib.check(rc)
     return hq, hs
 
 
 @functools.lru_cache(maxsize=1024)
 def _moe_scratch_bytes(device: int, T: int, H: int, I: int, E: int, top_k: int) -> int:
-    with torch.cuda.device(device):
-        return _lib.lib.fp8attn_fp8_moe_workspace_bytes(T, H, I, E, top_k)
+    """By the current device's number of SMs, which ``device`` stands for."""
+    return _lib.lib.fp8attn_fp8_moe_workspace_bytes(T, H, I, E, top_k)
 
 
 def _error_word(device: int) -> int:
@@ -159,10 +158,15 @@ def fp8_moe(x: torch.Tensor, xq: torch.Tensor, x_scale: torch.Tensor, router_wei
     [T, top_k]).
     """
     device = x.get_device()
-    assert device >= 0, "x must be a CUDA tensor"
-    x_stride, xq_stride = _rows(x, _BF16, device), _rows(xq, _E4M3, device)
+    assert device >= 0 and x.dtype == _BF16, "x must be a bf16 CUDA tensor"
+    assert x.dim() == 2 and x.stride(1) == 1
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return fp8_moe(x, xq, x_scale, router_weight, gate_up_weight, gate_up_scale, down_weight,
+                           down_scale, top_k, renormalize, return_router)
     T, H = x.shape
-    assert xq.shape == x.shape and H % BLOCK_SIZE == 0 and H > 0
+    assert xq.get_device() == device and xq.dtype == _E4M3
+    assert xq.shape == x.shape and xq.stride(1) == 1 and H % BLOCK_SIZE == 0 and H > 0
     assert x_scale.get_device() == device and x_scale.dtype == _BF16 and x_scale.is_contiguous()
     assert x_scale.shape == (T, H // BLOCK_SIZE)
     assert router_weight.get_device() == device and router_weight.dtype == _BF16
@@ -172,20 +176,24 @@ def fp8_moe(x: torch.Tensor, xq: torch.Tensor, x_scale: torch.Tensor, router_wei
     _check_experts(gate_up_weight, gate_up_scale, device, E, 2 * I, H)
     _check_experts(down_weight, down_scale, device, E, H, I)
     dev = x.device
-    out = _new(T, H, _BF16, dev)
+    out = _empty((T, H), (H, 1), dtype=_BF16, device=dev)
     weights = ids = None
     weights_out = ids_out = 0
     if return_router:
-        weights = _new(T, top_k, torch.float32, dev)
-        ids = _new(T, top_k, torch.int32, dev)
+        weights = _empty((T, top_k), (top_k, 1), dtype=torch.float32, device=dev)
+        ids = _empty((T, top_k), (top_k, 1), dtype=torch.int32, device=dev)
         weights_out, ids_out = weights.data_ptr(), ids.data_ptr()
     if T > 0:
         nbytes = _moe_scratch_bytes(device, T, H, I, E, top_k)
         # scratch of this call alone: calls on other streams and captured graphs share none
-        scratch = _new(1, max(nbytes, 0), torch.uint8, dev)
-        _launch(device, _lib.lib.fp8attn_fp8_moe, x.data_ptr(), x_stride, xq.data_ptr(), xq_stride,
-                x_scale.data_ptr(), router_weight.data_ptr(), gate_up_weight.data_ptr(),
-                gate_up_scale.data_ptr(), down_weight.data_ptr(), down_scale.data_ptr(),
-                out.data_ptr(), H, weights_out, ids_out, T, H, I, E, top_k, 1 if renormalize else 0,
-                scratch.data_ptr(), nbytes, _error_word(device))
+        scratch = _empty((max(nbytes, 0),), (1,), dtype=torch.uint8, device=dev)
+        # the row stride of a single row is never used, and torch leaves it arbitrary
+        rc = _moe(x.data_ptr(), x.stride(0) if T > 1 else H, xq.data_ptr(),
+                  xq.stride(0) if T > 1 else H, x_scale.data_ptr(), router_weight.data_ptr(),
+                  gate_up_weight.data_ptr(), gate_up_scale.data_ptr(), down_weight.data_ptr(),
+                  down_scale.data_ptr(), out.data_ptr(), H, weights_out, ids_out, T, H, I, E, top_k,
+                  1 if renormalize else 0, scratch.data_ptr(), nbytes, _error_word(device),
+                  _raw_stream(device))
+        if rc:
+            _lib.check(rc)
     return (out, weights, ids) if return_router else out
