@@ -287,7 +287,8 @@ FP8ATTN_API int fp8attn_silu_mul_quant(const void* gate_up, int64_t row_stride, 
 /*
  * A mixture-of-experts layer for a few tokens, weights in the format of fp8attn_fp8_block_linear (no
  * counterpart in the reference, whose model is dense).  Per token: l = x . router^T; p = softmax(l);
- * the top_k largest p (ties: the lower expert first; a NaN is chosen last) with weights c = p, divided
+ * the top_k largest p (as l summed in fp64 orders them; ties: the lower expert first; a NaN is chosen
+ * last) with weights c = p, divided
  * by their sum if renormalize; for each chosen expert e: g, u = the halves of xq . w13[e]^T,
  * h = g / (1 + exp(-g)) * u quantised as above, y_e = hq . w2[e]^T (block-scaled products as in
  * fp8attn_fp8_block_gemm); out = bf16(sum of c_e y_e, in the order chosen).

@@ -75,18 +75,12 @@ __device__ __forceinline__ uint32_t choice_key(float x) {
   const uint32_t u = __float_as_uint(x);
   return x == x ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 1u;  // -infinity: 0x007FFFFF
 }
-
-// One token's choice by one warp, its logits in shared memory.  Lane l keeps experts l, l + 32, ...,
-// kPer of them at most.
+// The top_k largest keys by one warp, ties to the lower expert.  Lane l keeps experts l, l + 32, ..., kPer
+// of them at most.  Returns the expert of place `lane`; the keys of chosen experts become 0.
 template <int kPer>
-__device__ __forceinline__ void choose_experts(const MoeParams& p, int64_t token,
-                                               const float* logits, int lane) {
-  uint32_t key[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j)
-    key[j] = lane + 32 * j < p.E ? choice_key(logits[lane + 32 * j]) : 0u;
+__device__ __forceinline__ int choose(uint32_t (&key)[kPer], int top_k, int lane) {
   int my_id = 0;
-  for (int k = 0; k < p.top_k; ++k) {
+  for (int k = 0; k < top_k; ++k) {
     uint32_t best = 0u;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) best = max(best, key[j]);
@@ -101,11 +95,15 @@ __device__ __forceinline__ void choose_experts(const MoeParams& p, int64_t token
       if (static_cast<int>(at) == lane + 32 * j) key[j] = 0u;
     if (lane == k) my_id = static_cast<int>(at);
   }
+  return my_id;
+}
+
+// A token's weights, and its choice with them, written by one warp: my_id is the expert of place `lane`.
+__device__ __forceinline__ void write_choice(const MoeParams& p, int64_t token, const float* logits,
+                                             int my_id, int lane) {
   const float chosen = logits[my_id], top = __shfl_sync(0xffffffffu, chosen, 0);
   float sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j)
-    if (lane + 32 * j < p.E) sum += expf(logits[lane + 32 * j] - top);
+  for (int e = lane; e < p.E; e += 32) sum += expf(logits[e] - top);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   float c = lane < p.top_k ? expf(chosen - top) / sum : 0.f;
@@ -121,30 +119,112 @@ __device__ __forceinline__ void choose_experts(const MoeParams& p, int64_t token
   }
 }
 
+// One token's choice by one warp from logits that may be off by up to the largest of `bounds`, B; my_id: the
+// expert of place `lane`.  Where no two neighbours in the order differ by 2 B or less, from the first to the
+// first that is not chosen, the order is that of exact sums.  Else `open` gets the experts whose order is
+// not known; returns how many.
+template <int kPer>
+__device__ __forceinline__ int choose_or_list(const MoeParams& p, const float* logits, const float* bounds,
+                                              uint16_t* open, int& my_id, int lane) {
+  uint32_t key[kPer];
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const bool ok = lane + 32 * j < p.E;
+    key[j] = ok ? choice_key(logits[lane + 32 * j]) : 0u;
+    const float b = ok ? bounds[lane + 32 * j] : 0.f;
+    if (b < INFINITY) most = fmaxf(most, b);  // an infinite or NaN logit is no sum that rounding moved
+  }
+  const float gap = 2.f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+  my_id = choose<kPer>(key, p.top_k, lane);
+  uint32_t rest = 0u;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) rest = max(rest, key[j]);
+  rest = __reduce_max_sync(0xffffffffu, rest);
+  const float mine = logits[my_id];
+  float next = __shfl_down_sync(0xffffffffu, mine, 1);
+  if (lane == p.top_k - 1)  // the best that is not chosen
+    next = rest > 1u ? __uint_as_float(rest & 0x80000000u ? rest ^ 0x80000000u : ~rest) : -INFINITY;
+  // places that are open against the next; a bound of 0 has no term but zeros
+  const unsigned places = __ballot_sync(0xffffffffu, lane < p.top_k && gap > 0.f && mine - next <= gap);
+  if (places == 0u) return 0;
+  const bool listed = ((places | places << 1) >> lane & 1u) != 0u && lane < p.top_k;
+  const unsigned who = __ballot_sync(0xffffffffu, listed);
+  if (listed) open[__popc(who & ((1u << lane) - 1u))] = static_cast<uint16_t>(my_id);
+  int count = __popc(who);
+  if (places >> (p.top_k - 1) & 1u) {  // and whatever else may belong to the chosen
+    const float last = __shfl_sync(0xffffffffu, mine, p.top_k - 1) - gap;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const bool more = key[j] != 0u && logits[lane + 32 * j] >= last;  // key 0: chosen, or no expert
+      const unsigned them = __ballot_sync(0xffffffffu, more);
+      if (more) open[count + __popc(them & ((1u << lane) - 1u))] = static_cast<uint16_t>(lane + 32 * j);
+      count += __popc(them);
+    }
+  }
+  return count;
+}
+
 // d += a . b^T: a 16 x 16, b 8 x 16 bf16.  Lane l holds a's rows l / 4 and l / 4 + 8, b's row l / 4, and
 // d's rows l / 4 (d0, d1) and l / 4 + 8 (d2, d3), columns 2 (l % 4) and the next.
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 8 bf16 values without their signs.
+__device__ __forceinline__ uint4 magnitudes(const uint4& v) {
+  constexpr uint32_t kMask = 0x7FFF7FFFu;
+  return make_uint4(v.x & kMask, v.y & kMask, v.z & kMask, v.w & kMask);
+}
+
+// This thread's share of x . w in fp64 (a product has 16 bits: fp32 holds it), the same columns in the same
+// order whatever the row: equal rows have equal sums.
+__device__ __forceinline__ double exact_part(const uint16_t* x, const uint16_t* w, int H) {
+  double sum = 0.0;
+  for (int v = threadIdx.x; v < H / 8; v += kRouterThreads) {
+    const uint4 a = *reinterpret_cast<const uint4*>(x + 8 * v);
+    const uint4 b = __ldg(reinterpret_cast<const uint4*>(w + 8 * v));
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum += __uint_as_float(aw[i] << 16) * __uint_as_float(bw[i] << 16);
+      sum += __uint_as_float(aw[i] & 0xFFFF0000u) * __uint_as_float(bw[i] & 0xFFFF0000u);
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  return sum;
+}
+
 // Cluster c: tokens 8 c .. 8 c + 7; CTA r of it: experts 16 r .. 16 r + 15, then 128 on, ...; a CTA's
 // warps share the columns, 32 at a time, each lane loading 16 contiguous bytes of a row (which
 // columns a product's step takes does not matter as long as both operands agree), a warp's loads
-// all in flight.  Sums of 32 products in fp32, then fp64, so that which experts are chosen does not
-// hang on the order of a sum.  The logits of token 8 c + r meet in CTA r.
-// Bound: latency (a launch, a load from HBM, two cluster barriers, the choice).
+// all in flight.  Sums of 32 products in fp32, then fp64, and beside them the sums of the products'
+// magnitudes, which bound what the fp32 sums may be off by.  The logits of token 8 c + r meet in CTA r, which
+// chooses by them where the bound leaves no doubt, and else sums those in doubt again in fp64 (a few
+// percent of the tokens of 128 experts): the experts and their order are those of exact sums.
+// Bound: latency (a launch, a load from HBM, two cluster barriers, the choice): 5.4 us by itself for a token
+// of 2048 columns and 128 experts, 0.7 of them for the bound, and 7.4 where some are summed again.  Two CTAs
+// an SM (128 registers): 250 tokens of 60 experts take 7.9 us, 13.8 with one.
 constexpr int kRouterTokens = 8;
 static_assert(kRouterTokens <= kRouterCluster, "a CTA chooses for one token at most");
+// Of the magnitudes' sum, what a logit may be off by: 32 additions of at most 2^-23 each (tensor cores
+// truncate) and the rounding to fp32, 2^-18 + 2^-24; the magnitudes' own sum, by 32 additions a step over up
+// to 64 steps, may be 2^-12 too small.
+constexpr float kLogitError = 3.9e-6f;
 
-__global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads)
+__global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouterThreads, 2)
     moe_router_kernel(const MoeParams p) {
-  __shared__ float logits[kMoeMaxExperts];
+  __shared__ float logits[kMoeMaxExperts], bounds[kMoeMaxExperts];
   __shared__ double part[kRouterWarps][16][kRouterTokens];
+  __shared__ float part_most[kRouterWarps][16][kRouterTokens];
+  __shared__ uint16_t open[kMoeMaxExperts];
+  __shared__ int num_open, ids[kMoeMaxTopK];
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();  // this CTA has started: its shared memory may be written
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -164,6 +244,7 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
     const uint16_t* w = p.router + static_cast<int64_t>(e0 + row) * p.H + col;
     const bool lo = e0 + row < p.E, hi = e0 + row + 8 < p.E;
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    float most[4] = {0.f, 0.f, 0.f, 0.f};
     constexpr int kAhead = 8;  // steps whose loads are in flight
     const int stride = 32 * kRouterWarps;
     for (int c0 = 32 * warp; c0 < p.H; c0 += kAhead * stride) {
@@ -185,33 +266,78 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
         mma_bf16(d, wl[s].z, wh[s].z, wl[s].w, wh[s].w, xv[s].z, xv[s].w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] += d[i];
+        const uint4 a = magnitudes(wl[s]), b = magnitudes(wh[s]), m = magnitudes(xv[s]);
+        mma_bf16(most, a.x, b.x, a.y, b.y, m.x, m.y);
+        mma_bf16(most, a.z, b.z, a.w, b.w, m.z, m.w);
       }
     }
-    part[warp][row][2 * (lane & 3)] = acc[0];
-    part[warp][row][2 * (lane & 3) + 1] = acc[1];
-    part[warp][row + 8][2 * (lane & 3)] = acc[2];
-    part[warp][row + 8][2 * (lane & 3) + 1] = acc[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      part[warp][row + 8 * (i >> 1)][2 * (lane & 3) + (i & 1)] = acc[i];
+      part_most[warp][row + 8 * (i >> 1)][2 * (lane & 3) + (i & 1)] = most[i];
+    }
     __syncthreads();
     if (!started) cluster.barrier_wait();
     started = true;
+    const int at = threadIdx.x % (16 * kRouterTokens), e = at / kRouterTokens, t = at % kRouterTokens;
+    static_assert(kRouterThreads == 2 * 16 * kRouterTokens, "half the threads for either sum");
     if (threadIdx.x < 16 * kRouterTokens) {
-      const int e = threadIdx.x / kRouterTokens, t = threadIdx.x % kRouterTokens;
       double sum = 0.0;
 #pragma unroll
       for (int k = 0; k < kRouterWarps; ++k) sum += part[k][e][t];
       if (e0 + e < p.E) *cluster.map_shared_rank(&logits[e0 + e], t) = static_cast<float>(sum);
+    } else {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kRouterWarps; ++k) sum += part_most[k][e][t];
+      if (e0 + e < p.E) *cluster.map_shared_rank(&bounds[e0 + e], t) = sum * kLogitError;
     }
     __syncthreads();
   }
   if (!started) cluster.barrier_wait();  // no experts left for this CTA
   cluster.sync();
-  if (warp == 0 && rank < kRouterTokens && t0 + rank < p.T) {
-    if (p.E <= 128) {  // 128 experts: 1.1 instead of 2 us
-      choose_experts<4>(p, t0 + rank, logits, lane);
-    } else {
-      choose_experts<kMoeMaxExperts / 32>(p, t0 + rank, logits, lane);
-    }
+  const int64_t token = t0 + rank;
+  if (rank >= kRouterTokens || token >= p.T) return;
+  int my_id = 0;
+  if (warp == 0) {
+    const int n = p.E <= 128  // 128 experts: 1.1 instead of 2 us
+                      ? choose_or_list<4>(p, logits, bounds, open, my_id, lane)
+                      : choose_or_list<kMoeMaxExperts / 32>(p, logits, bounds, open, my_id, lane);
+    if (n == 0) write_choice(p, token, logits, my_id, lane);
+    ids[lane] = my_id;
+    if (lane == 0) num_open = n;
   }
+  __syncthreads();
+  const int n = num_open;
+  if (n == 0) return;
+  // exact sums for the open ones; this CTA's `part` is free and no other CTA's business
+  double* const exact = &part[0][0][0];  // of every expert
+  double* const sums = exact + kMoeMaxExperts;
+  static_assert(sizeof(part) >= (kMoeMaxExperts + kRouterWarps) * sizeof(double), "exact");
+  for (int e = threadIdx.x; e < p.E; e += kRouterThreads) exact[e] = logits[e];
+  for (int i = 0; i < n; ++i) {
+    const double mine = exact_part(p.x + token * p.x_row_stride, p.router + static_cast<int64_t>(open[i]) * p.H, p.H);
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double sum = 0.0;
+      for (int k = 0; k < kRouterWarps; ++k) sum += sums[k];
+      exact[open[i]] = sum;
+      logits[open[i]] = static_cast<float>(sum);
+    }
+    __syncthreads();
+  }
+  // an open expert's place: how many come before it
+  for (int i = warp; i < n; i += kRouterWarps) {
+    const int e = open[i];
+    const double mine = exact[e];
+    int place = 0;
+    for (int f = lane; f < p.E; f += 32) place += exact[f] > mine || (exact[f] == mine && f < e);
+    place = __reduce_add_sync(0xffffffffu, place);
+    if (lane == 0 && place < p.top_k) ids[place] = e;
+  }
+  __syncthreads();
+  if (warp == 0) write_choice(p, token, logits, ids[lane], lane);
 }
 
 // ------------------------------------------------------------------ experts
