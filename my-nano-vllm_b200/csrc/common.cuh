@@ -261,19 +261,26 @@ __device__ __forceinline__ float rcp(float x) {
 }
 
 // The scale of a quantised group, a / 448 for its largest magnitude a (1 for an all-zero group), and the
-// group's values divided by it.
+// group's values divided by it; both quotients rounded to nearest (the values' within 2^-30 more of half
+// an ulp).
 template <int N>
 __device__ __forceinline__ float divide_by_scale(float (&v)[N], float a) {
   if (a > 1.0e-30f && a < INFINITY) {
-    // a / 448 rounded to nearest: a product with the rounded 1 / 448 and one correction by the exact
-    // remainder (Markstein); v / scale as v times 1 / scale, two ulps from the quotient at most
+    // a / 448: a product with the rounded 1 / 448 and one correction by the exact remainder (Markstein).
+    // v / scale: 1 / scale as the approximate inverse and what it lacks, so that only the last addition
+    // rounds.  Values times the approximate inverse alone are up to 2.5 ulps off and fall on the other side of
+    // a midpoint between e4m3 values a fifth more often (8192 x 12288 SiLU: 79.4 us, 79.9 with what it lacks,
+    // 84.7 with a remainder for each value).
     const float k = 1.0f / 448.0f, q = a * k;
     const float scale = fmaf(fmaf(-448.0f, q, a), k, q);
-    const float inv = rcp(scale);
+    const float near = rcp(scale), rest = fmaf(-scale, near, 1.0f) * near;  // 1 / scale = near + rest
+    const uint64_t near2 = f2_pack(near, near), rest2 = f2_pack(rest, rest);
     static_assert(N % 2 == 0, "pairs");
 #pragma unroll
-    for (int i = 0; i < N; i += 2)
-      f2_unpack(f2_mul(f2_pack(v[i], v[i + 1]), f2_pack(inv, inv)), v[i], v[i + 1]);
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t x = f2_pack(v[i], v[i + 1]);
+      f2_unpack(f2_fma(x, near2, f2_mul(x, rest2)), v[i], v[i + 1]);
+    }
     return scale;
   }
   // where remainders and inverses leave fp32's range, and infinity
