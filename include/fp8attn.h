@@ -273,8 +273,9 @@ FP8ATTN_API int fp8attn_fp8_tp_linear(const void* x, int64_t x_row_stride, const
  *     q [M, K], scale [M, K / 128]; residual_out [M, K]: s rounded to dtype (given exactly when
  *     residual is; may be the residual itself where its rows are K apart); norm_out [M, K]: y rounded
  *     to dtype, or NULL.
- *   fp8attn_silu_mul_quant: y = g / (1 + exp(-g)) * u.  gate_up [M, 2 I]: g's columns, then u's; I a
- *     multiple of 128 up to 2^20.  q [M, I], scale [M, I / 128].
+ *   fp8attn_silu_mul_quant: y = g / (1 + exp(-g)) * u, 0 for a finite u where exp(-g) passes fp32's range
+ *     (g below -88.7).  gate_up [M, 2 I]: g's columns, then u's; I a multiple of 128 up to 2^20.
+ *     q [M, I], scale [M, I / 128].
  */
 #define FP8ATTN_BF16 0
 #define FP8ATTN_FP16 1
@@ -288,10 +289,9 @@ FP8ATTN_API int fp8attn_silu_mul_quant(const void* gate_up, int64_t row_stride, 
  * A mixture-of-experts layer for a few tokens, weights in the format of fp8attn_fp8_block_linear (no
  * counterpart in the reference, whose model is dense).  Per token: l = x . router^T; p = softmax(l);
  * the top_k largest p (as l summed in fp64 orders them; ties: the lower expert first; a NaN is chosen
- * last) with weights c = p, divided
- * by their sum if renormalize; for each chosen expert e: g, u = the halves of xq . w13[e]^T,
- * h = g / (1 + exp(-g)) * u quantised as above, y_e = hq . w2[e]^T (block-scaled products as in
- * fp8attn_fp8_block_gemm); out = bf16(sum of c_e y_e, in the order chosen).
+ * last) with weights c = p, divided by their sum if renormalize; for each chosen expert e: g, u = the
+ * halves of xq . w13[e]^T, h = g / (1 + exp(-g)) * u quantised as above, y_e = hq . w2[e]^T (block-scaled
+ * products as in fp8attn_fp8_block_gemm); out = bf16(sum of c_e y_e, in the order chosen).
  *   x bf16 [T, H] and its quantised form xq e4m3 [T, H], x_scale bf16 [T, H / 128] (contiguous), as
  *     fp8attn_add_rms_norm_quant or fp8attn_fp8_dyn_quant leave them; router bf16 [E, H];
  *     w13 e4m3 [E, 2 I, H] (gate rows, then up rows), w13_scale bf16 [E, 2 I / 128, H / 128];

@@ -291,12 +291,13 @@ __device__ __forceinline__ float divide_by_scale(float (&v)[N], float a) {
   return scale;
 }
 
-// g / (1 + e^-g) of two values.  e^-g = 2^(-g log2 e): the product's rounding error, which the power
-// would multiply by |g|, is recovered by a fused multiply-add (error-free product) and applied to first
-// order, 2^(t + d) = 2^t (1 + d ln 2).  g is held below 200, where e^-g is 0, so that the product does not
-// overflow; where it overflows below, 1 + e^-g is infinite either way.
+// g / (1 + e^-g) of two values; 0 where e^-g passes fp32's range (g below -88.7).  e^-g = 2^(-g log2 e): the
+// product's rounding error, which the power would multiply by |g|, is recovered by a fused multiply-add
+// (error-free product) and applied to first order, 2^(t + d) = 2^t (1 + d ln 2).  g is held below 200,
+// where e^-g is 0, so that the product does not overflow; where it overflows below, 1 + e^-g is infinite
+// either way.  All over four: the inverse of more than 2^126 would be below fp32's normal numbers, and 0.
 __device__ __forceinline__ uint64_t silu2(uint64_t g) {
-  const float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+  const float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f, kQuarter = 0.25f;
   // log2 e - float(log2 e)
   const float kLog2eRest = static_cast<float>(1.44269504088896340736 - 1.44269502162933349609375);
   float g0, g1;
@@ -307,10 +308,11 @@ __device__ __forceinline__ uint64_t silu2(uint64_t g) {
   const uint64_t d = f2_fma(c, f2_pack(-kLog2eRest, -kLog2eRest), rest);
   float t0, t1;
   f2_unpack(t, t0, t1);
-  const uint64_t e = f2_mul(f2_pack(ex2(-t0), ex2(-t1)), f2_fma(d, f2_pack(kLn2, kLn2), f2_pack(1.f, 1.f)));
+  const uint64_t quarter = f2_pack(kQuarter, kQuarter);
+  const uint64_t e = f2_mul(f2_pack(ex2(-t0), ex2(-t1)), f2_fma(d, f2_pack(kLn2 * kQuarter, kLn2 * kQuarter), quarter));
   float q0, q1;
-  f2_unpack(f2_add(e, f2_pack(1.f, 1.f)), q0, q1);
-  return f2_mul(g, f2_pack(rcp(q0), rcp(q1)));
+  f2_unpack(f2_add(e, quarter), q0, q1);
+  return f2_mul(f2_mul(g, quarter), f2_pack(rcp(q0), rcp(q1)));
 }
 
 // fp32 -> fp16 -> bf16, the reference output path (.to(tl.float16) stored into bf16).
