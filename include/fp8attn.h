@@ -323,9 +323,14 @@ FP8ATTN_API int fp8attn_fp8_moe(const void* x, int64_t x_row_stride, const void*
  *     and wait on an mbarrier that nothing arrives on, with the library's bounded wait given a
  *     limit of limit_ns: every wait must give up, record 1 (wait timed out) in the error word and
  *     let the launch finish with [1] and [2] back at zero.
+ *   fp8attn_diag_counter_wait: one warp, lane l on the device int32 counters[l], waits until all are at least
+ *     `want`, for limit_ns at most; reached[l] (device int32) = 1 in every lane, or 0 in every lane with 1
+ *     (wait timed out) recorded in *error (device int32, or NULL).  32 counters and 32 results.
  *   fp8attn_diag_exp2: poly[i] = the prefill softmax's FMA-pipe 2^x(i), mufu[i] = ex2.approx(x[i]).
  */
 FP8ATTN_API int fp8attn_diag_wait_timeout(void* workspace, int64_t limit_ns, int num_ctas, void* stream);
+FP8ATTN_API int fp8attn_diag_counter_wait(const int32_t* counters, int want, int64_t limit_ns,
+                   int32_t* reached, int32_t* error, void* stream);
 FP8ATTN_API int fp8attn_diag_exp2(const float* x, float* poly, float* mufu, int64_t n, void* stream);
 
 #ifdef __cplusplus

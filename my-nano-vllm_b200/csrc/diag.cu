@@ -4,6 +4,9 @@
 //                              nothing ever arrives on: the wait must give up after its limit,
 //                              record kDevErrWaitTimeout in the error word and let the launch end
 //                              with the control block's work counters back at zero;
+//   fp8attn_diag_counter_wait  the bounded wait on a counter in global memory that the mixture of experts
+//                              uses (moe.cu), on counters that the caller sets: it ends by itself
+//                              whether they reach the value or not, with the same answer in every lane;
 //   fp8attn_diag_exp2          the FMA-pipe exp2 of the prefill softmax (exp2_poly_x2) next to
 //                              the MUFU ex2.approx, element by element.
 #include "../../include/fp8attn.h"
@@ -58,6 +61,15 @@ int fp8attn_diag_wait_timeout(void* workspace, int64_t limit_ns, int num_ctas, v
                                  static_cast<cudaStream_t>(stream)>>>(
       static_cast<int*>(workspace), static_cast<unsigned long long>(limit_ns));
   return cudaGetLastError() == cudaSuccess ? FP8ATTN_OK : FP8ATTN_ECUDA;
+}
+
+int fp8attn_diag_counter_wait(const int32_t* counters, int want, int64_t limit_ns, int32_t* reached,
+                              int32_t* error, void* stream) {
+  if (counters == nullptr || reached == nullptr || limit_ns < 0) return FP8ATTN_EINVAL;
+  return fp8attn::launch_counter_wait(counters, want, static_cast<unsigned long long>(limit_ns), reached, error,
+                                      static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? FP8ATTN_OK
+             : FP8ATTN_ECUDA;
 }
 
 int fp8attn_diag_exp2(const float* x, float* poly, float* mufu, int64_t n, void* stream) {

@@ -177,6 +177,9 @@ struct MoeParams {
 // Lays the workspace out (pointers set where `workspace` is not null); returns its bytes.
 int64_t moe_layout(MoeParams& p, void* workspace, int num_sms);
 cudaError_t launch_moe(const MoeParams& p, int num_sms, cudaStream_t stream);
+// Its wait on a counter in global memory, by itself: 32 counters, a lane each.
+cudaError_t launch_counter_wait(const int* counters, int want, unsigned long long limit_ns, int* reached, int* err,
+                                cudaStream_t stream);
 
 // ------------------------------------------------------------------ decode engine
 // Control block at the head of the decode workspace (ints):

@@ -490,12 +490,13 @@ __device__ __forceinline__ void tma_load_once(void* dst, const CUtensorMap* map,
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
       : "memory");
 }
-// A warp's wait until *p >= want; gives up after kWaitLimitNs, recording kDevErrWaitTimeout.  Lane 0
+// A warp's wait until *p >= want; gives up after limit_ns, recording kDevErrWaitTimeout.  Lane 0
 // decides for all.
 __device__ __forceinline__ bool counter_reached(const int* p, int want) {
   return __shfl_sync(0xffffffffu, load_acquire(p), 0) >= want;
 }
-__device__ __noinline__ bool wait_counter(const int* p, int want, int* err) {
+__device__ __noinline__ bool wait_counter(const int* p, int want, int* err,
+                                          unsigned long long limit_ns = kWaitLimitNs) {
   unsigned long long t0 = 0;
   for (uint32_t polls = 1;; ++polls) {
     if (counter_reached(p, want)) return true;
@@ -503,12 +504,18 @@ __device__ __noinline__ bool wait_counter(const int* p, int want, int* err) {
       const unsigned long long now = __shfl_sync(0xffffffffu, globaltimer_ns(), 0);
       if (t0 == 0) {
         t0 = now;
-      } else if (now - t0 > kWaitLimitNs) {
+      } else if (now - t0 > limit_ns) {
         if (err) atomicExch(err, kDevErrWaitTimeout);
         return false;
       }
     }
   }
+}
+
+// The wait by itself: lane l of one warp on counters[l].
+__global__ void __launch_bounds__(32)
+    counter_wait_kernel(const int* counters, int want, unsigned long long limit_ns, int* reached, int* err) {
+  reached[threadIdx.x] = wait_counter(counters + threadIdx.x, want, err, limit_ns) ? 1 : 0;
 }
 
 // Slots sorted by expert (stable: results must not depend on timing), the tiles, and the two phases'
@@ -1286,6 +1293,12 @@ cudaError_t launch_router(const MoeParams& p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+cudaError_t launch_counter_wait(const int* counters, int want, unsigned long long limit_ns, int* reached, int* err,
+                                cudaStream_t stream) {
+  counter_wait_kernel<<<1, 32, 0, stream>>>(counters, want, limit_ns, reached, err);
+  return cudaGetLastError();
+}
 
 int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
   uint8_t* const base = static_cast<uint8_t*>(workspace);

@@ -82,6 +82,8 @@ def _load() -> ctypes.CDLL:
                                     i32, i32, i32, i32, i32, vp, i64, vp, vp]
     lib.fp8attn_diag_wait_timeout.restype = i32
     lib.fp8attn_diag_wait_timeout.argtypes = [vp, i64, i32, vp]
+    lib.fp8attn_diag_counter_wait.restype = i32
+    lib.fp8attn_diag_counter_wait.argtypes = [vp, i32, i64, vp, vp, vp]
     lib.fp8attn_diag_exp2.restype = i32
     lib.fp8attn_diag_exp2.argtypes = [vp, vp, vp, i64, vp]
     lib.fp8attn_qk_norm_rope_store.restype = i32
