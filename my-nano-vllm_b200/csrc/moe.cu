@@ -490,10 +490,10 @@ __device__ __forceinline__ void tma_load_once(void* dst, const CUtensorMap* map,
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
       : "memory");
 }
-// A warp's wait until *p >= want; gives up after limit_ns, recording kDevErrWaitTimeout.  Lane 0
-// decides for all.
+// A warp's wait until *p >= want; gives up after limit_ns, recording kDevErrWaitTimeout.  Every lane has to
+// have read the value: what it reads next is ordered by its own acquire (a shuffle orders no memory).
 __device__ __forceinline__ bool counter_reached(const int* p, int want) {
-  return __shfl_sync(0xffffffffu, load_acquire(p), 0) >= want;
+  return __all_sync(0xffffffffu, load_acquire(p) >= want);
 }
 __device__ __noinline__ bool wait_counter(const int* p, int want, int* err,
                                           unsigned long long limit_ns = kWaitLimitNs) {

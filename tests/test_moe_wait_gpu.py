@@ -41,3 +41,13 @@ def test_refusals():
     assert wait(None, 1, 10, 4096, 0, None) == _lib.EINVAL
     assert wait(4096, 1, 10, None, 0, None) == _lib.EINVAL
     assert wait(4096, 1, -1, 4096, 0, None) == _lib.EINVAL
+
+
+@pytest.mark.parametrize("lane", [0, 1, 5, 31])
+def test_every_lane_decides_by_the_value_that_it_read_itself(lane):
+    """What a lane reads after the wait is ordered by its own reading of the counter, so one lane that
+    has not seen the value keeps the warp waiting."""
+    counters = torch.full((32,), 9, dtype=torch.int32, device="cuda")
+    counters[lane] = 6
+    reached, error, _ = _wait(counters, 7)
+    assert reached == [0] * 32 and error == 1
