@@ -306,7 +306,10 @@ FP8ATTN_API int fp8attn_silu_mul_quant(const void* gate_up, int64_t row_stride, 
  *     aligned; its contents need not be initialised and are not kept.  One workspace must not serve
  *     two calls that can overlap.
  *   error: device int32 (4-byte aligned) that a bounded device wait which gives up sets to 1 (see
- *     fp8attn_read_error, which takes it for a workspace's word), or NULL.
+ *     fp8attn_read_error, which takes it for a workspace's word), or NULL: the library's own word on the
+ *     current device, which starts at 0 and stays where it is, also for captured launches.
+ *   fp8attn_fp8_moe_read_error: the library's word, copied into *dst (host or device memory) in stream
+ *     order; clear != 0 zeroes it after the copy.  Not during a stream capture.
  */
 FP8ATTN_API int64_t fp8attn_fp8_moe_workspace_bytes(int64_t T, int H, int I, int E, int top_k);
 FP8ATTN_API int fp8attn_fp8_moe(const void* x, int64_t x_row_stride, const void* xq,
@@ -315,6 +318,7 @@ FP8ATTN_API int fp8attn_fp8_moe(const void* x, int64_t x_row_stride, const void*
                    int64_t out_row_stride, float* topk_weights, int32_t* topk_ids, int64_t T, int H,
                    int I, int E, int top_k, int renormalize, void* workspace,
                    int64_t workspace_bytes, int32_t* error, void* stream);
+FP8ATTN_API int fp8attn_fp8_moe_read_error(int32_t* dst, int clear, void* stream);
 
 /*
  * Self-checks of device-side mechanisms (no counterpart in the reference; used by the tests).
@@ -325,7 +329,8 @@ FP8ATTN_API int fp8attn_fp8_moe(const void* x, int64_t x_row_stride, const void*
  *     let the launch finish with [1] and [2] back at zero.
  *   fp8attn_diag_counter_wait: one warp, lane l on the device int32 counters[l], waits until all are at least
  *     `want`, for limit_ns at most; reached[l] (device int32) = 1 in every lane, or 0 in every lane with 1
- *     (wait timed out) recorded in *error (device int32, or NULL).  32 counters and 32 results.
+ *     (wait timed out) recorded in *error (device int32, or NULL: as fp8attn_fp8_moe).  32 counters and
+ *     32 results.
  *   fp8attn_diag_exp2: poly[i] = the prefill softmax's FMA-pipe 2^x(i), mufu[i] = ex2.approx(x[i]).
  */
 FP8ATTN_API int fp8attn_diag_wait_timeout(void* workspace, int64_t limit_ns, int num_ctas, void* stream);

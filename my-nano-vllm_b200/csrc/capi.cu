@@ -989,4 +989,12 @@ int fp8attn_fp8_moe(const void* x, int64_t x_row_stride, const void* xq, int64_t
   return e == cudaSuccess ? FP8ATTN_OK : cuda_fail(e, "moe launch");
 }
 
+int fp8attn_fp8_moe_read_error(int32_t* dst, int clear, void* stream) {
+  if (dst == nullptr) return fail(FP8ATTN_EINVAL, "null destination");
+  void* word = nullptr;
+  const cudaError_t e = fp8attn::moe_error_word(&word);
+  if (e != cudaSuccess) return cuda_fail(e, "moe error word");
+  return fp8attn_read_error(static_cast<uint8_t*>(word) - FP8ATTN_WS_ERROR_OFFSET, dst, clear, stream);
+}
+
 }  // extern "C"

@@ -164,7 +164,7 @@ struct MoeParams {
   float* weights;  // [T, top_k]
   int64_t T;
   int H, I, E, top_k, renormalize;
-  int* err;  // device error word, or null
+  int* err;  // device error word, or null: moe_error_word's
   // workspace
   int* counters;      // see moe_layout
   int64_t num_counters;
@@ -177,6 +177,8 @@ struct MoeParams {
 // Lays the workspace out (pointers set where `workspace` is not null); returns its bytes.
 int64_t moe_layout(MoeParams& p, void* workspace, int num_sms);
 cudaError_t launch_moe(const MoeParams& p, int num_sms, cudaStream_t stream);
+// The error word, on the current device, of launches that bring none.
+cudaError_t moe_error_word(void** word);
 // Its wait on a counter in global memory, by itself: 32 counters, a lane each.
 cudaError_t launch_counter_wait(const int* counters, int want, unsigned long long limit_ns, int* reached, int* err,
                                 cudaStream_t stream);

@@ -42,9 +42,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+// The error word of calls that bring none.  It lives as long as the library's module, so launches in captured
+// graphs may hold it, and it needs no scratch that a call would have to clear.
+__device__ int g_error = 0;
+__device__ __forceinline__ int* error_word(int* err) { return err != nullptr ? err : &g_error; }
+
 // mbar_wait with its polling loop out of line: the roles' loops stay small (1 % of the layer's time).
 __device__ __noinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, int* err) {
-  return mbar_wait(bar, parity, err);
+  return mbar_wait(bar, parity, error_word(err));
 }
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int* err) {
   return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, err);
@@ -505,7 +510,7 @@ __device__ __noinline__ bool wait_counter(const int* p, int want, int* err,
       if (t0 == 0) {
         t0 = now;
       } else if (now - t0 > limit_ns) {
-        if (err) atomicExch(err, kDevErrWaitTimeout);
+        atomicExch(error_word(err), kDevErrWaitTimeout);
         return false;
       }
     }
@@ -1299,6 +1304,8 @@ cudaError_t launch_counter_wait(const int* counters, int want, unsigned long lon
   counter_wait_kernel<<<1, 32, 0, stream>>>(counters, want, limit_ns, reached, err);
   return cudaGetLastError();
 }
+
+cudaError_t moe_error_word(void** word) { return cudaGetSymbolAddress(word, g_error); }
 
 int64_t moe_layout(MoeParams& p, void* workspace, int num_sms) {
   uint8_t* const base = static_cast<uint8_t*>(workspace);

@@ -80,6 +80,8 @@ def _load() -> ctypes.CDLL:
     lib.fp8attn_fp8_moe.restype = i32
     lib.fp8attn_fp8_moe.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp, vp, i64,
                                     i32, i32, i32, i32, i32, vp, i64, vp, vp]
+    lib.fp8attn_fp8_moe_read_error.restype = i32
+    lib.fp8attn_fp8_moe_read_error.argtypes = [vp, i32, vp]
     lib.fp8attn_diag_wait_timeout.restype = i32
     lib.fp8attn_diag_wait_timeout.argtypes = [vp, i64, i32, vp]
     lib.fp8attn_diag_counter_wait.restype = i32

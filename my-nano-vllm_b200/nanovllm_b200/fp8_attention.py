@@ -16,6 +16,7 @@ import torch
 from . import _lib
 
 _WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
+_MOE_DEVICES: set[int] = set()  # where fp8_moe has run: it has an error word of the library's own
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -32,12 +33,18 @@ def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
 
 
 def device_error(device: torch.device | None = None) -> int:
-    """Largest device-side error word over the workspaces of ``device`` (0 = none).  Reads device
-    memory: for tests and diagnostics only."""
+    """Largest device-side error word over the workspaces of ``device`` and its mixture-of-experts calls
+    (0 = none).  Reads device memory: for tests and diagnostics only."""
     worst = 0
     for (dev, _), ws in _WORKSPACES.items():
         if device is None or dev == torch.device(device).index:
             worst = max(worst, int(ws[:4].view(torch.int32).item()))
+    for dev in sorted(_MOE_DEVICES):
+        if device is None or dev == torch.device(device).index:
+            with torch.cuda.device(dev):
+                word = torch.empty(1, dtype=torch.int32, device=dev)
+                _lib.check(_lib.lib.fp8attn_fp8_moe_read_error(word.data_ptr(), 0, _stream(word.device)))
+                worst = max(worst, int(word.item()))
     return worst
 
 

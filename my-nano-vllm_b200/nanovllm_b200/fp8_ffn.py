@@ -20,7 +20,8 @@ and a mixture of experts:
     x = fp8_moe(y, xq, xs, router_weight, gate_up_weight, gate_up_scale, down_weight, down_scale, 8)
 
 All launch on ``torch.cuda.current_stream()`` of the tensors' device, allocate outputs and scratch
-with ``torch.empty`` and never synchronise, so they can be captured into CUDA graphs.
+with ``torch.empty`` and never synchronise, so they can be captured into CUDA graphs.  A device wait of
+``fp8_moe`` that gives up is recorded in a word of the library's own (``fp8_attention.device_error``).
 """
 from __future__ import annotations
 
@@ -29,7 +30,7 @@ import functools
 import torch
 
 from . import _lib
-from .fp8_attention import _WORKSPACES, workspace
+from .fp8_attention import _MOE_DEVICES
 from .fp8_linear import BLOCK_SIZE
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
@@ -126,14 +127,6 @@ def _moe_scratch_bytes(device: int, T: int, H: int, I: int, E: int, top_k: int) 
     return _lib.lib.fp8attn_fp8_moe_workspace_bytes(T, H, I, E, top_k)
 
 
-def _error_word(device: int) -> int:
-    """Address of the device error word of the current stream's workspace (``device_error``)."""
-    ws = _WORKSPACES.get((device, _raw_stream(device)))
-    if ws is None:
-        ws = workspace(torch.device("cuda", device), 4)
-    return ws.data_ptr() + _lib.WS_ERROR_OFFSET
-
-
 def _check_experts(w: torch.Tensor, scale: torch.Tensor, device: int, e: int, n: int, k: int):
     assert w.get_device() == device and w.dtype == _E4M3 and w.is_contiguous()
     assert scale.get_device() == device and scale.dtype == _BF16 and scale.is_contiguous()
@@ -184,6 +177,7 @@ def fp8_moe(x: torch.Tensor, xq: torch.Tensor, x_scale: torch.Tensor, router_wei
         ids = _empty((T, top_k), (top_k, 1), dtype=torch.int32, device=dev)
         weights_out, ids_out = weights.data_ptr(), ids.data_ptr()
     if T > 0:
+        _MOE_DEVICES.add(device)
         nbytes = _moe_scratch_bytes(device, T, H, I, E, top_k)
         # scratch of this call alone: calls on other streams and captured graphs share none
         scratch = _empty((max(nbytes, 0),), (1,), dtype=torch.uint8, device=dev)
@@ -192,8 +186,7 @@ def fp8_moe(x: torch.Tensor, xq: torch.Tensor, x_scale: torch.Tensor, router_wei
                   xq.stride(0) if T > 1 else H, x_scale.data_ptr(), router_weight.data_ptr(),
                   gate_up_weight.data_ptr(), gate_up_scale.data_ptr(), down_weight.data_ptr(),
                   down_scale.data_ptr(), out.data_ptr(), H, weights_out, ids_out, T, H, I, E, top_k,
-                  1 if renormalize else 0, scratch.data_ptr(), nbytes, _error_word(device),
-                  _raw_stream(device))
+                  1 if renormalize else 0, scratch.data_ptr(), nbytes, 0, _raw_stream(device))
         if rc:
             _lib.check(rc)
     return (out, weights, ids) if return_router else out
