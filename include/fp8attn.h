@@ -190,6 +190,15 @@ FP8ATTN_API int fp8attn_noalloc_read_error(int32_t* dst, int clear, void* stream
  * hot path; clear != 0 zeroes it after the copy.  Diagnostics: no counterpart in the reference. */
 FP8ATTN_API int fp8attn_read_error(const void* workspace, int32_t* dst, int clear, void* stream);
 
+/* For hosts that keep workspaces across calls.  A workspace that captured launches use has to outlive
+ * their graph, to be zeroed before its first replay and outside of it, and to serve no other graph that may
+ * run at the same time.
+ *   fp8attn_capture_id: *id = a number of its own for the capture that `stream` is in, 0 outside captures.
+ *   fp8attn_exchange_capture_mode: cudaThreadExchangeStreamCaptureMode (0 global, 1 thread-local, 2 relaxed:
+ *     the thread may allocate while it captures); *mode is replaced by the mode before. */
+FP8ATTN_API int fp8attn_capture_id(void* stream, uint64_t* id);
+FP8ATTN_API int fp8attn_exchange_capture_mode(int* mode);
+
 /* Tuning knob (process-wide, atomic): minimum key positions per split-KV work item, a multiple of
  * 128 (default 128).  Returns the previous value; other values are rejected with -1.  Calls that
  * are already launched keep the value they were planned with. */

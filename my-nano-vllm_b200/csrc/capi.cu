@@ -344,6 +344,25 @@ int fp8attn_read_error(const void* workspace, int32_t* dst, int clear, void* str
   return FP8ATTN_OK;
 }
 
+int fp8attn_capture_id(void* stream, uint64_t* id) {
+  if (id == nullptr) return fail(FP8ATTN_EINVAL, "null destination");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long unique = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &unique);
+  if (e != cudaSuccess) return cuda_fail(e, "capture info");
+  *id = status == cudaStreamCaptureStatusActive ? unique : 0;
+  return FP8ATTN_OK;
+}
+
+int fp8attn_exchange_capture_mode(int* mode) {
+  if (mode == nullptr || *mode < 0 || *mode > 2) return fail(FP8ATTN_EINVAL, "capture mode must be 0, 1 or 2");
+  cudaStreamCaptureMode m = static_cast<cudaStreamCaptureMode>(*mode);
+  const cudaError_t e = cudaThreadExchangeStreamCaptureMode(&m);
+  if (e != cudaSuccess) return cuda_fail(e, "capture mode");
+  *mode = static_cast<int>(m);
+  return FP8ATTN_OK;
+}
+
 int fp8attn_decode(void* out, const void* q, int64_t q_row_stride, const void* k_cache,
                    const void* v_cache, const float* k_scale, const float* v_scale,
                    const int32_t* block_tables, int64_t block_tables_stride, int max_num_blocks,

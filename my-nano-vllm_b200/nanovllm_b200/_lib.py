@@ -51,6 +51,10 @@ def _load() -> ctypes.CDLL:
                                            i32, i32, i64, i32, f32, vp]
     lib.fp8attn_read_error.restype = i32
     lib.fp8attn_read_error.argtypes = [vp, vp, i32, vp]
+    lib.fp8attn_capture_id.restype = i32
+    lib.fp8attn_capture_id.argtypes = [vp, vp]
+    lib.fp8attn_exchange_capture_mode.restype = i32
+    lib.fp8attn_exchange_capture_mode.argtypes = [vp]
     lib.fp8attn_noalloc_read_error.restype = i32
     lib.fp8attn_noalloc_read_error.argtypes = [vp, i32, vp]
     lib.fp8attn_fp8_gemm_workspace_bytes.restype = i64

@@ -11,24 +11,66 @@ cache format; ``None`` is the reference's unit-scale cache.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
 
-_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
+_WORKSPACES: dict[tuple[int, int, int], torch.Tensor] = {}  # by device, stream, capture (0: none)
+_REPLACED: list[tuple[int, torch.Tensor]] = []  # that captured launches still hold, by device
 _MOE_DEVICES: set[int] = set()  # where fp8_moe has run: it has an error word of the library's own
+_RELAXED = 2  # cudaStreamCaptureModeRelaxed
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Zero-initialised scratch for the current stream of ``device`` (grown on demand).  The
-    kernels leave its counters at zero after every call, so it is reused without clearing."""
+    kernels leave its counters at zero after every call, so it is reused without clearing.  Every
+    capture has its own, kept for good: its graph may be replayed at any time, beside others."""
     stream = torch.cuda.current_stream(device)
-    key = (device.index if device.index is not None else torch.cuda.current_device(),
-           stream.cuda_stream)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    capture = 0
+    if index != torch.cuda.current_device() or torch.cuda.is_current_stream_capturing():
+        capture = _capture_id(stream)
+    key = (index, stream.cuda_stream, capture)
     ws = _WORKSPACES.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+        nbytes = max(nbytes, 1 << 16)
+        if capture:
+            if ws is not None:
+                _REPLACED.append((index, ws))
+            ws = _zeros_beside_capture(index, nbytes)
+        else:
+            new = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            if ws is not None:
+                new[:4].copy_(ws[:4])  # an error that nobody has read yet
+            ws = new
         _WORKSPACES[key] = ws
+    return ws
+
+
+def _capture_id(stream: torch.cuda.Stream) -> int:
+    number = ctypes.c_uint64(0)
+    _lib.check(_lib.lib.fp8attn_capture_id(stream.cuda_stream, ctypes.byref(number)))
+    return number.value
+
+
+def _zeros_beside_capture(index: int, nbytes: int) -> torch.Tensor:
+    """Zeros that are there before the graph under capture is first replayed, and not of its memory
+    pool: neither its replays nor those of graphs that share the pool write to them, so the error
+    word keeps its value.  Allocated and cleared on a stream that does not capture."""
+    mode = ctypes.c_int(_RELAXED)
+    _lib.check(_lib.lib.fp8attn_exchange_capture_mode(ctypes.byref(mode)))
+    try:
+        for _ in range(64):  # streams come from a pool, which may hand out one that captures
+            side = torch.cuda.Stream(index)
+            if _capture_id(side) == 0:
+                break
+        with torch.cuda.stream(side):
+            ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        side.synchronize()
+    finally:
+        _lib.check(_lib.lib.fp8attn_exchange_capture_mode(ctypes.byref(mode)))
     return ws
 
 
@@ -36,7 +78,7 @@ def device_error(device: torch.device | None = None) -> int:
     """Largest device-side error word over the workspaces of ``device`` and its mixture-of-experts calls
     (0 = none).  Reads device memory: for tests and diagnostics only."""
     worst = 0
-    for (dev, _), ws in _WORKSPACES.items():
+    for dev, ws in [(key[0], ws) for key, ws in _WORKSPACES.items()] + _REPLACED:
         if device is None or dev == torch.device(device).index:
             worst = max(worst, int(ws[:4].view(torch.int32).item()))
     for dev in sorted(_MOE_DEVICES):
