@@ -104,13 +104,32 @@ def route(x, router, top_k, renormalize):
     return (c / c.sum(-1, keepdim=True) if renormalize else c), order
 
 
+def router_halves(c):
+    """The columns of each of the two products that the router chains, of the 32 from c on."""
+    return [[c + i for i in range(32) if i % 8 < 4], [c + i for i in range(32) if i % 8 >= 4]]
+
+
 def route_rel(x, router):
-    """[T, 1]: how far, relatively, the router's weights may be off.  A logit is a sum of fp32 sums of 32
-    products, 32 additions of at most 2^-23 of their absolute terms each (tensor cores truncate), and
-    one rounding to fp32; a weight is a ratio of exponentials of differences of logits: twice a logit's
-    error, and a few ulps of the exponentials and the fp32 sums of up to 512 of them."""
-    terms = (x.double().abs() @ router.double().abs().t()).amax(-1, keepdim=True)
-    return 2 * terms * (32 * 2.0 ** -23 + 2.0 ** -24) + 2.0 ** -19
+    """[T, 1]: how far, relatively, the router's weights may be off.
+
+    A logit is an fp64 sum over groups of 32 columns, rounded to fp32 once (2^-24 of it); a group is two
+    tensor-core sums of 16 products, one on top of the other.  Such a sum truncates at 2^-23 of the
+    largest of its terms and partial sums, m.  Rounding errors of different groups have the signs of
+    different sums, so they add up as squares; eight times that, two sums a group and a factor of four.
+    (The worst case, 32 additions of 2^-23 of a group's absolute terms, all of one sign, is used where
+    it is smaller.)  A weight is a ratio of exponentials of differences of logits: twice a logit's
+    error, the rounded difference, and a few ulps of the exponentials and the fp32 sums of up to 512 of them."""
+    x, router = x.double(), router.double()
+    logits, squares = x.new_zeros(x.shape[0], router.shape[0]), x.new_zeros(x.shape[0], router.shape[0])
+    for c in range(0, x.shape[1], 32):
+        a, b = [x[:, half] @ router[:, half].t() for half in router_halves(c)]
+        term = (x[:, None, c:c + 32] * router[None, :, c:c + 32]).abs().amax(-1)
+        squares += torch.maximum(term, torch.maximum(a.abs(), (a + b).abs())).square()
+        logits += a + b
+    worst = (x.abs() @ router.abs().t()) * 32 * 2.0 ** -23
+    off = torch.minimum(8 * 2.0 ** -23 * squares.sqrt(), worst) + logits.abs() * 2.0 ** -24
+    spread_ = (logits.amax(-1) - logits.amin(-1))[:, None]
+    return 2 * off.amax(-1, keepdim=True) + spread_ * 2.0 ** -24 + 2.0 ** -19
 
 
 def moe(x, xq, x_scale, router, w13, w13_scale, w2, w2_scale, top_k, renormalize):
