@@ -1,5 +1,9 @@
 """Workspaces that captured graphs use (nanovllm_b200.fp8_attention.workspace): every graph has its own, zero
 before the first replay, outside the graph's memory pool, and for good; and a recorded error stays."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -137,3 +141,26 @@ def test_an_error_outlives_a_replaced_workspace():
         larger[:4].zero_()
     torch.cuda.synchronize()
     assert fp8_attention.device_error(DEVICE) == 0
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing has run before: the workspace's stream and memory are made during the capture."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = (
+        "import sys; sys.path[:0] = ['.', 'my-nano-vllm_b200']\n"
+        "import torch\n"
+        "from nanovllm_b200 import fp8_attention, fp8_decode_attention, workloads\n"
+        "c = workloads.decode_case(5, 32, 8, 1, 700, seed=1, device='cuda', block_size=64)\n"
+        "call = lambda: fp8_decode_attention(c.q, c.k_cache, c.v_cache, c.block_tables, c.context_lens, c.scale)\n"
+        "torch.cuda.synchronize()\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    out = call()\n"
+        "for _ in range(3):\n"
+        "    out.zero_(); g.replay(); torch.cuda.synchronize()\n"
+        "    got = out.clone()\n"
+        "assert torch.equal(got, call())\n"
+        "assert fp8_attention.device_error() == 0\n"
+        "print('captured first')\n")
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured first" in run.stdout, run.stderr[-2000:]
