@@ -315,20 +315,27 @@ __global__ void __cluster_dims__(kRouterCluster, 1, 1) __launch_bounds__(kRouter
   __syncthreads();
   const int n = num_open;
   if (n == 0) return;
-  // exact sums for the open ones; this CTA's `part` is free and no other CTA's business
+  // exact sums for the open ones, a warp's share of each at a time; this CTA's `part` is free and no other
+  // CTA's business
+  constexpr int kSums = 64;  // experts between two barriers
   double* const exact = &part[0][0][0];  // of every expert
   double* const sums = exact + kMoeMaxExperts;
-  static_assert(sizeof(part) >= (kMoeMaxExperts + kRouterWarps) * sizeof(double), "exact");
+  static_assert(sizeof(part) >= (kMoeMaxExperts + kSums * kRouterWarps) * sizeof(double), "exact");
   for (int e = threadIdx.x; e < p.E; e += kRouterThreads) exact[e] = logits[e];
-  for (int i = 0; i < n; ++i) {
-    const double mine = exact_part(p.x + token * p.x_row_stride, p.router + static_cast<int64_t>(open[i]) * p.H, p.H);
-    if (lane == 0) sums[warp] = mine;
+  for (int i0 = 0; i0 < n; i0 += kSums) {
+    const int some = min(kSums, n - i0);
+    for (int i = 0; i < some; ++i) {
+      const double mine =
+          exact_part(p.x + token * p.x_row_stride, p.router + static_cast<int64_t>(open[i0 + i]) * p.H, p.H);
+      if (lane == 0) sums[i * kRouterWarps + warp] = mine;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < some) {
       double sum = 0.0;
-      for (int k = 0; k < kRouterWarps; ++k) sum += sums[k];
-      exact[open[i]] = sum;
-      logits[open[i]] = static_cast<float>(sum);
+#pragma unroll
+      for (int k = 0; k < kRouterWarps; ++k) sum += sums[threadIdx.x * kRouterWarps + k];
+      exact[open[i0 + threadIdx.x]] = sum;
+      logits[open[i0 + threadIdx.x]] = static_cast<float>(sum);
     }
     __syncthreads();
   }
