@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) add_rms_norm_quant_kernel(
 }
 
 // ------------------------------------------------------------------ SiLU * up + quantise
-constexpr int kSiluThreads = 128;  // 78.7 us for 8192 x 12288, 8.1 for 333 x 25600 (256: 79.5 and 8.7)
+constexpr int kSiluThreads = 128;  // 80.2 us for 8192 x 12288, 8.5 for 333 x 25600 (256: 82.9 and 9.1)
 constexpr int kSiluThreadsLog2 = 7;
 static_assert(kSiluThreads == 1 << kSiluThreadsLog2, "shifts");
 
@@ -235,10 +235,10 @@ cudaError_t launch_norm(const NormQuantParams& p, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t launch_norm_for(const NormQuantParams& p, cudaStream_t stream) {
-  // Few rows: a row over as many threads as there are, for its latency (1 row of 4096: 1.75 us with one
-  // vector a thread, 1.92 with two, 2.56 with four; 256 of 8192: 4.3, two, and 5.1, four).  Many: more work
-  // a thread, but rows of 320 threads or fewer (8192 of 4096: 46.4, 39.6 and 40.3 us; of 8192: 93.1, two,
-  // and 80.4, four).  512 rows is where they meet.
+  // Few rows: a row over as many threads as there are, for its latency (1 row of 4096: 2.2 us with one
+  // vector a thread, 2.4 with two, 3.1 with four; 256 of 8192: 4.5, two, and 5.3, four).  Many: more work
+  // a thread, but rows of 320 threads or fewer (8192 of 4096: 47.6, 40.2 and 41.2 us; of 5120: 50.9, two, and
+  // 56.6, four; of 8192: 94.4, two, and 81.4, four).  512 rows is where they meet (of 4096: 4.7 us either way).
   const bool few = p.M <= 512;
   if (few && p.K <= 4096) return launch_norm<T, 1>(p, stream);
   if (p.K <= (few ? 8192 : 5120)) return launch_norm<T, 2>(p, stream);

@@ -213,9 +213,9 @@ __device__ __forceinline__ double exact_part(const uint16_t* x, const uint16_t* 
 // magnitudes, which bound what the fp32 sums may be off by.  The logits of token 8 c + r meet in CTA r, which
 // chooses by them where the bound leaves no doubt, and else sums those in doubt again in fp64 (a few
 // percent of the tokens of 128 experts): the experts and their order are those of exact sums.
-// Bound: latency (a launch, a load from HBM, two cluster barriers, the choice): 5.4 us by itself for a token
-// of 2048 columns and 128 experts, 0.7 of them for the bound, and 7.4 where some are summed again.  Two CTAs
-// an SM (128 registers): 250 tokens of 60 experts take 7.9 us, 13.8 with one.
+// Bound: latency (a launch, a load from HBM, two cluster barriers, the choice): 5.6 us by itself for a token
+// of 2048 columns and 128 experts, 0.8 of them for the bound, and 7.2 to 8 where some are summed again.  Two
+// CTAs an SM (128 registers): the layer takes 60.1 us for 250 tokens of 60 experts, 65.3 with one.
 constexpr int kRouterTokens = 8;
 static_assert(kRouterTokens <= kRouterCluster, "a CTA chooses for one token at most");
 // Of the magnitudes' sum, what a logit may be off by: 32 additions of at most 2^-23 each (tensor cores
@@ -365,10 +365,12 @@ constexpr int kDBufs = 4;
 // counters: the next ticket, finished ranges of phase 1, finished items of each tile (phase 0), arrived
 // parts of the item that each range leaves unfinished (by phase)
 constexpr int kDoneAt = 1, kReadyAt = 2;
-// Tokens per tile: 16 where an expert has 12 tokens or fewer on average (its tiles past the first read
-// the weights again, from L2), which leaves the ring more room for weights and the promotion threads
-// less to do; else 32.  64 experts of 4096 x 1408, 9 tokens each: 187 us with 16, 195 with 32; 12
-// each: the same; 60 experts of 1152 x 640, 25 each: 59 us with 32.
+// Tokens per tile: 16 where an expert has 12 tokens or fewer on average, which leaves the ring more room for
+// weights and the promotion threads less to do; else 32.  64 experts of 4096 x 1408, 9 tokens each: 187 us
+// with 16, 195 with 32; 12 each: the same; 60 experts of 1152 x 640, 25 each: 59 us with 32.  An expert's
+// tiles past the first read its weights again, and from HBM: between two readings of a weight tile the
+// CTAs read more than L2 holds (8 experts of 4096 x 7168, top 2: 256 tokens read 1.75 GB for 0.70 GB of
+// weights and take 311 us, 1024 tokens 5.9 GB and 1005 us).
 constexpr int kFewTokens = 12;
 constexpr int kMaxTiles = 896;  // at most the experts and the full tiles
 static_assert(kMoeMaxExperts + kMoeMaxSlots / 32 <= kMaxTiles &&
@@ -1122,8 +1124,8 @@ __device__ void promote(MoeSmem<NT>& sm, const MoeParams& p, int warp, int lane)
         if (!sm.last) continue;
       }
       // kLanes lanes take a token: lane l columns 4 (l + kLanes i) .. + 3. With up to 32 tokens an item, two
-      // tokens a warp halve the turns (250 tokens, 60 experts, top 6: 59.7 to 56.4 us); with few, a warp a
-      // token has the shorter chain (1 token: 24.5 us against 25.0; 16 tokens: 73.9 against 74.9).
+      // tokens a warp halve the turns (250 tokens, 60 experts, top 6: 63.1 to 60.1 us); with few, a warp a
+      // token has the shorter chain (1 token: 26.8 us against 27.2; 16 tokens: 78.1 against 78.9).
       constexpr int kLanes = NT == 16 ? 32 : 16, kQuads = 32 / kLanes, kTokens = kPromoWarps * 32 / kLanes;
       constexpr int kTogether = NT == 16 ? 4 : 2;  // parts whose loads are in flight together
       const int at = 4 * (lane % kLanes);
