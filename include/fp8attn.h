@@ -347,6 +347,79 @@ FP8ATTN_API int fp8attn_diag_counter_wait(const int32_t* counters, int want, int
                    int32_t* reached, int32_t* error, void* stream);
 FP8ATTN_API int fp8attn_diag_exp2(const float* x, float* poly, float* mufu, int64_t n, void* stream);
 
+/* ---------------------------------------------------------------- rotary positions
+ * Turns the first rotary_dim values of every head of q and k by their token's position; the others pass
+ * through.  Pairs are (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where `interleaved` is not 0:
+ *   y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin in fp32, rounded once.
+ * (The reference's RotaryEmbedding, nanovllm/layers/rotary_embedding.py:6-47, is rotary_dim = head_dim
+ * by halves.)
+ *   q, k      bf16 or fp16 (`dtype`: FP8ATTN_BF16, FP8ATTN_FP16) [num_tokens, heads, head_dim]; token and
+ *             head strides in elements, any; num_kv_heads 0: no k
+ *   q_out, k_out  the same, rows that do not overlap; may be q and k themselves (same strides)
+ *   positions int64 [num_tokens]; positions outside the table take its first or last row
+ *   cos_sin   fp32 [max_position, rotary_dim]: cos of the rotary_dim / 2 angles, then sin; 16-byte aligned
+ * head_dim: even, up to 4096; rotary_dim: even, 2 .. head_dim. */
+FP8ATTN_API int fp8attn_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                             int64_t k_token_stride, int64_t k_head_stride, const int64_t* positions,
+                             const float* cos_sin, int64_t max_position, void* q_out, int64_t q_out_token_stride,
+                             int64_t q_out_head_stride, void* k_out, int64_t k_out_token_stride,
+                             int64_t k_out_head_stride, int64_t num_tokens, int num_heads, int num_kv_heads,
+                             int head_dim, int rotary_dim, int interleaved, int dtype, void* stream);
+
+/* ---------------------------------------------------------------- 4-bit key/value cache
+ * A row (one token of one kv head, 128 values x) is held as
+ *   low = min x,  step = bf16((max x - min x) / 15),
+ *   code = nearest integer to (x - low) / step (ties to even) in 0 .. 15, 0 where step is 0,
+ * and stands for low + step * code.  A row that holds a NaN or an infinity, or whose range passes bf16's
+ * largest value, has a NaN as its step and reads as NaN.
+ *   k_cache, v_cache  bytes [num_blocks, num_kv_heads, block_size, 64]: value 2 i in the low half of byte
+ *                     i, value 2 i + 1 in the high half
+ *   kv_scale          bf16 [num_blocks, num_kv_heads, block_size, 4]: k step, k low, v step, v low
+ * all contiguous and 16-byte aligned; block_size a multiple of 16; num_blocks * block_size < 2^31.
+ * No counterpart in the reference, whose cache is e4m3 (nanovllm/layers/attention.py:11-40). */
+
+/* New rows into the cache: row i of key and value (bf16 [num_tokens, num_kv_heads, 128], token and head
+ * strides in elements, any) to slot slot_mapping[i]; slots that are -1 or outside the cache are skipped.
+ * Slots that are given must differ. */
+FP8ATTN_API int fp8attn_int4_store(const void* key, int64_t key_token_stride, int64_t key_head_stride,
+                                   const void* value, int64_t value_token_stride, int64_t value_head_stride,
+                                   void* k_cache, void* v_cache, void* kv_scale, const int32_t* slot_mapping,
+                                   int64_t num_tokens, int num_kv_heads, int head_dim, int64_t num_blocks,
+                                   int block_size, void* stream);
+
+/* Rows of the cache as bf16 (low + step * code in fp32, rounded once): key_out and value_out
+ * [num_tokens, num_kv_heads, 128], contiguous; zeros for slots that are -1 or outside the cache. */
+FP8ATTN_API int fp8attn_int4_load(const void* k_cache, const void* v_cache, const void* kv_scale,
+                                  const int32_t* slot_mapping, void* key_out, void* value_out, int64_t num_tokens,
+                                  int num_kv_heads, int head_dim, int64_t num_blocks, int block_size, void* stream);
+
+/* Bytes of workspace for the two calls below on the current device (decode: max_seqlen_q 1); -1 for bad
+ * arguments.  The workspace needs no clearing and keeps nothing from one call to the next; calls that may run at
+ * the same time, and graphs that may, need one each. */
+FP8ATTN_API int64_t fp8attn_int4_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int max_seqlen_q);
+
+/* Attention of one token per sequence over the paged 4-bit cache; arguments as fp8attn_decode's, num_seqs up
+ * to 65535.  Positions in pages that the table does not name (-1, out of range) are masked; a sequence
+ * without any position gives zeros. */
+FP8ATTN_API int fp8attn_int4_decode(void* out, const void* q, int64_t q_row_stride, const void* k_cache,
+                                    const void* v_cache, const void* kv_scale, const int32_t* block_tables,
+                                    int64_t block_tables_stride, int max_num_blocks, const int32_t* context_lens,
+                                    int num_seqs, int num_heads, int num_kv_heads, int head_dim, int64_t num_blocks,
+                                    int block_size, float softmax_scale, void* workspace, int64_t workspace_bytes,
+                                    void* stream);
+
+/* Causal attention of each sequence's last cu_seqlens_q[s + 1] - cu_seqlens_q[s] tokens over its
+ * cu_seqlens_k[s + 1] - cu_seqlens_k[s] positions in the paged 4-bit cache (their own rows stored before);
+ * arguments as fp8attn_prefill's paged form.  Query row i of a sequence sees positions up to
+ * i + (keys - queries); rows that see nothing give zeros.  No sequence may have more than max_seqlen_q new
+ * tokens; rows of q behind the last sequence's are not written. */
+FP8ATTN_API int fp8attn_int4_prefill(void* out, const void* q, int64_t q_row_stride, const void* k_cache,
+                                     const void* v_cache, const void* kv_scale, const int32_t* block_tables,
+                                     int64_t block_tables_stride, int max_num_blocks, const int32_t* cu_seqlens_q,
+                                     const int32_t* cu_seqlens_k, int num_seqs, int max_seqlen_q, int num_heads,
+                                     int num_kv_heads, int head_dim, int64_t num_blocks, int block_size,
+                                     float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

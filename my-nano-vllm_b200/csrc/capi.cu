@@ -1017,3 +1017,248 @@ int fp8attn_fp8_moe_read_error(int32_t* dst, int clear, void* stream) {
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------- rotary positions, 4-bit cache
+namespace {
+
+// Whether writing rows of `width` elements at i * a + j * b, i < n and j < m, never meets the same element
+// twice.
+bool rows_apart(int64_t a, int64_t n, int64_t b, int64_t m, int64_t width) {
+  if (n <= 1 && m <= 1) return true;
+  if (n <= 1) return b >= width;
+  if (m <= 1) return a >= width;
+  return a <= b ? a >= width && b >= a * (n - 1) + width : b >= width && a >= b * (m - 1) + width;
+}
+
+int check_int4_cache(const void* k_cache, const void* v_cache, const void* kv_scale, int num_kv_heads, int head_dim,
+                     int64_t num_blocks, int block_size) {
+  if (head_dim != fp8attn::kHeadDim) return fail(FP8ATTN_EINVAL, "head_dim must be 128 (got %d)", head_dim);
+  if (num_kv_heads <= 0) return fail(FP8ATTN_EINVAL, "num_kv_heads must be positive (got %d)", num_kv_heads);
+  if (block_size <= 0 || block_size % 16 != 0)
+    return fail(FP8ATTN_EINVAL, "block_size must be a positive multiple of 16 (got %d)", block_size);
+  if (num_blocks <= 0 || num_blocks > INT32_MAX / block_size)
+    return fail(FP8ATTN_EINVAL, "num_blocks * block_size must be in (0, 2^31)");
+  if (!k_cache || !v_cache || !kv_scale) return fail(FP8ATTN_EINVAL, "null cache pointer");
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(kv_scale))
+    return fail(FP8ATTN_EINVAL, "caches and scales must be 16-byte aligned");
+  return FP8ATTN_OK;
+}
+
+int check_int4_attention(const void* out, const void* q, int64_t q_row_stride, const int32_t* block_tables,
+                         int64_t block_tables_stride, int max_num_blocks, int num_seqs, int num_heads,
+                         int num_kv_heads, int block_size) {
+  if (num_heads <= 0 || num_heads % num_kv_heads != 0)
+    return fail(FP8ATTN_EINVAL, "num_heads (%d) must be a positive multiple of num_kv_heads (%d)", num_heads,
+                num_kv_heads);
+  if (num_seqs < 0 || num_seqs > 65535)
+    return fail(FP8ATTN_EINVAL, "num_seqs must be in [0, 65535] (got %d)", num_seqs);
+  if (!out || !q || !block_tables) return fail(FP8ATTN_EINVAL, "null pointer argument");
+  if (!aligned16(out) || !aligned16(q) || q_row_stride % 8 != 0 ||
+      q_row_stride < static_cast<int64_t>(num_heads) * fp8attn::kHeadDim)
+    return fail(FP8ATTN_EINVAL, "q/out must be 16-byte aligned with rows of num_heads*128");
+  if (max_num_blocks < 0 || block_tables_stride < max_num_blocks)
+    return fail(FP8ATTN_EINVAL, "bad block table geometry (max_num_blocks %d, stride %lld)", max_num_blocks,
+                static_cast<long long>(block_tables_stride));
+  if (static_cast<int64_t>(max_num_blocks) * block_size >= (1 << 24))
+    return fail(FP8ATTN_EINVAL, "max_num_blocks * block_size must be < 2^24");
+  return FP8ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fp8attn_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                 int64_t k_head_stride, const int64_t* positions, const float* cos_sin, int64_t max_position,
+                 void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride, void* k_out,
+                 int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t num_tokens, int num_heads,
+                 int num_kv_heads, int head_dim, int rotary_dim, int interleaved, int dtype, void* stream) {
+  if (dtype != FP8ATTN_BF16 && dtype != FP8ATTN_FP16) return fail(FP8ATTN_EINVAL, "dtype must be bf16 or fp16");
+  if (num_tokens < 0 || num_heads <= 0 || num_kv_heads < 0 || max_position <= 0)
+    return fail(FP8ATTN_EINVAL, "bad sizes");
+  if (head_dim <= 0 || head_dim % 2 != 0 || head_dim > 4096)
+    return fail(FP8ATTN_EINVAL, "head_dim must be even and in [2, 4096] (got %d)", head_dim);
+  if (rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
+    return fail(FP8ATTN_EINVAL, "rotary_dim must be even and in [2, head_dim] (got %d)", rotary_dim);
+  // a thread's number has 32 bits
+  const int64_t per_token = static_cast<int64_t>(num_heads + num_kv_heads) * (head_dim / 2);
+  if (per_token > (1 << 24) || num_tokens > (int64_t{1} << 31) / per_token)
+    return fail(FP8ATTN_EINVAL, "num_tokens * heads * head_dim must be at most 2^32");
+  if (num_tokens == 0) return FP8ATTN_OK;
+  if (!q || !q_out || !positions || !cos_sin || (num_kv_heads > 0 && (!k || !k_out)))
+    return fail(FP8ATTN_EINVAL, "null pointer argument");
+  if (!aligned(q, 2) || !aligned(q_out, 2) || !aligned(k, 2) || !aligned(k_out, 2) || !aligned(positions, 8) ||
+      !aligned(cos_sin, 16))
+    return fail(FP8ATTN_EINVAL, "misaligned pointer argument");
+  if (!rows_apart(q_out_token_stride, num_tokens, q_out_head_stride, num_heads, head_dim) ||
+      (num_kv_heads > 0 && !rows_apart(k_out_token_stride, num_tokens, k_out_head_stride, num_kv_heads, head_dim)))
+    return fail(FP8ATTN_EINVAL, "output rows overlap");
+  if (num_kv_heads > 0 && q_out == k_out) return fail(FP8ATTN_EINVAL, "q and k outputs are the same memory");
+  fp8attn::RopeParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_token_stride = q_token_stride;
+  p.q_head_stride = q_head_stride;
+  p.k = static_cast<const uint16_t*>(k);
+  p.k_token_stride = k_token_stride;
+  p.k_head_stride = k_head_stride;
+  p.positions = positions;
+  p.cos_sin = cos_sin;
+  p.max_position = max_position;
+  p.q_out = static_cast<uint16_t*>(q_out);
+  p.q_out_token_stride = q_out_token_stride;
+  p.q_out_head_stride = q_out_head_stride;
+  p.k_out = static_cast<uint16_t*>(k_out);
+  p.k_out_token_stride = k_out_token_stride;
+  p.k_out_head_stride = k_out_head_stride;
+  p.num_tokens = num_tokens;
+  p.num_heads = num_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.rotary_dim = rotary_dim;
+  p.interleaved = interleaved ? 1 : 0;
+  p.fp16 = dtype == FP8ATTN_FP16;
+  p.in_place = q_out == q && q_out_token_stride == q_token_stride && q_out_head_stride == q_head_stride &&
+               (num_kv_heads == 0 || (k_out == k && k_out_token_stride == k_token_stride &&
+                                      k_out_head_stride == k_head_stride));
+  const cudaError_t e = fp8attn::launch_rope(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rope launch");
+  return FP8ATTN_OK;
+}
+
+static int int4_rows(fp8attn::Int4RowsParams& p, const void* k_cache, const void* v_cache, const void* kv_scale,
+                     const int32_t* slot_mapping, int64_t num_tokens, int num_kv_heads, int head_dim,
+                     int64_t num_blocks, int block_size) {
+  const int rc = check_int4_cache(k_cache, v_cache, kv_scale, num_kv_heads, head_dim, num_blocks, block_size);
+  if (rc) return rc;
+  if (num_tokens < 0 || num_kv_heads > 4096 || num_tokens > (int64_t{1} << 31) / num_kv_heads)
+    return fail(FP8ATTN_EINVAL, "num_tokens * num_kv_heads must be in [0, 2^31], num_kv_heads at most 4096");
+  if (num_tokens > 0 && !slot_mapping) return fail(FP8ATTN_EINVAL, "null pointer argument");
+  p.k_cache = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  p.v_cache = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  p.kv_scale = static_cast<uint16_t*>(const_cast<void*>(kv_scale));
+  p.slot_mapping = slot_mapping;
+  p.num_tokens = num_tokens;
+  p.num_slots = num_blocks * block_size;
+  p.num_kv_heads = num_kv_heads;
+  p.block_size = block_size;
+  return FP8ATTN_OK;
+}
+
+int fp8attn_int4_store(const void* key, int64_t key_token_stride, int64_t key_head_stride, const void* value,
+                       int64_t value_token_stride, int64_t value_head_stride, void* k_cache, void* v_cache,
+                       void* kv_scale, const int32_t* slot_mapping, int64_t num_tokens, int num_kv_heads,
+                       int head_dim, int64_t num_blocks, int block_size, void* stream) {
+  fp8attn::Int4RowsParams p{};
+  const int rc = int4_rows(p, k_cache, v_cache, kv_scale, slot_mapping, num_tokens, num_kv_heads, head_dim, num_blocks,
+                           block_size);
+  if (rc) return rc;
+  if (num_tokens == 0) return FP8ATTN_OK;
+  if (!key || !value) return fail(FP8ATTN_EINVAL, "null pointer argument");
+  if (!aligned(key, 2) || !aligned(value, 2)) return fail(FP8ATTN_EINVAL, "key/value must be 2-byte aligned");
+  p.key = static_cast<const uint16_t*>(key);
+  p.key_token_stride = key_token_stride;
+  p.key_head_stride = key_head_stride;
+  p.value = static_cast<const uint16_t*>(value);
+  p.value_token_stride = value_token_stride;
+  p.value_head_stride = value_head_stride;
+  const cudaError_t e = fp8attn::launch_int4_store(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "4-bit store launch");
+  return FP8ATTN_OK;
+}
+
+int fp8attn_int4_load(const void* k_cache, const void* v_cache, const void* kv_scale, const int32_t* slot_mapping,
+                      void* key_out, void* value_out, int64_t num_tokens, int num_kv_heads, int head_dim,
+                      int64_t num_blocks, int block_size, void* stream) {
+  fp8attn::Int4RowsParams p{};
+  const int rc = int4_rows(p, k_cache, v_cache, kv_scale, slot_mapping, num_tokens, num_kv_heads, head_dim, num_blocks,
+                           block_size);
+  if (rc) return rc;
+  if (num_tokens == 0) return FP8ATTN_OK;
+  if (!key_out || !value_out) return fail(FP8ATTN_EINVAL, "null pointer argument");
+  if (!aligned16(key_out) || !aligned16(value_out))
+    return fail(FP8ATTN_EINVAL, "outputs must be 16-byte aligned");
+  p.key_out = static_cast<uint16_t*>(key_out);
+  p.value_out = static_cast<uint16_t*>(value_out);
+  const cudaError_t e = fp8attn::launch_int4_load(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "4-bit load launch");
+  return FP8ATTN_OK;
+}
+
+int64_t fp8attn_int4_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int max_seqlen_q) {
+  if (num_seqs < 0 || num_seqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads) return -1;
+  const int group = num_heads / num_kv_heads, max_q = max_seqlen_q < 1 ? 1 : max_seqlen_q;
+  const int grid = fp8attn::int4_decode_grid(group, max_q);
+  if (grid <= 0) return -1;
+  return fp8attn::int4_decode_workspace_bytes(num_seqs, group, max_q, grid);
+}
+
+static int int4_attention(void* out, const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                          const void* kv_scale, const int32_t* block_tables, int64_t block_tables_stride,
+                          int max_num_blocks, const int32_t* context_lens, const int32_t* cu_q, const int32_t* cu_k,
+                          int max_q, int num_seqs, int num_heads, int num_kv_heads, int head_dim, int64_t num_blocks,
+                          int block_size, float softmax_scale, void* workspace, int64_t workspace_bytes,
+                          void* stream) {
+  int rc = check_int4_cache(k_cache, v_cache, kv_scale, num_kv_heads, head_dim, num_blocks, block_size);
+  if (rc) return rc;
+  rc = check_int4_attention(out, q, q_row_stride, block_tables, block_tables_stride, max_num_blocks, num_seqs,
+                            num_heads, num_kv_heads, block_size);
+  if (rc) return rc;
+  if (num_seqs == 0) return FP8ATTN_OK;
+  fp8attn::Int4AttnParams p{};
+  p.out = static_cast<uint16_t*>(out);
+  p.out_row_stride = static_cast<int64_t>(num_heads) * head_dim;
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_row_stride = q_row_stride;
+  p.k_cache = static_cast<const uint8_t*>(k_cache);
+  p.v_cache = static_cast<const uint8_t*>(v_cache);
+  p.kv_scale = static_cast<const uint16_t*>(kv_scale);
+  p.block_tables = block_tables;
+  p.bt_stride = block_tables_stride;
+  p.max_blocks = max_num_blocks;
+  p.context_lens = context_lens;
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.num_seqs = num_seqs;
+  p.num_kv_heads = num_kv_heads;
+  p.group = num_heads / num_kv_heads;
+  p.block_size = block_size;
+  p.num_blocks = num_blocks;
+  p.max_q = max_q;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  const int grid = fp8attn::int4_decode_grid(p.group, max_q);
+  if (grid <= 0) return fail(FP8ATTN_ECUDA, "no kernel for this device");
+  const int64_t need = fp8attn::int4_decode_workspace_bytes(num_seqs, p.group, max_q, grid);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(FP8ATTN_EWORKSPACE, "workspace of %lld bytes is smaller than the %lld needed",
+                static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  if (!aligned16(workspace)) return fail(FP8ATTN_EINVAL, "workspace must be 16-byte aligned");
+  const cudaError_t e = fp8attn::launch_int4_decode(p, workspace, grid, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "4-bit attention launch");
+  return FP8ATTN_OK;
+}
+
+int fp8attn_int4_decode(void* out, const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                        const void* kv_scale, const int32_t* block_tables, int64_t block_tables_stride,
+                        int max_num_blocks, const int32_t* context_lens, int num_seqs, int num_heads, int num_kv_heads,
+                        int head_dim, int64_t num_blocks, int block_size, float softmax_scale, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  if (num_seqs > 0 && !context_lens) return fail(FP8ATTN_EINVAL, "null pointer argument");
+  return int4_attention(out, q, q_row_stride, k_cache, v_cache, kv_scale, block_tables, block_tables_stride,
+                        max_num_blocks, context_lens, nullptr, nullptr, 1, num_seqs, num_heads, num_kv_heads, head_dim,
+                        num_blocks, block_size, softmax_scale, workspace, workspace_bytes, stream);
+}
+
+int fp8attn_int4_prefill(void* out, const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                         const void* kv_scale, const int32_t* block_tables, int64_t block_tables_stride,
+                         int max_num_blocks, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int num_seqs,
+                         int max_seqlen_q, int num_heads, int num_kv_heads, int head_dim, int64_t num_blocks,
+                         int block_size, float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (num_seqs > 0 && (!cu_seqlens_q || !cu_seqlens_k)) return fail(FP8ATTN_EINVAL, "null pointer argument");
+  if (max_seqlen_q <= 0) return max_seqlen_q < 0 ? fail(FP8ATTN_EINVAL, "bad max_seqlen_q") : FP8ATTN_OK;
+  return int4_attention(out, q, q_row_stride, k_cache, v_cache, kv_scale, block_tables, block_tables_stride,
+                        max_num_blocks, nullptr, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_seqs, num_heads,
+                        num_kv_heads, head_dim, num_blocks, block_size, softmax_scale, workspace, workspace_bytes,
+                        stream);
+}
+
+}  // extern "C"

@@ -183,6 +183,73 @@ cudaError_t moe_error_word(void** word);
 cudaError_t launch_counter_wait(const int* counters, int want, unsigned long long limit_ns, int* reached, int* err,
                                 cudaStream_t stream);
 
+// ------------------------------------------------------------------ rotary positions
+struct RopeParams {
+  const uint16_t* q;  // bf16 or fp16 [N, Hq, D], strides in elements
+  int64_t q_token_stride, q_head_stride;
+  const uint16_t* k;  // [N, KVH, D] (num_kv_heads 0: none)
+  int64_t k_token_stride, k_head_stride;
+  uint16_t* q_out;
+  int64_t q_out_token_stride, q_out_head_stride;
+  uint16_t* k_out;
+  int64_t k_out_token_stride, k_out_head_stride;
+  const int64_t* positions;  // [N], clamped to [0, max_position)
+  const float* cos_sin;      // fp32 [max_position, rotary_dim]: cos of rotary_dim / 2 frequencies, then sin
+  int64_t max_position, num_tokens;
+  int num_heads, num_kv_heads, head_dim, rotary_dim;
+  int interleaved, fp16, in_place;
+  int chunks, turned_chunks, head_groups;  // set by the launch
+};
+cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream);
+
+// ------------------------------------------------------------------ 4-bit key/value cache
+struct Int4RowsParams {
+  const uint16_t* key;  // store: bf16 [N, KVH, 128], strides in elements
+  int64_t key_token_stride, key_head_stride;
+  const uint16_t* value;
+  int64_t value_token_stride, value_head_stride;
+  uint16_t* key_out;  // load: bf16 [N, KVH, 128], contiguous
+  uint16_t* value_out;
+  uint8_t* k_cache;  // [num_blocks, KVH, block_size, 64] bytes of two codes
+  uint8_t* v_cache;
+  uint16_t* kv_scale;  // bf16 [num_blocks, KVH, block_size, 4]: k step, k low, v step, v low
+  const int32_t* slot_mapping;  // [N]; -1 (or out of range): not stored, read as zeros
+  int64_t num_tokens;
+  int64_t num_slots;
+  int num_kv_heads;
+  int block_size;
+};
+cudaError_t launch_int4_store(const Int4RowsParams& p, cudaStream_t stream);
+cudaError_t launch_int4_load(const Int4RowsParams& p, cudaStream_t stream);
+
+struct Int4AttnParams {
+  uint16_t* out;  // bf16
+  int64_t out_row_stride;  // elements per token row
+  const uint16_t* q;  // bf16
+  int64_t q_row_stride;
+  const uint8_t* k_cache;  // as above
+  const uint8_t* v_cache;
+  const uint16_t* kv_scale;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* context_lens;  // decode, or null
+  const int32_t* cu_q;  // chunks, or null
+  const int32_t* cu_k;
+  int num_seqs;
+  int num_kv_heads;
+  int group;  // query heads per kv head
+  int block_size;
+  int64_t num_blocks;
+  int max_q;  // sequences with more new tokens are left to the other kernel
+  float scale_log2;  // softmax_scale * log2(e)
+  int64_t* prefix;  // workspace: units before each sequence, [num_seqs + 1]
+  float* partials;  // workspace: two parts for each CTA
+};
+int int4_decode_grid(int group, int max_q);  // CTAs that run at once on the current device; 0: error
+int64_t int4_decode_workspace_bytes(int num_seqs, int group, int max_q, int grid);
+cudaError_t launch_int4_decode(Int4AttnParams p, void* workspace, int grid, cudaStream_t stream);
+
 // ------------------------------------------------------------------ decode engine
 // Control block at the head of the decode workspace (ints):
 //   [0] sticky device error code, [1] next work item, [2] CTAs finished.

@@ -98,6 +98,22 @@ def _load() -> ctypes.CDLL:
     lib.fp8attn_prefill.restype = i32
     lib.fp8attn_prefill.argtypes = [vp, vp, i64, vp, vp, i64, vp, vp, vp, i64, i32, vp, vp, i32,
                                     i32, i32, i32, i32, i32, i64, i32, f32, vp, i64, vp]
+    lib.fp8attn_rope.restype = i32
+    lib.fp8attn_rope.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, i64, vp, i64, i64, vp, i64, i64,
+                                 i64, i32, i32, i32, i32, i32, i32, vp]
+    lib.fp8attn_int4_store.restype = i32
+    lib.fp8attn_int4_store.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, i64, i32, i32, i64,
+                                       i32, vp]
+    lib.fp8attn_int4_load.restype = i32
+    lib.fp8attn_int4_load.argtypes = [vp, vp, vp, vp, vp, vp, i64, i32, i32, i64, i32, vp]
+    lib.fp8attn_int4_workspace_bytes.restype = i64
+    lib.fp8attn_int4_workspace_bytes.argtypes = [i32, i32, i32, i32]
+    lib.fp8attn_int4_decode.restype = i32
+    lib.fp8attn_int4_decode.argtypes = [vp, vp, i64, vp, vp, vp, vp, i64, i32, vp, i32, i32, i32, i32,
+                                        i64, i32, f32, vp, i64, vp]
+    lib.fp8attn_int4_prefill.restype = i32
+    lib.fp8attn_int4_prefill.argtypes = [vp, vp, i64, vp, vp, vp, vp, i64, i32, vp, vp, i32, i32, i32,
+                                         i32, i32, i64, i32, f32, vp, i64, vp]
     return lib
 
 
