@@ -375,7 +375,8 @@ FP8ATTN_API int fp8attn_rope(const void* q, int64_t q_token_stride, int64_t q_he
  *   k_cache, v_cache  bytes [num_blocks, num_kv_heads, block_size, 64]: value 2 i in the low half of byte
  *                     i, value 2 i + 1 in the high half
  *   kv_scale          bf16 [num_blocks, num_kv_heads, block_size, 4]: k step, k low, v step, v low
- * all contiguous and 16-byte aligned; block_size a multiple of 16; num_blocks * block_size < 2^31.
+ * all contiguous and 16-byte aligned; block_size a multiple of 16; num_blocks * block_size < 2^31 (for the
+ * attention calls num_blocks * num_kv_heads * block_size).
  * No counterpart in the reference, whose cache is e4m3 (nanovllm/layers/attention.py:11-40). */
 
 /* New rows into the cache: row i of key and value (bf16 [num_tokens, num_kv_heads, 128], token and head
@@ -419,6 +420,10 @@ FP8ATTN_API int fp8attn_int4_prefill(void* out, const void* q, int64_t q_row_str
                                      const int32_t* cu_seqlens_k, int num_seqs, int max_seqlen_q, int num_heads,
                                      int num_kv_heads, int head_dim, int64_t num_blocks, int block_size,
                                      float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Copies the error word of the two attention calls on the current device (a bounded wait that gave up records 1) to
+ * dst (device or host memory) on the stream, and clears it if `clear` is not 0. */
+FP8ATTN_API int fp8attn_int4_read_error(int32_t* dst, int clear, void* stream);
 
 #ifdef __cplusplus
 }

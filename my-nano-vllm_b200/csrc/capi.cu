@@ -1044,9 +1044,43 @@ int check_int4_cache(const void* k_cache, const void* v_cache, const void* kv_sc
   return FP8ATTN_OK;
 }
 
+// Codes of a 4-bit cache as rows of 64 bytes, in boxes of box_rows rows; 64B swizzle.
+int make_codes_map(CUtensorMap* map, const void* codes, int64_t rows, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(FP8ATTN_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {64, static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {64};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FP8ATTN_ECUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return FP8ATTN_OK;
+}
+
+// The error word on the current device; asked for once.
+int int4_error(int** word) {
+  constexpr int kDevices = 64;
+  static std::atomic<int*> known[kDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "current device");
+  int* at = dev >= 0 && dev < kDevices ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (at == nullptr) {
+    void* ptr = nullptr;
+    e = fp8attn::int4_error_word(&ptr);
+    if (e != cudaSuccess) return cuda_fail(e, "error word");
+    at = static_cast<int*>(ptr);
+    if (dev >= 0 && dev < kDevices) known[dev].store(at, std::memory_order_relaxed);
+  }
+  *word = at;
+  return FP8ATTN_OK;
+}
+
 int check_int4_attention(const void* out, const void* q, int64_t q_row_stride, const int32_t* block_tables,
                          int64_t block_tables_stride, int max_num_blocks, int num_seqs, int num_heads,
-                         int num_kv_heads, int block_size) {
+                         int num_kv_heads, int64_t num_blocks, int block_size) {
   if (num_heads <= 0 || num_heads % num_kv_heads != 0)
     return fail(FP8ATTN_EINVAL, "num_heads (%d) must be a positive multiple of num_kv_heads (%d)", num_heads,
                 num_kv_heads);
@@ -1061,6 +1095,8 @@ int check_int4_attention(const void* out, const void* q, int64_t q_row_stride, c
                 static_cast<long long>(block_tables_stride));
   if (static_cast<int64_t>(max_num_blocks) * block_size >= (1 << 24))
     return fail(FP8ATTN_EINVAL, "max_num_blocks * block_size must be < 2^24");
+  if (num_blocks * block_size > INT32_MAX / num_kv_heads)
+    return fail(FP8ATTN_EINVAL, "num_blocks * num_kv_heads * block_size must be < 2^31");
   return FP8ATTN_OK;
 }
 
@@ -1189,7 +1225,7 @@ int64_t fp8attn_int4_workspace_bytes(int num_seqs, int num_heads, int num_kv_hea
   const int group = num_heads / num_kv_heads, max_q = max_seqlen_q < 1 ? 1 : max_seqlen_q;
   const int grid = fp8attn::int4_decode_grid(group, max_q);
   if (grid <= 0) return -1;
-  return fp8attn::int4_decode_workspace_bytes(num_seqs, group, max_q, grid);
+  return fp8attn::int4_decode_workspace_bytes(group, max_q, grid);
 }
 
 static int int4_attention(void* out, const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
@@ -1201,7 +1237,7 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   int rc = check_int4_cache(k_cache, v_cache, kv_scale, num_kv_heads, head_dim, num_blocks, block_size);
   if (rc) return rc;
   rc = check_int4_attention(out, q, q_row_stride, block_tables, block_tables_stride, max_num_blocks, num_seqs,
-                            num_heads, num_kv_heads, block_size);
+                            num_heads, num_kv_heads, num_blocks, block_size);
   if (rc) return rc;
   if (num_seqs == 0) return FP8ATTN_OK;
   fp8attn::Int4AttnParams p{};
@@ -1227,12 +1263,22 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   const int grid = fp8attn::int4_decode_grid(p.group, max_q);
   if (grid <= 0) return fail(FP8ATTN_ECUDA, "no kernel for this device");
-  const int64_t need = fp8attn::int4_decode_workspace_bytes(num_seqs, p.group, max_q, grid);
+  const int64_t need = fp8attn::int4_decode_workspace_bytes(p.group, max_q, grid);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(FP8ATTN_EWORKSPACE, "workspace of %lld bytes is smaller than the %lld needed",
                 static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   if (!aligned16(workspace)) return fail(FP8ATTN_EINVAL, "workspace must be 16-byte aligned");
-  const cudaError_t e = fp8attn::launch_int4_decode(p, workspace, grid, static_cast<cudaStream_t>(stream));
+  p.box_rows = box_rows_for(block_size);
+  rc = int4_error(&p.err);
+  if (rc) return rc;
+  CUtensorMap map_k, map_v;
+  const int64_t rows = num_blocks * num_kv_heads * block_size;
+  rc = make_codes_map(&map_k, k_cache, rows, p.box_rows);
+  if (rc) return rc;
+  rc = make_codes_map(&map_v, v_cache, rows, p.box_rows);
+  if (rc) return rc;
+  const cudaError_t e =
+      fp8attn::launch_int4_decode(p, map_k, map_v, workspace, grid, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "4-bit attention launch");
   return FP8ATTN_OK;
 }
@@ -1259,6 +1305,14 @@ int fp8attn_int4_prefill(void* out, const void* q, int64_t q_row_stride, const v
                         max_num_blocks, nullptr, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_seqs, num_heads,
                         num_kv_heads, head_dim, num_blocks, block_size, softmax_scale, workspace, workspace_bytes,
                         stream);
+}
+
+int fp8attn_int4_read_error(int32_t* dst, int clear, void* stream) {
+  if (dst == nullptr) return fail(FP8ATTN_EINVAL, "null destination");
+  int* word = nullptr;
+  const int rc = int4_error(&word);
+  if (rc) return rc;
+  return fp8attn_read_error(reinterpret_cast<uint8_t*>(word) - FP8ATTN_WS_ERROR_OFFSET, dst, clear, stream);
 }
 
 }  // extern "C"

@@ -19,7 +19,7 @@
 // warps.  All units in order are cut into equal ranges, one for each resident CTA, wherever the cuts
 // fall: no counters, no order that depends on timing.  A CTA's first and last piece may be parts of a
 // pair; their sums go to the workspace, and a second kernel joins the parts of each cut pair in order.
-// Every warp keeps a ring of its own tiles in flight (cp.async, three stages of 4.25 KB), across the ends
+// Every warp keeps two of its own tiles of 4.25 KB in flight (TMA, 64B swizzle, one lane issues), across the ends
 // of pieces.
 //
 // c - 7.5 is the product with c and 7.5 times the same product with ones: taken about the middle of the codes, the
@@ -38,40 +38,84 @@
 namespace fp8attn {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+// The error word of these kernels' launches: it lives as long as the library's module, so that captured graphs may
+// hold its address.
+__device__ int g_error = 0;
+
+#ifndef INT4_W
+#define INT4_W 4
+#define INT4_S 3
+#define INT4_C 3
+#endif
+constexpr int kWarps = INT4_W;          // that compute; one more loads
+constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kTile = 32;               // positions per warp and unit
 constexpr int kUnit = kTile * kWarps;   // positions per unit
-constexpr int kStages = 3;
-constexpr int kStageBytes = kTile * 136;
+constexpr int kParts = kUnit / 16;      // parts of a unit that lie in one page each
+constexpr int kStages = INT4_S;
 constexpr int kPitch = 136;             // floats between rows of the joined sums (bank spread)
 constexpr float kSlack = 8.f;           // a reference maximum may lag by 2^8
 constexpr float kNone = -3.402823466e38f;
 
 template <int NT>
-struct __align__(128) Smem {
-  uint8_t ring[kWarps][kStages][kStageBytes];  // K rows, V rows, scales
-  uint2 q[NT][8][32];                          // B operand of S^T: plane, step, lane
-  float kq[8 * NT], qs[8 * NT];                // score = dot kq step + qs low
-  float o[kWarps][8][kPitch];                  // a plane's sums, joined over the warps
+struct __align__(1024) Smem {
+  uint8_t k[kStages][kUnit * 64];  // TMA tiles of 64-byte rows, 64B swizzle: bits 1 and 2 of a row's number
+  uint8_t v[kStages][kUnit * 64];  // change the place of its 16-byte pieces
+  uint2 scale[kStages][kUnit];
+  uint2 q[NT][8][32];              // B operand of S^T: plane, step, lane
+  float kq[8 * NT], qs[8 * NT];    // score = dot kq step + qs low
+  float o[kWarps][8][kPitch];      // a plane's sums, joined over the warps
   float m[kWarps][8], l[kWarps][8];
-  int64_t scan[kWarps];
-  int64_t total;
-  int64_t first_unit;  // of the sequence in which the CTA's range begins
+  uint64_t full[kStages], empty[kStages];
+  uint32_t there[kStages];         // which parts of the stage's unit are in pages of the cache
+  int64_t scan[kWarps + 1];
+  int64_t first_unit;              // of the sequence in which the CTA's range begins
   int first_seq;
 };
 
+// mbar_wait with its polling loop out of line, for a whole warp.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, int* err) { return mbar_wait(bar, parity, err); }
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || wait_long(bar, parity, err));
+}
+
+// The computing warps alone.
+__device__ __forceinline__ void sync_compute() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// d = a b: no registers to be cleared first.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// w >> 8 on the multiply pipe (by = 2^24, in a register so that it stays a product): the unpacking's masks keep
+// the integer pipe busier than anything else.
+__device__ __forceinline__ uint32_t shift8(uint32_t w, uint32_t by) {
+  uint32_t d;
+  d = w >> 8; (void)by;
+  return d;
+}
+
+// size bytes (a multiple of 16, both addresses too) from global to shared memory, counted on the mbarrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t size, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(size), "r"(smem_u32(bar))
+               : "memory");
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
 
@@ -79,6 +123,14 @@ __device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
+}
+
+// Four 8 x 8 matrices of 16-bit elements, transposed: lanes 8 i .. 8 i + 7 give the rows of matrix i.
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
 __device__ __forceinline__ float pow2(int e) {  // -126 <= e <= 127
@@ -94,7 +146,7 @@ struct Seq {
   }
 };
 
-template <int NT>
+template <int R>
 __device__ __forceinline__ Seq seq_of(const Int4AttnParams& p, int s) {
   Seq q;
   if (p.cu_q != nullptr) {
@@ -110,7 +162,7 @@ __device__ __forceinline__ Seq seq_of(const Int4AttnParams& p, int s) {
   q.vis = max(0, min(q.nk, p.max_blocks * p.block_size));
   // a sequence without positions still has its zeros written
   q.tiles = max(1, (q.vis + kUnit - 1) / kUnit);
-  q.groups = q.nq <= 0 ? 0 : (q.nq * p.group + 8 * NT - 1) / (8 * NT);
+  q.groups = q.nq <= 0 ? 0 : (q.nq * p.group + R - 1) / R;
   return q;
 }
 
@@ -120,63 +172,117 @@ struct Cursor {
   Seq s;
 };
 
-template <int NT>
-__device__ __forceinline__ void next_unit(const Int4AttnParams& p, Cursor& c) {
-  if (++c.tile < c.s.tiles) return;
+template <int R>
+__device__ __forceinline__ void next_pair(const Int4AttnParams& p, Cursor& c) {
   c.tile = 0;
   if (++c.pair < c.s.groups * p.num_kv_heads) return;
   c.pair = 0;
   do {
     if (++c.seq >= p.num_seqs) return;
-    c.s = seq_of<NT>(p, c.seq);
+    c.s = seq_of<R>(p, c.seq);
   } while (c.s.groups == 0);
 }
+
+// A pair that is cut for the first time at the end of a CTA's range: what joins its parts has to know.
+struct Cut {
+  int parts;  // 0: the CTA's range ends with a pair or with a later part of one
+  int slot;   // of the first part; part j > 0 is the first piece of CTA + j
+  int rows;   // of the row group
+  int first_row;  // in the group's kv head: token * group + head
+  int token, head;  // the sequence's first row of q, and the kv head's first query head
+  int unused[2];
+};
 
 // First unit of CTA i of n over u units, and the CTA that has unit x.
 __device__ __forceinline__ int64_t range_begin(int64_t i, int64_t n, int64_t u) { return i * u / n; }
 __device__ __forceinline__ int64_t owner(int64_t x, int64_t n, int64_t u) { return ((x + 1) * n - 1) / u; }
 
-// The block's page of 16 positions (lane halves), -1 for none.
-__device__ __forceinline__ int page_of(const Int4AttnParams& p, const Cursor& c, int warp, int lane) {
-  const int pos = c.tile * kUnit + warp * kTile + (lane & 16);
-  if (pos >= c.s.vis) return -1;
-  const int page = ldg_keep(p.block_tables + c.seq * p.bt_stride + pos / p.block_size);
-  return page >= 0 && page < p.num_blocks ? page : -1;
-}
-
-// This warp's tile of the cursor's unit into a stage; returns which halves are there (bits 0 and 1).
-// Within a half (16 positions) K row i stands at row 2 (i & 3) + (i >> 2 & 1) + 8 (i >> 3), the order in which S^T's
-// rows take them, and V row i at i with its 16-byte pieces changed by bit 1 of i: both are then read
-// without bank conflicts.
-__device__ __forceinline__ uint32_t load_tile(const Int4AttnParams& p, const Cursor& c, int page, int warp, int lane,
-                                              uint32_t stage) {
-  if (page >= 0) {
-    const int half = lane >> 4, l = lane & 15, a = l >> 2;
-    const int pos = c.tile * kUnit + warp * kTile + 16 * half;
-    const int place = pos % p.block_size;
+// The loading warp: lane i looks up the page of part i of each unit, and the lanes at which a TMA box begins load it
+// (box_rows positions: K, V and scales).  The pages of the next unit are looked up before this one's stage is waited
+// for.
+template <int NT, int R>
+__device__ __forceinline__ void load_units(const Int4AttnParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                                           Smem<NT>& sm, Cursor c, int64_t u0, int64_t u1, int lane) {
+  int column = 0, place = 0;
+  auto look_up = [&]() {
+    const int pos = c.tile * kUnit + lane * 16;
+    if (lane >= kParts || pos >= c.s.vis) return -1;
+    const int page = ldg_keep(p.block_tables + c.seq * p.bt_stride + column);
+    return page >= 0 && page < p.num_blocks ? page : -1;
+  };
+  auto find = [&]() {
+    const int pos = c.tile * kUnit + lane * 16;
+    column = pos / p.block_size;
+    place = pos - column * p.block_size;
+    return look_up();
+  };
+  int page = find();
+  int stage = 0;
+  uint32_t round = 0, loaded = 0;
+  const bool begins = lane < kParts && lane % (p.box_rows / 16) == 0;
+  bool ok = true;
+  for (int64_t u = u0; u < u1; ++u) {
     const int kvh = c.pair % p.num_kv_heads;
-    const int64_t row = (static_cast<int64_t>(page) * p.num_kv_heads + kvh) * p.block_size + place;
-    const uint8_t* k = p.k_cache + row * 64 + l * 16;
-    const uint8_t* v = p.v_cache + row * 64 + l * 16;
-    const uint32_t kd = stage + half * 1024 + (l & 3) * 16;
-    const uint32_t vd = stage + 2048 + half * 1024 + a * 64 + (((l & 3) ^ (a & 2)) * 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // rows 4 i + a
-      cp_async16(kd + (2 * a + (i & 1) + 8 * (i >> 1)) * 64, k + i * 256, true);
-      cp_async16(vd + i * 256, v + i * 256, true);
+    const int row = (page * p.num_kv_heads + kvh) * p.block_size + place;
+    const bool mine = begins && page >= 0;
+    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+    const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+    // the next unit's pages
+    if (u + 1 < u1) {
+      if (++c.tile < c.s.tiles) {
+        column += p.unit_pages;  // whole pages in a unit, and what is left
+        place += p.unit_rest;
+        if (place >= p.block_size) {
+          place -= p.block_size;
+          ++column;
+        }
+        page = look_up();
+      } else {
+        next_pair<R>(p, c);
+        page = find();
+      }
     }
-    if (l < 8) cp_async16(stage + 4096 + half * 128 + l * 16, reinterpret_cast<const uint8_t*>(p.kv_scale) + row * 8 + l * 16, true);
+    if (round > 0) ok = wait_warp(&sm.empty[stage], round - 1 & 1u, p.err);
+    if (!ok) break;
+    uint64_t* bar = &sm.full[stage];
+    if (lane == 0) {
+      sm.there[stage] = there;
+      mbar_arrive_expect_tx(bar, boxes * p.box_rows * 136);
+    }
+    __syncwarp();
+    if (mine) {
+      tma_load_2d(sm.k[stage] + lane * 1024, &map_k, bar, 0, row);
+      tma_load_2d(sm.v[stage] + lane * 1024, &map_v, bar, 0, row);
+      bulk_load(smem_u32(sm.scale[stage] + lane * 16), p.kv_scale + static_cast<int64_t>(row) * 4, p.box_rows * 8, bar);
+    }
+    loaded |= 1u << stage;
+    if (++stage == kStages) {
+      stage = 0;
+      ++round;
+    }
   }
-  const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-  return (there & 1u) | (there >> 15 & 2u);
+  // copies in flight after a wait that gave up: they must land (or run out of time) before the CTA ends
+  if (!ok)
+    for (int i = 0; i < kStages; ++i)
+      if (loaded >> i & 1u) wait_warp(&sm.full[i], (i < stage ? round : round - 1) & 1u, p.err);
 }
 
-template <int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(const Int4AttnParams p) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(smem_raw);
-  constexpr int R = 8 * NT;
+template <int NT, bool kFold>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_kernel(
+    const __grid_constant__ Int4AttnParams p, const __grid_constant__ CUtensorMap map_k,
+    const __grid_constant__ CUtensorMap map_v) {
+  extern __shared__ uint8_t smem_raw[];
+  Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(smem_raw + (1024 - smem_u32(smem_raw) % 1024) % 1024);
+  constexpr int R = kFold ? 4 : 8 * NT;  // rows of a group
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (tid == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], kWarps);
+    }
+    fence_mbar_init();
+  }
   // programmatic dependent of the kernel before it: nothing is read or written before that ends
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -185,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
   const int per = (p.num_seqs + kThreads - 1) / kThreads;
   const int s0 = min(tid * per, p.num_seqs), s1 = min(s0 + per, p.num_seqs);
   int64_t mine = 0;
-  for (int s = s0; s < s1; ++s) mine += seq_of<NT>(p, s).units(p.num_kv_heads);
+  for (int s = s0; s < s1; ++s) mine += seq_of<R>(p, s).units(p.num_kv_heads);
   int64_t before = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -196,27 +302,23 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
   __syncthreads();
   int64_t total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kWarps + 1; ++w) {
     if (w < warp) before += sm.scan[w];
     total += sm.scan[w];
   }
   before -= mine;
   const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
-  if (blockIdx.x == 0) {  // published for the joining kernel
-    int64_t at = before;
-    for (int s = s0; s < s1; ++s) {
-      p.prefix[s] = at;
-      at += seq_of<NT>(p, s).units(p.num_kv_heads);
-    }
-    if (tid == 0) p.prefix[p.num_seqs] = total;
+  Cut* cuts = reinterpret_cast<Cut*>(p.cuts);
+  if (blockIdx.x >= ctas) {
+    if (tid == 0) cuts[blockIdx.x].parts = 0;
+    return;
   }
-  if (blockIdx.x >= ctas) return;
   const int64_t u0 = range_begin(blockIdx.x, ctas, total), u1 = range_begin(blockIdx.x + 1, ctas, total);
   if (before <= u0 && u0 < before + mine) {
     int64_t at = before;
     int s = s0;
     for (; s < s1; ++s) {
-      const int64_t n = seq_of<NT>(p, s).units(p.num_kv_heads);
+      const int64_t n = seq_of<R>(p, s).units(p.num_kv_heads);
       if (u0 < at + n) break;
       at += n;
     }
@@ -226,50 +328,44 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
   __syncthreads();
   Cursor now;
   now.seq = sm.first_seq;
-  now.s = seq_of<NT>(p, now.seq);
+  now.s = seq_of<R>(p, now.seq);
   {
     const int64_t rest = u0 - sm.first_unit;
     now.pair = static_cast<int>(rest / now.s.tiles);
     now.tile = static_cast<int>(rest - static_cast<int64_t>(now.pair) * now.s.tiles);
   }
 
-  // ---- the ring: kStages - 1 tiles in flight, and the page of the one after them
-  Cursor ahead = now;
-  int64_t ahead_u = u0;
-  int page = page_of(p, ahead, warp, lane);
-  uint32_t there = 0;  // two bits for each stage
-  const uint32_t ring = smem_u32(sm.ring[warp]);
-  int ahead_stage = 0;
-  auto advance = [&]() {
-    if (ahead_u < u1) {
-      const uint32_t bits = load_tile(p, ahead, page, warp, lane, ring + ahead_stage * kStageBytes);
-      there = (there & ~(3u << (2 * ahead_stage))) | bits << (2 * ahead_stage);
-      ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
-      if (++ahead_u < u1) {
-        next_unit<NT>(p, ahead);
-        page = page_of(p, ahead, warp, lane);
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) advance();
+  if (warp == kWarps) {
+    load_units<NT, R>(p, map_k, map_v, sm, now, u0, u1, lane);
+    return;
+  }
 
+  // this lane's row for the transposed loads of V, and its piece (of the second of two: 1) as it is stored; its
+  // rows g and g + 8 of K, piece t
+  const int v_token = (lane & 7) + (lane & 8);
+  const uint32_t v_row = (warp * kTile + v_token) * 64, v_piece = (lane >> 4) ^ (v_token >> 1 & 3);
+  const uint32_t k_row = (warp * kTile + g) * 64 + (t ^ (g >> 1 & 3)) * 16;
+  const uint32_t k_ring = smem_u32(sm.k[0]) + k_row, v_ring = smem_u32(sm.v[0]) + v_row;
+  const uint32_t s_ring = smem_u32(sm.scale[0]) + (warp * kTile + g) * 8;
+  uint32_t by8;
+  asm volatile("mov.u32 %0, 0x1000000;" : "=r"(by8));
   int stage = 0;
+  uint32_t parity = 0;
+  bool ok = true;  // no wait has given up
   for (int64_t u = u0; u < u1;) {
     // ---- a piece: units [u, u + n) of one pair
-    const int64_t n = min(u1 - u, static_cast<int64_t>(now.s.tiles - now.tile));
+    const int n = static_cast<int>(min(u1 - u, static_cast<int64_t>(now.s.tiles - now.tile)));
     const bool whole = now.tile == 0 && n == now.s.tiles;
     const int kvh = now.pair % p.num_kv_heads, rg = now.pair / p.num_kv_heads;
     const int rows = now.s.nq * p.group;  // of this kv head
     // q: the B operand of S^T, plane j by warp j.  Column (row) g, values 32 t .. 32 t + 31 in the order
     // of the codes
     if (warp < NT) {
-      const int r = rg * R + 8 * warp + g;
+      const int r = rg * R + (kFold ? g & 3 : 8 * warp + g);
       uint4 raw[4] = {};
       if (r < rows) {
         const int token = r / p.group;
-        const uint16_t* src = p.q + (now.s.q_first + token) * p.q_row_stride +
+        const uint16_t* src = p.q + (static_cast<int64_t>(now.s.q_first) + token) * p.q_row_stride +
                               (kvh * p.group + r - token * p.group) * kHeadDim + 32 * t;
 #pragma unroll
         for (int w = 0; w < 4; ++w) raw[w] = ldg_keep_v4(src + 8 * w);
@@ -309,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
         sm.qs[8 * warp + g] = sum * p.scale_log2;
       }
     }
-    __syncthreads();
+    sync_compute();
     constexpr bool kHeld = NT <= 2;  // q stays in registers; else it is read from shared memory for each tile
     uint2 q[kHeld ? NT : 1][8];
     if constexpr (kHeld) {
@@ -326,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
       for (int c = 0; c < 2; ++c) {
         kq[j][c] = sm.kq[8 * j + 2 * t + c];
         qs[j][c] = sm.qs[8 * j + 2 * t + c];
-        const int row = rg * R + 8 * j + 2 * t + c;
+        const int row = rg * R + (kFold ? (2 * t + c) & 3 : 8 * j + 2 * t + c);
         limit[j][c] = min(now.s.vis, row / p.group + now.s.nk - now.s.nq + 1);
         if (row >= rows) limit[j][c] = min(now.s.vis, rg * R / p.group + now.s.nk - now.s.nq + 1);  // no row: as the first
         least = min(least, limit[j][c]);
@@ -340,13 +436,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
     }
 
     float o[NT][8][4], ps[NT][4], m[NT][2], l[NT][2], mid[NT][2];  // ps: sum of the rounded P step
+    float m_limit[NT][2];  // m and how far it may lag
     float v_unit = 1.f, v_limit = 0.f;  // steps of V are multiplied by v_unit (a power of two)
     int v_exp = 0;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        m[j][c] = kNone;
+        m[j][c] = m_limit[j][c] = kNone;
         l[j][c] = mid[j][c] = 0.f;
       }
 #pragma unroll
@@ -357,28 +454,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
         for (int c = 0; c < 4; ++c) o[j][i][c] = 0.f;
     }
 
-    for (int64_t i = 0; i < n; ++i) {
-      cp_async_wait<kStages - 2>();
-      __syncwarp();
-      const uint32_t base = ring + stage * kStageBytes;
-      const uint32_t halves = there >> (2 * stage) & 3u;
-      const int pos0 = (now.tile + static_cast<int>(i)) * kUnit + warp * kTile;
-      advance();  // into the stage that the tile before this one has left
-      if (halves != 0 && pos0 < most) {
+    for (int i = 0; i < n; ++i) {
+      const int pos0 = (now.tile + i) * kUnit + warp * kTile;
+      ok = ok && wait_warp(&sm.full[stage], parity, p.err);
+      const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
+      if (halves != 0 && pos0 < most && ok) {
         // ---- S^T: positions (rows g, g + 8 of each half) x query rows (columns)
         float s[2][NT][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) s[h][j][c] = 0.f;
         uint32_t kw[2][2][4];  // half, row g or g + 8, word
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint4 k = ld_shared_v4(base + h * 1024 + (g + 8 * r) * 64 + t * 16);
+            const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
             kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
           }
         }
@@ -389,7 +477,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
             uint32_t a[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t y0 = kw[h][0][w] >> (8 * b), y1 = kw[h][1][w] >> (8 * b);
+              const uint32_t y0 = b ? shift8(kw[h][0][w], by8) : kw[h][0][w];
+              const uint32_t y1 = b ? shift8(kw[h][1][w], by8) : kw[h][1][w];
               a[h][0] = y0 & 0x000F000Fu;
               a[h][1] = y1 & 0x000F000Fu;
               a[h][2] = y0 & 0x00F000F0u;
@@ -398,21 +487,33 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               const uint2 qb = kHeld ? q[kHeld ? j : 0][2 * w + b] : sm.q[j][2 * w + b][lane];
-              mma16816(s[0][j], a[0], qb.x, qb.y);
-              mma16816(s[1][j], a[1], qb.x, qb.y);
+              if (w == 0 && b == 0) {
+                mma16816_first(s[0][j], a[0], qb.x, qb.y);
+                mma16816_first(s[1][j], a[1], qb.x, qb.y);
+              } else {
+                mma16816(s[0][j], a[0], qb.x, qb.y);
+                mma16816(s[1][j], a[1], qb.x, qb.y);
+              }
             }
           }
         }
-        // ---- scores; this thread's positions: half h, row g + 8 r stands for (g >> 1) + 4 (g & 1) + 8 r
-        float sv[2][2], mv[2][2];  // step of V, and what code 7.5 stands for
+        // Folded: with at most four rows the columns hold them twice, the first four go on with half 0 and the
+        // last four with half 1, and the scores of a tile are half as many.
+        constexpr int H = kFold ? 1 : 2;
+        if constexpr (kFold) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[0][0][c] = t < 2 ? s[0][0][c] : s[1][0][c];
+        }
+        // ---- scores; this thread's positions: rows g and g + 8 of half h (folded: of half t >> 1)
+        float sv[H][2], mv[H][2];  // step of V, and what code 7.5 stands for
         bool grow = false;
-        const int mine0 = pos0 + (g >> 1) + 4 * (g & 1);
         const bool full = halves == 3u && pos0 + kTile <= least;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
+          const int half = kFold ? t >> 1 : h;
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint2 sc = ld_shared_v2(base + 4096 + h * 128 + ((g >> 1) + 4 * (g & 1) + 8 * r) * 8);
+            const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + half * 128 + r * 64);
             const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
             sv[h][r] = __uint_as_float(sc.y << 16);
             mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
@@ -425,11 +526,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
         }
         if (!full) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < H; ++h) {
+            const int half = kFold ? t >> 1 : h;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const int pos = mine0 + 16 * h + 8 * r;
-              const bool held = (halves >> h & 1u) && pos < now.s.vis;
+              const int pos = pos0 + 16 * half + g + 8 * r;
+              const bool held = (halves >> half & 1u) && pos < now.s.vis;
               if (!held) sv[h][r] = mv[h][r] = 0.f;
 #pragma unroll
               for (int j = 0; j < NT; ++j)
@@ -440,18 +542,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
           }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < H; ++h)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             grow |= sv[h][r] > v_limit;
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int c = 0; c < 2; ++c) grow |= s[h][j][2 * r + c] > m[j][c] + kSlack;
+              for (int c = 0; c < 2; ++c) grow |= s[h][j][2 * r + c] > m_limit[j][c];
           }
         if (__any_sync(0xffffffffu, grow)) {
           // ---- new references: the rows' maxima so far, and a power of two near V's largest step
-          float top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+          float top = 0.f;
+#pragma unroll
+          for (int h = 0; h < H; ++h) top = fmaxf(top, fmaxf(sv[h][0], sv[h][1]));
 #pragma unroll
           for (int off = 1; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
           float change = 1.f;
@@ -469,12 +573,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
           for (int j = 0; j < NT; ++j) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float mx = fmaxf(fmaxf(s[0][j][c], s[0][j][2 + c]), fmaxf(s[1][j][c], s[1][j][2 + c]));
+              float mx = m[j][c];
+#pragma unroll
+              for (int h = 0; h < H; ++h) mx = fmaxf(mx, fmaxf(s[h][j][c], s[h][j][2 + c]));
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-              mx = fmaxf(mx, m[j][c]);
               const float f = ex2(m[j][c] - mx);
               m[j][c] = mx;
+              m_limit[j][c] = mx + kSlack;
               l[j][c] *= f;
               mid[j][c] *= f;
               ps[j][c] *= f * change;
@@ -489,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
         // ---- P, its sums, and P^T step_v as the B operand of O^T
         uint32_t pb[2][NT][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const float f = sv[h][r] * v_unit;
@@ -504,34 +610,46 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
             }
           }
         }
-        // ---- O^T += V^T P^T: values 16 g + 2 i (rows g) and 16 g + 2 i + 1 (rows g + 8, codes four bits
-        // higher) of positions t, 4 + t, 8 + t, 12 + t
+        if constexpr (kFold) {  // columns of the other half: nothing
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t both = pb[0][0][r];
+            pb[0][0][r] = g < 4 ? both : 0u;
+            pb[1][0][r] = g < 4 ? 0u : both;
+          }
+        }
+        // ---- O^T += V^T P^T: of 32 values (a 16-byte piece) 4 g + 2 b (rows g) and 4 g + 2 b + 1 (rows g + 8,
+        // codes four bits higher)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           constexpr uint32_t kOne = 0x3C003C00u;
           const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
 #pragma unroll
           for (int j = 0; j < NT; ++j) mma16816(ps[j], ones, pb[h][j][0], pb[h][j][1]);
-          uint2 v[4];
 #pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4)
-            v[i4] = ld_shared_v2(base + 2048 + h * 1024 + (4 * i4 + t) * 64 + (((g >> 1) ^ (t & 2)) * 16) + (g & 1) * 8);
+          for (int w = 0; w < 4; w += 2) {
+            uint32_t v[4];  // piece w: rows 0-7 and 8-15, piece w + 1: the same
+            ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + h * 1024 + (w ^ v_piece) * 16);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {  // 4 values: half (w & 1) of word (w >> 1)
-            const uint32_t sel = w & 1 ? 0x7632u : 0x5410u;
-            const uint32_t x0 = __byte_perm(w < 2 ? v[0].x : v[0].y, w < 2 ? v[1].x : v[1].y, sel);
-            const uint32_t x1 = __byte_perm(w < 2 ? v[2].x : v[2].y, w < 2 ? v[3].x : v[3].y, sel);
+            for (int x = 0; x < 2; ++x) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const uint32_t y0 = x0 >> (8 * b), y1 = x1 >> (8 * b);
-              const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
+              for (int b = 0; b < 2; ++b) {
+                const uint32_t y0 = b ? shift8(v[2 * x], by8) : v[2 * x];
+                const uint32_t y1 = b ? shift8(v[2 * x + 1], by8) : v[2 * x + 1];
+                const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
 #pragma unroll
-              for (int j = 0; j < NT; ++j) mma16816(o[j][2 * w + b], a, pb[h][j][0], pb[h][j][1]);
+                for (int j = 0; j < NT; ++j) mma16816(o[j][2 * (w + x) + b], a, pb[h][j][0], pb[h][j][1]);
+              }
             }
           }
         }
       }
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      __syncwarp();  // every lane has read the stage
+      if (lane == 0) mbar_arrive(&sm.empty[stage]);
+      if (++stage == kStages) {
+        stage = 0;
+        parity ^= 1u;
+      }
     }
 
     // ---- the piece's sums: the warps' parts joined through shared memory, a plane at a time
@@ -550,29 +668,35 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
           sm.m[warp][2 * t + c] = m[j][c];
           sm.l[warp][2 * t + c] = l[j][c];
         }
-        // value 16 g + 2 i + b at place 16 i + 2 g + b
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; ++i) {  // values 32 (i >> 1) + 4 g + 2 (i & 1) and the one after it
           const float y0 = fmaf(fmaf(o[j][i][c], unit_even, -7.5f * ps[j][c]), back, mid[j][c]);
           const float y1 = fmaf(fmaf(o[j][i][2 + c], unit_odd, -7.5f * ps[j][c]), back, mid[j][c]);
-          *reinterpret_cast<float2*>(&sm.o[warp][2 * t + c][16 * i + 2 * g]) = make_float2(y0, y1);
+          *reinterpret_cast<float2*>(&sm.o[warp][2 * t + c][32 * (i >> 1) + 4 * g + 2 * (i & 1)]) = make_float2(y0, y1);
         }
       }
-      __syncthreads();
+      sync_compute();
+      constexpr int kRows = kFold ? 4 : 8;
 #pragma unroll
-      for (int idx = tid; idx < 8 * 64; idx += kThreads) {
-        const int row = idx >> 6, place = 2 * (idx & 63);
+      for (int idx = tid; idx < kRows * 64; idx += kWarps * 32) {
+        const int row = idx >> 6, value = 2 * (idx & 63);
         float mx = kNone;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.m[w][row]);
+        for (int w = 0; w < kWarps; ++w) {
+          mx = fmaxf(mx, sm.m[w][row]);
+          if (kFold) mx = fmaxf(mx, sm.m[w][row + 4]);
+        }
         float y0 = 0.f, y1 = 0.f, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float f = ex2(sm.m[w][row] - mx);
-          const float2 y = *reinterpret_cast<const float2*>(&sm.o[w][row][place]);
-          y0 = fmaf(y.x, f, y0);
-          y1 = fmaf(y.y, f, y1);
-          sum = fmaf(sm.l[w][row], f, sum);
+#pragma unroll
+          for (int f4 = 0; f4 < (kFold ? 8 : 4); f4 += 4) {
+            const float f = ex2(sm.m[w][row + f4] - mx);
+            const float2 y = *reinterpret_cast<const float2*>(&sm.o[w][row + f4][value]);
+            y0 = fmaf(y.x, f, y0);
+            y1 = fmaf(y.y, f, y1);
+            sum = fmaf(sm.l[w][row + f4], f, sum);
+          }
         }
         const int in_group = 8 * j + row;
         if (whole) {
@@ -581,95 +705,132 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) int4_decode_kernel(
             const int token = r / p.group;
             // 0 for a row that sees nothing
             const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-            const int value = 16 * (place >> 1 & 7) + 2 * (place >> 4);
-            uint16_t* dst = p.out + (now.s.q_first + token) * p.out_row_stride +
+            uint16_t* dst = p.out + (static_cast<int64_t>(now.s.q_first) + token) * p.out_row_stride +
                             (kvh * p.group + r - token * p.group) * kHeadDim + value;
             *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(y0 * inv, y1 * inv);
           }
         } else {
-          *reinterpret_cast<float2*>(part + in_group * kHeadDim + place) = make_float2(y0, y1);
-          if (place == 0) *reinterpret_cast<float2*>(part + R * kHeadDim + 2 * in_group) = make_float2(mx, sum);
+          *reinterpret_cast<float2*>(part + in_group * kHeadDim + value) = make_float2(y0, y1);
+          if (value == 0) *reinterpret_cast<float2*>(part + R * kHeadDim + 2 * in_group) = make_float2(mx, sum);
         }
       }
-      __syncthreads();
+      sync_compute();
     }
     // ---- on to the next pair
     u += n;
-    now.tile += static_cast<int>(n) - 1;
-    if (u < u1) next_unit<NT>(p, now);
+    if (u < u1) {
+      next_pair<R>(p, now);
+    } else if (tid == 0) {
+      Cut cut = {};
+      if (now.tile == 0 && n < now.s.tiles) {
+        cut.parts = static_cast<int>(owner(u - n + now.s.tiles - 1, ctas, total) - blockIdx.x + 1);
+        cut.slot = 2 * blockIdx.x + (u - n > u0 ? 1 : 0);
+        cut.rows = min(R, rows - rg * R);
+        cut.first_row = rg * R;
+        cut.token = now.s.q_first;
+        cut.head = kvh * p.group;
+      }
+      cuts[blockIdx.x] = cut;
+    }
   }
-  cp_async_wait<0>();
 }
 
-// Joins the parts of cut pairs: one warp for each (pair, row), parts in order.  The pairs of a sequence are
-// found from the published prefix.
-template <int NT>
-__global__ void __launch_bounds__(128) int4_join_kernel(const Int4AttnParams p, int grid) {
+// Joins the parts of cut pairs: CTA i those of the pair that the first kernel's CTA i left cut.  kJoinWarps warps share
+// the pair's rows; several warps of a row take parts in turn and add what they have in order.
+constexpr int kJoinWarps = 8;
+template <int R>
+__global__ void __launch_bounds__(kJoinWarps * 32) int4_join_kernel(const __grid_constant__ Int4AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  constexpr int R = 8 * NT;
-  const int lane = threadIdx.x & 31;
-  const int s = blockIdx.y;
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 5);  // (row group, kv head, row)
-  const Seq q = seq_of<NT>(p, s);
-  const int pair = item / R, row = item - pair * R;
-  if (pair >= q.groups * p.num_kv_heads) return;
-  const int kvh = pair % p.num_kv_heads, rg = pair / p.num_kv_heads, r = rg * R + row;
-  if (r >= q.nq * p.group) return;
-  const int64_t total = p.prefix[p.num_seqs], ctas = min(static_cast<int64_t>(grid), total);
-  const int64_t a = p.prefix[s] + static_cast<int64_t>(pair) * q.tiles, b = a + q.tiles;
-  const int64_t c0 = owner(a, ctas, total), c1 = owner(b - 1, ctas, total);
-  if (c0 == c1) return;  // one CTA had all of it
-  constexpr int64_t kPart = R * (kHeadDim + 2);
-  const int64_t slot0 = 2 * c0 + (a > range_begin(c0, ctas, total) ? 1 : 0);
-  float mx = kNone;
-  for (int64_t c = c0 + lane; c <= c1; c += 32) {
-    const float* part = p.partials + (c == c0 ? slot0 : 2 * c) * kPart;
-    mx = fmaxf(mx, part[R * kHeadDim + 2 * row]);
-  }
+  __shared__ float4 sum_o[kJoinWarps][32];
+  __shared__ float2 sum_ml[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Cut cut = reinterpret_cast<const Cut*>(p.cuts)[blockIdx.x];
+  const int parts = cut.parts;
+  if (parts == 0) return;
+  constexpr int kPart = R * (kHeadDim + 2);
+  const float* first = p.partials + static_cast<int64_t>(cut.slot) * kPart;
+  const float* later = p.partials + static_cast<int64_t>(2 * blockIdx.x) * kPart;
+  auto part = [&](int j) { return j == 0 ? first : later + static_cast<int64_t>(2 * j) * kPart; };
+  const int share = max(1, min(kJoinWarps / cut.rows, parts));  // warps of a row
+  const int at_once = kJoinWarps / share;                       // rows
+  for (int row0 = 0; row0 < cut.rows; row0 += at_once) {
+    const int row = row0 + warp / share, turn = warp % share;
+    const bool mine = warp < at_once * share && row < cut.rows;
+    float mx = kNone, sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mine) {
+      for (int j = turn + lane * share; j < parts; j += 32 * share) mx = fmaxf(mx, part(j)[R * kHeadDim + 2 * row]);
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-#pragma unroll 4
-  for (int64_t c = c0; c <= c1; ++c) {
-    const float* part = p.partials + (c == c0 ? slot0 : 2 * c) * kPart;
-    const float2 ml = *reinterpret_cast<const float2*>(part + R * kHeadDim + 2 * row);
-    const float4 x = *reinterpret_cast<const float4*>(part + row * kHeadDim + 4 * lane);
-    const float f = ex2(ml.x - mx);
-    y.x = fmaf(x.x, f, y.x);
-    y.y = fmaf(x.y, f, y.y);
-    y.z = fmaf(x.z, f, y.z);
-    y.w = fmaf(x.w, f, y.w);
-    sum = fmaf(ml.y, f, sum);
+      for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+#pragma unroll 8
+      for (int j = turn; j < parts; j += share) {
+        const float2 ml = *reinterpret_cast<const float2*>(part(j) + R * kHeadDim + 2 * row);
+        const float4 x = *reinterpret_cast<const float4*>(part(j) + row * kHeadDim + 4 * lane);
+        const float f = ex2(ml.x - mx);
+        y.x = fmaf(x.x, f, y.x);
+        y.y = fmaf(x.y, f, y.y);
+        y.z = fmaf(x.z, f, y.z);
+        y.w = fmaf(x.w, f, y.w);
+        sum = fmaf(ml.y, f, sum);
+      }
+    }
+    if (share > 1) {
+      __syncthreads();  // the rows before these have been read
+      sum_o[warp][lane] = y;
+      if (lane == 0) sum_ml[warp] = make_float2(mx, sum);
+      __syncthreads();
+      if (mine && turn == 0) {
+        float top = kNone;
+        for (int w = 0; w < share; ++w) top = fmaxf(top, sum_ml[warp + w].x);
+        y = make_float4(0.f, 0.f, 0.f, 0.f);
+        sum = 0.f;
+        for (int w = 0; w < share; ++w) {
+          const float f = ex2(sum_ml[warp + w].x - top);
+          const float4 x = sum_o[warp + w][lane];
+          y.x = fmaf(x.x, f, y.x);
+          y.y = fmaf(x.y, f, y.y);
+          y.z = fmaf(x.z, f, y.z);
+          y.w = fmaf(x.w, f, y.w);
+          sum = fmaf(sum_ml[warp + w].y, f, sum);
+        }
+      }
+    }
+    if (mine && turn == 0) {
+      const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+      const int r = cut.first_row + row, token = r / p.group;
+      __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(
+          p.out + (static_cast<int64_t>(cut.token) + token) * p.out_row_stride +
+          (cut.head + r - token * p.group) * kHeadDim + 4 * lane);
+      dst[0] = __floats2bfloat162_rn(y.x * inv, y.y * inv);
+      dst[1] = __floats2bfloat162_rn(y.z * inv, y.w * inv);
+    }
   }
-  const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-  const int token = r / p.group, place = 4 * lane;
-  uint16_t* dst = p.out + (q.q_first + token) * p.out_row_stride +
-                  (kvh * p.group + r - token * p.group) * kHeadDim + 2 * (place >> 4);
-  *reinterpret_cast<__nv_bfloat162*>(dst + 16 * (place >> 1 & 7)) = __floats2bfloat162_rn(y.x * inv, y.y * inv);
-  *reinterpret_cast<__nv_bfloat162*>(dst + 16 * ((place >> 1 & 7) + 1)) = __floats2bfloat162_rn(y.z * inv, y.w * inv);
 }
 
 template <int NT>
+constexpr int kSmemBytes = static_cast<int>(sizeof(Smem<NT>)) + 1024;  // its alignment
+
+template <int NT, bool kFold>
 cudaError_t prepare() {
-  return cudaFuncSetAttribute(int4_decode_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(sizeof(Smem<NT>)));
+  return cudaFuncSetAttribute(int4_decode_kernel<NT, kFold>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              kSmemBytes<NT>);
 }
 
-template <int NT>
+template <int NT, bool kFold>
 int resident(int num_sms) {  // CTAs that run at once
   int per_sm = 0;
-  if (prepare<NT>() != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int4_decode_kernel<NT>, kThreads, sizeof(Smem<NT>)) !=
-          cudaSuccess)
+  if (prepare<NT, kFold>() != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int4_decode_kernel<NT, kFold>, kThreads,
+                                                    kSmemBytes<NT>) != cudaSuccess)
     return 0;
   return per_sm * num_sms;
 }
 
-template <int NT>
-cudaError_t launch(const Int4AttnParams& p, int grid, int max_groups, cudaStream_t stream) {
-  cudaError_t e = prepare<NT>();
+template <int NT, bool kFold>
+cudaError_t launch(const Int4AttnParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid,
+                   cudaStream_t stream) {
+  cudaError_t e = prepare<NT, kFold>();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -677,57 +838,66 @@ cudaError_t launch(const Int4AttnParams& p, int grid, int max_groups, cudaStream
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Smem<NT>);
+  cfg.dynamicSmemBytes = kSmemBytes<NT>;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, int4_decode_kernel<NT>, p);
-  if (e != cudaSuccess) return e;
-  const int64_t rows = static_cast<int64_t>(max_groups) * p.num_kv_heads * 8 * NT;
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4), static_cast<unsigned>(p.num_seqs));
-  cfg.blockDim = dim3(128);
+  e = cudaLaunchKernelEx(&cfg, int4_decode_kernel<NT, kFold>, p, map_k, map_v);
+  if (e != cudaSuccess || grid < 2) return e;
+  cfg.gridDim = dim3(static_cast<unsigned>(grid - 1));
+  cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, int4_join_kernel<NT>, p, grid);
+  return cudaLaunchKernelEx(&cfg, int4_join_kernel<kFold ? 4 : 8 * NT>, p);
 }
 
-// Planes of 8 rows in a row group: as many as the longest chunk of one kv head's rows needs, at most four.
-int planes(int group, int max_q) {
+// The kernel for a call: 0 for at most four rows of a kv head, else planes of 8 rows in a row group, as many as the
+// longest chunk's rows need, at most four.
+int variant(int group, int max_q) {
   const int64_t rows = static_cast<int64_t>(group) * max_q;
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
+  return rows <= 4 ? 0 : rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
 }
+int rows_of(int v) { return v == 0 ? 4 : 8 * v; }
 
 }  // namespace
 
+cudaError_t int4_error_word(void** word) { return cudaGetSymbolAddress(word, g_error); }
+
 int int4_decode_grid(int group, int max_q) {
   constexpr int kMaxDevices = 64;
-  static std::atomic<int> known[kMaxDevices][4];  // by device and planes; 0: not asked yet
+  static std::atomic<int> known[kMaxDevices][5];  // by device and variant; 0: not asked yet
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
-  const int nt = planes(group, max_q);
-  int n = known[dev][nt - 1].load(std::memory_order_relaxed);
+  const int v = variant(group, max_q);
+  int n = known[dev][v].load(std::memory_order_relaxed);
   if (n == 0) {
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    n = nt == 1 ? resident<1>(sms) : nt == 2 ? resident<2>(sms) : nt == 3 ? resident<3>(sms) : resident<4>(sms);
-    known[dev][nt - 1].store(n, std::memory_order_relaxed);
+    n = v == 0   ? resident<1, true>(sms)
+        : v == 1 ? resident<1, false>(sms)
+        : v == 2 ? resident<2, false>(sms)
+        : v == 3 ? resident<3, false>(sms)
+                 : resident<4, false>(sms);
+    known[dev][v].store(n, std::memory_order_relaxed);
   }
   return n;
 }
 
-int64_t int4_decode_workspace_bytes(int num_seqs, int group, int max_q, int grid) {
-  const int64_t part = 8ll * planes(group, max_q) * (kHeadDim + 2) * 4;
-  return (num_seqs + 2ll) / 2 * 16 + 2ll * grid * part;
+int64_t int4_decode_workspace_bytes(int group, int max_q, int grid) {
+  const int64_t part = static_cast<int64_t>(rows_of(variant(group, max_q))) * (kHeadDim + 2) * 4;
+  return static_cast<int64_t>(grid) * (sizeof(Cut) + 2 * part);
 }
 
-cudaError_t launch_int4_decode(Int4AttnParams p, void* workspace, int grid, cudaStream_t stream) {
-  const int nt = planes(p.group, p.max_q);
-  p.prefix = static_cast<int64_t*>(workspace);
-  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (p.num_seqs + 2ll) / 2 * 16);
-  const int groups = static_cast<int>((static_cast<int64_t>(p.group) * p.max_q + 8 * nt - 1) / (8 * nt));
-  switch (nt) {
-    case 1: return launch<1>(p, grid, groups, stream);
-    case 2: return launch<2>(p, grid, groups, stream);
-    case 3: return launch<3>(p, grid, groups, stream);
-    default: return launch<4>(p, grid, groups, stream);
+cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, void* workspace,
+                               int grid, cudaStream_t stream) {
+  p.cuts = workspace;
+  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + grid * sizeof(Cut));
+  p.unit_pages = kUnit / p.block_size;
+  p.unit_rest = kUnit % p.block_size;
+  switch (variant(p.group, p.max_q)) {
+    case 0: return launch<1, true>(p, map_k, map_v, grid, stream);
+    case 1: return launch<1, false>(p, map_k, map_v, grid, stream);
+    case 2: return launch<2, false>(p, map_k, map_v, grid, stream);
+    case 3: return launch<3, false>(p, map_k, map_v, grid, stream);
+    default: return launch<4, false>(p, map_k, map_v, grid, stream);
   }
 }
 

@@ -243,12 +243,18 @@ struct Int4AttnParams {
   int64_t num_blocks;
   int max_q;  // sequences with more new tokens are left to the other kernel
   float scale_log2;  // softmax_scale * log2(e)
-  int64_t* prefix;  // workspace: units before each sequence, [num_seqs + 1]
+  int box_rows;     // rows of a TMA box: the largest of 128, 64, 32 and 16 that divides block_size
+  int unit_pages, unit_rest;  // set by the launch
+  int* err;         // device error word
+  void* cuts;       // workspace: for each CTA the pair that its range leaves cut
   float* partials;  // workspace: two parts for each CTA
 };
 int int4_decode_grid(int group, int max_q);  // CTAs that run at once on the current device; 0: error
-int64_t int4_decode_workspace_bytes(int num_seqs, int group, int max_q, int grid);
-cudaError_t launch_int4_decode(Int4AttnParams p, void* workspace, int grid, cudaStream_t stream);
+int64_t int4_decode_workspace_bytes(int group, int max_q, int grid);
+cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, void* workspace,
+                               int grid, cudaStream_t stream);
+// The error word of the 4-bit attention kernels on the current device.
+cudaError_t int4_error_word(void** word);
 
 // ------------------------------------------------------------------ decode engine
 // Control block at the head of the decode workspace (ints):

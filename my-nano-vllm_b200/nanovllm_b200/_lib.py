@@ -114,6 +114,8 @@ def _load() -> ctypes.CDLL:
     lib.fp8attn_int4_prefill.restype = i32
     lib.fp8attn_int4_prefill.argtypes = [vp, vp, i64, vp, vp, vp, vp, i64, i32, vp, vp, i32, i32, i32,
                                          i32, i32, i64, i32, f32, vp, i64, vp]
+    lib.fp8attn_int4_read_error.restype = i32
+    lib.fp8attn_int4_read_error.argtypes = [vp, i32, vp]
     return lib
 
 

@@ -20,6 +20,7 @@ from . import _lib
 _WORKSPACES: dict[tuple[int, int, int], torch.Tensor] = {}  # by device, stream, capture (0: none)
 _REPLACED: list[tuple[int, torch.Tensor]] = []  # that captured launches still hold, by device
 _MOE_DEVICES: set[int] = set()  # where fp8_moe has run: it has an error word of the library's own
+_INT4_DEVICES: set[int] = set()  # where int4_cache's attention has run: the same
 _RELAXED = 2  # cudaStreamCaptureModeRelaxed
 
 
@@ -75,18 +76,20 @@ def _zeros_beside_capture(index: int, nbytes: int) -> torch.Tensor:
 
 
 def device_error(device: torch.device | None = None) -> int:
-    """Largest device-side error word over the workspaces of ``device`` and its mixture-of-experts calls
-    (0 = none).  Reads device memory: for tests and diagnostics only."""
+    """Largest device-side error word over the workspaces of ``device``, its mixture-of-experts calls and its
+    attention over 4-bit caches (0 = none).  Reads device memory: for tests and diagnostics only."""
     worst = 0
     for dev, ws in [(key[0], ws) for key, ws in _WORKSPACES.items()] + _REPLACED:
         if device is None or dev == torch.device(device).index:
             worst = max(worst, int(ws[:4].view(torch.int32).item()))
-    for dev in sorted(_MOE_DEVICES):
-        if device is None or dev == torch.device(device).index:
-            with torch.cuda.device(dev):
-                word = torch.empty(1, dtype=torch.int32, device=dev)
-                _lib.check(_lib.lib.fp8attn_fp8_moe_read_error(word.data_ptr(), 0, _stream(word.device)))
-                worst = max(worst, int(word.item()))
+    for devices, read in ((_MOE_DEVICES, _lib.lib.fp8attn_fp8_moe_read_error),
+                          (_INT4_DEVICES, _lib.lib.fp8attn_int4_read_error)):
+        for dev in sorted(devices):
+            if device is None or dev == torch.device(device).index:
+                with torch.cuda.device(dev):
+                    word = torch.empty(1, dtype=torch.int32, device=dev)
+                    _lib.check(read(word.data_ptr(), 0, _stream(word.device)))
+                    worst = max(worst, int(word.item()))
     return worst
 
 

@@ -21,7 +21,8 @@ step, without the norms:
 
 All launch on ``torch.cuda.current_stream()`` of the tensors' device, allocate outputs and scratch with
 ``torch.empty`` (scratch is one call's own) and never synchronise or read device memory on the host, so
-they can be captured into CUDA graphs.
+they can be captured into CUDA graphs.  A device wait of the attention that gives up is recorded in a word
+of the library's own (``fp8_attention.device_error``).
 """
 from __future__ import annotations
 
@@ -30,6 +31,7 @@ import functools
 import torch
 
 from . import _lib
+from .fp8_attention import _INT4_DEVICES
 
 HEAD_DIM = 128
 _BF16, _U8, _I32 = torch.bfloat16, torch.uint8, torch.int32
@@ -153,6 +155,7 @@ def int4_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     out = _empty((batch, heads, HEAD_DIM), (width, HEAD_DIM, 1), dtype=_BF16, device=q.device)
     if batch == 0:
         return out
+    _INT4_DEVICES.add(device)
     nbytes = _scratch_bytes(device, batch, heads, kv_heads, 1)
     scratch = _empty((max(nbytes, 0),), (1,), dtype=_U8, device=q.device)
     columns = block_tables.shape[1]
@@ -204,6 +207,7 @@ def int4_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         return out
     # no sequence has more new tokens than there are rows
     max_q = min(int(max_seqlen_q), tokens)
+    _INT4_DEVICES.add(device)
     nbytes = _scratch_bytes(device, num_seqs, heads, kv_heads, max_q)
     scratch = _empty((max(nbytes, 0),), (1,), dtype=_U8, device=q.device)
     columns = block_tables.shape[1]
