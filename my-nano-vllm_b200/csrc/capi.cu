@@ -1220,12 +1220,33 @@ int fp8attn_int4_load(const void* k_cache, const void* v_cache, const void* kv_s
   return FP8ATTN_OK;
 }
 
+// Which kernels a call takes: sequences with at most short_q new tokens (32 query rows of a kv head) go to the
+// split-context kernel, longer ones to the kernel for long chunks.
+struct Int4Plan {
+  int short_q;       // 0: no sequence goes to the first kernel
+  bool longer;       // whether the second is launched
+  int grid;          // of the first
+  int64_t short_bytes, bytes;
+};
+
+static int int4_plan(Int4Plan* plan, int group, int max_q) {
+  constexpr int kShortRows = 32;
+  // a single token of any group stays with the first kernel, which takes wider groups in parts
+  const int limit = group >= kShortRows ? 1 : kShortRows / group;
+  plan->short_q = max_q < limit ? max_q : limit;
+  plan->longer = max_q > limit;
+  plan->grid = fp8attn::int4_decode_grid(group, plan->short_q);
+  if (plan->grid <= 0) return fail(FP8ATTN_ECUDA, "no kernel for this device");
+  plan->short_bytes = (fp8attn::int4_decode_workspace_bytes(group, plan->short_q, plan->grid) + 255) / 256 * 256;
+  plan->bytes = plan->short_bytes + (plan->longer ? fp8attn::int4_prefill_workspace_bytes(device_sms()) : 0);
+  return FP8ATTN_OK;
+}
+
 int64_t fp8attn_int4_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int max_seqlen_q) {
   if (num_seqs < 0 || num_seqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads) return -1;
-  const int group = num_heads / num_kv_heads, max_q = max_seqlen_q < 1 ? 1 : max_seqlen_q;
-  const int grid = fp8attn::int4_decode_grid(group, max_q);
-  if (grid <= 0) return -1;
-  return fp8attn::int4_decode_workspace_bytes(group, max_q, grid);
+  Int4Plan plan;
+  if (int4_plan(&plan, num_heads / num_kv_heads, max_seqlen_q < 1 ? 1 : max_seqlen_q)) return -1;
+  return plan.bytes;
 }
 
 static int int4_attention(void* out, const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
@@ -1261,12 +1282,12 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   p.num_blocks = num_blocks;
   p.max_q = max_q;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  const int grid = fp8attn::int4_decode_grid(p.group, max_q);
-  if (grid <= 0) return fail(FP8ATTN_ECUDA, "no kernel for this device");
-  const int64_t need = fp8attn::int4_decode_workspace_bytes(p.group, max_q, grid);
-  if (workspace == nullptr || workspace_bytes < need)
+  Int4Plan plan;
+  rc = int4_plan(&plan, p.group, max_q);
+  if (rc) return rc;
+  if (workspace == nullptr || workspace_bytes < plan.bytes)
     return fail(FP8ATTN_EWORKSPACE, "workspace of %lld bytes is smaller than the %lld needed",
-                static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+                static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
   if (!aligned16(workspace)) return fail(FP8ATTN_EINVAL, "workspace must be 16-byte aligned");
   p.box_rows = box_rows_for(block_size);
   rc = int4_error(&p.err);
@@ -1277,8 +1298,17 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   if (rc) return rc;
   rc = make_codes_map(&map_v, v_cache, rows, p.box_rows);
   if (rc) return rc;
-  const cudaError_t e =
-      fp8attn::launch_int4_decode(p, map_k, map_v, workspace, grid, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (plan.longer) {
+    p.min_q = plan.short_q;
+    p.max_q = max_q;
+    const cudaError_t e = fp8attn::launch_int4_prefill(
+        p, map_k, map_v, static_cast<uint8_t*>(workspace) + plan.short_bytes, device_sms(), st);
+    if (e != cudaSuccess) return cuda_fail(e, "4-bit chunk attention launch");
+  }
+  p.min_q = 0;
+  p.max_q = plan.short_q;
+  const cudaError_t e = fp8attn::launch_int4_decode(p, map_k, map_v, workspace, plan.grid, st);
   if (e != cudaSuccess) return cuda_fail(e, "4-bit attention launch");
   return FP8ATTN_OK;
 }

@@ -241,6 +241,7 @@ struct Int4AttnParams {
   int group;  // query heads per kv head
   int block_size;
   int64_t num_blocks;
+  int min_q;  // chunks, long: sequences with at most so many new tokens are left to the other kernel
   int max_q;  // sequences with more new tokens are left to the other kernel
   float scale_log2;  // softmax_scale * log2(e)
   int box_rows;     // rows of a TMA box: the largest of 128, 64, 32 and 16 that divides block_size
@@ -253,6 +254,9 @@ int int4_decode_grid(int group, int max_q);  // CTAs that run at once on the cur
 int64_t int4_decode_workspace_bytes(int group, int max_q, int grid);
 cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, void* workspace,
                                int grid, cudaStream_t stream);
+int64_t int4_prefill_workspace_bytes(int num_sms);
+cudaError_t launch_int4_prefill(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, void* workspace,
+                                int num_sms, cudaStream_t stream);
 // The error word of the 4-bit attention kernels on the current device.
 cudaError_t int4_error_word(void** word);
 

@@ -22,8 +22,9 @@ LIB_PATH = os.path.join(PKG_DIR, "libfp8attn.so")
 
 SOURCES = ["capi.cu", "store.cu", "decode.cu", "prefill.cu", "prefill_persistent.cu", "diag.cu",
            "qknorm.cu", "fp8linear.cu", "ffn_quant.cu", "moe.cu", "rope.cu", "int4_cache.cu",
-           "int4_decode.cu"]
-HEADERS = ["common.cuh", "kernels.h", "tcgen05.cuh", "prefill_common.cuh"]
+           "int4_decode.cu", "int4_prefill.cu"]
+HEADERS = ["common.cuh", "kernels.h", "tcgen05.cuh", "prefill_common.cuh",
+           "int4_attention.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
