@@ -31,30 +31,33 @@ namespace {
 constexpr int kRows = 128;          // of a group
 constexpr int kItem = 2 * kRows;    // rows of a work item
 constexpr int kTile = 128;          // positions
-constexpr int kRaw = 3;             // stages of codes
+constexpr int kPieceUnits = 2;      // what a work item costs beside its tiles, in units of a tile
+constexpr int kRaw = 3;             // stages of codes, K 0, K 1, V 0, K 2, V 1, ...
 constexpr int kThreads = 512;
 constexpr int kUnpackWarp = 8, kLoadWarp = 12, kMmaWarp = 13;
-constexpr int kSoftmaxRegs = 184, kUnpackRegs = 88, kOtherRegs = 56;
+#ifndef PS
+#define PS 184
+#define PU 88
+#define PO 56
+#endif
+constexpr int kSoftmaxRegs = PS, kUnpackRegs = PU, kOtherRegs = PO;
 static_assert(2 * kSoftmaxRegs + kUnpackRegs + kOtherRegs == 4 * 128, "all of the registers, and no more");
 constexpr float kSlack = 8.f;  // a reference maximum may lag by 2^8
 constexpr float kLift = 4.f;   // P and its sums are 2^4 times as large: P between 2^-14 and 2^12 is a normal number
 constexpr int kOBytes = kTile * 128;  // a 64-value block of an operand: 128 rows of 128 bytes
 
-constexpr uint32_t kWild = 1u << 8;   // beside the eight parts of a tile: it has rows that are not finite
-
 struct __align__(1024) Smem {
   uint8_t q[2][2 * kOBytes];   // K-major, 128B swizzle, two blocks of 64 values
   uint8_t k[2][2 * kOBytes];
-  uint8_t v[2 * kOBytes];      // MN-major, the same layout
-  uint8_t raw_k[kRaw][kTile * 64];  // codes, 64B swizzle
-  uint8_t raw_v[kRaw][kTile * 64];
-  uint2 raw_scale[kRaw][kTile];
-  uint32_t raw_there[kRaw];    // which 16 positions are in pages of the cache
+  uint8_t v[2][2 * kOBytes];   // MN-major, the same layout
+  uint8_t raw[kRaw][kTile * 64];  // codes of K or V, 64B swizzle
+  uint2 raw_scale[kRaw][kTile];   // beside codes of K: scales of both
+  uint32_t raw_there[kRaw];       // and which 16 positions are in pages of the cache
   // of a tile, by unit mod 4: its power of two of K; what V's power changes O by; V's power; raw_there
   float k_back[4], v_change[4], v_back[4];
   uint32_t there[4];
   uint64_t raw_full[kRaw], raw_empty[kRaw];
-  uint64_t k_full[2], k_free[2], v_full, v_free;
+  uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
   uint64_t drained;
   int64_t scan[kThreads / 32];
@@ -77,43 +80,79 @@ __device__ __forceinline__ Seq seq_of(const Int4AttnParams& p, int s) {
   q.groups = (q.nq * p.group + kItem - 1) / kItem;
   return q;
 }
-// Tiles that a row group sees: those of its last row, and one where it sees none (zeros are written).
-__device__ __forceinline__ int tiles_of(const Int4AttnParams& p, const Seq& q, int rg) {
-  const int last = (min(q.nq * p.group, (rg + 1) * kItem) - 1) / p.group;
-  return max(1, (min(q.vis, last + q.nk - q.nq + 1) + kTile - 1) / kTile);
-}
+// Row groups of a sequence one after another: how many tiles each sees (those of its last row, and one where it sees
+// none: zeros are written), without a division for each.
+struct Groups {
+  int last, rest;  // token of the group's last row, and what is left of the division
+  __device__ __forceinline__ Groups(const Int4AttnParams& p, int rg) {
+    const int row = (rg + 1) * kItem - 1;
+    last = row / p.group;
+    rest = row - last * p.group;
+  }
+  __device__ __forceinline__ int tiles(const Seq& q) const {
+    return max(1, (min(q.vis, min(last, q.nq - 1) + q.nk - q.nq + 1) + kTile - 1) >> 7);
+  }
+  __device__ __forceinline__ void next(const Int4AttnParams& p) {
+    last += p.item_tokens;
+    rest += p.item_rest;
+    if (rest >= p.group) {
+      rest -= p.group;
+      ++last;
+    }
+  }
+};
+static_assert(kTile == 128, "the shift in Groups::tiles");
+__device__ __forceinline__ int tiles_of(const Int4AttnParams& p, const Seq& q, int rg) { return Groups(p, rg).tiles(q); }
 __device__ __forceinline__ int64_t units_of(const Int4AttnParams& p, const Seq& q) {
   int64_t n = 0;
-  for (int rg = 0; rg < q.groups; ++rg) n += tiles_of(p, q, rg);
+  Groups at(p, 0);
+  for (int rg = 0; rg < q.groups; ++rg) {
+    n += at.tiles(q) + kPieceUnits;
+    at.next(p);
+  }
   return n * p.num_kv_heads;
 }
 
-// Where in the order of units a warp is: sequence, row group, kv head, tile.
+// The piece of a work item that a warp is at: sequence, row group, kv head, its tiles [tile, end) of `tiles`.  An item's
+// units are kPieceUnits for what it costs beside its tiles, and then its tiles; a piece is what of it lies in the CTA's
+// range, which ends at unit `until`.
 struct Cursor {
-  int seq, rg, kvh, tile, tiles;
+  int seq, rg, kvh, tile, end, tiles;
+  int64_t begin, until;  // the item's first unit
   Seq s;
+  // Whether another piece with a tile follows.
+  __device__ __forceinline__ bool more() const { return begin + tiles + 2 * kPieceUnits < until; }
+  __device__ __forceinline__ void set_end() {
+    end = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(tiles), until - begin - kPieceUnits)));
+  }
+  __device__ __forceinline__ bool whole() const { return tile == 0 && end == tiles; }
 };
 
-__device__ __forceinline__ void next_pair(const Int4AttnParams& p, Cursor& c) {
+__device__ __forceinline__ void next_piece(const Int4AttnParams& p, Cursor& c) {
   c.tile = 0;
-  if (++c.kvh < p.num_kv_heads) return;
-  c.kvh = 0;
-  if (++c.rg >= c.s.groups) {
-    c.rg = 0;
-    do {
-      if (++c.seq >= p.num_seqs) return;
-      c.s = seq_of(p, c.seq);
-    } while (c.s.groups == 0);
+  c.begin += c.tiles + kPieceUnits;
+  if (++c.kvh >= p.num_kv_heads) {
+    c.kvh = 0;
+    if (++c.rg >= c.s.groups) {
+      c.rg = 0;
+      do {  // there is one: more()
+        c.s = seq_of(p, ++c.seq);
+      } while (c.s.groups == 0);
+    }
+    c.tiles = tiles_of(p, c.s, c.rg);
   }
-  c.tiles = tiles_of(p, c.s, c.rg);
+  c.set_end();
 }
 
-__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, int* err) {
-  return mbar_wait(bar, parity, err);
-}
-
+// A warp's wait, bounded by a number of polls (each of some tens of cycles: a second or more).  Small, since it stands in
+// many places: the roles' loops share the instruction cache.
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, int* err) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+  bool done = false;
+#pragma unroll 1
+  for (uint32_t polls = 0; polls < (1u << 26) && !done; ++polls) done = mbar_try_wait(bar, parity);
+  done = __all_sync(0xffffffffu, done);
+  if (!done) atomicExch(err, kDevErrWaitTimeout);
+  return done;
 }
 
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
@@ -143,21 +182,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-
 // ------------------------------------------------------------------------------------------ loading
 // Lane i < 8 looks up the page of positions 16 i of each tile, and the lanes at which a TMA box begins load it.
 __device__ __forceinline__ void load_role(const Int4AttnParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
-                                          Smem& sm, Cursor c, int64_t units, int lane) {
+                                          Smem& sm, Cursor c, int lane) {
   int column = 0, place = 0;
   auto look_up = [&]() {
     const int pos = c.tile * kTile + lane * 16;
@@ -172,17 +200,32 @@ __device__ __forceinline__ void load_role(const Int4AttnParams& p, const CUtenso
     return look_up();
   };
   int page = find();
-  int stage = 0;
-  uint32_t round = 0, loaded = 0;
+  int stage = 0, v_row = 0;
+  uint32_t round = 0, loaded = 0, v_boxes = 0;
+  bool v_mine = false, ok = true;
   const bool begins = lane < 8 && lane % (p.box_rows / 16) == 0;
-  bool ok = true;
-  for (int64_t u = 0; u < units; ++u) {
+  // The next stage's barrier, once the stage is free; null when a wait has given up.
+  auto take = [&]() -> uint64_t* {
+    ok = ok && (round == 0 || wait_all(&sm.raw_empty[stage], (round - 1) & 1u, p.err));
+    return ok ? &sm.raw_full[stage] : nullptr;
+  };
+  auto done = [&]() {
+    loaded |= 1u << stage;
+    if (++stage == kRaw) {
+      stage = 0;
+      ++round;
+    }
+  };
+  bool here = true, before = false;  // a unit, and one before it
+  while ((here || before) && ok) {
     const int row = (page * p.num_kv_heads + c.kvh) * p.block_size + place;
     const bool mine = begins && page >= 0;
     const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-    const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
-    if (u + 1 < units) {  // the next unit's pages
-      if (++c.tile < c.tiles) {
+    const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, mine)) * p.box_rows;
+    const bool k_now = here, v_now = before;
+    before = here;
+    if (here) {  // the next unit's pages
+      if (++c.tile < c.end) {
         column += p.unit_pages;  // whole pages in a tile, and what is left
         place += p.unit_rest;
         if (place >= p.block_size) {
@@ -190,30 +233,39 @@ __device__ __forceinline__ void load_role(const Int4AttnParams& p, const CUtenso
           ++column;
         }
         page = look_up();
-      } else {
-        next_pair(p, c);
+      } else if (c.more()) {
+        next_piece(p, c);
         page = find();
+      } else {
+        here = false;
       }
     }
-    if (round > 0) ok = wait_all(&sm.raw_empty[stage], (round - 1) & 1u, p.err);
-    if (!ok) break;
-    uint64_t* bar = &sm.raw_full[stage];
-    if (lane == 0) {
-      sm.raw_there[stage] = there;
-      mbar_arrive_expect_tx(bar, boxes * p.box_rows * 136);
+    if (k_now) {
+      uint64_t* bar = take();
+      if (bar == nullptr) break;
+      if (lane == 0) {
+        sm.raw_there[stage] = there;
+        mbar_arrive_expect_tx(bar, boxes * 72);
+      }
+      __syncwarp();
+      if (mine) {
+        tma_load_2d(sm.raw[stage] + lane * 1024, &map_k, bar, 0, row);
+        bulk_load(smem_u32(sm.raw_scale[stage] + lane * 16), p.kv_scale + static_cast<int64_t>(row) * 4, p.box_rows * 8,
+                  bar);
+      }
+      done();
     }
-    __syncwarp();
-    if (mine) {
-      tma_load_2d(sm.raw_k[stage] + lane * 1024, &map_k, bar, 0, row);
-      tma_load_2d(sm.raw_v[stage] + lane * 1024, &map_v, bar, 0, row);
-      bulk_load(smem_u32(sm.raw_scale[stage] + lane * 16), p.kv_scale + static_cast<int64_t>(row) * 4, p.box_rows * 8,
-                bar);
+    if (v_now) {
+      uint64_t* bar = take();
+      if (bar == nullptr) break;
+      if (lane == 0) mbar_arrive_expect_tx(bar, v_boxes * 64);
+      __syncwarp();
+      if (v_mine) tma_load_2d(sm.raw[stage] + lane * 1024, &map_v, bar, 0, v_row);
+      done();
     }
-    loaded |= 1u << stage;
-    if (++stage == kRaw) {
-      stage = 0;
-      ++round;
-    }
+    v_row = row;
+    v_mine = mine;
+    v_boxes = boxes;
   }
   // copies in flight after a wait that gave up: they must land (or run out of time) before the CTA ends
   if (!ok)
@@ -222,24 +274,11 @@ __device__ __forceinline__ void load_role(const Int4AttnParams& p, const CUtenso
 }
 
 // ------------------------------------------------------------------------------------------ codes -> f16
-// Eight rows of codes (lane: row g, 16-byte piece t) -> f16 rows of an operand, value = low + step code times 2^-e.
-__device__ __forceinline__ void unpack_rows(uint32_t raw, uint32_t dst, int row, int t, uint32_t even, uint32_t odd,
-                                            uint32_t low) {
-  const uint4 x = ld_shared_v4(raw + row * 64 + ((t ^ (row >> 1 & 3)) * 16));
-  // pieces 2 and 3 (the second block of values) in another order: no bank conflicts
-  const bool swap = t & 2;
-  const uint32_t w[4] = {swap ? x.z : x.x, swap ? x.w : x.y, swap ? x.x : x.z, swap ? x.y : x.w};
-  const uint32_t out = dst + (t >> 1) * kOBytes + row * 128;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t y = w[i] >> 8;
-    const uint32_t a = fma_f16x2(w[i] & 0x000F000Fu, even, low), b = fma_f16x2(w[i] & 0x00F000F0u, odd, low);
-    const uint32_t c = fma_f16x2(y & 0x000F000Fu, even, low), d = fma_f16x2(y & 0x00F000F0u, odd, low);
-    const int chunk = (t & 1) * 4 + (i ^ (t & 2));
-    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(out + ((chunk ^ (row & 7)) * 16)), "r"(a), "r"(b), "r"(c),
-                 "r"(d)
-                 : "memory");
-  }
+// Eight values (a word of codes) -> four f16 pairs, values 0 4, 1 5, 2 6 and 3 7.
+__device__ __forceinline__ uint4 unpack8(uint32_t w, uint32_t even, uint32_t odd, uint32_t low) {
+  const uint32_t y = w >> 8;
+  return make_uint4(fma_f16x2(w & 0x000F000Fu, even, low), fma_f16x2(w & 0x00F000F0u, odd, low),
+                    fma_f16x2(y & 0x000F000Fu, even, low), fma_f16x2(y & 0x00F000F0u, odd, low));
 }
 
 __device__ __forceinline__ uint32_t twice_f16(float x) {
@@ -247,273 +286,344 @@ __device__ __forceinline__ uint32_t twice_f16(float x) {
   return h | h << 16;
 }
 
-__device__ __forceinline__ void unpack_role(const Int4AttnParams& p, Smem& sm, Cursor c, int64_t units, int warp, int lane) {
+// What a row's codes are multiplied by (in the low and in the high half of a byte), and its lowest value; f16 twice.
+struct RowScale {
+  uint32_t even, odd, low;
+};
+__device__ __forceinline__ RowScale row_scale(float step, float low) {
+  return {twice_f16(step * 16777216.f), twice_f16(step * 1048576.f), twice_f16(low)};
+}
+
+// K is one tile ahead of V (steps K 0, K 1, V 0, K 2, V 1, ...): the scores of the next tile are never waited for.
+// One body for both, so that the loop stays small.
+__device__ __forceinline__ void unpack_role(const Int4AttnParams& p, Smem& sm, Cursor c, int warp, int lane) {
   const int g = lane >> 2, t = lane & 3;
-  int v_exp = 0, v_exp_set = 0;
+  int v_exp = 0;
+  bool v_exp_set = false;
+  RowScale v_scale = {0, 0, 0}, next_v = {0, 0, 0};
   int stage = 0;
   uint32_t raw_parity = 0;
-  for (int64_t u = 0; u < units; ++u) {
-    const int buf = static_cast<int>(u & 1);
-    const uint32_t reuse = static_cast<uint32_t>(u >> 1);  // of the K buffer
-    if (!wait_all(&sm.raw_full[stage], raw_parity, p.err)) return;
-    // ---- the tile's largest magnitudes, over rows that are there (all warps alike)
-    const uint32_t there = sm.raw_there[stage];
-    const int pos0 = c.tile * kTile;
-    float k_top = 0.f, v_top = 0.f;
-    bool wild = false;  // a row that is not finite
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 32 * i + lane;
-      const uint2 sc = sm.raw_scale[stage][row];
-      const float ks = __uint_as_float(sc.x << 16), kl = __uint_as_float(sc.x & 0xFFFF0000u);
-      const float vs = __uint_as_float(sc.y << 16), vl = __uint_as_float(sc.y & 0xFFFF0000u);
-      const float kt = fmaxf(fabsf(kl), fabsf(fmaf(15.f, ks, kl))), vt = fmaxf(fabsf(vl), fabsf(fmaf(15.f, vs, vl)));
-      const bool held = (there >> (row >> 4) & 1u) && pos0 + row < c.s.vis;
-      if (held) {
-        if (kt + fabsf(ks) + vt + fabsf(vs) < INFINITY) {  // a sum: NaN and infinity do not get lost
-          k_top = fmaxf(k_top, kt);
-          v_top = fmaxf(v_top, vt);
-        } else {
-          wild = true;
-        }
-      }
-    }
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      k_top = fmaxf(k_top, __shfl_xor_sync(0xffffffffu, k_top, off));
-      v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, off));
-    }
-    wild = __any_sync(0xffffffffu, wild);
-    // largest magnitudes to between 2^-7 and 2^-6: steps times 2^24 stay below 2^16
-    const int k_exp = k_top > 0.f ? max(-96, min(exponent(k_top), 110)) + 7 : 0;
-    float change = 1.f;
-    if (v_top > 0.f) {
-      const int e = max(-96, min(exponent(v_top), 110)) + 7;
-      if (!v_exp_set) {
-        v_exp = e;
-        v_exp_set = 1;
-      } else if (e > v_exp) {
-        change = v_exp - e < -126 ? 0.f : pow2(v_exp - e);
-        v_exp = e;
-      }
-    }
-    // ---- K
-    if (reuse > 0 && !wait_all(&sm.k_free[buf], (reuse - 1) & 1u, p.err)) return;
-    if (warp == 0 && lane == 0) {
-      const int slot = static_cast<int>(u & 3);
-      sm.k_back[slot] = pow2(k_exp);
-      sm.v_change[slot] = change;
-      sm.v_back[slot] = pow2(v_exp);
-      sm.there[slot] = there | (wild ? kWild : 0u);
-    }
-    const float k_to = pow2(-k_exp), v_to = pow2(-v_exp);
+  int k_unit = 0, v_unit = 0;
+  bool more_k = true;
 #pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-      if (half == 1 && u > 0 && !wait_all(&sm.v_free, static_cast<uint32_t>(u - 1) & 1u, p.err)) return;
-      const uint32_t raw = smem_u32(half ? sm.raw_v[stage] : sm.raw_k[stage]);
-      const uint32_t dst = smem_u32(half ? sm.v : sm.k[buf]);
+  for (int step = 0; more_k || v_unit < k_unit; ++step) {
+    const bool is_k = more_k && (step == 0 || (step & 1));
+    if (!wait_all(&sm.raw_full[stage], raw_parity, p.err)) return;
+    RowScale mine = v_scale;
+    uint32_t there = 0;
+    int k_exp = 0;
+    float change = 1.f;
+    if (is_k) {
+      // ---- the tile's largest magnitudes, over rows that are there (all warps alike)
+      there = sm.raw_there[stage];
+      const int pos0 = c.tile * kTile;
+      uint32_t k_bits = 0, v_bits = 0;
+      float ks = 0.f, kl = 0.f, vs = 0.f, vl = 0.f;  // of this lane's own row, 32 warp + lane
+      bool held = false, fine = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = 32 * warp + 8 * i + g;
+        const int row = 32 * (i ^ warp) + lane;  // its own first
         const uint2 sc = sm.raw_scale[stage][row];
-        const bool held = (there >> (row >> 4) & 1u) && pos0 + row < c.s.vis;
-        const float ks = __uint_as_float(sc.x << 16), kl = __uint_as_float(sc.x & 0xFFFF0000u);
-        const float vs = __uint_as_float(sc.y << 16), vl = __uint_as_float(sc.y & 0xFFFF0000u);
-        const bool fine = fabsf(fmaf(15.f, ks, kl)) + fabsf(ks) + fabsf(fmaf(15.f, vs, vl)) + fabsf(vs) < INFINITY;
-        float step = half ? vs * v_to : ks * k_to, low = half ? vl * v_to : kl * k_to;
-        if (!held || !fine) {
-          step = 0.f;
-          low = held && half == 0 ? __uint_as_float(0x7FC00000u) : 0.f;
-        }
-        unpack_rows(raw, dst, row, t, twice_f16(step * 16777216.f), twice_f16(step * 1048576.f), twice_f16(low));
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        if (half == 0) {
-          mbar_arrive(&sm.k_full[buf]);
-        } else {
-          mbar_arrive(&sm.v_full);
-          mbar_arrive(&sm.raw_empty[stage]);
+        const float a = __uint_as_float(sc.x << 16), b = __uint_as_float(sc.x & 0xFFFF0000u);
+        const float d = __uint_as_float(sc.y << 16), e = __uint_as_float(sc.y & 0xFFFF0000u);
+        const float kt = fmaxf(fabsf(b), fabsf(fmaf(15.f, a, b))), vt = fmaxf(fabsf(e), fabsf(fmaf(15.f, d, e)));
+        const bool in = (there >> (row >> 4) & 1u) && pos0 + row < c.s.vis;
+        const bool sane = kt + fabsf(a) + vt + fabsf(d) < INFINITY;  // a sum: NaN and infinity do not get lost
+        k_bits = max(k_bits, in && sane ? __float_as_uint(kt) : 0u);
+        v_bits = max(v_bits, in && sane ? __float_as_uint(vt) : 0u);
+        if (i == 0) {
+          ks = a;
+          kl = b;
+          vs = d;
+          vl = e;
+          held = in;
+          fine = in && sane;
         }
       }
+      const float k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, k_bits));
+      const float v_top = __uint_as_float(__reduce_max_sync(0xffffffffu, v_bits));
+      // largest magnitudes to between 2^-7 and 2^-6: steps times 2^24 stay below 2^16
+      k_exp = k_top > 0.f ? max(-96, min(exponent(k_top), 110)) + 7 : 0;
+      if (v_top > 0.f) {
+        const int e = max(-96, min(exponent(v_top), 110)) + 7;
+        if (!v_exp_set) {
+          v_exp = e;
+          v_exp_set = true;
+        } else if (e > v_exp) {
+          change = v_exp - e < -126 ? 0.f : pow2(v_exp - e);
+          v_exp = e;
+        }
+      }
+      const float k_to = pow2(-k_exp), v_to = pow2(-v_exp);
+      const float wild_low = held ? __uint_as_float(0x7FC00000u) : 0.f;
+      mine = fine ? row_scale(ks * k_to, kl * k_to) : row_scale(0.f, wild_low);
+      next_v = fine ? row_scale(vs * v_to, vl * v_to) : row_scale(0.f, 0.f);
+    }
+    // ---- 32 rows of codes (lane: rows 8 i + g, 16-byte piece t) into the operand
+    uint4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 32 * warp + 8 * i + g;
+      x[i] = ld_shared_v4(smem_u32(sm.raw[stage]) + row * 64 + ((t ^ (row >> 1 & 3)) * 16));
+    }
+    const int unit = is_k ? k_unit : v_unit;
+    const int buf = unit & 1;
+    // its last readers
+    if (unit > 1 && !wait_all(is_k ? &sm.k_free[buf] : &sm.v_free[buf], static_cast<uint32_t>((unit >> 1) - 1) & 1u, p.err))
+      return;
+    const uint32_t dst = smem_u32(is_k ? sm.k[buf] : sm.v[buf]) + (t >> 1) * kOBytes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 32 * warp + 8 * i + g;
+      const uint32_t a = __shfl_sync(0xffffffffu, mine.even, 8 * i + g), b = __shfl_sync(0xffffffffu, mine.odd, 8 * i + g);
+      const uint32_t d = __shfl_sync(0xffffffffu, mine.low, 8 * i + g);
+      // pieces 2 and 3 (the second block of values) in another order: no bank conflicts
+      const bool swap = t & 2;
+      const uint32_t w[4] = {swap ? x[i].z : x[i].x, swap ? x[i].w : x[i].y, swap ? x[i].x : x[i].z, swap ? x[i].y : x[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 y = unpack8(w[k], a, b, d);
+        const int chunk = (t & 1) * 4 + (k ^ (t & 2));
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + row * 128 + ((chunk ^ (row & 7)) * 16)), "r"(y.x),
+                     "r"(y.y), "r"(y.z), "r"(y.w));
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (is_k && warp == 0) {
+        const int slot = k_unit & 3;
+        sm.k_back[slot] = pow2(k_exp);
+        sm.v_change[slot] = change;
+        sm.v_back[slot] = pow2(v_exp);
+        sm.there[slot] = there;
+      }
+      mbar_arrive(is_k ? &sm.k_full[buf] : &sm.v_full[buf]);
+      mbar_arrive(&sm.raw_empty[stage]);
     }
     if (++stage == kRaw) {
       stage = 0;
       raw_parity ^= 1u;
     }
-    if (++c.tile == c.tiles && u + 1 < units) {
-      next_pair(p, c);
-      v_exp = v_exp_set = 0;
+    if (is_k) {
+      ++k_unit;
+      if (++c.tile == c.end) {
+        more_k = c.more();
+        if (more_k) next_piece(p, c);
+        v_exp = 0;
+        v_exp_set = false;
+      }
+    } else {
+      ++v_unit;
     }
+    if (!is_k || step == 0) v_scale = next_v;
   }
 }
 
 // ------------------------------------------------------------------------------------------ products
-__device__ __forceinline__ void mma_role(const Int4AttnParams& p, Smem& sm, Cursor c, int64_t units) {
-  const uint32_t idesc_s = tc::idesc_f16(128, 128, false, false), idesc_pv = tc::idesc_f16(128, 128, false, true);
-  const uint32_t tmem = sm.tmem;
-  uint64_t dq[2], dk[2];
-  for (int i = 0; i < 2; ++i) {
-    dq[i] = tc::smem_desc(smem_u32(sm.q[i]), 16, 1024, tc::kSw128);
-    dk[i] = tc::smem_desc(smem_u32(sm.k[i]), 16, 1024, tc::kSw128);
-  }
-  const uint64_t dv = tc::smem_desc(smem_u32(sm.v), kOBytes, 1024, tc::kSw128);
-  uint32_t q_parity = 0, p_parity[2] = {0, 0};
+// The whole warp goes through the loop, so that descriptors and addresses are uniform, and one lane issues.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t chosen;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+  return chosen != 0;
+}
+
+__device__ __forceinline__ void mma_role(const Int4AttnParams& p, Smem& sm, Cursor c) {
+  constexpr uint32_t idesc_s = tc::idesc_f16(128, 128, false, false), idesc_pv = tc::idesc_f16(128, 128, false, true);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+  const uint64_t dq = tc::smem_desc(smem_u32(sm.q[0]), 16, 1024, tc::kSw128);
+  const uint64_t dk = tc::smem_desc(smem_u32(sm.k[0]), 16, 1024, tc::kSw128);
+  const uint64_t dv = tc::smem_desc(smem_u32(sm.v[0]), kOBytes, 1024, tc::kSw128);
+  uint32_t q_parity = 0, p_parity = 0;
   bool ok = true;
-  // O_g += P_g V, 16 positions at a time: V's rows are 128 bytes
-  auto values = [&](int g, bool first) {
-    ok = ok && wait_one(&sm.p_full[g], p_parity[g], p.err);
-    p_parity[g] ^= 1u;
-    if (!ok) return;
-    tc::fence_after_sync();
-#pragma unroll
-    for (int i = 0; i < kTile / 16; ++i)
-      tc::mma_f16_ts(tmem + 256 * g + 128, tmem + 256 * g + 8 * i, dv + static_cast<uint64_t>(i * (16 * 128 >> 4)), idesc_pv,
-                     !first || i > 0 ? 1u : 0u);
-  };
-  for (int64_t u = 0; u < units && ok;) {
-    const int n = static_cast<int>(min(units - u, static_cast<int64_t>(c.tiles - c.tile)));
+  for (int u = 0; ok;) {
+    const int n = c.end - c.tile;
     const int groups = c.s.nq * p.group - c.rg * kItem > kRows ? 2 : 1;
-    for (int i = 0; i <= n && ok; ++i, ++u) {
+    for (int i = 0; i <= n && ok; ++i) {
+      const int at = u + i;  // scores of this unit, values of the one before it
       for (int g = 0; g < groups && ok; ++g) {
-        if (i > 0) {
-          if (g == 0) ok = wait_one(&sm.v_full, static_cast<uint32_t>(u - 1) & 1u, p.err);
-          values(g, i == 1);
-          if (ok && i == n) tc::commit(&sm.o_full[g]);
+        if (i > 0) {  // O_g += P_g V, 16 positions at a time: V's rows are 128 bytes
+          const int buf = (at - 1) & 1;
+          if (g == 0) ok = wait_all(&sm.v_full[buf], static_cast<uint32_t>((at - 1) >> 1) & 1u, p.err);
+          ok = ok && wait_all(&sm.p_full[g], p_parity >> g & 1u, p.err);
+          if (!ok) break;
+          p_parity ^= 1u << g;
+          tc::fence_after_sync();
+          if (elect_one()) {
+            const uint64_t b = dv + static_cast<uint64_t>(buf * (2 * kOBytes >> 4));
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+              tc::mma_f16_ts(tmem + 256 * g + 128, tmem + 256 * g + 8 * k, b + static_cast<uint64_t>(k * (16 * 128 >> 4)),
+                             idesc_pv, i > 1 || k > 0 ? 1u : 0u);
+            if (i == n) tc::commit(&sm.o_full[g]);
+            if (g == groups - 1) tc::commit(&sm.v_free[buf]);
+          }
+          __syncwarp();
         }
-        if (i < n && ok) {
-          const int buf = static_cast<int>(u & 1);
-          if (g == 0) ok = wait_one(&sm.k_full[buf], static_cast<uint32_t>(u >> 1) & 1u, p.err);
-          if (i == 0) ok = ok && wait_one(&sm.q_full[g], q_parity >> g & 1u, p.err);
+        if (i < n) {
+          const int buf = at & 1;
+          if (g == 0) ok = wait_all(&sm.k_full[buf], static_cast<uint32_t>(at >> 1) & 1u, p.err);
+          if (i == 0) ok = ok && wait_all(&sm.q_full[g], q_parity >> g & 1u, p.err);
           if (!ok) break;
           tc::fence_after_sync();
+          if (elect_one()) {
+            const uint64_t a = dq + static_cast<uint64_t>(g * (2 * kOBytes >> 4)), b = dk + static_cast<uint64_t>(buf * (2 * kOBytes >> 4));
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {  // 16 values: 32 bytes, four to a block
-            const uint64_t step = static_cast<uint64_t>((k >> 2) * (kOBytes >> 4) + (k & 3) * 2);
-            mma_f16_ss(tmem + 256 * g, dq[g] + step, dk[buf] + step, idesc_s, k > 0 ? 1u : 0u);
+            for (int k = 0; k < 8; ++k) {  // 16 values: 32 bytes, four to a block
+              const uint64_t step = static_cast<uint64_t>((k >> 2) * (kOBytes >> 4) + (k & 3) * 2);
+              mma_f16_ss(tmem + 256 * g, a + step, b + step, idesc_s, k > 0 ? 1u : 0u);
+            }
+            tc::commit(&sm.s_full[g]);
+            if (g == groups - 1) tc::commit(&sm.k_free[buf]);
           }
-          tc::commit(&sm.s_full[g]);
+          __syncwarp();
         }
       }
-      if (!ok) break;
-      if (i > 0) tc::commit(&sm.v_free);
-      if (i < n) tc::commit(&sm.k_free[u & 1]);
-      if (i == n) --u;  // the loop's last step issued no scores
     }
     q_parity ^= groups == 2 ? 3u : 1u;
-    c.tile += n;
-    if (u < units) next_pair(p, c);
+    u += n;
+    if (!c.more()) break;
+    next_piece(p, c);
   }
   if (!ok) {  // products in flight must end before the CTA does
-    tc::commit(&sm.drained);
-    wait_one(&sm.drained, 0, p.err);
+    if (elect_one()) tc::commit(&sm.drained);
+    wait_all(&sm.drained, 0, p.err);
   }
 }
 
 // ------------------------------------------------------------------------------------------ softmax
-// P of two scores: 2^(s cs + bias), and its part of the row's sum.
-__device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor c, int64_t units, int64_t ctas,
-                                             int64_t total, int64_t u0, int g, int tid) {
-  const int r = tid & 127, warp = r >> 5;
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Rows of a work item, every other one: row of the kv head, its token's row of q and its query head.
+struct Walk {
+  int row, head, in_group;
+  int64_t token;
+  __device__ __forceinline__ Walk(const Int4AttnParams& p, const Cursor& c, int in_item) {
+    row = c.rg * kItem + in_item;
+    const int t = row / p.group;
+    in_group = row - t * p.group;
+    head = c.kvh * p.group + in_group;
+    token = static_cast<int64_t>(c.s.q_first) + t;
+  }
+  __device__ __forceinline__ void two_on(const Int4AttnParams& p) {
+    row += 2;
+    token += p.two_tokens;
+    in_group += p.two_heads;
+    head += p.two_heads;
+    if (in_group >= p.group) {
+      in_group -= p.group;
+      head -= p.group;
+      ++token;
+    }
+  }
+};
+
+// Which of the columns c0 .. c0 + 31 of a tile a row sees: in pages that are there, and below `seen`.
+__device__ __forceinline__ uint32_t seen_of(uint32_t there, int seen, int c0) {
+  const uint32_t part = there >> (c0 >> 4);
+  const uint32_t held = ((part & 1u) ? 0xFFFFu : 0u) | ((part & 2u) ? 0xFFFF0000u : 0u);
+  const int left = seen - c0;
+  return held & (left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u);
+}
+
+// The 16-byte piece of a 256-byte row (of q, or of outputs on their way out) in a group's q.
+__device__ __forceinline__ uint32_t q_piece(uint32_t q, int row, int piece) {
+  return q + (piece >> 3) * kOBytes + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
+}
+
+__device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor next, int64_t ctas,
+                                             int64_t total, int g, int tid) {
+  const int r = tid & 127, warp = r >> 5, lane = tid & 31;
   const uint32_t s_tmem = sm.tmem + (static_cast<uint32_t>(32 * warp) << 16) + 256 * g, o_tmem = s_tmem + 128;
+  const uint32_t q = smem_u32(sm.q[g]);
   uint32_t s_parity = 0, o_parity = 0;
   constexpr int kPart = kItem * (kHeadDim + 2);
   bool first_piece = true;
-  for (int64_t u = 0; u < units;) {
-    const int n = static_cast<int>(min(units - u, static_cast<int64_t>(c.tiles - c.tile)));
+  uint4 raw[16];
+  Cursor c = next;
+  bool started = false, more = true;
+  for (int u = 0, n = 0;;) {
     const int rows = c.s.nq * p.group;
-    if (rows - c.rg * kItem > g * kRows) {
+    const bool active = started && rows - c.rg * kItem > g * kRows;
+    float m = kNone, l = 0.f, back = 1.f;
+    if (active) {
       const int row = c.rg * kItem + g * kRows + r;
-      const bool real = row < rows;
       const int token = row / p.group;
-      const int64_t q_row = static_cast<int64_t>(c.s.q_first) + token;
-      const int head = c.kvh * p.group + row - token * p.group;
-      const int limit = real ? min(c.s.vis, token + c.s.nk - c.s.nq + 1) : c.s.vis;  // no row: zeros that see anything
-      // ---- q: a power of two puts the largest value between 2^13 and 2^14
-      float cs;
-      {
-        uint4 raw[16];
-        const uint16_t* src = p.q + q_row * p.q_row_stride + head * kHeadDim;
+      const int limit = row < rows ? min(c.s.vis, token + c.s.nk - c.s.nq + 1) : c.s.vis;  // no row: zeros that see anything
+      // ---- q: each thread turns its row into f16; a power of two puts the largest value between 2^13 and 2^14
 #pragma unroll
-        for (int i = 0; i < 16; ++i) raw[i] = real ? ldg_keep_v4(src + 8 * i) : make_uint4(0, 0, 0, 0);
-        float amax = 0.f;
+      for (int i = 0; i < 16; ++i)
+        st_shared_v4(q_piece(q, 32 * warp + 2 * i + (lane >> 4), lane & 15), raw[i].x, raw[i].y, raw[i].z, raw[i].w);
+      __syncwarp();
+      uint32_t top_bits = 0;  // bf16 magnitudes in order as integers, two at a time
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const uint4 w = ld_shared_v4(q_piece(q, r, i));
+        top_bits = __vmaxu2(__vmaxu2(top_bits, w.x & 0x7FFF7FFFu), w.y & 0x7FFF7FFFu);
+        top_bits = __vmaxu2(__vmaxu2(top_bits, w.z & 0x7FFF7FFFu), w.w & 0x7FFF7FFFu);
+      }
+      const float amax = __uint_as_float(max(top_bits & 0xFFFFu, top_bits >> 16) << 16);
+      const int e = amax > 0.f && amax < INFINITY ? max(-100, min(exponent(amax), 110)) - 13 : 0;
+      const float to = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);  // a negative scale turns q around
+      const float cs = fabsf(p.scale_log2) * pow2(e);
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const uint4 raw_w = ld_shared_v4(q_piece(q, r, i));
+        const uint32_t w[4] = {raw_w.x, raw_w.y, raw_w.z, raw_w.w};
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xFFFF0000u))));
+        for (int k = 0; k < 4; ++k) {
+          x[2 * k] = __uint_as_float(w[k] << 16) * to;
+          x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u) * to;
         }
-        const int e = amax > 0.f && amax < INFINITY ? max(-100, min(exponent(amax), 110)) - 13 : 0;
-        const float to = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);  // a negative scale turns q around
-        cs = fabsf(p.scale_log2) * pow2(e);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {  // values 8 i .. 8 i + 7 in the order 0 4 1 5 2 6 3 7
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          float x[8];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[2 * k] = __uint_as_float(w[k] << 16) * to;
-            x[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u) * to;
-          }
-          uint8_t* dst = sm.q[g] + (i >> 3) * kOBytes + r * 128 + (((i & 7) ^ (r & 7)) * 16);
-          *reinterpret_cast<uint4*>(dst) = make_uint4(pack_f16x2(x[0], x[4]), pack_f16x2(x[1], x[5]),
-                                                      pack_f16x2(x[2], x[6]), pack_f16x2(x[3], x[7]));
-        }
+        // values 8 i .. 8 i + 7 in the order 0 4 1 5 2 6 3 7
+        st_shared_v4(q_piece(q, r, i), pack_f16x2(x[0], x[4]), pack_f16x2(x[1], x[5]), pack_f16x2(x[2], x[6]),
+                     pack_f16x2(x[3], x[7]));
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if ((tid & 31) == 0) mbar_arrive(&sm.q_full[g]);
+      if (lane == 0) mbar_arrive(&sm.q_full[g]);
 
-      float m = kNone, l = 0.f, back = 1.f;
       for (int i = 0; i < n; ++i) {
-        const int slot = static_cast<int>((u + i) & 3);
+        const int slot = (u + i) & 3;
         // S_g of this tile done: so is O_g of the one before it
         if (!wait_all(&sm.s_full[g], s_parity, p.err)) return;
         s_parity ^= 1u;
         tc::fence_after_sync();
-        const float ct = cs * sm.k_back[slot];
-      back = sm.v_back[slot];
-        const float change = sm.v_change[slot];
+        // never 0, so that what is not seen (minus infinity) stays so; scores are below 2^16
+        const float ct = fmaxf(cs * sm.k_back[slot], 1.0e-30f);
+        back = sm.v_back[slot];
+        float f = sm.v_change[slot];
         const uint32_t there = sm.there[slot];
         const int seen = limit - (c.tile + i) * kTile;  // columns below this one
-        // the polynomial would lose a NaN
-        const bool full = __all_sync(0xffffffffu, there == 0xFFu && seen >= kTile);
-        // ---- the row's maximum
-        float top = kNone;
-        uint32_t v[32];
-        if (full) {
-          float t0 = kNone, t1 = kNone, t2 = kNone, t3 = kNone;
+        uint32_t v[4][32];
 #pragma unroll
-          for (int c0 = 0; c0 < kTile; c0 += 32) {
-            tmem_ld32(s_tmem + c0, v);
-            tc::wait_ld();
+        for (int q = 0; q < 4; ++q) tmem_ld32(s_tmem + 32 * q, v[q]);
+        tc::wait_ld();
+        if (!__all_sync(0xffffffffu, (there & 0xFFu) == 0xFFu && seen >= kTile)) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              t0 = fmaxf(t0, fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
-              t1 = fmaxf(t1, fmaxf(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])));
-              t2 = fmaxf(t2, fmaxf(__uint_as_float(v[k + 4]), __uint_as_float(v[k + 5])));
-              t3 = fmaxf(t3, fmaxf(__uint_as_float(v[k + 6]), __uint_as_float(v[k + 7])));
-            }
-          }
-          top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
-        } else {
-#pragma unroll 1
-          for (int c0 = 0; c0 < kTile; c0 += 32) {
-            tmem_ld32(s_tmem + c0, v);
-            tc::wait_ld();
-            const uint32_t part = there >> (c0 >> 4);
-            const uint32_t held = ((part & 1u) ? 0xFFFFu : 0u) | ((part & 2u) ? 0xFFFF0000u : 0u);
-            const int left = seen - c0;
-            const uint32_t mask = held & (left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u);
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t mask = seen_of(there, seen, 32 * q);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) top = fmaxf(top, mask >> k & 1u ? __uint_as_float(v[k]) : kNone);
+            for (int k = 0; k < 32; ++k)
+              if (!(mask >> k & 1u)) v[q][k] = 0xFF800000u;
           }
         }
-        top = top == kNone ? kNone : top * ct;  // ct is not negative
+        // ---- the row's maximum
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int k = 0; k < 32; k += 2)
+            t[k / 2 & 3] = fmaxf(t[k / 2 & 3], fmaxf(__uint_as_float(v[q][k]), __uint_as_float(v[q][k + 1])));
+        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * ct;
         // ---- a new reference maximum where it lags too far, and V's power of two
-        float f = change;
         if (top > m + kSlack) {
           const float lag = ex2(m - top);
           m = top;
@@ -522,83 +632,64 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         }
         if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll 1
-          for (int c0 = 0; c0 < kHeadDim; c0 += 32) {
-            tmem_ld32(o_tmem + c0, v);
+          for (int c0 = 0; c0 < kHeadDim; c0 += 8) {
+            float y[8];
+            tc::ld8(o_tmem + c0, y);
             tc::wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
-            tmem_st32(o_tmem + c0, v);
+            for (int k = 0; k < 8; ++k) y[k] *= f;
+            tc::st8(o_tmem + c0, y);
           }
-          tc::wait_st();
         }
-        // ---- P over the columns of S that have been read
+        // ---- P over the columns of S, all of which have been read
         const float bias = kLift - m;
-        uint64_t sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
         const uint64_t ct2 = f2_pack(ct, ct), bias2 = f2_pack(bias, bias);
-        if (full) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < kTile; c0 += 32) {
-            tmem_ld32(s_tmem + c0, v);
-            tc::wait_ld();
-            uint32_t pw[16];
+        uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const uint64_t x = f2_fma(f2_pack(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), ct2, bias2);
-              float x0, x1, p0, p1;
-              f2_unpack(x, x0, x1);
-              if (k % 3 == 2) {
-                exp2_poly_x2(x0, x1, p0, p1);
-              } else {
-                p0 = ex2(x0);
-                p1 = ex2(x1);
-              }
-              if (k & 1) {
-                sum1 = f2_add(sum1, f2_pack(p0, p1));
-              } else {
-                sum0 = f2_add(sum0, f2_pack(p0, p1));
-              }
-              pw[k] = pack_f16x2(p0, p1);
-            }
-            tc::st16u(s_tmem + c0 / 2, pw);
-          }
-        } else {
-#pragma unroll 1
-          for (int c0 = 0; c0 < kTile; c0 += 32) {
-            tmem_ld32(s_tmem + c0, v);
-            tc::wait_ld();
-            const uint32_t part = there >> (c0 >> 4);
-            const uint32_t held = ((part & 1u) ? 0xFFFFu : 0u) | ((part & 2u) ? 0xFFFF0000u : 0u);
-            const int left = seen - c0;
-            const uint32_t mask = held & (left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u);
-            uint32_t pw[16];
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pw[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float p0 = mask >> (2 * k) & 1u ? ex2(fmaf(__uint_as_float(v[2 * k]), ct, bias)) : 0.f;
-              const float p1 = mask >> (2 * k + 1) & 1u ? ex2(fmaf(__uint_as_float(v[2 * k + 1]), ct, bias)) : 0.f;
-              sum0 = f2_add(sum0, f2_pack(p0, p1));
-              pw[k] = pack_f16x2(p0, p1);
-            }
-            tc::st16u(s_tmem + c0 / 2, pw);
+          for (int k = 0; k < 16; ++k) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[q][2 * k]), __uint_as_float(v[q][2 * k + 1])), ct2, bias2), x0, x1);
+            const float p0 = ex2(x0), p1 = ex2(x1);
+            sum[k & 1] = f2_add(sum[k & 1], f2_pack(p0, p1));
+            pw[k] = pack_f16x2(p0, p1);
           }
+          tc::st16u(s_tmem + 16 * q, pw);
         }
         float a0, a1, b0, b1;
-        f2_unpack(sum0, a0, a1);
-        f2_unpack(sum1, b0, b1);
+        f2_unpack(sum[0], a0, a1);
+        f2_unpack(sum[1], b0, b1);
         l += (a0 + a1) + (b0 + b1);
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
         if ((tid & 31) == 0) mbar_arrive(&sm.p_full[g]);
       }
-      // ---- the piece's end
+    }
+    // ---- the next piece's q, before this one's outputs are stored: a warp loads its 32 rows two at a time, 16 lanes to
+    // a row (whole lines)
+    if (more) {
+      const int next_rows = next.s.nq * p.group;
+      Walk at(p, next, g * kRows + 32 * warp + (lane >> 4));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (at.row < next_rows) raw[i] = ldg_keep_v4(p.q + at.token * p.q_row_stride + at.head * kHeadDim + 8 * (lane & 15));
+        at.two_on(p);
+      }
+    }
+    // ---- the piece's end
+    if (active) {
       if (!wait_all(&sm.o_full[g], o_parity, p.err)) return;
       o_parity ^= 1u;
       tc::fence_after_sync();
-      const bool whole = c.tile == 0 && n == c.tiles;
+      const bool whole = c.whole();
       const float f = !whole ? back : l == 0.f ? 0.f : __fdiv_rn(back, l);
-      float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart +
-                    (g * kRows + r) * kHeadDim;
-      uint16_t* dst = p.out + q_row * p.out_row_stride + head * kHeadDim;
+      // rows leave through the group's q, which no product reads any more, so that stores are whole lines: 256 bytes of
+      // a row at a time, 128 bf16 values or 64 fp32 ones
+      float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart;
 #pragma unroll 1
       for (int c0 = 0; c0 < kHeadDim; c0 += 32) {
         uint32_t v[32];
@@ -609,42 +700,60 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
           const float y[8] = {__uint_as_float(v[k]) * f,     __uint_as_float(v[k + 2]) * f, __uint_as_float(v[k + 4]) * f,
                               __uint_as_float(v[k + 6]) * f, __uint_as_float(v[k + 1]) * f, __uint_as_float(v[k + 3]) * f,
                               __uint_as_float(v[k + 5]) * f, __uint_as_float(v[k + 7]) * f};
-          if (!whole) {
-            *reinterpret_cast<float4*>(part + c0 + k) = make_float4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<float4*>(part + c0 + k + 4) = make_float4(y[4], y[5], y[6], y[7]);
-          } else if (real) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
-              w[j] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            *reinterpret_cast<uint4*>(dst + c0 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (whole) {
+            st_shared_v4(q_piece(q, r, (c0 + k) / 8), pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                         pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+          } else {
+            const int at = (c0 & 32) / 4 + k / 4;
+            st_shared_v4(q_piece(q, r, at), __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]),
+                         __float_as_uint(y[3]));
+            st_shared_v4(q_piece(q, r, at + 1), __float_as_uint(y[4]), __float_as_uint(y[5]), __float_as_uint(y[6]),
+                         __float_as_uint(y[7]));
           }
         }
+        if (whole ? c0 == 96 : (c0 & 32) != 0) {
+          __syncwarp();
+          Walk out(p, c, g * kRows + 32 * warp + (lane >> 4));
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            const int at = 32 * warp + 2 * i + (lane >> 4);
+            const uint4 y = ld_shared_v4(q_piece(q, at, lane & 15));
+            if (!whole) {
+              *reinterpret_cast<uint4*>(part + (g * kRows + at) * kHeadDim + (c0 & 64) + 4 * (lane & 15)) = y;
+            } else if (out.row < rows) {
+              *reinterpret_cast<uint4*>(p.out + out.token * p.out_row_stride + out.head * kHeadDim + 8 * (lane & 15)) = y;
+            }
+            out.two_on(p);
+          }
+          __syncwarp();
+        }
       }
-      if (!whole)
-        *reinterpret_cast<float2*>(p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart +
-                                   kItem * kHeadDim + 2 * (g * kRows + r)) = make_float2(m, l);
+      if (!whole) *reinterpret_cast<float2*>(part + kItem * kHeadDim + 2 * (g * kRows + r)) = make_float2(m, l);
       tc::fence_before_sync();  // O has been read before the next piece's first P is announced
     }
-    u += n;
-    if (u < units) {
-      c.tile += n;
-      next_pair(p, c);
-    } else if (tid == 0) {  // group 0 always has rows
-      Cut cut = {};
-      if (c.tile == 0 && n < c.tiles) {
-        cut.parts = static_cast<int>(owner(u0 + u - n + c.tiles - 1, ctas, total) - blockIdx.x + 1);
-        cut.slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
-        cut.rows = min(kItem, rows - c.rg * kItem);
-        cut.first_row = c.rg * kItem;
-        cut.token = c.s.q_first;
-        cut.head = c.kvh * p.group;
+    if (!more) {
+      if (tid == 0) {
+        Cut cut = {};
+        if (c.tile == 0 && c.end < c.tiles) {
+          const int64_t first = c.begin + kPieceUnits, last = first + c.tiles - 1;  // its tiles, as units
+          cut.parts = static_cast<int>(owner(last, ctas, total) - owner(first, ctas, total) + 1);
+          cut.slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
+          cut.rows = min(kItem, rows - c.rg * kItem);
+          cut.first_row = c.rg * kItem;
+          cut.token = c.s.q_first;
+          cut.head = c.kvh * p.group;
+        }
+        reinterpret_cast<Cut*>(p.cuts)[blockIdx.x] = cut;
       }
-      reinterpret_cast<Cut*>(p.cuts)[blockIdx.x] = cut;
+      return;
     }
-    first_piece = false;
+    u += n;
+    first_piece = !started;
+    started = true;
+    c = next;
+    n = c.end - c.tile;
+    more = c.more();
+    if (more) next_piece(p, next);
   }
 }
 
@@ -662,13 +771,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.k_full[i], 4);
       mbar_init(&sm.k_free[i], 1);
+      mbar_init(&sm.v_full[i], 4);
+      mbar_init(&sm.v_free[i], 1);
       mbar_init(&sm.q_full[i], 4);
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.p_full[i], 4);
       mbar_init(&sm.o_full[i], 1);
     }
-    mbar_init(&sm.v_full, 4);
-    mbar_init(&sm.v_free, 1);
     mbar_init(&sm.drained, 1);
     fence_mbar_init();
   }
@@ -701,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
     return;
   }
-  const int64_t u0 = range_begin(blockIdx.x, ctas, total), units = range_begin(blockIdx.x + 1, ctas, total) - u0;
+  const int64_t u0 = range_begin(blockIdx.x, ctas, total), u1 = range_begin(blockIdx.x + 1, ctas, total);
   if (before <= u0 && u0 < before + mine) {
     int64_t at = before;
     int s = s0;
@@ -724,28 +833,35 @@ __global__ void __launch_bounds__(kThreads, 1)
   c.seq = sm.first_seq;
   c.s = seq_of(p, c.seq);
   {
-    int64_t rest = u0 - sm.first_unit;
+    c.begin = sm.first_unit;
+    Groups at(p, 0);
     for (c.rg = 0;; ++c.rg) {
-      c.tiles = tiles_of(p, c.s, c.rg);
-      if (rest < static_cast<int64_t>(c.tiles) * p.num_kv_heads) break;
-      rest -= static_cast<int64_t>(c.tiles) * p.num_kv_heads;
+      c.tiles = at.tiles(c.s);
+      const int64_t of_group = static_cast<int64_t>(c.tiles + kPieceUnits) * p.num_kv_heads;
+      if (u0 < c.begin + of_group) break;
+      c.begin += of_group;
+      at.next(p);
     }
-    c.kvh = static_cast<int>(rest / c.tiles);
-    c.tile = static_cast<int>(rest - static_cast<int64_t>(c.kvh) * c.tiles);
+    c.kvh = static_cast<int>(u0 - c.begin) / (c.tiles + kPieceUnits);
+    c.begin += c.kvh * (c.tiles + kPieceUnits);
+    c.tile = max(0, static_cast<int>(u0 - c.begin) - kPieceUnits);
+    c.until = u1;
+    c.set_end();
   }
-
-  if (warp < kUnpackWarp) {
+  if (c.tile >= c.end) {  // none but what is counted for an item beside its tiles
+    if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
+  } else   if (warp < kUnpackWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    softmax_role(p, sm, c, units, ctas, total, u0, warp >> 2, tid);
+    softmax_role(p, sm, c, ctas, total, warp >> 2, tid);
   } else if (warp < kLoadWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegs));
-    unpack_role(p, sm, c, units, warp - kUnpackWarp, lane);
+    unpack_role(p, sm, c, warp - kUnpackWarp, lane);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kLoadWarp) {
-      load_role(p, map_k, map_v, sm, c, units, lane);
-    } else if (warp == kMmaWarp && lane == 0) {
-      mma_role(p, sm, c, units);
+      load_role(p, map_k, map_v, sm, c, lane);
+    } else if (warp == kMmaWarp) {
+      mma_role(p, sm, c);
     }
     __syncwarp();
   }
@@ -767,6 +883,10 @@ cudaError_t launch_int4_prefill(Int4AttnParams p, const CUtensorMap& map_k, cons
                                 int num_sms, cudaStream_t stream) {
   p.cuts = workspace;
   p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + num_sms * sizeof(Cut));
+  p.item_tokens = kItem / p.group;
+  p.item_rest = kItem % p.group;
+  p.two_tokens = 2 / p.group;
+  p.two_heads = 2 % p.group;
   p.unit_pages = kTile / p.block_size;
   p.unit_rest = kTile % p.block_size;
   cudaError_t e = cudaFuncSetAttribute(int4_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
