@@ -1299,17 +1299,31 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   rc = make_codes_map(&map_v, v_cache, rows, p.box_rows);
   if (rc) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // both kernels, then one that joins the parts of what they cut
+  auto lists = [](uint8_t* at, int rows, int ctas) {
+    return fp8attn::Int4JoinList{
+        at, reinterpret_cast<const float*>(at + static_cast<int64_t>(ctas) * fp8attn::kInt4CutBytes), rows, ctas};
+  };
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  const fp8attn::Int4JoinList few = lists(ws, fp8attn::int4_decode_rows(p.group, plan.short_q), plan.grid);
+  fp8attn::Int4JoinList many = lists(ws + plan.short_bytes, fp8attn::kInt4LongRows, plan.longer ? device_sms() : 0);
+  cudaError_t e = cudaSuccess;
   if (plan.longer) {
     p.min_q = plan.short_q;
     p.max_q = max_q;
-    const cudaError_t e = fp8attn::launch_int4_prefill(
-        p, map_k, map_v, static_cast<uint8_t*>(workspace) + plan.short_bytes, device_sms(), st);
+    p.cuts = const_cast<void*>(many.cuts);
+    p.partials = const_cast<float*>(many.partials);
+    e = fp8attn::launch_int4_prefill(p, map_k, map_v, many.ctas, st);
     if (e != cudaSuccess) return cuda_fail(e, "4-bit chunk attention launch");
   }
   p.min_q = 0;
   p.max_q = plan.short_q;
-  const cudaError_t e = fp8attn::launch_int4_decode(p, map_k, map_v, workspace, plan.grid, st);
+  p.cuts = const_cast<void*>(few.cuts);
+  p.partials = const_cast<float*>(few.partials);
+  e = fp8attn::launch_int4_decode(p, map_k, map_v, plan.grid, st);
   if (e != cudaSuccess) return cuda_fail(e, "4-bit attention launch");
+  e = fp8attn::launch_int4_join(p, few, many, st);
+  if (e != cudaSuccess) return cuda_fail(e, "4-bit attention join launch");
   return FP8ATTN_OK;
 }
 

@@ -735,12 +735,7 @@ cudaError_t launch(const Int4AttnParams& p, const CUtensorMap& map_k, const CUte
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, int4_decode_kernel<NT, kFold>, p, map_k, map_v);
-  if (e != cudaSuccess || grid < 2) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(grid - 1));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, int4_join_kernel<kFold ? 4 : 8 * NT>, p);
+  return cudaLaunchKernelEx(&cfg, int4_decode_kernel<NT, kFold>, p, map_k, map_v);
 }
 
 // The kernel for a call: 0 for at most four rows of a kv head, else planes of 8 rows in a row group, as many as the
@@ -776,13 +771,13 @@ int int4_decode_grid(int group, int max_q) {
 
 int64_t int4_decode_workspace_bytes(int group, int max_q, int grid) {
   const int64_t part = static_cast<int64_t>(rows_of(variant(group, max_q))) * (kHeadDim + 2) * 4;
-  return static_cast<int64_t>(grid) * (sizeof(Cut) + 2 * part);
+  return static_cast<int64_t>(grid) * (kInt4CutBytes + 2 * part);
 }
 
-cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, void* workspace,
-                               int grid, cudaStream_t stream) {
-  p.cuts = workspace;
-  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + grid * sizeof(Cut));
+int int4_decode_rows(int group, int max_q) { return rows_of(variant(group, max_q)); }
+
+cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid,
+                               cudaStream_t stream) {
   p.unit_pages = kUnit / p.block_size;
   p.unit_rest = kUnit % p.block_size;
   switch (variant(p.group, p.max_q)) {

@@ -1,0 +1,160 @@
+// Joins the parts of row groups that the 4-bit attention kernels' even cuts left in several CTAs.
+//
+// Part c has sums O_c, l_c of its positions for the reference maximum m_c; with M = max m_c
+//   out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c,
+// added in the order of the parts.  CTA i takes what the cut of CTA i says.  Bound by latency (descriptor, maxima, sums,
+// output: four dependent accesses of L2), so few rows with many parts are shared by several warps, and many rows with
+// few parts go four to a warp with all loads in flight.
+#include "int4_attention.cuh"
+
+namespace fp8attn {
+namespace {
+
+constexpr int kWarps = 8;
+
+__device__ __forceinline__ void add_part(float4& y, float& sum, const float4& x, float l, float f) {
+  y.x = fmaf(x.x, f, y.x);
+  y.y = fmaf(x.y, f, y.y);
+  y.z = fmaf(x.z, f, y.z);
+  y.w = fmaf(x.w, f, y.w);
+  sum = fmaf(l, f, sum);
+}
+
+__device__ __forceinline__ void store_row(const Int4AttnParams& p, const Cut& cut, int row, int lane, const float4& y,
+                                          float sum) {
+  const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+  const int r = cut.first_row + row, token = r / p.group;
+  const __nv_bfloat162 a = __floats2bfloat162_rn(y.x * inv, y.y * inv), b = __floats2bfloat162_rn(y.z * inv, y.w * inv);
+  *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(cut.token) + token) * p.out_row_stride +
+                            (cut.head + r - token * p.group) * kHeadDim + 4 * lane) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// At most 32 rows, up to as many parts as there are CTAs: several warps of a row take parts in turn, and their sums are
+// added in order.
+__device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4JoinList& list, int index) {
+  __shared__ float4 sum_o[kWarps][32];
+  __shared__ float2 sum_ml[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Cut cut = reinterpret_cast<const Cut*>(list.cuts)[index];
+  const int parts = cut.parts, part_size = list.rows * (kHeadDim + 2);
+  if (parts == 0) return;
+  const float* first = list.partials + static_cast<int64_t>(cut.slot) * part_size;
+  const float* later = list.partials + static_cast<int64_t>(2 * index) * part_size;
+  auto part = [&](int j) { return j == 0 ? first : later + static_cast<int64_t>(2 * j) * part_size; };
+  const int ml_at = list.rows * kHeadDim;
+  const int share = max(1, min(kWarps / cut.rows, parts));  // warps of a row
+  const int at_once = kWarps / share;                       // rows
+  for (int row0 = 0; row0 < cut.rows; row0 += at_once) {
+    const int row = row0 + warp / share, turn = warp % share;
+    const bool mine = warp < at_once * share && row < cut.rows;
+    float mx = kNone, sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mine) {
+      for (int j = turn + lane * share; j < parts; j += 32 * share) mx = fmaxf(mx, part(j)[ml_at + 2 * row]);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+#pragma unroll 8
+      for (int j = turn; j < parts; j += share) {
+        const float2 ml = *reinterpret_cast<const float2*>(part(j) + ml_at + 2 * row);
+        const float4 x = *reinterpret_cast<const float4*>(part(j) + row * kHeadDim + 4 * lane);
+        add_part(y, sum, x, ml.y, ex2(ml.x - mx));
+      }
+    }
+    if (share > 1) {
+      __syncthreads();  // the rows before these have been read
+      sum_o[warp][lane] = y;
+      if (lane == 0) sum_ml[warp] = make_float2(mx, sum);
+      __syncthreads();
+      if (mine && turn == 0) {
+        float top = kNone;
+        for (int w = 0; w < share; ++w) top = fmaxf(top, sum_ml[warp + w].x);
+        y = make_float4(0.f, 0.f, 0.f, 0.f);
+        sum = 0.f;
+        for (int w = 0; w < share; ++w)
+          add_part(y, sum, sum_o[warp + w][lane], sum_ml[warp + w].y, ex2(sum_ml[warp + w].x - top));
+      }
+    }
+    if (mine && turn == 0) store_row(p, cut, row, lane, y, sum);
+  }
+}
+
+// Up to kInt4LongRows rows, four to a warp.
+constexpr int kRowsPerCta = 4 * kWarps;
+__device__ __forceinline__ void join_many(const Int4AttnParams& p, const Int4JoinList& list, int index, int block) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Cut cut = reinterpret_cast<const Cut*>(list.cuts)[index];
+  const int parts = cut.parts, part_size = list.rows * (kHeadDim + 2), row0 = block * kRowsPerCta + 4 * warp;
+  if (parts == 0 || row0 >= cut.rows) return;
+  const float* first = list.partials + static_cast<int64_t>(cut.slot) * part_size;
+  const float* later = list.partials + static_cast<int64_t>(2 * index) * part_size;
+  auto part = [&](int j) { return j == 0 ? first : later + static_cast<int64_t>(2 * j) * part_size; };
+  const int ml_at = list.rows * kHeadDim + 2 * row0;
+  float mx[4] = {kNone, kNone, kNone, kNone}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = lane; j < parts; j += 32) {
+    const float4 a = *reinterpret_cast<const float4*>(part(j) + ml_at);  // (m, l) of two rows
+    const float4 b = *reinterpret_cast<const float4*>(part(j) + ml_at + 4);
+    mx[0] = fmaxf(mx[0], a.x);
+    mx[1] = fmaxf(mx[1], a.z);
+    mx[2] = fmaxf(mx[2], b.x);
+    mx[3] = fmaxf(mx[3], b.z);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], off));
+  float4 y[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int j = 0; j < parts; ++j) {
+    const float4 a = *reinterpret_cast<const float4*>(part(j) + ml_at);
+    const float4 b = *reinterpret_cast<const float4*>(part(j) + ml_at + 4);
+    float4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(part(j) + (row0 + k) * kHeadDim + 4 * lane);
+    add_part(y[0], sum[0], x[0], a.y, ex2(a.x - mx[0]));
+    add_part(y[1], sum[1], x[1], a.w, ex2(a.z - mx[1]));
+    add_part(y[2], sum[2], x[2], b.y, ex2(b.x - mx[2]));
+    add_part(y[3], sum[3], x[3], b.w, ex2(b.z - mx[3]));
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (row0 + k < cut.rows) store_row(p, cut, row0 + k, lane, y[k], sum[k]);
+}
+
+// CTAs [0, few.ctas) join the cuts of the kernel for few rows, the others those of the kernel for long chunks.
+__global__ void __launch_bounds__(kWarps * 32)
+    int4_join_kernel(const __grid_constant__ Int4AttnParams p, const Int4JoinList few, const Int4JoinList many) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int at = static_cast<int>(blockIdx.x) - few.ctas;
+  if (at < 0) {
+    join_few(p, few, blockIdx.x);
+  } else {
+    constexpr int kBlocks = kInt4LongRows / kRowsPerCta;
+    join_many(p, many, at / kBlocks, at % kBlocks);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_int4_join(const Int4AttnParams& p, Int4JoinList few, Int4JoinList many, cudaStream_t stream) {
+  // the last CTA's range ends with a pair
+  few.ctas = few.ctas > 1 ? few.ctas - 1 : 0;
+  many.ctas = many.ctas > 1 ? many.ctas - 1 : 0;
+  const int blocks = few.ctas + many.ctas * (kInt4LongRows / kRowsPerCta);
+  if (blocks == 0) return cudaSuccess;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, int4_join_kernel, p, few, many);
+}
+
+}  // namespace fp8attn

@@ -31,16 +31,11 @@ namespace {
 constexpr int kRows = 128;          // of a group
 constexpr int kItem = 2 * kRows;    // rows of a work item
 constexpr int kTile = 128;          // positions
-constexpr int kPieceUnits = 2;      // what a work item costs beside its tiles, in units of a tile
+constexpr int kPieceUnits = 3;      // what a work item costs beside its tiles, in units of a tile
 constexpr int kRaw = 3;             // stages of codes, K 0, K 1, V 0, K 2, V 1, ...
 constexpr int kThreads = 512;
 constexpr int kUnpackWarp = 8, kLoadWarp = 12, kMmaWarp = 13;
-#ifndef PS
-#define PS 184
-#define PU 88
-#define PO 56
-#endif
-constexpr int kSoftmaxRegs = PS, kUnpackRegs = PU, kOtherRegs = PO;
+constexpr int kSoftmaxRegs = 184, kUnpackRegs = 88, kOtherRegs = 56;
 static_assert(2 * kSoftmaxRegs + kUnpackRegs + kOtherRegs == 4 * 128, "all of the registers, and no more");
 constexpr float kSlack = 8.f;  // a reference maximum may lag by 2^8
 constexpr float kLift = 4.f;   // P and its sums are 2^4 times as large: P between 2^-14 and 2^12 is a normal number
@@ -439,45 +434,46 @@ __device__ __forceinline__ void mma_role(const Int4AttnParams& p, Smem& sm, Curs
   for (int u = 0; ok;) {
     const int n = c.end - c.tile;
     const int groups = c.s.nq * p.group - c.rg * kItem > kRows ? 2 : 1;
+#pragma unroll 1
     for (int i = 0; i <= n && ok; ++i) {
       const int at = u + i;  // scores of this unit, values of the one before it
-      for (int g = 0; g < groups && ok; ++g) {
-        if (i > 0) {  // O_g += P_g V, 16 positions at a time: V's rows are 128 bytes
-          const int buf = (at - 1) & 1;
-          if (g == 0) ok = wait_all(&sm.v_full[buf], static_cast<uint32_t>((at - 1) >> 1) & 1u, p.err);
+      const int k_buf = at & 1, v_buf = (at - 1) & 1;
+#pragma unroll 1
+      for (int g = 0; g < groups; ++g) {
+        // all that the group's products wait for, and then all of them: the tensor cores run dry between two blocks
+        if (g == 0) {
+          if (i > 0) ok = wait_all(&sm.v_full[v_buf], static_cast<uint32_t>((at - 1) >> 1) & 1u, p.err);
+          if (i < n) ok = ok && wait_all(&sm.k_full[k_buf], static_cast<uint32_t>(at >> 1) & 1u, p.err);
+        }
+        if (i == 0) ok = ok && wait_all(&sm.q_full[g], q_parity >> g & 1u, p.err);
+        if (i > 0) {
           ok = ok && wait_all(&sm.p_full[g], p_parity >> g & 1u, p.err);
-          if (!ok) break;
           p_parity ^= 1u << g;
-          tc::fence_after_sync();
-          if (elect_one()) {
-            const uint64_t b = dv + static_cast<uint64_t>(buf * (2 * kOBytes >> 4));
+        }
+        if (!ok) break;
+        tc::fence_after_sync();
+        if (elect_one()) {
+          if (i > 0) {  // O_g += P_g V, 16 positions at a time: V's rows are 128 bytes
+            const uint64_t b = dv + static_cast<uint64_t>(v_buf * (2 * kOBytes >> 4));
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
               tc::mma_f16_ts(tmem + 256 * g + 128, tmem + 256 * g + 8 * k, b + static_cast<uint64_t>(k * (16 * 128 >> 4)),
                              idesc_pv, i > 1 || k > 0 ? 1u : 0u);
             if (i == n) tc::commit(&sm.o_full[g]);
-            if (g == groups - 1) tc::commit(&sm.v_free[buf]);
+            if (g == groups - 1) tc::commit(&sm.v_free[v_buf]);
           }
-          __syncwarp();
-        }
-        if (i < n) {
-          const int buf = at & 1;
-          if (g == 0) ok = wait_all(&sm.k_full[buf], static_cast<uint32_t>(at >> 1) & 1u, p.err);
-          if (i == 0) ok = ok && wait_all(&sm.q_full[g], q_parity >> g & 1u, p.err);
-          if (!ok) break;
-          tc::fence_after_sync();
-          if (elect_one()) {
-            const uint64_t a = dq + static_cast<uint64_t>(g * (2 * kOBytes >> 4)), b = dk + static_cast<uint64_t>(buf * (2 * kOBytes >> 4));
+          if (i < n) {
+            const uint64_t a = dq + static_cast<uint64_t>(g * (2 * kOBytes >> 4)), b = dk + static_cast<uint64_t>(k_buf * (2 * kOBytes >> 4));
 #pragma unroll
             for (int k = 0; k < 8; ++k) {  // 16 values: 32 bytes, four to a block
               const uint64_t step = static_cast<uint64_t>((k >> 2) * (kOBytes >> 4) + (k & 3) * 2);
               mma_f16_ss(tmem + 256 * g, a + step, b + step, idesc_s, k > 0 ? 1u : 0u);
             }
             tc::commit(&sm.s_full[g]);
-            if (g == groups - 1) tc::commit(&sm.k_free[buf]);
+            if (g == groups - 1) tc::commit(&sm.k_free[k_buf]);
           }
-          __syncwarp();
         }
+        __syncwarp();
       }
     }
     q_parity ^= groups == 2 ? 3u : 1u;
@@ -532,6 +528,23 @@ __device__ __forceinline__ uint32_t seen_of(uint32_t there, int seen, int c0) {
   return held & (left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u);
 }
 
+// Minus infinity for the columns that a row does not see.
+__device__ __forceinline__ void hide(uint32_t (&w)[4][32], uint32_t there, int seen) {
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const uint32_t mask = seen_of(there, seen, 32 * h);
+#pragma unroll
+    for (int k = 0; k < 32; ++k)
+      if (!(mask >> k & 1u)) w[h][k] = 0xFF800000u;
+  }
+}
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // The 16-byte piece of a 256-byte row (of q, or of outputs on their way out) in a group's q.
 __device__ __forceinline__ uint32_t q_piece(uint32_t q, int row, int piece) {
   return q + (piece >> 3) * kOBytes + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
@@ -545,7 +558,6 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
   uint32_t s_parity = 0, o_parity = 0;
   constexpr int kPart = kItem * (kHeadDim + 2);
   bool first_piece = true;
-  uint4 raw[16];
   Cursor c = next;
   bool started = false, more = true;
   for (int u = 0, n = 0;;) {
@@ -557,10 +569,19 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
       const int token = row / p.group;
       const int limit = row < rows ? min(c.s.vis, token + c.s.nk - c.s.nq + 1) : c.s.vis;  // no row: zeros that see anything
       // ---- q: each thread turns its row into f16; a power of two puts the largest value between 2^13 and 2^14
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        st_shared_v4(q_piece(q, 32 * warp + 2 * i + (lane >> 4), lane & 15), raw[i].x, raw[i].y, raw[i].z, raw[i].w);
-      __syncwarp();
+      // A warp brings its 32 rows two at a time, 16 lanes to a row: whole lines.
+      {
+        Walk at(p, c, g * kRows + 32 * warp + (lane >> 4));
+#pragma unroll 2
+        for (int i = 0; i < 16; ++i) {
+          cp_async16(q_piece(q, 32 * warp + 2 * i + (lane >> 4), lane & 15),
+                     p.q + at.token * p.q_row_stride + at.head * kHeadDim + 8 * (lane & 15), at.row < rows);
+          at.two_on(p);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncwarp();
+      }
       uint32_t top_bits = 0;  // bf16 magnitudes in order as integers, two at a time
 #pragma unroll 4
       for (int i = 0; i < 16; ++i) {
@@ -602,29 +623,22 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         float f = sm.v_change[slot];
         const uint32_t there = sm.there[slot];
         const int seen = limit - (c.tile + i) * kTile;  // columns below this one
-        uint32_t v[4][32];
+        const bool masked = !__all_sync(0xffffffffu, there == 0xFFu && seen >= kTile);
+        uint32_t w[4][32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32(s_tmem + 32 * q, v[q]);
+        for (int h = 0; h < 4; ++h) tmem_ld32(s_tmem + 32 * h, w[h]);
         tc::wait_ld();
-        if (!__all_sync(0xffffffffu, (there & 0xFFu) == 0xFFu && seen >= kTile)) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t mask = seen_of(there, seen, 32 * q);
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (!(mask >> k & 1u)) v[q][k] = 0xFF800000u;
-          }
-        }
-        // ---- the row's maximum
+        if (masked) hide(w, there, seen);
+        // ---- the row's maximum; NaN where it sees one
         float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int h = 0; h < 4; ++h)
 #pragma unroll
           for (int k = 0; k < 32; k += 2)
-            t[k / 2 & 3] = fmaxf(t[k / 2 & 3], fmaxf(__uint_as_float(v[q][k]), __uint_as_float(v[q][k + 1])));
-        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * ct;
+            t[k / 2 & 3] = max3_nan(t[k / 2 & 3], __uint_as_float(w[h][k]), __uint_as_float(w[h][k + 1]));
+        const float top = max3_nan(max3_nan(t[0], t[1], t[2]), t[3], t[3]) * ct;
         // ---- a new reference maximum where it lags too far, and V's power of two
-        if (top > m + kSlack) {
+        if (!(top <= m + kSlack)) {  // also for NaN: the row's sums and outputs become NaN
           const float lag = ex2(m - top);
           m = top;
           l *= lag;
@@ -646,17 +660,22 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         const uint64_t ct2 = f2_pack(ct, ct), bias2 = f2_pack(bias, bias);
         uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int h = 0; h < 4; ++h) {
           uint32_t pw[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(v[q][2 * k]), __uint_as_float(v[q][2 * k + 1])), ct2, bias2), x0, x1);
-            const float p0 = ex2(x0), p1 = ex2(x1);
+            float x0, x1, p0, p1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(w[h][2 * k]), __uint_as_float(w[h][2 * k + 1])), ct2, bias2), x0, x1);
+            if (k % 4 == 3) {
+              exp2_poly_x2(x0, x1, p0, p1);
+            } else {
+              p0 = ex2(x0);
+              p1 = ex2(x1);
+            }
             sum[k & 1] = f2_add(sum[k & 1], f2_pack(p0, p1));
             pw[k] = pack_f16x2(p0, p1);
           }
-          tc::st16u(s_tmem + 16 * q, pw);
+          tc::st16u(s_tmem + 16 * h, pw);
         }
         float a0, a1, b0, b1;
         f2_unpack(sum[0], a0, a1);
@@ -668,17 +687,13 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         if ((tid & 31) == 0) mbar_arrive(&sm.p_full[g]);
       }
     }
-    // ---- the next piece's q, before this one's outputs are stored: a warp loads its 32 rows two at a time, 16 lanes to
-    // a row (whole lines)
+    // ---- the next piece's q on its way to L2
     if (more) {
-      const int next_rows = next.s.nq * p.group;
-      Walk at(p, next, g * kRows + 32 * warp + (lane >> 4));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        raw[i] = make_uint4(0, 0, 0, 0);
-        if (at.row < next_rows) raw[i] = ldg_keep_v4(p.q + at.token * p.q_row_stride + at.head * kHeadDim + 8 * (lane & 15));
-        at.two_on(p);
-      }
+      const int next_row = min(next.rg * kItem + g * kRows + r, next.s.nq * p.group - 1), next_token = next_row / p.group;
+      const uint16_t* src = p.q + (static_cast<int64_t>(next.s.q_first) + next_token) * p.q_row_stride +
+                            (next.kvh * p.group + next_row - next_token * p.group) * kHeadDim;
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 64));
     }
     // ---- the piece's end
     if (active) {
@@ -686,7 +701,7 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
       o_parity ^= 1u;
       tc::fence_after_sync();
       const bool whole = c.whole();
-      const float f = !whole ? back : l == 0.f ? 0.f : __fdiv_rn(back, l);
+      const float f = !whole ? back : m == kNone ? 0.f : __fdiv_rn(back, l);  // 0 for a row that sees nothing
       // rows leave through the group's q, which no product reads any more, so that stores are whole lines: 256 bytes of
       // a row at a time, 128 bf16 values or 64 fp32 ones
       float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart;
@@ -875,14 +890,14 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of an SM");
 
 }  // namespace
 
+static_assert(kItem == kInt4LongRows, "the joining kernel's rows");
+
 int64_t int4_prefill_workspace_bytes(int num_sms) {
-  return static_cast<int64_t>(num_sms) * (sizeof(Cut) + 2ll * kItem * (kHeadDim + 2) * 4);
+  return static_cast<int64_t>(num_sms) * (kInt4CutBytes + 2ll * kItem * (kHeadDim + 2) * 4);
 }
 
-cudaError_t launch_int4_prefill(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, void* workspace,
-                                int num_sms, cudaStream_t stream) {
-  p.cuts = workspace;
-  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + num_sms * sizeof(Cut));
+cudaError_t launch_int4_prefill(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int num_sms,
+                                cudaStream_t stream) {
   p.item_tokens = kItem / p.group;
   p.item_rest = kItem % p.group;
   p.two_tokens = 2 / p.group;
@@ -901,12 +916,7 @@ cudaError_t launch_int4_prefill(Int4AttnParams p, const CUtensorMap& map_k, cons
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, int4_prefill_kernel, p, map_k, map_v);
-  if (e != cudaSuccess || num_sms < 2) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(num_sms - 1), 16);
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, int4_join_kernel<kItem>, p);
+  return cudaLaunchKernelEx(&cfg, int4_prefill_kernel, p, map_k, map_v);
 }
 
 }  // namespace fp8attn

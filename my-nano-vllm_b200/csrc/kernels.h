@@ -250,13 +250,25 @@ struct Int4AttnParams {
   void* cuts;       // workspace: for each CTA the pair that its range leaves cut
   float* partials;  // workspace: two parts for each CTA
 };
+// What the joining kernel reads of one of the two: for each of its CTAs a cut and two parts.
+struct Int4JoinList {
+  const void* cuts;
+  const float* partials;
+  int rows;  // of a row group
+  int ctas;
+};
+constexpr int kInt4LongRows = 256;
 int int4_decode_grid(int group, int max_q);  // CTAs that run at once on the current device; 0: error
+int int4_decode_rows(int group, int max_q);  // of a row group
 int64_t int4_decode_workspace_bytes(int group, int max_q, int grid);
-cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, void* workspace,
-                               int grid, cudaStream_t stream);
+// p.cuts and p.partials: one Cut of kInt4CutBytes for each CTA and two parts
+constexpr int kInt4CutBytes = 32;
+cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid,
+                               cudaStream_t stream);
 int64_t int4_prefill_workspace_bytes(int num_sms);
-cudaError_t launch_int4_prefill(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, void* workspace,
-                                int num_sms, cudaStream_t stream);
+cudaError_t launch_int4_prefill(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int num_sms,
+                                cudaStream_t stream);
+cudaError_t launch_int4_join(const Int4AttnParams& p, Int4JoinList few, Int4JoinList many, cudaStream_t stream);
 // The error word of the 4-bit attention kernels on the current device.
 cudaError_t int4_error_word(void** word);
 

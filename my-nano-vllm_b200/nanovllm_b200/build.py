@@ -22,7 +22,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libfp8attn.so")
 
 SOURCES = ["capi.cu", "store.cu", "decode.cu", "prefill.cu", "prefill_persistent.cu", "diag.cu",
            "qknorm.cu", "fp8linear.cu", "ffn_quant.cu", "moe.cu", "rope.cu", "int4_cache.cu",
-           "int4_decode.cu", "int4_prefill.cu"]
+           "int4_decode.cu", "int4_prefill.cu", "int4_join.cu"]
 HEADERS = ["common.cuh", "kernels.h", "tcgen05.cuh", "prefill_common.cuh",
            "int4_attention.cuh"]
 
