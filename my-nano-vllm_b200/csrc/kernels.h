@@ -218,6 +218,8 @@ struct Int4RowsParams {
   int64_t num_slots;
   int num_kv_heads;
   int block_size;
+  uint32_t block_inverse;  // set by the launch
+  int block_shift;
 };
 cudaError_t launch_int4_store(const Int4RowsParams& p, cudaStream_t stream);
 cudaError_t launch_int4_load(const Int4RowsParams& p, cudaStream_t stream);
