@@ -17,7 +17,7 @@
 namespace fp8attn {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 
 template <bool kFp16>
 __device__ __forceinline__ float widen(uint32_t bits16) {
@@ -194,7 +194,7 @@ cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
                                     rows(p.k_out, p.k_out_token_stride, p.k_out_head_stride)));
   };
   const bool small = p.num_tokens * (p.num_heads + p.num_kv_heads) < 8192;
-  if (fits(8, 16)) return small ? launch<8, 1>(p, stream) : launch<8, 4>(p, stream);
+  if (fits(8, 16)) return small ? launch<8, 1>(p, stream) : launch<8, 2>(p, stream);
   if (fits(2, 4)) return launch<2, 4>(p, stream);
   return launch<1, 4>(p, stream);
 }
