@@ -11,10 +11,15 @@ namespace {
 
 constexpr float kNone = -3.402823466e38f;
 
-// mbar_wait with its polling loop out of line, for a whole warp.
-__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, int* err) { return mbar_wait(bar, parity, err); }
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
-  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || wait_long(bar, parity, err));
+// A warp's wait, bounded by a number of polls (each of some tens of cycles: a second or more).  Small, since it stands in
+// many places: the roles' loops share the instruction cache.
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, int* err) {
+  bool done = false;
+#pragma unroll 1
+  for (uint32_t polls = 0; polls < (1u << 26) && !done; ++polls) done = mbar_try_wait(bar, parity);
+  done = __all_sync(0xffffffffu, done);
+  if (!done) atomicExch(err, kDevErrWaitTimeout);
+  return done;
 }
 
 // size bytes (a multiple of 16, both addresses too) from global to shared memory, counted on the mbarrier.
@@ -40,9 +45,19 @@ struct Cut {
 };
 static_assert(sizeof(Cut) == kInt4CutBytes, "as in kernels.h");
 
-// First unit of CTA i of n over u units, and the CTA that has unit x.
-__device__ __forceinline__ int64_t range_begin(int64_t i, int64_t n, int64_t u) { return i * u / n; }
-__device__ __forceinline__ int64_t owner(int64_t x, int64_t n, int64_t u) { return ((x + 1) * n - 1) / u; }
+// u units in n ranges of equal size, the first u % n of them one longer.
+struct Ranges {
+  int64_t each, longer;
+  __device__ __forceinline__ Ranges(int64_t u, int n) {
+    each = u >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(u) / static_cast<uint32_t>(n)) : u / n;
+    longer = u - each * n;
+  }
+  __device__ __forceinline__ int64_t begin(int i) const { return i * each + min(static_cast<int64_t>(i), longer); }
+  __device__ __forceinline__ int owner(int64_t x) const {  // range of unit x
+    const int64_t split = longer * (each + 1);
+    return static_cast<int>(x < split ? x / (each + 1) : longer + (x - split) / each);
+  }
+};
 
 }  // namespace
 }  // namespace fp8attn

@@ -41,38 +41,53 @@ namespace {
 // hold its address.
 __device__ int g_error = 0;
 
-#ifndef INT4_W
-#define INT4_W 4
-#define INT4_S 3
-#define INT4_C 3
-#endif
-constexpr int kWarps = INT4_W;          // that compute; one more loads
-constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kTile = 32;               // positions per warp and unit
-constexpr int kUnit = kTile * kWarps;   // positions per unit
-constexpr int kParts = kUnit / 16;      // parts of a unit that lie in one page each
-constexpr int kStages = INT4_S;
-constexpr int kPitch = 136;             // floats between rows of the joined sums (bank spread)
+constexpr int kPitch = 136;             // floats between rows of the sums on their way out (bank spread)
 constexpr float kSlack = 8.f;           // a reference maximum may lag by 2^8
+constexpr int kPieceUnits = 1;          // what a pair costs beside its tiles, in units of a tile
 
-template <int NT>
-struct __align__(1024) Smem {
-  uint8_t k[kStages][kUnit * 64];  // TMA tiles of 64-byte rows, 64B swizzle: bits 1 and 2 of a row's number
-  uint8_t v[kStages][kUnit * 64];  // change the place of its 16-byte pieces
-  uint2 scale[kStages][kUnit];
-  uint2 q[NT][8][32];              // B operand of S^T: plane, step, lane
-  float kq[8 * NT], qs[8 * NT];    // score = dot kq step + qs low
-  float o[kWarps][8][kPitch];      // a plane's sums, joined over the warps
-  float m[kWarps][8], l[kWarps][8];
-  uint64_t full[kStages], empty[kStages];
-  uint32_t there[kStages];         // which parts of the stage's unit are in pages of the cache
-  int64_t scan[kWarps + 1];
-  int64_t first_unit;              // of the sequence in which the CTA's range begins
-  int first_seq;
+// How a CTA is made up: computing warps and one that loads.  One plane of query rows: four, and three CTAs on an SM
+// (128 registers).  More planes: eight with 224 registers.
+template <int NT_, bool kFold_>
+struct Shape {
+  static constexpr int NT = NT_;            // planes of 8 columns
+  static constexpr bool kFold = kFold_;     // at most four rows, held twice in the eight columns
+  static constexpr int R = kFold ? 4 : 8 * NT;  // rows of a group
+  static constexpr bool kWide = NT > 1;
+  static constexpr int kWarps = kWide ? 8 : 4;
+  static constexpr int kThreads = kWarps * 32 + (kWide ? 128 : 32);
+  static constexpr int kCtas = kWide ? 1 : 3;
+  static constexpr int kStages = kWide ? 4 : 3;
+  static constexpr int kUnit = kTile * kWarps;  // positions per unit
+  static constexpr int kParts = kUnit / 16;     // parts of a unit that lie in one page each
 };
 
-// The computing warps alone.
-__device__ __forceinline__ void sync_compute() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+constexpr int kWideRegs = 216, kLoadRegs = 72;
+static_assert(2 * kWideRegs + kLoadRegs == 3 * 168, "all of the registers of 384 threads, and no more");
+
+// A piece's rows, and where its sums go.
+struct Done {
+  int first_row, rows;  // of the kv head; rows of it in all
+  int token, head;      // the sequence's first row of q, the kv head's first query head
+  int slot;             // of the partial sums, -1: the piece is a whole pair
+};
+
+template <typename S>
+struct __align__(1024) Smem {
+  uint8_t k[S::kStages][S::kUnit * 64];  // TMA tiles of 64-byte rows, 64B swizzle: bits 1 and 2 of a row's number
+  uint8_t v[S::kStages][S::kUnit * 64];  // change the place of its 16-byte pieces
+  uint2 scale[S::kStages][S::kUnit];
+  uint16_t rows[2][S::R][kHeadDim];      // q of two pieces
+  uint2 q[S::kWide ? S::NT : 1][8][S::kWide ? 32 : 1];  // as the B operand of S^T: plane, step, lane
+  alignas(8) float kq[8 * S::NT], qs[8 * S::NT];  // score = dot kq step + qs low
+  float o[S::kWarps][8][kPitch];         // a plane's sums
+  float m[S::kWarps][8], l[S::kWarps][8];
+  uint64_t full[S::kStages], empty[S::kStages], q_full[2], q_free[2], o_full, o_free;
+  uint32_t there[S::kStages];            // which parts of the stage's unit are in pages of the cache
+  int64_t scan[S::kThreads / 32];
+  int64_t first_unit;                    // of the sequence in which the CTA's range begins
+  int first_seq;
+};
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
@@ -88,14 +103,6 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-// w >> 8 on the multiply pipe (by = 2^24, in a register so that it stays a product): the unpacking's masks keep
-// the integer pipe busier than anything else.
-__device__ __forceinline__ uint32_t shift8(uint32_t w, uint32_t by) {
-  uint32_t d;
-  d = w >> 8; (void)by;
-  return d;
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -122,18 +129,18 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) 
 struct Seq {
   int q_first, nq, nk, vis, tiles, groups;
   __device__ __forceinline__ int64_t units(int kvh) const {
-    return static_cast<int64_t>(tiles) * groups * kvh;
+    return static_cast<int64_t>(tiles + kPieceUnits) * groups * kvh;
   }
 };
 
-template <int R>
+template <typename S>
 __device__ __forceinline__ Seq seq_of(const Int4AttnParams& p, int s) {
   Seq q;
   if (p.cu_q != nullptr) {
     q.q_first = __ldg(p.cu_q + s);
     q.nq = __ldg(p.cu_q + s + 1) - q.q_first;
     q.nk = __ldg(p.cu_k + s + 1) - __ldg(p.cu_k + s);
-    if (q.nq > p.max_q) q.nq = 0;  // the chunk kernel's
+    if (q.nq > p.max_q) q.nq = 0;  // the other kernel's
   } else {
     q.q_first = s;
     q.nq = 1;
@@ -141,74 +148,193 @@ __device__ __forceinline__ Seq seq_of(const Int4AttnParams& p, int s) {
   }
   q.vis = max(0, min(q.nk, p.max_blocks * p.block_size));
   // a sequence without positions still has its zeros written
-  q.tiles = max(1, (q.vis + kUnit - 1) / kUnit);
-  q.groups = q.nq <= 0 ? 0 : (q.nq * p.group + R - 1) / R;
+  q.tiles = max(1, (q.vis + S::kUnit - 1) / S::kUnit);
+  q.groups = q.nq <= 0 ? 0 : (q.nq * p.group + S::R - 1) / S::R;
   return q;
 }
 
-// Where in the order of units a warp is.
+// The token of a kv head's row r, of nq group < 2^31 / group
+__device__ __forceinline__ int token_of(const Int4AttnParams& p, int r) { return __umulhi(2 * r, p.group_inverse); }
+
+// The piece that a warp is at: tiles [tile, end) of a pair (row group, kv head).  A pair's units are kPieceUnits for what
+// it costs beside its tiles, and then its tiles; a piece is what of it lies in the CTA's range, which ends at unit `until`.
 struct Cursor {
-  int seq, pair, tile;  // pair: row group * KVH + kv head
+  int seq, rg, kvh, tile, end;
+  int64_t begin, until;  // the pair's first unit
   Seq s;
+  // Whether another piece with a tile follows.
+  __device__ __forceinline__ bool more() const { return begin + s.tiles + 2 * kPieceUnits < until; }
+  __device__ __forceinline__ void set_end() {
+    end = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(s.tiles), until - begin - kPieceUnits)));
+  }
 };
 
-template <int R>
-__device__ __forceinline__ void next_pair(const Int4AttnParams& p, Cursor& c) {
+template <typename S>
+__device__ __forceinline__ void next_piece(const Int4AttnParams& p, Cursor& c) {
   c.tile = 0;
-  if (++c.pair < c.s.groups * p.num_kv_heads) return;
-  c.pair = 0;
-  do {
-    if (++c.seq >= p.num_seqs) return;
-    c.s = seq_of<R>(p, c.seq);
-  } while (c.s.groups == 0);
+  c.begin += c.s.tiles + kPieceUnits;
+  if (++c.kvh >= p.num_kv_heads) {
+    c.kvh = 0;
+    if (++c.rg >= c.s.groups) {
+      c.rg = 0;
+      do {  // there is one: more()
+        c.s = seq_of<S>(p, ++c.seq);
+      } while (c.s.groups == 0);
+    }
+  }
+  c.set_end();
 }
 
-// The loading warp: lane i looks up the page of part i of each unit, and the lanes at which a TMA box begins load it
-// (box_rows positions: K, V and scales).  The pages of the next unit are looked up before this one's stage is waited
-// for.
-template <int NT, int R>
-__device__ __forceinline__ void load_units(const Int4AttnParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
-                                           Smem<NT>& sm, Cursor c, int64_t u0, int64_t u1, int lane) {
-  int column = 0, place = 0;
+// A row of q as lanes 4 g .. 4 g + 3 hold it for column g of the B operand of S^T: values 32 t .. 32 t + 31 in the order
+// of the codes.  A power of two puts the row's largest value between 2^13 and 2^14; odd values, whose codes stand four
+// bits higher, / 16.
+__device__ __forceinline__ void convert_q(const uint16_t* row, bool is_row, int t, float scale_log2, uint2 (&q)[8],
+                                          float& kq, float& qs) {
+  uint4 raw[4] = {};
+  if (is_row) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) raw[w] = *reinterpret_cast<const uint4*>(row + 32 * t + 8 * w);
+  }
+  float amax = 0.f, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t word[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x0 = __uint_as_float(word[i] << 16), x1 = __uint_as_float(word[i] & 0xFFFF0000u);
+      amax = fmaxf(amax, fmaxf(fabsf(x0), fabsf(x1)));
+      sum += x0 + x1;
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  }
+  const int e = amax > 0.f && amax < INFINITY ? max(-100, min(exponent(amax), 110)) - 13 : 0;
+  const float even = pow2(-e), odd = pow2(-e - 4);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t word[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {  // values 2 b and 2 b + 4; 2 b + 1 and 2 b + 5
+      const uint32_t lo = word[b], hi = word[b + 2];
+      q[2 * w + b] = make_uint2(pack_f16x2(__uint_as_float(lo << 16) * even, __uint_as_float(hi << 16) * even),
+                                pack_f16x2(__uint_as_float(lo & 0xFFFF0000u) * odd, __uint_as_float(hi & 0xFFFF0000u) * odd));
+    }
+  }
+  kq = pow2(e) * 16777216.f * scale_log2;  // e + 24 <= 121
+  qs = sum * scale_log2;
+}
+
+// This warp's share of a plane's rows, the warps' sums joined: outputs of a whole pair, or a part for the joining kernel.
+template <typename S>
+__device__ __forceinline__ void merge_plane(const Int4AttnParams& p, const Smem<S>& sm, const Done& d, int j, int warp,
+                                            int lane) {
+  constexpr int kRows = S::kFold ? 4 : 8, kFrom = S::kFold ? 2 : 1;
+#pragma unroll 1
+  for (int row = warp; row < kRows; row += S::kWarps) {
+    const int in_group = 8 * j + row, r = d.first_row + in_group;
+    if (r >= d.rows) break;
+    float mx = kNone;
+#pragma unroll
+    for (int w = 0; w < S::kWarps; ++w)
+#pragma unroll
+      for (int f = 0; f < kFrom; ++f) mx = fmaxf(mx, sm.m[w][row + 4 * f]);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < S::kWarps; ++w) {
+#pragma unroll
+      for (int f = 0; f < kFrom; ++f) {
+        const float weight = ex2(sm.m[w][row + 4 * f] - mx);
+        const float4 x = *reinterpret_cast<const float4*>(&sm.o[w][row + 4 * f][4 * lane]);
+        y.x = fmaf(x.x, weight, y.x);
+        y.y = fmaf(x.y, weight, y.y);
+        y.z = fmaf(x.z, weight, y.z);
+        y.w = fmaf(x.w, weight, y.w);
+        sum = fmaf(sm.l[w][row + 4 * f], weight, sum);
+      }
+    }
+    if (d.slot < 0) {
+      const int token = token_of(p, r);
+      const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);  // 0 for a row that sees nothing
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(y.x * inv, y.y * inv), hi = __floats2bfloat162_rn(y.z * inv, y.w * inv);
+      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(d.token) + token) * p.out_row_stride +
+                                (d.head + r - token * p.group) * kHeadDim + 4 * lane) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+      float* const part = p.partials + static_cast<int64_t>(d.slot) * (S::R * (kHeadDim + 2));
+      *reinterpret_cast<float4*>(part + in_group * kHeadDim + 4 * lane) = y;
+      if (lane == 0) *reinterpret_cast<float2*>(part + S::R * kHeadDim + 2 * in_group) = make_float2(mx, sum);
+    }
+  }
+}
+
+// Loads by one warp: a piece's rows of q (lane i: row i), and its units: lane i looks up the page of part i, and the
+// lanes at which a TMA box of box_rows positions begins load K, V and scales.
+template <typename S>
+__device__ __forceinline__ void load(const Int4AttnParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                                     Smem<S>& sm, Cursor c, int lane) {
+  int column = 0, place = 0, page = -1, stage = 0;
+  uint32_t round = 0, loaded = 0, pieces = 0;
+  const bool begins = lane < S::kParts && lane % (p.box_rows / 16) == 0;
+  bool ok = true, first = true;  // the unit is its piece's first
   auto look_up = [&]() {
-    const int pos = c.tile * kUnit + lane * 16;
-    if (lane >= kParts || pos >= c.s.vis) return -1;
-    const int page = ldg_keep(p.block_tables + c.seq * p.bt_stride + column);
-    return page >= 0 && page < p.num_blocks ? page : -1;
+    const int pos = c.tile * S::kUnit + lane * 16;
+    page = -1;
+    if (lane < S::kParts && pos < c.s.vis) {
+      const int found = ldg_keep(p.block_tables + c.seq * p.bt_stride + column);
+      if (found >= 0 && found < p.num_blocks) page = found;
+    }
   };
   auto find = [&]() {
-    const int pos = c.tile * kUnit + lane * 16;
+    const int pos = c.tile * S::kUnit + lane * 16;
     column = pos / p.block_size;
     place = pos - column * p.block_size;
-    return look_up();
+    look_up();
   };
-  int page = find();
-  int stage = 0;
-  uint32_t round = 0, loaded = 0;
-  const bool begins = lane < kParts && lane % (p.box_rows / 16) == 0;
-  bool ok = true;
-  for (int64_t u = u0; u < u1; ++u) {
-    const int kvh = c.pair % p.num_kv_heads;
-    const int row = (page * p.num_kv_heads + kvh) * p.block_size + place;
+  find();
+#pragma unroll 1
+  for (;;) {
+    if (first) {
+      const int b = pieces & 1, rows = c.s.nq * p.group - c.rg * S::R;  // from the group's first on
+      if (pieces > 1) ok = wait_all(&sm.q_free[b], ((pieces >> 1) - 1) & 1u, p.err);
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&sm.q_full[b], min(S::R, rows) * kHeadDim * 2);
+      __syncwarp();
+      if (lane < S::R && lane < rows) {
+        const int r = c.rg * S::R + lane, token = token_of(p, r);
+        bulk_load(smem_u32(sm.rows[b][lane]),
+                  p.q + (static_cast<int64_t>(c.s.q_first) + token) * p.q_row_stride +
+                      (c.kvh * p.group + r - token * p.group) * kHeadDim,
+                  kHeadDim * 2, &sm.q_full[b]);
+      }
+      ++pieces;
+      first = false;
+    }
+    const int row = (page * p.num_kv_heads + c.kvh) * p.block_size + place;
     const bool mine = begins && page >= 0;
     const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
     const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
     // the next unit's pages
-    if (u + 1 < u1) {
-      if (++c.tile < c.s.tiles) {
-        column += p.unit_pages;  // whole pages in a unit, and what is left
-        place += p.unit_rest;
-        if (place >= p.block_size) {
-          place -= p.block_size;
-          ++column;
-        }
-        page = look_up();
-      } else {
-        next_pair<R>(p, c);
-        page = find();
+    bool more = true;
+    if (++c.tile < c.end) {
+      column += p.unit_pages;  // whole pages in a unit, and what is left
+      place += p.unit_rest;
+      if (place >= p.block_size) {
+        place -= p.block_size;
+        ++column;
       }
+      look_up();
+    } else if (c.more()) {
+      next_piece<S>(p, c);
+      find();
+      first = true;
+    } else {
+      more = false;
     }
-    if (round > 0) ok = wait_warp(&sm.empty[stage], round - 1 & 1u, p.err);
+    if (round > 0) ok = wait_all(&sm.empty[stage], (round - 1) & 1u, p.err);
     if (!ok) break;
     uint64_t* bar = &sm.full[stage];
     if (lane == 0) {
@@ -222,90 +348,24 @@ __device__ __forceinline__ void load_units(const Int4AttnParams& p, const CUtens
       bulk_load(smem_u32(sm.scale[stage] + lane * 16), p.kv_scale + static_cast<int64_t>(row) * 4, p.box_rows * 8, bar);
     }
     loaded |= 1u << stage;
-    if (++stage == kStages) {
+    if (++stage == S::kStages) {
       stage = 0;
       ++round;
     }
+    if (!more) return;
   }
-  // copies in flight after a wait that gave up: they must land (or run out of time) before the CTA ends
-  if (!ok)
-    for (int i = 0; i < kStages; ++i)
-      if (loaded >> i & 1u) wait_warp(&sm.full[i], (i < stage ? round : round - 1) & 1u, p.err);
+  // a wait gave up: the copies in flight must land (or run out of time) before the CTA ends
+  for (int i = 0; i < S::kStages; ++i)
+    if (loaded >> i & 1u) wait_all(&sm.full[i], (i < stage ? round : round - 1) & 1u, p.err);
+  for (uint32_t i = pieces > 2 ? pieces - 2 : 0; i < pieces; ++i) wait_all(&sm.q_full[i & 1], (i >> 1) & 1u, p.err);
 }
 
-template <int NT, bool kFold>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_kernel(
-    const __grid_constant__ Int4AttnParams p, const __grid_constant__ CUtensorMap map_k,
-    const __grid_constant__ CUtensorMap map_v) {
-  extern __shared__ uint8_t smem_raw[];
-  Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(smem_raw + (1024 - smem_u32(smem_raw) % 1024) % 1024);
-  constexpr int R = kFold ? 4 : 8 * NT;  // rows of a group
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  if (tid == 0) {
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], kWarps);
-    }
-    fence_mbar_init();
-  }
-  // programmatic dependent of the kernel before it: nothing is read or written before that ends
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  // ---- plan: units before each sequence; thread i has sequences [i * per, (i + 1) * per)
-  const int per = (p.num_seqs + kThreads - 1) / kThreads;
-  const int s0 = min(tid * per, p.num_seqs), s1 = min(s0 + per, p.num_seqs);
-  int64_t mine = 0;
-  for (int s = s0; s < s1; ++s) mine += seq_of<R>(p, s).units(p.num_kv_heads);
-  int64_t before = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, before, off);
-    if (lane >= off) before += v;
-  }
-  if (lane == 31) sm.scan[warp] = before;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps + 1; ++w) {
-    if (w < warp) before += sm.scan[w];
-    total += sm.scan[w];
-  }
-  before -= mine;
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
-  Cut* cuts = reinterpret_cast<Cut*>(p.cuts);
-  if (blockIdx.x >= ctas) {
-    if (tid == 0) cuts[blockIdx.x].parts = 0;
-    return;
-  }
-  const int64_t u0 = range_begin(blockIdx.x, ctas, total), u1 = range_begin(blockIdx.x + 1, ctas, total);
-  if (before <= u0 && u0 < before + mine) {
-    int64_t at = before;
-    int s = s0;
-    for (; s < s1; ++s) {
-      const int64_t n = seq_of<R>(p, s).units(p.num_kv_heads);
-      if (u0 < at + n) break;
-      at += n;
-    }
-    sm.first_seq = s;
-    sm.first_unit = at;
-  }
-  __syncthreads();
-  Cursor now;
-  now.seq = sm.first_seq;
-  now.s = seq_of<R>(p, now.seq);
-  {
-    const int64_t rest = u0 - sm.first_unit;
-    now.pair = static_cast<int>(rest / now.s.tiles);
-    now.tile = static_cast<int>(rest - static_cast<int64_t>(now.pair) * now.s.tiles);
-  }
-
-  if (warp == kWarps) {
-    load_units<NT, R>(p, map_k, map_v, sm, now, u0, u1, lane);
-    return;
-  }
-
+template <typename S>
+__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges& ranges, int warp,
+                                        int lane) {
+  constexpr int NT = S::NT, R = S::R;
+  constexpr bool kFold = S::kFold;
+  const int g = lane >> 2, t = lane & 3;
   // this lane's row for the transposed loads of V, and its piece (of the second of two: 1) as it is stored; its
   // rows g and g + 8 of K, piece t
   const int v_token = (lane & 7) + (lane & 8);
@@ -313,86 +373,75 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
   const uint32_t k_row = (warp * kTile + g) * 64 + (t ^ (g >> 1 & 3)) * 16;
   const uint32_t k_ring = smem_u32(sm.k[0]) + k_row, v_ring = smem_u32(sm.v[0]) + v_row;
   const uint32_t s_ring = smem_u32(sm.scale[0]) + (warp * kTile + g) * 8;
-  uint32_t by8;
-  asm volatile("mov.u32 %0, 0x1000000;" : "=r"(by8));
   int stage = 0;
-  uint32_t parity = 0;
+  uint32_t parity = 0, pieces = 0;
   bool ok = true;  // no wait has given up
-  for (int64_t u = u0; u < u1;) {
-    // ---- a piece: units [u, u + n) of one pair
-    const int n = static_cast<int>(min(u1 - u, static_cast<int64_t>(now.s.tiles - now.tile)));
-    const bool whole = now.tile == 0 && n == now.s.tiles;
-    const int kvh = now.pair % p.num_kv_heads, rg = now.pair / p.num_kv_heads;
+  Done done = {};  // the piece before
+  auto all_warps = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(S::kWarps * 32) : "memory"); };
+  auto merge_last = [&](int j) {  // one plane: a warp joins its rows of the piece before when it has begun the next
+    ok = ok && wait_all(&sm.o_full, (pieces - 1) & 1u, p.err);
+    if (ok) merge_plane(p, sm, done, j, warp, lane);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.o_free);
+  };
+#pragma unroll 1
+  for (;; ++pieces) {
+    const int n = now.end - now.tile, kvh = now.kvh, rg = now.rg;
     const int rows = now.s.nq * p.group;  // of this kv head
-    // q: the B operand of S^T, plane j by warp j.  Column (row) g, values 32 t .. 32 t + 31 in the order
-    // of the codes
-    if (warp < NT) {
-      const int r = rg * R + (kFold ? g & 3 : 8 * warp + g);
-      uint4 raw[4] = {};
-      if (r < rows) {
-        const int token = r / p.group;
-        const uint16_t* src = p.q + (static_cast<int64_t>(now.s.q_first) + token) * p.q_row_stride +
-                              (kvh * p.group + r - token * p.group) * kHeadDim + 32 * t;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) raw[w] = ldg_keep_v4(src + 8 * w);
-      }
-      float amax = 0.f, sum = 0.f;
-      float x[4][8];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t word[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[w][2 * i] = __uint_as_float(word[i] << 16);
-          x[w][2 * i + 1] = __uint_as_float(word[i] & 0xFFFF0000u);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          amax = fmaxf(amax, fabsf(x[w][i]));
-          sum += x[w][i];
-        }
-      }
-#pragma unroll
-      for (int off = 1; off < 4; off <<= 1) {
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-        sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      }
-      // the largest value between 2^13 and 2^14; odd values, whose codes stand four bits higher, / 16
-      const int e = amax > 0.f && amax < INFINITY ? max(-100, min(exponent(amax), 110)) - 13 : 0;
-      const float even = pow2(-e), odd = pow2(-e - 4);
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          sm.q[warp][2 * w + b][lane] = make_uint2(pack_f16x2(x[w][2 * b] * even, x[w][2 * b + 4] * even),
-                                                   pack_f16x2(x[w][2 * b + 1] * odd, x[w][2 * b + 5] * odd));
-      if (t == 0) {
-        sm.kq[8 * warp + g] = pow2(e) * 16777216.f * p.scale_log2;  // e + 24 <= 121
-        sm.qs[8 * warp + g] = sum * p.scale_log2;
-      }
-    }
-    sync_compute();
+    const int buf = pieces & 1;
+    ok = ok && wait_all(&sm.q_full[buf], (pieces >> 1) & 1u, p.err);
     constexpr bool kHeld = NT <= 2;  // q stays in registers; else it is read from shared memory for each tile
     uint2 q[kHeld ? NT : 1][8];
-    if constexpr (kHeld) {
+    [[maybe_unused]] uint64_t kq[NT], qs[NT];  // for this thread's columns 2 t and 2 t + 1; wide: in shared memory
+    if constexpr (!S::kWide) {
+      const int in_group = kFold ? g & 3 : g;
+      float a, b;
+      convert_q(sm.rows[buf][in_group], rg * R + in_group < rows, t, p.scale_log2, q[0], a, b);
+      kq[0] = f2_pack(__shfl_sync(0xffffffffu, a, 8 * t), __shfl_sync(0xffffffffu, a, 8 * t + 4));
+      qs[0] = f2_pack(__shfl_sync(0xffffffffu, b, 8 * t), __shfl_sync(0xffffffffu, b, 8 * t + 4));
+      if (lane == 0) mbar_arrive(&sm.q_free[buf]);
+      if (pieces > 0) merge_last(0);
+    } else {
+      if (warp < NT) {
+        uint2 y[8];
+        float a, b;
+        convert_q(sm.rows[buf][8 * warp + g], rg * R + 8 * warp + g < rows, t, p.scale_log2, y, a, b);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+        for (int i = 0; i < 8; ++i) sm.q[warp][i][lane] = y[i];
+        if (t == 0) {
+          sm.kq[8 * warp + g] = a;
+          sm.qs[8 * warp + g] = b;
+        }
+      }
+      all_warps();
+      if (lane == 0) mbar_arrive(&sm.q_free[buf]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[j][i] = sm.q[j][i][lane];
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int i = 0; i < 8 && kHeld; ++i) q[kHeld ? j : 0][i] = sm.q[j][i][lane];
+      }
     }
-    float kq[NT][2], qs[NT][2];  // for this thread's columns 2 t and 2 t + 1
-    int limit[NT][2], least = INT_MAX, most = 0;
+    auto kq_of = [&](int j) {
+      if constexpr (S::kWide) return reinterpret_cast<const uint64_t*>(sm.kq)[4 * j + t];
+      else return kq[j];
+    };
+    auto qs_of = [&](int j) {
+      if constexpr (S::kWide) return reinterpret_cast<const uint64_t*>(sm.qs)[4 * j + t];
+      else return qs[j];
+    };
+    int least = INT_MAX, most = 0;
+    auto limit_of = [&](int j, int c) {  // positions that a column's row sees; where there is no row, as the group's first
+      int row = rg * R + (kFold ? (2 * t + c) & 3 : 8 * j + 2 * t + c);
+      if (row >= rows) row = rg * R;
+      return min(now.s.vis, token_of(p, row) + now.s.nk - now.s.nq + 1);
+    };
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        kq[j][c] = sm.kq[8 * j + 2 * t + c];
-        qs[j][c] = sm.qs[8 * j + 2 * t + c];
-        const int row = rg * R + (kFold ? (2 * t + c) & 3 : 8 * j + 2 * t + c);
-        limit[j][c] = min(now.s.vis, row / p.group + now.s.nk - now.s.nq + 1);
-        if (row >= rows) limit[j][c] = min(now.s.vis, rg * R / p.group + now.s.nk - now.s.nq + 1);  // no row: as the first
-        least = min(least, limit[j][c]);
-        most = max(most, limit[j][c]);
+        const int limit = limit_of(j, c);
+        least = min(least, limit);
+        most = max(most, limit);
       }
     }
 #pragma unroll
@@ -401,17 +450,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
       most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
     }
 
-    float o[NT][8][4], ps[NT][4], m[NT][2], l[NT][2], mid[NT][2];  // ps: sum of the rounded P step
-    float m_limit[NT][2];  // m and how far it may lag
+    float o[NT][8][4], ps[NT][4];     // ps: sum of the rounded P step
+    uint64_t minus_m[NT], l[NT], mid[NT];  // pairs of columns
+    uint32_t unset = (1u << 2 * NT) - 1;   // columns that have seen nothing: their m counts as 0
+    float limit = -INFINITY;               // how far a score may be above its m: kSlack when none is unset
     float v_unit = 1.f, v_limit = 0.f;  // steps of V are multiplied by v_unit (a power of two)
     int v_exp = 0;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        m[j][c] = m_limit[j][c] = kNone;
-        l[j][c] = mid[j][c] = 0.f;
-      }
+      minus_m[j] = l[j] = mid[j] = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) ps[j][c] = 0.f;
 #pragma unroll
@@ -420,9 +467,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
         for (int c = 0; c < 4; ++c) o[j][i][c] = 0.f;
     }
 
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      const int pos0 = (now.tile + i) * kUnit + warp * kTile;
-      ok = ok && wait_warp(&sm.full[stage], parity, p.err);
+      const int pos0 = (now.tile + i) * S::kUnit + warp * kTile;
+      ok = ok && wait_all(&sm.full[stage], parity, p.err);
       const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
       if (halves != 0 && pos0 < most && ok) {
         // ---- S^T: positions (rows g, g + 8 of each half) x query rows (columns)
@@ -432,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
+            const uint4 k = ld_shared_v4(k_ring + stage * (S::kUnit * 64) + h * 1024 + r * 512);
             kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
           }
         }
@@ -443,8 +491,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
             uint32_t a[2][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t y0 = b ? shift8(kw[h][0][w], by8) : kw[h][0][w];
-              const uint32_t y1 = b ? shift8(kw[h][1][w], by8) : kw[h][1][w];
+              const uint32_t y0 = kw[h][0][w] >> (8 * b);
+              const uint32_t y1 = kw[h][1][w] >> (8 * b);
               a[h][0] = y0 & 0x000F000Fu;
               a[h][1] = y1 & 0x000F000Fu;
               a[h][2] = y0 & 0x00F000F0u;
@@ -452,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const uint2 qb = kHeld ? q[kHeld ? j : 0][2 * w + b] : sm.q[j][2 * w + b][lane];
+              const uint2 qb = kHeld ? q[kHeld ? j : 0][2 * w + b] : sm.q[kHeld ? 0 : j][2 * w + b][lane];
               if (w == 0 && b == 0) {
                 mma16816_first(s[0][j], a[0], qb.x, qb.y);
                 mma16816_first(s[1][j], a[1], qb.x, qb.y);
@@ -479,18 +527,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
           const int half = kFold ? t >> 1 : h;
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + half * 128 + r * 64);
+            const uint2 sc = ld_shared_v2(s_ring + stage * (S::kUnit * 8) + half * 128 + r * 64);
             const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
             sv[h][r] = __uint_as_float(sc.y << 16);
             mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
+            const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int c = 0; c < 2; ++c)
-                s[h][j][2 * r + c] = fmaf(s[h][j][2 * r + c], sk * kq[j][c], lk * qs[j][c]);
+            for (int j = 0; j < NT; ++j) {
+              const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq_of(j)),
+                                        f2_fma(lk2, qs_of(j), minus_m[j]));
+              f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
+            }
           }
         }
         if (!full) {
+          int sees[NT][2];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            sees[j][0] = limit_of(j, 0);
+            sees[j][1] = limit_of(j, 1);
+          }
 #pragma unroll
           for (int h = 0; h < H; ++h) {
             const int half = kFold ? t >> 1 : h;
@@ -503,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
               for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                  if (!held || pos >= limit[j][c]) s[h][j][2 * r + c] = -INFINITY;
+                  if (!held || pos >= sees[j][c]) s[h][j][2 * r + c] = -INFINITY;
             }
           }
         }
@@ -513,9 +569,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
           for (int r = 0; r < 2; ++r) {
             grow |= sv[h][r] > v_limit;
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) grow |= s[h][j][2 * r + c] > m_limit[j][c];
+            for (int j = 0; j < NT; ++j) grow |= fmaxf(s[h][j][2 * r], s[h][j][2 * r + 1]) > limit;
           }
         if (__any_sync(0xffffffffu, grow)) {
           // ---- new references: the rows' maxima so far, and a power of two near V's largest step
@@ -537,26 +591,38 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
           }
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
+            float was[2], now_m[2], f[2];
+            f2_unpack(minus_m[j], was[0], was[1]);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float mx = m[j][c];
+              float mx = -INFINITY;  // above m
 #pragma unroll
               for (int h = 0; h < H; ++h) mx = fmaxf(mx, fmaxf(s[h][j][c], s[h][j][2 + c]));
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-              const float f = ex2(m[j][c] - mx);
-              m[j][c] = mx;
-              m_limit[j][c] = mx + kSlack;
-              l[j][c] *= f;
-              mid[j][c] *= f;
-              ps[j][c] *= f * change;
+              const bool first = unset >> (2 * j + c) & 1u;
+              if (first && mx == -INFINITY) mx = 0.f;  // still unset
+              else unset &= ~(1u << (2 * j + c));
+              if (!first) mx = fmaxf(mx, 0.f);
+              f[c] = first ? 0.f : ex2(-mx);
+              now_m[c] = was[c] - mx;
+#pragma unroll
+              for (int h = 0; h < H; ++h) {
+                s[h][j][c] -= mx;
+                s[h][j][2 + c] -= mx;
+              }
+              ps[j][c] *= f[c] * change;
 #pragma unroll
               for (int d = 0; d < 8; ++d) {
-                o[j][d][c] *= f * change;
-                o[j][d][2 + c] *= f * change;
+                o[j][d][c] *= f[c] * change;
+                o[j][d][2 + c] *= f[c] * change;
               }
             }
+            minus_m[j] = f2_pack(now_m[0], now_m[1]);
+            l[j] = f2_mul(l[j], f2_pack(f[0], f[1]));
+            mid[j] = f2_mul(mid[j], f2_pack(f[0], f[1]));
           }
+          limit = __any_sync(0xffffffffu, unset != 0) ? -INFINITY : kSlack;
         }
         // ---- P, its sums, and P^T step_v as the B operand of O^T
         uint32_t pb[2][NT][2];
@@ -565,14 +631,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const float f = sv[h][r] * v_unit;
+            const uint64_t f2 = f2_pack(f, f), mv2 = f2_pack(mv[h][r], mv[h][r]);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const float p0 = ex2(s[h][j][2 * r] - m[j][0]), p1 = ex2(s[h][j][2 * r + 1] - m[j][1]);
-              l[j][0] += p0;
-              l[j][1] += p1;
-              mid[j][0] = fmaf(p0, mv[h][r], mid[j][0]);
-              mid[j][1] = fmaf(p1, mv[h][r], mid[j][1]);
-              pb[h][j][r] = transpose8x8(pack_f16x2(p0 * f, p1 * f));
+              const uint64_t x = f2_pack(ex2(s[h][j][2 * r]), ex2(s[h][j][2 * r + 1]));
+              l[j] = f2_add(l[j], x);
+              mid[j] = f2_fma(x, mv2, mid[j]);
+              float p0, p1;
+              f2_unpack(f2_mul(x, f2), p0, p1);
+              pb[h][j][r] = transpose8x8(pack_f16x2(p0, p1));
             }
           }
         }
@@ -595,13 +662,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
 #pragma unroll
           for (int w = 0; w < 4; w += 2) {
             uint32_t v[4];  // piece w: rows 0-7 and 8-15, piece w + 1: the same
-            ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + h * 1024 + (w ^ v_piece) * 16);
+            ldmatrix_trans(v, v_ring + stage * (S::kUnit * 64) + h * 1024 + (w ^ v_piece) * 16);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
 #pragma unroll
               for (int b = 0; b < 2; ++b) {
-                const uint32_t y0 = b ? shift8(v[2 * x], by8) : v[2 * x];
-                const uint32_t y1 = b ? shift8(v[2 * x + 1], by8) : v[2 * x + 1];
+                const uint32_t y0 = v[2 * x] >> (8 * b);
+                const uint32_t y1 = v[2 * x + 1] >> (8 * b);
                 const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
 #pragma unroll
                 for (int j = 0; j < NT; ++j) mma16816(o[j][2 * (w + x) + b], a, pb[h][j][0], pb[h][j][1]);
@@ -612,130 +679,207 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? INT4_C : 2) int4_decode_ke
       }
       __syncwarp();  // every lane has read the stage
       if (lane == 0) mbar_arrive(&sm.empty[stage]);
-      if (++stage == kStages) {
+      if (++stage == S::kStages) {
         stage = 0;
         parity ^= 1u;
       }
     }
 
-    // ---- the piece's sums: the warps' parts joined through shared memory, a plane at a time
+    // ---- the piece's sums
+    const bool whole = now.tile == 0 && now.end == now.s.tiles;
+    done = {rg * R, rows, now.s.q_first, kvh * p.group, whole ? -1 : 2 * static_cast<int>(blockIdx.x) + (pieces > 0 ? 1 : 0)};
     const float unit_even = 16777216.f, unit_odd = 1048576.f, back = pow2(v_exp);
-    float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (u == u0 ? 0 : 1)) * (R * (kHeadDim + 2));
+    if (!S::kWide && pieces > 0) ok = ok && wait_all(&sm.o_free, (pieces - 1) & 1u, p.err);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
+      float m[2], sum[2], middle[2];
+      f2_unpack(minus_m[j], m[0], m[1]);
+      f2_unpack(l[j], sum[0], sum[1]);
+      f2_unpack(mid[j], middle[0], middle[1]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
-          l[j][c] += __shfl_xor_sync(0xffffffffu, l[j][c], off);
-          mid[j][c] += __shfl_xor_sync(0xffffffffu, mid[j][c], off);
+          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], off);
+          middle[c] += __shfl_xor_sync(0xffffffffu, middle[c], off);
         }
         if (g == 0) {
-          sm.m[warp][2 * t + c] = m[j][c];
-          sm.l[warp][2 * t + c] = l[j][c];
+          sm.m[warp][2 * t + c] = unset >> (2 * j + c) & 1u ? kNone : -m[c];
+          sm.l[warp][2 * t + c] = sum[c];
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // values 32 (i >> 1) + 4 g + 2 (i & 1) and the one after it
-          const float y0 = fmaf(fmaf(o[j][i][c], unit_even, -7.5f * ps[j][c]), back, mid[j][c]);
-          const float y1 = fmaf(fmaf(o[j][i][2 + c], unit_odd, -7.5f * ps[j][c]), back, mid[j][c]);
+          const float y0 = fmaf(fmaf(o[j][i][c], unit_even, -7.5f * ps[j][c]), back, middle[c]);
+          const float y1 = fmaf(fmaf(o[j][i][2 + c], unit_odd, -7.5f * ps[j][c]), back, middle[c]);
           *reinterpret_cast<float2*>(&sm.o[warp][2 * t + c][32 * (i >> 1) + 4 * g + 2 * (i & 1)]) = make_float2(y0, y1);
         }
       }
-      sync_compute();
-      constexpr int kRows = kFold ? 4 : 8;
-#pragma unroll
-      for (int idx = tid; idx < kRows * 64; idx += kWarps * 32) {
-        const int row = idx >> 6, value = 2 * (idx & 63);
-        float mx = kNone;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          mx = fmaxf(mx, sm.m[w][row]);
-          if (kFold) mx = fmaxf(mx, sm.m[w][row + 4]);
-        }
-        float y0 = 0.f, y1 = 0.f, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-#pragma unroll
-          for (int f4 = 0; f4 < (kFold ? 8 : 4); f4 += 4) {
-            const float f = ex2(sm.m[w][row + f4] - mx);
-            const float2 y = *reinterpret_cast<const float2*>(&sm.o[w][row + f4][value]);
-            y0 = fmaf(y.x, f, y0);
-            y1 = fmaf(y.y, f, y1);
-            sum = fmaf(sm.l[w][row + f4], f, sum);
-          }
-        }
-        const int in_group = 8 * j + row;
-        if (whole) {
-          const int r = rg * R + in_group;
-          if (r < rows) {
-            const int token = r / p.group;
-            // 0 for a row that sees nothing
-            const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-            uint16_t* dst = p.out + (static_cast<int64_t>(now.s.q_first) + token) * p.out_row_stride +
-                            (kvh * p.group + r - token * p.group) * kHeadDim + value;
-            *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(y0 * inv, y1 * inv);
-          }
-        } else {
-          *reinterpret_cast<float2*>(part + in_group * kHeadDim + value) = make_float2(y0, y1);
-          if (value == 0) *reinterpret_cast<float2*>(part + R * kHeadDim + 2 * in_group) = make_float2(mx, sum);
-        }
+      if constexpr (S::kWide) {
+        all_warps();
+        if (ok) merge_plane(p, sm, done, j, warp, lane);
+        all_warps();
       }
-      sync_compute();
+    }
+    if constexpr (!S::kWide) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.o_full);
     }
     // ---- on to the next pair
-    u += n;
-    if (u < u1) {
-      next_pair<R>(p, now);
-    } else if (tid == 0) {
-      Cut cut = {};
-      if (now.tile == 0 && n < now.s.tiles) {
-        cut.parts = static_cast<int>(owner(u - n + now.s.tiles - 1, ctas, total) - blockIdx.x + 1);
-        cut.slot = 2 * blockIdx.x + (u - n > u0 ? 1 : 0);
-        cut.rows = min(R, rows - rg * R);
-        cut.first_row = rg * R;
-        cut.token = now.s.q_first;
-        cut.head = kvh * p.group;
+    if (!now.more()) {
+      if (warp == 0 && lane == 0) {
+        Cut cut = {};
+        if (now.tile == 0 && now.end < now.s.tiles) {
+          const int64_t first = now.begin + kPieceUnits, last = first + now.s.tiles - 1;  // its tiles, as units
+          cut.parts = ranges.owner(last) - ranges.owner(first) + 1;
+          cut.slot = 2 * blockIdx.x + (pieces > 0 ? 1 : 0);
+          cut.rows = min(R, rows - rg * R);
+          cut.first_row = rg * R;
+          cut.token = now.s.q_first;
+          cut.head = kvh * p.group;
+        }
+        reinterpret_cast<Cut*>(p.cuts)[blockIdx.x] = cut;
       }
-      cuts[blockIdx.x] = cut;
+      break;
     }
+    next_piece<S>(p, now);
+  }
+  if constexpr (!S::kWide) {
+    ++pieces;
+    merge_last(0);
   }
 }
 
-template <int NT>
-constexpr int kSmemBytes = static_cast<int>(sizeof(Smem<NT>)) + 1024;  // its alignment
+template <typename S>
+__global__ void __launch_bounds__(S::kThreads, S::kCtas)
+    int4_decode_kernel(const __grid_constant__ Int4AttnParams p, const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v) {
+  extern __shared__ uint8_t smem_raw[];
+  Smem<S>& sm = *reinterpret_cast<Smem<S>*>(smem_raw + (1024 - smem_u32(smem_raw) % 1024) % 1024);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+#pragma unroll
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], S::kWarps);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_full[i], 1);
+      mbar_init(&sm.q_free[i], S::kWarps);
+    }
+    mbar_init(&sm.o_full, S::kWarps);
+    mbar_init(&sm.o_free, S::kWarps);
+    fence_mbar_init();
+  }
+  // programmatic dependent of the kernel before it: nothing is read or written before that ends
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-template <int NT, bool kFold>
-cudaError_t prepare() {
-  return cudaFuncSetAttribute(int4_decode_kernel<NT, kFold>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              kSmemBytes<NT>);
+  // ---- plan: units before each sequence; thread i has sequences [i * per, (i + 1) * per)
+  const int per = (p.num_seqs + S::kThreads - 1) / S::kThreads;
+  const int s0 = min(tid * per, p.num_seqs), s1 = min(s0 + per, p.num_seqs);
+  int64_t mine = 0;
+  for (int s = s0; s < s1; ++s) mine += seq_of<S>(p, s).units(p.num_kv_heads);
+  int64_t before = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += v;
+  }
+  if (lane == 31) sm.scan[warp] = before;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < S::kThreads / 32; ++w) {
+    if (w < warp) before += sm.scan[w];
+    total += sm.scan[w];
+  }
+  before -= mine;
+  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+  Cut* cuts = reinterpret_cast<Cut*>(p.cuts);
+  if (static_cast<int>(blockIdx.x) >= ctas) {
+    if (tid == 0) cuts[blockIdx.x].parts = 0;
+    return;
+  }
+  const Ranges ranges(total, ctas);
+  const int64_t u0 = ranges.begin(blockIdx.x);
+  if (before <= u0 && u0 < before + mine) {
+    int64_t at = before;
+    int s = s0;
+    for (; s < s1; ++s) {
+      const int64_t n = seq_of<S>(p, s).units(p.num_kv_heads);
+      if (u0 < at + n) break;
+      at += n;
+    }
+    sm.first_seq = s;
+    sm.first_unit = at;
+  }
+  __syncthreads();
+  Cursor c;
+  c.seq = sm.first_seq;
+  c.s = seq_of<S>(p, c.seq);
+  {
+    const int64_t rest = u0 - sm.first_unit;
+    const int each = c.s.tiles + kPieceUnits;
+    const int pair = rest >> 32 == 0 ? static_cast<int>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(each))
+                                     : static_cast<int>(rest / each);
+    c.begin = sm.first_unit + static_cast<int64_t>(pair) * each;
+    c.rg = pair / p.num_kv_heads;
+    c.kvh = pair - c.rg * p.num_kv_heads;
+    c.tile = max(0, static_cast<int>(u0 - c.begin) - kPieceUnits);
+    c.until = ranges.begin(blockIdx.x + 1);
+    c.set_end();
+  }
+  if (c.tile >= c.end) {  // none but what is counted for a pair beside its tiles
+    if (tid == 0) cuts[blockIdx.x].parts = 0;
+    return;
+  }
+  if (warp < S::kWarps) {
+    if constexpr (S::kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegs));
+    compute<S>(p, sm, c, ranges, warp, lane);
+  } else {
+    if constexpr (S::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+    if (warp == S::kWarps) load<S>(p, map_k, map_v, sm, c, lane);
+  }
 }
 
-template <int NT, bool kFold>
+template <typename S>
+constexpr int kSmemBytes = static_cast<int>(sizeof(Smem<S>)) + 1024;  // its alignment
+
+template <typename S>
+cudaError_t prepare() {
+  static_assert(kSmemBytes<S> * S::kCtas <= (227 - (S::kCtas - 1)) * 1024, "shared memory of an SM");
+  return cudaFuncSetAttribute(int4_decode_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes<S>);
+}
+
+template <typename S>
 int resident(int num_sms) {  // CTAs that run at once
   int per_sm = 0;
-  if (prepare<NT, kFold>() != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int4_decode_kernel<NT, kFold>, kThreads,
-                                                    kSmemBytes<NT>) != cudaSuccess)
+  if (prepare<S>() != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int4_decode_kernel<S>, S::kThreads, kSmemBytes<S>) !=
+          cudaSuccess)
     return 0;
   return per_sm * num_sms;
 }
 
-template <int NT, bool kFold>
-cudaError_t launch(const Int4AttnParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid,
-                   cudaStream_t stream) {
-  cudaError_t e = prepare<NT, kFold>();
+template <typename S>
+cudaError_t launch(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid, cudaStream_t stream) {
+  cudaError_t e = prepare<S>();
   if (e != cudaSuccess) return e;
+  p.unit_pages = S::kUnit / p.block_size;
+  p.unit_rest = S::kUnit % p.block_size;
+  p.group_inverse = static_cast<uint32_t>(((int64_t{1} << 31) + p.group - 1) / p.group);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes<NT>;
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes<S>;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, int4_decode_kernel<NT, kFold>, p, map_k, map_v);
+  return cudaLaunchKernelEx(&cfg, int4_decode_kernel<S>, p, map_k, map_v);
 }
 
 // The kernel for a call: 0 for at most four rows of a kv head, else planes of 8 rows in a row group, as many as the
@@ -759,11 +903,11 @@ int int4_decode_grid(int group, int max_q) {
   int n = known[dev][v].load(std::memory_order_relaxed);
   if (n == 0) {
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    n = v == 0   ? resident<1, true>(sms)
-        : v == 1 ? resident<1, false>(sms)
-        : v == 2 ? resident<2, false>(sms)
-        : v == 3 ? resident<3, false>(sms)
-                 : resident<4, false>(sms);
+    n = v == 0   ? resident<Shape<1, true>>(sms)
+        : v == 1 ? resident<Shape<1, false>>(sms)
+        : v == 2 ? resident<Shape<2, false>>(sms)
+        : v == 3 ? resident<Shape<3, false>>(sms)
+                 : resident<Shape<4, false>>(sms);
     known[dev][v].store(n, std::memory_order_relaxed);
   }
   return n;
@@ -778,14 +922,12 @@ int int4_decode_rows(int group, int max_q) { return rows_of(variant(group, max_q
 
 cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid,
                                cudaStream_t stream) {
-  p.unit_pages = kUnit / p.block_size;
-  p.unit_rest = kUnit % p.block_size;
   switch (variant(p.group, p.max_q)) {
-    case 0: return launch<1, true>(p, map_k, map_v, grid, stream);
-    case 1: return launch<1, false>(p, map_k, map_v, grid, stream);
-    case 2: return launch<2, false>(p, map_k, map_v, grid, stream);
-    case 3: return launch<3, false>(p, map_k, map_v, grid, stream);
-    default: return launch<4, false>(p, map_k, map_v, grid, stream);
+    case 0: return launch<Shape<1, true>>(p, map_k, map_v, grid, stream);
+    case 1: return launch<Shape<1, false>>(p, map_k, map_v, grid, stream);
+    case 2: return launch<Shape<2, false>>(p, map_k, map_v, grid, stream);
+    case 3: return launch<Shape<3, false>>(p, map_k, map_v, grid, stream);
+    default: return launch<Shape<4, false>>(p, map_k, map_v, grid, stream);
   }
 }
 

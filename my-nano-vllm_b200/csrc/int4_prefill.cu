@@ -139,17 +139,6 @@ __device__ __forceinline__ void next_piece(const Int4AttnParams& p, Cursor& c) {
   c.set_end();
 }
 
-// A warp's wait, bounded by a number of polls (each of some tens of cycles: a second or more).  Small, since it stands in
-// many places: the roles' loops share the instruction cache.
-__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, int* err) {
-  bool done = false;
-#pragma unroll 1
-  for (uint32_t polls = 0; polls < (1u << 26) && !done; ++polls) done = mbar_try_wait(bar, parity);
-  done = __all_sync(0xffffffffu, done);
-  if (!done) atomicExch(err, kDevErrWaitTimeout);
-  return done;
-}
-
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -550,8 +539,8 @@ __device__ __forceinline__ uint32_t q_piece(uint32_t q, int row, int piece) {
   return q + (piece >> 3) * kOBytes + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
 }
 
-__device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor next, int64_t ctas,
-                                             int64_t total, int g, int tid) {
+__device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor next, const Ranges& ranges,
+                                             int g, int tid) {
   const int r = tid & 127, warp = r >> 5, lane = tid & 31;
   const uint32_t s_tmem = sm.tmem + (static_cast<uint32_t>(32 * warp) << 16) + 256 * g, o_tmem = s_tmem + 128;
   const uint32_t q = smem_u32(sm.q[g]);
@@ -751,7 +740,7 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         Cut cut = {};
         if (c.tile == 0 && c.end < c.tiles) {
           const int64_t first = c.begin + kPieceUnits, last = first + c.tiles - 1;  // its tiles, as units
-          cut.parts = static_cast<int>(owner(last, ctas, total) - owner(first, ctas, total) + 1);
+          cut.parts = ranges.owner(last) - ranges.owner(first) + 1;
           cut.slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
           cut.rows = min(kItem, rows - c.rg * kItem);
           cut.first_row = c.rg * kItem;
@@ -820,12 +809,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     total += sm.scan[w];
   }
   before -= mine;
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
-  if (blockIdx.x >= ctas) {
+  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+  if (static_cast<int>(blockIdx.x) >= ctas) {
     if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
     return;
   }
-  const int64_t u0 = range_begin(blockIdx.x, ctas, total), u1 = range_begin(blockIdx.x + 1, ctas, total);
+  const Ranges ranges(total, ctas);
+  const int64_t u0 = ranges.begin(blockIdx.x), u1 = ranges.begin(blockIdx.x + 1);
   if (before <= u0 && u0 < before + mine) {
     int64_t at = before;
     int s = s0;
@@ -867,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
   } else   if (warp < kUnpackWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    softmax_role(p, sm, c, ctas, total, warp >> 2, tid);
+    softmax_role(p, sm, c, ranges, warp >> 2, tid);
   } else if (warp < kLoadWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegs));
     unpack_role(p, sm, c, warp - kUnpackWarp, lane);

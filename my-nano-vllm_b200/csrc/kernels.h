@@ -248,6 +248,7 @@ struct Int4AttnParams {
   float scale_log2;  // softmax_scale * log2(e)
   int box_rows;     // rows of a TMA box: the largest of 128, 64, 32 and 16 that divides block_size
   int unit_pages, unit_rest, item_tokens, item_rest, two_tokens, two_heads;  // set by the launch
+  uint32_t group_inverse;  // of 2^31, rounded up; set by the launch
   int* err;         // device error word
   void* cuts;       // workspace: for each CTA the pair that its range leaves cut
   float* partials;  // workspace: two parts for each CTA
