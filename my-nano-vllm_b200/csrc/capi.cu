@@ -1298,6 +1298,10 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   if (rc) return rc;
   rc = make_codes_map(&map_v, v_cache, rows, p.box_rows);
   if (rc) return rc;
+  if (!fp8attn::int4_decode_fits(p.group, plan.short_q, num_seqs, num_kv_heads,
+                                 static_cast<int64_t>(max_num_blocks) * block_size))
+    return fail(FP8ATTN_EINVAL, "%d sequences of %d kv heads with block tables of %d pages are too much for one call",
+                num_seqs, num_kv_heads, max_num_blocks);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // both kernels, then one that joins the parts of what they cut
   auto lists = [](uint8_t* at, int rows, int ctas) {

@@ -2,6 +2,7 @@
 // int4_prefill.cu: many): the work is units of 128 positions in an order, cut into equal ranges, one for each CTA,
 // wherever the cuts fall; the parts of a pair (row group, kv head) that was cut are joined by a kernel of its own.
 #pragma once
+#include <climits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -46,15 +47,16 @@ struct Cut {
 static_assert(sizeof(Cut) == kInt4CutBytes, "as in kernels.h");
 
 // u units in n ranges of equal size, the first u % n of them one longer.
+template <typename T>
 struct Ranges {
-  int64_t each, longer;
-  __device__ __forceinline__ Ranges(int64_t u, int n) {
-    each = u >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(u) / static_cast<uint32_t>(n)) : u / n;
+  T each, longer;
+  __device__ __forceinline__ Ranges(T u, int n) {
+    each = u <= INT_MAX ? static_cast<T>(static_cast<uint32_t>(u) / static_cast<uint32_t>(n)) : u / n;
     longer = u - each * n;
   }
-  __device__ __forceinline__ int64_t begin(int i) const { return i * each + min(static_cast<int64_t>(i), longer); }
-  __device__ __forceinline__ int owner(int64_t x) const {  // range of unit x
-    const int64_t split = longer * (each + 1);
+  __device__ __forceinline__ T begin(int i) const { return i * each + min(static_cast<T>(i), longer); }
+  __device__ __forceinline__ int owner(T x) const {  // range of unit x
+    const T split = longer * (each + 1);
     return static_cast<int>(x < split ? x / (each + 1) : longer + (x - split) / each);
   }
 };

@@ -31,6 +31,7 @@
 // reference maximum and a power of two near the largest step of V are taken out, so it stays below 2^14.
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 #include "int4_attention.cuh"
 
@@ -46,24 +47,22 @@ constexpr int kPitch = 136;             // floats between rows of the sums on th
 constexpr float kSlack = 8.f;           // a reference maximum may lag by 2^8
 constexpr int kPieceUnits = 1;          // what a pair costs beside its tiles, in units of a tile
 
-// How a CTA is made up: computing warps and one that loads.  One plane of query rows: four, and three CTAs on an SM
-// (128 registers).  More planes: eight with 224 registers.
+constexpr int kWarps = 4;                    // that compute; one more loads
+constexpr int kThreads = kWarps * 32 + 32;
+constexpr int kUnit = kTile * kWarps;        // positions per unit
+constexpr int kParts = kUnit / 16;           // parts of a unit that lie in one page each
+
+// A kernel by the rows of a group: NT planes of 8 columns; folded: at most four rows, held twice in the eight columns.
 template <int NT_, bool kFold_>
 struct Shape {
-  static constexpr int NT = NT_;            // planes of 8 columns
-  static constexpr bool kFold = kFold_;     // at most four rows, held twice in the eight columns
-  static constexpr int R = kFold ? 4 : 8 * NT;  // rows of a group
+  static constexpr int NT = NT_;
+  static constexpr bool kFold = kFold_;
+  static constexpr int R = kFold ? 4 : 8 * NT;
   static constexpr bool kWide = NT > 1;
-  static constexpr int kWarps = kWide ? 8 : 4;
-  static constexpr int kThreads = kWarps * 32 + (kWide ? 128 : 32);
-  static constexpr int kCtas = kWide ? 1 : 3;
-  static constexpr int kStages = kWide ? 4 : 3;
-  static constexpr int kUnit = kTile * kWarps;  // positions per unit
-  static constexpr int kParts = kUnit / 16;     // parts of a unit that lie in one page each
+  static constexpr int kCtas = NT < 4 ? 3 : 2;    // on an SM
+  static constexpr int kStages = NT < 3 ? 3 : 2;
+  static constexpr int kRowBuffers = kWide ? 1 : 2;  // of a piece's q as it comes
 };
-
-constexpr int kWideRegs = 216, kLoadRegs = 72;
-static_assert(2 * kWideRegs + kLoadRegs == 3 * 168, "all of the registers of 384 threads, and no more");
 
 // A piece's rows, and where its sums go.
 struct Done {
@@ -72,21 +71,34 @@ struct Done {
   int slot;             // of the partial sums, -1: the piece is a whole pair
 };
 
+// What the warps exchange.  One plane: each has sums of its positions for all values.
+template <int NT>
+struct Exchange {
+  float o[kWarps][8][kPitch];
+  float m[kWarps][8], l[kWarps][8];
+};
+// More: each has sums of all positions for its 32 values, so P goes through shared memory.
+constexpr int kPPitch = kUnit + 8;  // bank spread
+template <int NT>
+struct ExchangeP {
+  uint2 q[NT][8][32];               // B operand of S^T: plane, step, lane
+  uint16_t p[2][8 * NT][kPPitch];   // f16, of this unit and the one before
+  float kq[8 * NT], qs[8 * NT];     // score = dot kq step + qs low
+  float top[kWarps][8 * NT], top_v[kWarps];
+  float l[kWarps][8 * NT], mid[kWarps][8 * NT], ps[kWarps][8 * NT];
+};
+
 template <typename S>
 struct __align__(1024) Smem {
-  uint8_t k[S::kStages][S::kUnit * 64];  // TMA tiles of 64-byte rows, 64B swizzle: bits 1 and 2 of a row's number
-  uint8_t v[S::kStages][S::kUnit * 64];  // change the place of its 16-byte pieces
-  uint2 scale[S::kStages][S::kUnit];
-  uint16_t rows[2][S::R][kHeadDim];      // q of two pieces
-  uint2 q[S::kWide ? S::NT : 1][8][S::kWide ? 32 : 1];  // as the B operand of S^T: plane, step, lane
-  alignas(8) float kq[8 * S::NT], qs[8 * S::NT];  // score = dot kq step + qs low
-  float o[S::kWarps][8][kPitch];         // a plane's sums
-  float m[S::kWarps][8], l[S::kWarps][8];
+  uint8_t k[S::kStages][kUnit * 64];  // TMA tiles of 64-byte rows, 64B swizzle: bits 1 and 2 of a row's number
+  uint8_t v[S::kStages][kUnit * 64];  // change the place of its 16-byte pieces
+  uint2 scale[S::kStages][kUnit];
+  uint16_t rows[S::kRowBuffers][S::R][kHeadDim];  // q
+  std::conditional_t<S::kWide, ExchangeP<S::NT>, Exchange<S::NT>> x;
   uint64_t full[S::kStages], empty[S::kStages], q_full[2], q_free[2], o_full, o_free;
-  uint32_t there[S::kStages];            // which parts of the stage's unit are in pages of the cache
-  int64_t scan[S::kThreads / 32];
-  int64_t first_unit;                    // of the sequence in which the CTA's range begins
-  int first_seq;
+  uint32_t there[S::kStages];  // which parts of the stage's unit are in pages of the cache
+  int scan[kThreads / 32];
+  int first_seq, first_unit;   // the sequence in which the CTA's range begins, its first unit
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -125,12 +137,35 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) 
                : "memory");
 }
 
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// Four 8 x 8 matrices stored transposed: lanes 8 i .. 8 i + 7 give the rows of matrix i in shared memory.
+__device__ __forceinline__ void stmatrix_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+
+// A barrier of the computing warps: whether x holds in any thread.
+__device__ __forceinline__ bool any_warp(bool x) {
+  uint32_t any;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, 1, %2, p;\nselp.u32 %0, 1, 0, q;\n}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(x)), "n"(kWarps * 32)
+      : "memory");
+  return any != 0;
+}
+
 // A sequence's rows and visible positions; units in all.
 struct Seq {
   int q_first, nq, nk, vis, tiles, groups;
-  __device__ __forceinline__ int64_t units(int kvh) const {
-    return static_cast<int64_t>(tiles + kPieceUnits) * groups * kvh;
-  }
+  __device__ __forceinline__ int units(int kvh) const { return (tiles + kPieceUnits) * groups * kvh; }  // launch: < 2^31
 };
 
 template <typename S>
@@ -148,7 +183,7 @@ __device__ __forceinline__ Seq seq_of(const Int4AttnParams& p, int s) {
   }
   q.vis = max(0, min(q.nk, p.max_blocks * p.block_size));
   // a sequence without positions still has its zeros written
-  q.tiles = max(1, (q.vis + S::kUnit - 1) / S::kUnit);
+  q.tiles = max(1, (q.vis + kUnit - 1) / kUnit);
   q.groups = q.nq <= 0 ? 0 : (q.nq * p.group + S::R - 1) / S::R;
   return q;
 }
@@ -160,12 +195,12 @@ __device__ __forceinline__ int token_of(const Int4AttnParams& p, int r) { return
 // it costs beside its tiles, and then its tiles; a piece is what of it lies in the CTA's range, which ends at unit `until`.
 struct Cursor {
   int seq, rg, kvh, tile, end;
-  int64_t begin, until;  // the pair's first unit
+  int begin, until;  // the pair's first unit
   Seq s;
   // Whether another piece with a tile follows.
   __device__ __forceinline__ bool more() const { return begin + s.tiles + 2 * kPieceUnits < until; }
   __device__ __forceinline__ void set_end() {
-    end = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(s.tiles), until - begin - kPieceUnits)));
+    end = max(0, min(s.tiles, until - begin - kPieceUnits));
   }
 };
 
@@ -227,33 +262,32 @@ __device__ __forceinline__ void convert_q(const uint16_t* row, bool is_row, int 
   qs = sum * scale_log2;
 }
 
-// This warp's share of a plane's rows, the warps' sums joined: outputs of a whole pair, or a part for the joining kernel.
+// This warp's share of the rows, the warps' sums joined: outputs of a whole pair, or a part for the joining kernel.
 template <typename S>
-__device__ __forceinline__ void merge_plane(const Int4AttnParams& p, const Smem<S>& sm, const Done& d, int j, int warp,
-                                            int lane) {
+__device__ __forceinline__ void merge(const Int4AttnParams& p, const Smem<S>& sm, const Done& d, int warp, int lane) {
   constexpr int kRows = S::kFold ? 4 : 8, kFrom = S::kFold ? 2 : 1;
 #pragma unroll 1
-  for (int row = warp; row < kRows; row += S::kWarps) {
-    const int in_group = 8 * j + row, r = d.first_row + in_group;
+  for (int row = warp; row < kRows; row += kWarps) {
+    const int r = d.first_row + row;
     if (r >= d.rows) break;
     float mx = kNone;
 #pragma unroll
-    for (int w = 0; w < S::kWarps; ++w)
+    for (int w = 0; w < kWarps; ++w)
 #pragma unroll
-      for (int f = 0; f < kFrom; ++f) mx = fmaxf(mx, sm.m[w][row + 4 * f]);
+      for (int f = 0; f < kFrom; ++f) mx = fmaxf(mx, sm.x.m[w][row + 4 * f]);
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < S::kWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
 #pragma unroll
       for (int f = 0; f < kFrom; ++f) {
-        const float weight = ex2(sm.m[w][row + 4 * f] - mx);
-        const float4 x = *reinterpret_cast<const float4*>(&sm.o[w][row + 4 * f][4 * lane]);
+        const float weight = ex2(sm.x.m[w][row + 4 * f] - mx);
+        const float4 x = *reinterpret_cast<const float4*>(&sm.x.o[w][row + 4 * f][4 * lane]);
         y.x = fmaf(x.x, weight, y.x);
         y.y = fmaf(x.y, weight, y.y);
         y.z = fmaf(x.z, weight, y.z);
         y.w = fmaf(x.w, weight, y.w);
-        sum = fmaf(sm.l[w][row + 4 * f], weight, sum);
+        sum = fmaf(sm.x.l[w][row + 4 * f], weight, sum);
       }
     }
     if (d.slot < 0) {
@@ -265,8 +299,8 @@ __device__ __forceinline__ void merge_plane(const Int4AttnParams& p, const Smem<
           make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     } else {
       float* const part = p.partials + static_cast<int64_t>(d.slot) * (S::R * (kHeadDim + 2));
-      *reinterpret_cast<float4*>(part + in_group * kHeadDim + 4 * lane) = y;
-      if (lane == 0) *reinterpret_cast<float2*>(part + S::R * kHeadDim + 2 * in_group) = make_float2(mx, sum);
+      *reinterpret_cast<float4*>(part + row * kHeadDim + 4 * lane) = y;
+      if (lane == 0) *reinterpret_cast<float2*>(part + S::R * kHeadDim + 2 * row) = make_float2(mx, sum);
     }
   }
 }
@@ -278,18 +312,18 @@ __device__ __forceinline__ void load(const Int4AttnParams& p, const CUtensorMap&
                                      Smem<S>& sm, Cursor c, int lane) {
   int column = 0, place = 0, page = -1, stage = 0;
   uint32_t round = 0, loaded = 0, pieces = 0;
-  const bool begins = lane < S::kParts && lane % (p.box_rows / 16) == 0;
+  const bool begins = lane < kParts && lane % (p.box_rows / 16) == 0;
   bool ok = true, first = true;  // the unit is its piece's first
   auto look_up = [&]() {
-    const int pos = c.tile * S::kUnit + lane * 16;
+    const int pos = c.tile * kUnit + lane * 16;
     page = -1;
-    if (lane < S::kParts && pos < c.s.vis) {
+    if (lane < kParts && pos < c.s.vis) {
       const int found = ldg_keep(p.block_tables + c.seq * p.bt_stride + column);
       if (found >= 0 && found < p.num_blocks) page = found;
     }
   };
   auto find = [&]() {
-    const int pos = c.tile * S::kUnit + lane * 16;
+    const int pos = c.tile * kUnit + lane * 16;
     column = pos / p.block_size;
     place = pos - column * p.block_size;
     look_up();
@@ -298,8 +332,8 @@ __device__ __forceinline__ void load(const Int4AttnParams& p, const CUtensorMap&
 #pragma unroll 1
   for (;;) {
     if (first) {
-      const int b = pieces & 1, rows = c.s.nq * p.group - c.rg * S::R;  // from the group's first on
-      if (pieces > 1) ok = wait_all(&sm.q_free[b], ((pieces >> 1) - 1) & 1u, p.err);
+      const int b = pieces % S::kRowBuffers, rows = c.s.nq * p.group - c.rg * S::R;  // from the group's first on
+      if (pieces >= S::kRowBuffers) ok = wait_all(&sm.q_free[b], (pieces / S::kRowBuffers - 1) & 1u, p.err);
       if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(&sm.q_full[b], min(S::R, rows) * kHeadDim * 2);
       __syncwarp();
@@ -357,11 +391,28 @@ __device__ __forceinline__ void load(const Int4AttnParams& p, const CUtensorMap&
   // a wait gave up: the copies in flight must land (or run out of time) before the CTA ends
   for (int i = 0; i < S::kStages; ++i)
     if (loaded >> i & 1u) wait_all(&sm.full[i], (i < stage ? round : round - 1) & 1u, p.err);
-  for (uint32_t i = pieces > 2 ? pieces - 2 : 0; i < pieces; ++i) wait_all(&sm.q_full[i & 1], (i >> 1) & 1u, p.err);
+  for (uint32_t i = pieces > S::kRowBuffers ? pieces - S::kRowBuffers : 0; i < pieces; ++i)
+    wait_all(&sm.q_full[i % S::kRowBuffers], (i / S::kRowBuffers) & 1u, p.err);
+}
+
+// The pair that the CTA's range leaves cut, if its last piece is one's beginning: for the joining kernel.
+template <typename S>
+__device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor& now, const Ranges<int>& ranges, uint32_t pieces) {
+  Cut cut = {};
+  if (now.tile == 0 && now.end < now.s.tiles) {
+    const int first = now.begin + kPieceUnits, last = first + now.s.tiles - 1;  // its tiles, as units
+    cut.parts = ranges.owner(last) - ranges.owner(first) + 1;
+    cut.slot = 2 * blockIdx.x + (pieces > 0 ? 1 : 0);
+    cut.rows = min(S::R, now.s.nq * p.group - now.rg * S::R);
+    cut.first_row = now.rg * S::R;
+    cut.token = now.s.q_first;
+    cut.head = now.kvh * p.group;
+  }
+  reinterpret_cast<Cut*>(p.cuts)[blockIdx.x] = cut;
 }
 
 template <typename S>
-__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges& ranges, int warp,
+__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges<int>& ranges, int warp,
                                         int lane) {
   constexpr int NT = S::NT, R = S::R;
   constexpr bool kFold = S::kFold;
@@ -377,10 +428,9 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
   uint32_t parity = 0, pieces = 0;
   bool ok = true;  // no wait has given up
   Done done = {};  // the piece before
-  auto all_warps = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(S::kWarps * 32) : "memory"); };
-  auto merge_last = [&](int j) {  // one plane: a warp joins its rows of the piece before when it has begun the next
+  auto merge_last = [&]() {  // a warp joins its rows of the piece before when it has begun the next
     ok = ok && wait_all(&sm.o_full, (pieces - 1) & 1u, p.err);
-    if (ok) merge_plane(p, sm, done, j, warp, lane);
+    if (ok) merge(p, sm, done, warp, lane);
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.o_free);
   };
@@ -390,45 +440,17 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
     const int rows = now.s.nq * p.group;  // of this kv head
     const int buf = pieces & 1;
     ok = ok && wait_all(&sm.q_full[buf], (pieces >> 1) & 1u, p.err);
-    constexpr bool kHeld = NT <= 2;  // q stays in registers; else it is read from shared memory for each tile
-    uint2 q[kHeld ? NT : 1][8];
-    [[maybe_unused]] uint64_t kq[NT], qs[NT];  // for this thread's columns 2 t and 2 t + 1; wide: in shared memory
-    if constexpr (!S::kWide) {
+    uint2 q[NT][8];
+    uint64_t kq[NT], qs[NT];  // for this thread's columns 2 t and 2 t + 1
+    {
       const int in_group = kFold ? g & 3 : g;
       float a, b;
       convert_q(sm.rows[buf][in_group], rg * R + in_group < rows, t, p.scale_log2, q[0], a, b);
       kq[0] = f2_pack(__shfl_sync(0xffffffffu, a, 8 * t), __shfl_sync(0xffffffffu, a, 8 * t + 4));
       qs[0] = f2_pack(__shfl_sync(0xffffffffu, b, 8 * t), __shfl_sync(0xffffffffu, b, 8 * t + 4));
-      if (lane == 0) mbar_arrive(&sm.q_free[buf]);
-      if (pieces > 0) merge_last(0);
-    } else {
-      if (warp < NT) {
-        uint2 y[8];
-        float a, b;
-        convert_q(sm.rows[buf][8 * warp + g], rg * R + 8 * warp + g < rows, t, p.scale_log2, y, a, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sm.q[warp][i][lane] = y[i];
-        if (t == 0) {
-          sm.kq[8 * warp + g] = a;
-          sm.qs[8 * warp + g] = b;
-        }
-      }
-      all_warps();
-      if (lane == 0) mbar_arrive(&sm.q_free[buf]);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int i = 0; i < 8 && kHeld; ++i) q[kHeld ? j : 0][i] = sm.q[j][i][lane];
-      }
     }
-    auto kq_of = [&](int j) {
-      if constexpr (S::kWide) return reinterpret_cast<const uint64_t*>(sm.kq)[4 * j + t];
-      else return kq[j];
-    };
-    auto qs_of = [&](int j) {
-      if constexpr (S::kWide) return reinterpret_cast<const uint64_t*>(sm.qs)[4 * j + t];
-      else return qs[j];
-    };
+    if (lane == 0) mbar_arrive(&sm.q_free[buf]);
+    if (pieces > 0) merge_last();
     int least = INT_MAX, most = 0;
     auto limit_of = [&](int j, int c) {  // positions that a column's row sees; where there is no row, as the group's first
       int row = rg * R + (kFold ? (2 * t + c) & 3 : 8 * j + 2 * t + c);
@@ -469,7 +491,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
 
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      const int pos0 = (now.tile + i) * S::kUnit + warp * kTile;
+      const int pos0 = (now.tile + i) * kUnit + warp * kTile;
       ok = ok && wait_all(&sm.full[stage], parity, p.err);
       const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
       if (halves != 0 && pos0 < most && ok) {
@@ -480,7 +502,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint4 k = ld_shared_v4(k_ring + stage * (S::kUnit * 64) + h * 1024 + r * 512);
+            const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
             kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
           }
         }
@@ -500,7 +522,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const uint2 qb = kHeld ? q[kHeld ? j : 0][2 * w + b] : sm.q[kHeld ? 0 : j][2 * w + b][lane];
+              const uint2 qb = q[j][2 * w + b];
               if (w == 0 && b == 0) {
                 mma16816_first(s[0][j], a[0], qb.x, qb.y);
                 mma16816_first(s[1][j], a[1], qb.x, qb.y);
@@ -527,15 +549,15 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
           const int half = kFold ? t >> 1 : h;
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint2 sc = ld_shared_v2(s_ring + stage * (S::kUnit * 8) + half * 128 + r * 64);
+            const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + half * 128 + r * 64);
             const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
             sv[h][r] = __uint_as_float(sc.y << 16);
             mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
             const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq_of(j)),
-                                        f2_fma(lk2, qs_of(j), minus_m[j]));
+              const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq[j]),
+                                        f2_fma(lk2, qs[j], minus_m[j]));
               f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
             }
           }
@@ -554,12 +576,17 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
             for (int r = 0; r < 2; ++r) {
               const int pos = pos0 + 16 * half + g + 8 * r;
               const bool held = (halves >> half & 1u) && pos < now.s.vis;
-              if (!held) sv[h][r] = mv[h][r] = 0.f;
+              // a row of V that is no number goes to those that see it by their scores
+              const bool number = fabsf(mv[h][r]) < INFINITY;
+              if (!held || !number) sv[h][r] = mv[h][r] = 0.f;
 #pragma unroll
-              for (int j = 0; j < NT; ++j)
+              for (int j = 0; j < NT; ++j) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+                for (int c = 0; c < 2; ++c) {
+                  if (!number) s[h][j][2 * r + c] = NAN;
                   if (!held || pos >= sees[j][c]) s[h][j][2 * r + c] = -INFINITY;
+                }
+              }
             }
           }
         }
@@ -662,7 +689,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
 #pragma unroll
           for (int w = 0; w < 4; w += 2) {
             uint32_t v[4];  // piece w: rows 0-7 and 8-15, piece w + 1: the same
-            ldmatrix_trans(v, v_ring + stage * (S::kUnit * 64) + h * 1024 + (w ^ v_piece) * 16);
+            ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + h * 1024 + (w ^ v_piece) * 16);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
 #pragma unroll
@@ -689,7 +716,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
     const bool whole = now.tile == 0 && now.end == now.s.tiles;
     done = {rg * R, rows, now.s.q_first, kvh * p.group, whole ? -1 : 2 * static_cast<int>(blockIdx.x) + (pieces > 0 ? 1 : 0)};
     const float unit_even = 16777216.f, unit_odd = 1048576.f, back = pow2(v_exp);
-    if (!S::kWide && pieces > 0) ok = ok && wait_all(&sm.o_free, (pieces - 1) & 1u, p.err);
+    if (pieces > 0) ok = ok && wait_all(&sm.o_free, (pieces - 1) & 1u, p.err);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float m[2], sum[2], middle[2];
@@ -704,53 +731,391 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
           middle[c] += __shfl_xor_sync(0xffffffffu, middle[c], off);
         }
         if (g == 0) {
-          sm.m[warp][2 * t + c] = unset >> (2 * j + c) & 1u ? kNone : -m[c];
-          sm.l[warp][2 * t + c] = sum[c];
+          sm.x.m[warp][2 * t + c] = unset >> (2 * j + c) & 1u ? kNone : -m[c];
+          sm.x.l[warp][2 * t + c] = sum[c];
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // values 32 (i >> 1) + 4 g + 2 (i & 1) and the one after it
           const float y0 = fmaf(fmaf(o[j][i][c], unit_even, -7.5f * ps[j][c]), back, middle[c]);
           const float y1 = fmaf(fmaf(o[j][i][2 + c], unit_odd, -7.5f * ps[j][c]), back, middle[c]);
-          *reinterpret_cast<float2*>(&sm.o[warp][2 * t + c][32 * (i >> 1) + 4 * g + 2 * (i & 1)]) = make_float2(y0, y1);
+          *reinterpret_cast<float2*>(&sm.x.o[warp][2 * t + c][32 * (i >> 1) + 4 * g + 2 * (i & 1)]) = make_float2(y0, y1);
         }
       }
-      if constexpr (S::kWide) {
-        all_warps();
-        if (ok) merge_plane(p, sm, done, j, warp, lane);
-        all_warps();
-      }
     }
-    if constexpr (!S::kWide) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.o_full);
-    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.o_full);
     // ---- on to the next pair
     if (!now.more()) {
-      if (warp == 0 && lane == 0) {
-        Cut cut = {};
-        if (now.tile == 0 && now.end < now.s.tiles) {
-          const int64_t first = now.begin + kPieceUnits, last = first + now.s.tiles - 1;  // its tiles, as units
-          cut.parts = ranges.owner(last) - ranges.owner(first) + 1;
-          cut.slot = 2 * blockIdx.x + (pieces > 0 ? 1 : 0);
-          cut.rows = min(R, rows - rg * R);
-          cut.first_row = rg * R;
-          cut.token = now.s.q_first;
-          cut.head = kvh * p.group;
-        }
-        reinterpret_cast<Cut*>(p.cuts)[blockIdx.x] = cut;
-      }
+      if (warp == 0 && lane == 0) store_cut<S>(p, now, ranges, pieces);
       break;
     }
     next_piece<S>(p, now);
   }
-  if constexpr (!S::kWide) {
-    ++pieces;
-    merge_last(0);
+  ++pieces;
+  merge_last();
+}
+
+// More than one plane.  Sums of 128 values for every row would take 32 registers a plane, and two warps on a scheduler
+// do not hide the tensor cores' latency; so a warp computes S and P of its 32 positions, and of all 128 positions the
+// products with its 32 values.  P goes through shared memory (stmatrix turns it), the references are the CTA's.
+template <typename S>
+__device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges<int>& ranges,
+                                             int warp, int lane) {
+  constexpr int NT = S::NT, R = S::R;
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t k_ring = smem_u32(sm.k[0]) + (warp * kTile + g) * 64 + (t ^ (g >> 1 & 3)) * 16;
+  const uint32_t v_ring = smem_u32(sm.v[0]) + lane * 64 + (warp ^ (lane >> 1 & 3)) * 16;
+  const uint32_t s_ring = smem_u32(sm.scale[0]) + (warp * kTile + g) * 8;
+  const uint32_t p_lane = smem_u32(sm.x.p[0]) + ((lane & 7) * kPPitch + (lane >> 3) * 8) * 2;  // row of a plane, 8 positions
+  auto all_warps = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); };
+  int stage = 0;
+  uint32_t parity = 0, pieces = 0, p_buf = 0;
+  bool ok = true;  // no wait has given up
+#pragma unroll 1
+  for (;; ++pieces) {
+    const int n = now.end - now.tile, kvh = now.kvh, rg = now.rg;
+    const int rows = now.s.nq * p.group;  // of this kv head
+    ok = ok && wait_all(&sm.q_full[0], pieces & 1u, p.err);
+    if (warp < NT) {
+      uint2 y[8];
+      float a, b;
+      convert_q(sm.rows[0][8 * warp + g], rg * R + 8 * warp + g < rows, t, p.scale_log2, y, a, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sm.x.q[warp][i][lane] = y[i];
+      if (t == 0) {
+        sm.x.kq[8 * warp + g] = a;
+        sm.x.qs[8 * warp + g] = b;
+      }
+    }
+    all_warps();
+    if (lane == 0) mbar_arrive(&sm.q_free[0]);
+    auto limit_of = [&](int j, int c) {  // positions that a column's row sees; where there is no row, as the group's first
+      int row = rg * R + 8 * j + 2 * t + c;
+      if (row >= rows) row = rg * R;
+      return min(now.s.vis, token_of(p, row) + now.s.nk - now.s.nq + 1);
+    };
+    int least = INT_MAX;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) least = min(least, min(limit_of(j, 0), limit_of(j, 1)));
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
+
+    float o[NT][2][4], ps[NT][4];          // ps: sum of the rounded P step, of this warp's positions
+    uint64_t minus_m[NT], l[NT], mid[NT];  // pairs of columns
+    uint32_t unset = (1u << 2 * NT) - 1;   // columns that have seen nothing: their m counts as 0
+    float limit = -INFINITY;               // how far a score may be above its m: kSlack when none is unset
+    float v_unit = 1.f, v_limit = 0.f;     // steps of V are multiplied by v_unit (a power of two)
+    int v_exp = 0;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      minus_m[j] = l[j] = mid[j] = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ps[j][c] = o[j][0][c] = o[j][1][c] = 0.f;
+    }
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int pos0 = (now.tile + i) * kUnit + warp * kTile;
+      ok = ok && wait_all(&sm.full[stage], parity, p.err);
+      const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
+      // ---- S^T: positions (rows g, g + 8 of each half) x query rows (columns)
+      float s[2][NT][4];
+      uint32_t kw[2][2][4];  // half, row g or g + 8, word
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
+          kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t a[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t y0 = kw[h][0][w] >> (8 * b);
+            const uint32_t y1 = kw[h][1][w] >> (8 * b);
+            a[h][0] = y0 & 0x000F000Fu;
+            a[h][1] = y1 & 0x000F000Fu;
+            a[h][2] = y0 & 0x00F000F0u;
+            a[h][3] = y1 & 0x00F000F0u;
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint2 q = sm.x.q[j][2 * w + b][lane];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (w == 0 && b == 0) mma16816_first(s[h][j], a[h], q.x, q.y);
+              else mma16816(s[h][j], a[h], q.x, q.y);
+            }
+          }
+        }
+      }
+      // ---- scores above their m; this thread's positions: rows g and g + 8 of half h
+      float sv[2][2], mv[2][2];  // step of V, and what code 7.5 stands for
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + h * 128 + r * 64);
+          const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
+          sv[h][r] = __uint_as_float(sc.y << 16);
+          mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
+          const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint64_t kq = reinterpret_cast<const uint64_t*>(sm.x.kq)[4 * j + t];
+            const uint64_t qs = reinterpret_cast<const uint64_t*>(sm.x.qs)[4 * j + t];
+            const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq), f2_fma(lk2, qs, minus_m[j]));
+            f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
+          }
+        }
+      }
+      if (halves != 3u || pos0 + kTile > least) {
+        int sees[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          sees[j][0] = limit_of(j, 0);
+          sees[j][1] = limit_of(j, 1);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int pos = pos0 + 16 * h + g + 8 * r;
+            const bool held = (halves >> h & 1u) && pos < now.s.vis;
+            // a row of V that is no number goes to those that see it by their scores
+            const bool number = fabsf(mv[h][r]) < INFINITY;
+            if (!held || !number) sv[h][r] = mv[h][r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                if (!number) s[h][j][2 * r + c] = NAN;
+                if (!held || pos >= sees[j][c]) s[h][j][2 * r + c] = -INFINITY;
+              }
+            }
+          }
+        }
+      }
+      bool grow = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        grow |= fmaxf(sv[h][0], sv[h][1]) > v_limit;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          grow |= fmaxf(fmaxf(s[h][j][0], s[h][j][1]), fmaxf(s[h][j][2], s[h][j][3])) > limit;
+      }
+      // ---- P, and P step_v to shared memory: [row][position]
+      const uint32_t p_at = p_lane + p_buf * (R * kPPitch * 2);
+      float e[2][NT][4];
+      auto give_p = [&]() {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint32_t x[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              e[h][j][2 * r] = ex2(s[h][j][2 * r]);
+              e[h][j][2 * r + 1] = ex2(s[h][j][2 * r + 1]);
+              const float f = sv[h][r] * v_unit;
+              x[h][r] = pack_f16x2(e[h][j][2 * r] * f, e[h][j][2 * r + 1] * f);
+            }
+          }
+          stmatrix_trans(p_at + (8 * j * kPPitch + warp * kTile) * 2, x[0][0], x[0][1], x[1][0], x[1][1]);
+        }
+      };
+      give_p();
+      if (any_warp(grow)) {
+        // ---- new references, of the CTA: the rows' maxima so far, and a power of two near V's largest step
+        float top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (lane == 0) sm.x.top_v[warp] = top;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(fmaxf(s[0][j][c], s[0][j][2 + c]), fmaxf(s[1][j][c], s[1][j][2 + c]));
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            if (g == 0) sm.x.top[warp][8 * j + 2 * t + c] = mx;
+          }
+        }
+        all_warps();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.x.top_v[w]);
+        float change = 1.f;
+        if (top > v_limit && top < INFINITY) {
+          const int x = max(-120, min(exponent(top), 120));
+          if (v_limit > 0.f) {
+            const int d = v_exp - x;
+            change = d < -126 ? 0.f : pow2(d);
+          }
+          v_exp = x;
+          v_unit = pow2(-x);
+          v_limit = pow2(min(x + 6, 127));
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float was[2], now_m[2], f[2];
+          f2_unpack(minus_m[j], was[0], was[1]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float mx = -INFINITY;  // above m
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.x.top[w][8 * j + 2 * t + c]);
+            const bool first = unset >> (2 * j + c) & 1u;
+            if (first && mx == -INFINITY) mx = 0.f;  // still unset
+            else unset &= ~(1u << (2 * j + c));
+            if (!first) mx = fmaxf(mx, 0.f);
+            f[c] = first ? 0.f : ex2(-mx);
+            now_m[c] = was[c] - mx;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[h][j][c] -= mx;
+              s[h][j][2 + c] -= mx;
+            }
+            ps[j][c] *= f[c] * change;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              o[j][b][c] *= f[c] * change;
+              o[j][b][2 + c] *= f[c] * change;
+            }
+          }
+          minus_m[j] = f2_pack(now_m[0], now_m[1]);
+          l[j] = f2_mul(l[j], f2_pack(f[0], f[1]));
+          mid[j] = f2_mul(mid[j], f2_pack(f[0], f[1]));
+        }
+        limit = __any_sync(0xffffffffu, unset != 0) ? -INFINITY : kSlack;
+        give_p();
+        all_warps();
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint64_t mv2 = f2_pack(mv[h][r], mv[h][r]);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint64_t x = f2_pack(e[h][j][2 * r], e[h][j][2 * r + 1]);
+            l[j] = f2_add(l[j], x);
+            mid[j] = f2_fma(x, mv2, mid[j]);
+          }
+        }
+      }
+      // ---- sums of P step_v: of this warp's positions
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        constexpr uint32_t kOne = 0x3C003C00u;
+        const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+        uint32_t b[4];
+        ldmatrix(b, p_at + (8 * j * kPPitch + warp * kTile) * 2);
+        mma16816(ps[j], ones, b[0], b[1]);
+        mma16816(ps[j], ones, b[2], b[3]);
+      }
+      // ---- O^T += V^T P^T: of its 32 values 4 g + 2 b (rows g) and 4 g + 2 b + 1 (rows g + 8, codes four bits higher)
+#pragma unroll
+      for (int x = 0; x < kUnit / 32; ++x) {
+        uint32_t v[4], pb[NT][4];  // of 8 positions each
+        ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + x * 2048);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) ldmatrix(pb[j], p_at + (8 * j * kPPitch + x * 32) * 2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t y0 = v[2 * h] >> (8 * b), y1 = v[2 * h + 1] >> (8 * b);
+            const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma16816(o[j][b], a, pb[j][2 * h], pb[j][2 * h + 1]);
+          }
+        }
+      }
+      p_buf ^= 1u;
+      __syncwarp();  // every lane has read the stage
+      if (lane == 0) mbar_arrive(&sm.empty[stage]);
+      if (++stage == S::kStages) {
+        stage = 0;
+        parity ^= 1u;
+      }
+    }
+
+    // ---- the rows' sums over the warps' positions, and outputs of a whole pair or a part for the joining kernel
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float sum[2], middle[2];
+      f2_unpack(l[j], sum[0], sum[1]);
+      f2_unpack(mid[j], middle[0], middle[1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], off);
+          middle[c] += __shfl_xor_sync(0xffffffffu, middle[c], off);
+        }
+        if (g == 0) {
+          sm.x.l[warp][8 * j + 2 * t + c] = sum[c];
+          sm.x.mid[warp][8 * j + 2 * t + c] = middle[c];
+          sm.x.ps[warp][8 * j + 2 * t + c] = ps[j][c];
+        }
+      }
+    }
+    all_warps();
+    const bool whole = now.tile == 0 && now.end == now.s.tiles;
+    const float unit_even = 16777216.f, unit_odd = 1048576.f, back = pow2(v_exp);
+    float* const part = p.partials + static_cast<int64_t>(2 * blockIdx.x + (pieces > 0 ? 1 : 0)) * (R * (kHeadDim + 2));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float m[2];
+      f2_unpack(minus_m[j], m[0], m[1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int column = 8 * j + 2 * t + c, r = rg * R + column;
+        float sum = 0.f, middle = 0.f, steps = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          sum += sm.x.l[w][column];
+          middle += sm.x.mid[w][column];
+          steps += sm.x.ps[w][column];
+        }
+        float y[4];  // values 4 g .. 4 g + 3 of the warp's
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          y[2 * b] = fmaf(fmaf(o[j][b][c], unit_even, -7.5f * steps), back, middle);
+          y[2 * b + 1] = fmaf(fmaf(o[j][b][2 + c], unit_odd, -7.5f * steps), back, middle);
+        }
+        if (r >= rows || !ok) continue;
+        const int value = 32 * warp + 4 * g;
+        if (whole) {
+          const int token = token_of(p, r);
+          const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);  // 0 for a row that sees nothing
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0] * inv, y[1] * inv), hi = __floats2bfloat162_rn(y[2] * inv, y[3] * inv);
+          *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(now.s.q_first) + token) * p.out_row_stride +
+                                    (kvh * p.group + r - token * p.group) * kHeadDim + value) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else {
+          *reinterpret_cast<float4*>(part + column * kHeadDim + value) = make_float4(y[0], y[1], y[2], y[3]);
+          if (warp == 0 && g == 0)
+            *reinterpret_cast<float2*>(part + R * kHeadDim + 2 * column) =
+                make_float2(unset >> (2 * j + c) & 1u ? kNone : -m[c], sum);
+        }
+      }
+    }
+    // ---- on to the next pair
+    if (!now.more()) {
+      if (warp == 0 && lane == 0) store_cut<S>(p, now, ranges, pieces);
+      return;
+    }
+    next_piece<S>(p, now);
   }
 }
 
 template <typename S>
-__global__ void __launch_bounds__(S::kThreads, S::kCtas)
+__global__ void __launch_bounds__(kThreads, S::kCtas)
     int4_decode_kernel(const __grid_constant__ Int4AttnParams p, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v) {
   extern __shared__ uint8_t smem_raw[];
@@ -760,15 +1125,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
 #pragma unroll
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], S::kWarps);
+      mbar_init(&sm.empty[i], kWarps);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.q_full[i], 1);
-      mbar_init(&sm.q_free[i], S::kWarps);
+      mbar_init(&sm.q_free[i], kWarps);
     }
-    mbar_init(&sm.o_full, S::kWarps);
-    mbar_init(&sm.o_free, S::kWarps);
+    mbar_init(&sm.o_full, kWarps);
+    mbar_init(&sm.o_free, kWarps);
     fence_mbar_init();
   }
   // programmatic dependent of the kernel before it: nothing is read or written before that ends
@@ -776,38 +1141,38 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- plan: units before each sequence; thread i has sequences [i * per, (i + 1) * per)
-  const int per = (p.num_seqs + S::kThreads - 1) / S::kThreads;
+  const int per = (p.num_seqs + kThreads - 1) / kThreads;
   const int s0 = min(tid * per, p.num_seqs), s1 = min(s0 + per, p.num_seqs);
-  int64_t mine = 0;
+  int mine = 0;
   for (int s = s0; s < s1; ++s) mine += seq_of<S>(p, s).units(p.num_kv_heads);
-  int64_t before = mine;
+  int before = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, before, off);
+    const int v = __shfl_up_sync(0xffffffffu, before, off);
     if (lane >= off) before += v;
   }
   if (lane == 31) sm.scan[warp] = before;
   __syncthreads();
-  int64_t total = 0;
+  int total = 0;
 #pragma unroll
-  for (int w = 0; w < S::kThreads / 32; ++w) {
+  for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += sm.scan[w];
     total += sm.scan[w];
   }
   before -= mine;
-  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+  const int ctas = min(static_cast<int>(gridDim.x), total);
   Cut* cuts = reinterpret_cast<Cut*>(p.cuts);
   if (static_cast<int>(blockIdx.x) >= ctas) {
     if (tid == 0) cuts[blockIdx.x].parts = 0;
     return;
   }
-  const Ranges ranges(total, ctas);
-  const int64_t u0 = ranges.begin(blockIdx.x);
+  const Ranges<int> ranges(total, ctas);
+  const int u0 = ranges.begin(blockIdx.x);
   if (before <= u0 && u0 < before + mine) {
-    int64_t at = before;
+    int at = before;
     int s = s0;
     for (; s < s1; ++s) {
-      const int64_t n = seq_of<S>(p, s).units(p.num_kv_heads);
+      const int n = seq_of<S>(p, s).units(p.num_kv_heads);
       if (u0 < at + n) break;
       at += n;
     }
@@ -819,14 +1184,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
   c.seq = sm.first_seq;
   c.s = seq_of<S>(p, c.seq);
   {
-    const int64_t rest = u0 - sm.first_unit;
+    const int rest = u0 - sm.first_unit;
     const int each = c.s.tiles + kPieceUnits;
-    const int pair = rest >> 32 == 0 ? static_cast<int>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(each))
-                                     : static_cast<int>(rest / each);
-    c.begin = sm.first_unit + static_cast<int64_t>(pair) * each;
+    const int pair = rest / each;
+    c.begin = sm.first_unit + pair * each;
     c.rg = pair / p.num_kv_heads;
     c.kvh = pair - c.rg * p.num_kv_heads;
-    c.tile = max(0, static_cast<int>(u0 - c.begin) - kPieceUnits);
+    c.tile = max(0, u0 - c.begin - kPieceUnits);
     c.until = ranges.begin(blockIdx.x + 1);
     c.set_end();
   }
@@ -834,12 +1198,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kCtas)
     if (tid == 0) cuts[blockIdx.x].parts = 0;
     return;
   }
-  if (warp < S::kWarps) {
-    if constexpr (S::kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegs));
-    compute<S>(p, sm, c, ranges, warp, lane);
+  if (warp == kWarps) {
+    load<S>(p, map_k, map_v, sm, c, lane);
+  } else if constexpr (S::kWide) {
+    compute_wide<S>(p, sm, c, ranges, warp, lane);
   } else {
-    if constexpr (S::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
-    if (warp == S::kWarps) load<S>(p, map_k, map_v, sm, c, lane);
+    compute<S>(p, sm, c, ranges, warp, lane);
   }
 }
 
@@ -856,7 +1220,7 @@ template <typename S>
 int resident(int num_sms) {  // CTAs that run at once
   int per_sm = 0;
   if (prepare<S>() != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int4_decode_kernel<S>, S::kThreads, kSmemBytes<S>) !=
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int4_decode_kernel<S>, kThreads, kSmemBytes<S>) !=
           cudaSuccess)
     return 0;
   return per_sm * num_sms;
@@ -866,15 +1230,15 @@ template <typename S>
 cudaError_t launch(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid, cudaStream_t stream) {
   cudaError_t e = prepare<S>();
   if (e != cudaSuccess) return e;
-  p.unit_pages = S::kUnit / p.block_size;
-  p.unit_rest = S::kUnit % p.block_size;
+  p.unit_pages = kUnit / p.block_size;
+  p.unit_rest = kUnit % p.block_size;
   p.group_inverse = static_cast<uint32_t>(((int64_t{1} << 31) + p.group - 1) / p.group);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(S::kThreads);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemBytes<S>;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -911,6 +1275,13 @@ int int4_decode_grid(int group, int max_q) {
     known[dev][v].store(n, std::memory_order_relaxed);
   }
   return n;
+}
+
+bool int4_decode_fits(int group, int max_q, int num_seqs, int num_kv_heads, int64_t longest) {
+  const int rows = rows_of(variant(group, max_q));
+  const int64_t groups = (static_cast<int64_t>(group) * max_q + rows - 1) / rows;
+  const int64_t each = (longest / kUnit + 1 + kPieceUnits) * groups * num_kv_heads;  // of a sequence, at most
+  return each < INT_MAX && each * num_seqs < INT_MAX;
 }
 
 int64_t int4_decode_workspace_bytes(int group, int max_q, int grid) {

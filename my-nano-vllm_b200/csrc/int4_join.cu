@@ -10,7 +10,8 @@
 namespace fp8attn {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
+constexpr int kAtOnce = 8;  // parts of which a warp has the loads in flight
 
 __device__ __forceinline__ void add_part(float4& y, float& sum, const float4& x, float l, float f) {
   y.x = fmaf(x.x, f, y.x);
@@ -50,16 +51,30 @@ __device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4Join
     const bool mine = warp < at_once * share && row < cut.rows;
     float mx = kNone, sum = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (mine) {
-      for (int j = turn + lane * share; j < parts; j += 32 * share) mx = fmaxf(mx, part(j)[ml_at + 2 * row]);
+    for (int j0 = turn; mine && j0 < parts; j0 += kAtOnce * share) {
+      float2 ml[kAtOnce];
+      float4 x[kAtOnce];
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-#pragma unroll 8
-      for (int j = turn; j < parts; j += share) {
-        const float2 ml = *reinterpret_cast<const float2*>(part(j) + ml_at + 2 * row);
-        const float4 x = *reinterpret_cast<const float4*>(part(j) + row * kHeadDim + 4 * lane);
-        add_part(y, sum, x, ml.y, ex2(ml.x - mx));
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + i * share;
+        ml[i] = make_float2(kNone, 0.f);
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j < parts) {
+          ml[i] = *reinterpret_cast<const float2*>(part(j) + ml_at + 2 * row);
+          x[i] = *reinterpret_cast<const float4*>(part(j) + row * kHeadDim + 4 * lane);
+        }
       }
+      const float was = mx;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) mx = fmaxf(mx, ml[i].x);
+      const float f = ex2(was - mx);
+      const float4 old = y;
+      const float old_sum = sum;
+      y = make_float4(0.f, 0.f, 0.f, 0.f);
+      sum = 0.f;
+      add_part(y, sum, old, old_sum, f);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) add_part(y, sum, x[i], ml[i].y, ex2(ml[i].x - mx));
     }
     if (share > 1) {
       __syncthreads();  // the rows before these have been read
@@ -124,7 +139,7 @@ __device__ __forceinline__ void join_many(const Int4AttnParams& p, const Int4Joi
 }
 
 // CTAs [0, few.ctas) join the cuts of the kernel for few rows, the others those of the kernel for long chunks.
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, 2)
     int4_join_kernel(const __grid_constant__ Int4AttnParams p, const Int4JoinList few, const Int4JoinList many) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -539,7 +539,7 @@ __device__ __forceinline__ uint32_t q_piece(uint32_t q, int row, int piece) {
   return q + (piece >> 3) * kOBytes + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
 }
 
-__device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor next, const Ranges& ranges,
+__device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor next, const Ranges<int64_t>& ranges,
                                              int g, int tid) {
   const int r = tid & 127, warp = r >> 5, lane = tid & 31;
   const uint32_t s_tmem = sm.tmem + (static_cast<uint32_t>(32 * warp) << 16) + 256 * g, o_tmem = s_tmem + 128;
@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
     return;
   }
-  const Ranges ranges(total, ctas);
+  const Ranges<int64_t> ranges(total, ctas);
   const int64_t u0 = ranges.begin(blockIdx.x), u1 = ranges.begin(blockIdx.x + 1);
   if (before <= u0 && u0 < before + mine) {
     int64_t at = before;

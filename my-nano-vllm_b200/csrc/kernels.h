@@ -263,6 +263,8 @@ struct Int4JoinList {
 constexpr int kInt4LongRows = 256;
 int int4_decode_grid(int group, int max_q);  // CTAs that run at once on the current device; 0: error
 int int4_decode_rows(int group, int max_q);  // of a row group
+// Whether the work is counted in 32 bits: units of a call < 2^31
+bool int4_decode_fits(int group, int max_q, int num_seqs, int num_kv_heads, int64_t longest);
 int64_t int4_decode_workspace_bytes(int group, int max_q, int grid);
 // p.cuts and p.partials: one Cut of kInt4CutBytes for each CTA and two parts
 constexpr int kInt4CutBytes = 32;
