@@ -31,7 +31,6 @@
 // reference maximum and a power of two near the largest step of V are taken out, so it stays below 2^14.
 #include <atomic>
 #include <climits>
-#include <type_traits>
 
 #include "int4_attention.cuh"
 
@@ -43,7 +42,6 @@ namespace {
 __device__ int g_error = 0;
 
 constexpr int kTile = 32;               // positions per warp and unit
-constexpr int kPitch = 136;             // floats between rows of the sums on their way out (bank spread)
 constexpr float kSlack = 8.f;           // a reference maximum may lag by 2^8
 constexpr int kPieceUnits = 1;          // what a pair costs beside its tiles, in units of a tile
 
@@ -52,50 +50,29 @@ constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kUnit = kTile * kWarps;        // positions per unit
 constexpr int kParts = kUnit / 16;           // parts of a unit that lie in one page each
 
-// A kernel by the rows of a group: NT planes of 8 columns; folded: at most four rows, held twice in the eight columns.
-template <int NT_, bool kFold_>
+// A kernel by the rows of a group: NT planes of 8.
+template <int NT_>
 struct Shape {
   static constexpr int NT = NT_;
-  static constexpr bool kFold = kFold_;
-  static constexpr int R = kFold ? 4 : 8 * NT;
-  static constexpr bool kWide = NT > 1;
-  static constexpr int kCtas = NT < 4 ? 3 : 2;    // on an SM
-  static constexpr int kStages = NT < 3 ? 3 : 2;
-  static constexpr int kRowBuffers = kWide ? 1 : 2;  // of a piece's q as it comes
+  static constexpr int R = 8 * NT;
+  static constexpr int kCtas = NT < 3 ? 3 : 2;    // on an SM
+  static constexpr int kStages = 3;
 };
 
-// A piece's rows, and where its sums go.
-struct Done {
-  int first_row, rows;  // of the kv head; rows of it in all
-  int token, head;      // the sequence's first row of q, the kv head's first query head
-  int slot;             // of the partial sums, -1: the piece is a whole pair
-};
-
-// What the warps exchange.  One plane: each has sums of its positions for all values.
-template <int NT>
-struct Exchange {
-  float o[kWarps][8][kPitch];
-  float m[kWarps][8], l[kWarps][8];
-};
-// More: each has sums of all positions for its 32 values, so P goes through shared memory.
 constexpr int kPPitch = kUnit + 8;  // bank spread
-template <int NT>
-struct ExchangeP {
-  uint2 q[NT][8][32];               // B operand of S^T: plane, step, lane
-  uint16_t p[2][8 * NT][kPPitch];   // f16, of this unit and the one before
-  float kq[8 * NT], qs[8 * NT];     // score = dot kq step + qs low
-  float top[kWarps][8 * NT], top_v[kWarps];
-  float l[kWarps][8 * NT], mid[kWarps][8 * NT], ps[kWarps][8 * NT];
-};
 
 template <typename S>
 struct __align__(1024) Smem {
   uint8_t k[S::kStages][kUnit * 64];  // TMA tiles of 64-byte rows, 64B swizzle: bits 1 and 2 of a row's number
   uint8_t v[S::kStages][kUnit * 64];  // change the place of its 16-byte pieces
   uint2 scale[S::kStages][kUnit];
-  uint16_t rows[S::kRowBuffers][S::R][kHeadDim];  // q
-  std::conditional_t<S::kWide, ExchangeP<S::NT>, Exchange<S::NT>> x;
-  uint64_t full[S::kStages], empty[S::kStages], q_full[2], q_free[2], o_full, o_free;
+  uint16_t rows[S::R][kHeadDim];            // q of a piece
+  uint2 q[S::NT][8][32];                    // as the B operand of S^T: plane, step, lane
+  uint16_t p[2][S::R][kPPitch];             // P step, f16, of this unit and the one before
+  float kq[S::R], qs[S::R];                 // score = dot kq step + qs low
+  float top[kWarps][S::R], top_v[kWarps];   // of the warps' positions: largest score and step,
+  float l[kWarps][S::R], mid[kWarps][S::R], ps[kWarps][S::R];  // sums
+  uint64_t full[S::kStages], empty[S::kStages], q_full, q_free;
   uint32_t there[S::kStages];  // which parts of the stage's unit are in pages of the cache
   int scan[kThreads / 32];
   int first_seq, first_unit;   // the sequence in which the CTA's range begins, its first unit
@@ -115,12 +92,6 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
-  uint32_t d;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
-  return d;
 }
 
 __device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
@@ -262,49 +233,6 @@ __device__ __forceinline__ void convert_q(const uint16_t* row, bool is_row, int 
   qs = sum * scale_log2;
 }
 
-// This warp's share of the rows, the warps' sums joined: outputs of a whole pair, or a part for the joining kernel.
-template <typename S>
-__device__ __forceinline__ void merge(const Int4AttnParams& p, const Smem<S>& sm, const Done& d, int warp, int lane) {
-  constexpr int kRows = S::kFold ? 4 : 8, kFrom = S::kFold ? 2 : 1;
-#pragma unroll 1
-  for (int row = warp; row < kRows; row += kWarps) {
-    const int r = d.first_row + row;
-    if (r >= d.rows) break;
-    float mx = kNone;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-      for (int f = 0; f < kFrom; ++f) mx = fmaxf(mx, sm.x.m[w][row + 4 * f]);
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-#pragma unroll
-      for (int f = 0; f < kFrom; ++f) {
-        const float weight = ex2(sm.x.m[w][row + 4 * f] - mx);
-        const float4 x = *reinterpret_cast<const float4*>(&sm.x.o[w][row + 4 * f][4 * lane]);
-        y.x = fmaf(x.x, weight, y.x);
-        y.y = fmaf(x.y, weight, y.y);
-        y.z = fmaf(x.z, weight, y.z);
-        y.w = fmaf(x.w, weight, y.w);
-        sum = fmaf(sm.x.l[w][row + 4 * f], weight, sum);
-      }
-    }
-    if (d.slot < 0) {
-      const int token = token_of(p, r);
-      const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);  // 0 for a row that sees nothing
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(y.x * inv, y.y * inv), hi = __floats2bfloat162_rn(y.z * inv, y.w * inv);
-      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(d.token) + token) * p.out_row_stride +
-                                (d.head + r - token * p.group) * kHeadDim + 4 * lane) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    } else {
-      float* const part = p.partials + static_cast<int64_t>(d.slot) * (S::R * (kHeadDim + 2));
-      *reinterpret_cast<float4*>(part + row * kHeadDim + 4 * lane) = y;
-      if (lane == 0) *reinterpret_cast<float2*>(part + S::R * kHeadDim + 2 * row) = make_float2(mx, sum);
-    }
-  }
-}
-
 // Loads by one warp: a piece's rows of q (lane i: row i), and its units: lane i looks up the page of part i, and the
 // lanes at which a TMA box of box_rows positions begins load K, V and scales.
 template <typename S>
@@ -332,17 +260,17 @@ __device__ __forceinline__ void load(const Int4AttnParams& p, const CUtensorMap&
 #pragma unroll 1
   for (;;) {
     if (first) {
-      const int b = pieces % S::kRowBuffers, rows = c.s.nq * p.group - c.rg * S::R;  // from the group's first on
-      if (pieces >= S::kRowBuffers) ok = wait_all(&sm.q_free[b], (pieces / S::kRowBuffers - 1) & 1u, p.err);
+      const int rows = c.s.nq * p.group - c.rg * S::R;  // from the group's first on
+      if (pieces > 0) ok = wait_all(&sm.q_free, (pieces - 1) & 1u, p.err);
       if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(&sm.q_full[b], min(S::R, rows) * kHeadDim * 2);
+      if (lane == 0) mbar_arrive_expect_tx(&sm.q_full, min(S::R, rows) * kHeadDim * 2);
       __syncwarp();
       if (lane < S::R && lane < rows) {
         const int r = c.rg * S::R + lane, token = token_of(p, r);
-        bulk_load(smem_u32(sm.rows[b][lane]),
+        bulk_load(smem_u32(sm.rows[lane]),
                   p.q + (static_cast<int64_t>(c.s.q_first) + token) * p.q_row_stride +
                       (c.kvh * p.group + r - token * p.group) * kHeadDim,
-                  kHeadDim * 2, &sm.q_full[b]);
+                  kHeadDim * 2, &sm.q_full);
       }
       ++pieces;
       first = false;
@@ -391,8 +319,7 @@ __device__ __forceinline__ void load(const Int4AttnParams& p, const CUtensorMap&
   // a wait gave up: the copies in flight must land (or run out of time) before the CTA ends
   for (int i = 0; i < S::kStages; ++i)
     if (loaded >> i & 1u) wait_all(&sm.full[i], (i < stage ? round : round - 1) & 1u, p.err);
-  for (uint32_t i = pieces > S::kRowBuffers ? pieces - S::kRowBuffers : 0; i < pieces; ++i)
-    wait_all(&sm.q_full[i % S::kRowBuffers], (i / S::kRowBuffers) & 1u, p.err);
+  if (pieces > 0) wait_all(&sm.q_full, (pieces - 1) & 1u, p.err);
 }
 
 // The pair that the CTA's range leaves cut, if its last piece is one's beginning: for the joining kernel.
@@ -411,362 +338,18 @@ __device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor&
   reinterpret_cast<Cut*>(p.cuts)[blockIdx.x] = cut;
 }
 
-template <typename S>
-__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges<int>& ranges, int warp,
-                                        int lane) {
-  constexpr int NT = S::NT, R = S::R;
-  constexpr bool kFold = S::kFold;
-  const int g = lane >> 2, t = lane & 3;
-  // this lane's row for the transposed loads of V, and its piece (of the second of two: 1) as it is stored; its
-  // rows g and g + 8 of K, piece t
-  const int v_token = (lane & 7) + (lane & 8);
-  const uint32_t v_row = (warp * kTile + v_token) * 64, v_piece = (lane >> 4) ^ (v_token >> 1 & 3);
-  const uint32_t k_row = (warp * kTile + g) * 64 + (t ^ (g >> 1 & 3)) * 16;
-  const uint32_t k_ring = smem_u32(sm.k[0]) + k_row, v_ring = smem_u32(sm.v[0]) + v_row;
-  const uint32_t s_ring = smem_u32(sm.scale[0]) + (warp * kTile + g) * 8;
-  int stage = 0;
-  uint32_t parity = 0, pieces = 0;
-  bool ok = true;  // no wait has given up
-  Done done = {};  // the piece before
-  auto merge_last = [&]() {  // a warp joins its rows of the piece before when it has begun the next
-    ok = ok && wait_all(&sm.o_full, (pieces - 1) & 1u, p.err);
-    if (ok) merge(p, sm, done, warp, lane);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.o_free);
-  };
-#pragma unroll 1
-  for (;; ++pieces) {
-    const int n = now.end - now.tile, kvh = now.kvh, rg = now.rg;
-    const int rows = now.s.nq * p.group;  // of this kv head
-    const int buf = pieces & 1;
-    ok = ok && wait_all(&sm.q_full[buf], (pieces >> 1) & 1u, p.err);
-    uint2 q[NT][8];
-    uint64_t kq[NT], qs[NT];  // for this thread's columns 2 t and 2 t + 1
-    {
-      const int in_group = kFold ? g & 3 : g;
-      float a, b;
-      convert_q(sm.rows[buf][in_group], rg * R + in_group < rows, t, p.scale_log2, q[0], a, b);
-      kq[0] = f2_pack(__shfl_sync(0xffffffffu, a, 8 * t), __shfl_sync(0xffffffffu, a, 8 * t + 4));
-      qs[0] = f2_pack(__shfl_sync(0xffffffffu, b, 8 * t), __shfl_sync(0xffffffffu, b, 8 * t + 4));
-    }
-    if (lane == 0) mbar_arrive(&sm.q_free[buf]);
-    if (pieces > 0) merge_last();
-    int least = INT_MAX, most = 0;
-    auto limit_of = [&](int j, int c) {  // positions that a column's row sees; where there is no row, as the group's first
-      int row = rg * R + (kFold ? (2 * t + c) & 3 : 8 * j + 2 * t + c);
-      if (row >= rows) row = rg * R;
-      return min(now.s.vis, token_of(p, row) + now.s.nk - now.s.nq + 1);
-    };
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int limit = limit_of(j, c);
-        least = min(least, limit);
-        most = max(most, limit);
-      }
-    }
-#pragma unroll
-    for (int off = 1; off < 4; off <<= 1) {
-      least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-    }
-
-    float o[NT][8][4], ps[NT][4];     // ps: sum of the rounded P step
-    uint64_t minus_m[NT], l[NT], mid[NT];  // pairs of columns
-    uint32_t unset = (1u << 2 * NT) - 1;   // columns that have seen nothing: their m counts as 0
-    float limit = -INFINITY;               // how far a score may be above its m: kSlack when none is unset
-    float v_unit = 1.f, v_limit = 0.f;  // steps of V are multiplied by v_unit (a power of two)
-    int v_exp = 0;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      minus_m[j] = l[j] = mid[j] = 0;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ps[j][c] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[j][i][c] = 0.f;
-    }
-
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      const int pos0 = (now.tile + i) * kUnit + warp * kTile;
-      ok = ok && wait_all(&sm.full[stage], parity, p.err);
-      const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
-      if (halves != 0 && pos0 < most && ok) {
-        // ---- S^T: positions (rows g, g + 8 of each half) x query rows (columns)
-        float s[2][NT][4];
-        uint32_t kw[2][2][4];  // half, row g or g + 8, word
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
-            kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            uint32_t a[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t y0 = kw[h][0][w] >> (8 * b);
-              const uint32_t y1 = kw[h][1][w] >> (8 * b);
-              a[h][0] = y0 & 0x000F000Fu;
-              a[h][1] = y1 & 0x000F000Fu;
-              a[h][2] = y0 & 0x00F000F0u;
-              a[h][3] = y1 & 0x00F000F0u;
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              const uint2 qb = q[j][2 * w + b];
-              if (w == 0 && b == 0) {
-                mma16816_first(s[0][j], a[0], qb.x, qb.y);
-                mma16816_first(s[1][j], a[1], qb.x, qb.y);
-              } else {
-                mma16816(s[0][j], a[0], qb.x, qb.y);
-                mma16816(s[1][j], a[1], qb.x, qb.y);
-              }
-            }
-          }
-        }
-        // Folded: with at most four rows the columns hold them twice, the first four go on with half 0 and the
-        // last four with half 1, and the scores of a tile are half as many.
-        constexpr int H = kFold ? 1 : 2;
-        if constexpr (kFold) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[0][0][c] = t < 2 ? s[0][0][c] : s[1][0][c];
-        }
-        // ---- scores; this thread's positions: rows g and g + 8 of half h (folded: of half t >> 1)
-        float sv[H][2], mv[H][2];  // step of V, and what code 7.5 stands for
-        bool grow = false;
-        const bool full = halves == 3u && pos0 + kTile <= least;
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          const int half = kFold ? t >> 1 : h;
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + half * 128 + r * 64);
-            const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
-            sv[h][r] = __uint_as_float(sc.y << 16);
-            mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
-            const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq[j]),
-                                        f2_fma(lk2, qs[j], minus_m[j]));
-              f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
-            }
-          }
-        }
-        if (!full) {
-          int sees[NT][2];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            sees[j][0] = limit_of(j, 0);
-            sees[j][1] = limit_of(j, 1);
-          }
-#pragma unroll
-          for (int h = 0; h < H; ++h) {
-            const int half = kFold ? t >> 1 : h;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int pos = pos0 + 16 * half + g + 8 * r;
-              const bool held = (halves >> half & 1u) && pos < now.s.vis;
-              // a row of V that is no number goes to those that see it by their scores
-              const bool number = fabsf(mv[h][r]) < INFINITY;
-              if (!held || !number) sv[h][r] = mv[h][r] = 0.f;
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  if (!number) s[h][j][2 * r + c] = NAN;
-                  if (!held || pos >= sees[j][c]) s[h][j][2 * r + c] = -INFINITY;
-                }
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            grow |= sv[h][r] > v_limit;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) grow |= fmaxf(s[h][j][2 * r], s[h][j][2 * r + 1]) > limit;
-          }
-        if (__any_sync(0xffffffffu, grow)) {
-          // ---- new references: the rows' maxima so far, and a power of two near V's largest step
-          float top = 0.f;
-#pragma unroll
-          for (int h = 0; h < H; ++h) top = fmaxf(top, fmaxf(sv[h][0], sv[h][1]));
-#pragma unroll
-          for (int off = 1; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          float change = 1.f;
-          if (top > v_limit && top < INFINITY) {
-            const int e = max(-120, min(exponent(top), 120));
-            if (v_limit > 0.f) {
-              const int d = v_exp - e;
-              change = d < -126 ? 0.f : pow2(d);
-            }
-            v_exp = e;
-            v_unit = pow2(-e);
-            v_limit = pow2(min(e + 6, 127));
-          }
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            float was[2], now_m[2], f[2];
-            f2_unpack(minus_m[j], was[0], was[1]);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float mx = -INFINITY;  // above m
-#pragma unroll
-              for (int h = 0; h < H; ++h) mx = fmaxf(mx, fmaxf(s[h][j][c], s[h][j][2 + c]));
-#pragma unroll
-              for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-              const bool first = unset >> (2 * j + c) & 1u;
-              if (first && mx == -INFINITY) mx = 0.f;  // still unset
-              else unset &= ~(1u << (2 * j + c));
-              if (!first) mx = fmaxf(mx, 0.f);
-              f[c] = first ? 0.f : ex2(-mx);
-              now_m[c] = was[c] - mx;
-#pragma unroll
-              for (int h = 0; h < H; ++h) {
-                s[h][j][c] -= mx;
-                s[h][j][2 + c] -= mx;
-              }
-              ps[j][c] *= f[c] * change;
-#pragma unroll
-              for (int d = 0; d < 8; ++d) {
-                o[j][d][c] *= f[c] * change;
-                o[j][d][2 + c] *= f[c] * change;
-              }
-            }
-            minus_m[j] = f2_pack(now_m[0], now_m[1]);
-            l[j] = f2_mul(l[j], f2_pack(f[0], f[1]));
-            mid[j] = f2_mul(mid[j], f2_pack(f[0], f[1]));
-          }
-          limit = __any_sync(0xffffffffu, unset != 0) ? -INFINITY : kSlack;
-        }
-        // ---- P, its sums, and P^T step_v as the B operand of O^T
-        uint32_t pb[2][NT][2];
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float f = sv[h][r] * v_unit;
-            const uint64_t f2 = f2_pack(f, f), mv2 = f2_pack(mv[h][r], mv[h][r]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              const uint64_t x = f2_pack(ex2(s[h][j][2 * r]), ex2(s[h][j][2 * r + 1]));
-              l[j] = f2_add(l[j], x);
-              mid[j] = f2_fma(x, mv2, mid[j]);
-              float p0, p1;
-              f2_unpack(f2_mul(x, f2), p0, p1);
-              pb[h][j][r] = transpose8x8(pack_f16x2(p0, p1));
-            }
-          }
-        }
-        if constexpr (kFold) {  // columns of the other half: nothing
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t both = pb[0][0][r];
-            pb[0][0][r] = g < 4 ? both : 0u;
-            pb[1][0][r] = g < 4 ? 0u : both;
-          }
-        }
-        // ---- O^T += V^T P^T: of 32 values (a 16-byte piece) 4 g + 2 b (rows g) and 4 g + 2 b + 1 (rows g + 8,
-        // codes four bits higher)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          constexpr uint32_t kOne = 0x3C003C00u;
-          const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
-#pragma unroll
-          for (int j = 0; j < NT; ++j) mma16816(ps[j], ones, pb[h][j][0], pb[h][j][1]);
-#pragma unroll
-          for (int w = 0; w < 4; w += 2) {
-            uint32_t v[4];  // piece w: rows 0-7 and 8-15, piece w + 1: the same
-            ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + h * 1024 + (w ^ v_piece) * 16);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-#pragma unroll
-              for (int b = 0; b < 2; ++b) {
-                const uint32_t y0 = v[2 * x] >> (8 * b);
-                const uint32_t y1 = v[2 * x + 1] >> (8 * b);
-                const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
-#pragma unroll
-                for (int j = 0; j < NT; ++j) mma16816(o[j][2 * (w + x) + b], a, pb[h][j][0], pb[h][j][1]);
-              }
-            }
-          }
-        }
-      }
-      __syncwarp();  // every lane has read the stage
-      if (lane == 0) mbar_arrive(&sm.empty[stage]);
-      if (++stage == S::kStages) {
-        stage = 0;
-        parity ^= 1u;
-      }
-    }
-
-    // ---- the piece's sums
-    const bool whole = now.tile == 0 && now.end == now.s.tiles;
-    done = {rg * R, rows, now.s.q_first, kvh * p.group, whole ? -1 : 2 * static_cast<int>(blockIdx.x) + (pieces > 0 ? 1 : 0)};
-    const float unit_even = 16777216.f, unit_odd = 1048576.f, back = pow2(v_exp);
-    if (pieces > 0) ok = ok && wait_all(&sm.o_free, (pieces - 1) & 1u, p.err);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      float m[2], sum[2], middle[2];
-      f2_unpack(minus_m[j], m[0], m[1]);
-      f2_unpack(l[j], sum[0], sum[1]);
-      f2_unpack(mid[j], middle[0], middle[1]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], off);
-          middle[c] += __shfl_xor_sync(0xffffffffu, middle[c], off);
-        }
-        if (g == 0) {
-          sm.x.m[warp][2 * t + c] = unset >> (2 * j + c) & 1u ? kNone : -m[c];
-          sm.x.l[warp][2 * t + c] = sum[c];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // values 32 (i >> 1) + 4 g + 2 (i & 1) and the one after it
-          const float y0 = fmaf(fmaf(o[j][i][c], unit_even, -7.5f * ps[j][c]), back, middle[c]);
-          const float y1 = fmaf(fmaf(o[j][i][2 + c], unit_odd, -7.5f * ps[j][c]), back, middle[c]);
-          *reinterpret_cast<float2*>(&sm.x.o[warp][2 * t + c][32 * (i >> 1) + 4 * g + 2 * (i & 1)]) = make_float2(y0, y1);
-        }
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.o_full);
-    // ---- on to the next pair
-    if (!now.more()) {
-      if (warp == 0 && lane == 0) store_cut<S>(p, now, ranges, pieces);
-      break;
-    }
-    next_piece<S>(p, now);
-  }
-  ++pieces;
-  merge_last();
-}
-
 // More than one plane.  Sums of 128 values for every row would take 32 registers a plane, and two warps on a scheduler
 // do not hide the tensor cores' latency; so a warp computes S and P of its 32 positions, and of all 128 positions the
 // products with its 32 values.  P goes through shared memory (stmatrix turns it), the references are the CTA's.
 template <typename S>
-__device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges<int>& ranges,
+__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges<int>& ranges,
                                              int warp, int lane) {
   constexpr int NT = S::NT, R = S::R;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t k_ring = smem_u32(sm.k[0]) + (warp * kTile + g) * 64 + (t ^ (g >> 1 & 3)) * 16;
   const uint32_t v_ring = smem_u32(sm.v[0]) + lane * 64 + (warp ^ (lane >> 1 & 3)) * 16;
   const uint32_t s_ring = smem_u32(sm.scale[0]) + (warp * kTile + g) * 8;
-  const uint32_t p_lane = smem_u32(sm.x.p[0]) + ((lane & 7) * kPPitch + (lane >> 3) * 8) * 2;  // row of a plane, 8 positions
+  const uint32_t p_lane = smem_u32(sm.p[0]) + ((lane & 7) * kPPitch + (lane >> 3) * 8) * 2;  // row of a plane, 8 positions
   auto all_warps = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); };
   int stage = 0;
   uint32_t parity = 0, pieces = 0, p_buf = 0;
@@ -775,20 +358,20 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
   for (;; ++pieces) {
     const int n = now.end - now.tile, kvh = now.kvh, rg = now.rg;
     const int rows = now.s.nq * p.group;  // of this kv head
-    ok = ok && wait_all(&sm.q_full[0], pieces & 1u, p.err);
+    ok = ok && wait_all(&sm.q_full, pieces & 1u, p.err);
     if (warp < NT) {
       uint2 y[8];
       float a, b;
-      convert_q(sm.rows[0][8 * warp + g], rg * R + 8 * warp + g < rows, t, p.scale_log2, y, a, b);
+      convert_q(sm.rows[8 * warp + g], rg * R + 8 * warp + g < rows, t, p.scale_log2, y, a, b);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sm.x.q[warp][i][lane] = y[i];
+      for (int i = 0; i < 8; ++i) sm.q[warp][i][lane] = y[i];
       if (t == 0) {
-        sm.x.kq[8 * warp + g] = a;
-        sm.x.qs[8 * warp + g] = b;
+        sm.kq[8 * warp + g] = a;
+        sm.qs[8 * warp + g] = b;
       }
     }
     all_warps();
-    if (lane == 0) mbar_arrive(&sm.q_free[0]);
+    if (lane == 0) mbar_arrive(&sm.q_free);
     auto limit_of = [&](int j, int c) {  // positions that a column's row sees; where there is no row, as the group's first
       int row = rg * R + 8 * j + 2 * t + c;
       if (row >= rows) row = rg * R;
@@ -844,11 +427,11 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
           }
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            const uint2 q = sm.x.q[j][2 * w + b][lane];
+            const uint2 y = sm.q[j][2 * w + b][lane];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (w == 0 && b == 0) mma16816_first(s[h][j], a[h], q.x, q.y);
-              else mma16816(s[h][j], a[h], q.x, q.y);
+              if (w == 0 && b == 0) mma16816_first(s[h][j], a[h], y.x, y.y);
+              else mma16816(s[h][j], a[h], y.x, y.y);
             }
           }
         }
@@ -866,8 +449,8 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
           const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            const uint64_t kq = reinterpret_cast<const uint64_t*>(sm.x.kq)[4 * j + t];
-            const uint64_t qs = reinterpret_cast<const uint64_t*>(sm.x.qs)[4 * j + t];
+            const uint64_t kq = reinterpret_cast<const uint64_t*>(sm.kq)[4 * j + t];
+            const uint64_t qs = reinterpret_cast<const uint64_t*>(sm.qs)[4 * j + t];
             const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq), f2_fma(lk2, qs, minus_m[j]));
             f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
           }
@@ -910,19 +493,24 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
       }
       // ---- P, and P step_v to shared memory: [row][position]
       const uint32_t p_at = p_lane + p_buf * (R * kPPitch * 2);
-      float e[2][NT][4];
+      uint64_t l_now[NT], mid_now[NT];
       auto give_p = [&]() {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           uint32_t x[2][2];
+          l_now[j] = l[j];
+          mid_now[j] = mid[j];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              e[h][j][2 * r] = ex2(s[h][j][2 * r]);
-              e[h][j][2 * r + 1] = ex2(s[h][j][2 * r + 1]);
+              const uint64_t e = f2_pack(ex2(s[h][j][2 * r]), ex2(s[h][j][2 * r + 1]));
               const float f = sv[h][r] * v_unit;
-              x[h][r] = pack_f16x2(e[h][j][2 * r] * f, e[h][j][2 * r + 1] * f);
+              l_now[j] = f2_add(l_now[j], e);
+              mid_now[j] = f2_fma(e, f2_pack(mv[h][r], mv[h][r]), mid_now[j]);
+              float p0, p1;
+              f2_unpack(f2_mul(e, f2_pack(f, f)), p0, p1);
+              x[h][r] = pack_f16x2(p0, p1);
             }
           }
           stmatrix_trans(p_at + (8 * j * kPPitch + warp * kTile) * 2, x[0][0], x[0][1], x[1][0], x[1][1]);
@@ -934,7 +522,7 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
         float top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        if (lane == 0) sm.x.top_v[warp] = top;
+        if (lane == 0) sm.top_v[warp] = top;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -942,12 +530,12 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
             float mx = fmaxf(fmaxf(s[0][j][c], s[0][j][2 + c]), fmaxf(s[1][j][c], s[1][j][2 + c]));
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            if (g == 0) sm.x.top[warp][8 * j + 2 * t + c] = mx;
+            if (g == 0) sm.top[warp][8 * j + 2 * t + c] = mx;
           }
         }
         all_warps();
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.x.top_v[w]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.top_v[w]);
         float change = 1.f;
         if (top > v_limit && top < INFINITY) {
           const int x = max(-120, min(exponent(top), 120));
@@ -967,7 +555,7 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
           for (int c = 0; c < 2; ++c) {
             float mx = -INFINITY;  // above m
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.x.top[w][8 * j + 2 * t + c]);
+            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.top[w][8 * j + 2 * t + c]);
             const bool first = unset >> (2 * j + c) & 1u;
             if (first && mx == -INFINITY) mx = 0.f;  // still unset
             else unset &= ~(1u << (2 * j + c));
@@ -995,17 +583,9 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
         all_warps();
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint64_t mv2 = f2_pack(mv[h][r], mv[h][r]);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const uint64_t x = f2_pack(e[h][j][2 * r], e[h][j][2 * r + 1]);
-            l[j] = f2_add(l[j], x);
-            mid[j] = f2_fma(x, mv2, mid[j]);
-          }
-        }
+      for (int j = 0; j < NT; ++j) {
+        l[j] = l_now[j];
+        mid[j] = mid_now[j];
       }
       // ---- sums of P step_v: of this warp's positions
 #pragma unroll
@@ -1058,9 +638,9 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
           middle[c] += __shfl_xor_sync(0xffffffffu, middle[c], off);
         }
         if (g == 0) {
-          sm.x.l[warp][8 * j + 2 * t + c] = sum[c];
-          sm.x.mid[warp][8 * j + 2 * t + c] = middle[c];
-          sm.x.ps[warp][8 * j + 2 * t + c] = ps[j][c];
+          sm.l[warp][8 * j + 2 * t + c] = sum[c];
+          sm.mid[warp][8 * j + 2 * t + c] = middle[c];
+          sm.ps[warp][8 * j + 2 * t + c] = ps[j][c];
         }
       }
     }
@@ -1078,9 +658,9 @@ __device__ __forceinline__ void compute_wide(const Int4AttnParams& p, Smem<S>& s
         float sum = 0.f, middle = 0.f, steps = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          sum += sm.x.l[w][column];
-          middle += sm.x.mid[w][column];
-          steps += sm.x.ps[w][column];
+          sum += sm.l[w][column];
+          middle += sm.mid[w][column];
+          steps += sm.ps[w][column];
         }
         float y[4];  // values 4 g .. 4 g + 3 of the warp's
 #pragma unroll
@@ -1127,13 +707,8 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], kWarps);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.q_full[i], 1);
-      mbar_init(&sm.q_free[i], kWarps);
-    }
-    mbar_init(&sm.o_full, kWarps);
-    mbar_init(&sm.o_free, kWarps);
+    mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_free, kWarps);
     fence_mbar_init();
   }
   // programmatic dependent of the kernel before it: nothing is read or written before that ends
@@ -1200,8 +775,6 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
   }
   if (warp == kWarps) {
     load<S>(p, map_k, map_v, sm, c, lane);
-  } else if constexpr (S::kWide) {
-    compute_wide<S>(p, sm, c, ranges, warp, lane);
   } else {
     compute<S>(p, sm, c, ranges, warp, lane);
   }
@@ -1246,13 +819,11 @@ cudaError_t launch(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap
   return cudaLaunchKernelEx(&cfg, int4_decode_kernel<S>, p, map_k, map_v);
 }
 
-// The kernel for a call: 0 for at most four rows of a kv head, else planes of 8 rows in a row group, as many as the
-// longest chunk's rows need, at most four.
-int variant(int group, int max_q) {
+// Planes of rows in a row group: as many as the longest chunk's rows need, at most four.
+int planes_of(int group, int max_q) {
   const int64_t rows = static_cast<int64_t>(group) * max_q;
-  return rows <= 4 ? 0 : rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
 }
-int rows_of(int v) { return v == 0 ? 4 : 8 * v; }
 
 }  // namespace
 
@@ -1260,45 +831,43 @@ cudaError_t int4_error_word(void** word) { return cudaGetSymbolAddress(word, g_e
 
 int int4_decode_grid(int group, int max_q) {
   constexpr int kMaxDevices = 64;
-  static std::atomic<int> known[kMaxDevices][5];  // by device and variant; 0: not asked yet
+  static std::atomic<int> known[kMaxDevices][5];  // by device and planes; 0: not asked yet
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
-  const int v = variant(group, max_q);
+  const int v = planes_of(group, max_q);
   int n = known[dev][v].load(std::memory_order_relaxed);
   if (n == 0) {
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    n = v == 0   ? resident<Shape<1, true>>(sms)
-        : v == 1 ? resident<Shape<1, false>>(sms)
-        : v == 2 ? resident<Shape<2, false>>(sms)
-        : v == 3 ? resident<Shape<3, false>>(sms)
-                 : resident<Shape<4, false>>(sms);
+    n = v == 1   ? resident<Shape<1>>(sms)
+        : v == 2 ? resident<Shape<2>>(sms)
+        : v == 3 ? resident<Shape<3>>(sms)
+                 : resident<Shape<4>>(sms);
     known[dev][v].store(n, std::memory_order_relaxed);
   }
   return n;
 }
 
 bool int4_decode_fits(int group, int max_q, int num_seqs, int num_kv_heads, int64_t longest) {
-  const int rows = rows_of(variant(group, max_q));
+  const int rows = 8 * planes_of(group, max_q);
   const int64_t groups = (static_cast<int64_t>(group) * max_q + rows - 1) / rows;
   const int64_t each = (longest / kUnit + 1 + kPieceUnits) * groups * num_kv_heads;  // of a sequence, at most
   return each < INT_MAX && each * num_seqs < INT_MAX;
 }
 
 int64_t int4_decode_workspace_bytes(int group, int max_q, int grid) {
-  const int64_t part = static_cast<int64_t>(rows_of(variant(group, max_q))) * (kHeadDim + 2) * 4;
+  const int64_t part = static_cast<int64_t>(8 * planes_of(group, max_q)) * (kHeadDim + 2) * 4;
   return static_cast<int64_t>(grid) * (kInt4CutBytes + 2 * part);
 }
 
-int int4_decode_rows(int group, int max_q) { return rows_of(variant(group, max_q)); }
+int int4_decode_rows(int group, int max_q) { return 8 * planes_of(group, max_q); }
 
 cudaError_t launch_int4_decode(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid,
                                cudaStream_t stream) {
-  switch (variant(p.group, p.max_q)) {
-    case 0: return launch<Shape<1, true>>(p, map_k, map_v, grid, stream);
-    case 1: return launch<Shape<1, false>>(p, map_k, map_v, grid, stream);
-    case 2: return launch<Shape<2, false>>(p, map_k, map_v, grid, stream);
-    case 3: return launch<Shape<3, false>>(p, map_k, map_v, grid, stream);
-    default: return launch<Shape<4, false>>(p, map_k, map_v, grid, stream);
+  switch (planes_of(p.group, p.max_q)) {
+    case 1: return launch<Shape<1>>(p, map_k, map_v, grid, stream);
+    case 2: return launch<Shape<2>>(p, map_k, map_v, grid, stream);
+    case 3: return launch<Shape<3>>(p, map_k, map_v, grid, stream);
+    default: return launch<Shape<4>>(p, map_k, map_v, grid, stream);
   }
 }
 
