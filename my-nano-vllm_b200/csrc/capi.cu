@@ -1306,7 +1306,7 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   // both kernels, then one that joins the parts of what they cut
   auto lists = [](uint8_t* at, int rows, int ctas) {
     return fp8attn::Int4JoinList{
-        at, reinterpret_cast<const float*>(at + static_cast<int64_t>(ctas) * fp8attn::kInt4CutBytes), rows, ctas};
+        at, reinterpret_cast<const float*>(at + static_cast<int64_t>(ctas) * fp8attn::kInt4CutBytes), rows, ctas, 1};
   };
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   const fp8attn::Int4JoinList few = lists(ws, fp8attn::int4_decode_rows(p.group, plan.short_q), plan.grid);

@@ -10,7 +10,8 @@
 namespace fp8attn {
 namespace {
 
-constexpr int kWarps = 16;
+constexpr int kWarps = 8;
+constexpr int kFewBlocks = 4;  // CTAs that share the rows of a cut
 constexpr int kAtOnce = 8;  // parts of which a warp has the loads in flight
 
 __device__ __forceinline__ void add_part(float4& y, float& sum, const float4& x, float l, float f) {
@@ -33,7 +34,7 @@ __device__ __forceinline__ void store_row(const Int4AttnParams& p, const Cut& cu
 
 // At most 32 rows, up to as many parts as there are CTAs: several warps of a row take parts in turn, and their sums are
 // added in order.
-__device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4JoinList& list, int index) {
+__device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4JoinList& list, int index, int block) {
   __shared__ float4 sum_o[kWarps][32];
   __shared__ float2 sum_ml[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -44,11 +45,13 @@ __device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4Join
   const float* later = list.partials + static_cast<int64_t>(2 * index) * part_size;
   auto part = [&](int j) { return j == 0 ? first : later + static_cast<int64_t>(2 * j) * part_size; };
   const int ml_at = list.rows * kHeadDim;
-  const int share = max(1, min(kWarps / cut.rows, parts));  // warps of a row
-  const int at_once = kWarps / share;                       // rows
-  for (int row0 = 0; row0 < cut.rows; row0 += at_once) {
+  const int each = (cut.rows + list.blocks - 1) / list.blocks, begin = block * each, end = min(begin + each, cut.rows);
+  if (begin >= end) return;
+  const int share = max(1, min(kWarps / (end - begin), parts));  // warps of a row
+  const int at_once = kWarps / share;                            // rows
+  for (int row0 = begin; row0 < end; row0 += at_once) {
     const int row = row0 + warp / share, turn = warp % share;
-    const bool mine = warp < at_once * share && row < cut.rows;
+    const bool mine = warp < at_once * share && row < end;
     float mx = kNone, sum = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int j0 = turn; mine && j0 < parts; j0 += kAtOnce * share) {
@@ -138,14 +141,14 @@ __device__ __forceinline__ void join_many(const Int4AttnParams& p, const Int4Joi
     if (row0 + k < cut.rows) store_row(p, cut, row0 + k, lane, y[k], sum[k]);
 }
 
-// CTAs [0, few.ctas) join the cuts of the kernel for few rows, the others those of the kernel for long chunks.
-__global__ void __launch_bounds__(kWarps * 32, 2)
+// CTAs [0, few.ctas few.blocks) join the cuts of the kernel for few rows, the others those of the kernel for long chunks.
+__global__ void __launch_bounds__(kWarps * 32, 4)
     int4_join_kernel(const __grid_constant__ Int4AttnParams p, const Int4JoinList few, const Int4JoinList many) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int at = static_cast<int>(blockIdx.x) - few.ctas;
+  const int at = static_cast<int>(blockIdx.x) - few.ctas * few.blocks;
   if (at < 0) {
-    join_few(p, few, blockIdx.x);
+    join_few(p, few, blockIdx.x / few.blocks, blockIdx.x % few.blocks);
   } else {
     constexpr int kBlocks = kInt4LongRows / kRowsPerCta;
     join_many(p, many, at / kBlocks, at % kBlocks);
@@ -158,7 +161,8 @@ cudaError_t launch_int4_join(const Int4AttnParams& p, Int4JoinList few, Int4Join
   // the last CTA's range ends with a pair
   few.ctas = few.ctas > 1 ? few.ctas - 1 : 0;
   many.ctas = many.ctas > 1 ? many.ctas - 1 : 0;
-  const int blocks = few.ctas + many.ctas * (kInt4LongRows / kRowsPerCta);
+  few.blocks = few.rows < kFewBlocks ? few.rows : kFewBlocks;
+  const int blocks = few.ctas * few.blocks + many.ctas * (kInt4LongRows / kRowsPerCta);
   if (blocks == 0) return cudaSuccess;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -257,8 +257,9 @@ struct Int4AttnParams {
 struct Int4JoinList {
   const void* cuts;
   const float* partials;
-  int rows;  // of a row group
+  int rows;    // of a row group
   int ctas;
+  int blocks;  // that share the rows of a cut; set by the launch
 };
 constexpr int kInt4LongRows = 256;
 int int4_decode_grid(int group, int max_q);  // CTAs that run at once on the current device; 0: error
