@@ -1229,12 +1229,16 @@ struct Int4Plan {
   int64_t short_bytes, bytes;
 };
 
-static int int4_plan(Int4Plan* plan, int group, int max_q) {
+static int int4_short_q(int group, int max_q) {
   constexpr int kShortRows = 32;
   // a single token of any group stays with the first kernel, which takes wider groups in parts
   const int limit = group >= kShortRows ? 1 : kShortRows / group;
-  plan->short_q = max_q < limit ? max_q : limit;
-  plan->longer = max_q > limit;
+  return max_q < limit ? max_q : limit;
+}
+
+static int int4_plan(Int4Plan* plan, int group, int max_q) {
+  plan->short_q = int4_short_q(group, max_q);
+  plan->longer = max_q > plan->short_q;
   plan->grid = fp8attn::int4_decode_grid(group, plan->short_q);
   if (plan->grid <= 0) return fail(FP8ATTN_ECUDA, "no kernel for this device");
   plan->short_bytes = (fp8attn::int4_decode_workspace_bytes(group, plan->short_q, plan->grid) + 255) / 256 * 256;
@@ -1282,6 +1286,10 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   p.num_blocks = num_blocks;
   p.max_q = max_q;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (!fp8attn::int4_decode_fits(p.group, int4_short_q(p.group, max_q), num_seqs, num_kv_heads,
+                                 static_cast<int64_t>(max_num_blocks) * block_size))
+    return fail(FP8ATTN_EINVAL, "%d sequences of %d kv heads with block tables of %d pages are too much for one call",
+                num_seqs, num_kv_heads, max_num_blocks);
   Int4Plan plan;
   rc = int4_plan(&plan, p.group, max_q);
   if (rc) return rc;
@@ -1298,10 +1306,6 @@ static int int4_attention(void* out, const void* q, int64_t q_row_stride, const 
   if (rc) return rc;
   rc = make_codes_map(&map_v, v_cache, rows, p.box_rows);
   if (rc) return rc;
-  if (!fp8attn::int4_decode_fits(p.group, plan.short_q, num_seqs, num_kv_heads,
-                                 static_cast<int64_t>(max_num_blocks) * block_size))
-    return fail(FP8ATTN_EINVAL, "%d sequences of %d kv heads with block tables of %d pages are too much for one call",
-                num_seqs, num_kv_heads, max_num_blocks);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // both kernels, then one that joins the parts of what they cut
   auto lists = [](uint8_t* at, int rows, int ctas) {

@@ -9,18 +9,22 @@
 // code * 2^-20: one mask makes a pair of operands of the tensor cores, and the powers of two are put
 // into q and into the outputs.  q is exact in f16 after a power-of-two scale per row.
 //
-// Bound by HBM: 136 bytes of K and V for each position and kv head, read once for all of the rows of its
-// query heads.  At 5.8 SM cycles per position (6.55 TB/s over 148 SMs) the math has to stay near one
-// mma.sync per position, so everything stays in registers: a warp computes S^T = K q^T for 32 positions
-// (A = codes, 16 positions x 16 values), turns P^T by movmatrix and adds O^T += V^T P^T (A = codes again,
-// pairs of positions made by byte permutes).
+// Bound by HBM up to 8 rows: 136 bytes of K and V for each position and kv head, read once for all of the rows of
+// its query heads (64 sequences of 32,768, 8 rows: 382 us, 0.91 of the floor at 6.55 TB/s; 4 rows: 380 us).  Above,
+// by the tensor cores of mma.sync: 34 products of 8 cycles for each 32 positions and plane of 8 rows, which fp32
+// arithmetic does not overlap (8 fma beside one product: 14.9 cycles, and 8 without it), against 186 cycles of
+// HBM: 16 rows 529 us, 24 rows 720, 32 rows 946.
 //
-// Work: a unit is 128 positions of one (sequence, row group, kv head), 32 for each of the CTA's four
-// warps.  All units in order are cut into equal ranges, one for each resident CTA, wherever the cuts
-// fall: no counters, no order that depends on timing.  A CTA's first and last piece may be parts of a
-// pair; their sums go to the workspace, and a second kernel joins the parts of each cut pair in order.
-// Every warp keeps two of its own tiles of 4.25 KB in flight (TMA, 64B swizzle, one lane issues), across the ends
-// of pieces.
+// Work: a unit is 128 positions of one (sequence, row group, kv head), and a warp computes S^T = K q^T and P of 32 of
+// them (A = codes, 16 positions x 16 values).  P goes through shared memory (stmatrix turns it), and of all 128
+// positions the warp adds O^T += V^T P^T for its 32 values (A = codes again, turned by ldmatrix).  So a warp's sums are
+// 8 registers for 8 rows and not 32, and no sums are added at the end.  With all values in one warp 8 rows took 410 us
+// instead of 382, 24 rows 800 instead of 720; q in registers instead of shared memory 845 (24 rows, spills).
+//
+// All units in order are cut into equal ranges, one for each resident CTA, wherever the cuts fall: no counters, no
+// order that depends on timing.  A CTA's first and last piece may be parts of a pair; their sums go to the workspace,
+// and a second kernel joins the parts of each cut pair in order.  One warp loads (TMA, 64B swizzle), three units ahead
+// and across the ends of pieces.
 //
 // c - 7.5 is the product with c and 7.5 times the same product with ones: taken about the middle of the codes, the
 // roundings of P and the cuts of the tensor cores' sums (2^-24 of each partial sum, all one way: 2e-5 of the sum
@@ -41,7 +45,7 @@ namespace {
 // hold its address.
 __device__ int g_error = 0;
 
-constexpr int kTile = 32;               // positions per warp and unit
+constexpr int kTile = 32;               // positions of a unit whose scores a warp computes
 constexpr float kSlack = 8.f;           // a reference maximum may lag by 2^8
 constexpr int kPieceUnits = 1;          // what a pair costs beside its tiles, in units of a tile
 
@@ -50,7 +54,8 @@ constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kUnit = kTile * kWarps;        // positions per unit
 constexpr int kParts = kUnit / 16;           // parts of a unit that lie in one page each
 
-// A kernel by the rows of a group: NT planes of 8.
+// A kernel by the rows of a group: NT planes of 8.  As many CTAs on an SM as have room for their sums without spilling
+// (24 rows: three CTAs of 128 registers 736 us, two 721; 8 rows: four with two stages 393 us, three with three 382).
 template <int NT_>
 struct Shape {
   static constexpr int NT = NT_;
@@ -338,9 +343,8 @@ __device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor&
   reinterpret_cast<Cut*>(p.cuts)[blockIdx.x] = cut;
 }
 
-// More than one plane.  Sums of 128 values for every row would take 32 registers a plane, and two warps on a scheduler
-// do not hide the tensor cores' latency; so a warp computes S and P of its 32 positions, and of all 128 positions the
-// products with its 32 values.  P goes through shared memory (stmatrix turns it), the references are the CTA's.
+// Scores, softmax and sums by four warps, which meet once for each unit: whether one of them needs new reference
+// maxima, and with it, that P is there.
 template <typename S>
 __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges<int>& ranges,
                                              int warp, int lane) {

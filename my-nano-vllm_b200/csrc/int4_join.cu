@@ -3,8 +3,9 @@
 // Part c has sums O_c, l_c of its positions for the reference maximum m_c; with M = max m_c
 //   out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c,
 // added in the order of the parts.  CTA i takes what the cut of CTA i says.  Bound by latency (descriptor, maxima, sums,
-// output: four dependent accesses of L2), so few rows with many parts are shared by several warps, and many rows with
-// few parts go four to a warp with all loads in flight.
+// output: three dependent accesses of L2), so few rows with many parts are shared by up to four CTAs and their warps,
+// with eight parts of a warp in flight, and many rows with few parts go four to a warp (4 rows of 55 parts: 2 us; one
+// CTA for a pair, maxima first: 6).
 #include "int4_attention.cuh"
 
 namespace fp8attn {
@@ -141,7 +142,8 @@ __device__ __forceinline__ void join_many(const Int4AttnParams& p, const Int4Joi
     if (row0 + k < cut.rows) store_row(p, cut, row0 + k, lane, y[k], sum[k]);
 }
 
-// CTAs [0, few.ctas few.blocks) join the cuts of the kernel for few rows, the others those of the kernel for long chunks.
+// CTAs [0, few.ctas * few.blocks) join the cuts of the kernel for few rows, the others those of the kernel for long
+// chunks.
 __global__ void __launch_bounds__(kWarps * 32, 4)
     int4_join_kernel(const __grid_constant__ Int4AttnParams p, const Int4JoinList few, const Int4JoinList many) {
   asm volatile("griddepcontrol.wait;" ::: "memory");

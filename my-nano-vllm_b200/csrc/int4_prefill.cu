@@ -14,8 +14,13 @@
 // it: q is laid out in the same order, outputs are put back.  A row of K or V that is not finite becomes NaN in K
 // and zero in V, so that it reaches just those query rows that see it.
 //
-// Tensor work: 2 * 2 * 128 * 128 * 256 flop in 2,048 cycles a tile (4,096 multiply-adds a cycle and SM); a softmax
-// row of 128 needs 1,024 cycles of the exponential unit for each group, so 5 of 16 pairs take a polynomial instead.
+// Bound by the chain of a group: products of its tile (1,056 cycles: one every 66), then its softmax (about 3,200
+// beside the other group's and the unpacking), 4,200 cycles for a tile of both groups; tensor cores and issue slots are
+// half busy (2,048 new tokens of 32,768 positions, 32 heads: 947 us, 1,124 TFLOP/s).  A softmax row of 128 needs 1,024
+// cycles of the exponential unit for each group, so 1 of 4 pairs takes a polynomial instead (7 prompts: 182 to 176 us).
+// Tried: scores and P by halves of a tile, so that softmax and products of a group overlap (1,404 us: products of 64
+// columns take as long as those of 128), P alone by halves (1,041: the issuing warp waits for one group while the
+// other is ready), an issuing warp for each group (1,250).
 //
 // Warps: 0-3 and 4-7 softmax of the groups, a row each thread; 8-11 turn codes into f16; 12 loads (TMA); 13 issues
 // the products.  Registers are moved from the others to the softmax (setmaxnreg).  Units of 128 positions of all items
@@ -855,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (c.tile >= c.end) {  // none but what is counted for an item beside its tiles
     if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
-  } else   if (warp < kUnpackWarp) {
+  } else if (warp < kUnpackWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     softmax_role(p, sm, c, ranges, warp >> 2, tid);
   } else if (warp < kLoadWarp) {

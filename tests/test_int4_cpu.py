@@ -98,7 +98,8 @@ ATTENTION = CACHE + [(dict(heads=30), "multiple"), (dict(heads=0), "multiple"), 
                      (dict(seqs=-1), "num_seqs"), (dict(q=None), "null"), (dict(bt=None), "null"),
                      (dict(q=P + 8), "aligned"), (dict(qs=4000), "aligned"), (dict(qs=4100), "aligned"),
                      (dict(bts=3), "block table"), (dict(mb=-1), "block table"),
-                     (dict(mb=1 << 16, bts=1 << 16), "2^24")]
+                     (dict(mb=1 << 16, bts=1 << 16), "2^24"),
+                     (dict(seqs=60000, mb=(1 << 16) - 1, bts=1 << 16), "too much")]
 
 
 @pytest.mark.parametrize("bad,msg", ATTENTION + [(dict(ctx=None), "null")])
