@@ -28,8 +28,10 @@
 //
 // c - 7.5 is the product with c and 7.5 times the same product with ones: taken about the middle of the codes, the
 // roundings of P and the cuts of the tensor cores' sums (2^-24 of each partial sum, all one way: 2e-5 of the sum
-// after 512 of them) are in proportion to the values and not to their distance from the row's lowest one
-// (32,768 positions: 2.1e-3 off in the 2-norm without it, 1.7e-3 with, all but the output's own rounding).
+// after 512 of them) are in proportion to the values and not to their distance from the row's lowest one.  So the
+// product with ones is taken for all 128 positions one after another, as the others are, a plane by one warp
+// (32,768 positions: 1.7e-3 off in the 2-norm, all but the output's own rounding; 5.3e-3 when each warp took the
+// ones of its own 32 positions, 2.1e-3 without the middle and with a quarter of the sums).
 //
 // Precision: scores, statistics and sums in fp32; P is rounded once, to f16 (2^-12), after its row's
 // reference maximum and a power of two near the largest step of V are taken out, so it stays below 2^14.
@@ -76,7 +78,7 @@ struct __align__(1024) Smem {
   uint16_t p[2][S::R][kPPitch];             // P step, f16, of this unit and the one before
   float kq[S::R], qs[S::R];                 // score = dot kq step + qs low
   float top[kWarps][S::R], top_v[kWarps];   // of the warps' positions: largest score and step,
-  float l[kWarps][S::R], mid[kWarps][S::R], ps[kWarps][S::R];  // sums
+  float l[kWarps][S::R], mid[kWarps][S::R], ps[S::R];  // sums
   uint64_t full[S::kStages], empty[S::kStages], q_full, q_free;
   uint32_t there[S::kStages];  // which parts of the stage's unit are in pages of the cache
   int scan[kThreads / 32];
@@ -387,7 +389,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
 
-    float o[NT][2][4], ps[NT][4];          // ps: sum of the rounded P step, of this warp's positions
+    float o[NT][2][4], ps[4] = {};         // ps: sums of the rounded P step of plane `warp`
     uint64_t minus_m[NT], l[NT], mid[NT];  // pairs of columns
     uint32_t unset = (1u << 2 * NT) - 1;   // columns that have seen nothing: their m counts as 0
     float limit = -INFINITY;               // how far a score may be above its m: kSlack when none is unset
@@ -397,7 +399,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
     for (int j = 0; j < NT; ++j) {
       minus_m[j] = l[j] = mid[j] = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) ps[j][c] = o[j][0][c] = o[j][1][c] = 0.f;
+      for (int c = 0; c < 4; ++c) o[j][0][c] = o[j][1][c] = 0.f;
     }
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
@@ -571,7 +573,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
               s[h][j][c] -= mx;
               s[h][j][2 + c] -= mx;
             }
-            ps[j][c] *= f[c] * change;
+            if (j == warp) ps[c] *= f[c] * change;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               o[j][b][c] *= f[c] * change;
@@ -591,15 +593,17 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         l[j] = l_now[j];
         mid[j] = mid_now[j];
       }
-      // ---- sums of P step_v: of this warp's positions
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
+      // ---- sums of P step_v of a plane, in the order and number of products of O
+      if (warp < NT) {
         constexpr uint32_t kOne = 0x3C003C00u;
         const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
-        uint32_t b[4];
-        ldmatrix(b, p_at + (8 * j * kPPitch + warp * kTile) * 2);
-        mma16816(ps[j], ones, b[0], b[1]);
-        mma16816(ps[j], ones, b[2], b[3]);
+#pragma unroll
+        for (int x = 0; x < kUnit / 32; ++x) {
+          uint32_t b[4];
+          ldmatrix(b, p_at + (8 * warp * kPPitch + x * 32) * 2);
+          mma16816(ps, ones, b[0], b[1]);
+          mma16816(ps, ones, b[2], b[3]);
+        }
       }
       // ---- O^T += V^T P^T: of its 32 values 4 g + 2 b (rows g) and 4 g + 2 b + 1 (rows g + 8, codes four bits higher)
 #pragma unroll
@@ -644,7 +648,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         if (g == 0) {
           sm.l[warp][8 * j + 2 * t + c] = sum[c];
           sm.mid[warp][8 * j + 2 * t + c] = middle[c];
-          sm.ps[warp][8 * j + 2 * t + c] = ps[j][c];
+          if (j == warp) sm.ps[8 * j + 2 * t + c] = ps[c];
         }
       }
     }
@@ -659,12 +663,12 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int column = 8 * j + 2 * t + c, r = rg * R + column;
-        float sum = 0.f, middle = 0.f, steps = 0.f;
+        float sum = 0.f, middle = 0.f;
+        const float steps = sm.ps[column];
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           sum += sm.l[w][column];
           middle += sm.mid[w][column];
-          steps += sm.ps[w][column];
         }
         float y[4];  // values 4 g .. 4 g + 3 of the warp's
 #pragma unroll
