@@ -62,8 +62,8 @@ template <int NT_>
 struct Shape {
   static constexpr int NT = NT_;
   static constexpr int R = 8 * NT;
-  static constexpr int kCtas = NT < 3 ? 3 : 2;    // on an SM
-  static constexpr int kStages = 3;
+  static constexpr int kCtas = NT < 4 ? 3 : 2;    // on an SM
+  static constexpr int kStages = NT == 3 ? 2 : 3;
 };
 
 constexpr int kPPitch = kUnit + 8;  // bank spread

@@ -75,20 +75,21 @@ def store_kvcache_int4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Te
     device = key.get_device()
     assert device >= 0 and key.dtype == _BF16, "key must be a bf16 CUDA tensor"
     assert value.get_device() == device and value.dtype == _BF16
-    assert key.dim() == 3 and value.shape == key.shape
-    assert key.stride(2) == 1 and value.stride(2) == 1
+    assert key.dim() == 3
     if device != _current_device():
         with torch.cuda.device(device):
             return store_kvcache_int4(key, value, k_cache, v_cache, kv_scale, slot_mapping)
     num_blocks, kv_heads, block_size, _ = _check_cache(k_cache, v_cache, kv_scale, device)
-    N = key.shape[0]
-    assert key.shape[1] == kv_heads and key.shape[2] == HEAD_DIM
+    shape = key.shape
+    N = shape[0]
+    assert shape[1] == kv_heads and shape[2] == HEAD_DIM and value.shape == shape
+    (k_ts, k_hs, k_unit), (v_ts, v_hs, v_unit) = key.stride(), value.stride()
+    assert k_unit == 1 and v_unit == 1
     assert slot_mapping.get_device() == device and slot_mapping.dtype == _I32
     assert slot_mapping.is_contiguous() and slot_mapping.numel() == N
-    rc = _store(key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-                value.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(),
-                slot_mapping.data_ptr(), N, kv_heads, HEAD_DIM, num_blocks, block_size,
-                _raw_stream(device))
+    rc = _store(key.data_ptr(), k_ts, k_hs, value.data_ptr(), v_ts, v_hs, k_cache.data_ptr(),
+                v_cache.data_ptr(), kv_scale.data_ptr(), slot_mapping.data_ptr(), N, kv_heads,
+                HEAD_DIM, num_blocks, block_size, _raw_stream(device))
     if rc:
         _lib.check(rc)
 
@@ -107,8 +108,9 @@ def load_kvcache_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scale: to
     assert slot_mapping.is_contiguous() and slot_mapping.dim() == 1
     N = slot_mapping.shape[0]
     shape, strides = (N, kv_heads, HEAD_DIM), (kv_heads * HEAD_DIM, HEAD_DIM, 1)
-    key = _empty(shape, strides, dtype=_BF16, device=k_cache.device)
-    value = _empty(shape, strides, dtype=_BF16, device=k_cache.device)
+    on = k_cache.device
+    key = _empty(shape, strides, dtype=_BF16, device=on)
+    value = _empty(shape, strides, dtype=_BF16, device=on)
     rc = _load(k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(), slot_mapping.data_ptr(),
                key.data_ptr(), value.data_ptr(), N, kv_heads, HEAD_DIM, num_blocks, block_size,
                _raw_stream(device))
@@ -143,26 +145,29 @@ def int4_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         with torch.cuda.device(device):
             return int4_decode_attention(q, k_cache, v_cache, kv_scale, block_tables, context_lens,
                                          softmax_scale)
-    assert q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1
-    batch, heads = q.shape[0], q.shape[1]
-    assert q.stride(1) == HEAD_DIM or heads == 1
+    assert q.dim() == 3
+    batch, heads, dim = q.shape
+    row, head, unit = q.stride()
+    assert dim == HEAD_DIM and unit == 1 and (head == HEAD_DIM or heads == 1)
     num_blocks, kv_heads, block_size, _ = _check_cache(k_cache, v_cache, kv_scale, device)
-    assert block_tables.get_device() == device and block_tables.dtype == _I32
-    assert block_tables.dim() == 2 and block_tables.shape[0] >= batch and block_tables.stride(1) == 1
+    assert block_tables.get_device() == device and block_tables.dtype == _I32 and block_tables.dim() == 2
+    sequences, columns = block_tables.shape
+    table_row, unit = block_tables.stride()
+    assert sequences >= batch and unit == 1
     assert context_lens.get_device() == device and context_lens.dtype == _I32
     assert context_lens.is_contiguous() and context_lens.numel() >= batch
     width = heads * HEAD_DIM
-    out = _empty((batch, heads, HEAD_DIM), (width, HEAD_DIM, 1), dtype=_BF16, device=q.device)
+    on = q.device
+    out = _empty((batch, heads, HEAD_DIM), (width, HEAD_DIM, 1), dtype=_BF16, device=on)
     if batch == 0:
         return out
     _INT4_DEVICES.add(device)
     nbytes = _scratch_bytes(device, batch, heads, kv_heads, 1)
-    scratch = _empty((max(nbytes, 0),), (1,), dtype=_U8, device=q.device)
-    columns = block_tables.shape[1]
+    scratch = _empty((max(nbytes, 0),), (1,), dtype=_U8, device=on)
     # the row stride of a single row is never used, and torch leaves it arbitrary
-    rc = _decode(out.data_ptr(), q.data_ptr(), q.stride(0) if batch > 1 else width, k_cache.data_ptr(),
+    rc = _decode(out.data_ptr(), q.data_ptr(), row if batch > 1 else width, k_cache.data_ptr(),
                  v_cache.data_ptr(), kv_scale.data_ptr(), block_tables.data_ptr(),
-                 block_tables.stride(0) if batch > 1 else columns, columns, context_lens.data_ptr(),
+                 table_row if batch > 1 else columns, columns, context_lens.data_ptr(),
                  batch, heads, kv_heads, HEAD_DIM, num_blocks, block_size, softmax_scale,
                  scratch.data_ptr(), nbytes, _raw_stream(device))
     if rc:
@@ -191,29 +196,32 @@ def int4_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         with torch.cuda.device(device):
             return int4_prefill_attention(q, k_cache, v_cache, kv_scale, block_tables, cu_seqlens_q,
                                           cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale)
-    assert q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1
-    tokens, heads = q.shape[0], q.shape[1]
-    assert q.stride(1) == HEAD_DIM or heads == 1
+    assert q.dim() == 3
+    tokens, heads, dim = q.shape
+    row, head, unit = q.stride()
+    assert dim == HEAD_DIM and unit == 1 and (head == HEAD_DIM or heads == 1)
     num_blocks, kv_heads, block_size, _ = _check_cache(k_cache, v_cache, kv_scale, device)
     for cu in (cu_seqlens_q, cu_seqlens_k):
         assert cu.get_device() == device and cu.dtype == _I32 and cu.is_contiguous()
     num_seqs = cu_seqlens_q.numel() - 1
     assert cu_seqlens_k.numel() >= num_seqs + 1
-    assert block_tables.get_device() == device and block_tables.dtype == _I32
-    assert block_tables.dim() == 2 and block_tables.shape[0] >= num_seqs and block_tables.stride(1) == 1
+    assert block_tables.get_device() == device and block_tables.dtype == _I32 and block_tables.dim() == 2
+    sequences, columns = block_tables.shape
+    table_row, unit = block_tables.stride()
+    assert sequences >= num_seqs and unit == 1
     width = heads * HEAD_DIM
-    out = _empty((tokens, heads, HEAD_DIM), (width, HEAD_DIM, 1), dtype=_BF16, device=q.device)
+    on = q.device
+    out = _empty((tokens, heads, HEAD_DIM), (width, HEAD_DIM, 1), dtype=_BF16, device=on)
     if tokens == 0 or num_seqs <= 0:
         return out
     # no sequence has more new tokens than there are rows
     max_q = min(int(max_seqlen_q), tokens)
     _INT4_DEVICES.add(device)
     nbytes = _scratch_bytes(device, num_seqs, heads, kv_heads, max_q)
-    scratch = _empty((max(nbytes, 0),), (1,), dtype=_U8, device=q.device)
-    columns = block_tables.shape[1]
-    rc = _prefill(out.data_ptr(), q.data_ptr(), q.stride(0) if tokens > 1 else width,
+    scratch = _empty((max(nbytes, 0),), (1,), dtype=_U8, device=on)
+    rc = _prefill(out.data_ptr(), q.data_ptr(), row if tokens > 1 else width,
                   k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(),
-                  block_tables.data_ptr(), block_tables.stride(0) if num_seqs > 1 else columns, columns,
+                  block_tables.data_ptr(), table_row if num_seqs > 1 else columns, columns,
                   cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), num_seqs, max_q, heads, kv_heads,
                   HEAD_DIM, num_blocks, block_size, softmax_scale, scratch.data_ptr(), nbytes,
                   _raw_stream(device))

@@ -39,33 +39,36 @@ def apply_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     dtype, device = q.dtype, q.get_device()
     code = _DTYPES.get(dtype)
     assert code is not None and device >= 0, "q must be a bf16 or fp16 CUDA tensor"
-    assert q.dim() == 3 and q.stride(2) == 1
+    assert q.dim() == 3
     if device != _current_device():
         with torch.cuda.device(device):
             return apply_rope(q, k, positions, cos_sin_cache, interleaved, inplace)
     N, heads, D = q.shape
+    q_ts, q_hs, unit = q.stride()
+    assert unit == 1
     assert positions.get_device() == device and positions.dtype == torch.int64
     assert positions.is_contiguous() and positions.numel() == N
     assert cos_sin_cache.get_device() == device and cos_sin_cache.dtype == torch.float32
-    R = cos_sin_cache.shape[-1]
-    assert cos_sin_cache.is_contiguous() and cos_sin_cache.numel() > 0
+    R, size = cos_sin_cache.shape[-1], cos_sin_cache.numel()
+    assert size > 0 and cos_sin_cache.is_contiguous()
     assert D % 2 == 0 and D > 0 and R % 2 == 0 and R <= D
-    kv_heads = k_ptr = k_ts = k_hs = k_out_ptr = k_out_ts = k_out_hs = 0
-    q_out = q if inplace else _empty((N, heads, D), (heads * D, D, 1), dtype=dtype, device=q.device)
+    on = q.device
+    kv_heads = k_ptr = k_ts = k_hs = k_out_ptr = 0
     k_out = None
     if k is not None:
-        assert k.get_device() == device and k.dtype == dtype
-        assert k.dim() == 3 and k.shape[0] == N and k.shape[2] == D and k.stride(2) == 1
-        kv_heads = k.shape[1]
-        k_out = k if inplace else _empty((N, kv_heads, D), (kv_heads * D, D, 1), dtype=dtype,
-                                         device=q.device)
-        k_ptr, (k_ts, k_hs, _) = k.data_ptr(), k.stride()
-        k_out_ptr, (k_out_ts, k_out_hs, _) = k_out.data_ptr(), k_out.stride()
+        assert k.get_device() == device and k.dtype == dtype and k.dim() == 3
+        k_tokens, kv_heads, k_width = k.shape
+        k_ts, k_hs, unit = k.stride()
+        assert k_tokens == N and k_width == D and unit == 1
+        k_out = k if inplace else _empty((N, kv_heads, D), (kv_heads * D, D, 1), dtype=dtype, device=on)
+        k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
+    q_out = q if inplace else _empty((N, heads, D), (heads * D, D, 1), dtype=dtype, device=on)
     if N > 0 and heads > 0:
-        rc = _rope(q.data_ptr(), q.stride(0), q.stride(1), k_ptr, k_ts, k_hs, positions.data_ptr(),
-                   cos_sin_cache.data_ptr(), cos_sin_cache.numel() // R, q_out.data_ptr(),
-                   q_out.stride(0), q_out.stride(1), k_out_ptr, k_out_ts, k_out_hs, N, heads,
-                   kv_heads, D, R, 1 if interleaved else 0, code, _raw_stream(device))
+        out = (q_ts, q_hs, k_ts, k_hs) if inplace else (heads * D, D, kv_heads * D, D)
+        rc = _rope(q.data_ptr(), q_ts, q_hs, k_ptr, k_ts, k_hs, positions.data_ptr(),
+                   cos_sin_cache.data_ptr(), size // R, q_out.data_ptr(), out[0], out[1], k_out_ptr,
+                   out[2], out[3], N, heads, kv_heads, D, R, 1 if interleaved else 0, code,
+                   _raw_stream(device))
         if rc:
             _lib.check(rc)
     return q_out, k_out
