@@ -10,16 +10,16 @@
 // into q and into the outputs.  q is exact in f16 after a power-of-two scale per row.
 //
 // Bound by HBM up to 8 rows: 136 bytes of K and V for each position and kv head, read once for all of the rows of
-// its query heads (64 sequences of 32,768, 8 rows: 382 us, 0.91 of the floor at 6.55 TB/s; 4 rows: 380 us).  Above,
+// its query heads (64 sequences of 32,768, 8 rows: 392 us, 0.89 of the floor at 6.55 TB/s; 4 rows: 390 us).  Above,
 // by the tensor cores of mma.sync: 34 products of 8 cycles for each 32 positions and plane of 8 rows, which fp32
 // arithmetic does not overlap (8 fma beside one product: 14.9 cycles, and 8 without it), against 186 cycles of
-// HBM: 16 rows 529 us, 24 rows 720, 32 rows 946.
+// HBM: 16 rows 536 us, 24 rows 724, 32 rows 955.
 //
 // Work: a unit is 128 positions of one (sequence, row group, kv head), and a warp computes S^T = K q^T and P of 32 of
 // them (A = codes, 16 positions x 16 values).  P goes through shared memory (stmatrix turns it), and of all 128
 // positions the warp adds O^T += V^T P^T for its 32 values (A = codes again, turned by ldmatrix).  So a warp's sums are
 // 8 registers for 8 rows and not 32, and no sums are added at the end.  With all values in one warp 8 rows took 410 us
-// instead of 382, 24 rows 800 instead of 720; q in registers instead of shared memory 845 (24 rows, spills).
+// and 24 rows 800; with q in registers instead of shared memory 24 rows took 845 (spills).
 //
 // All units in order are cut into equal ranges, one for each resident CTA, wherever the cuts fall: no counters, no
 // order that depends on timing.  A CTA's first and last piece may be parts of a pair; their sums go to the workspace,
@@ -57,7 +57,8 @@ constexpr int kUnit = kTile * kWarps;        // positions per unit
 constexpr int kParts = kUnit / 16;           // parts of a unit that lie in one page each
 
 // A kernel by the rows of a group: NT planes of 8.  As many CTAs on an SM as have room for their sums without spilling
-// (24 rows: three CTAs of 128 registers 736 us, two 721; 8 rows: four with two stages 393 us, three with three 382).
+// (24 rows: three CTAs of 128 registers 724 us, two of 168 754; 8 rows: four with two stages 393 us, three with three
+// 382, both before the ones' products were taken in full).
 template <int NT_>
 struct Shape {
   static constexpr int NT = NT_;
