@@ -421,7 +421,8 @@ FP8ATTN_API int fp8attn_int4_prefill(void* out, const void* q, int64_t q_row_str
                                      int num_kv_heads, int head_dim, int64_t num_blocks, int block_size,
                                      float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Copies the error word of the two attention calls on the current device (a bounded wait that gave up records 1) to
+/* Copies the error word of the two attention calls on the current device (a bounded wait that gave up records 1, a
+ * chunk call whose work is more than 2^31 units of 128 positions of 256 query rows records 5 and computes nothing) to
  * dst (device or host memory) on the stream, and clears it if `clear` is not 0. */
 FP8ATTN_API int fp8attn_int4_read_error(int32_t* dst, int clear, void* stream);
 

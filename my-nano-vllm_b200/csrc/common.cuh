@@ -26,6 +26,7 @@ enum DeviceError : int {
   kDevErrBadBlock = 2,
   kDevErrTmemAlloc = 3,
   kDevErrWorkspace = 4,
+  kDevErrTooLarge = 5,
 };
 
 __device__ __forceinline__ unsigned long long globaltimer_ns() {

@@ -12,12 +12,12 @@ namespace {
 
 constexpr float kNone = -3.402823466e38f;
 
-// A warp's wait, bounded by a number of polls (each of some tens of cycles: a second or more).  Small, since it stands in
-// many places: the roles' loops share the instruction cache.
+// A warp's wait, bounded by a number of polls (the hardware ends each after 7,800 cycles when nothing comes: a second in
+// all).  Small, since it stands in many places: the roles' loops share the instruction cache.
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, int* err) {
   bool done = false;
 #pragma unroll 1
-  for (uint32_t polls = 0; polls < (1u << 26) && !done; ++polls) done = mbar_try_wait(bar, parity);
+  for (uint32_t polls = 0; polls < (1u << 18) && !done; ++polls) done = mbar_try_wait(bar, parity);
   done = __all_sync(0xffffffffu, done);
   if (!done) atomicExch(err, kDevErrWaitTimeout);
   return done;
@@ -47,17 +47,13 @@ struct Cut {
 static_assert(sizeof(Cut) == kInt4CutBytes, "as in kernels.h");
 
 // u units in n ranges of equal size, the first u % n of them one longer.
-template <typename T>
 struct Ranges {
-  T each, longer;
-  __device__ __forceinline__ Ranges(T u, int n) {
-    each = u <= INT_MAX ? static_cast<T>(static_cast<uint32_t>(u) / static_cast<uint32_t>(n)) : u / n;
-    longer = u - each * n;
-  }
-  __device__ __forceinline__ T begin(int i) const { return i * each + min(static_cast<T>(i), longer); }
-  __device__ __forceinline__ int owner(T x) const {  // range of unit x
-    const T split = longer * (each + 1);
-    return static_cast<int>(x < split ? x / (each + 1) : longer + (x - split) / each);
+  int each, longer;
+  __device__ __forceinline__ Ranges(int u, int n) : each(u / n), longer(u % n) {}
+  __device__ __forceinline__ int begin(int i) const { return i * each + min(i, longer); }
+  __device__ __forceinline__ int owner(int x) const {  // range of unit x
+    const int split = longer * (each + 1);
+    return x < split ? x / (each + 1) : longer + (x - split) / each;
   }
 };
 

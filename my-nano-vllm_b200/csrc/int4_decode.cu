@@ -332,7 +332,7 @@ __device__ __forceinline__ void load(const Int4AttnParams& p, const CUtensorMap&
 
 // The pair that the CTA's range leaves cut, if its last piece is one's beginning: for the joining kernel.
 template <typename S>
-__device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor& now, const Ranges<int>& ranges, uint32_t pieces) {
+__device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor& now, const Ranges& ranges, uint32_t pieces) {
   Cut cut = {};
   if (now.tile == 0 && now.end < now.s.tiles) {
     const int first = now.begin + kPieceUnits, last = first + now.s.tiles - 1;  // its tiles, as units
@@ -349,7 +349,7 @@ __device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor&
 // Scores, softmax and sums by four warps, which meet once for each unit: whether one of them needs new reference
 // maxima, and with it, that P is there.
 template <typename S>
-__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges<int>& ranges,
+__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges& ranges,
                                              int warp, int lane) {
   constexpr int NT = S::NT, R = S::R;
   const int g = lane >> 2, t = lane & 3;
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, S::kCtas)
     if (tid == 0) cuts[blockIdx.x].parts = 0;
     return;
   }
-  const Ranges<int> ranges(total, ctas);
+  const Ranges ranges(total, ctas);
   const int u0 = ranges.begin(blockIdx.x);
   if (before <= u0 && u0 < before + mine) {
     int at = before;

@@ -16,11 +16,13 @@
 //
 // Bound by the chain of a group: products of its tile (1,056 cycles: one every 66), then its softmax (about 3,200
 // beside the other group's and the unpacking), 4,200 cycles for a tile of both groups; tensor cores and issue slots are
-// half busy (2,048 new tokens of 32,768 positions, 32 heads: 947 us, 1,124 TFLOP/s).  A softmax row of 128 needs 1,024
+// half busy (2,048 new tokens of 32,768 positions, 32 heads: 941 us, 1,131 TFLOP/s).  A softmax row of 128 needs 1,024
 // cycles of the exponential unit for each group, so 1 of 4 pairs takes a polynomial instead (7 prompts: 182 to 176 us).
 // Tried: scores and P by halves of a tile, so that softmax and products of a group overlap (1,404 us: products of 64
 // columns take as long as those of 128), P alone by halves (1,041: the issuing warp waits for one group while the
-// other is ready), an issuing warp for each group (1,250).
+// other is ready), an issuing warp for each group (1,250).  Short items (7 prompts: 174 us) pay 9,000 cycles for q and
+// outputs beside some 4 tiles; q brought by bulk copies of 128 bytes took 322 us, by two warps of its own 182, before
+// the outputs of the item before it 175; outputs through shared memory 180.
 //
 // Warps: 0-3 and 4-7 softmax of the groups, a row each thread; 8-11 turn codes into f16; 12 loads (TMA); 13 issues
 // the products.  Registers are moved from the others to the softmax (setmaxnreg).  Units of 128 positions of all items
@@ -61,8 +63,7 @@ struct __align__(1024) Smem {
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
   uint64_t drained;
   int64_t scan[kThreads / 32];
-  int64_t first_unit;  // of the sequence in which the CTA's range begins
-  int first_seq;
+  int first_seq, first_unit;  // the sequence in which the CTA's range begins, its first unit
   uint32_t tmem;
 };
 
@@ -118,12 +119,12 @@ __device__ __forceinline__ int64_t units_of(const Int4AttnParams& p, const Seq& 
 // range, which ends at unit `until`.
 struct Cursor {
   int seq, rg, kvh, tile, end, tiles;
-  int64_t begin, until;  // the item's first unit
+  int begin, until;  // the item's first unit
   Seq s;
   // Whether another piece with a tile follows.
   __device__ __forceinline__ bool more() const { return begin + tiles + 2 * kPieceUnits < until; }
   __device__ __forceinline__ void set_end() {
-    end = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(tiles), until - begin - kPieceUnits)));
+    end = max(0, min(tiles, until - begin - kPieceUnits));
   }
   __device__ __forceinline__ bool whole() const { return tile == 0 && end == tiles; }
 };
@@ -490,6 +491,19 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// 32 bytes; wide: on a boundary of 32 (else of 16).
+__device__ __forceinline__ void st_global_32(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
+                                             uint32_t g, uint32_t h, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f),
+                 "r"(g), "r"(h)
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(a, b, c, d);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(e, f, g, h);
+  }
+}
+
 // Rows of a work item, every other one: row of the kv head, its token's row of q and its query head.
 struct Walk {
   int row, head, in_group;
@@ -544,7 +558,7 @@ __device__ __forceinline__ uint32_t q_piece(uint32_t q, int row, int piece) {
   return q + (piece >> 3) * kOBytes + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
 }
 
-__device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor next, const Ranges<int64_t>& ranges,
+__device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor next, const Ranges& ranges,
                                              int g, int tid) {
   const int r = tid & 127, warp = r >> 5, lane = tid & 31;
   const uint32_t s_tmem = sm.tmem + (static_cast<uint32_t>(32 * warp) << 16) + 256 * g, o_tmem = s_tmem + 128;
@@ -696,45 +710,38 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
       tc::fence_after_sync();
       const bool whole = c.whole();
       const float f = !whole ? back : m == kNone ? 0.f : __fdiv_rn(back, l);  // 0 for a row that sees nothing
-      // rows leave through the group's q, which no product reads any more, so that stores are whole lines: 256 bytes of
-      // a row at a time, 128 bf16 values or 64 fp32 ones
+      // a thread stores its row, 32 bytes at a time: whole sectors
+      const int row = c.rg * kItem + g * kRows + r, token = row / p.group;
       float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart;
+      uint8_t* dst = whole ? reinterpret_cast<uint8_t*>(p.out + (static_cast<int64_t>(c.s.q_first) + token) * p.out_row_stride +
+                                                        (c.kvh * p.group + row - token * p.group) * kHeadDim)
+                           : reinterpret_cast<uint8_t*>(part + (g * kRows + r) * kHeadDim);
+      const bool wide = __all_sync(0xffffffffu, (reinterpret_cast<uintptr_t>(dst) & 31) == 0);
 #pragma unroll 1
       for (int c0 = 0; c0 < kHeadDim; c0 += 32) {
         uint32_t v[32];
         tmem_ld32(o_tmem + c0, v);
         tc::wait_ld();
 #pragma unroll
-        for (int k = 0; k < 32; k += 8) {  // back from the order 0 4 1 5 2 6 3 7
-          const float y[8] = {__uint_as_float(v[k]) * f,     __uint_as_float(v[k + 2]) * f, __uint_as_float(v[k + 4]) * f,
-                              __uint_as_float(v[k + 6]) * f, __uint_as_float(v[k + 1]) * f, __uint_as_float(v[k + 3]) * f,
-                              __uint_as_float(v[k + 5]) * f, __uint_as_float(v[k + 7]) * f};
-          if (whole) {
-            st_shared_v4(q_piece(q, r, (c0 + k) / 8), pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
-                         pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
-          } else {
-            const int at = (c0 & 32) / 4 + k / 4;
-            st_shared_v4(q_piece(q, r, at), __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]),
-                         __float_as_uint(y[3]));
-            st_shared_v4(q_piece(q, r, at + 1), __float_as_uint(y[4]), __float_as_uint(y[5]), __float_as_uint(y[6]),
-                         __float_as_uint(y[7]));
-          }
-        }
-        if (whole ? c0 == 96 : (c0 & 32) != 0) {
-          __syncwarp();
-          Walk out(p, c, g * kRows + 32 * warp + (lane >> 4));
-#pragma unroll 4
-          for (int i = 0; i < 16; ++i) {
-            const int at = 32 * warp + 2 * i + (lane >> 4);
-            const uint4 y = ld_shared_v4(q_piece(q, at, lane & 15));
-            if (!whole) {
-              *reinterpret_cast<uint4*>(part + (g * kRows + at) * kHeadDim + (c0 & 64) + 4 * (lane & 15)) = y;
-            } else if (out.row < rows) {
-              *reinterpret_cast<uint4*>(p.out + out.token * p.out_row_stride + out.head * kHeadDim + 8 * (lane & 15)) = y;
+        for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+        if (whole) {  // back from the order 0 4 1 5 2 6 3 7
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              w[k / 2 + 2 * x] = pack_bf16x2(__uint_as_float(v[k + x]), __uint_as_float(v[k + x + 2]));
+              w[k / 2 + 2 * x + 1] = pack_bf16x2(__uint_as_float(v[k + x + 4]), __uint_as_float(v[k + x + 6]));
             }
-            out.two_on(p);
           }
-          __syncwarp();
+          if (row < rows) {
+            st_global_32(dst + 2 * c0, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], wide);
+            st_global_32(dst + 2 * c0 + 32, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15], wide);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            st_global_32(dst + 4 * (c0 + k), v[k], v[k + 2], v[k + 4], v[k + 6], v[k + 1], v[k + 3], v[k + 5], v[k + 7], wide);
         }
       }
       if (!whole) *reinterpret_cast<float2*>(part + kItem * kHeadDim + 2 * (g * kRows + r)) = make_float2(m, l);
@@ -744,7 +751,7 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
       if (tid == 0) {
         Cut cut = {};
         if (c.tile == 0 && c.end < c.tiles) {
-          const int64_t first = c.begin + kPieceUnits, last = first + c.tiles - 1;  // its tiles, as units
+          const int first = c.begin + kPieceUnits, last = first + c.tiles - 1;  // its tiles, as units
           cut.parts = ranges.owner(last) - ranges.owner(first) + 1;
           cut.slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
           cut.rows = min(kItem, rows - c.rg * kItem);
@@ -814,13 +821,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     total += sm.scan[w];
   }
   before -= mine;
-  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+  if (total > INT_MAX) {  // hours of work: what follows counts in 32 bits
+    if (tid == 0) {
+      atomicExch(p.err, kDevErrTooLarge);
+      reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
+    }
+    return;
+  }
+  const int ctas = min(static_cast<int>(gridDim.x), static_cast<int>(total));
   if (static_cast<int>(blockIdx.x) >= ctas) {
     if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
     return;
   }
-  const Ranges<int64_t> ranges(total, ctas);
-  const int64_t u0 = ranges.begin(blockIdx.x), u1 = ranges.begin(blockIdx.x + 1);
+  const Ranges ranges(static_cast<int>(total), ctas);
+  const int u0 = ranges.begin(blockIdx.x), u1 = ranges.begin(blockIdx.x + 1);
   if (before <= u0 && u0 < before + mine) {
     int64_t at = before;
     int s = s0;
@@ -830,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       at += n;
     }
     sm.first_seq = s;
-    sm.first_unit = at;
+    sm.first_unit = static_cast<int>(at);
   }
   if (warp == kMmaWarp) {
     tc::tmem_alloc(&sm.tmem, 512);
@@ -847,14 +861,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     Groups at(p, 0);
     for (c.rg = 0;; ++c.rg) {
       c.tiles = at.tiles(c.s);
-      const int64_t of_group = static_cast<int64_t>(c.tiles + kPieceUnits) * p.num_kv_heads;
+      const int of_group = (c.tiles + kPieceUnits) * p.num_kv_heads;
       if (u0 < c.begin + of_group) break;
       c.begin += of_group;
       at.next(p);
     }
-    c.kvh = static_cast<int>(u0 - c.begin) / (c.tiles + kPieceUnits);
+    c.kvh = (u0 - c.begin) / (c.tiles + kPieceUnits);
     c.begin += c.kvh * (c.tiles + kPieceUnits);
-    c.tile = max(0, static_cast<int>(u0 - c.begin) - kPieceUnits);
+    c.tile = max(0, u0 - c.begin - kPieceUnits);
     c.until = u1;
     c.set_end();
   }
