@@ -14,13 +14,13 @@
 // it: q is laid out in the same order, outputs are put back.  A row of K or V that is not finite becomes NaN in K
 // and zero in V, so that it reaches just those query rows that see it.
 //
-// Bound by the chain of a group: products of its tile (1,056 cycles: one every 66), then its softmax (about 3,200
-// beside the other group's and the unpacking), 4,200 cycles for a tile of both groups; tensor cores and issue slots are
-// half busy (2,048 new tokens of 32,768 positions, 32 heads: 941 us, 1,131 TFLOP/s).  A softmax row of 128 needs 1,024
+// Bound by the chain of a group: products of its tile (1,056 cycles: one every 66) behind the other group's, then its
+// softmax (about 2,050), 4,100 cycles for a tile of both groups; tensor cores and issue slots are half busy (2,048 new tokens of 32,768 positions, 32 heads: 910 us, 1,170 TFLOP/s).  A softmax row of 128 needs 1,024
 // cycles of the exponential unit for each group, so 1 of 4 pairs takes a polynomial instead (7 prompts: 182 to 176 us).
 // Tried: scores and P by halves of a tile, so that softmax and products of a group overlap (1,404 us: products of 64
 // columns take as long as those of 128), P alone by halves (1,041: the issuing warp waits for one group while the
-// other is ready), an issuing warp for each group (1,250).  Short items (7 prompts: 174 us) pay 9,000 cycles for q and
+// other is ready), an issuing warp for each group (1,250), the groups' blocks of products in a loop
+// (941), barriers looked at between two blocks (1,107).  Short items (7 prompts: 170 us) pay 9,000 cycles for q and
 // outputs beside some 4 tiles; q brought by bulk copies of 128 bytes took 322 us, by two warps of its own 182, before
 // the outputs of the item before it 175; outputs through shared memory 180.
 //
@@ -433,8 +433,13 @@ __device__ __forceinline__ void mma_role(const Int4AttnParams& p, Smem& sm, Curs
     for (int i = 0; i <= n && ok; ++i) {
       const int at = u + i;  // scores of this unit, values of the one before it
       const int k_buf = at & 1, v_buf = (at - 1) & 1;
-#pragma unroll 1
-      for (int g = 0; g < groups; ++g) {
+      const uint64_t v_desc = dv + static_cast<uint64_t>(v_buf * (2 * kOBytes >> 4));
+      const uint64_t k_desc = dk + static_cast<uint64_t>(k_buf * (2 * kOBytes >> 4));
+      uint64_t* const v_free = &sm.v_free[v_buf];
+      uint64_t* const k_free = &sm.k_free[k_buf];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (g >= groups) break;
         // all that the group's products wait for, and then all of them: the tensor cores run dry between two blocks
         if (g == 0) {
           if (i > 0) ok = wait_all(&sm.v_full[v_buf], static_cast<uint32_t>((at - 1) >> 1) & 1u, p.err);
@@ -449,23 +454,22 @@ __device__ __forceinline__ void mma_role(const Int4AttnParams& p, Smem& sm, Curs
         tc::fence_after_sync();
         if (elect_one()) {
           if (i > 0) {  // O_g += P_g V, 16 positions at a time: V's rows are 128 bytes
-            const uint64_t b = dv + static_cast<uint64_t>(v_buf * (2 * kOBytes >> 4));
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              tc::mma_f16_ts(tmem + 256 * g + 128, tmem + 256 * g + 8 * k, b + static_cast<uint64_t>(k * (16 * 128 >> 4)),
+              tc::mma_f16_ts(tmem + 256 * g + 128, tmem + 256 * g + 8 * k, v_desc + static_cast<uint64_t>(k * (16 * 128 >> 4)),
                              idesc_pv, i > 1 || k > 0 ? 1u : 0u);
             if (i == n) tc::commit(&sm.o_full[g]);
-            if (g == groups - 1) tc::commit(&sm.v_free[v_buf]);
+            if (g == groups - 1) tc::commit(v_free);
           }
           if (i < n) {
-            const uint64_t a = dq + static_cast<uint64_t>(g * (2 * kOBytes >> 4)), b = dk + static_cast<uint64_t>(k_buf * (2 * kOBytes >> 4));
+            const uint64_t a = dq + static_cast<uint64_t>(g * (2 * kOBytes >> 4));
 #pragma unroll
             for (int k = 0; k < 8; ++k) {  // 16 values: 32 bytes, four to a block
               const uint64_t step = static_cast<uint64_t>((k >> 2) * (kOBytes >> 4) + (k & 3) * 2);
-              mma_f16_ss(tmem + 256 * g, a + step, b + step, idesc_s, k > 0 ? 1u : 0u);
+              mma_f16_ss(tmem + 256 * g, a + step, k_desc + step, idesc_s, k > 0 ? 1u : 0u);
             }
             tc::commit(&sm.s_full[g]);
-            if (g == groups - 1) tc::commit(&sm.k_free[k_buf]);
+            if (g == groups - 1) tc::commit(k_free);
           }
         }
         __syncwarp();
