@@ -234,7 +234,8 @@ __device__ __forceinline__ void convert_q(const uint16_t* row, bool is_row, int 
     for (int b = 0; b < 2; ++b) {  // values 2 b and 2 b + 4; 2 b + 1 and 2 b + 5
       const uint32_t lo = word[b], hi = word[b + 2];
       q[2 * w + b] = make_uint2(pack_f16x2(__uint_as_float(lo << 16) * even, __uint_as_float(hi << 16) * even),
-                                pack_f16x2(__uint_as_float(lo & 0xFFFF0000u) * odd, __uint_as_float(hi & 0xFFFF0000u) * odd));
+                                pack_f16x2(__uint_as_float(lo & 0xFFFF0000u) * odd,
+                                           __uint_as_float(hi & 0xFFFF0000u) * odd));
     }
   }
   kq = pow2(e) * 16777216.f * scale_log2;  // e + 24 <= 121
@@ -332,7 +333,8 @@ __device__ __forceinline__ void load(const Int4AttnParams& p, const CUtensorMap&
 
 // The pair that the CTA's range leaves cut, if its last piece is one's beginning: for the joining kernel.
 template <typename S>
-__device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor& now, const Ranges& ranges, uint32_t pieces) {
+__device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor& now, const Ranges& ranges,
+                                          uint32_t pieces) {
   Cut cut = {};
   if (now.tile == 0 && now.end < now.s.tiles) {
     const int first = now.begin + kPieceUnits, last = first + now.s.tiles - 1;  // its tiles, as units
@@ -349,8 +351,8 @@ __device__ __forceinline__ void store_cut(const Int4AttnParams& p, const Cursor&
 // Scores, softmax and sums by four warps, which meet once for each unit: whether one of them needs new reference
 // maxima, and with it, that P is there.
 template <typename S>
-__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges& ranges,
-                                             int warp, int lane) {
+__device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cursor now, const Ranges& ranges, int warp,
+                                        int lane) {
   constexpr int NT = S::NT, R = S::R;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t k_ring = smem_u32(sm.k[0]) + (warp * kTile + g) * 64 + (t ^ (g >> 1 & 3)) * 16;
@@ -458,7 +460,8 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
           for (int j = 0; j < NT; ++j) {
             const uint64_t kq = reinterpret_cast<const uint64_t*>(sm.kq)[4 * j + t];
             const uint64_t qs = reinterpret_cast<const uint64_t*>(sm.qs)[4 * j + t];
-            const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq), f2_fma(lk2, qs, minus_m[j]));
+            const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq),
+                                      f2_fma(lk2, qs, minus_m[j]));
             f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
           }
         }
@@ -682,7 +685,8 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         if (whole) {
           const int token = token_of(p, r);
           const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);  // 0 for a row that sees nothing
-          const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0] * inv, y[1] * inv), hi = __floats2bfloat162_rn(y[2] * inv, y[3] * inv);
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0] * inv, y[1] * inv);
+          const __nv_bfloat162 hi = __floats2bfloat162_rn(y[2] * inv, y[3] * inv);
           *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(now.s.q_first) + token) * p.out_row_stride +
                                     (kvh * p.group + r - token * p.group) * kHeadDim + value) =
               make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
@@ -799,7 +803,7 @@ cudaError_t prepare() {
 }
 
 template <typename S>
-int resident(int num_sms) {  // CTAs that run at once
+int resident(int num_sms) {  // CTAs that run at once; asked before the first launch on a device, which it prepares
   int per_sm = 0;
   if (prepare<S>() != cudaSuccess ||
       cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, int4_decode_kernel<S>, kThreads, kSmemBytes<S>) !=
@@ -810,8 +814,6 @@ int resident(int num_sms) {  // CTAs that run at once
 
 template <typename S>
 cudaError_t launch(Int4AttnParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int grid, cudaStream_t stream) {
-  cudaError_t e = prepare<S>();
-  if (e != cudaSuccess) return e;
   p.unit_pages = kUnit / p.block_size;
   p.unit_rest = kUnit % p.block_size;
   p.group_inverse = static_cast<uint32_t>(((int64_t{1} << 31) + p.group - 1) / p.group);

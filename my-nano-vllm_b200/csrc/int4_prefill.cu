@@ -15,14 +15,15 @@
 // and zero in V, so that it reaches just those query rows that see it.
 //
 // Bound by the chain of a group: products of its tile (1,056 cycles: one every 66) behind the other group's, then its
-// softmax (about 2,050), 4,100 cycles for a tile of both groups; tensor cores and issue slots are half busy (2,048 new tokens of 32,768 positions, 32 heads: 910 us, 1,170 TFLOP/s).  A softmax row of 128 needs 1,024
-// cycles of the exponential unit for each group, so 1 of 4 pairs takes a polynomial instead (7 prompts: 182 to 176 us).
-// Tried: scores and P by halves of a tile, so that softmax and products of a group overlap (1,404 us: products of 64
-// columns take as long as those of 128), P alone by halves (1,041: the issuing warp waits for one group while the
-// other is ready), an issuing warp for each group (1,250), the groups' blocks of products in a loop
-// (941), barriers looked at between two blocks (1,107).  Short items (7 prompts: 170 us) pay 9,000 cycles for q and
-// outputs beside some 4 tiles; q brought by bulk copies of 128 bytes took 322 us, by two warps of its own 182, before
-// the outputs of the item before it 175; outputs through shared memory 180.
+// softmax (about 2,050), 4,100 cycles for a tile of both groups; tensor cores and issue slots are half busy (2,048 new
+// tokens of 32,768 positions, 32 heads: 910 us, 1,170 TFLOP/s).  A softmax row of 128 needs 1,024 cycles of the
+// exponential unit for each group, so 1 of 4 pairs takes a polynomial instead (7 prompts: 182 to 176 us).  Tried:
+// scores and P by halves of a tile, so that softmax and products of a group overlap (1,404 us: products of 64 columns
+// take as long as those of 128), P alone by halves (1,041: the issuing warp waits for one group while the other is
+// ready), an issuing warp for each group (1,250), the groups' blocks of products in a loop (941), barriers looked at
+// between two blocks (1,107).  Short items (7 prompts: 170 us) pay 9,000 cycles for q and outputs beside some 4 tiles;
+// q brought by bulk copies of 128 bytes took 322 us, by two warps of its own 182, before the outputs of the item before
+// it 175; outputs through shared memory 180.
 //
 // Warps: 0-3 and 4-7 softmax of the groups, a row each thread; 8-11 turn codes into f16; 12 loads (TMA); 13 issues
 // the products.  Registers are moved from the others to the softmax (setmaxnreg).  Units of 128 positions of all items
@@ -456,8 +457,8 @@ __device__ __forceinline__ void mma_role(const Int4AttnParams& p, Smem& sm, Curs
           if (i > 0) {  // O_g += P_g V, 16 positions at a time: V's rows are 128 bytes
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              tc::mma_f16_ts(tmem + 256 * g + 128, tmem + 256 * g + 8 * k, v_desc + static_cast<uint64_t>(k * (16 * 128 >> 4)),
-                             idesc_pv, i > 1 || k > 0 ? 1u : 0u);
+              tc::mma_f16_ts(tmem + 256 * g + 128, tmem + 256 * g + 8 * k,
+                             v_desc + static_cast<uint64_t>(k * (16 * 128 >> 4)), idesc_pv, i > 1 || k > 0 ? 1u : 0u);
             if (i == n) tc::commit(&sm.o_full[g]);
             if (g == groups - 1) tc::commit(v_free);
           }
@@ -499,8 +500,8 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
 __device__ __forceinline__ void st_global_32(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
                                              uint32_t g, uint32_t h, bool wide) {
   if (wide) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f),
-                 "r"(g), "r"(h)
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e),
+                 "r"(f), "r"(g), "r"(h)
                  : "memory");
   } else {
     reinterpret_cast<uint4*>(p)[0] = make_uint4(a, b, c, d);
@@ -557,7 +558,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// The 16-byte piece of a 256-byte row (of q, or of outputs on their way out) in a group's q.
+// The 16-byte piece of a 256-byte row in a group's q.
 __device__ __forceinline__ uint32_t q_piece(uint32_t q, int row, int piece) {
   return q + (piece >> 3) * kOBytes + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
 }
@@ -717,8 +718,9 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
       // a thread stores its row, 32 bytes at a time: whole sectors
       const int row = c.rg * kItem + g * kRows + r, token = row / p.group;
       float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart;
-      uint8_t* dst = whole ? reinterpret_cast<uint8_t*>(p.out + (static_cast<int64_t>(c.s.q_first) + token) * p.out_row_stride +
-                                                        (c.kvh * p.group + row - token * p.group) * kHeadDim)
+      uint16_t* const out = p.out + (static_cast<int64_t>(c.s.q_first) + token) * p.out_row_stride +
+                            (c.kvh * p.group + row - token * p.group) * kHeadDim;
+      uint8_t* dst = whole ? reinterpret_cast<uint8_t*>(out)
                            : reinterpret_cast<uint8_t*>(part + (g * kRows + r) * kHeadDim);
       const bool wide = __all_sync(0xffffffffu, (reinterpret_cast<uintptr_t>(dst) & 31) == 0);
 #pragma unroll 1
@@ -745,7 +747,8 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         } else {
 #pragma unroll
           for (int k = 0; k < 32; k += 8)
-            st_global_32(dst + 4 * (c0 + k), v[k], v[k + 2], v[k + 4], v[k + 6], v[k + 1], v[k + 3], v[k + 5], v[k + 7], wide);
+            st_global_32(dst + 4 * (c0 + k), v[k], v[k + 2], v[k + 4], v[k + 6], v[k + 1], v[k + 3], v[k + 5], v[k + 7],
+                         wide);
         }
       }
       if (!whole) *reinterpret_cast<float2*>(part + kItem * kHeadDim + 2 * (g * kRows + r)) = make_float2(m, l);
