@@ -10,10 +10,10 @@
 // into q and into the outputs.  q is exact in f16 after a power-of-two scale per row.
 //
 // Bound by HBM up to 8 rows: 136 bytes of K and V for each position and kv head, read once for all of the rows of
-// its query heads (64 sequences of 32,768, 8 rows: 392 us, 0.89 of the floor at 6.55 TB/s; 4 rows: 390 us).  Above,
+// its query heads (64 sequences of 32,768, 8 rows: 396 us, 0.88 of the floor at 6.55 TB/s; 4 rows: 390 us).  Above,
 // by the tensor cores of mma.sync: 34 products of 8 cycles for each 32 positions and plane of 8 rows, which fp32
 // arithmetic does not overlap (8 fma beside one product: 14.9 cycles, and 8 without it), against 186 cycles of
-// HBM: 16 rows 536 us, 24 rows 724, 32 rows 955.
+// HBM: 16 rows 549 us, 24 rows 759, 32 rows 963.
 //
 // Work: a unit is 128 positions of one (sequence, row group, kv head), and a warp computes S^T = K q^T and P of 32 of
 // them (A = codes, 16 positions x 16 values).  P goes through shared memory (stmatrix turns it), and of all 128
@@ -27,11 +27,12 @@
 // and across the ends of pieces.
 //
 // c - 7.5 is the product with c and 7.5 times the same product with ones: taken about the middle of the codes, the
-// roundings of P and the cuts of the tensor cores' sums (2^-24 of each partial sum, all one way: 2e-5 of the sum
-// after 512 of them) are in proportion to the values and not to their distance from the row's lowest one.  So the
-// product with ones is taken for all 128 positions one after another, as the others are, a plane by one warp
-// (32,768 positions: 1.7e-3 off in the 2-norm, all but the output's own rounding; 5.3e-3 when each warp took the
-// ones of its own 32 positions, 2.1e-3 without the middle and with a quarter of the sums).
+// roundings of P and the cuts of the tensor cores' sums (2^-24 of each partial sum, all one way) are in proportion to
+// the values and not to their distance from the row's lowest one.  A warp takes the ones of its own 32 positions, so
+// their cuts are not those of the other products; every 64 units the sums so far are put aside and later added with
+// rounding to nearest, so that the cuts do not grow with the context (32,768 positions: 1.8e-3 off in the 2-norm, all
+// but the output's own rounding; 5.3e-3 without that, 2.4e-3 and 1 % slower with the ones of all positions in one warp).
+// The loop over units stays as it is: a branch in it cost 5 %.
 //
 // Precision: scores, statistics and sums in fp32; P is rounded once, to f16 (2^-12), after its row's
 // reference maximum and a power of two near the largest step of V are taken out, so it stays below 2^14.
@@ -50,6 +51,7 @@ __device__ int g_error = 0;
 constexpr int kTile = 32;               // positions of a unit whose scores a warp computes
 constexpr float kSlack = 8.f;           // a reference maximum may lag by 2^8
 constexpr int kPieceUnits = 1;          // what a pair costs beside its tiles, in units of a tile
+constexpr int kFlush = 64;              // units whose products with V the tensor cores add up
 
 constexpr int kWarps = 4;                    // that compute; one more loads
 constexpr int kThreads = kWarps * 32 + 32;
@@ -57,14 +59,14 @@ constexpr int kUnit = kTile * kWarps;        // positions per unit
 constexpr int kParts = kUnit / 16;           // parts of a unit that lie in one page each
 
 // A kernel by the rows of a group: NT planes of 8.  As many CTAs on an SM as have room for their sums without spilling
-// (24 rows: three CTAs of 128 registers 724 us, two of 168 754; 8 rows: four with two stages 393 us, three with three
-// 382, both before the ones' products were taken in full).
+// (verification with 20 rows: three CTAs of 128 registers 217 us, two of 168 209; 8 rows, at an earlier step: four with
+// two stages 393 us, three with three 382).
 template <int NT_>
 struct Shape {
   static constexpr int NT = NT_;
   static constexpr int R = 8 * NT;
-  static constexpr int kCtas = NT < 4 ? 3 : 2;    // on an SM
-  static constexpr int kStages = NT == 3 ? 2 : 3;
+  static constexpr int kCtas = NT < 3 ? 3 : 2;    // on an SM
+  static constexpr int kStages = 3;
 };
 
 constexpr int kPPitch = kUnit + 8;  // bank spread
@@ -79,7 +81,7 @@ struct __align__(1024) Smem {
   uint16_t p[2][S::R][kPPitch];             // P step, f16, of this unit and the one before
   float kq[S::R], qs[S::R];                 // score = dot kq step + qs low
   float top[kWarps][S::R], top_v[kWarps];   // of the warps' positions: largest score and step,
-  float l[kWarps][S::R], mid[kWarps][S::R], ps[S::R];  // sums
+  float l[kWarps][S::R], mid[kWarps][S::R], ps[kWarps][S::R];  // sums
   uint64_t full[S::kStages], empty[S::kStages], q_full, q_free;
   uint32_t there[S::kStages];  // which parts of the stage's unit are in pages of the cache
   int scan[kThreads / 32];
@@ -392,7 +394,9 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
 
-    float o[NT][2][4], ps[4] = {};         // ps: sums of the rounded P step of plane `warp`
+    float o[NT][2][4], ps[NT][4];          // ps: sum of the rounded P step, of this warp's positions
+    volatile float kept[10 * NT], m_kept[2 * NT];  // o and ps of the units before, and their m: in local memory
+    volatile int v_kept;
     uint64_t minus_m[NT], l[NT], mid[NT];  // pairs of columns
     uint32_t unset = (1u << 2 * NT) - 1;   // columns that have seen nothing: their m counts as 0
     float limit = -INFINITY;               // how far a score may be above its m: kSlack when none is unset
@@ -402,237 +406,276 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
     for (int j = 0; j < NT; ++j) {
       minus_m[j] = l[j] = mid[j] = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[j][0][c] = o[j][1][c] = 0.f;
+      for (int c = 0; c < 4; ++c) ps[j][c] = o[j][0][c] = o[j][1][c] = 0.f;
     }
+    auto add_kept = [&]() {
+      const float change = pow2(max(-126, min(v_kept - v_exp, 0)));  // V's power of two only grows
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float m[2];
+        f2_unpack(minus_m[j], m[0], m[1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float f = ex2(m[c] - m_kept[2 * j + c]) * change;
+          auto add = [&](float& x, float y) { x += y == 0.f ? 0.f : y * f; };  // 0 where nothing had been seen
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            add(o[j][b][c], kept[8 * j + 4 * b + c]);
+            add(o[j][b][2 + c], kept[8 * j + 4 * b + 2 + c]);
+          }
+          add(ps[j][c], kept[8 * NT + 2 * j + c]);
+        }
+      }
+    };
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      const int pos0 = (now.tile + i) * kUnit + warp * kTile;
-      ok = ok && wait_all(&sm.full[stage], parity, p.err);
-      const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
-      // ---- S^T: positions (rows g, g + 8 of each half) x query rows (columns)
-      float s[2][NT][4];
-      uint32_t kw[2][2][4];  // half, row g or g + 8, word
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
-          kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          uint32_t a[2][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t y0 = kw[h][0][w] >> (8 * b);
-            const uint32_t y1 = kw[h][1][w] >> (8 * b);
-            a[h][0] = y0 & 0x000F000Fu;
-            a[h][1] = y1 & 0x000F000Fu;
-            a[h][2] = y0 & 0x00F000F0u;
-            a[h][3] = y1 & 0x00F000F0u;
-          }
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const uint2 y = sm.q[j][2 * w + b][lane];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (w == 0 && b == 0) mma16816_first(s[h][j], a[h], y.x, y.y);
-              else mma16816(s[h][j], a[h], y.x, y.y);
-            }
-          }
-        }
-      }
-      // ---- scores above their m; this thread's positions: rows g and g + 8 of half h
-      float sv[2][2], mv[2][2];  // step of V, and what code 7.5 stands for
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + h * 128 + r * 64);
-          const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
-          sv[h][r] = __uint_as_float(sc.y << 16);
-          mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
-          const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const uint64_t kq = reinterpret_cast<const uint64_t*>(sm.kq)[4 * j + t];
-            const uint64_t qs = reinterpret_cast<const uint64_t*>(sm.qs)[4 * j + t];
-            const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq),
-                                      f2_fma(lk2, qs, minus_m[j]));
-            f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
-          }
-        }
-      }
-      if (halves != 3u || pos0 + kTile > least) {
-        int sees[NT][2];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          sees[j][0] = limit_of(j, 0);
-          sees[j][1] = limit_of(j, 1);
-        }
+    for (int i = 0; i < n;) {
+#pragma unroll 1
+      for (const int stop = min(n, (i / kFlush + 1) * kFlush); i < stop; ++i) {
+        const int pos0 = (now.tile + i) * kUnit + warp * kTile;
+        ok = ok && wait_all(&sm.full[stage], parity, p.err);
+        const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
+        // ---- S^T: positions (rows g, g + 8 of each half) x query rows (columns)
+        float s[2][NT][4];
+        uint32_t kw[2][2][4];  // half, row g or g + 8, word
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int pos = pos0 + 16 * h + g + 8 * r;
-            const bool held = (halves >> h & 1u) && pos < now.s.vis;
-            // a row of V that is no number goes to those that see it by their scores
-            const bool number = fabsf(mv[h][r]) < INFINITY;
-            if (!held || !number) sv[h][r] = mv[h][r] = 0.f;
+            const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
+            kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            uint32_t a[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t y0 = kw[h][0][w] >> (8 * b);
+              const uint32_t y1 = kw[h][1][w] >> (8 * b);
+              a[h][0] = y0 & 0x000F000Fu;
+              a[h][1] = y1 & 0x000F000Fu;
+              a[h][2] = y0 & 0x00F000F0u;
+              a[h][3] = y1 & 0x00F000F0u;
+            }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
+              const uint2 y = sm.q[j][2 * w + b][lane];
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                if (!number) s[h][j][2 * r + c] = NAN;
-                if (!held || pos >= sees[j][c]) s[h][j][2 * r + c] = -INFINITY;
+              for (int h = 0; h < 2; ++h) {
+                if (w == 0 && b == 0) mma16816_first(s[h][j], a[h], y.x, y.y);
+                else mma16816(s[h][j], a[h], y.x, y.y);
               }
             }
           }
         }
-      }
-      bool grow = false;
+        // ---- scores above their m; this thread's positions: rows g and g + 8 of half h
+        float sv[2][2], mv[2][2];  // step of V, and what code 7.5 stands for
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        grow |= fmaxf(sv[h][0], sv[h][1]) > v_limit;
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          grow |= fmaxf(fmaxf(s[h][j][0], s[h][j][1]), fmaxf(s[h][j][2], s[h][j][3])) > limit;
-      }
-      // ---- P, and P step_v to shared memory: [row][position]
-      const uint32_t p_at = p_lane + p_buf * (R * kPPitch * 2);
-      uint64_t l_now[NT], mid_now[NT];
-      auto give_p = [&]() {
+          for (int r = 0; r < 2; ++r) {
+            const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + h * 128 + r * 64);
+            const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
+            sv[h][r] = __uint_as_float(sc.y << 16);
+            mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
+            const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          uint32_t x[2][2];
-          l_now[j] = l[j];
-          mid_now[j] = mid[j];
+            for (int j = 0; j < NT; ++j) {
+              const uint64_t kq = reinterpret_cast<const uint64_t*>(sm.kq)[4 * j + t];
+              const uint64_t qs = reinterpret_cast<const uint64_t*>(sm.qs)[4 * j + t];
+              const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq),
+                                        f2_fma(lk2, qs, minus_m[j]));
+              f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
+            }
+          }
+        }
+        if (halves != 3u || pos0 + kTile > least) {
+          int sees[NT][2];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            sees[j][0] = limit_of(j, 0);
+            sees[j][1] = limit_of(j, 1);
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const uint64_t e = f2_pack(ex2(s[h][j][2 * r]), ex2(s[h][j][2 * r + 1]));
-              const float f = sv[h][r] * v_unit;
-              l_now[j] = f2_add(l_now[j], e);
-              mid_now[j] = f2_fma(e, f2_pack(mv[h][r], mv[h][r]), mid_now[j]);
-              float p0, p1;
-              f2_unpack(f2_mul(e, f2_pack(f, f)), p0, p1);
-              x[h][r] = pack_f16x2(p0, p1);
+              const int pos = pos0 + 16 * h + g + 8 * r;
+              const bool held = (halves >> h & 1u) && pos < now.s.vis;
+              // a row of V that is no number goes to those that see it by their scores
+              const bool number = fabsf(mv[h][r]) < INFINITY;
+              if (!held || !number) sv[h][r] = mv[h][r] = 0.f;
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  if (!number) s[h][j][2 * r + c] = NAN;
+                  if (!held || pos >= sees[j][c]) s[h][j][2 * r + c] = -INFINITY;
+                }
+              }
             }
           }
-          stmatrix_trans(p_at + (8 * j * kPPitch + warp * kTile) * 2, x[0][0], x[0][1], x[1][0], x[1][1]);
         }
-      };
-      give_p();
-      if (any_warp(grow)) {
-        // ---- new references, of the CTA: the rows' maxima so far, and a power of two near V's largest step
-        float top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        if (lane == 0) sm.top_v[warp] = top;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(fmaxf(s[0][j][c], s[0][j][2 + c]), fmaxf(s[1][j][c], s[1][j][2 + c]));
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            if (g == 0) sm.top[warp][8 * j + 2 * t + c] = mx;
-          }
-        }
-        all_warps();
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.top_v[w]);
-        float change = 1.f;
-        if (top > v_limit && top < INFINITY) {
-          const int x = max(-120, min(exponent(top), 120));
-          if (v_limit > 0.f) {
-            const int d = v_exp - x;
-            change = d < -126 ? 0.f : pow2(d);
-          }
-          v_exp = x;
-          v_unit = pow2(-x);
-          v_limit = pow2(min(x + 6, 127));
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          float was[2], now_m[2], f[2];
-          f2_unpack(minus_m[j], was[0], was[1]);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float mx = -INFINITY;  // above m
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.top[w][8 * j + 2 * t + c]);
-            const bool first = unset >> (2 * j + c) & 1u;
-            if (first && mx == -INFINITY) mx = 0.f;  // still unset
-            else unset &= ~(1u << (2 * j + c));
-            if (!first) mx = fmaxf(mx, 0.f);
-            f[c] = first ? 0.f : ex2(-mx);
-            now_m[c] = was[c] - mx;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              s[h][j][c] -= mx;
-              s[h][j][2 + c] -= mx;
-            }
-            if (j == warp) ps[c] *= f[c] * change;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              o[j][b][c] *= f[c] * change;
-              o[j][b][2 + c] *= f[c] * change;
-            }
-          }
-          minus_m[j] = f2_pack(now_m[0], now_m[1]);
-          l[j] = f2_mul(l[j], f2_pack(f[0], f[1]));
-          mid[j] = f2_mul(mid[j], f2_pack(f[0], f[1]));
-        }
-        limit = __any_sync(0xffffffffu, unset != 0) ? -INFINITY : kSlack;
-        give_p();
-        all_warps();
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        l[j] = l_now[j];
-        mid[j] = mid_now[j];
-      }
-      // ---- sums of P step_v of a plane, in the order and number of products of O
-      if (warp < NT) {
-        constexpr uint32_t kOne = 0x3C003C00u;
-        const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
-#pragma unroll
-        for (int x = 0; x < kUnit / 32; ++x) {
-          uint32_t b[4];
-          ldmatrix(b, p_at + (8 * warp * kPPitch + x * 32) * 2);
-          mma16816(ps, ones, b[0], b[1]);
-          mma16816(ps, ones, b[2], b[3]);
-        }
-      }
-      // ---- O^T += V^T P^T: of its 32 values 4 g + 2 b (rows g) and 4 g + 2 b + 1 (rows g + 8, codes four bits higher)
-#pragma unroll
-      for (int x = 0; x < kUnit / 32; ++x) {
-        uint32_t v[4], pb[NT][4];  // of 8 positions each
-        ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + x * 2048);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) ldmatrix(pb[j], p_at + (8 * j * kPPitch + x * 32) * 2);
+        bool grow = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          grow |= fmaxf(sv[h][0], sv[h][1]) > v_limit;
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t y0 = v[2 * h] >> (8 * b), y1 = v[2 * h + 1] >> (8 * b);
-            const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
+          for (int j = 0; j < NT; ++j)
+            grow |= fmaxf(fmaxf(s[h][j][0], s[h][j][1]), fmaxf(s[h][j][2], s[h][j][3])) > limit;
+        }
+        // ---- P, and P step_v to shared memory: [row][position]
+        const uint32_t p_at = p_lane + p_buf * (R * kPPitch * 2);
+        uint64_t l_now[NT], mid_now[NT];
+        auto give_p = [&]() {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma16816(o[j][b], a, pb[j][2 * h], pb[j][2 * h + 1]);
+          for (int j = 0; j < NT; ++j) {
+            uint32_t x[2][2];
+            l_now[j] = l[j];
+            mid_now[j] = mid[j];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const uint64_t e = f2_pack(ex2(s[h][j][2 * r]), ex2(s[h][j][2 * r + 1]));
+                const float f = sv[h][r] * v_unit;
+                l_now[j] = f2_add(l_now[j], e);
+                mid_now[j] = f2_fma(e, f2_pack(mv[h][r], mv[h][r]), mid_now[j]);
+                float p0, p1;
+                f2_unpack(f2_mul(e, f2_pack(f, f)), p0, p1);
+                x[h][r] = pack_f16x2(p0, p1);
+              }
+            }
+            stmatrix_trans(p_at + (8 * j * kPPitch + warp * kTile) * 2, x[0][0], x[0][1], x[1][0], x[1][1]);
+          }
+        };
+        give_p();
+        if (any_warp(grow)) {
+          // ---- new references, of the CTA: the rows' maxima so far, and a power of two near V's largest step
+          float top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          if (lane == 0) sm.top_v[warp] = top;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = fmaxf(fmaxf(s[0][j][c], s[0][j][2 + c]), fmaxf(s[1][j][c], s[1][j][2 + c]));
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              if (g == 0) sm.top[warp][8 * j + 2 * t + c] = mx;
+            }
+          }
+          all_warps();
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.top_v[w]);
+          float change = 1.f;
+          if (top > v_limit && top < INFINITY) {
+            const int x = max(-120, min(exponent(top), 120));
+            if (v_limit > 0.f) {
+              const int d = v_exp - x;
+              change = d < -126 ? 0.f : pow2(d);
+            }
+            v_exp = x;
+            v_unit = pow2(-x);
+            v_limit = pow2(min(x + 6, 127));
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            float was[2], now_m[2], f[2];
+            f2_unpack(minus_m[j], was[0], was[1]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = -INFINITY;  // above m
+#pragma unroll
+              for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.top[w][8 * j + 2 * t + c]);
+              const bool first = unset >> (2 * j + c) & 1u;
+              if (first && mx == -INFINITY) mx = 0.f;  // still unset
+              else unset &= ~(1u << (2 * j + c));
+              if (!first) mx = fmaxf(mx, 0.f);
+              f[c] = first ? 0.f : ex2(-mx);
+              now_m[c] = was[c] - mx;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                s[h][j][c] -= mx;
+                s[h][j][2 + c] -= mx;
+              }
+              ps[j][c] *= f[c] * change;
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                o[j][b][c] *= f[c] * change;
+                o[j][b][2 + c] *= f[c] * change;
+              }
+            }
+            minus_m[j] = f2_pack(now_m[0], now_m[1]);
+            l[j] = f2_mul(l[j], f2_pack(f[0], f[1]));
+            mid[j] = f2_mul(mid[j], f2_pack(f[0], f[1]));
+          }
+          limit = __any_sync(0xffffffffu, unset != 0) ? -INFINITY : kSlack;
+          give_p();
+          all_warps();
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          l[j] = l_now[j];
+          mid[j] = mid_now[j];
+        }
+        // ---- sums of P step_v: of this warp's positions
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          constexpr uint32_t kOne = 0x3C003C00u;
+          const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+          uint32_t b[4];
+          ldmatrix(b, p_at + (8 * j * kPPitch + warp * kTile) * 2);
+          mma16816(ps[j], ones, b[0], b[1]);
+          mma16816(ps[j], ones, b[2], b[3]);
+        }
+        // ---- O^T += V^T P^T: of its 32 values 4 g + 2 b (rows g) and 4 g + 2 b + 1 (rows g + 8, codes four bits higher)
+#pragma unroll
+        for (int x = 0; x < kUnit / 32; ++x) {
+          uint32_t v[4], pb[NT][4];  // of 8 positions each
+          ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + x * 2048);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) ldmatrix(pb[j], p_at + (8 * j * kPPitch + x * 32) * 2);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const uint32_t y0 = v[2 * h] >> (8 * b), y1 = v[2 * h + 1] >> (8 * b);
+              const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
+#pragma unroll
+              for (int j = 0; j < NT; ++j) mma16816(o[j][b], a, pb[j][2 * h], pb[j][2 * h + 1]);
+            }
           }
         }
+        p_buf ^= 1u;
+        __syncwarp();  // every lane has read the stage
+        if (lane == 0) mbar_arrive(&sm.empty[stage]);
+        if (++stage == S::kStages) {
+          stage = 0;
+          parity ^= 1u;
+        }
       }
-      p_buf ^= 1u;
-      __syncwarp();  // every lane has read the stage
-      if (lane == 0) mbar_arrive(&sm.empty[stage]);
-      if (++stage == S::kStages) {
-        stage = 0;
-        parity ^= 1u;
+      // ---- the sums so far, rounded to nearest: the tensor cores' cuts, all one way, stay those of kFlush units
+      if (i > kFlush) add_kept();
+      if (i < n) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float m[2];
+          f2_unpack(minus_m[j], m[0], m[1]);
+          m_kept[2 * j] = m[0];
+          m_kept[2 * j + 1] = m[1];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            kept[8 * j + c] = o[j][0][c];
+            kept[8 * j + 4 + c] = o[j][1][c];
+            if (c < 2) kept[8 * NT + 2 * j + c] = ps[j][c];
+            ps[j][c] = o[j][0][c] = o[j][1][c] = 0.f;
+          }
+        }
+        v_kept = v_exp;
       }
     }
 
@@ -652,7 +695,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         if (g == 0) {
           sm.l[warp][8 * j + 2 * t + c] = sum[c];
           sm.mid[warp][8 * j + 2 * t + c] = middle[c];
-          if (j == warp) sm.ps[8 * j + 2 * t + c] = ps[c];
+          sm.ps[warp][8 * j + 2 * t + c] = ps[j][c];
         }
       }
     }
@@ -667,12 +710,12 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int column = 8 * j + 2 * t + c, r = rg * R + column;
-        float sum = 0.f, middle = 0.f;
-        const float steps = sm.ps[column];
+        float sum = 0.f, middle = 0.f, steps = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           sum += sm.l[w][column];
           middle += sm.mid[w][column];
+          steps += sm.ps[w][column];
         }
         float y[4];  // values 4 g .. 4 g + 3 of the warp's
 #pragma unroll

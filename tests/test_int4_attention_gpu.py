@@ -306,6 +306,36 @@ def test_chunk_cut_over_ctas(news, lens, spread):
     _check_chunk(_q(sum(news), 4, 51), cache, table, news, lens)
 
 
+@pytest.mark.parametrize("new", [1, 2, 5])
+def test_long_pieces(new):
+    """So much work that a CTA has thousands of positions of a pair: sums put aside on the way, where a row has seen
+    nothing yet, where its maximum and V's largest step come after that."""
+    from nanovllm_b200.int4_cache import int4_decode_attention, int4_prefill_attention
+    seqs, n, block, kv, heads = 40, 20000, 64, 8, 32
+    pages = -(-n // block)
+    cache = _cache(3 * pages, block, kv, 71)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(seqs, 1)  # all but two share their pages
+    table[3] += pages
+    table[5] += 2 * pages
+    table[3, :170] = -1                                      # sees nothing in its first 10,880 positions
+    cache[2][2 * pages + 180:, :, :, 2:] *= 2.0 ** 12        # V's steps and lowest values grow late
+    q = _q(seqs * new, heads, 72)
+    late = int(table[5, 250])
+    for h in range(kv):                                      # and the rows' maxima
+        code, step, low = int4.quantise((q[5 * new, 4 * h].float() * 1.5).to(torch.bfloat16))
+        cache[0][late, h, 7] = int4.pack(code)
+        cache[2][late, h, 7, 0], cache[2][late, h, 7, 1] = step, low
+    cum = lambda m: torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * m  # noqa: E731
+    if new == 1:
+        out = int4_decode_attention(q, *cache, table, torch.full((seqs,), n, dtype=torch.int32, device="cuda"), SCALE)
+    else:
+        out = int4_prefill_attention(q, *cache, table, cum(new), cum(n), new, n, SCALE)
+    for i in (0, 3, 5, 17, seqs - 1):
+        at = slice(i * new, (i + 1) * new)
+        ref, bound = int4.attention(q[at], *cache, table[i], n, SCALE)
+        _assert_near(out[at], ref, bound, f"sequence {i}")
+
+
 def test_chunk_many_sequences():
     g = torch.Generator().manual_seed(52)
     news = torch.randint(0, 4, (600,), generator=g).tolist()
