@@ -49,7 +49,8 @@ def _check(got, x, positions, table, interleaved):
 @pytest.mark.parametrize("n,heads,kv,d,r", [(1, 32, 8, 128, 128), (7, 3, 1, 128, 64), (300, 40, 8, 128, 128),
                                             (5, 4, 4, 80, 80), (6, 2, 2, 80, 32), (9, 5, 1, 64, 20),
                                             (4, 2, 1, 96, 90), (3, 1, 1, 2, 2), (11, 7, 7, 192, 64),
-                                            (2, 16, 16, 256, 256), (2000, 9, 2, 128, 96), (3, 2, 1, 6, 4)])
+                                            (2, 16, 16, 256, 256), (2000, 9, 2, 128, 96), (3, 2, 1, 6, 4),
+                                            (900, 9, 2, 80, 34), (800, 10, 1, 96, 44)])
 def test_against_definition(n, heads, kv, d, r, interleaved, dtype):
     from nanovllm_b200.rope import apply_rope
     q, k = _randn((n, heads, d), n, dtype), _randn((n, kv, d), n + 1, dtype)
