@@ -725,11 +725,13 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         }
         if (r >= rows || !ok) continue;
         const int value = 32 * warp + 4 * g;
+        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);  // 0 for a row that sees nothing
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] *= inv;
         if (whole) {
           const int token = token_of(p, r);
-          const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);  // 0 for a row that sees nothing
-          const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0] * inv, y[1] * inv);
-          const __nv_bfloat162 hi = __floats2bfloat162_rn(y[2] * inv, y[3] * inv);
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]);
+          const __nv_bfloat162 hi = __floats2bfloat162_rn(y[2], y[3]);
           *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(now.s.q_first) + token) * p.out_row_stride +
                                     (kvh * p.group + r - token * p.group) * kHeadDim + value) =
               make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));

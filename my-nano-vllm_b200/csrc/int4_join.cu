@@ -1,8 +1,9 @@
 // Joins the parts of row groups that the 4-bit attention kernels' even cuts left in several CTAs.
 //
-// Part c has sums O_c, l_c of its positions for the reference maximum m_c; with M = max m_c
-//   out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c,
-// added in the order of the parts.  CTA i takes what the cut of CTA i says.  Bound by latency (descriptor, maxima, sums,
+// Part c has the output o_c of its own positions, and their sum l_c for the reference maximum m_c; with M = max m_c
+//   out = sum_c w_c o_c,  w_c = 2^(m_c - M) l_c / sum_d 2^(m_d - M) l_d,
+// added in the order of the parts.  Means weighted by 0 .. 1 stay inside fp32 wherever the values do; sums of p v
+// times a part's l would not.  CTA i takes what the cut of CTA i says.  Bound by latency (descriptor, maxima, sums,
 // output: three dependent accesses of L2), so few rows with many parts are shared by up to four CTAs and their warps,
 // with eight parts of a warp in flight, and many rows with few parts go four to a warp (4 rows of 55 parts: 2 us; one
 // CTA for a pair, maxima first: 6).
@@ -15,19 +16,18 @@ constexpr int kWarps = 8;
 constexpr int kFewBlocks = 4;  // CTAs that share the rows of a cut
 constexpr int kAtOnce = 8;  // parts of which a warp has the loads in flight
 
-__device__ __forceinline__ void add_part(float4& y, float& sum, const float4& x, float l, float f) {
-  y.x = fmaf(x.x, f, y.x);
-  y.y = fmaf(x.y, f, y.y);
-  y.z = fmaf(x.z, f, y.z);
-  y.w = fmaf(x.w, f, y.w);
-  sum = fmaf(l, f, sum);
+__device__ __forceinline__ void add_part(float4& y, const float4& x, float w) {
+  y.x = fmaf(x.x, w, y.x);
+  y.y = fmaf(x.y, w, y.y);
+  y.z = fmaf(x.z, w, y.z);
+  y.w = fmaf(x.w, w, y.w);
 }
 
-__device__ __forceinline__ void store_row(const Int4AttnParams& p, const Cut& cut, int row, int lane, const float4& y,
-                                          float sum) {
-  const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : __fdiv_rn(1.f, sum); }
+
+__device__ __forceinline__ void store_row(const Int4AttnParams& p, const Cut& cut, int row, int lane, const float4& y) {
   const int r = cut.first_row + row, token = r / p.group;
-  const __nv_bfloat162 a = __floats2bfloat162_rn(y.x * inv, y.y * inv), b = __floats2bfloat162_rn(y.z * inv, y.w * inv);
+  const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
   *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(cut.token) + token) * p.out_row_stride +
                             (cut.head + r - token * p.group) * kHeadDim + 4 * lane) =
       make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
@@ -71,14 +71,16 @@ __device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4Join
       const float was = mx;
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) mx = fmaxf(mx, ml[i].x);
-      const float f = ex2(was - mx);
-      const float4 old = y;
-      const float old_sum = sum;
-      y = make_float4(0.f, 0.f, 0.f, 0.f);
-      sum = 0.f;
-      add_part(y, sum, old, old_sum, f);
+      const float before = sum * ex2(was - mx);
+      sum = before;
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) add_part(y, sum, x[i], ml[i].y, ex2(ml[i].x - mx));
+      for (int i = 0; i < kAtOnce; ++i) sum += ml[i].y *= ex2(ml[i].x - mx);
+      const float inv = inverse(sum);
+      const float4 old = y;
+      y = make_float4(0.f, 0.f, 0.f, 0.f);
+      add_part(y, old, before * inv);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) add_part(y, x[i], ml[i].y * inv);
     }
     if (share > 1) {
       __syncthreads();  // the rows before these have been read
@@ -90,11 +92,13 @@ __device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4Join
         for (int w = 0; w < share; ++w) top = fmaxf(top, sum_ml[warp + w].x);
         y = make_float4(0.f, 0.f, 0.f, 0.f);
         sum = 0.f;
+        for (int w = 0; w < share; ++w) sum = fmaf(sum_ml[warp + w].y, ex2(sum_ml[warp + w].x - top), sum);
+        const float inv = inverse(sum);
         for (int w = 0; w < share; ++w)
-          add_part(y, sum, sum_o[warp + w][lane], sum_ml[warp + w].y, ex2(sum_ml[warp + w].x - top));
+          add_part(y, sum_o[warp + w][lane], sum_ml[warp + w].y * ex2(sum_ml[warp + w].x - top) * inv);
       }
     }
-    if (mine && turn == 0) store_row(p, cut, row, lane, y, sum);
+    if (mine && turn == 0) store_row(p, cut, row, lane, y);
   }
 }
 
@@ -109,7 +113,7 @@ __device__ __forceinline__ void join_many(const Int4AttnParams& p, const Int4Joi
   const float* later = list.partials + static_cast<int64_t>(2 * index) * part_size;
   auto part = [&](int j) { return j == 0 ? first : later + static_cast<int64_t>(2 * j) * part_size; };
   const int ml_at = list.rows * kHeadDim + 2 * row0;
-  float mx[4] = {kNone, kNone, kNone, kNone}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+  float mx[4] = {kNone, kNone, kNone, kNone}, inv[4] = {0.f, 0.f, 0.f, 0.f};
   for (int j = lane; j < parts; j += 32) {
     const float4 a = *reinterpret_cast<const float4*>(part(j) + ml_at);  // (m, l) of two rows
     const float4 b = *reinterpret_cast<const float4*>(part(j) + ml_at + 4);
@@ -122,6 +126,20 @@ __device__ __forceinline__ void join_many(const Int4AttnParams& p, const Int4Joi
   for (int off = 16; off > 0; off >>= 1)
 #pragma unroll
     for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], off));
+  for (int j = lane; j < parts; j += 32) {
+    const float4 a = *reinterpret_cast<const float4*>(part(j) + ml_at);
+    const float4 b = *reinterpret_cast<const float4*>(part(j) + ml_at + 4);
+    inv[0] = fmaf(a.y, ex2(a.x - mx[0]), inv[0]);
+    inv[1] = fmaf(a.w, ex2(a.z - mx[1]), inv[1]);
+    inv[2] = fmaf(b.y, ex2(b.x - mx[2]), inv[2]);
+    inv[3] = fmaf(b.w, ex2(b.z - mx[3]), inv[3]);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) inv[k] += __shfl_xor_sync(0xffffffffu, inv[k], off);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) inv[k] = inverse(inv[k]);
   float4 y[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -132,14 +150,14 @@ __device__ __forceinline__ void join_many(const Int4AttnParams& p, const Int4Joi
     float4 x[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(part(j) + (row0 + k) * kHeadDim + 4 * lane);
-    add_part(y[0], sum[0], x[0], a.y, ex2(a.x - mx[0]));
-    add_part(y[1], sum[1], x[1], a.w, ex2(a.z - mx[1]));
-    add_part(y[2], sum[2], x[2], b.y, ex2(b.x - mx[2]));
-    add_part(y[3], sum[3], x[3], b.w, ex2(b.z - mx[3]));
+    add_part(y[0], x[0], a.y * ex2(a.x - mx[0]) * inv[0]);
+    add_part(y[1], x[1], a.w * ex2(a.z - mx[1]) * inv[1]);
+    add_part(y[2], x[2], b.y * ex2(b.x - mx[2]) * inv[2]);
+    add_part(y[3], x[3], b.w * ex2(b.z - mx[3]) * inv[3]);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (row0 + k < cut.rows) store_row(p, cut, row0 + k, lane, y[k], sum[k]);
+    if (row0 + k < cut.rows) store_row(p, cut, row0 + k, lane, y[k]);
 }
 
 // CTAs [0, few.ctas * few.blocks) join the cuts of the kernel for few rows, the others those of the kernel for long

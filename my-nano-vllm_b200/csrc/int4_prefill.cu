@@ -714,7 +714,7 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
       o_parity ^= 1u;
       tc::fence_after_sync();
       const bool whole = c.whole();
-      const float f = !whole ? back : m == kNone ? 0.f : __fdiv_rn(back, l);  // 0 for a row that sees nothing
+      const float f = m == kNone ? 0.f : __fdiv_rn(back, l);  // 0 for a row that sees nothing
       // a thread stores its row, 32 bytes at a time: whole sectors
       const int row = c.rg * kItem + g * kRows + r, token = row / p.group;
       float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart;
@@ -751,7 +751,8 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
                          wide);
         }
       }
-      if (!whole) *reinterpret_cast<float2*>(part + kItem * kHeadDim + 2 * (g * kRows + r)) = make_float2(m, l);
+      if (!whole)
+        *reinterpret_cast<float2*>(part + kItem * kHeadDim + 2 * (g * kRows + r)) = make_float2(m, m == kNone ? 0.f : l);
       tc::fence_before_sync();  // O has been read before the next piece's first P is announced
     }
     if (!more) {

@@ -115,3 +115,45 @@ def attention(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale, in_f16=Fa
         bound[:, h] += (2 * e + 2.0 ** -13) * whole + 2.0 ** -11 * coded + 2.0 ** -21 * vsg.max() * p.sum(-1, keepdim=True)
         out[~some, h] = 0
     return out, bound
+
+
+def attention_norm(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale):
+    """q [nq, heads, 128] as ``attention``'s: (out float64, room float64 [nq, heads]), what an output row of 128 may be off by
+    in the 2-norm.  ``attention``'s bound holds for each value whatever the signs of the errors; this one counts them as
+    independent, and so is narrow enough that a page left out or a scale 1 % off shows.
+
+      rounding of the output to bf16: errors are spread evenly over half a step either way, at most 2^-8 / sqrt(3) of the
+        value in the mean square; 2.5e-3 with what 128 values scatter;
+      the weights p: P (2^-12), values (2^-12) and scores are rounded at each position for itself, so errors d of that size
+        add up as d sqrt(sum p^2 |v|^2).  A score's 128 terms carry 2^-12 of each (f16 operands), which is an error of
+        2^-12 (sum of squares of the terms)^1/2 in the exponent; some exponentials are off by 1e-4.  All below
+        d = 2^-10 max(1, that root without its 2^-12);
+      what is alike at all positions (sums cut in one direction): 2^-16 sum p |v|.
+    """
+    nq, heads, _ = q.shape
+    kv = k_cache.shape[1]
+    (kc, ks, kl), (vc, vs, vl), there = sequence(k_cache, v_cache, kv_scale, table, max(nk, 0))
+    n = kc.shape[0]
+    out = torch.zeros(nq, heads, D, dtype=torch.float64, device=q.device)
+    room = torch.zeros(nq, heads, dtype=torch.float64, device=q.device)
+    if n == 0:
+        return out, room
+    last = torch.arange(nq, device=q.device) + nk - nq
+    seen = (torch.arange(n, device=q.device)[None] <= last[:, None]) & there[None]
+    some = seen.any(-1)
+    used = seen.any(0)[:, None]
+    clean = lambda t: torch.where(used, t, torch.zeros_like(t))  # noqa: E731
+    for h in range(heads):
+        g = h // (heads // kv)
+        x = q[:, h].double()
+        k = clean(kl[:, g]) + clean(ks[:, g]) * kc[:, g]
+        v = clean(vl[:, g]) + clean(vs[:, g]) * vc[:, g]
+        s = (x @ k.T * softmax_scale).masked_fill(~seen, -math.inf)
+        p = torch.where(some[:, None], torch.softmax(s, -1), torch.zeros_like(s))
+        out[:, h] = p @ v
+        root = (x.square() @ k.square().T).sqrt() * abs(softmax_scale)
+        d = 2.0 ** -10 * torch.where(seen, root, 0.0).clamp(min=1.0)
+        size = v.norm(dim=-1)
+        room[:, h] = (2.5e-3 * out[:, h].norm(dim=-1) + ((d * p * size) ** 2).sum(-1).sqrt()
+                      + 2.0 ** -16 * (p @ v.abs()).norm(dim=-1))
+    return out, room

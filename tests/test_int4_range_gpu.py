@@ -1,0 +1,70 @@
+"""Attention over the 4-bit cache at the ends of bf16's range and between rows of very different size, held to the 2-norm
+of each output row (oracle/int4.py, ``attention_norm``)."""
+import math
+
+import pytest
+import torch
+
+from oracle import int4
+
+pytestmark = pytest.mark.gpu
+SCALE = 128 ** -0.5
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(*shape, seed):
+    return torch.randn(*shape, generator=_gen(seed), device="cuda", dtype=torch.float64)
+
+
+def _cum(v):
+    return torch.tensor([sum(v[:i]) for i in range(len(v) + 1)], dtype=torch.int32, device="cuda")
+
+
+def _filled(key, value, block):
+    """A cache that holds the rows of key and value [positions, kv_heads, 128] of one sequence, its pages in any order, and
+    the sequence's table."""
+    from nanovllm_b200.int4_cache import new_kvcache_int4
+    n, kv, _ = key.shape
+    pages = -(-n // block)
+    cache = new_kvcache_int4(pages + 1, block, kv)
+    table = (torch.randperm(pages, generator=torch.Generator().manual_seed(n)) + 1).to(torch.int32).cuda()
+    at = torch.arange(n, device="cuda")
+    int4.store(key.to(torch.bfloat16), value.to(torch.bfloat16), *cache,
+               (table[at // block] * block + at % block).to(torch.int32))
+    return cache, table
+
+
+def _attend(q, cache, table, n, scale=SCALE):
+    """The last rows of one sequence: a single token through decode, more as a chunk."""
+    from nanovllm_b200.int4_cache import int4_decode_attention, int4_prefill_attention
+    if q.shape[0] == 1:
+        return int4_decode_attention(q, *cache, table[None], torch.tensor([n], dtype=torch.int32, device="cuda"), scale)
+    return int4_prefill_attention(q, *cache, table[None], _cum([q.shape[0]]), _cum([n]), q.shape[0], n, scale)
+
+
+def _check(q, cache, table, n, rows=slice(None), scale=SCALE):
+    out = _attend(q, cache, table, n, scale)
+    ref, room = int4.attention_norm(q, *cache, table, n, scale)
+    far = (out.double() - ref).norm(dim=-1)
+    bad = ~(far <= room)[rows]
+    assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} rows off, first at {bad.nonzero()[0].tolist()}, "
+                           f"{float((far / room)[rows].nan_to_num(math.inf).max()):.2f} of what they may be")
+    return out
+
+
+# query rows of one token (the split-context kernel), of a few, and of a long chunk
+NEWS = [1, 5, 150]
+
+
+@pytest.mark.parametrize("new", NEWS)
+@pytest.mark.parametrize("n", [300, 200000])
+def test_sums_over_a_long_context_stay_finite(new, n):
+    """Values of 2^111: the sum over all positions of p v, before it is divided by the sum of p, passes fp32's range,
+    the parts' own sums do not."""
+    kv, heads = 1, 4
+    key, value = _randn(n, kv, 128, seed=1), (2 + 0.2 * _randn(n, kv, 128, seed=2)) * 2.0 ** 110
+    q = (0.1 * _randn(new, heads, 128, seed=3)).to(torch.bfloat16)
+    _check(q, *_filled(key, value, 64), n)
