@@ -9,8 +9,8 @@
 // Tiles arrive as codes (17 KB instead of 64) and are turned into f16 once for all 256 rows: a masked pair of codes
 // is a pair of f16 numbers (code * 2^-24, or * 2^-20 for the high half of a byte), and one packed multiply-add with
 // (step, low) makes the values.  A power of two for each tile of K (taken back in the scores) and one that only
-// grows for V (taken back at the end) put the largest value of a tile between 2^-7 and 2^-6, so that any bf16 cache
-// fits f16; values are rounded once, to 11 bits.  Within eight values the order is 0 4 1 5 2 6 3 7, as the masks give
+// grows for V (taken back at the end) put the largest value of a tile between 2^-7 and 2^-6, over all of bf16's range;
+// values are rounded once, to 11 bits.  Within eight values the order is 0 4 1 5 2 6 3 7, as the masks give
 // it: q is laid out in the same order, outputs are put back.  A row of K or V that is not finite becomes NaN in K
 // and zero in V, so that it reaches just those query rows that see it.
 //
@@ -46,6 +46,7 @@ constexpr int kUnpackWarp = 8, kLoadWarp = 12, kMmaWarp = 13;
 constexpr int kSoftmaxRegs = 184, kUnpackRegs = 88, kOtherRegs = 56;
 static_assert(2 * kSoftmaxRegs + kUnpackRegs + kOtherRegs == 4 * 128, "all of the registers, and no more");
 constexpr float kSlack = 8.f;  // a reference maximum may lag by 2^8
+constexpr float kDown = 1.f / 128.f;  // codes are f16 numbers code * 2^-24: steps of numbers below 2^-6 times 2^24 fit f16
 constexpr float kLift = 4.f;   // P and its sums are 2^4 times as large: P between 2^-14 and 2^12 is a normal number
 constexpr int kOBytes = kTile * 128;  // a 64-value block of an operand: 128 rows of 128 bytes
 
@@ -57,7 +58,7 @@ struct __align__(1024) Smem {
   uint2 raw_scale[kRaw][kTile];   // beside codes of K: scales of both
   uint32_t raw_there[kRaw];       // and which 16 positions are in pages of the cache
   // of a tile, by unit mod 4: its power of two of K; what V's power changes O by; V's power; raw_there
-  float k_back[4], v_change[4], v_back[4];
+  float k_back[4], v_change[4], v_back[4];  // powers without the 2^7 of kDown
   uint32_t there[4];
   uint64_t raw_full[kRaw], raw_empty[kRaw];
   uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
@@ -282,8 +283,11 @@ struct RowScale {
   uint32_t even, odd, low;
 };
 __device__ __forceinline__ RowScale row_scale(float step, float low) {
-  return {twice_f16(step * 16777216.f), twice_f16(step * 1048576.f), twice_f16(low)};
+  return {twice_f16(step * (16777216.f * kDown)), twice_f16(step * (1048576.f * kDown)), twice_f16(low * kDown)};
 }
+// The power of two that takes a number to between 1 and 2; it and its inverse are normal numbers (the largest and the
+// smallest numbers come out up to twice as large, and smaller).
+__device__ __forceinline__ int power_of(float x) { return max(-126, min(exponent(x), 126)); }
 
 // K is one tile ahead of V (steps K 0, K 1, V 0, K 2, V 1, ...): the scores of the next tile are never waited for.
 // One body for both, so that the loop stays small.
@@ -319,7 +323,8 @@ __device__ __forceinline__ void unpack_role(const Int4AttnParams& p, Smem& sm, C
         const float d = __uint_as_float(sc.y << 16), e = __uint_as_float(sc.y & 0xFFFF0000u);
         const float kt = fmaxf(fabsf(b), fabsf(fmaf(15.f, a, b))), vt = fmaxf(fabsf(e), fabsf(fmaf(15.f, d, e)));
         const bool in = (there >> (row >> 4) & 1u) && pos0 + row < c.s.vis;
-        const bool sane = kt + fabsf(a) + vt + fabsf(d) < INFINITY;  // a sum: NaN and infinity do not get lost
+        // a sum: NaN and infinity do not get lost; of an eighth each, which numbers cannot bring past fp32's range
+        const bool sane = fmaf(kt, 0.125f, fmaf(fabsf(a), 0.125f, fmaf(vt, 0.125f, fabsf(d) * 0.125f))) < INFINITY;
         k_bits = max(k_bits, in && sane ? __float_as_uint(kt) : 0u);
         v_bits = max(v_bits, in && sane ? __float_as_uint(vt) : 0u);
         if (i == 0) {
@@ -333,10 +338,9 @@ __device__ __forceinline__ void unpack_role(const Int4AttnParams& p, Smem& sm, C
       }
       const float k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, k_bits));
       const float v_top = __uint_as_float(__reduce_max_sync(0xffffffffu, v_bits));
-      // largest magnitudes to between 2^-7 and 2^-6: steps times 2^24 stay below 2^16
-      k_exp = k_top > 0.f ? max(-96, min(exponent(k_top), 110)) + 7 : 0;
+      k_exp = k_top > 0.f ? power_of(k_top) : 0;
       if (v_top > 0.f) {
-        const int e = max(-96, min(exponent(v_top), 110)) + 7;
+        const int e = power_of(v_top);
         if (!v_exp_set) {
           v_exp = e;
           v_exp_set = true;
@@ -570,6 +574,17 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
   const uint32_t q = smem_u32(sm.q[g]);
   uint32_t s_parity = 0, o_parity = 0;
   constexpr int kPart = kItem * (kHeadDim + 2);
+  auto scale_o = [&](float f) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < kHeadDim; c0 += 8) {
+      float y[8];
+      tc::ld8(o_tmem + c0, y);
+      tc::wait_ld();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] *= f;
+      tc::st8(o_tmem + c0, y);
+    }
+  };
   bool first_piece = true;
   Cursor c = next;
   bool started = false, more = true;
@@ -603,9 +618,9 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         top_bits = __vmaxu2(__vmaxu2(top_bits, w.z & 0x7FFF7FFFu), w.w & 0x7FFF7FFFu);
       }
       const float amax = __uint_as_float(max(top_bits & 0xFFFFu, top_bits >> 16) << 16);
-      const int e = amax > 0.f && amax < INFINITY ? max(-100, min(exponent(amax), 110)) - 13 : 0;
+      const int e = amax > 0.f && amax < INFINITY ? max(-113, exponent(amax)) - 13 : 0;
       const float to = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);  // a negative scale turns q around
-      const float cs = fabsf(p.scale_log2) * pow2(e);
+      const float cs = fabsf(p.scale_log2) * pow2(e + 7);  // with K's kDown
 #pragma unroll 4
       for (int i = 0; i < 16; ++i) {
         const uint4 raw_w = ld_shared_v4(q_piece(q, r, i));
@@ -657,17 +672,7 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
           l *= lag;
           f *= lag;
         }
-        if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < kHeadDim; c0 += 8) {
-            float y[8];
-            tc::ld8(o_tmem + c0, y);
-            tc::wait_ld();
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] *= f;
-            tc::st8(o_tmem + c0, y);
-          }
-        }
+        if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) scale_o(f);
         // ---- P over the columns of S, all of which have been read
         const float bias = kLift - m;
         const uint64_t ct2 = f2_pack(ct, ct), bias2 = f2_pack(bias, bias);
@@ -714,7 +719,12 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
       o_parity ^= 1u;
       tc::fence_after_sync();
       const bool whole = c.whole();
-      const float f = m == kNone ? 0.f : __fdiv_rn(back, l);  // 0 for a row that sees nothing
+      if (back > 0x1p100f) {  // the same for all rows: back / kDown / l might pass fp32's range where the outputs do not
+        scale_o(0x1p16f);
+        tc::wait_st();
+        back *= 0x1p-16f;
+      }
+      const float f = m == kNone ? 0.f : __fdiv_rn(back * (1.f / kDown), l);  // 0 for a row that sees nothing
       // a thread stores its row, 32 bytes at a time: whole sectors
       const int row = c.rg * kItem + g * kRows + r, token = row / p.group;
       float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart;

@@ -123,7 +123,8 @@ def attention_norm(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale):
     independent, and so is narrow enough that a page left out or a scale 1 % off shows.
 
       rounding of the output to bf16: errors are spread evenly over half a step either way, at most 2^-8 / sqrt(3) of the
-        value in the mean square; 2.5e-3 with what 128 values scatter;
+        value in the mean square; 2.5e-3 with what 128 values scatter; below 2^-126, where bf16's steps are 2^-133
+        whatever the value, at most 2^-134 for each;
       the weights p: P (2^-12), values (2^-12) and scores are rounded at each position for itself, so errors d of that size
         add up as d sqrt(sum p^2 |v|^2).  A score's 128 terms carry 2^-12 of each (f16 operands), which is an error of
         2^-12 (sum of squares of the terms)^1/2 in the exponent; some exponentials are off by 1e-4.  All below
@@ -155,5 +156,5 @@ def attention_norm(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale):
         d = 2.0 ** -10 * torch.where(seen, root, 0.0).clamp(min=1.0)
         size = v.norm(dim=-1)
         room[:, h] = (2.5e-3 * out[:, h].norm(dim=-1) + ((d * p * size) ** 2).sum(-1).sqrt()
-                      + 2.0 ** -16 * (p @ v.abs()).norm(dim=-1))
+                      + 2.0 ** -16 * (p @ v.abs()).norm(dim=-1) + 2.0 ** -134 * D ** 0.5)
     return out, room

@@ -68,3 +68,17 @@ def test_sums_over_a_long_context_stay_finite(new, n):
     key, value = _randn(n, kv, 128, seed=1), (2 + 0.2 * _randn(n, kv, 128, seed=2)) * 2.0 ** 110
     q = (0.1 * _randn(new, heads, 128, seed=3)).to(torch.bfloat16)
     _check(q, *_filled(key, value, 64), n)
+
+
+# powers of two of K's and V's rows, and q's, such that scores are ordinary numbers
+POWERS = [(0, 113), (0, 120), (0, 125), (0, -115), (0, -126), (113, 0), (125, 0), (-100, 0), (-115, 0), (112, 126), (-112, -120)]
+
+
+@pytest.mark.parametrize("new", [33, 150])
+@pytest.mark.parametrize("k_power,v_power", POWERS, ids=str)
+def test_chunk_over_bf16s_range(new, k_power, v_power):
+    n, kv, heads = 333, 2, 8
+    key, value = (_randn(n, kv, 128, seed=s).clamp(-3, 3) * 2.0 ** (p - 1) for s, p in ((4, k_power), (5, v_power)))
+    q = (1.5 * _randn(new, heads, 128, seed=6) * 2.0 ** (1 - k_power)).to(torch.bfloat16)
+    out = _check(q, *_filled(key, value, 16), n)
+    assert torch.isfinite(out).all()
