@@ -8,11 +8,16 @@
 //   O_g += P_g V         8 products, P from tensor memory, V from shared memory
 // Tiles arrive as codes (17 KB instead of 64) and are turned into f16 once for all 256 rows: a masked pair of codes
 // is a pair of f16 numbers (code * 2^-24, or * 2^-20 for the high half of a byte), and one packed multiply-add with
-// (step, low) makes the values.  A power of two for each tile of K (taken back in the scores) and one that only
-// grows for V (taken back at the end) put the largest value of a tile between 2^-7 and 2^-6, over all of bf16's range;
-// values are rounded once, to 11 bits.  Within eight values the order is 0 4 1 5 2 6 3 7, as the masks give
-// it: q is laid out in the same order, outputs are put back.  A row of K or V that is not finite becomes NaN in K
-// and zero in V, so that it reaches just those query rows that see it.
+// (step, low) makes the values.  A block of 32 rows of K or V has a power of two that puts its largest value between 2^-7
+// and 2^-6, over all of bf16's range; values are rounded once, to 11 bits.  K's power is put back into the block's columns
+// of scores.  V's goes into P, whose reference is the query row's own largest p |v| and not its largest p, so that
+// what a query row gets does not depend on the size of rows that it does not see.  Within eight values the order is
+// 0 4 1 5 2 6 3 7, as the masks give it: q is laid out in the same order, outputs are put back.  A row of K or V that is not
+// finite becomes NaN in K and zero in V, so that it reaches just those query rows that see it.
+//
+// Rows of one block that differ by more than 2^kSpread cannot share a power: the small ones would leave f16's normal numbers
+// (below 2^-14).  In such a block each row of K and V has its own, at the cost of a second pass over the tile's scores and a
+// second exponential (all tiles of 2,048 of 32,768: 3,540 us for 940; each sequence's first row alone: 955).
 //
 // Bound by the chain of a group: products of its tile (1,056 cycles: one every 66) behind the other group's, then its
 // softmax (about 2,050), 4,100 cycles for a tile of both groups; tensor cores and issue slots are half busy (2,048 new
@@ -47,6 +52,9 @@ constexpr int kSoftmaxRegs = 184, kUnpackRegs = 88, kOtherRegs = 56;
 static_assert(2 * kSoftmaxRegs + kUnpackRegs + kOtherRegs == 4 * 128, "all of the registers, and no more");
 constexpr float kSlack = 8.f;  // a reference maximum may lag by 2^8
 constexpr float kDown = 1.f / 128.f;  // codes are f16 numbers code * 2^-24: steps of numbers below 2^-6 times 2^24 fit f16
+constexpr int kSpread = 6;  // within 2^7 of the largest a row's error is 2^-18 2^6 of its largest value at most: f16's own
+constexpr int kBlock = 32;  // rows of K and V that share a power of two
+constexpr float kGap = 60.f;  // a block's V may be 2^-60 of a row's reference, so that P of it, of which l is summed, is there
 constexpr float kLift = 4.f;   // P and its sums are 2^4 times as large: P between 2^-14 and 2^12 is a normal number
 constexpr int kOBytes = kTile * 128;  // a 64-value block of an operand: 128 rows of 128 bytes
 
@@ -57,9 +65,11 @@ struct __align__(1024) Smem {
   uint8_t raw[kRaw][kTile * 64];  // codes of K or V, 64B swizzle
   uint2 raw_scale[kRaw][kTile];   // beside codes of K: scales of both
   uint32_t raw_there[kRaw];       // and which 16 positions are in pages of the cache
-  // of a tile, by unit mod 4: its power of two of K; what V's power changes O by; V's power; raw_there
-  float k_back[4], v_change[4], v_back[4];  // powers without the 2^7 of kDown
+  // of a tile, by unit mod 4, and its blocks: K's power of two (without kDown; negative: each row has its own); the exponent of
+  // V's; raw_there; and rows' own powers: their exponents + 127, of K and V
+  float4 k_back[4], v_power[4];  // a component for each block
   uint32_t there[4];
+  uint16_t powers[4][kTile];
   uint64_t raw_full[kRaw], raw_empty[kRaw];
   uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
@@ -104,7 +114,7 @@ struct Groups {
     }
   }
 };
-static_assert(kTile == 128, "the shift in Groups::tiles");
+static_assert(kTile == 128 && kTile / kBlock == 4, "the shift in Groups::tiles, Smem's float4");
 __device__ __forceinline__ int tiles_of(const Int4AttnParams& p, const Seq& q, int rg) { return Groups(p, rg).tiles(q); }
 __device__ __forceinline__ int64_t units_of(const Int4AttnParams& p, const Seq& q) {
   int64_t n = 0;
@@ -293,8 +303,6 @@ __device__ __forceinline__ int power_of(float x) { return max(-126, min(exponent
 // One body for both, so that the loop stays small.
 __device__ __forceinline__ void unpack_role(const Int4AttnParams& p, Smem& sm, Cursor c, int warp, int lane) {
   const int g = lane >> 2, t = lane & 3;
-  int v_exp = 0;
-  bool v_exp_set = false;
   RowScale v_scale = {0, 0, 0}, next_v = {0, 0, 0};
   int stage = 0;
   uint32_t raw_parity = 0;
@@ -306,53 +314,31 @@ __device__ __forceinline__ void unpack_role(const Int4AttnParams& p, Smem& sm, C
     if (!wait_all(&sm.raw_full[stage], raw_parity, p.err)) return;
     RowScale mine = v_scale;
     uint32_t there = 0;
-    int k_exp = 0;
-    float change = 1.f;
+    float k_back = 1.f, v_power = 0.f;
     if (is_k) {
-      // ---- the tile's largest magnitudes, over rows that are there (all warps alike)
+      // ---- the warp's 32 rows, a lane each: the largest and the smallest of those that are there
       there = sm.raw_there[stage];
-      const int pos0 = c.tile * kTile;
-      uint32_t k_bits = 0, v_bits = 0;
-      float ks = 0.f, kl = 0.f, vs = 0.f, vl = 0.f;  // of this lane's own row, 32 warp + lane
-      bool held = false, fine = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 32 * (i ^ warp) + lane;  // its own first
-        const uint2 sc = sm.raw_scale[stage][row];
-        const float a = __uint_as_float(sc.x << 16), b = __uint_as_float(sc.x & 0xFFFF0000u);
-        const float d = __uint_as_float(sc.y << 16), e = __uint_as_float(sc.y & 0xFFFF0000u);
-        const float kt = fmaxf(fabsf(b), fabsf(fmaf(15.f, a, b))), vt = fmaxf(fabsf(e), fabsf(fmaf(15.f, d, e)));
-        const bool in = (there >> (row >> 4) & 1u) && pos0 + row < c.s.vis;
-        // a sum: NaN and infinity do not get lost; of an eighth each, which numbers cannot bring past fp32's range
-        const bool sane = fmaf(kt, 0.125f, fmaf(fabsf(a), 0.125f, fmaf(vt, 0.125f, fabsf(d) * 0.125f))) < INFINITY;
-        k_bits = max(k_bits, in && sane ? __float_as_uint(kt) : 0u);
-        v_bits = max(v_bits, in && sane ? __float_as_uint(vt) : 0u);
-        if (i == 0) {
-          ks = a;
-          kl = b;
-          vs = d;
-          vl = e;
-          held = in;
-          fine = in && sane;
-        }
-      }
-      const float k_top = __uint_as_float(__reduce_max_sync(0xffffffffu, k_bits));
-      const float v_top = __uint_as_float(__reduce_max_sync(0xffffffffu, v_bits));
-      k_exp = k_top > 0.f ? power_of(k_top) : 0;
-      if (v_top > 0.f) {
-        const int e = power_of(v_top);
-        if (!v_exp_set) {
-          v_exp = e;
-          v_exp_set = true;
-        } else if (e > v_exp) {
-          change = v_exp - e < -126 ? 0.f : pow2(v_exp - e);
-          v_exp = e;
-        }
-      }
+      const int row = 32 * warp + lane;
+      const uint2 sc = sm.raw_scale[stage][row];
+      const float ks = __uint_as_float(sc.x << 16), kl = __uint_as_float(sc.x & 0xFFFF0000u);
+      const float vs = __uint_as_float(sc.y << 16), vl = __uint_as_float(sc.y & 0xFFFF0000u);
+      const float kt = fmaxf(fabsf(kl), fabsf(fmaf(15.f, ks, kl))), vt = fmaxf(fabsf(vl), fabsf(fmaf(15.f, vs, vl)));
+      const bool held = (there >> (row >> 4) & 1u) && c.tile * kTile + row < c.s.vis;
+      // a sum: NaN and infinity do not get lost; of an eighth each, which numbers cannot bring past fp32's range
+      const bool fine = held && fmaf(kt, 0.125f, fmaf(fabsf(ks), 0.125f, fmaf(vt, 0.125f, fabsf(vs) * 0.125f))) < INFINITY;
+      const int ke = power_of(kt), ve = power_of(vt);
+      const int k_most = __reduce_max_sync(0xffffffffu, fine ? ke : -126), v_most = __reduce_max_sync(0xffffffffu, fine ? ve : -126);
+      // small rows.  Zeros are exact with any power, but in V they count: P of the others must not sink beside theirs
+      const bool small = fine && ((kt > 0.f && k_most - ke > kSpread) || v_most - ve > kSpread);
+      const bool own = __any_sync(0xffffffffu, small);
+      const int k_exp = own && fine ? ke : k_most, v_exp = own && fine ? ve : v_most;
       const float k_to = pow2(-k_exp), v_to = pow2(-v_exp);
-      const float wild_low = held ? __uint_as_float(0x7FC00000u) : 0.f;
-      mine = fine ? row_scale(ks * k_to, kl * k_to) : row_scale(0.f, wild_low);
+      mine = fine ? row_scale(ks * k_to, kl * k_to) : row_scale(0.f, held ? __uint_as_float(0x7FC00000u) : 0.f);
       next_v = fine ? row_scale(vs * v_to, vl * v_to) : row_scale(0.f, 0.f);
+      if (own) sm.powers[k_unit & 3][row] = static_cast<uint16_t>((k_exp + 127) | (v_exp + 127) << 8);
+      k_back = own ? -1.f : pow2(k_most);
+      // a block without rows: the largest power, so that it is never a row's smallest
+      v_power = __any_sync(0xffffffffu, fine) ? static_cast<float>(v_most) : 126.f;
     }
     // ---- 32 rows of codes (lane: rows 8 i + g, 16-byte piece t) into the operand
     uint4 x[4];
@@ -386,12 +372,11 @@ __device__ __forceinline__ void unpack_role(const Int4AttnParams& p, Smem& sm, C
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      if (is_k && warp == 0) {
+      if (is_k) {
         const int slot = k_unit & 3;
-        sm.k_back[slot] = pow2(k_exp);
-        sm.v_change[slot] = change;
-        sm.v_back[slot] = pow2(v_exp);
-        sm.there[slot] = there;
+        reinterpret_cast<float*>(&sm.k_back[slot])[warp] = k_back;
+        reinterpret_cast<float*>(&sm.v_power[slot])[warp] = v_power;
+        if (warp == 0) sm.there[slot] = there;
       }
       mbar_arrive(is_k ? &sm.k_full[buf] : &sm.v_full[buf]);
       mbar_arrive(&sm.raw_empty[stage]);
@@ -405,8 +390,6 @@ __device__ __forceinline__ void unpack_role(const Int4AttnParams& p, Smem& sm, C
       if (++c.tile == c.end) {
         more_k = c.more();
         if (more_k) next_piece(p, c);
-        v_exp = 0;
-        v_exp_set = false;
       }
     } else {
       ++v_unit;
@@ -567,6 +550,83 @@ __device__ __forceinline__ uint32_t q_piece(uint32_t q, int row, int piece) {
   return q + (piece >> 3) * kOBytes + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
 }
 
+// A row's references: m of its largest score, and power, 2^power being its largest p |v| so far.
+struct Reference {
+  float m, power;
+  // New ones where they lag too far (also for NaN: the row's sums and outputs become NaN).
+  __device__ __forceinline__ Reference after(float top, float top_v) const {
+    const bool higher = !(top <= m + kSlack);
+    const float now = higher ? top : m;
+    return {now, higher || top_v - now > power + kSlack ? ceilf(fmaxf(power + (m - now), top_v - now)) : power};
+  }
+};
+
+// O's row in tensor memory, times f.
+__device__ __forceinline__ void scale_o(uint32_t o_tmem, float f) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < kHeadDim; c0 += 8) {
+    float y[8];
+    tc::ld8(o_tmem + c0, y);
+    tc::wait_ld();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] *= f;
+    tc::st8(o_tmem + c0, y);
+  }
+}
+
+// A tile with rows that have powers of their own, or blocks of V that differ by more than 2^kGap:
+// l's terms 2^(score - m + kLift) and P = 2^(score - m + kLift - power) of V's power are exponentials for themselves.
+__device__ __noinline__ float3 wide_tile(const Smem& sm, uint32_t s_tmem, float cs, int slot, uint32_t there, int seen, bool rest,
+                                       Reference at, float l) {
+  // 32 scores, -infinity where the row does not see one; v: exponents of V's powers
+  auto scores = [&](int h, float (&x)[32], float (&v)[32]) {
+    uint32_t w[32];
+    tmem_ld32(s_tmem + 32 * h, w);
+    tc::wait_ld();
+    const uint32_t mask = seen_of(there, seen, 32 * h);
+    const float back = reinterpret_cast<const float*>(&sm.k_back[slot])[h];
+    const float v_power = reinterpret_cast<const float*>(&sm.v_power[slot])[h];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const int own = sm.powers[slot][32 * h + k];
+      const float k_back = back < 0.f ? pow2((own & 255) - 127) : back;
+      v[k] = back < 0.f ? static_cast<float>((own >> 8) - 127) : v_power;
+      x[k] = mask >> k & 1u ? __uint_as_float(w[k]) * (cs * k_back) : -INFINITY;
+    }
+  };
+  float top = -INFINITY, top_v = -INFINITY;
+#pragma unroll 1
+  for (int h = 0; h < 4; ++h) {
+    float x[32], v[32];
+    scores(h, x, v);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      top = max3_nan(top, x[k], x[k]);
+      top_v = fmaxf(top_v, x[k] + v[k]);
+    }
+  }
+  const Reference to = at.after(top, top_v);
+  const float f = ex2((at.m - to.m) + (at.power - to.power));
+  l *= ex2(at.m - to.m);
+  at = to;
+  if (rest && __any_sync(0xffffffffu, f != 1.f)) scale_o(s_tmem + 128, f);
+  float sum = 0.f;
+#pragma unroll 1
+  for (int h = 0; h < 4; ++h) {  // P's columns lie over those of S that have been read
+    float x[32], v[32];
+    scores(h, x, v);
+    uint32_t pw[16];
+#pragma unroll
+    for (int k = 0; k < 32; k += 2) {
+      const float a = x[k] - at.m + kLift, b = x[k + 1] - at.m + kLift;
+      sum += ex2(a) + ex2(b);
+      pw[k / 2] = pack_f16x2(ex2(a + (v[k] - at.power)), ex2(b + (v[k + 1] - at.power)));
+    }
+    tc::st16u(s_tmem + 16 * h, pw);
+  }
+  return make_float3(at.m, at.power, l + sum);
+}
+
 __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, Cursor next, const Ranges& ranges,
                                              int g, int tid) {
   const int r = tid & 127, warp = r >> 5, lane = tid & 31;
@@ -574,24 +634,14 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
   const uint32_t q = smem_u32(sm.q[g]);
   uint32_t s_parity = 0, o_parity = 0;
   constexpr int kPart = kItem * (kHeadDim + 2);
-  auto scale_o = [&](float f) {
-#pragma unroll 1
-    for (int c0 = 0; c0 < kHeadDim; c0 += 8) {
-      float y[8];
-      tc::ld8(o_tmem + c0, y);
-      tc::wait_ld();
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] *= f;
-      tc::st8(o_tmem + c0, y);
-    }
-  };
   bool first_piece = true;
   Cursor c = next;
   bool started = false, more = true;
   for (int u = 0, n = 0;;) {
     const int rows = c.s.nq * p.group;
     const bool active = started && rows - c.rg * kItem > g * kRows;
-    float m = kNone, l = 0.f, back = 1.f;
+    Reference at = {kNone, 0.f};
+    float l = 0.f;  // sum of 2^(score - m + kLift); O: of 2^(score - m - power + kLift) v kDown
     if (active) {
       const int row = c.rg * kItem + g * kRows + r;
       const int token = row / p.group;
@@ -645,60 +695,77 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         if (!wait_all(&sm.s_full[g], s_parity, p.err)) return;
         s_parity ^= 1u;
         tc::fence_after_sync();
-        // never 0, so that what is not seen (minus infinity) stays so; scores are below 2^16
-        const float ct = fmaxf(cs * sm.k_back[slot], 1.0e-30f);
-        back = sm.v_back[slot];
-        float f = sm.v_change[slot];
         const uint32_t there = sm.there[slot];
         const int seen = limit - (c.tile + i) * kTile;  // columns below this one
+        const float4 k_back = sm.k_back[slot], v_power = sm.v_power[slot];
+        // up to this score the references stay; NaN: not a tile for what follows
+        const float v_least = fminf(fminf(v_power.x, v_power.y), fminf(v_power.z, v_power.w));
+        const float v_most = fmaxf(fmaxf(v_power.x, v_power.y), fmaxf(v_power.z, v_power.w));
+        const bool own = fminf(fminf(k_back.x, k_back.y), fminf(k_back.z, k_back.w)) < 0.f;
+        const float stay = own || at.power - v_least > kGap ? NAN : at.m + fminf(kSlack, at.power + kSlack - v_most);
+        // never 0, so that what is not seen (minus infinity) stays so; products are below 2^16
+        const float ct[4] = {fmaxf(cs * k_back.x, 1.0e-30f), fmaxf(cs * k_back.y, 1.0e-30f),
+                             fmaxf(cs * k_back.z, 1.0e-30f), fmaxf(cs * k_back.w, 1.0e-30f)};
         const bool masked = !__all_sync(0xffffffffu, there == 0xFFu && seen >= kTile);
         uint32_t w[4][32];
 #pragma unroll
         for (int h = 0; h < 4; ++h) tmem_ld32(s_tmem + 32 * h, w[h]);
         tc::wait_ld();
         if (masked) hide(w, there, seen);
-        // ---- the row's maximum; NaN where it sees one
-        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int h = 0; h < 4; ++h)
-#pragma unroll
-          for (int k = 0; k < 32; k += 2)
-            t[k / 2 & 3] = max3_nan(t[k / 2 & 3], __uint_as_float(w[h][k]), __uint_as_float(w[h][k + 1]));
-        const float top = max3_nan(max3_nan(t[0], t[1], t[2]), t[3], t[3]) * ct;
-        // ---- a new reference maximum where it lags too far, and V's power of two
-        if (!(top <= m + kSlack)) {  // also for NaN: the row's sums and outputs become NaN
-          const float lag = ex2(m - top);
-          m = top;
-          l *= lag;
-          f *= lag;
-        }
-        if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) scale_o(f);
-        // ---- P over the columns of S, all of which have been read
-        const float bias = kLift - m;
-        const uint64_t ct2 = f2_pack(ct, ct), bias2 = f2_pack(bias, bias);
-        uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+        // ---- the blocks' maxima; NaN where the row sees one
+        float t[4];
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-          uint32_t pw[16];
+          t[h] = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float x0, x1, p0, p1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(w[h][2 * k]), __uint_as_float(w[h][2 * k + 1])), ct2, bias2), x0, x1);
-            if (k % 4 == 3) {
-              exp2_poly_x2(x0, x1, p0, p1);
-            } else {
-              p0 = ex2(x0);
-              p1 = ex2(x1);
-            }
-            sum[k & 1] = f2_add(sum[k & 1], f2_pack(p0, p1));
-            pw[k] = pack_f16x2(p0, p1);
-          }
-          tc::st16u(s_tmem + 16 * h, pw);
+          for (int k = 0; k < 32; k += 2) t[h] = max3_nan(t[h], __uint_as_float(w[h][k]), __uint_as_float(w[h][k + 1]));
+          t[h] *= ct[h];
         }
-        float a0, a1, b0, b1;
-        f2_unpack(sum[0], a0, a1);
-        f2_unpack(sum[1], b0, b1);
-        l += (a0 + a1) + (b0 + b1);
+        const float top = max3_nan(max3_nan(t[0], t[1], t[2]), t[3], t[3]);
+        bool wide = false;
+        if (!__all_sync(0xffffffffu, top <= stay)) {
+          const Reference to = at.after(
+              top, fmaxf(fmaxf(t[0] + v_power.x, t[1] + v_power.y), fmaxf(t[2] + v_power.z, t[3] + v_power.w)));
+          wide = __any_sync(0xffffffffu, own || to.power - v_least > kGap);
+          if (!wide) {
+            const float f = ex2((at.m - to.m) + (at.power - to.power));
+            l *= ex2(at.m - to.m);
+            at = to;
+            if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) scale_o(o_tmem, f);
+          }
+        }
+        if (wide) {
+          const float3 y = wide_tile(sm, s_tmem, cs, slot, there, seen, i > 0, at, l);
+          at = {y.x, y.y};
+          l = y.z;
+        } else {
+          // ---- P over the columns of S, all of which have been read
+          const float ev[4] = {v_power.x - at.power, v_power.y - at.power, v_power.z - at.power, v_power.w - at.power};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const float bias = kLift - at.m + ev[h];
+            const uint64_t ct2 = f2_pack(ct[h], ct[h]), bias2 = f2_pack(bias, bias);
+            uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+            uint32_t pw[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float x0, x1, p0, p1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(w[h][2 * k]), __uint_as_float(w[h][2 * k + 1])), ct2, bias2), x0, x1);
+              if (k % 4 == 3) {
+                exp2_poly_x2(x0, x1, p0, p1);
+              } else {
+                p0 = ex2(x0);
+                p1 = ex2(x1);
+              }
+              sum[k & 1] = f2_add(sum[k & 1], f2_pack(p0, p1));
+              pw[k] = pack_f16x2(p0, p1);
+            }
+            tc::st16u(s_tmem + 16 * h, pw);
+            float a0, a1;
+            f2_unpack(f2_add(sum[0], sum[1]), a0, a1);
+            l = fmaf(a0 + a1, ex2(-ev[h]), l);
+          }
+        }
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
@@ -719,12 +786,14 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
       o_parity ^= 1u;
       tc::fence_after_sync();
       const bool whole = c.whole();
-      if (back > 0x1p100f) {  // the same for all rows: back / kDown / l might pass fp32's range where the outputs do not
-        scale_o(0x1p16f);
+      // V's power / kDown / l might pass fp32's range where the outputs do not
+      const float over = at.power > 100.f ? 16.f : at.power < -100.f ? -16.f : 0.f;
+      if (__any_sync(0xffffffffu, over != 0.f)) {
+        scale_o(o_tmem, pow2(static_cast<int>(over)));
         tc::wait_st();
-        back *= 0x1p-16f;
       }
-      const float f = m == kNone ? 0.f : __fdiv_rn(back * (1.f / kDown), l);  // 0 for a row that sees nothing
+      const float back = pow2(max(-126, min(static_cast<int>(at.power - over), 126)));
+      const float f = at.m == kNone ? 0.f : __fdiv_rn(back * (1.f / kDown), l);  // 0 for a row that sees nothing
       // a thread stores its row, 32 bytes at a time: whole sectors
       const int row = c.rg * kItem + g * kRows + r, token = row / p.group;
       float* part = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (first_piece ? 0 : 1)) * kPart;
@@ -762,7 +831,7 @@ __device__ __forceinline__ void softmax_role(const Int4AttnParams& p, Smem& sm, 
         }
       }
       if (!whole)
-        *reinterpret_cast<float2*>(part + kItem * kHeadDim + 2 * (g * kRows + r)) = make_float2(m, m == kNone ? 0.f : l);
+        *reinterpret_cast<float2*>(part + kItem * kHeadDim + 2 * (g * kRows + r)) = make_float2(at.m, at.m == kNone ? 0.f : l);
       tc::fence_before_sync();  // O has been read before the next piece's first P is announced
     }
     if (!more) {

@@ -82,3 +82,56 @@ def test_chunk_over_bf16s_range(new, k_power, v_power):
     q = (1.5 * _randn(new, heads, 128, seed=6) * 2.0 ** (1 - k_power)).to(torch.bfloat16)
     out = _check(q, *_filled(key, value, 16), n)
     assert torch.isfinite(out).all()
+
+
+def _ordinary(n, kv, heads, new, seed=7):
+    return _randn(n, kv, 128, seed=seed), _randn(n, kv, 128, seed=seed + 1), 1.5 * _randn(new, heads, 128, seed=seed + 2)
+
+
+@pytest.mark.parametrize("new,n", [(150, 400), (40, 9000)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("power", [5, 10, 14, 20, 60, 100, -20, -100])
+def test_chunk_beside_a_row_of_another_size(new, n, which, power):
+    """The last token's row of K or V, which the queries before it do not see."""
+    key, value, q = _ordinary(n, 1, 4, new)
+    (key if which == "k" else value)[-1] *= 2.0 ** power
+    _check(q.to(torch.bfloat16), *_filled(key, value, 64), n, slice(0, -1))
+
+
+def _peaks(key, q, places):
+    """Makes query row r of head 0 look at positions places[r], by a key along it."""
+    for r, at in enumerate(places):
+        key[at, 0] = q[r, 0] * 3
+
+
+@pytest.mark.parametrize("new", [40, 150])
+@pytest.mark.parametrize("powers", [{0: -9}, {0: -40, 500: 5}, {3: 12}, {0: 40, 130: -40, 700: 3}, {5: "zero"},
+                                    {130: -20, 131: 20, 300: 0, 600: -20}], ids=str)
+def test_chunk_values_of_many_sizes(new, powers):
+    """Rows of V whose sizes differ by far more than f16 holds: queries that look at one of them alone, at an ordinary one,
+    or at all; tiles with such a row and without take turns."""
+    n = 1000
+    key, value, q = _ordinary(n, 1, 4, new)
+    for at, power in powers.items():
+        value[at] *= 0.0 if power == "zero" else 2.0 ** power
+    _peaks(key, q, list(powers) + [1, 129, 400, 801])
+    _check(q.to(torch.bfloat16), *_filled(key, value, 16), n)
+
+
+@pytest.mark.parametrize("new", [40, 150])
+def test_chunk_keys_of_many_sizes(new):
+    n = 700
+    key, value, q = _ordinary(n, 1, 4, new)
+    key *= torch.exp2(torch.randint(-25, 2, (n, 1, 1), generator=_gen(10), device="cuda").double())
+    key[5], key[300:303] = 0, 0
+    _check(q.to(torch.bfloat16), *_filled(key, value, 16), n)
+
+
+@pytest.mark.parametrize("new", [40, 150])
+def test_chunk_rows_of_any_size_at_all(new):
+    """Every row of V with a power of its own, 2^-120 to 2^120, over several tiles and CTAs."""
+    for n in (200, 5000):
+        key, value, q = _ordinary(n, 2, 4, new)
+        value *= torch.exp2(torch.randint(-120, 120, (n, 2, 1), generator=_gen(11), device="cuda").double())
+        _peaks(key, q, range(0, n, max(1, n // 30)))
+        _check(q.to(torch.bfloat16), *_filled(key, value, 32), n)
