@@ -34,10 +34,14 @@
 // but the output's own rounding; 5.3e-3 without that, 2.4e-3 and 1 % slower with the ones of all positions in one warp).
 // The loop over units stays as it is: a branch in it cost 5 %.
 //
-// Precision: scores, statistics and sums in fp32; P is rounded once, to f16 (2^-12), after its row's
-// reference maximum and a power of two near the largest step of V are taken out, so it stays below 2^14.
+// Precision: scores, statistics and sums in fp32; P step is rounded once, to f16 (2^-12), after its row's
+// reference maximum and a power of two near the largest step of V so far are taken out, so it stays below 2^15.  That power
+// is the CTA's, and so comes from rows as well that a query row does not look at.  Where steps of V differ by more than
+// some 2^15 (or are zero beside others), or values pass 2^90, the rest of the piece is done with a power for each query row instead, that of its own largest
+// p |v| so far, found with one more exchange of maxima for each unit; what a row gets is then as exact as its own largest terms.
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 #include "int4_attention.cuh"
 
@@ -50,6 +54,11 @@ __device__ int g_error = 0;
 
 constexpr int kTile = 32;               // positions of a unit whose scores a warp computes
 constexpr float kSlack = 8.f;           // a reference maximum may lag by 2^8
+constexpr int kStepBits = 3;            // V's largest step is 2^3 .. 2^4 when it is new, and may grow to 2^7: P step < 2^15
+constexpr int kSpreadBits = 15;          // and the smallest 2^-15 of what the largest was when it was new: P step of p = 1 is 2^-12
+                                        // or more there, f16's absolute error of 2^-25 relative 2^-13
+constexpr float kHuge = 0x1p90f;        // sums over the positions of larger values could pass fp32's range
+constexpr int kOwnBits = 14;            // of a query row's own power: P step < 2^13
 constexpr int kPieceUnits = 1;          // what a pair costs beside its tiles, in units of a tile
 constexpr int kFlush = 64;              // units whose products with V the tensor cores add up
 
@@ -80,7 +89,8 @@ struct __align__(1024) Smem {
   uint2 q[S::NT][8][32];                    // as the B operand of S^T: plane, step, lane
   uint16_t p[2][S::R][kPPitch];             // P step, f16, of this unit and the one before
   float kq[S::R], qs[S::R];                 // score = dot kq step + qs low
-  float top[kWarps][S::R], top_v[kWarps];   // of the warps' positions: largest score and step,
+  float top[kWarps][S::R], term[kWarps][S::R];  // of the warps' positions: largest score and term,
+  float top_v[kWarps], least_v[kWarps];  // largest and smallest step (-1: huge values),
   float l[kWarps][S::R], mid[kWarps][S::R], ps[kWarps][S::R];  // sums
   uint64_t full[S::kStages], empty[S::kStages], q_full, q_free;
   uint32_t there[S::kStages];  // which parts of the stage's unit are in pages of the cache
@@ -102,6 +112,12 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
 }
 
 __device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
@@ -227,7 +243,7 @@ __device__ __forceinline__ void convert_q(const uint16_t* row, bool is_row, int 
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
     sum += __shfl_xor_sync(0xffffffffu, sum, off);
   }
-  const int e = amax > 0.f && amax < INFINITY ? max(-100, min(exponent(amax), 110)) - 13 : 0;
+  const int e = amax > 0.f && amax < INFINITY ? max(-113, exponent(amax)) - 13 : 0;
   const float even = pow2(-e), odd = pow2(-e - 4);
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -240,7 +256,7 @@ __device__ __forceinline__ void convert_q(const uint16_t* row, bool is_row, int 
                                            __uint_as_float(hi & 0xFFFF0000u) * odd));
     }
   }
-  kq = pow2(e) * 16777216.f * scale_log2;  // e + 24 <= 121
+  kq = pow2(e) * scale_log2 * 16777216.f;  // inside fp32 up to q = 2^116 / scale
   qs = sum * scale_log2;
 }
 
@@ -360,6 +376,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
   const uint32_t k_ring = smem_u32(sm.k[0]) + (warp * kTile + g) * 64 + (t ^ (g >> 1 & 3)) * 16;
   const uint32_t v_ring = smem_u32(sm.v[0]) + lane * 64 + (warp ^ (lane >> 1 & 3)) * 16;
   const uint32_t s_ring = smem_u32(sm.scale[0]) + (warp * kTile + g) * 8;
+  const uint32_t s_own = s_ring + (t >> 1) * 128 + (t & 1) * 64 + 4;
   const uint32_t p_lane = smem_u32(sm.p[0]) + ((lane & 7) * kPPitch + (lane >> 3) * 8) * 2;  // row of a plane, 8 positions
   auto all_warps = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); };
   int stage = 0;
@@ -395,28 +412,30 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
     for (int off = 1; off < 4; off <<= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
 
     float o[NT][2][4], ps[NT][4];          // ps: sum of the rounded P step, of this warp's positions
-    volatile float kept[10 * NT], m_kept[2 * NT];  // o and ps of the units before, and their m: in local memory
-    volatile int v_kept;
+    // in local memory: o and ps of the units before, their m and power; columns' own powers (`own`)
+    volatile float kept[10 * NT], m_kept[2 * NT], power_kept[2 * NT], power[2 * NT];
     uint64_t minus_m[NT], l[NT], mid[NT];  // pairs of columns
     uint32_t unset = (1u << 2 * NT) - 1;   // columns that have seen nothing: their m counts as 0
     float limit = -INFINITY;               // how far a score may be above its m: kSlack when none is unset
     float v_unit = 1.f, v_limit = 0.f;     // steps of V are multiplied by v_unit (a power of two)
+    float v_floor = 0.f, v_least = 3.402823466e38f;  // steps are to be v_floor or more; the smallest so far
     int v_exp = 0;
+    bool own = false;                      // columns have powers of their own: o is in units of 2^(power - kOwnBits), mid of 2^power
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       minus_m[j] = l[j] = mid[j] = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) ps[j][c] = o[j][0][c] = o[j][1][c] = 0.f;
     }
+    auto unit_of = [&](int column) { return own ? power[column] - kOwnBits : static_cast<float>(v_exp); };
     auto add_kept = [&]() {
-      const float change = pow2(max(-126, min(v_kept - v_exp, 0)));  // V's power of two only grows
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         float m[2];
         f2_unpack(minus_m[j], m[0], m[1]);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float f = ex2(m[c] - m_kept[2 * j + c]) * change;
+          const float f = ex2((m[c] - m_kept[2 * j + c]) + (power_kept[2 * j + c] - unit_of(2 * j + c)));
           auto add = [&](float& x, float y) { x += y == 0.f ? 0.f : y * f; };  // 0 where nothing had been seen
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
@@ -427,108 +446,118 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         }
       }
     };
-#pragma unroll 1
-    for (int i = 0; i < n;) {
-#pragma unroll 1
-      for (const int stop = min(n, (i / kFlush + 1) * kFlush); i < stop; ++i) {
-        const int pos0 = (now.tile + i) * kUnit + warp * kTile;
-        ok = ok && wait_all(&sm.full[stage], parity, p.err);
-        const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
-        // ---- S^T: positions (rows g, g + 8 of each half) x query rows (columns)
-        float s[2][NT][4];
-        uint32_t kw[2][2][4];  // half, row g or g + 8, word
+    // Unit i of the piece.  False (and nothing done): its rows of V need columns' own powers, as they have with kOwn.
+    auto unit = [&](const int i, auto with_own) -> bool {
+      constexpr bool kOwn = decltype(with_own)::value;
+      const int pos0 = (now.tile + i) * kUnit + warp * kTile;
+      ok = ok && wait_all(&sm.full[stage], parity, p.err);
+      const uint32_t halves = sm.there[stage] >> (2 * warp) & 3u;
+      // ---- S^T: positions (rows g, g + 8 of each half) x query rows (columns)
+      float s[2][NT][4];
+      uint32_t kw[2][2][4];  // half, row g or g + 8, word
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
-            kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
-          }
+        for (int r = 0; r < 2; ++r) {
+          const uint4 k = ld_shared_v4(k_ring + stage * (kUnit * 64) + h * 1024 + r * 512);
+          kw[h][r][0] = k.x; kw[h][r][1] = k.y; kw[h][r][2] = k.z; kw[h][r][3] = k.w;
         }
+      }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 4; ++w) {
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            uint32_t a[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t y0 = kw[h][0][w] >> (8 * b);
-              const uint32_t y1 = kw[h][1][w] >> (8 * b);
-              a[h][0] = y0 & 0x000F000Fu;
-              a[h][1] = y1 & 0x000F000Fu;
-              a[h][2] = y0 & 0x00F000F0u;
-              a[h][3] = y1 & 0x00F000F0u;
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              const uint2 y = sm.q[j][2 * w + b][lane];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                if (w == 0 && b == 0) mma16816_first(s[h][j], a[h], y.x, y.y);
-                else mma16816(s[h][j], a[h], y.x, y.y);
-              }
-            }
-          }
-        }
-        // ---- scores above their m; this thread's positions: rows g and g + 8 of half h
-        float sv[2][2], mv[2][2];  // step of V, and what code 7.5 stands for
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + h * 128 + r * 64);
-            const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
-            sv[h][r] = __uint_as_float(sc.y << 16);
-            mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
-            const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              const uint64_t kq = reinterpret_cast<const uint64_t*>(sm.kq)[4 * j + t];
-              const uint64_t qs = reinterpret_cast<const uint64_t*>(sm.qs)[4 * j + t];
-              const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq),
-                                        f2_fma(lk2, qs, minus_m[j]));
-              f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
-            }
-          }
-        }
-        if (halves != 3u || pos0 + kTile > least) {
-          int sees[NT][2];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            sees[j][0] = limit_of(j, 0);
-            sees[j][1] = limit_of(j, 1);
-          }
+        for (int b = 0; b < 2; ++b) {
+          uint32_t a[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            const uint32_t y0 = kw[h][0][w] >> (8 * b);
+            const uint32_t y1 = kw[h][1][w] >> (8 * b);
+            a[h][0] = y0 & 0x000F000Fu;
+            a[h][1] = y1 & 0x000F000Fu;
+            a[h][2] = y0 & 0x00F000F0u;
+            a[h][3] = y1 & 0x00F000F0u;
+          }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int pos = pos0 + 16 * h + g + 8 * r;
-              const bool held = (halves >> h & 1u) && pos < now.s.vis;
-              // a row of V that is no number goes to those that see it by their scores
-              const bool number = fabsf(mv[h][r]) < INFINITY;
-              if (!held || !number) sv[h][r] = mv[h][r] = 0.f;
+          for (int j = 0; j < NT; ++j) {
+            const uint2 y = sm.q[j][2 * w + b][lane];
 #pragma unroll
-              for (int j = 0; j < NT; ++j) {
+            for (int h = 0; h < 2; ++h) {
+              if (w == 0 && b == 0) mma16816_first(s[h][j], a[h], y.x, y.y);
+              else mma16816(s[h][j], a[h], y.x, y.y);
+            }
+          }
+        }
+      }
+      // ---- scores above their m; this thread's positions: rows g and g + 8 of half h
+      float sv[2][2], mv[2][2];  // step of V, and what code 7.5 stands for
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  if (!number) s[h][j][2 * r + c] = NAN;
-                  if (!held || pos >= sees[j][c]) s[h][j][2 * r + c] = -INFINITY;
-                }
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint2 sc = ld_shared_v2(s_ring + stage * (kUnit * 8) + h * 128 + r * 64);
+          const float sk = __uint_as_float(sc.x << 16), lk = __uint_as_float(sc.x & 0xFFFF0000u);
+          sv[h][r] = __uint_as_float(sc.y << 16);
+          mv[h][r] = fmaf(7.5f, sv[h][r], __uint_as_float(sc.y & 0xFFFF0000u));
+          const uint64_t sk2 = f2_pack(sk, sk), lk2 = f2_pack(lk, lk);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint64_t kq = reinterpret_cast<const uint64_t*>(sm.kq)[4 * j + t];
+            const uint64_t qs = reinterpret_cast<const uint64_t*>(sm.qs)[4 * j + t];
+            const uint64_t x = f2_fma(f2_pack(s[h][j][2 * r], s[h][j][2 * r + 1]), f2_mul(sk2, kq),
+                                      f2_fma(lk2, qs, minus_m[j]));
+            f2_unpack(x, s[h][j][2 * r], s[h][j][2 * r + 1]);
+          }
+        }
+      }
+      // of the four threads that have the same positions, each looks after one: V's step and lowest value
+      float step, low;
+      {
+        const uint32_t sc = ld_shared_u32(s_own + stage * (kUnit * 8));
+        step = __uint_as_float(sc << 16);
+        low = __uint_as_float(sc & 0xFFFF0000u);
+      }
+      if (halves != 3u || pos0 + kTile > least) {
+        int sees[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          sees[j][0] = limit_of(j, 0);
+          sees[j][1] = limit_of(j, 1);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int pos = pos0 + 16 * h + g + 8 * r;
+            const bool held = (halves >> h & 1u) && pos < now.s.vis;
+            // a row of V that is no number goes to those that see it by their scores
+            const bool number = fabsf(mv[h][r]) < INFINITY;
+            if (!held || !number) {
+              sv[h][r] = mv[h][r] = 0.f;
+              if (t == 2 * h + r) step = low = NAN;  // neither large nor small
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                if (!number) s[h][j][2 * r + c] = NAN;
+                if (!held || pos >= sees[j][c]) s[h][j][2 * r + c] = -INFINITY;
               }
             }
           }
         }
-        bool grow = false;
+      }
+      const uint32_t p_at = p_lane + p_buf * (R * kPPitch * 2);
+      uint64_t l_now[NT], mid_now[NT];
+      if constexpr (!kOwn) {
+        v_least = fminf(v_least, step);
+        bool grow = step > v_limit || v_least < v_floor || fabsf(low) > kHuge;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          grow |= fmaxf(sv[h][0], sv[h][1]) > v_limit;
 #pragma unroll
           for (int j = 0; j < NT; ++j)
             grow |= fmaxf(fmaxf(s[h][j][0], s[h][j][1]), fmaxf(s[h][j][2], s[h][j][3])) > limit;
         }
         // ---- P, and P step_v to shared memory: [row][position]
-        const uint32_t p_at = p_lane + p_buf * (R * kPPitch * 2);
-        uint64_t l_now[NT], mid_now[NT];
         auto give_p = [&]() {
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
@@ -554,10 +583,15 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         give_p();
         if (any_warp(grow)) {
           // ---- new references, of the CTA: the rows' maxima so far, and a power of two near V's largest step
-          float top = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
+          float top = fmaxf(step, 0.f);
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          if (lane == 0) sm.top_v[warp] = top;
+          for (int off = 1; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const uint32_t small = __reduce_min_sync(0xffffffffu, __float_as_uint(v_least));  // none is negative
+          const bool big = __any_sync(0xffffffffu, fabsf(low) > kHuge || step > kHuge);
+          if (lane == 0) {
+            sm.top_v[warp] = top;
+            sm.least_v[warp] = big ? -1.f : __uint_as_float(small);
+          }
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -569,18 +603,24 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
             }
           }
           all_warps();
+          float change = 1.f, smallest = sm.least_v[0];
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.top_v[w]);
-          float change = 1.f;
-          if (top > v_limit && top < INFINITY) {
-            const int x = max(-120, min(exponent(top), 120));
+          for (int w = 0; w < kWarps; ++w) {
+            top = fmaxf(top, sm.top_v[w]);
+            smallest = fminf(smallest, sm.least_v[w]);
+          }
+          const bool larger = top > v_limit && top < INFINITY;
+          const int x = max(-120, min(exponent(top), 120));
+          if (larger) v_floor = pow2(max(x - kSpreadBits, -126));
+          if (smallest < v_floor) return false;
+          if (larger) {
             if (v_limit > 0.f) {
-              const int d = v_exp - x;
+              const int d = v_exp - (x - kStepBits);
               change = d < -126 ? 0.f : pow2(d);
             }
-            v_exp = x;
-            v_unit = pow2(-x);
-            v_limit = pow2(min(x + 6, 127));
+            v_exp = x - kStepBits;
+            v_unit = pow2(-v_exp);
+            v_limit = pow2(x + 4);
           }
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
@@ -617,47 +657,147 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
           give_p();
           all_warps();
         }
+      } else {
+        // ---- rows' maxima, and their largest terms (of the units before the first of these: their sums), each time anew
+        float ex[2][2];  // exponents of V's rows
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            ex[h][r] = static_cast<float>(max(-126, min(exponent(fmaf(7.5f, sv[h][r], fabsf(mv[h][r]))), 126)));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          l[j] = l_now[j];
-          mid[j] = mid_now[j];
-        }
-        // ---- sums of P step_v: of this warp's positions
+          float middle[2];
+          f2_unpack(mid[j], middle[0], middle[1]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          constexpr uint32_t kOne = 0x3C003C00u;
-          const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
-          uint32_t b[4];
-          ldmatrix(b, p_at + (8 * j * kPPitch + warp * kTile) * 2);
-          mma16816(ps[j], ones, b[0], b[1]);
-          mma16816(ps[j], ones, b[2], b[3]);
-        }
-        // ---- O^T += V^T P^T: of its 32 values 4 g + 2 b (rows g) and 4 g + 2 b + 1 (rows g + 8, codes four bits higher)
+          for (int c = 0; c < 2; ++c) {
+            auto power_of = [](float x, int e) { return x == 0.f ? -1000.f : static_cast<float>(exponent(fabsf(x)) + e); };
+            float term = own ? power[2 * j + c] : fmaxf(power_of(middle[c], 1), power_of(ps[j][c], v_exp + 4));
+            float mx = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < kUnit / 32; ++x) {
-          uint32_t v[4], pb[NT][4];  // of 8 positions each
-          ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + x * 2048);
+            for (int h = 0; h < 2; ++h) {
+              mx = fmaxf(mx, fmaxf(s[h][j][c], s[h][j][2 + c]));
+              term = fmaxf(term, fmaxf(s[h][j][c] + ex[h][0], s[h][j][2 + c] + ex[h][1]));
+            }
 #pragma unroll
-          for (int j = 0; j < NT; ++j) ldmatrix(pb[j], p_at + (8 * j * kPPitch + x * 32) * 2);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const uint32_t y0 = v[2 * h] >> (8 * b), y1 = v[2 * h + 1] >> (8 * b);
-              const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
-#pragma unroll
-              for (int j = 0; j < NT; ++j) mma16816(o[j][b], a, pb[j][2 * h], pb[j][2 * h + 1]);
+            for (int off = 4; off < 32; off <<= 1) {
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              term = fmaxf(term, __shfl_xor_sync(0xffffffffu, term, off));
+            }
+            if (g == 0) {
+              sm.top[warp][8 * j + 2 * t + c] = mx;
+              sm.term[warp][8 * j + 2 * t + c] = term;
             }
           }
         }
-        p_buf ^= 1u;
-        __syncwarp();  // every lane has read the stage
-        if (lane == 0) mbar_arrive(&sm.empty[stage]);
-        if (++stage == S::kStages) {
-          stage = 0;
-          parity ^= 1u;
+        all_warps();
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float was[2], now_m[2], f[2], mid_to[2], to[2];
+          f2_unpack(minus_m[j], was[0], was[1]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int column = 8 * j + 2 * t + c;
+            float mx = -INFINITY, term = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              mx = fmaxf(mx, sm.top[w][column]);
+              term = fmaxf(term, sm.term[w][column]);
+            }
+            const bool first = unset >> (2 * j + c) & 1u;
+            if (first && mx == -INFINITY) mx = 0.f;
+            else unset &= ~(1u << (2 * j + c));
+            if (!first) mx = fmaxf(mx, 0.f);
+            f[c] = first ? 0.f : ex2(-mx);
+            now_m[c] = was[c] - mx;
+            to[c] = fmaxf(ceilf(term - mx), -200.f);
+            // sums of nothing may be multiplied by anything
+            const float o_to = ex2(fminf((own ? power[2 * j + c] : static_cast<float>(v_exp + kOwnBits)) - mx - to[c], 100.f));
+            mid_to[c] = ex2(fminf((own ? power[2 * j + c] : 0.f) - mx - to[c], 100.f));
+            power[2 * j + c] = to[c];
+            ps[j][c] *= o_to;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              o[j][b][c] *= o_to;
+              o[j][b][2 + c] *= o_to;
+            }
+          }
+          minus_m[j] = f2_pack(now_m[0], now_m[1]);
+          l_now[j] = f2_mul(l[j], f2_pack(f[0], f[1]));
+          mid_now[j] = f2_mul(mid[j], f2_pack(mid_to[0], mid_to[1]));
+          // ---- P: V's row by its own power, and that power beside the score's
+          uint32_t x[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float down = pow2(-static_cast<int>(ex[h][r])), step = sv[h][r] * down * static_cast<float>(1 << kOwnBits);
+              const float s0 = s[h][j][2 * r] + (now_m[0] - was[0]), s1 = s[h][j][2 * r + 1] + (now_m[1] - was[1]);
+              const uint64_t e = f2_pack(ex2(s0 + (ex[h][r] - to[0])), ex2(s1 + (ex[h][r] - to[1])));
+              float p0, p1;
+              l_now[j] = f2_add(l_now[j], f2_pack(ex2(s0), ex2(s1)));
+              mid_now[j] = f2_fma(e, f2_pack(mv[h][r] * down, mv[h][r] * down), mid_now[j]);
+              f2_unpack(f2_mul(e, f2_pack(step, step)), p0, p1);
+              x[h][r] = pack_f16x2(p0, p1);
+            }
+          }
+          stmatrix_trans(p_at + (8 * j * kPPitch + warp * kTile) * 2, x[0][0], x[0][1], x[1][0], x[1][1]);
+        }
+        own = true;
+        all_warps();
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        l[j] = l_now[j];
+        mid[j] = mid_now[j];
+      }
+      // ---- sums of P step_v: of this warp's positions
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        constexpr uint32_t kOne = 0x3C003C00u;
+        const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+        uint32_t b[4];
+        ldmatrix(b, p_at + (8 * j * kPPitch + warp * kTile) * 2);
+        mma16816(ps[j], ones, b[0], b[1]);
+        mma16816(ps[j], ones, b[2], b[3]);
+      }
+      // ---- O^T += V^T P^T: of its 32 values 4 g + 2 b (rows g) and 4 g + 2 b + 1 (rows g + 8, codes four bits higher)
+#pragma unroll
+      for (int x = 0; x < kUnit / 32; ++x) {
+        uint32_t v[4], pb[NT][4];  // of 8 positions each
+        ldmatrix_trans(v, v_ring + stage * (kUnit * 64) + x * 2048);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) ldmatrix(pb[j], p_at + (8 * j * kPPitch + x * 32) * 2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t y0 = v[2 * h] >> (8 * b), y1 = v[2 * h + 1] >> (8 * b);
+            const uint32_t a[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma16816(o[j][b], a, pb[j][2 * h], pb[j][2 * h + 1]);
+          }
         }
       }
+      p_buf ^= 1u;
+      __syncwarp();  // every lane has read the stage
+      if (lane == 0) mbar_arrive(&sm.empty[stage]);
+      if (++stage == S::kStages) {
+        stage = 0;
+        parity ^= 1u;
+      }
+      return true;
+    };
+#pragma unroll 1
+    for (int i = 0; i < n;) {
+      const int stop = min(n, (i / kFlush + 1) * kFlush);
+      if (!own) {
+#pragma unroll 1
+        for (; i < stop; ++i)
+          if (!unit(i, std::false_type())) break;
+      }
+#pragma unroll 1
+      for (; i < stop; ++i) unit(i, std::true_type());
       // ---- the sums so far, rounded to nearest: the tensor cores' cuts, all one way, stay those of kFlush units
       if (i > kFlush) add_kept();
       if (i < n) {
@@ -665,8 +805,11 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         for (int j = 0; j < NT; ++j) {
           float m[2];
           f2_unpack(minus_m[j], m[0], m[1]);
-          m_kept[2 * j] = m[0];
-          m_kept[2 * j + 1] = m[1];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            m_kept[2 * j + c] = m[c];
+            power_kept[2 * j + c] = unit_of(2 * j + c);
+          }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             kept[8 * j + c] = o[j][0][c];
@@ -675,7 +818,6 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
             ps[j][c] = o[j][0][c] = o[j][1][c] = 0.f;
           }
         }
-        v_kept = v_exp;
       }
     }
 
@@ -701,7 +843,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
     }
     all_warps();
     const bool whole = now.tile == 0 && now.end == now.s.tiles;
-    const float unit_even = 16777216.f, unit_odd = 1048576.f, back = pow2(v_exp);
+    const float unit_even = 16777216.f, unit_odd = 1048576.f, back = own ? 1.f / (1 << kOwnBits) : pow2(v_exp);
     float* const part = p.partials + static_cast<int64_t>(2 * blockIdx.x + (pieces > 0 ? 1 : 0)) * (R * (kHeadDim + 2));
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -728,6 +870,11 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
         const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);  // 0 for a row that sees nothing
 #pragma unroll
         for (int k = 0; k < 4; ++k) y[k] *= inv;
+        if (own) {  // in two steps: the power may be beyond fp32's
+          const int e = static_cast<int>(power[2 * j + c]), e0 = e / 2;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = y[k] * pow2(e0) * pow2(e - e0);
+        }
         if (whole) {
           const int token = token_of(p, r);
           const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]);

@@ -3,7 +3,8 @@
 // Part c has the output o_c of its own positions, and their sum l_c for the reference maximum m_c; with M = max m_c
 //   out = sum_c w_c o_c,  w_c = 2^(m_c - M) l_c / sum_d 2^(m_d - M) l_d,
 // added in the order of the parts.  Means weighted by 0 .. 1 stay inside fp32 wherever the values do; sums of p v
-// times a part's l would not.  CTA i takes what the cut of CTA i says.  Bound by latency (descriptor, maxima, sums,
+// times a part's l would not.  2^(m_c - M) is put in as its root, twice: it may be below fp32's range where its product with
+// large values is not.  CTA i takes what the cut of CTA i says.  Bound by latency (descriptor, maxima, sums,
 // output: three dependent accesses of L2), so few rows with many parts are shared by up to four CTAs and their warps,
 // with eight parts of a warp in flight, and many rows with few parts go four to a warp (4 rows of 55 parts: 2 us; one
 // CTA for a pair, maxima first: 6).
@@ -16,12 +17,14 @@ constexpr int kWarps = 8;
 constexpr int kFewBlocks = 4;  // CTAs that share the rows of a cut
 constexpr int kAtOnce = 8;  // parts of which a warp has the loads in flight
 
-__device__ __forceinline__ void add_part(float4& y, const float4& x, float w) {
-  y.x = fmaf(x.x, w, y.x);
-  y.y = fmaf(x.y, w, y.y);
-  y.z = fmaf(x.z, w, y.z);
-  y.w = fmaf(x.w, w, y.w);
+// y += x w root.
+__device__ __forceinline__ void add_part(float4& y, const float4& x, float w, float root) {
+  y.x = fmaf(x.x * root, w, y.x);
+  y.y = fmaf(x.y * root, w, y.y);
+  y.z = fmaf(x.z * root, w, y.z);
+  y.w = fmaf(x.w * root, w, y.w);
 }
+__device__ __forceinline__ float root_of(float m, float top) { return ex2(0.5f * (m - top)); }  // of 2^(m - top)
 
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : __fdiv_rn(1.f, sum); }
 
@@ -71,16 +74,20 @@ __device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4Join
       const float was = mx;
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) mx = fmaxf(mx, ml[i].x);
-      const float before = sum * ex2(was - mx);
-      sum = before;
+      const float old_root = root_of(was, mx), before = sum * old_root;
+      sum = before * old_root;
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) sum += ml[i].y *= ex2(ml[i].x - mx);
+      for (int i = 0; i < kAtOnce; ++i) {
+        ml[i].x = root_of(ml[i].x, mx);
+        ml[i].y *= ml[i].x;
+        sum = fmaf(ml[i].y, ml[i].x, sum);
+      }
       const float inv = inverse(sum);
       const float4 old = y;
       y = make_float4(0.f, 0.f, 0.f, 0.f);
-      add_part(y, old, before * inv);
+      add_part(y, old, before * inv, old_root);
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) add_part(y, x[i], ml[i].y * inv);
+      for (int i = 0; i < kAtOnce; ++i) add_part(y, x[i], ml[i].y * inv, ml[i].x);
     }
     if (share > 1) {
       __syncthreads();  // the rows before these have been read
@@ -94,8 +101,10 @@ __device__ __forceinline__ void join_few(const Int4AttnParams& p, const Int4Join
         sum = 0.f;
         for (int w = 0; w < share; ++w) sum = fmaf(sum_ml[warp + w].y, ex2(sum_ml[warp + w].x - top), sum);
         const float inv = inverse(sum);
-        for (int w = 0; w < share; ++w)
-          add_part(y, sum_o[warp + w][lane], sum_ml[warp + w].y * ex2(sum_ml[warp + w].x - top) * inv);
+        for (int w = 0; w < share; ++w) {
+          const float root = root_of(sum_ml[warp + w].x, top);
+          add_part(y, sum_o[warp + w][lane], sum_ml[warp + w].y * root * inv, root);
+        }
       }
     }
     if (mine && turn == 0) store_row(p, cut, row, lane, y);
@@ -150,10 +159,14 @@ __device__ __forceinline__ void join_many(const Int4AttnParams& p, const Int4Joi
     float4 x[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4*>(part(j) + (row0 + k) * kHeadDim + 4 * lane);
-    add_part(y[0], x[0], a.y * ex2(a.x - mx[0]) * inv[0]);
-    add_part(y[1], x[1], a.w * ex2(a.z - mx[1]) * inv[1]);
-    add_part(y[2], x[2], b.y * ex2(b.x - mx[2]) * inv[2]);
-    add_part(y[3], x[3], b.w * ex2(b.z - mx[3]) * inv[3]);
+    const float r0 = root_of(a.x, mx[0]);
+    add_part(y[0], x[0], a.y * r0 * inv[0], r0);
+    const float r1 = root_of(a.z, mx[1]);
+    add_part(y[1], x[1], a.w * r1 * inv[1], r1);
+    const float r2 = root_of(b.x, mx[2]);
+    add_part(y[2], x[2], b.y * r2 * inv[2], r2);
+    const float r3 = root_of(b.z, mx[3]);
+    add_part(y[3], x[3], b.w * r3 * inv[3], r3);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)

@@ -135,3 +135,67 @@ def test_chunk_rows_of_any_size_at_all(new):
         value *= torch.exp2(torch.randint(-120, 120, (n, 2, 1), generator=_gen(11), device="cuda").double())
         _peaks(key, q, range(0, n, max(1, n // 30)))
         _check(q.to(torch.bfloat16), *_filled(key, value, 32), n)
+
+
+# ------------------------------------------------------------ the split-context kernel: up to 32 rows of a kv head
+@pytest.mark.parametrize("new,heads", [(1, 4), (1, 8), (3, 4), (5, 4), (8, 4)])
+@pytest.mark.parametrize("k_power,v_power", POWERS, ids=str)
+def test_few_rows_over_bf16s_range(new, heads, k_power, v_power):
+    n, kv = 333, 1
+    key, value = (_randn(n, kv, 128, seed=s).clamp(-3, 3) * 2.0 ** (p - 1) for s, p in ((4, k_power), (5, v_power)))
+    q = (1.5 * _randn(new, heads, 128, seed=6) * 2.0 ** (1 - k_power)).to(torch.bfloat16)
+    out = _check(q, *_filled(key, value, 16), n)
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("new,n", [(2, 400), (5, 9000), (8, 40000)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("power", [5, 10, 14, 20, 60, 100, -20, -100])
+def test_few_rows_beside_a_row_of_another_size(new, n, which, power):
+    key, value, q = _ordinary(n, 1, 4, new)
+    (key if which == "k" else value)[-1] *= 2.0 ** power
+    _check(q.to(torch.bfloat16), *_filled(key, value, 64), n, slice(0, -1))
+
+
+@pytest.mark.parametrize("new,heads", [(1, 4), (1, 32), (8, 4)])
+@pytest.mark.parametrize("powers", [{0: -9}, {0: -40, 500: 5}, {3: 12}, {0: 40, 130: -40, 700: 3}, {5: "zero"},
+                                    {130: -20, 131: 20, 300: 0, 600: -20}, {0: "zero", 1: "zero", 2: -126, 600: 126}], ids=str)
+@pytest.mark.parametrize("n", [1000, 30000])
+def test_few_rows_values_of_many_sizes(new, heads, powers, n):
+    """Every query row looks at one position; tiles with a row of another size and without take turns."""
+    key, value, q = _ordinary(n, 1, heads, new)
+    value.clamp_(-1, 1)
+    for at, power in powers.items():
+        value[at] *= 0.0 if power == "zero" else 2.0 ** power
+    places = list(powers) + [1, 129, 400, 801, n - 9]
+    for i in range(new * heads):
+        key[places[i % len(places)], 0] = q.view(-1, 128)[i] * 3
+    _check(q.to(torch.bfloat16), *_filled(key, value, 16), n)
+
+
+@pytest.mark.parametrize("new,heads", [(1, 4), (5, 4), (8, 4)])
+@pytest.mark.parametrize("n", [200, 5000, 300000])
+def test_few_rows_of_any_size_at_all(new, heads, n):
+    key, value, q = _ordinary(n, 1, heads, new)
+    value *= torch.exp2(torch.randint(-120, 120, (n, 1, 1), generator=_gen(11), device="cuda").double())
+    step = max(1, n // 30)
+    for i in range(new * heads):
+        key[i % 30 * step, 0] = q.view(-1, 128)[i] * 3
+    _check(q.to(torch.bfloat16), *_filled(key, value, 32), n)
+
+
+def test_few_rows_constant_rows_and_none():
+    """Steps of zero beside others, and a cache of zeros."""
+    key, value, q = _ordinary(500, 1, 4, 1)
+    value[::3] = value[::3, :, :1]
+    _check(q.to(torch.bfloat16), *_filled(key, value, 32), 500)
+    value[:] = 0
+    out = _check(q.to(torch.bfloat16), *_filled(key, value, 32), 500)
+    assert torch.all(out == 0)
+
+
+def test_few_rows_huge_constant_rows():
+    """Steps of zero all through, and lowest values whose sum passes fp32's range."""
+    key, value, q = _ordinary(5000, 1, 4, 1)
+    value = value[:, :, :1].abs().clamp(1, 2).expand(-1, -1, 128) * 2.0 ** 120
+    _check((0.1 * q).to(torch.bfloat16), *_filled(key, value, 32), 5000)
