@@ -29,16 +29,18 @@
 // c - 7.5 is the product with c and 7.5 times the same product with ones: taken about the middle of the codes, the
 // roundings of P and the cuts of the tensor cores' sums (2^-24 of each partial sum, all one way) are in proportion to
 // the values and not to their distance from the row's lowest one.  A warp takes the ones of its own 32 positions, so
-// their cuts are not those of the other products; every 64 units the sums so far are put aside and later added with
-// rounding to nearest, so that the cuts do not grow with the context (32,768 positions: 1.8e-3 off in the 2-norm, all
-// but the output's own rounding; 5.3e-3 without that, 2.4e-3 and 1 % slower with the ones of all positions in one warp).
-// The loop over units stays as it is: a branch in it cost 5 %.
+// their cuts are not those of the other products and do not cancel them; every 8 units the sums so far are put aside and
+// later added with rounding to nearest, so that the cuts stay those of 64 instructions and do not grow with the context.
+// Off in the 2-norm, of which the output's own rounding is 1.66e-3: 32,768 positions 1.70e-3, 131,072 1.84e-3 (every 64
+// units: 1.86e-3 to 2.07e-3 and 2.05e-3, 2.5 % faster; every 16: 1.72e-3 and 1.95e-3, 1 % faster).  The ones of all positions in
+// one warp cancel more (every 32 units 1.70e-3 and 1.83e-3), but decode takes 4 % longer and verification 9 %.
 //
 // Precision: scores, statistics and sums in fp32; P step is rounded once, to f16 (2^-12), after its row's
 // reference maximum and a power of two near the largest step of V so far are taken out, so it stays below 2^15.  That power
 // is the CTA's, and so comes from rows as well that a query row does not look at.  Where steps of V differ by more than
-// some 2^15 (or are zero beside others), or values pass 2^90, the rest of the piece is done with a power for each query row instead, that of its own largest
-// p |v| so far, found with one more exchange of maxima for each unit; what a row gets is then as exact as its own largest terms.
+// some 2^15 (or are zero beside others), or values pass 2^90, the rest of the piece is done with a power for each query row
+// instead, that of its own largest p |v| so far, found with an exchange of maxima in every unit; what a row gets is then as
+// exact as its own largest terms.
 #include <atomic>
 #include <climits>
 #include <type_traits>
@@ -60,7 +62,7 @@ constexpr int kSpreadBits = 15;          // and the smallest 2^-15 of what the l
 constexpr float kHuge = 0x1p90f;        // sums over the positions of larger values could pass fp32's range
 constexpr int kOwnBits = 14;            // of a query row's own power: P step < 2^13
 constexpr int kPieceUnits = 1;          // what a pair costs beside its tiles, in units of a tile
-constexpr int kFlush = 64;              // units whose products with V the tensor cores add up
+constexpr int kFlush = 8;              // units whose products with V the tensor cores add up
 
 constexpr int kWarps = 4;                    // that compute; one more loads
 constexpr int kThreads = kWarps * 32 + 32;

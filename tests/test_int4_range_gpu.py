@@ -199,3 +199,41 @@ def test_few_rows_huge_constant_rows():
     key, value, q = _ordinary(5000, 1, 4, 1)
     value = value[:, :, :1].abs().clamp(1, 2).expand(-1, -1, 128) * 2.0 ** 120
     _check((0.1 * q).to(torch.bfloat16), *_filled(key, value, 32), 5000)
+
+
+def _sum_of_sizes(q, cache, table, n):
+    """sum p |v| of query rows that see nearly all of n positions."""
+    (kc, ks, kl), (vc, vs, vl), _ = int4.sequence(*cache, table, n)
+    group = q.shape[1] // kc.shape[1]
+    out = torch.empty(q.shape, dtype=torch.float64, device="cuda")
+    for h in range(q.shape[1]):
+        g = h // group
+        p = torch.softmax(q[:, h].double() @ (kl[:, g] + ks[:, g] * kc[:, g]).T * SCALE, -1)
+        out[:, h] = p @ (vl[:, g] + vs[:, g] * vc[:, g]).abs()
+    return out
+
+
+@pytest.mark.parametrize("new", [1, 5])
+def test_few_rows_cuts_do_not_grow_with_the_context(new):
+    """So many sequences (on the same pages) that a CTA has all units of a pair: beside the output's rounding, what the tensor
+    cores cut off.  Each instruction cuts up to 17 terms at 2^-24 of the largest, 2^-25 on average; between two times
+    that sums are put aside there are 64 instructions, on sums that grow from zero: 64 * 17 * 2^-25 / 2 = 2^-15.9 of
+    sum p |v| in all."""
+    from nanovllm_b200.int4_cache import int4_decode_attention, int4_prefill_attention
+    n, kv, heads, seqs, block = 32768, 8, 32, 64, 256
+    key, value = _randn(n, kv, 128, seed=21), _randn(n, kv, 128, seed=22)
+    q = (1.5 * _randn(seqs * new, heads, 128, seed=23)).to(torch.bfloat16)
+    cache, table = _filled(key, value, block)
+    tables = table.repeat(seqs, 1)
+    if new == 1:
+        out = int4_decode_attention(q, *cache, tables, torch.full((seqs,), n, dtype=torch.int32, device="cuda"), SCALE)
+    else:
+        out = int4_prefill_attention(q, *cache, tables, _cum([new] * seqs), _cum([n] * seqs), new, n, SCALE)
+    far, rounding, room = 0.0, 0.0, 0.0
+    for i in (0, 31, 63):
+        at = slice(i * new, (i + 1) * new)
+        ref, _ = int4.attention_norm(q[at], *cache, table, n, SCALE)
+        far += float((out[at].double() - ref).square().sum())
+        rounding += float((ref.to(torch.bfloat16).double() - ref).square().sum())
+        room += float(_sum_of_sizes(q[at], cache, table, n).square().sum())
+    assert (far - rounding) ** 0.5 <= 2.0 ** -15.9 * room ** 0.5
