@@ -29,11 +29,12 @@
 // c - 7.5 is the product with c and 7.5 times the same product with ones: taken about the middle of the codes, the
 // roundings of P and the cuts of the tensor cores' sums (2^-24 of each partial sum, all one way) are in proportion to
 // the values and not to their distance from the row's lowest one.  A warp takes the ones of its own 32 positions, so
-// their cuts are not those of the other products and do not cancel them; every 8 units the sums so far are put aside and
-// later added with rounding to nearest, so that the cuts stay those of 64 instructions and do not grow with the context.
-// Off in the 2-norm, of which the output's own rounding is 1.66e-3: 32,768 positions 1.70e-3, 131,072 1.84e-3 (every 64
-// units: 1.86e-3 to 2.07e-3 and 2.05e-3, 2.5 % faster; every 16: 1.72e-3 and 1.95e-3, 1 % faster).  The ones of all positions in
-// one warp cancel more (every 32 units 1.70e-3 and 1.83e-3), but decode takes 4 % longer and verification 9 %.
+// their cuts are not those of the other products and do not cancel them; every 8 units (16 for more than 16 rows) the sums
+// so far are put aside and later added with rounding to nearest, so that the cuts stay those of 64 instructions and do
+// not grow with the context.  Off in the 2-norm, of which the output's own rounding is 1.66e-3: decode of 32,768 positions
+// 1.70e-3, of 131,072 1.84e-3 (every 64 units: 1.86e-3 and 2.05e-3, 2.5 % faster; every 16: 1.72e-3 and 1.95e-3, 1 %
+// faster).  The ones of all positions in one warp cancel more (every 32 units 1.70e-3 and 1.83e-3), but decode takes 4 %
+// longer and verification 9 %.
 //
 // Precision: scores, statistics and sums in fp32; P step is rounded once, to f16 (2^-12), after its row's
 // reference maximum and a power of two near the largest step of V so far are taken out, so it stays below 2^15.  That power
@@ -62,7 +63,6 @@ constexpr int kSpreadBits = 15;          // and the smallest 2^-15 of what the l
 constexpr float kHuge = 0x1p90f;        // sums over the positions of larger values could pass fp32's range
 constexpr int kOwnBits = 14;            // of a query row's own power: P step < 2^13
 constexpr int kPieceUnits = 1;          // what a pair costs beside its tiles, in units of a tile
-constexpr int kFlush = 8;              // units whose products with V the tensor cores add up
 
 constexpr int kWarps = 4;                    // that compute; one more loads
 constexpr int kThreads = kWarps * 32 + 32;
@@ -70,14 +70,17 @@ constexpr int kUnit = kTile * kWarps;        // positions per unit
 constexpr int kParts = kUnit / 16;           // parts of a unit that lie in one page each
 
 // A kernel by the rows of a group: NT planes of 8.  As many CTAs on an SM as have room for their sums without spilling
-// (verification with 20 rows: three CTAs of 128 registers 217 us, two of 168 209; 8 rows, at an earlier step: four with
-// two stages 393 us, three with three 382).
+// (verification with 20 rows: three CTAs of 128 registers and two stages 242 us, two of 168 with three 222; 64 sequences of
+// 32,768 with 32 rows: 1,413 and 1,090 us).  kFlush: units whose products with V the tensor cores add up; more
+// registers take longer to be put aside (24 rows at 32,768 positions, every 8 units: 800 us and 1.70e-3 off, every 16: 780
+// and 1.72e-3).
 template <int NT_>
 struct Shape {
   static constexpr int NT = NT_;
   static constexpr int R = 8 * NT;
   static constexpr int kCtas = NT < 3 ? 3 : 2;    // on an SM
   static constexpr int kStages = 3;
+  static constexpr int kFlush = NT < 3 ? 8 : 16;
 };
 
 constexpr int kPPitch = kUnit + 8;  // bank spread
@@ -792,7 +795,7 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
     };
 #pragma unroll 1
     for (int i = 0; i < n;) {
-      const int stop = min(n, (i / kFlush + 1) * kFlush);
+      const int stop = min(n, (i / S::kFlush + 1) * S::kFlush);
       if (!own) {
 #pragma unroll 1
         for (; i < stop; ++i)
@@ -800,8 +803,8 @@ __device__ __forceinline__ void compute(const Int4AttnParams& p, Smem<S>& sm, Cu
       }
 #pragma unroll 1
       for (; i < stop; ++i) unit(i, std::true_type());
-      // ---- the sums so far, rounded to nearest: the tensor cores' cuts, all one way, stay those of kFlush units
-      if (i > kFlush) add_kept();
+      // ---- the sums so far, rounded to nearest: the tensor cores' cuts, all one way, stay those of so many
+      if (i > S::kFlush) add_kept();
       if (i < n) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {

@@ -213,12 +213,12 @@ def _sum_of_sizes(q, cache, table, n):
     return out
 
 
-@pytest.mark.parametrize("new", [1, 5])
-def test_few_rows_cuts_do_not_grow_with_the_context(new):
+@pytest.mark.parametrize("new,instructions", [(1, 64), (5, 128)])
+def test_few_rows_cuts_do_not_grow_with_the_context(new, instructions):
     """So many sequences (on the same pages) that a CTA has all units of a pair: beside the output's rounding, what the tensor
     cores cut off.  Each instruction cuts up to 17 terms at 2^-24 of the largest, 2^-25 on average; between two times
-    that sums are put aside there are 64 instructions, on sums that grow from zero: 64 * 17 * 2^-25 / 2 = 2^-15.9 of
-    sum p |v| in all."""
+    that sums are put aside there are 64 or 128 instructions, on sums that grow from zero: 64 * 17 * 2^-25 / 2 = 2^-15.9 of
+    sum p |v| in all, or twice that."""
     from nanovllm_b200.int4_cache import int4_decode_attention, int4_prefill_attention
     n, kv, heads, seqs, block = 32768, 8, 32, 64, 256
     key, value = _randn(n, kv, 128, seed=21), _randn(n, kv, 128, seed=22)
@@ -236,4 +236,4 @@ def test_few_rows_cuts_do_not_grow_with_the_context(new):
         far += float((out[at].double() - ref).square().sum())
         rounding += float((ref.to(torch.bfloat16).double() - ref).square().sum())
         room += float(_sum_of_sizes(q[at], cache, table, n).square().sum())
-    assert (far - rounding) ** 0.5 <= 2.0 ** -15.9 * room ** 0.5
+    assert (far - rounding) ** 0.5 <= instructions * 17 * 2.0 ** -26 * room ** 0.5
