@@ -908,18 +908,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     total += sm.scan[w];
   }
   before -= mine;
+  // Nothing to be joined until the CTA's last piece says so: the joining kernel reads this of every CTA, of one as well
+  // whose waits have given up, and the workspace holds anything.
+  if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
   if (total > INT_MAX) {  // hours of work: what follows counts in 32 bits
-    if (tid == 0) {
-      atomicExch(p.err, kDevErrTooLarge);
-      reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
-    }
+    if (tid == 0) atomicExch(p.err, kDevErrTooLarge);
     return;
   }
   const int ctas = min(static_cast<int>(gridDim.x), static_cast<int>(total));
-  if (static_cast<int>(blockIdx.x) >= ctas) {
-    if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
-    return;
-  }
+  if (static_cast<int>(blockIdx.x) >= ctas) return;
   const Ranges ranges(static_cast<int>(total), ctas);
   const int u0 = ranges.begin(blockIdx.x), u1 = ranges.begin(blockIdx.x + 1);
   if (before <= u0 && u0 < before + mine) {
@@ -959,8 +956,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     c.until = u1;
     c.set_end();
   }
-  if (c.tile >= c.end) {  // none but what is counted for an item beside its tiles
-    if (tid == 0) reinterpret_cast<Cut*>(p.cuts)[blockIdx.x].parts = 0;
+  if (c.tile >= c.end) {
+    // none but what is counted for an item beside its tiles
   } else if (warp < kUnpackWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     softmax_role(p, sm, c, ranges, warp >> 2, tid);

@@ -1,0 +1,55 @@
+"""Calls of the rotary operators and of attention over the 4-bit cache that the documentation allows and that are easily
+forgotten."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+SCALE = 128 ** -0.5
+
+
+def _randn(*shape, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(torch.bfloat16)
+
+
+def _ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _filled(blocks, block, kv, seed):
+    from nanovllm_b200.int4_cache import new_kvcache_int4, store_kvcache_int4
+    cache = new_kvcache_int4(blocks, block, kv)
+    n = blocks * block
+    store_kvcache_int4(_randn(n, kv, 128, seed=seed), _randn(n, kv, 128, seed=seed + 1), *cache,
+                       torch.arange(n, dtype=torch.int32, device="cuda"))
+    return cache
+
+
+@pytest.mark.parametrize("news,lens", [([1], [3000]), ([5, 1], [900, 40]), ([300, 40, 0], [3000, 800, 16]),
+                                       ([700], [700])], ids=str)
+def test_workspace_may_hold_anything(news, lens):
+    """The joining kernel goes by what the attention kernels have written, whatever stood there."""
+    from nanovllm_b200 import _lib
+    block, kv, heads = 16, 2, 8
+    blocks = sum(-(-n // block) for n in lens)
+    cache = _filled(blocks, block, kv, 1)
+    table = torch.full((len(lens), max(-(-n // block) for n in lens)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for i, n in enumerate(lens):
+        pages = -(-n // block)
+        table[i, :pages] = torch.arange(at, at + pages, device="cuda")
+        at += pages
+    q = _randn(sum(news), heads, 128, seed=3)
+    cum = lambda v: _ints(*[sum(v[:i]) for i in range(len(v) + 1)])  # noqa: E731
+    cq, ck = cum(news), cum(lens)
+    nbytes = _lib.lib.fp8attn_int4_workspace_bytes(len(news), heads, kv, max(news))
+    outs = []
+    for fill in (0, 255, 127, 1):
+        work = torch.full((nbytes,), fill, dtype=torch.uint8, device="cuda")
+        out = torch.empty_like(q)
+        assert _lib.lib.fp8attn_int4_prefill(
+            out.data_ptr(), q.data_ptr(), q.stride(0), *(t.data_ptr() for t in cache), table.data_ptr(), table.stride(0),
+            table.shape[1], cq.data_ptr(), ck.data_ptr(), len(news), max(news), heads, kv, 128, blocks, block, SCALE,
+            work.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream) == 0
+        outs.append(out)
+    assert all(torch.equal(o, outs[0]) for o in outs) and torch.isfinite(outs[0]).all()
