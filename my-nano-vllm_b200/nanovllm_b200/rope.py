@@ -60,6 +60,9 @@ def apply_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
         k_tokens, kv_heads, k_width = k.shape
         k_ts, k_hs, unit = k.stride()
         assert k_tokens == N and k_width == D and unit == 1
+        if heads == 0:  # all there is to turn is k
+            return (q if inplace else torch.empty_like(q),
+                    apply_rope(k, None, positions, cos_sin_cache, interleaved, inplace)[0])
         k_out = k if inplace else _empty((N, kv_heads, D), (kv_heads * D, D, 1), dtype=dtype, device=on)
         k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
     q_out = q if inplace else _empty((N, heads, D), (heads * D, D, 1), dtype=dtype, device=on)

@@ -53,3 +53,19 @@ def test_workspace_may_hold_anything(news, lens):
             work.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream) == 0
         outs.append(out)
     assert all(torch.equal(o, outs[0]) for o in outs) and torch.isfinite(outs[0]).all()
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("tokens", [0, 1, 300])
+def test_rope_of_keys_alone(tokens, inplace):
+    """q without heads: k is turned all the same."""
+    from nanovllm_b200.rope import apply_rope, rope_table
+    table, pos = rope_table(500, 128), torch.arange(tokens, device="cuda")
+    k = _randn(tokens, 4, 128, seed=5)
+    want, none = apply_rope(k, None, pos, table)
+    assert none is None
+    q, given = torch.empty(tokens, 0, 128, dtype=torch.bfloat16, device="cuda"), k.clone()
+    torch.full_like(k, 7.0)  # freed at once: an output that nobody writes would hold it
+    got_q, got = apply_rope(q, given, pos, table, inplace=inplace)
+    assert got_q.shape == q.shape and torch.equal(got, want)
+    assert not inplace or got is given
