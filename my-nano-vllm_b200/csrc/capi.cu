@@ -1086,7 +1086,8 @@ int check_int4_attention(const void* out, const void* q, int64_t q_row_stride, c
                 num_kv_heads);
   if (num_seqs < 0 || num_seqs > 65535)
     return fail(FP8ATTN_EINVAL, "num_seqs must be in [0, 65535] (got %d)", num_seqs);
-  if (!out || !q || !block_tables) return fail(FP8ATTN_EINVAL, "null pointer argument");
+  // a table of no columns has no address
+  if (!out || !q || (!block_tables && max_num_blocks != 0)) return fail(FP8ATTN_EINVAL, "null pointer argument");
   if (!aligned16(out) || !aligned16(q) || q_row_stride % 8 != 0 ||
       q_row_stride < static_cast<int64_t>(num_heads) * fp8attn::kHeadDim)
     return fail(FP8ATTN_EINVAL, "q/out must be 16-byte aligned with rows of num_heads*128");

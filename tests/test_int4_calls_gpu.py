@@ -69,3 +69,15 @@ def test_rope_of_keys_alone(tokens, inplace):
     got_q, got = apply_rope(q, given, pos, table, inplace=inplace)
     assert got_q.shape == q.shape and torch.equal(got, want)
     assert not inplace or got is given
+
+
+def test_block_table_without_columns():
+    """Nothing is seen, as with a table of -1."""
+    from nanovllm_b200.int4_cache import int4_decode_attention, int4_prefill_attention
+    cache, table = _filled(2, 16, 2, 6), torch.empty(3, 0, dtype=torch.int32, device="cuda")
+    out = int4_decode_attention(_randn(3, 8, 128, seed=7), *cache, table, _ints(0, 5, 0), SCALE)
+    assert out.shape == (3, 8, 128) and torch.all(out == 0)
+    for new in (2, 100):
+        out = int4_prefill_attention(_randn(3 * new, 8, 128, seed=8), *cache, table, _ints(0, new, 2 * new, 3 * new),
+                                     _ints(0, 0, 30, 30), new, 30, SCALE)
+        assert torch.all(out == 0)
