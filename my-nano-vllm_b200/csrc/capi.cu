@@ -1250,7 +1250,14 @@ static int int4_plan(Int4Plan* plan, int group, int max_q) {
 }
 
 int64_t fp8attn_int4_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int max_seqlen_q) {
-  if (num_seqs < 0 || num_seqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads) return -1;
+  if (num_seqs < 0 || num_seqs > 65535) {
+    fail(FP8ATTN_EINVAL, "num_seqs must be in [0, 65535] (got %d)", num_seqs);
+    return -1;
+  }
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads) {
+    fail(FP8ATTN_EINVAL, "num_heads (%d) must be a positive multiple of num_kv_heads (%d)", num_heads, num_kv_heads);
+    return -1;
+  }
   Int4Plan plan;
   if (int4_plan(&plan, num_heads / num_kv_heads, max_seqlen_q < 1 ? 1 : max_seqlen_q)) return -1;
   return plan.bytes;

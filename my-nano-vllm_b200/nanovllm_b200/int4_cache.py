@@ -121,8 +121,11 @@ def load_kvcache_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scale: to
 
 @functools.lru_cache(maxsize=1024)
 def _scratch_bytes(device: int, num_seqs: int, heads: int, kv_heads: int, max_q: int) -> int:
-    """On the current device, which ``device`` stands for."""
-    return _lib.lib.fp8attn_int4_workspace_bytes(num_seqs, heads, kv_heads, max_q)
+    """On the current device, which ``device`` stands for.  A failure is raised, and so not remembered."""
+    nbytes = _lib.lib.fp8attn_int4_workspace_bytes(num_seqs, heads, kv_heads, max_q)
+    if nbytes < 0:
+        _lib.check(_lib.EINVAL)
+    return nbytes
 
 
 def int4_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -163,7 +166,7 @@ def int4_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         return out
     _INT4_DEVICES.add(device)
     nbytes = _scratch_bytes(device, batch, heads, kv_heads, 1)
-    scratch = _empty((max(nbytes, 0),), (1,), dtype=_U8, device=on)
+    scratch = _empty((nbytes,), (1,), dtype=_U8, device=on)
     # the row stride of a single row is never used, and torch leaves it arbitrary
     rc = _decode(out.data_ptr(), q.data_ptr(), row if batch > 1 else width, k_cache.data_ptr(),
                  v_cache.data_ptr(), kv_scale.data_ptr(), block_tables.data_ptr(),
@@ -218,7 +221,7 @@ def int4_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     max_q = min(int(max_seqlen_q), tokens)
     _INT4_DEVICES.add(device)
     nbytes = _scratch_bytes(device, num_seqs, heads, kv_heads, max_q)
-    scratch = _empty((max(nbytes, 0),), (1,), dtype=_U8, device=on)
+    scratch = _empty((nbytes,), (1,), dtype=_U8, device=on)
     rc = _prefill(out.data_ptr(), q.data_ptr(), row if tokens > 1 else width,
                   k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(),
                   block_tables.data_ptr(), table_row if num_seqs > 1 else columns, columns,

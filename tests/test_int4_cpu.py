@@ -236,3 +236,31 @@ def test_restated_attention_is_softmax_of_the_rows():
         s = s.masked_fill(torch.arange(n)[None] > torch.arange(n - 5, n)[:, None], -math.inf)
         assert torch.allclose(out[:, h], torch.softmax(s, -1) @ (vl + vs * vc)[:, h // 2], rtol=1e-12, atol=1e-13)
     assert torch.all(bound > 0) and torch.all(bound < 0.02)
+
+
+def test_a_failed_size_is_asked_for_again(monkeypatch):
+    """What the workspace needs is remembered, that it could not be had is not."""
+    answers, asked = [-1, -1, 4096], []
+
+    class Lib:
+        def fp8attn_int4_workspace_bytes(self, *args):
+            asked.append(args)
+            return answers[len(asked) - 1]
+
+        fp8attn_last_error = _lib.lib.fp8attn_last_error
+
+    monkeypatch.setattr(_lib, "lib", Lib())
+    int4_cache._scratch_bytes.cache_clear()
+    for _ in range(2):
+        with pytest.raises(RuntimeError):
+            int4_cache._scratch_bytes(0, 3, 8, 2, 1)
+    assert int4_cache._scratch_bytes(0, 3, 8, 2, 1) == 4096 == int4_cache._scratch_bytes(0, 3, 8, 2, 1)
+    assert len(asked) == 3
+    int4_cache._scratch_bytes.cache_clear()
+
+
+@pytest.mark.parametrize("args,msg", [((-1, 32, 8, 1), "num_seqs"), ((65536, 32, 8, 1), "num_seqs"),
+                                      ((4, 30, 8, 1), "multiple"), ((4, 32, 0, 1), "multiple")])
+def test_workspace_refusals_say_why(args, msg):
+    assert _lib.lib.fp8attn_int4_workspace_bytes(*args) == -1
+    assert msg in _message()
