@@ -36,6 +36,7 @@
 #include "int4_attention.cuh"
 #include "tcgen05.cuh"
 
+#include <atomic>
 #include <climits>
 
 namespace fp8attn {
@@ -997,8 +998,16 @@ cudaError_t launch_int4_prefill(Int4AttnParams p, const CUtensorMap& map_k, cons
   p.two_heads = 2 % p.group;
   p.unit_pages = kTile / p.block_size;
   p.unit_rest = kTile % p.block_size;
-  cudaError_t e = cudaFuncSetAttribute(int4_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  constexpr int kMaxDevices = 64;
+  static std::atomic<bool> prepared[kMaxDevices];  // the kernel's shared memory asked for, once on each device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev >= kMaxDevices || !prepared[dev].load(std::memory_order_relaxed)) {
+    e = cudaFuncSetAttribute(int4_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) prepared[dev].store(true, std::memory_order_relaxed);
+  }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
