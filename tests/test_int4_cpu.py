@@ -264,3 +264,33 @@ def test_a_failed_size_is_asked_for_again(monkeypatch):
 def test_workspace_refusals_say_why(args, msg):
     assert _lib.lib.fp8attn_int4_workspace_bytes(*args) == -1
     assert msg in _message()
+
+
+def _filled_cpu(n, kv, block, seed, spread=0.0):
+    g = torch.Generator().manual_seed(seed)
+    cache = int4_cache.new_kvcache_int4(-(-n // block), block, kv, device="cpu")
+    k, v = (torch.randn(n, kv, 128, generator=g) * torch.exp2(spread * torch.randn(n, kv, 1, generator=g)) for _ in range(2))
+    slots = torch.arange(n, dtype=torch.int32)
+    int4.store(k.to(torch.bfloat16), v.to(torch.bfloat16), *cache, slots)
+    return cache, torch.arange(-(-n // block), dtype=torch.int32), torch.randn(3, 4 * kv, 128, generator=g).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("n,block,spread", [(50, 16, 0.0), (2000, 16, 0.0), (2000, 16, 1.0), (20000, 64, 0.0)])
+def test_the_norm_tells_wrong_outputs(n, block, spread):
+    """What ``attention_norm`` allows is far less than what zeros, a page left out, a scale 1 % off, values 1 % off, or
+    rows one place off make of an output.  (With rows of many sizes some queries look at one position alone: neither the
+    scale nor another page changes those.)"""
+    all_or_some = torch.all if spread == 0 else torch.any
+    cache, table, q = _filled_cpu(n, 1, block, 3, spread)
+    ref, room = int4.attention_norm(q, *cache, table, n, 0.09)
+    off = lambda out: ((out - ref).norm(dim=-1) / room)  # noqa: E731
+    assert torch.all(off(ref.to(torch.bfloat16).double()) < 1)       # the rounding alone
+    assert torch.all(off(torch.zeros_like(ref)) > 20)
+    assert all_or_some(off(int4.attention_norm(q, *cache, table, n, 0.09 * 1.01)[0]) > 1)
+    assert torch.all(off(ref * 1.01) > 1)
+    assert torch.all(off(ref.roll(1, 0)) > 20) and torch.all(off(ref.roll(1, 1)) > 20)
+    for page in (0, table.numel() // 2, table.numel() - 2) if spread == 0 else ():
+        without = table.clone()
+        without[page] = -1
+        worst = off(int4.attention_norm(q, *cache, without, n, 0.09)[0])
+        assert torch.all(worst > 1), f"page {page}"
