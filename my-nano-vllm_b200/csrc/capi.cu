@@ -1230,8 +1230,10 @@ struct Int4Plan {
   int64_t short_bytes, bytes;
 };
 
-// New tokens of a sequence that the split-context kernel takes: those of at most 32 query rows of a kv head (64 sequences
-// of 32,768 positions: 32 rows 963 us there and 1,647 in the kernel for long chunks, whose tiles have 128 rows).
+// New tokens of a sequence that the split-context kernel takes: those of at most 32 query rows of a kv head.  The kernel for
+// long chunks, whose tiles have 128 rows, takes longer for any of them (32 rows of 8 kv heads: one sequence of 200 positions
+// 21.4 us for 17.9, of 16,384 43 for 35; 16 of 2,000 55 for 40; 192 of 200 114 for 73, of 2,000 397 for 242, of 16,384
+// 2,575 for 1,585; with 12 rows 2,565 for 869).
 static int int4_short_q(int group, int max_q) {
   constexpr int kShortRows = 32;
   // a single token of any group stays with the first kernel, which takes wider groups in parts
