@@ -237,3 +237,74 @@ def test_few_rows_cuts_do_not_grow_with_the_context(new, instructions):
         rounding += float((ref.to(torch.bfloat16).double() - ref).square().sum())
         room += float(_sum_of_sizes(q[at], cache, table, n).square().sum())
     assert (far - rounding) ** 0.5 <= instructions * 17 * 2.0 ** -26 * room ** 0.5
+
+
+@pytest.mark.parametrize("new", [1, 3, 5, 8])
+@pytest.mark.parametrize("from_unit", [0, 40])
+def test_few_rows_of_many_sizes_in_long_pieces(new, from_unit):
+    """So many sequences (on the same pages) that a CTA has a whole pair, whose sums are put aside many times while its query
+    rows have powers of their own: from its first unit of 128 positions on, or from a later one."""
+    from nanovllm_b200.int4_cache import int4_decode_attention, int4_prefill_attention
+    n, kv, heads, seqs = 20000, 2, 8, 220
+    key, value = _randn(n, kv, 128, seed=31), _randn(n, kv, 128, seed=32)
+    powers = torch.randint(-30, 30, (n, kv, 1), generator=_gen(33), device="cuda").double()
+    powers[:128 * from_unit] = 0
+    value *= torch.exp2(powers)
+    q = 1.5 * _randn(seqs * new, heads, 128, seed=34)
+    checked = (0, 7, 219)
+    for x, i in enumerate(checked):  # rows that look at one position each, early, late and small ones among them
+        for r in range(new * heads):
+            key[(r * 613 + 97 * x) % (n - new), r % heads // 4] = 2 * q[i * new + r // heads, r % heads]
+    q = q.to(torch.bfloat16)
+    cache, table = _filled(key, value, 32)
+    tables = table.repeat(seqs, 1)
+    if new == 1:
+        out = int4_decode_attention(q, *cache, tables, torch.full((seqs,), n, dtype=torch.int32, device="cuda"), SCALE)
+    else:
+        out = int4_prefill_attention(q, *cache, tables, _cum([new] * seqs), _cum([n] * seqs), new, n, SCALE)
+    for i in checked:
+        at = slice(i * new, (i + 1) * new)
+        ref, room = int4.attention_norm(q[at], *cache, table, n, SCALE)
+        far = (out[at].double() - ref).norm(dim=-1)
+        assert torch.all(far <= room), f"sequence {i}: {float((far / room).nan_to_num(math.inf).max()):.2f}"
+
+
+@pytest.mark.parametrize("new,heads", [(2, 4), (6, 4), (8, 4), (150, 4)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_row_that_is_no_number_beside_rows_of_many_sizes(new, heads, which, bad):
+    """It reaches the queries that see it, and those before it get what they see.  (As it is stored: with a step that is no
+    number, whatever its values were.)"""
+    n = 900
+    key, value, q = _ordinary(n, 1, heads, new)
+    value *= torch.exp2(torch.randint(-40, 40, (n, 1, 1), generator=_gen(41), device="cuda").double())
+    (key if which == "k" else value)[n - 2, 0, 17] = bad
+    cache, table = _filled(key, value, 32)
+    q = q.to(torch.bfloat16)
+    out = _attend(q, cache, table, n)
+    ref, room = int4.attention_norm(q[:new - 2], *cache, table, n - 2, SCALE)
+    assert torch.all((out[:new - 2].double() - ref).norm(dim=-1) <= room)
+    assert not torch.isfinite(out[new - 2:]).any()
+
+
+@pytest.mark.parametrize("new", [1, 5, 150])
+def test_rows_of_many_sizes_give_the_same_bits_in_a_graph(new):
+    n = 5000
+    key, value, q = _ordinary(n, 1, 4, new)
+    value *= torch.exp2(torch.randint(-60, 60, (n, 1, 1), generator=_gen(42), device="cuda").double())
+    cache, table = _filled(key, value, 32)
+    q = q.to(torch.bfloat16)
+    first = _attend(q, cache, table, n)
+    ctx, tables = torch.tensor([n], dtype=torch.int32, device="cuda"), table[None].contiguous()
+    cq, ck = _cum([new]), _cum([n])
+    from nanovllm_b200.int4_cache import int4_decode_attention, int4_prefill_attention
+    call = lambda: (int4_decode_attention(q, *cache, tables, ctx, SCALE) if new == 1 else  # noqa: E731
+                    int4_prefill_attention(q, *cache, tables, cq, ck, new, n, SCALE))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first) and torch.equal(call(), first)
