@@ -10,16 +10,16 @@
 // into q and into the outputs.  q is exact in f16 after a power-of-two scale per row.
 //
 // Bound by HBM up to 8 rows: 136 bytes of K and V for each position and kv head, read once for all of the rows of
-// its query heads (64 sequences of 32,768, 8 rows: 396 us, 0.88 of the floor at 6.55 TB/s; 4 rows: 390 us).  Above,
+// its query heads (64 sequences of 32,768, 8 rows: 405 us, 0.86 of the floor at 6.55 TB/s; 4 rows: 399 us).  Above,
 // by the tensor cores of mma.sync: 34 products of 8 cycles for each 32 positions and plane of 8 rows, which fp32
 // arithmetic does not overlap (8 fma beside one product: 14.9 cycles, and 8 without it), against 186 cycles of
-// HBM: 16 rows 549 us, 24 rows 759, 32 rows 963.
+// HBM: 16 rows 587 us, 24 rows 779, 32 rows 1,059.
 //
 // Work: a unit is 128 positions of one (sequence, row group, kv head), and a warp computes S^T = K q^T and P of 32 of
 // them (A = codes, 16 positions x 16 values).  P goes through shared memory (stmatrix turns it), and of all 128
 // positions the warp adds O^T += V^T P^T for its 32 values (A = codes again, turned by ldmatrix).  So a warp's sums are
-// 8 registers for 8 rows and not 32, and no sums are added at the end.  With all values in one warp 8 rows took 410 us
-// and 24 rows 800; with q in registers instead of shared memory 24 rows took 845 (spills).
+// 8 registers for 8 rows and not 32, and no sums are added at the end.  (Measured when 8 rows took 382 us and 24 rows 720: with
+// all values in one warp 410 and 800, with q in registers instead of shared memory, which spills, 24 rows 845.)
 //
 // All units in order are cut into equal ranges, one for each resident CTA, wherever the cuts fall: no counters, no
 // order that depends on timing.  A CTA's first and last piece may be parts of a pair; their sums go to the workspace,
@@ -41,7 +41,8 @@
 // is the CTA's, and so comes from rows as well that a query row does not look at.  Where steps of V differ by more than
 // some 2^15 (or are zero beside others), or values pass 2^90, the rest of the piece is done with a power for each query row
 // instead, that of its own largest p |v| so far, found with an exchange of maxima in every unit; what a row gets is then as
-// exact as its own largest terms.
+// exact as its own largest terms (64 sequences of 32,768: 405 us, 541 with one row in 64 of 2^-24).  The units of such
+// pieces have a loop of their own: as a branch of the other one 24 rows took 3 % longer and 32 rows 4 % (spills).
 #include <atomic>
 #include <climits>
 #include <type_traits>

@@ -17,16 +17,26 @@
 //
 // Rows of one block that differ by more than 2^kSpread cannot share a power: the small ones would leave f16's normal numbers
 // (below 2^-14).  In such a block each row of K and V has its own, at the cost of a second pass over the tile's scores and a
-// second exponential (all tiles of 2,048 of 32,768: 3,540 us for 940; each sequence's first row alone: 955).
+// second exponential (all tiles of 2,048 of 32,768: 3,540 us for 940; each sequence's first row alone: 950).
+//
+// Measured for this (2,048 of 32,768 and 7 prompts in us; 915 to 945 and 171 with one power for a tile of K and one that grows for
+// V, which small rows do not survive; 937 to 950 and 184 as it is): one power for the four blocks of a tile, agreed on by the
+// unpacking warps, 962 and 181; found by each of them, 982 and 185; by a warp of its own, which prepares steps and lowest values
+// ahead of them, 1,250 and 234; codes made whole numbers by another f16
+// operation, so that a tile has 2^21 more room and rarely needs powers, 1,100 and 193.
+//
+// Roundings: q is exact; values of K and V 2^-12, P 2^-12, a fourth of the exponentials 1e-4; statistics and sums in fp32, those of
+// the tensor cores cut at 2^-24 of their largest term.  Off in the 2-norm: 1.68e-3 (7 prompts) and 1.69e-3 (2,048 of 32,768), of
+// which the output's own rounding is 1.66e-3.
 //
 // Bound by the chain of a group: products of its tile (1,056 cycles: one every 66) behind the other group's, then its
 // softmax (about 2,050), 4,100 cycles for a tile of both groups; tensor cores and issue slots are half busy (2,048 new
-// tokens of 32,768 positions, 32 heads: 910 us, 1,170 TFLOP/s).  A softmax row of 128 needs 1,024 cycles of the
-// exponential unit for each group, so 1 of 4 pairs takes a polynomial instead (7 prompts: 182 to 176 us).  Tried:
-// scores and P by halves of a tile, so that softmax and products of a group overlap (1,404 us: products of 64 columns
+// tokens of 32,768 positions, 32 heads: 937 to 950 us, 1,130 TFLOP/s).  A softmax row of 128 needs 1,024 cycles of the
+// exponential unit for each group, so 1 of 4 pairs takes a polynomial instead (7 prompts: 182 to 176 us).  Tried, when
+// these took 910 and 170 us: scores and P by halves of a tile, so that softmax and products of a group overlap (1,404 us: products of 64 columns
 // take as long as those of 128), P alone by halves (1,041: the issuing warp waits for one group while the other is
 // ready), an issuing warp for each group (1,250), the groups' blocks of products in a loop (941), barriers looked at
-// between two blocks (1,107).  Short items (7 prompts: 170 us) pay 9,000 cycles for q and outputs beside some 4 tiles;
+// between two blocks (1,107).  Short items (7 prompts) pay 9,000 cycles for q and outputs beside some 4 tiles;
 // q brought by bulk copies of 128 bytes took 322 us, by two warps of its own 182, before the outputs of the item before
 // it 175; outputs through shared memory 180.
 //

@@ -13,11 +13,17 @@ codes of 4 bits, and stands for low + step * code; include/fp8attn.h has the lay
 those of ``store_kvcache``, ``fp8_decode_attention`` and ``fp8_prefill_attention`` with the cache
 (k_cache, v_cache, kv_scale) in place of theirs; the reference has an e4m3 cache only
 (nanovllm/layers/attention.py:11-40, nanovllm/kernels/fp8_attention.py:173-207, :314-353).  One layer of a
-step, without the norms:
+step:
 
     q, k = apply_rope(q, k, positions, cos_sin_cache)
     store_kvcache_int4(k, v, *cache, slot_mapping)
     o = int4_decode_attention(q, *cache, block_tables, context_lens, softmax_scale)
+
+and of a model with q/k norms, the first call without a cache of its own:
+
+    q, k = qk_norm_rope_store(qkv, positions, q_norm_weight, k_norm_weight, eps, cos_sin_cache, num_heads,
+                              num_kv_heads, None, None, None, return_k=True)
+    store_kvcache_int4(k, v, *cache, slot_mapping)
 
 All launch on ``torch.cuda.current_stream()`` of the tensors' device, allocate outputs and scratch with
 ``torch.empty`` (scratch is one call's own) and never synchronise or read device memory on the host, so

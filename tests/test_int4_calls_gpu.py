@@ -81,3 +81,36 @@ def test_block_table_without_columns():
         out = int4_prefill_attention(_randn(3 * new, 8, 128, seed=8), *cache, table, _ints(0, new, 2 * new, 3 * new),
                                      _ints(0, 0, 30, 30), new, 30, SCALE)
         assert torch.all(out == 0)
+
+
+def test_a_layer_with_norms():
+    """The fused epilogue without a cache of its own, the store and the attention one after another: a prompt, then a token,
+    against a float64 layer on the rows as the cache holds them."""
+    from nanovllm_b200.int4_cache import (int4_decode_attention, int4_prefill_attention, load_kvcache_int4,
+                                          new_kvcache_int4, store_kvcache_int4)
+    from nanovllm_b200.qk_epilogue import qk_norm_rope_store
+    from nanovllm_b200.rope import rope_table
+    heads, kv, n = 8, 2, 100
+    qkv, w = _randn(n, (heads + 2 * kv) * 128, seed=9), _randn(128, seed=10)
+    table, cache = rope_table(200, 128), new_kvcache_int4(8, 16, kv)
+    pages = torch.tensor([[3, 1, 7, 0, 2, 6, 4]], dtype=torch.int32, device="cuda")
+
+    def layer(lo, hi):
+        pos = torch.arange(lo, hi, device="cuda")
+        q, k = qk_norm_rope_store(qkv[lo:hi], pos, w, w, 1e-6, table, heads, kv, None, None, None, return_k=True)
+        slots = (pages[0].long()[pos // 16] * 16 + pos % 16).to(torch.int32)
+        store_kvcache_int4(k, qkv[lo:hi, (heads + kv) * 128:].unflatten(1, (kv, 128)), *cache, slots)
+        if hi - lo == 1:
+            return q, int4_decode_attention(q, *cache, pages, _ints(hi), SCALE)
+        return q, int4_prefill_attention(q, *cache, pages, _ints(0, hi - lo), _ints(0, hi), hi - lo, hi, SCALE)
+
+    for lo, hi in ((0, n - 1), (n - 1, n)):
+        q, out = layer(lo, hi)
+        at = torch.arange(hi, device="cuda")
+        k, v = (x.double() for x in load_kvcache_int4(*cache, (pages[0].long()[at // 16] * 16 + at % 16).to(torch.int32)))
+        for h in range(heads):
+            s = q[:, h].double() @ k[:, h // 4].T * SCALE
+            s = s.masked_fill(at[None] > torch.arange(lo, hi, device="cuda")[:, None], -float("inf"))
+            want = torch.softmax(s, -1) @ v[:, h // 4]
+            # rows read back are rounded to bf16 (2^-9 in the mean square, in the scores and in the values), the output too
+            assert (out[:, h].double() - want).norm() <= 2.0 ** -6 * want.norm()
