@@ -308,3 +308,8 @@ def test_rows_of_many_sizes_give_the_same_bits_in_a_graph(new):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, first) and torch.equal(call(), first)
+
+
+def test_no_wait_has_run_out():
+    from nanovllm_b200 import fp8_attention
+    assert fp8_attention.device_error() == 0
