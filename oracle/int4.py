@@ -125,10 +125,11 @@ def attention_norm(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale):
       rounding of the output to bf16: errors are spread evenly over half a step either way, at most 2^-8 / sqrt(3) of the
         value in the mean square; 2.5e-3 with what 128 values scatter; below 2^-126, where bf16's steps are 2^-133
         whatever the value, at most 2^-134 for each;
-      the weights p: P (2^-12), values (2^-12) and scores are rounded at each position for itself, so errors d of that size
-        add up as d sqrt(sum p^2 |v|^2).  A score's 128 terms carry 2^-12 of each (f16 operands), which is an error of
-        2^-12 (sum of squares of the terms)^1/2 in the exponent; some exponentials are off by 1e-4.  All below
-        d = 2^-10 max(1, that root without its 2^-12);
+      P and values: rounded to f16 at each position for itself (2^-12 each), some exponentials 1e-4 off: errors of that size
+        add up as their root mean square, 2^-10 sqrt(sum p^2 |v|^2) at the most of some four standard deviations;
+      scores: 128 terms that carry 2^-12 of each (f16 operands), so off by e = 2^-12 (sum of squares of the terms)^1/2 and a
+        weight by e of itself.  A weight is in the numerator and in the denominator of sum p v / sum p: it moves the output by
+        e p (v - out).  Again for each position for itself, four times e;
       what is alike at all positions (sums cut in one direction): 2^-16 sum p |v|.
     """
     nq, heads, _ = q.shape
@@ -152,9 +153,10 @@ def attention_norm(q, k_cache, v_cache, kv_scale, table, nk, softmax_scale):
         s = (x @ k.T * softmax_scale).masked_fill(~seen, -math.inf)
         p = torch.where(some[:, None], torch.softmax(s, -1), torch.zeros_like(s))
         out[:, h] = p @ v
-        root = (x.square() @ k.square().T).sqrt() * abs(softmax_scale)
-        d = 2.0 ** -10 * torch.where(seen, root, 0.0).clamp(min=1.0)
+        root = torch.where(seen, (x.square() @ k.square().T).sqrt() * abs(softmax_scale), 0.0)
         size = v.norm(dim=-1)
-        room[:, h] = (2.5e-3 * out[:, h].norm(dim=-1) + ((d * p * size) ** 2).sum(-1).sqrt()
+        apart = (size.square() - 2 * out[:, h] @ v.T + out[:, h].square().sum(-1, keepdim=True)).clamp(min=0).sqrt()
+        room[:, h] = (2.5e-3 * out[:, h].norm(dim=-1) + 2.0 ** -10 * ((p * size).square() + (root * p * apart).square())
+                      .sum(-1).sqrt()
                       + 2.0 ** -16 * (p @ v.abs()).norm(dim=-1) + 2.0 ** -134 * D ** 0.5)
     return out, room

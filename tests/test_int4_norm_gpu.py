@@ -113,3 +113,32 @@ def test_every_page_counts_for_a_row(new, heads, n, block):
 def test_scales_of_scores(sd, scale, news, lens):
     cache, table = _cache(lens, 2, 16, 7)
     _run(_q(sum(news), 8, 8, sd), cache, table, news, lens, scale)
+
+
+@pytest.mark.parametrize("seed", range(32))
+def test_drawn(seed):
+    """Heads, pages, lengths, sizes of rows, missing pages and rows of zeros as they come."""
+    import random
+    rng = random.Random(seed)
+    kv, group = rng.choice([1, 2, 3]), rng.choice([1, 2, 3, 4, 5, 7, 8, 12, 16, 32, 40])
+    seqs, kind = rng.choice([1, 2, 5]), rng.choice(["one", "few", "chunk", "mixed"])
+    lens = [max(1, int(math.exp(rng.uniform(0, math.log(3000))))) for _ in range(seqs)]
+    news = [min(n, {"one": 1, "few": rng.randint(1, 8), "chunk": rng.randint(1, 300),
+                    "mixed": rng.choice([0, 1, 5, 200])}[kind]) for n in lens]
+    news[0] = max(news[0], 1)
+    cache, table = _cache(lens, kv, rng.choice([16, 32, 48, 64, 128, 256]), seed)
+    shape, scale, g = cache[2].shape[:3], cache[2], _gen(seed)
+    randn = lambda: torch.randn(*shape, generator=g, device="cuda")  # noqa: E731
+    spread = rng.choice([0.0, 0.5, 3.0, 10.0, 30.0])
+    size = torch.exp2((spread * randn()).round().clamp(-100, 100))
+    if rng.random() < 0.5:
+        size = torch.where(randn() > 2.3, size, 1.0)
+    scale[..., 2:] = (scale[..., 2:].float() * size[..., None]).to(torch.bfloat16)
+    if rng.random() < 0.5:  # smaller keys: scores stay numbers
+        size = torch.exp2((min(spread, 3.0) * randn()).round().clamp(-60, 2))
+        scale[..., :2] = (scale[..., :2].float() * size[..., None]).to(torch.bfloat16)
+    if rng.random() < 0.3:
+        scale[..., 2:][randn() > 2.0] = 0
+    if rng.random() < 0.3:
+        table[0, rng.randrange(table.shape[1])] = -1
+    _run(_q(sum(news), kv * group, seed + 1, rng.choice([0.1, 1.5, 3.0])), cache, table, news, lens)
