@@ -403,9 +403,9 @@ FP8ATTN_API int64_t fp8attn_int4_workspace_bytes(int num_seqs, int num_heads, in
  * to 65535.  Positions in pages that the table does not name (-1, out of range) are masked; a sequence
  * without any position gives zeros.  block_tables may be null where max_num_blocks is 0.
  * Rows of the cache may be of any size that bf16 holds, beside one another too: what a query gets is off by
- * what fp32 sums and one rounding to f16 of each of its own terms make of it (up to 1.84e-3 in the 2-norm at
- * 131,072 positions, the output's rounding to bf16 included, which is 1.66e-3), whatever rows it does not see
- * hold.  Scores have to be numbers in fp32, and |q| * softmax_scale below 2^115. */
+ * what fp32 sums and roundings to f16 of its own terms make of it (of each weight; of K's and V's values too where
+ * a kv head has more than 32 query rows of a sequence): up to 1.84e-3 in the 2-norm at 131,072 positions, the
+ * output's rounding to bf16 included, which is 1.66e-3, whatever rows that it does not see hold.  Scores have to be numbers in fp32, and |q| * softmax_scale below 2^115. */
 FP8ATTN_API int fp8attn_int4_decode(void* out, const void* q, int64_t q_row_stride, const void* k_cache,
                                     const void* v_cache, const void* kv_scale, const int32_t* block_tables,
                                     int64_t block_tables_stride, int max_num_blocks, const int32_t* context_lens,
